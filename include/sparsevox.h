@@ -49,7 +49,13 @@ typedef enum sv_status {
   SV_ERR_WORKSPACE = 7         /* workspace pointer null or smaller than required */
 } sv_status;
 
-typedef enum sv_dtype { SV_FLOAT32 = 0, SV_FLOAT16 = 1, SV_BFLOAT16 = 2 } sv_dtype;
+/* SV_FLOAT8_E4M3: operands of sv_linear_forward and the output of sv_rms_norm only. */
+typedef enum sv_dtype {
+  SV_FLOAT32 = 0,
+  SV_FLOAT16 = 1,
+  SV_BFLOAT16 = 2,
+  SV_FLOAT8_E4M3 = 3
+} sv_dtype;
 
 /* Weight layouts accepted by the convolution.
  *  SV_WEIGHT_KIO: (K, Cin, Cout), the view `sparse_conv3d` receives
@@ -356,6 +362,112 @@ SV_API int sv_rownorm(const void* x, int64_t n, int channels, int dtype, float e
                       const float* weight, const float* bias, const void* scale,
                       const void* shift, int64_t mod_stride, const int32_t* coords,
                       int64_t batch, int silu, void* out, int32_t* status, sv_stream_t stream);
+
+/* ---- root-mean-square norm with the residual's addition -------------------------------- */
+
+/* h = round(x + residual) (x without a residual), rstd = 1 / sqrt(mean(h^2) + eps),
+ * y = h * rstd * weight per row of [n, channels] (channels <= 8192), fp32 inside.
+ *   x, residual: rows `x_stride` / `residual_stride` elements apart, `dtype`; residual may be null.
+ *   weight: fp32 [channels] or null (ones).
+ *   h: receives the sum, [n, channels] in `dtype`, or null. rstd: fp32 [n] or null.
+ *   out: [n, channels] in `out_dtype`, which is `dtype`, or SV_FLOAT8_E4M3: then
+ *     scale[r] = max|y| / 448 (1 for a row of zeros) and out = e4m3(y / scale), y = out * scale.
+ * A row that holds a NaN or an infinity gives NaNs, its scale among them. */
+SV_API int sv_rms_norm(const void* x, int64_t x_stride, const void* residual,
+                       int64_t residual_stride, int64_t n, int channels, int dtype, float eps,
+                       const float* weight, void* h, float* rstd, void* out, int out_dtype,
+                       float* scale, sv_stream_t stream);
+
+/* Gradients of y with respect to h, plus `dh` (the gradient that reaches h itself; may be null):
+ * dx [n, channels] (also the residual's gradient) and dw fp32 [channels] (null: not wanted). The
+ * weight's sums run in a fixed order. h: rows `h_stride` apart; dy, dh, dx contiguous. */
+SV_API size_t sv_rms_norm_backward_workspace_bytes(int channels);
+SV_API int sv_rms_norm_backward(const void* h, int64_t h_stride, const void* dy, const void* dh,
+                                int64_t n, int channels, int dtype, const float* weight,
+                                const float* rstd, void* dx, float* dw, void* workspace,
+                                size_t workspace_bytes, sv_stream_t stream);
+
+/* ---- linear projection with bias, activation and residual ------------------------------ */
+
+typedef enum sv_activation {
+  SV_ACT_NONE = 0,
+  SV_ACT_SILU = 1,
+  SV_ACT_GELU = 2,     /* x Phi(x) */
+  SV_ACT_GELU_TANH = 3 /* the tanh form */
+} sv_activation;
+
+/* The product a workspace is for. */
+typedef enum sv_linear_pass {
+  SV_LINEAR_FORWARD = 0,
+  SV_LINEAR_DZ = 1,
+  SV_LINEAR_DX = 2,
+  SV_LINEAR_DW = 3
+} sv_linear_pass;
+
+/* Workspace of one pass over x [m, k] and weight [n, k]. `copies`: bit 0 / bit 1 set when the
+ * product's first / second operand (x, weight; dz, weight; dz, x) is not 16-byte aligned or its
+ * row stride is not a multiple of 16 bytes; it is then copied into padded rows. */
+SV_API size_t sv_linear_workspace_bytes(int pass, int64_t m, int64_t k, int64_t n, int dtype,
+                                        int copies);
+
+/* out = act(x weight^T * x_scale[i] * w_scale[j] + bias[j]) + residual, [m, n] contiguous in
+ * `out_dtype`; bias, residual (rows `ld_res` apart, `out_dtype`) and the fp32 scales may be null.
+ * `preact` (or null) receives the activation's argument, [m, n] in `out_dtype`. fp32 accumulation,
+ * one rounding. dtype fp32 / fp16 / bf16 (out_dtype the same) or e4m3 (out_dtype fp16 / bf16).
+ * fp16, bf16 and e4m3 run on the tensor cores; out must not overlap an operand. */
+SV_API int sv_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                             const void* bias, const void* residual, int64_t ld_res,
+                             const float* x_scale, const float* w_scale, int64_t m, int64_t k,
+                             int64_t n, int dtype, int out_dtype, int activation, void* out,
+                             void* preact, void* workspace, size_t workspace_bytes,
+                             int32_t* status, sv_stream_t stream);
+
+/* dz = dout * act'(preact), [m, n]; dbias = its column sums in a fixed order (null: not wanted).
+ * Without an activation dz is dout: preact and dz are not used. */
+SV_API int sv_linear_backward_z(const void* dout, const void* preact, int64_t m, int64_t n,
+                                int dtype, int activation, void* dz, void* dbias, void* workspace,
+                                size_t workspace_bytes, sv_stream_t stream);
+
+/* dx [m, k] = dz [m, n] weight [n, k]; dw [n, k] = dz^T x. dz and the results contiguous. */
+SV_API int sv_linear_dx(const void* dz, const void* weight, int64_t ldw, int64_t m, int64_t k,
+                        int64_t n, int dtype, void* dx, void* workspace, size_t workspace_bytes,
+                        int32_t* status, sv_stream_t stream);
+SV_API int sv_linear_dw(const void* dz, const void* x, int64_t ldx, int64_t m, int64_t k,
+                        int64_t n, int dtype, void* dw, void* workspace, size_t workspace_bytes,
+                        int32_t* status, sv_stream_t stream);
+
+/* ---- windowed attention with a learned relative position bias --------------------------- */
+
+/* The rows of a window grouping (sv_window_groups' perm [n] and offsets [groups + 1]) in window
+ * order with their coordinates and window bounds: sv_window_plan_bytes(n) bytes, built once per
+ * grouping. n <= 2^25. A perm entry outside [0, n) or a bad offset ORs SV_DEVICE_BAD_INDEX into
+ * `status`, and that position is left out. */
+SV_API size_t sv_window_plan_bytes(int64_t n);
+SV_API int sv_window_plan(const int32_t* coords, const int32_t* perm, const int32_t* offsets,
+                          int64_t groups, int64_t n, void* plan, int32_t* status,
+                          sv_stream_t stream);
+
+/* Self-attention inside the plan's windows, [n, heads, dim] (dim <= 128):
+ *   s_ij = scale q_i . k_j + table[h][lut[dx]][lut[dy]][lut[dz]], softmax over the window, o = p v.
+ * dx, dy, dz: the key's coordinates minus the query's, clamped to +-reach (<= 1023); lut: int32
+ * [2 reach + 1], values in [0, buckets) (others are clamped); table: [heads, buckets^3] in `dtype`,
+ * buckets <= 25. `strides`: row and head strides of q, k, v in elements, channels contiguous.
+ * out: contiguous. lse (or null): fp32 [heads, n] by position, for the backward pass. A row whose
+ * every score is -inf gives zeros. */
+SV_API int sv_window_attention(const void* q, const void* k, const void* v,
+                               const int64_t* strides, int64_t n, int heads, int dim, int dtype,
+                               const void* plan, const void* table, int buckets,
+                               const int32_t* lut, int reach, float scale, void* out, float* lse,
+                               sv_stream_t stream);
+
+/* Its gradients, from the forward pass's out (`o`) and lse: dq, dk, dv contiguous, and dtable
+ * [heads, buckets^3] (null: not wanted), whose sums do not depend on the order of execution. */
+SV_API size_t sv_window_attention_backward_workspace_bytes(int64_t n, int heads, int buckets);
+SV_API int sv_window_attention_backward(
+    const void* q, const void* k, const void* v, const int64_t* strides, const void* o,
+    const void* dout, const float* lse, int64_t n, int heads, int dim, int dtype, const void* plan,
+    const void* table, int buckets, const int32_t* lut, int reach, float scale, void* dq, void* dk,
+    void* dv, void* dtable, void* workspace, size_t workspace_bytes, sv_stream_t stream);
 
 /* ---- topology: occupancy -> coordinates, subdivision, attention windows --------------- */
 

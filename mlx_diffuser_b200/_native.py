@@ -7,6 +7,7 @@ tensors (other frameworks' arrays are accepted through DLPack, see :func:`as_ten
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -39,6 +40,11 @@ SV_DEVICE_BAD_INDEX = 0x2
 SV_DEVICE_WAIT_TIMEOUT = 0x4
 
 DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+SV_FLOAT8_E4M3 = 3  # operands of the projection, output of the root-mean-square norm
+
+# sv_activation / sv_linear_pass
+ACTIVATION_CODE = {None: 0, "none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
+SV_LINEAR_FORWARD, SV_LINEAR_DZ, SV_LINEAR_DX, SV_LINEAR_DW = range(4)
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -92,6 +98,38 @@ _SIGNATURES = {
         _I32,
         [_P, _I64, _I32, _I32, ctypes.c_float, _P, _P, _P, _P, _I64, _P, _I64, _I32, _P, _P,
          _P],
+    ),
+    "sv_rms_norm": (
+        _I32,
+        [_P, _I64, _P, _I64, _I64, _I32, _I32, ctypes.c_float, _P, _P, _P, _P, _I32, _P, _P],
+    ),
+    "sv_rms_norm_backward_workspace_bytes": (_SZ, [_I32]),
+    "sv_rms_norm_backward": (
+        _I32, [_P, _I64, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _SZ, _P]
+    ),
+    "sv_linear_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64, _I32, _I32]),
+    "sv_linear_forward": (
+        _I32,
+        [_P, _I64, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _P,
+         _SZ, _P, _P],
+    ),
+    "sv_linear_backward_z": (
+        _I32, [_P, _P, _I64, _I64, _I32, _I32, _P, _P, _P, _SZ, _P]
+    ),
+    "sv_linear_dx": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _SZ, _P, _P]),
+    "sv_linear_dw": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _SZ, _P, _P]),
+    "sv_window_plan_bytes": (_SZ, [_I64]),
+    "sv_window_plan": (_I32, [_P, _P, _P, _I64, _I64, _P, _P, _P]),
+    "sv_window_attention": (
+        _I32,
+        [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _I32, _P, _I32, ctypes.c_float, _P, _P,
+         _P],
+    ),
+    "sv_window_attention_backward_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
+    "sv_window_attention_backward": (
+        _I32,
+        [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _I32, _P, _I32,
+         ctypes.c_float, _P, _P, _P, _P, _P, _SZ, _P],
     ),
     "sv_downsample_workspace_bytes": (_SZ, [_I64]),
     "sv_downsample_coords": (_I32, [_P, _I64, _I32, _P, _P, _P, _P, _P, _P, _SZ, _P]),
@@ -176,6 +214,14 @@ def require_cuda(t: torch.Tensor, name: str) -> None:
             f"{name} must live on a CUDA device: this package runs only on the GPU "
             "(no CPU fallback)"
         )
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current CUDA device (the library launches there)."""
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

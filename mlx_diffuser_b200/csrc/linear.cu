@@ -1,0 +1,650 @@
+// Linear projection of feature rows with bias, activation and residual in its epilogue, and its
+// gradients.
+//
+//     z = x W^T [* x_scale[i] * w_scale[j]] + b        x [m, k], W [n, k]
+//     y = act(z) + residual
+//     dz = dy * act'(z),  db = column sums of dz,  dx = dz W,  dW = dz^T x
+//
+// Three kernels form the products:
+//   few_rows_kernel   up to FEW_ROWS rows (any type): one pass over W, which is all the bytes
+//                     there are; a warp or a block per output column;
+//   gemm_f32_kernel   fp32: register tiles of FFMAs, exact fp32 products and sums;
+//   linear_tc.cu      fp16 / bf16 / e4m3: tcgen05 tiles fed by TMA.
+// A product with too few tiles to fill the machine splits its k axis; the parts' fp32 sums are
+// joined in a fixed order by finish_kernel, which then applies the epilogue. TMA wants 16-byte
+// aligned rows: an operand that has none (an odd channel count, a sliced view) is first copied
+// into padded rows in the workspace, one pass over it.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "linear.h"
+
+namespace sv {
+namespace {
+
+constexpr int FEW_ROWS = 8;
+constexpr int COPY_ALIGN = 256;
+
+__device__ __forceinline__ float to_float(__nv_fp8_e4m3 v) { return static_cast<float>(v); }
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// ---- few rows ----------------------------------------------------------------------------------
+
+// W warps per output column (1: eight columns a block, 8: one), lanes along k in accesses of V
+// elements. Every lane holds the partial sums of all rows; x comes out of L1.
+template <typename T, typename O, int ROWS, int V, int W>
+__global__ void __launch_bounds__(256)
+    few_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
+                    int m, int64_t n, int64_t k, Epilogue ep) {
+  __shared__ float part[W > 1 ? 8 : 1][ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t j = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
+  const int slot = W > 1 ? (int)threadIdx.x : lane;
+  float acc[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) acc[r] = 0.f;
+  if (j < n) {
+    const T* wr = w + j * ldw;
+#pragma unroll 2
+    for (int64_t c = (int64_t)slot * V; c < k; c += 32 * W * V) {
+      T we[V];
+      if constexpr (V * sizeof(T) == 16)
+        *reinterpret_cast<uint4*>(we) = __ldg(reinterpret_cast<const uint4*>(wr + c));
+      else
+        we[0] = wr[c];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if (r < m) {
+          T xe[V];
+          if constexpr (V * sizeof(T) == 16)
+            *reinterpret_cast<uint4*>(xe) =
+                __ldg(reinterpret_cast<const uint4*>(x + r * ldx + c));
+          else
+            xe[0] = x[r * ldx + c];
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[r] = fmaf(to_float(xe[e]), to_float(we[e]), acc[r]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
+  }
+  if constexpr (W > 1) {
+    if (lane == 0) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) part[warp][r] = acc[r];
+    }
+    __syncthreads();
+    if (threadIdx.x < ROWS && (int)threadIdx.x < m) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += part[i][threadIdx.x];
+      epilogue_store<O>(ep, threadIdx.x, j, n, v);
+    }
+  } else if (j < n) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (lane == r && r < m) epilogue_store<O>(ep, r, j, n, acc[r]);
+  }
+}
+
+template <typename T, typename O, int ROWS>
+int launch_few(const Gemm& g, cudaStream_t s) {
+  constexpr int VE = 16 / sizeof(T);
+  const T* x = static_cast<const T*>(g.a.p);
+  const T* w = static_cast<const T*>(g.b.p);
+  const bool vec = aligned16(x) && aligned16(w) && g.k % VE == 0 && g.a.ld % VE == 0 &&
+                   g.b.ld % VE == 0;
+  // A warp per column needs n / 8 blocks to cover the machine; below that a block per column
+  // brings eight times the loads in flight.
+  const bool wide = g.n >= 8 * num_sms();
+  const unsigned blocks = (unsigned)(wide ? (g.n + 7) / 8 : g.n);
+  auto kernel = vec ? (wide ? few_rows_kernel<T, O, ROWS, VE, 1> : few_rows_kernel<T, O, ROWS, VE, 8>)
+                    : (wide ? few_rows_kernel<T, O, ROWS, 1, 1> : few_rows_kernel<T, O, ROWS, 1, 8>);
+  kernel<<<blocks, 256, 0, s>>>(x, g.a.ld, w, g.b.ld, (int)g.m, g.n, g.k, g.ep);
+  SV_LAUNCH_CHECK();
+  return SV_OK;
+}
+
+template <typename T, typename O>
+int few_typed(const Gemm& g, cudaStream_t s) {
+  if (g.m <= 1) return launch_few<T, O, 1>(g, s);
+  if (g.m <= 2) return launch_few<T, O, 2>(g, s);
+  if (g.m <= 4) return launch_few<T, O, 4>(g, s);
+  return launch_few<T, O, FEW_ROWS>(g, s);
+}
+
+int gemm_few(const Gemm& g, cudaStream_t s) {
+  switch (g.dtype) {
+    case SV_FLOAT32: return few_typed<float, float>(g, s);
+    case SV_FLOAT16: return few_typed<__half, __half>(g, s);
+    case SV_BFLOAT16: return few_typed<__nv_bfloat16, __nv_bfloat16>(g, s);
+    default:
+      return g.ep.out_dtype == SV_FLOAT16 ? few_typed<__nv_fp8_e4m3, __half>(g, s)
+                                          : few_typed<__nv_fp8_e4m3, __nv_bfloat16>(g, s);
+  }
+}
+
+// ---- fp32 tiles --------------------------------------------------------------------------------
+
+constexpr int FK = 16;  // k per shared-memory stage
+
+// C tile of 16 R x 16 R, 256 threads with R x R sums each (R / 4 groups of four rows and columns,
+// 64 apart, so that the shared-memory reads are 16-byte and conflict-free).
+template <int R>
+__global__ void __launch_bounds__(256)
+    gemm_f32_kernel(Operand a, Operand b, int64_t m, int64_t n, int64_t k, int64_t k_part,
+                    Epilogue ep) {
+  constexpr int T = 16 * R;
+  constexpr int PER = T * FK / 256;  // elements of each operand a thread stages
+  __shared__ float sa[2][FK][T + 4];
+  __shared__ float sb[2][FK][T + 4];
+  const int tid = threadIdx.x;
+  const int tx = tid % 16, ty = tid / 16;
+  // columns vary fastest: blocks that run together share the rows of A
+  const unsigned across = (unsigned)((n + T - 1) / T);
+  const int64_t i0 = (int64_t)(blockIdx.x / across) * T, j0 = (int64_t)(blockIdx.x % across) * T;
+  const int64_t k0 = (int64_t)blockIdx.y * k_part;
+  const int64_t k1 = k0 + k_part < k ? k0 + k_part : k;
+  float ra[PER], rb[PER];
+  auto fetch = [&](const Operand& o, int64_t r0, int64_t rows, int64_t l0, float (&v)[PER]) {
+    const float* p = static_cast<const float*>(o.p);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const int at = tid + 256 * e;
+      const int r = o.mn ? at % T : at / FK, l = o.mn ? at / T : at % FK;
+      const int64_t i = r0 + r, ll = l0 + l;
+      v[e] = i < rows && ll < k1 ? __ldg(p + (o.mn ? ll * o.ld + i : i * o.ld + ll)) : 0.f;
+    }
+  };
+  auto put = [&](const Operand& o, float (&s)[FK][T + 4], const float (&v)[PER]) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const int at = tid + 256 * e;
+      const int r = o.mn ? at % T : at / FK, l = o.mn ? at / T : at % FK;
+      s[l][r] = v[e];
+    }
+  };
+  float acc[R][R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) acc[i][j] = 0.f;
+  fetch(a, i0, m, k0, ra);
+  fetch(b, j0, n, k0, rb);
+  put(a, sa[0], ra);
+  put(b, sb[0], rb);
+  __syncthreads();
+  int buf = 0;
+  for (int64_t l0 = k0; l0 < k1; l0 += FK, buf ^= 1) {
+    const bool more = l0 + FK < k1;
+    if (more) {
+      fetch(a, i0, m, l0 + FK, ra);
+      fetch(b, j0, n, l0 + FK, rb);
+    }
+#pragma unroll
+    for (int l = 0; l < FK; ++l) {
+      float av[R], bv[R];
+#pragma unroll
+      for (int q = 0; q < R / 4; ++q) {
+        *reinterpret_cast<float4*>(av + 4 * q) =
+            *reinterpret_cast<const float4*>(&sa[buf][l][64 * q + 4 * ty]);
+        *reinterpret_cast<float4*>(bv + 4 * q) =
+            *reinterpret_cast<const float4*>(&sb[buf][l][64 * q + 4 * tx]);
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+    }
+    if (more) {
+      put(a, sa[buf ^ 1], ra);
+      put(b, sb[buf ^ 1], rb);
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int64_t row = i0 + 64 * (i / 4) + 4 * ty + i % 4;
+    if (row >= m) continue;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int64_t col = j0 + 64 * (j / 4) + 4 * tx + j % 4;
+      if (col >= n) continue;
+      if (ep.partial)
+        ep.partial[((int64_t)blockIdx.y * m + row) * n + col] = acc[i][j];
+      else
+        epilogue_store<float>(ep, row, col, n, acc[i][j]);
+    }
+  }
+}
+
+int gemm_f32(const Gemm& g, bool small, cudaStream_t s) {
+  const int tile = small ? 64 : 128;
+  const int64_t k_part = (((g.k + g.splits - 1) / g.splits + FK - 1) / FK) * FK;
+  const int64_t tiles = ((g.m + tile - 1) / tile) * ((g.n + tile - 1) / tile);
+  if (tiles > INT32_MAX) SV_FAIL(SV_ERR_UNSUPPORTED, "linear: too many tiles");
+  const dim3 grid((unsigned)tiles, (unsigned)g.splits);
+  if (small)
+    gemm_f32_kernel<4><<<grid, 256, 0, s>>>(g.a, g.b, g.m, g.n, g.k, k_part, g.ep);
+  else
+    gemm_f32_kernel<8><<<grid, 256, 0, s>>>(g.a, g.b, g.m, g.n, g.k, k_part, g.ep);
+  SV_LAUNCH_CHECK();
+  return SV_OK;
+}
+
+// ---- second passes -----------------------------------------------------------------------------
+
+// Adds the parts of a split product in order and applies the epilogue (no parts: sums of zero).
+template <typename O>
+__global__ void __launch_bounds__(256)
+    finish_kernel(const float* __restrict__ partial, int splits, int64_t m, int64_t n,
+                  Epilogue ep) {
+  const int64_t cells = m * n;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < cells;
+       at += (int64_t)gridDim.x * 256) {
+    float v = 0.f;
+    for (int p = 0; p < splits; ++p) v += partial[p * cells + at];
+    epilogue_store<O>(ep, at / n, at % n, n, v);
+  }
+}
+
+int finish(const Gemm& g, const float* partial, int splits, cudaStream_t s) {
+  Epilogue ep = g.ep;
+  ep.partial = nullptr;
+  const unsigned blocks =
+      (unsigned)std::min<int64_t>((g.m * g.n + 255) / 256, (int64_t)num_sms() * 8);
+  if (ep.out_dtype == SV_FLOAT32)
+    finish_kernel<float><<<blocks, 256, 0, s>>>(partial, splits, g.m, g.n, ep);
+  else if (ep.out_dtype == SV_FLOAT16)
+    finish_kernel<__half><<<blocks, 256, 0, s>>>(partial, splits, g.m, g.n, ep);
+  else
+    finish_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(partial, splits, g.m, g.n, ep);
+  SV_LAUNCH_CHECK();
+  return SV_OK;
+}
+
+// Rows of `bytes` bytes into rows `to` bytes apart (a multiple of 16); E is the widest word that
+// divides both sides.
+template <typename E>
+__global__ void __launch_bounds__(256)
+    pad_rows_kernel(const E* __restrict__ in, int64_t rows, int64_t words, int64_t ld_in,
+                    E* __restrict__ out, int64_t ld_out) {
+  const int64_t total = rows * words;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total;
+       at += (int64_t)gridDim.x * 256) {
+    const int64_t r = at / words, c = at - r * words;
+    out[r * ld_out + c] = in[r * ld_in + c];
+  }
+}
+
+template <typename E>
+int pad_rows(const void* in, int64_t rows, int64_t words, int64_t ld_in, void* out, int64_t ld_out,
+             cudaStream_t s) {
+  const unsigned blocks =
+      (unsigned)std::min<int64_t>((rows * words + 255) / 256, (int64_t)num_sms() * 16);
+  pad_rows_kernel<E><<<blocks, 256, 0, s>>>(static_cast<const E*>(in), rows, words, ld_in,
+                                            static_cast<E*>(out), ld_out);
+  SV_LAUNCH_CHECK();
+  return SV_OK;
+}
+
+// dz = dy * act'(z) and the column sums of dz: a block takes COLS columns (V to a thread) of a
+// strip of rows, eight rows at a time, and writes one row of `partial` for its strip.
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+    dz_kernel(const T* __restrict__ dy, const T* __restrict__ z, int64_t m, int64_t n, int act,
+              int64_t rows_per_strip, T* __restrict__ dz, float* __restrict__ partial) {
+  __shared__ float s_sum[8][32 * V + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * V;
+  const int64_t r0 = (int64_t)blockIdx.y * rows_per_strip;
+  const int64_t r1 = r0 + rows_per_strip < m ? r0 + rows_per_strip : m;
+  float sum[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) sum[e] = 0.f;
+  if (c < n) {
+#pragma unroll 4
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+      T d[V], zz[V];
+      if constexpr (V * sizeof(T) == 16) {
+        *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(dy + r * n + c);
+        if (z) *reinterpret_cast<uint4*>(zz) = *reinterpret_cast<const uint4*>(z + r * n + c);
+      } else {
+        d[0] = dy[r * n + c];
+        if (z) zz[0] = z[r * n + c];
+      }
+      if (z) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float v = to_float(d[e]) * activate_slope(to_float(zz[e]), act);
+          sum[e] += v;
+          d[e] = from_f32<T>(v);
+        }
+        if constexpr (V * sizeof(T) == 16)
+          *reinterpret_cast<uint4*>(dz + r * n + c) = *reinterpret_cast<const uint4*>(d);
+        else
+          dz[r * n + c] = d[0];
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] += to_float(d[e]);
+      }
+    }
+  }
+  if (partial == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < V; ++e) s_sum[warp][lane * V + e] = sum[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * V; i += 256) {
+    const int64_t col = (int64_t)blockIdx.x * 32 * V + i;
+    if (col < n) {
+      float v = s_sum[0][i];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) v += s_sum[w][i];
+      partial[(int64_t)blockIdx.y * n + col] = v;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    dbias_kernel(const float* __restrict__ partial, int strips, int64_t n, T* __restrict__ out) {
+  __shared__ float s[8][33];
+  const int lane = threadIdx.x & 31, r0 = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float v = 0.f;
+  if (c < n)
+    for (int r = r0; r < strips; r += 8) v += partial[(int64_t)r * n + c];
+  s[r0][lane] = v;
+  __syncthreads();
+  if (r0 == 0 && c < n) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v += s[i][lane];
+    out[c] = from_f32<T>(v);
+  }
+}
+
+constexpr int MAX_STRIPS = 592;
+
+int strips_for(int64_t m, int64_t n, int v) {
+  const int64_t across = (n + 32 * v - 1) / (32 * v);
+  const int64_t want = std::max<int64_t>(1, MAX_STRIPS / across);
+  return (int)std::min<int64_t>(want, (m + 7) / 8);
+}
+
+template <typename T, int V>
+int launch_dz(const void* dy, const void* z, int64_t m, int64_t n, int act, void* dz, void* db,
+              float* partial, cudaStream_t s) {
+  const int strips = strips_for(m, n, V);
+  const int64_t per = (m + strips - 1) / strips;
+  const dim3 grid((unsigned)((n + 32 * V - 1) / (32 * V)), (unsigned)strips);
+  dz_kernel<T, V><<<grid, 256, 0, s>>>(static_cast<const T*>(dy), static_cast<const T*>(z), m, n,
+                                       act, per, static_cast<T*>(dz), db ? partial : nullptr);
+  SV_LAUNCH_CHECK();
+  if (db) {
+    dbias_kernel<T><<<(unsigned)((n + 31) / 32), 256, 0, s>>>(partial, strips, n,
+                                                             static_cast<T*>(db));
+    SV_LAUNCH_CHECK();
+  }
+  return SV_OK;
+}
+
+template <typename T>
+int dz_typed(const void* dy, const void* z, int64_t m, int64_t n, int act, void* dz, void* db,
+             float* partial, cudaStream_t s) {
+  constexpr int VE = 16 / sizeof(T);
+  const bool vec = n % VE == 0 && aligned16(dy) && aligned16(z) && aligned16(dz);
+  return vec ? launch_dz<T, VE>(dy, z, m, n, act, dz, db, partial, s)
+             : launch_dz<T, 1>(dy, z, m, n, act, dz, db, partial, s);
+}
+
+// ---- the plan of one product -------------------------------------------------------------------
+
+enum class Path { kEmpty, kFew, kF32, kTensor };
+
+struct Plan {
+  Path path;
+  int bn;       // tensor-core tile width, or 64 / 128 for the fp32 tiles
+  int splits;
+  size_t partial_bytes;
+};
+
+// The operand's extent in memory: `rows` rows of `cols` consecutive elements.
+struct Extent {
+  int64_t rows, cols;
+};
+Extent extent(bool mn, int64_t outer, int64_t k) {
+  return mn ? Extent{k, outer} : Extent{outer, k};
+}
+
+bool tma_ready(const Operand& o, int dtype) {
+  return aligned16(o.p) && o.ld * elem_size(dtype) % 16 == 0;
+}
+
+size_t copy_bytes(const Extent& e, int dtype) {
+  return align_up((size_t)e.rows * align_up((size_t)e.cols * elem_size(dtype), 16), COPY_ALIGN);
+}
+
+Plan plan_gemm(int64_t m, int64_t n, int64_t k, int dtype, bool a_mn, bool b_mn) {
+  Plan p{};
+  p.splits = 1;
+  if (m == 0 || n == 0 || k == 0) {
+    p.path = Path::kEmpty;
+    return p;
+  }
+  if (m <= FEW_ROWS && !a_mn && !b_mn) {
+    p.path = Path::kFew;
+    return p;
+  }
+  const int64_t sms = num_sms();
+  int64_t tiles, steps;  // tiles of the result, k blocks of a tile
+  if (dtype == SV_FLOAT32) {
+    p.path = Path::kF32;
+    tiles = ((m + 127) / 128) * ((n + 127) / 128);
+    p.bn = 128;
+    if (tiles < sms) {
+      p.bn = 64;
+      tiles = ((m + 63) / 64) * ((n + 63) / 64);
+    }
+    steps = (k + 4 * FK - 1) / (4 * FK);
+  } else {
+    p.path = Path::kTensor;
+    const int64_t rows = (m + 127) / 128;
+    // the widest tile that still gives every SM one: 256 columns re-read A least
+    p.bn = 256;
+    while (p.bn > 64 && (rows * ((n + p.bn - 1) / p.bn) < sms || n <= p.bn / 2)) p.bn /= 2;
+    tiles = rows * ((n + p.bn - 1) / p.bn);
+    steps = (k * elem_size(dtype) + 127) / 128;
+  }
+  // Split the k axis while tiles are fewer than SMs, each part at least 4 blocks long: a part
+  // costs an fp32 tile written and read again.
+  if (tiles < sms && steps >= 8) {
+    const int64_t want = std::min(sms / tiles, steps / 4);
+    if (want > 1) {
+      const int64_t part = (steps + std::min<int64_t>(want, 64) - 1) / std::min<int64_t>(want, 64);
+      p.splits = (int)((steps + part - 1) / part);  // no part is empty
+      p.partial_bytes = align_up((size_t)p.splits * m * n * 4, COPY_ALIGN);
+    }
+  }
+  return p;
+}
+
+size_t plan_bytes(const Plan& p, int64_t m, int64_t n, int64_t k, int dtype, bool a_mn, bool b_mn,
+                  bool copy_a, bool copy_b) {
+  size_t bytes = p.partial_bytes;
+  if (p.path == Path::kTensor) {
+    if (copy_a) bytes += copy_bytes(extent(a_mn, m, k), dtype);
+    if (copy_b) bytes += copy_bytes(extent(b_mn, n, k), dtype);
+  }
+  return bytes;
+}
+
+int copy_operand(Operand* o, const Extent& e, int dtype, uint8_t** at, cudaStream_t s) {
+  const int es = elem_size(dtype);
+  const int64_t row_bytes = e.cols * es;
+  const int64_t to = (int64_t)align_up((size_t)row_bytes, 16);
+  int rc;
+  if (es == 2)
+    rc = pad_rows<uint16_t>(o->p, e.rows, e.cols, o->ld, *at, to / 2, s);
+  else
+    rc = pad_rows<uint8_t>(o->p, e.rows, e.cols, o->ld, *at, to, s);
+  o->p = *at;
+  o->ld = to / es;
+  *at += copy_bytes(e, dtype);
+  return rc;
+}
+
+int run_gemm(Gemm g, void* workspace, size_t workspace_bytes, int32_t* status, cudaStream_t s,
+             const char* what) {
+  const Plan p = plan_gemm(g.m, g.n, g.k, g.dtype, g.a.mn, g.b.mn);
+  if (g.m == 0 || g.n == 0) return SV_OK;
+  if (p.path == Path::kEmpty) return finish(g, nullptr, 0, s);
+  if (p.path == Path::kFew) return gemm_few(g, s);
+  const bool copy_a = !tma_ready(g.a, g.dtype), copy_b = !tma_ready(g.b, g.dtype);
+  const size_t need = plan_bytes(p, g.m, g.n, g.k, g.dtype, g.a.mn, g.b.mn, copy_a, copy_b);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    SV_FAIL(SV_ERR_WORKSPACE, std::string(what) + ": workspace too small or unaligned");
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  float* partial = nullptr;
+  g.splits = p.splits;
+  if (p.splits > 1) {
+    partial = reinterpret_cast<float*>(at);
+    at += p.partial_bytes;
+    g.ep.partial = partial;
+  }
+  int rc;
+  if (p.path == Path::kF32) {
+    rc = gemm_f32(g, p.bn == 64, s);
+  } else {
+    if (copy_a && (rc = copy_operand(&g.a, extent(g.a.mn, g.m, g.k), g.dtype, &at, s)) != SV_OK)
+      return rc;
+    if (copy_b && (rc = copy_operand(&g.b, extent(g.b.mn, g.n, g.k), g.dtype, &at, s)) != SV_OK)
+      return rc;
+    rc = gemm_tc(g, p.bn, status, s);
+  }
+  if (rc != SV_OK || p.splits == 1) return rc;
+  return finish(g, partial, p.splits, s);
+}
+
+bool float_dtype(int d) { return d == SV_FLOAT32 || d == SV_FLOAT16 || d == SV_BFLOAT16; }
+
+int check_sizes(int64_t m, int64_t k, int64_t n, const char* what) {
+  if (m < 0 || k < 0 || n < 0)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, std::string(what) + ": negative size");
+  if (m > INT32_MAX - 256 || k > INT32_MAX - 256 || n > INT32_MAX - 256)
+    SV_FAIL(SV_ERR_UNSUPPORTED, std::string(what) + ": sizes must be below 2^31 - 256");
+  return SV_OK;
+}
+
+}  // namespace
+}  // namespace sv
+
+using namespace sv;
+
+extern "C" size_t sv_linear_workspace_bytes(int pass, int64_t m, int64_t k, int64_t n, int dtype,
+                                            int copies) {
+  if (m < 0 || k < 0 || n < 0 || (!float_dtype(dtype) && dtype != SV_FLOAT8_E4M3)) return 0;
+  const bool a = copies & 1, b = copies & 2;
+  switch (pass) {
+    case SV_LINEAR_FORWARD:
+      return plan_bytes(plan_gemm(m, n, k, dtype, false, false), m, n, k, dtype, false, false, a, b);
+    case SV_LINEAR_DX:
+      return plan_bytes(plan_gemm(m, k, n, dtype, false, true), m, k, n, dtype, false, true, a, b);
+    case SV_LINEAR_DW:
+      return plan_bytes(plan_gemm(n, k, m, dtype, true, true), n, k, m, dtype, true, true, a, b);
+    case SV_LINEAR_DZ:
+      return (size_t)MAX_STRIPS * n * sizeof(float);
+    default:
+      return 0;
+  }
+}
+
+extern "C" int sv_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                                 const void* bias, const void* residual, int64_t ld_res,
+                                 const float* x_scale, const float* w_scale, int64_t m, int64_t k,
+                                 int64_t n, int dtype, int out_dtype, int activation, void* out,
+                                 void* preact, void* workspace, size_t workspace_bytes,
+                                 int32_t* status, sv_stream_t stream) {
+  const int rc = check_sizes(m, k, n, "sv_linear_forward");
+  if (rc != SV_OK) return rc;
+  const bool e4m3 = dtype == SV_FLOAT8_E4M3;
+  if (!float_dtype(dtype) && !e4m3)
+    SV_FAIL(SV_ERR_BAD_DTYPE, "sv_linear_forward: unknown dtype");
+  if (e4m3 ? (out_dtype != SV_FLOAT16 && out_dtype != SV_BFLOAT16) : out_dtype != dtype)
+    SV_FAIL(SV_ERR_BAD_DTYPE,
+            "sv_linear_forward: the output has the operands' type, or is fp16 / bf16 for e4m3");
+  if (activation < SV_ACT_NONE || activation > SV_ACT_GELU_TANH)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_linear_forward: unknown activation");
+  if (m == 0 || n == 0) return SV_OK;
+  if (!out || (k > 0 && (!x || !weight)))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_linear_forward: null pointer");
+  if (ldx < k || ldw < k || (residual && ld_res < n))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_linear_forward: row stride below the row length");
+  Gemm g{{x, ldx, false}, {weight, ldw, false}, m, n, k, dtype, 1,
+         {bias, residual, ld_res, x_scale, w_scale, out, preact, nullptr, out_dtype, activation}};
+  return run_gemm(g, workspace, workspace_bytes, status, to_stream(stream), "sv_linear_forward");
+}
+
+extern "C" int sv_linear_backward_z(const void* dout, const void* preact, int64_t m, int64_t n,
+                                    int dtype, int activation, void* dz, void* dbias,
+                                    void* workspace, size_t workspace_bytes, sv_stream_t stream) {
+  const int rc = check_sizes(m, 0, n, "sv_linear_backward_z");
+  if (rc != SV_OK) return rc;
+  if (!float_dtype(dtype)) SV_FAIL(SV_ERR_BAD_DTYPE, "sv_linear_backward_z: unknown dtype");
+  if (activation < SV_ACT_NONE || activation > SV_ACT_GELU_TANH)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_linear_backward_z: unknown activation");
+  cudaStream_t s = to_stream(stream);
+  if (n == 0) return SV_OK;
+  if (m == 0) {
+    if (dbias) SV_CUDA_TRY(cudaMemsetAsync(dbias, 0, n * elem_size(dtype), s));
+    return SV_OK;
+  }
+  const bool act = activation != SV_ACT_NONE;
+  if (!dout || (act && (!preact || !dz)))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_linear_backward_z: null pointer");
+  if (!act && !dbias) return SV_OK;
+  if (dbias && (!workspace || workspace_bytes < (size_t)MAX_STRIPS * n * sizeof(float)))
+    SV_FAIL(SV_ERR_WORKSPACE, "sv_linear_backward_z: workspace too small");
+  const void* z = act ? preact : nullptr;
+  void* d = act ? dz : nullptr;
+  float* partial = static_cast<float*>(workspace);
+  if (dtype == SV_FLOAT32) return dz_typed<float>(dout, z, m, n, activation, d, dbias, partial, s);
+  if (dtype == SV_FLOAT16) return dz_typed<__half>(dout, z, m, n, activation, d, dbias, partial, s);
+  return dz_typed<__nv_bfloat16>(dout, z, m, n, activation, d, dbias, partial, s);
+}
+
+extern "C" int sv_linear_dx(const void* dz, const void* weight, int64_t ldw, int64_t m, int64_t k,
+                            int64_t n, int dtype, void* dx, void* workspace,
+                            size_t workspace_bytes, int32_t* status, sv_stream_t stream) {
+  const int rc = check_sizes(m, k, n, "sv_linear_dx");
+  if (rc != SV_OK) return rc;
+  if (!float_dtype(dtype)) SV_FAIL(SV_ERR_BAD_DTYPE, "sv_linear_dx: unknown dtype");
+  if (m == 0 || k == 0) return SV_OK;
+  if (!dx || (n > 0 && (!dz || !weight)))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_linear_dx: null pointer");
+  if (ldw < k) SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_linear_dx: row stride below the row length");
+  Gemm g{{dz, n, false}, {weight, ldw, true}, m, k, n, dtype, 1,
+         {nullptr, nullptr, 0, nullptr, nullptr, dx, nullptr, nullptr, dtype, SV_ACT_NONE}};
+  return run_gemm(g, workspace, workspace_bytes, status, to_stream(stream), "sv_linear_dx");
+}
+
+extern "C" int sv_linear_dw(const void* dz, const void* x, int64_t ldx, int64_t m, int64_t k,
+                            int64_t n, int dtype, void* dw, void* workspace,
+                            size_t workspace_bytes, int32_t* status, sv_stream_t stream) {
+  const int rc = check_sizes(m, k, n, "sv_linear_dw");
+  if (rc != SV_OK) return rc;
+  if (!float_dtype(dtype)) SV_FAIL(SV_ERR_BAD_DTYPE, "sv_linear_dw: unknown dtype");
+  if (n == 0 || k == 0) return SV_OK;
+  if (!dw || (m > 0 && (!dz || !x)))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_linear_dw: null pointer");
+  if (ldx < k) SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_linear_dw: row stride below the row length");
+  Gemm g{{dz, n, true}, {x, ldx, true}, n, k, m, dtype, 1,
+         {nullptr, nullptr, 0, nullptr, nullptr, dw, nullptr, nullptr, dtype, SV_ACT_NONE}};
+  return run_gemm(g, workspace, workspace_bytes, status, to_stream(stream), "sv_linear_dw");
+}

@@ -1,0 +1,96 @@
+// The projection's shared pieces: operands, the fused epilogue, and what the two matrix-product
+// kernels (linear_tc.cu on the tensor cores, linear.cu on the CUDA cores) take.
+#pragma once
+
+#include "common.cuh"
+
+namespace sv {
+
+inline int elem_size(int dtype) {
+  return dtype == SV_FLOAT32 ? 4 : (dtype == SV_FLOAT8_E4M3 ? 1 : 2);
+}
+
+// One operand of C[i][j] = sum_l A(i, l) B(j, l): element (i, l) is at p[i * ld + l], or at
+// p[l * ld + i] when `mn` is set (the rows of the product run along memory).
+struct Operand {
+  const void* p;
+  int64_t ld;
+  bool mn;
+};
+
+// y = act(acc * row_scale[i] * col_scale[j] + bias[j]) + residual[i][j], every pointer optional;
+// `preact` receives the activation's argument. With `partial` set the kernel stores its raw fp32
+// sums there ([splits][M][N]) and a second pass applies the rest.
+struct Epilogue {
+  const void* bias;      // [N], out_dtype
+  const void* residual;  // out_dtype, rows ld_res apart
+  int64_t ld_res;
+  const float* row_scale;
+  const float* col_scale;
+  void* out;     // [M][N] contiguous, out_dtype
+  void* preact;  // [M][N] contiguous, out_dtype
+  float* partial;
+  int out_dtype;
+  int act;
+};
+
+struct Gemm {
+  Operand a, b;
+  int64_t m, n, k;
+  int dtype;
+  int splits;  // parts of the k axis
+  Epilogue ep;
+};
+
+// linear_tc.cu. `bn`: the tile's width. Operands 16-byte aligned with row strides of a multiple of 16 bytes.
+int gemm_tc(const Gemm& g, int bn, int32_t* status, cudaStream_t s);
+
+#ifdef __CUDACC__
+constexpr float SQRT_HALF = 0.70710678118654752f;
+constexpr float GELU_TANH_2C = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float GELU_CUBE = 0.044715f;
+
+// exp and the quotient are the fast forms: within a few fp32 ulp of the value over the whole
+// range (x / (1 + inf) is 0), which is the error the fp32 path's tolerance counts.
+__device__ __forceinline__ float sigmoid_f(float x) {
+  return __fdividef(1.0f, 1.0f + __expf(-x));
+}
+
+__device__ __forceinline__ float activate(float z, int act) {
+  if (act == SV_ACT_SILU) return z * sigmoid_f(z);
+  if (act == SV_ACT_GELU) return 0.5f * z * (1.0f + erff(z * SQRT_HALF));
+  // 0.5 (1 + tanh(u)) = sigmoid(2u): no cancellation for negative z
+  if (act == SV_ACT_GELU_TANH) return z * sigmoid_f(GELU_TANH_2C * (z + GELU_CUBE * z * z * z));
+  return z;
+}
+
+// The activation's derivative.
+__device__ __forceinline__ float activate_slope(float z, int act) {
+  if (act == SV_ACT_SILU) {
+    const float g = sigmoid_f(z);
+    return g * (1.0f + z * (1.0f - g));
+  }
+  if (act == SV_ACT_GELU)
+    return 0.5f * (1.0f + erff(z * SQRT_HALF)) +
+           z * 0.39894228040143268f * __expf(-0.5f * z * z);
+  if (act == SV_ACT_GELU_TANH) {
+    const float g = sigmoid_f(GELU_TANH_2C * (z + GELU_CUBE * z * z * z));
+    return g + z * g * (1.0f - g) * GELU_TANH_2C * (1.0f + 3.0f * GELU_CUBE * z * z);
+  }
+  return 1.0f;
+}
+
+template <typename O>
+__device__ __forceinline__ void epilogue_store(const Epilogue& ep, int64_t i, int64_t j, int64_t n,
+                                               float acc) {
+  if (ep.row_scale) acc *= __ldg(ep.row_scale + i);
+  if (ep.col_scale) acc *= __ldg(ep.col_scale + j);
+  if (ep.bias) acc += to_f32(static_cast<const O*>(ep.bias)[j]);
+  if (ep.preact) static_cast<O*>(ep.preact)[i * n + j] = from_f32<O>(acc);
+  acc = activate(acc, ep.act);
+  if (ep.residual) acc += to_f32(static_cast<const O*>(ep.residual)[i * ep.ld_res + j]);
+  static_cast<O*>(ep.out)[i * n + j] = from_f32<O>(acc);
+}
+#endif
+
+}  // namespace sv

@@ -1,0 +1,439 @@
+// Root-mean-square norm of feature rows with the residual's addition, an optional 8-bit output
+// with one scale per row, and its gradients.
+//
+//     h    = round(x + residual)                     (x itself without a residual)
+//     rstd = 1 / sqrt(mean(h^2) + eps)
+//     y    = h * rstd * w
+//     8 bits: s = max|y| / 448 (1 for a row of zeros), q = round_e4m3(y / s)
+//     dx   = rstd * (g - h * rstd^2 * mean(g h)) + dh,  g = dy * w   (the residual's gradient too)
+//     dw_c = sum over the rows of dy_c * h_c * rstd
+//
+// h is rounded to the feature type before it is normed: it is the residual stream that the next
+// block reads, and the backward pass then differentiates at the point the forward pass used.
+// Everything else stays in fp32 with one rounding at the end.
+//
+// Both passes move each row once and do about ten operations per element, so HBM bounds them. A
+// row lives in the registers of TPR threads (J accesses of V elements each; 16-byte accesses when
+// the rows allow them, single elements otherwise).
+#include <cuda_fp8.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace sv {
+namespace {
+
+constexpr int RMS_THREADS = 256;
+constexpr float E4M3_MAX = 448.0f;
+constexpr int RMS_MAX_CHANNELS = 8192;
+
+struct RmsArgs {
+  int64_t n;
+  int channels;
+  int64_t x_stride, res_stride;  // elements between rows
+  float eps;
+  const float* weight;  // [C] or null
+  float* rstd;          // [n] or null
+  float* scale;         // [n], 8-bit output only
+};
+
+// 16-byte vectors go through uint4, so that they are one access.
+template <typename T, int V>
+__device__ __forceinline__ void load_row(const T* p, float (&v)[V]) {
+  if constexpr (V * sizeof(T) == 16) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = to_f32(e[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = to_f32(p[k]);
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_row(T* p, const float (&v)[V]) {
+  if constexpr (V * sizeof(T) == 16) {
+    uint4 raw;
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int k = 0; k < V; ++k) e[k] = from_f32<T>(v[k]);
+    *reinterpret_cast<uint4*>(p) = raw;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) p[k] = from_f32<T>(v[k]);
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void load_weight(const float* w, int c, float (&v)[V]) {
+  if (w == nullptr) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 1.f;
+  } else if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(w + c + k));
+      v[k] = f.x; v[k + 1] = f.y; v[k + 2] = f.z; v[k + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = __ldg(w + c + k);
+  }
+}
+
+struct Sum {
+  static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+// Keeps a NaN (fmaxf drops it), so that a row with one gets a NaN scale.
+struct Max {
+  static __device__ __forceinline__ float of(float a, float b) {
+    return a > b || a != a ? a : b;
+  }
+};
+
+// Reduction over the TPR threads of a row; every thread gets the result. With TPR > 32 the block
+// is one row and `part` holds a word per warp.
+template <typename Op, int TPR>
+__device__ __forceinline__ float row_reduce(float v, float* part) {
+#pragma unroll
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
+    v = Op::of(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if constexpr (TPR > 32) {
+    constexpr int W = TPR / 32;
+    __syncthreads();  // the previous use of `part` is over
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) v = Op::of(v, part[i]);
+  }
+  return v;
+}
+
+template <int TPR>
+constexpr int kBlock = TPR > 32 ? TPR : RMS_THREADS;
+
+template <typename T, int V, int TPR, int J, bool Q8>
+__global__ void __launch_bounds__(kBlock<TPR>)
+    rms_kernel(const T* __restrict__ x, const T* __restrict__ res, RmsArgs a, T* __restrict__ h_out,
+               void* __restrict__ out) {
+  constexpr int ROWS = kBlock<TPR> / TPR;
+  __shared__ float part[TPR > 32 ? TPR / 32 : 1];
+  const int sub = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  const bool live = row < a.n;
+  const int C = a.channels;
+  float v[J][V];
+  float sq = 0.f;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int c = (sub + TPR * j) * V;
+    if (live && c < C) {
+      load_row<T, V>(x + row * a.x_stride + c, v[j]);
+      if (res != nullptr) {
+        float r[V];
+        load_row<T, V>(res + row * a.res_stride + c, r);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[j][k] = to_f32(from_f32<T>(v[j][k] + r[k]));
+        if (h_out != nullptr) store_row<T, V>(h_out + row * C + c, v[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) sq = fmaf(v[j][k], v[j][k], sq);
+    }
+  }
+  sq = row_reduce<Sum, TPR>(sq, part);
+  const float rstd = 1.0f / sqrtf(sq / (float)C + a.eps);
+  if (live && sub == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int c = (sub + TPR * j) * V;
+    if (live && c < C) {
+      float w[V];
+      load_weight<V>(a.weight, c, w);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[j][k] = v[j][k] * rstd * w[k];
+      if constexpr (Q8) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) top = Max::of(top, fabsf(v[j][k]));
+      } else {
+        store_row<T, V>(static_cast<T*>(out) + row * C + c, v[j]);
+      }
+    }
+  }
+  if constexpr (Q8) {
+    top = row_reduce<Max, TPR>(top, part);
+    const float scale = top == 0.f ? 1.f : top / E4M3_MAX;
+    if (!live) return;
+    if (sub == 0) a.scale[row] = scale;
+    uint8_t* q = static_cast<uint8_t*>(out) + row * C;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = (sub + TPR * j) * V;
+      if (c < C) {
+        if constexpr (V % 4 == 0) {
+          uint32_t packed[V / 4];
+#pragma unroll
+          for (int k = 0; k < V; k += 4) {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(
+                make_float2(v[j][k] / scale, v[j][k + 1] / scale), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(
+                make_float2(v[j][k + 2] / scale, v[j][k + 3] / scale), __NV_SATFINITE, __NV_E4M3);
+            packed[k / 4] = lo | hi << 16;
+          }
+          if constexpr (V == 8)
+            *reinterpret_cast<uint2*>(q + c) = make_uint2(packed[0], packed[1]);
+          else
+            *reinterpret_cast<uint32_t*>(q + c) = packed[0];
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            q[c + k] = __nv_cvt_float_to_fp8(v[j][k] / scale, __NV_SATFINITE, __NV_E4M3);
+        }
+      }
+    }
+  }
+}
+
+// Gradients: each group of TPR threads takes rows group, group + groups, ... and keeps its
+// channels' share of dw in registers; a block adds its groups in order through shared memory and
+// writes one row of `partial` ([gridDim.x, C]), which column_sum_kernel adds in a fixed order.
+template <typename T, int V, int TPR, int J>
+__global__ void __launch_bounds__(kBlock<TPR>)
+    rms_backward_kernel(const T* __restrict__ h, const T* __restrict__ dy,
+                        const T* __restrict__ dh, RmsArgs a, T* __restrict__ dx,
+                        float* __restrict__ partial) {
+  constexpr int ROWS = kBlock<TPR> / TPR;
+  extern __shared__ float s_dw[];  // [C] when dw is wanted
+  __shared__ float part[TPR > 32 ? TPR / 32 : 1];
+  const int sub = threadIdx.x % TPR;
+  const int group = threadIdx.x / TPR;
+  const int C = a.channels;
+  float w[J][V], dw[J][V];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int c = (sub + TPR * j) * V;
+#pragma unroll
+    for (int k = 0; k < V; ++k) dw[j][k] = 0.f;
+    if (c < C) load_weight<V>(a.weight, c, w[j]);
+  }
+  const float inv_c = 1.0f / (float)C;
+  // the block's groups take consecutive rows, so every group makes the same number of rounds
+  for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.n; base += (int64_t)gridDim.x * ROWS) {
+    const int64_t row = base + group;
+    const bool live = row < a.n;
+    float hv[J][V], g[J][V];
+    float dot = 0.f;
+    const float rstd = live ? __ldg(a.rstd + row) : 0.f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = (sub + TPR * j) * V;
+      if (live && c < C) {
+        load_row<T, V>(h + row * a.x_stride + c, hv[j]);
+        load_row<T, V>(dy + row * C + c, g[j]);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          dw[j][k] = fmaf(g[j][k], hv[j][k] * rstd, dw[j][k]);
+          g[j][k] *= w[j][k];
+          dot = fmaf(g[j][k], hv[j][k], dot);
+        }
+      }
+    }
+    dot = row_reduce<Sum, TPR>(dot, part);
+    const float pull = dot * rstd * rstd * inv_c;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = (sub + TPR * j) * V;
+      if (live && c < C) {
+        float d[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) d[k] = rstd * (g[j][k] - hv[j][k] * pull);
+        if (dh != nullptr) {
+          float e[V];
+          load_row<T, V>(dh + row * C + c, e);
+#pragma unroll
+          for (int k = 0; k < V; ++k) d[k] += e[k];
+        }
+        store_row<T, V>(dx + row * C + c, d);
+      }
+    }
+  }
+  if (partial == nullptr) return;
+  for (int r = 0; r < ROWS; ++r) {
+    if (group == r) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int c = (sub + TPR * j) * V;
+        if (c < C) {
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            s_dw[c + k] = r == 0 ? dw[j][k] : s_dw[c + k] + dw[j][k];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (int c = threadIdx.x; c < C; c += blockDim.x)
+    partial[(int64_t)blockIdx.x * C + c] = s_dw[c];
+}
+
+// out[c] = sum of partial[0..rows)[c] in a fixed order: 32 channels a block, 8 strided row sums
+// a channel, joined in order.
+__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ partial,
+                                                         int rows, int channels,
+                                                         float* __restrict__ out) {
+  __shared__ float s[8][33];
+  const int lane = threadIdx.x & 31, r0 = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  float v = 0.f;
+  if (c < channels)
+    for (int r = r0; r < rows; r += 8) v += partial[(int64_t)r * channels + c];
+  s[r0][lane] = v;
+  __syncthreads();
+  if (r0 == 0 && c < channels) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v += s[i][lane];
+    out[c] = v;
+  }
+}
+
+template <typename F>
+int by_width(int nv, F&& f) {
+  if (nv <= 8) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+  if (nv <= 32) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+  if (nv <= 64) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 2>{});
+  if (nv <= 128) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+  if (nv <= 512) return f(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
+  if (nv <= 2048) return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
+  return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 16>{});
+}
+
+constexpr int BACKWARD_BLOCKS = 296;  // two per SM; also the rows of the dw partials
+
+template <typename T, int V>
+int launch_rms(const void* x, const void* res, const RmsArgs& a, void* h_out, void* out, bool q8,
+               cudaStream_t s) {
+  return by_width((a.channels + V - 1) / V, [&](auto tpr, auto j) -> int {
+    constexpr int TPR = decltype(tpr)::value, J = decltype(j)::value;
+    constexpr int ROWS = kBlock<TPR> / TPR;
+    const int64_t blocks = (a.n + ROWS - 1) / ROWS;
+    auto kernel = q8 ? rms_kernel<T, V, TPR, J, true> : rms_kernel<T, V, TPR, J, false>;
+    kernel<<<(unsigned)blocks, kBlock<TPR>, 0, s>>>(
+        static_cast<const T*>(x), static_cast<const T*>(res), a, static_cast<T*>(h_out), out);
+    SV_LAUNCH_CHECK();
+    return SV_OK;
+  });
+}
+
+template <typename T, int V>
+int launch_rms_backward(const void* h, const void* dy, const void* dh, const RmsArgs& a, void* dx,
+                        float* partial, float* dw, cudaStream_t s) {
+  return by_width((a.channels + V - 1) / V, [&](auto tpr, auto j) -> int {
+    constexpr int TPR = decltype(tpr)::value, J = decltype(j)::value;
+    constexpr int ROWS = kBlock<TPR> / TPR;
+    const int64_t want = (a.n + ROWS - 1) / ROWS;
+    const int blocks = (int)(want < BACKWARD_BLOCKS ? want : BACKWARD_BLOCKS);
+    rms_backward_kernel<T, V, TPR, J>
+        <<<blocks, kBlock<TPR>, dw ? a.channels * sizeof(float) : 0, s>>>(
+            static_cast<const T*>(h), static_cast<const T*>(dy), static_cast<const T*>(dh), a,
+            static_cast<T*>(dx), dw ? partial : nullptr);
+    SV_LAUNCH_CHECK();
+    if (dw != nullptr) {
+      column_sum_kernel<<<(a.channels + 31) / 32, 256, 0, s>>>(partial, blocks, a.channels, dw);
+      SV_LAUNCH_CHECK();
+    }
+    return SV_OK;
+  });
+}
+
+bool vec_ok(const void* p, int64_t stride, int esize) {
+  return p == nullptr || (aligned16(p) && stride * esize % 16 == 0);
+}
+
+int check_common(int64_t n, int channels, int dtype, float eps, const char* what) {
+  if (dtype != SV_FLOAT32 && dtype != SV_FLOAT16 && dtype != SV_BFLOAT16)
+    SV_FAIL(SV_ERR_BAD_DTYPE, std::string(what) + ": unknown dtype");
+  if (n < 0 || channels < 0) SV_FAIL(SV_ERR_INVALID_ARGUMENT, std::string(what) + ": negative size");
+  if (channels > RMS_MAX_CHANNELS)
+    SV_FAIL(SV_ERR_UNSUPPORTED, std::string(what) + ": at most 8192 channels");
+  if (n > (int64_t)INT32_MAX)
+    SV_FAIL(SV_ERR_UNSUPPORTED, std::string(what) + ": at most 2^31 - 1 rows");
+  if (!(eps >= 0.f)) SV_FAIL(SV_ERR_INVALID_ARGUMENT, std::string(what) + ": negative eps");
+  return SV_OK;
+}
+
+}  // namespace
+}  // namespace sv
+
+using namespace sv;
+
+extern "C" int sv_rms_norm(const void* x, int64_t x_stride, const void* residual,
+                           int64_t residual_stride, int64_t n, int channels, int dtype, float eps,
+                           const float* weight, void* h, float* rstd, void* out, int out_dtype,
+                           float* scale, sv_stream_t stream) {
+  const int rc = check_common(n, channels, dtype, eps, "sv_rms_norm");
+  if (rc != SV_OK) return rc;
+  const bool q8 = out_dtype == SV_FLOAT8_E4M3;
+  if (!q8 && out_dtype != dtype)
+    SV_FAIL(SV_ERR_BAD_DTYPE, "sv_rms_norm: the output has the input's type or is e4m3");
+  if (n == 0 || channels == 0) return SV_OK;
+  if (!x || !out || (q8 && !scale))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_rms_norm: null pointer");
+  if (x_stride < channels || (residual && residual_stride < channels))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_rms_norm: row stride below the channel count");
+  RmsArgs a{n, channels, x_stride, residual_stride, eps, weight, rstd, scale};
+  const int es = dtype_size(dtype);
+  const bool vec = channels * es % 16 == 0 && vec_ok(x, x_stride, es) &&
+                   vec_ok(residual, residual_stride, es) && vec_ok(h, channels, es) &&
+                   aligned16(out) && (!weight || aligned16(weight));
+  cudaStream_t s = to_stream(stream);
+  if (dtype == SV_FLOAT32)
+    return vec ? launch_rms<float, 4>(x, residual, a, h, out, q8, s)
+               : launch_rms<float, 1>(x, residual, a, h, out, q8, s);
+  if (dtype == SV_FLOAT16)
+    return vec ? launch_rms<__half, 8>(x, residual, a, h, out, q8, s)
+               : launch_rms<__half, 1>(x, residual, a, h, out, q8, s);
+  return vec ? launch_rms<__nv_bfloat16, 8>(x, residual, a, h, out, q8, s)
+             : launch_rms<__nv_bfloat16, 1>(x, residual, a, h, out, q8, s);
+}
+
+extern "C" size_t sv_rms_norm_backward_workspace_bytes(int channels) {
+  if (channels <= 0 || channels > RMS_MAX_CHANNELS) return 0;
+  return (size_t)BACKWARD_BLOCKS * channels * sizeof(float);
+}
+
+extern "C" int sv_rms_norm_backward(const void* h, int64_t h_stride, const void* dy,
+                                    const void* dh, int64_t n, int channels, int dtype,
+                                    const float* weight, const float* rstd, void* dx, float* dw,
+                                    void* workspace, size_t workspace_bytes, sv_stream_t stream) {
+  const int rc = check_common(n, channels, dtype, 0.f, "sv_rms_norm_backward");
+  if (rc != SV_OK) return rc;
+  cudaStream_t s = to_stream(stream);
+  if (channels == 0) return SV_OK;
+  if (n == 0) {
+    if (dw) SV_CUDA_TRY(cudaMemsetAsync(dw, 0, channels * sizeof(float), s));
+    return SV_OK;
+  }
+  if (!h || !dy || !rstd || !dx)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_rms_norm_backward: null pointer");
+  if (h_stride < channels)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_rms_norm_backward: row stride below the channel count");
+  if (dw && (!workspace || workspace_bytes < sv_rms_norm_backward_workspace_bytes(channels)))
+    SV_FAIL(SV_ERR_WORKSPACE, "sv_rms_norm_backward: workspace too small");
+  RmsArgs a{n, channels, h_stride, 0, 0.f, weight, const_cast<float*>(rstd), nullptr};
+  float* partial = static_cast<float*>(workspace);
+  const int es = dtype_size(dtype);
+  const bool vec = channels * es % 16 == 0 && vec_ok(h, h_stride, es) &&
+                   vec_ok(dy, channels, es) && vec_ok(dh, channels, es) &&
+                   vec_ok(dx, channels, es) && (!weight || aligned16(weight));
+  if (dtype == SV_FLOAT32)
+    return vec ? launch_rms_backward<float, 4>(h, dy, dh, a, dx, partial, dw, s)
+               : launch_rms_backward<float, 1>(h, dy, dh, a, dx, partial, dw, s);
+  if (dtype == SV_FLOAT16)
+    return vec ? launch_rms_backward<__half, 8>(h, dy, dh, a, dx, partial, dw, s)
+               : launch_rms_backward<__half, 1>(h, dy, dh, a, dx, partial, dw, s);
+  return vec ? launch_rms_backward<__nv_bfloat16, 8>(h, dy, dh, a, dx, partial, dw, s)
+             : launch_rms_backward<__nv_bfloat16, 1>(h, dy, dh, a, dx, partial, dw, s);
+}

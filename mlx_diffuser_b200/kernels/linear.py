@@ -1,0 +1,190 @@
+"""Linear projection of feature rows with bias, activation and residual in its epilogue
+(``sv_linear_*``): ``act(x @ weight.T + bias) + residual`` in one pass, with gradients, and with
+8-bit operands. ``SparseLinear`` (``src/mlx_diffuser/layers/trellis_sparse.py:13-30``) calls it when
+it is given an activation or a residual."""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _native as N
+
+
+def _row_major(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [rows, cols] as it is when its rows are contiguous and do not overlap."""
+
+    if t.stride(1) == 1 or t.shape[1] <= 1:
+        if t.shape[0] <= 1 or t.stride(0) >= t.shape[1]:
+            return t
+    return t.contiguous()
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride in elements (that of a lone row does not matter)."""
+
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _unaligned(t: torch.Tensor) -> bool:
+    return t.data_ptr() % 16 != 0 or _ld(t) * t.element_size() % 16 != 0
+
+
+def _workspace(which: int, m: int, k: int, n: int, code: int, a: torch.Tensor, b: torch.Tensor):
+    nbytes = N.load().sv_linear_workspace_bytes(which, m, k, n, code,
+                                                _unaligned(a) + 2 * _unaligned(b))
+    return (N.workspace(nbytes, a.device) if nbytes else None), nbytes
+
+
+def _forward(x, weight, bias, residual, activation, x_scale, w_scale, out_dtype, keep_preact):
+    m, k = x.shape
+    n = weight.shape[0]
+    dev = x.device
+    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    preact = torch.empty_like(out) if keep_preact else None
+    if out.numel() == 0:
+        return out, preact
+    code = N.DTYPE_CODE.get(x.dtype, N.SV_FLOAT8_E4M3)
+    with N.on_device(dev):
+        ws, nbytes = _workspace(N.SV_LINEAR_FORWARD, m, k, n, code, x, weight)
+        rc = N.load().sv_linear_forward(
+            x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight), N.ptr(bias), N.ptr(residual),
+            _ld(residual) if residual is not None else 0, N.ptr(x_scale), N.ptr(w_scale), m, k, n,
+            code, N.DTYPE_CODE[out_dtype], N.ACTIVATION_CODE[activation], out.data_ptr(),
+            N.ptr(preact), N.ptr(ws), nbytes, N.status_word(dev).data_ptr(), N.stream(dev))
+    N.check(rc, "linear")
+    return out, preact
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        acts = N.ACTIVATION_CODE[activation] != 0
+        out, preact = _forward(x, weight, bias, residual, activation, None, None, x.dtype, acts)
+        ctx.activation = activation
+        ctx.save_for_backward(x, weight, preact)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, weight, preact = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dout = dout.contiguous()
+        m, k = x.shape
+        n = weight.shape[0]
+        dev, dtype = x.device, x.dtype
+        code = N.DTYPE_CODE[dtype]
+        lib = N.load()
+        dx = dw = db = None
+        dz = dout
+        with N.on_device(dev):
+            status, stream = N.status_word(dev).data_ptr(), N.stream(dev)
+            if need_b or (preact is not None and (need_x or need_w)):
+                if preact is not None:
+                    dz = torch.empty_like(dout)
+                db = torch.empty(n, dtype=dtype, device=dev) if need_b else None
+                nbytes = lib.sv_linear_workspace_bytes(N.SV_LINEAR_DZ, m, k, n, code, 0)
+                ws = N.workspace(nbytes, dev) if need_b else None
+                rc = lib.sv_linear_backward_z(
+                    dout.data_ptr(), N.ptr(preact), m, n, code,
+                    N.ACTIVATION_CODE[ctx.activation], dz.data_ptr(), N.ptr(db), N.ptr(ws),
+                    nbytes, stream)
+                N.check(rc, "linear (backward)")
+            if need_x:
+                dx = torch.empty((m, k), dtype=dtype, device=dev)
+                ws, nbytes = _workspace(N.SV_LINEAR_DX, m, k, n, code, dz, weight)
+                rc = lib.sv_linear_dx(dz.data_ptr(), weight.data_ptr(), _ld(weight), m, k, n, code,
+                                      dx.data_ptr(), N.ptr(ws), nbytes, status, stream)
+                N.check(rc, "linear (input gradient)")
+            if need_w:
+                dw = torch.empty((n, k), dtype=dtype, device=dev)
+                ws, nbytes = _workspace(N.SV_LINEAR_DW, m, k, n, code, dz, x)
+                rc = lib.sv_linear_dw(dz.data_ptr(), x.data_ptr(), _ld(x), m, k, n, code,
+                                      dw.data_ptr(), N.ptr(ws), nbytes, status, stream)
+                N.check(rc, "linear (weight gradient)")
+        return dx, dw, db, dout if need_r else None, None
+
+
+def linear(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    activation: str | None = None,
+    residual: torch.Tensor | None = None,
+    x_scale: torch.Tensor | None = None,
+    weight_scale: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` over the last axis of ``x`` (..., K), fp32
+    accumulation, one rounding.
+
+    ``weight`` is (N, K), ``bias`` (N,), ``residual`` (..., N); ``activation`` is None, ``"silu"``,
+    ``"gelu"`` or ``"gelu_tanh"``. float32 (exact fp32 products), float16 and bfloat16 (tensor
+    cores), every tensor of one type, with gradients for all of them.
+
+    8 bits: ``x`` and ``weight`` in ``torch.float8_e4m3fn`` stand for ``x * x_scale[..., None]`` and
+    ``weight * weight_scale[:, None]`` (fp32 scales per row, as ``rms_norm(..., quantize=True)``
+    gives them; None is 1). The result, the bias and the residual are bfloat16 or float16
+    (``out_dtype``, by default the bias's or the residual's type, else bfloat16). No gradients.
+    """
+
+    x, weight = N.as_tensor(x), N.as_tensor(weight)
+    if activation not in N.ACTIVATION_CODE:
+        raise ValueError(f"linear: unknown activation {activation!r}")
+    if x.ndim < 1 or weight.ndim != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"linear: weight must have shape (N, {x.shape[-1] if x.ndim else '?'}), "
+                         f"got {tuple(weight.shape)}")
+    n = weight.shape[0]
+    e4m3 = x.dtype == torch.float8_e4m3fn
+    if not e4m3 and x.dtype not in N.DTYPE_CODE:
+        raise ValueError(f"linear: unsupported dtype {x.dtype}")
+    if weight.dtype != x.dtype:
+        raise ValueError(f"linear: x is {x.dtype} and weight {weight.dtype}")
+    if e4m3:
+        if out_dtype is None:
+            out_dtype = next((t.dtype for t in (bias, residual) if t is not None), torch.bfloat16)
+        if out_dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"linear: 8-bit operands give float16 or bfloat16, not {out_dtype}")
+    else:
+        if x_scale is not None or weight_scale is not None:
+            raise ValueError("linear: scales go with float8_e4m3fn operands")
+        if out_dtype not in (None, x.dtype):
+            raise ValueError(f"linear: the result has the operands' type {x.dtype}")
+        out_dtype = x.dtype
+    shape = (*x.shape[:-1], n)
+    for name, t, want, dtype in (
+        ("bias", bias, (n,), out_dtype),
+        ("residual", residual, shape, out_dtype),
+        ("x_scale", x_scale, x.shape[:-1], torch.float32),
+        ("weight_scale", weight_scale, (n,), torch.float32),
+    ):
+        if t is not None and (tuple(t.shape) != tuple(want) or t.dtype != dtype):
+            raise ValueError(f"linear: {name} must be a {tuple(want)} {dtype} tensor, got "
+                             f"{tuple(t.shape)} {t.dtype}")
+    for name, t in (("weight", weight), ("bias", bias), ("residual", residual),
+                    ("x_scale", x_scale), ("weight_scale", weight_scale)):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"linear: {name} is on {t.device}, x on {x.device}")
+    grads = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, weight, bias, residual))
+    if grads and e4m3:
+        raise ValueError("linear: 8-bit operands have no gradients")
+    N.require_cuda(x, "x")
+    x2 = _row_major(x.reshape(-1, x.shape[-1]) if x.ndim != 2 else x)
+    w2 = _row_major(weight)
+    r2 = None
+    if residual is not None:
+        r2 = _row_major(residual.reshape(-1, n) if residual.ndim != 2 else residual)
+    b2 = None if bias is None else bias.contiguous()
+    if grads:
+        out = _Linear.apply(x2, w2, b2, r2, activation)
+    else:
+        xs = None if x_scale is None else x_scale.reshape(-1).contiguous()
+        ws = None if weight_scale is None else weight_scale.contiguous()
+        out, _ = _forward(x2, w2, b2, r2, activation, xs, ws, out_dtype, False)
+    return out if x.ndim == 2 else out.reshape(shape)
+
+
+__all__ = ["linear"]

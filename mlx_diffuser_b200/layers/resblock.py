@@ -25,6 +25,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from ..kernels.linear import linear
 from ..kernels.norm import row_norm
 from .sparse import SparseConv3D, SparseTensor, sparse_downsample, sparse_upsample
 
@@ -51,7 +52,9 @@ class LayerNorm32(nn.Module):
 
 class SparseLinear(nn.Module):
     """Linear projection of the feature rows (``src/mlx_diffuser/layers/trellis_sparse.py:
-    13-30``): ``x.features @ weight.T + bias``, uniform init in ±1/sqrt(in)."""
+    13-30``): ``x.features @ weight.T + bias``, uniform init in ±1/sqrt(in). With an ``activation``
+    or a ``residual`` (rows like the output's) the projection runs with them in its epilogue
+    (:func:`~mlx_diffuser_b200.kernels.linear.linear`)."""
 
     def __init__(self, input_dims: int, output_dims: int, bias: bool = True):
         super().__init__()
@@ -62,14 +65,18 @@ class SparseLinear(nn.Module):
         else:
             self.bias = None
 
-    def project(self, features: torch.Tensor) -> torch.Tensor:
+    def project(self, features: torch.Tensor, *, activation: str | None = None,
+                residual: torch.Tensor | None = None) -> torch.Tensor:
         w = self.weight.to(device=features.device, dtype=features.dtype)
         b = None if self.bias is None else self.bias.to(device=features.device,
                                                         dtype=features.dtype)
-        return F.linear(features, w, b)
+        if activation is None and residual is None:
+            return F.linear(features, w, b)
+        return linear(features, w, b, activation=activation, residual=residual)
 
-    def forward(self, x: SparseTensor) -> SparseTensor:
-        return x.replace(self.project(x.features))
+    def forward(self, x: SparseTensor, *, activation: str | None = None,
+                residual: torch.Tensor | None = None) -> SparseTensor:
+        return x.replace(self.project(x.features, activation=activation, residual=residual))
 
 
 class SparseResBlock3D(nn.Module):

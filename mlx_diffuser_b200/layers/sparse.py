@@ -29,6 +29,13 @@ import torch
 from torch import nn
 
 from .. import _native as N
+from ..kernels.attention import (
+    MAX_BUCKETS,
+    MAX_DIM,
+    MAX_REACH,
+    biased_window_attention,
+    window_plan,
+)
 from ..kernels.sparse import (
     SparseConv3DFunction,
     conv3d_forward,
@@ -621,11 +628,21 @@ class WindowGroups:
     ``perm[offsets[g]:offsets[g + 1]]``. Groups are in the order of their first row and rows
     ascend inside a group, the order of the reference's ``_attention_groups`` lists.
     ``buckets`` maps a group length L to the [groups, L] row-index matrix of all groups of that
-    length (built on first use; one host read of the lengths)."""
+    length (built on first use; one host read of the lengths). ``plan`` holds the rows in window
+    order with their coordinates and window bounds, for the biased attention kernels, next to the
+    coordinates it was built from (held, version-checked)."""
 
     perm: torch.Tensor
     offsets: torch.Tensor
     buckets: dict[int, torch.Tensor] | None = None
+    plan: tuple[torch.Tensor, int, torch.Tensor] | None = None
+
+    def plan_rows(self, coords: torch.Tensor) -> torch.Tensor:
+        if (self.plan is None or self.plan[0] is not coords
+                or self.plan[1] != coords._version):
+            rows = window_plan(coords.contiguous(), self.perm, self.offsets)
+            self.plan = (coords, coords._version, rows)
+        return self.plan[2]
 
     @property
     def num_groups(self) -> int:
@@ -702,14 +719,27 @@ def sparse_self_attention(
     *,
     window_size: int | None = None,
     shift_window=(0, 0, 0),
+    position_bias: torch.Tensor | None = None,
+    position_buckets: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """SDPA over each sparse batch or coordinate window
     (``src/mlx_diffuser/layers/sparse.py:343-377``). ``q``, ``k``, ``v``: ``(N, heads,
     head_dim)``. Windows of equal occupancy share one attention call, as in the reference; the
-    grouping is the library's, the attention itself is torch's SDPA."""
+    grouping is the library's, the attention itself is torch's SDPA.
+
+    With ``position_bias``, a learned table ``(heads, B, B, B)`` of the features' type, the scores
+    get ``position_bias[h, L[dx], L[dy], L[dz]]`` added, the differences being the key's
+    coordinates minus the query's and ``L`` the int32 ``position_buckets`` ``(2 * reach + 1,)`` at
+    the difference clamped to ``-reach..reach`` (:func:`position_buckets` makes one). Scores, bias,
+    softmax and sums then run in one kernel over all windows, with gradients for ``q``, ``k``, ``v``
+    and the table that do not depend on the order of execution. head_dim up to 128, B up to 25,
+    reach up to 1023. A row whose every score is -inf gives zeros."""
 
     if q.shape != k.shape or q.shape != v.shape or q.shape[0] != x.num_points:
         raise ValueError("q, k, and v must share shape (N, heads, head_dim)")
+    if position_bias is not None or position_buckets is not None:
+        return _biased_self_attention(x, q, k, v, window_size, shift_window, position_bias,
+                                      position_buckets)
     groups = attention_windows(x, window_size, shift_window)
     out = torch.zeros_like(v)
     scale = q.shape[-1] ** -0.5
@@ -721,6 +751,63 @@ def sparse_self_attention(
         attended = attended.transpose(1, 2).reshape(idx.numel(), *q.shape[1:])
         out.index_add_(0, idx.reshape(-1), attended)
     return out
+
+
+def _biased_self_attention(x, q, k, v, window_size, shift_window, table, lut) -> torch.Tensor:
+    if table is None or lut is None:
+        raise ValueError("position_bias and position_buckets go together")
+    if q.ndim != 3 or not (q.dtype == k.dtype == v.dtype == table.dtype):
+        raise ValueError("q, k, v (N, heads, head_dim) and position_bias must share a dtype")
+    if q.dtype not in N.DTYPE_CODE:
+        raise ValueError(f"unsupported feature dtype {q.dtype}")
+    _, heads, dim = q.shape
+    if table.ndim != 4 or tuple(table.shape) != (heads, *(table.shape[-1],) * 3):
+        raise ValueError(f"position_bias must have shape ({heads}, B, B, B), got "
+                         f"{tuple(table.shape)}")
+    if lut.ndim != 1 or lut.dtype != torch.int32 or lut.numel() % 2 == 0:
+        raise ValueError("position_buckets must be int32 of shape (2 * reach + 1,)")
+    if dim > MAX_DIM or not 1 <= table.shape[-1] <= MAX_BUCKETS or lut.numel() // 2 > MAX_REACH:
+        raise ValueError(f"position_bias needs head_dim <= {MAX_DIM}, 1 <= B <= {MAX_BUCKETS} and "
+                         f"reach <= {MAX_REACH}")
+    N.require_cuda(q, "q")
+    for name, t in (("k", k), ("v", v), ("position_bias", table), ("position_buckets", lut),
+                    ("coords", x.coords)):
+        if t.device != q.device:
+            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+    with N.on_device(q.device):
+        groups = attention_windows(x, window_size, shift_window)
+        if groups.perm.numel() != q.shape[0]:
+            raise ValueError("the cached attention windows belong to other coordinates")
+        plan = groups.plan_rows(x.coords)
+    return biased_window_attention(q, k, v, table, lut, plan, dim**-0.5)
+
+
+def position_buckets(reach: int, side: int, *, exact: int | None = None, device=None):
+    """int32 bucket of each coordinate difference ``-reach..reach`` for ``position_bias``:
+    differences up to ``exact`` (default: ``side`` when that covers the reach, else half of it)
+    have buckets of their own, those beyond share logarithmically wider ones, ``side`` on either
+    side of bucket ``side`` (difference 0), ``2 * side + 1`` in all. ``side >= reach`` gives every
+    difference its own bucket: the relative position bias of a window of ``reach + 1`` voxels."""
+
+    reach, side = int(reach), int(side)
+    if reach < 0 or side < 0 or (side == 0) != (reach == 0):
+        raise ValueError("position_buckets needs reach >= 1 and side >= 1 (or both 0)")
+    side = min(side, reach)
+    near = (side if side == reach else max(1, side // 2)) if exact is None else int(exact)
+    if side and not 1 <= near <= side:
+        raise ValueError("position_buckets: exact must be between 1 and side")
+    half = []
+    for a in range(reach + 1):
+        if a > near:
+            # the step whose bound (reach / near) ** (i / steps) * near is the first to hold a,
+            # in whole numbers: a ** steps <= near ** (steps - i) * reach ** i
+            steps = side - near
+            i = next((i for i in range(1, steps + 1)
+                      if a**steps <= near ** (steps - i) * reach**i), steps)
+            a = near + i if steps else side
+        half.append(a)
+    values = [side - a for a in half[:0:-1]] + [side + a for a in half]
+    return torch.tensor(values, dtype=torch.int32, device=device)
 
 
 def sparse_cross_attention(
@@ -791,6 +878,7 @@ __all__ = [
     "attention_windows",
     "build_neighbor_map",
     "occupied_coordinates",
+    "position_buckets",
     "sparse_cross_attention",
     "sparse_downsample",
     "sparse_self_attention",
