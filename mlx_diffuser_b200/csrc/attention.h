@@ -1,6 +1,8 @@
 // Windowed attention with a learned relative position bias: what its kernels share.
 #pragma once
 
+#include <limits.h>
+
 #include "common.cuh"
 
 namespace sv {
@@ -10,13 +12,19 @@ constexpr int ATTN_MAX_BUCKETS = 25;   // per axis
 constexpr int ATTN_MAX_REACH = 1023;   // offsets beyond it share the outermost entries
 constexpr int ATTN_MAX_HEADS = 65535;
 
+// attention_tc.cu: the fp16 / bf16 kernels.
+struct AttnArgs;
+int attention_tc_forward(const AttnArgs& a, bool bf16, cudaStream_t s);
+int attention_tc_backward(const AttnArgs& a, bool bf16, void* dtable, cudaStream_t s);
+
 // One row of the attention plan, in window order: the coordinates, the window's range of
 // positions, and the feature row.
 struct alignas(16) PlanRow {
   int32_t x, y, z;
   int32_t row;    // -1: not a row of the tensor (reported when the plan was built)
   int32_t start, end;
-  int32_t pad[2];
+  int32_t span;   // the window's largest extent along an axis
+  int32_t pad;
 };
 static_assert(sizeof(PlanRow) == 32, "sv_window_plan writes 32 bytes a row");
 
@@ -27,7 +35,7 @@ struct AttnArgs {
   const PlanRow* plan;               // [n]
   const void* table;                 // [heads, nb, nb, nb]
   const int32_t* lut;                // [2 * reach + 1]
-  float* lse;                        // [heads, n] by position: log of the softmax's denominator
+  float2* stats;                     // [heads, n] by position: the softmax's maximum and 1 / sum
   float* delta;                      // [heads, n] by position: sum_d dout * o
   unsigned long long* dtable;        // [heads, nb^3] fixed point, or null
   unsigned* norms;                   // [heads, 2]: bits of max |dout_i|^2 and max |v_j|^2
@@ -61,6 +69,246 @@ __device__ __forceinline__ int dtable_exponent(const AttnArgs& a, int head) {
   int e;
   frexp(bound, &e);  // bound < 2^e
   return 61 - e;
+}
+// A row's softmax: maximum and 1 / sum, kept apart because their joint logarithm would lose the sum
+// next to scores of the type's lowest value. A row whose every score is -inf has weights of zero.
+__device__ __forceinline__ float2 row_stats(float top, float sum) {
+  return sum == 0.f ? make_float2(0.f, 0.f) : make_float2(top, 1.0f / sum);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = v > w || v != v ? v : w;  // keeps a NaN
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float dot_row(const float* s, const T* p, int dim) {
+  float acc = 0.f;
+  constexpr int E = 16 / sizeof(T);
+  if (dim % E == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    for (int d = 0; d < dim; d += E) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p + d));
+      const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int k = 0; k < E; ++k) acc = fmaf(s[d + k], to_f32(e[k]), acc);
+    }
+  } else {
+    for (int d = 0; d < dim; ++d) acc = fmaf(s[d], to_f32(p[d]), acc);
+  }
+  return acc;
+}
+
+__device__ __forceinline__ int bucket_of(const AttnArgs& a, const PlanRow& query, const PlanRow& key) {
+  const int x = lut_at(a, sub_sat(key.x, query.x));
+  const int y = lut_at(a, sub_sat(key.y, query.y));
+  const int z = lut_at(a, sub_sat(key.z, query.z));
+  return (x * a.nb + y) * a.nb + z;
+}
+
+__device__ __forceinline__ PlanRow plan_at(const PlanRow* plan, int64_t p) {
+  PlanRow r;
+  const int4* s = reinterpret_cast<const int4*>(plan + p);
+  *reinterpret_cast<int4*>(&r) = __ldg(s);
+  *(reinterpret_cast<int4*>(&r) + 1) = __ldg(s + 1);
+  return r;
+}
+
+constexpr int ATTN_CH = ATTN_MAX_DIM / 32;  // channels a lane sums
+
+// ---- one row of one head, by a warp: lanes along the other side's rows for the scores, along the
+// ---- head's channels for the sums, fp32 throughout
+
+// `s_q`: ATTN_MAX_DIM floats of the warp's own.
+template <typename T>
+__device__ void row_forward(const AttnArgs& a, int64_t p, int h, float* s_q) {
+  const int lane = threadIdx.x & 31;
+  const PlanRow me = plan_at(a.plan, p);
+  if (me.row < 0) return;
+  const T* q = static_cast<const T*>(a.q) + me.row * a.q_row + h * a.q_head;
+  const T* k = static_cast<const T*>(a.k) + h * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + h * a.v_head;
+  const T* table = static_cast<const T*>(a.table) + (int64_t)h * a.nb * a.nb * a.nb;
+  for (int d = lane; d < a.dim; d += 32) s_q[d] = to_f32(q[d]) * a.scale;
+  __syncwarp();
+  float o[ATTN_CH] = {}, top = -INFINITY, sum = 0.f;
+  for (int j0 = me.start; j0 < me.end; j0 += 32) {
+    const int j = j0 + lane;
+    float s = -INFINITY;
+    int row = -1;
+    if (j < me.end) {
+      const PlanRow key = plan_at(a.plan, j);
+      row = key.row;
+      if (row >= 0)
+        s = dot_row(s_q, k + row * a.k_row, a.dim) + to_f32(table[bucket_of(a, me, key)]);
+    }
+    const float m = fmaxf(top, warp_max(s));
+    const float base = m == -INFINITY ? 0.f : m;
+    const float keep = expf(top - base);
+    const float e = expf(s - base);
+    sum = sum * keep + warp_sum(e);
+#pragma unroll
+    for (int c = 0; c < ATTN_CH; ++c) o[c] *= keep;
+    const int count = min(32, me.end - j0);
+    for (int i = 0; i < count; ++i) {
+      const float w = __shfl_sync(0xffffffffu, e, i);
+      const int r = __shfl_sync(0xffffffffu, row, i);
+      if (r < 0) continue;
+#pragma unroll
+      for (int c = 0; c < ATTN_CH; ++c) {
+        const int d = lane + 32 * c;
+        if (d < a.dim) o[c] = fmaf(w, to_f32(v[r * a.v_row + d]), o[c]);
+      }
+    }
+    top = m;
+  }
+  T* out = static_cast<T*>(a.out) + (me.row * (int64_t)a.heads + h) * a.dim;
+#pragma unroll
+  for (int c = 0; c < ATTN_CH; ++c) {
+    const int d = lane + 32 * c;
+    if (d < a.dim) out[d] = from_f32<T>(sum == 0.f ? 0.f : o[c] / sum);
+  }
+  if (lane == 0 && a.stats) a.stats[h * a.n + p] = row_stats(top, sum);
+  __syncwarp();
+}
+
+// dq of a query, and with TABLE delta and the table's gradient too. `scratch`: 2 * ATTN_MAX_DIM.
+template <typename T, bool TABLE>
+__device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
+  const int lane = threadIdx.x & 31;
+  const PlanRow me = plan_at(a.plan, p);
+  if (me.row < 0) return;
+  float *s_q = scratch, *s_g = scratch + ATTN_MAX_DIM;
+  const int64_t own = (me.row * (int64_t)a.heads + h) * a.dim;
+  const T* q = static_cast<const T*>(a.q) + me.row * a.q_row + h * a.q_head;
+  const T* k = static_cast<const T*>(a.k) + h * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + h * a.v_head;
+  const T* g = static_cast<const T*>(a.dout) + own;
+  const T* o = static_cast<const T*>(a.o) + own;
+  const int64_t cells = (int64_t)a.nb * a.nb * a.nb;
+  const T* table = static_cast<const T*>(a.table) + h * cells;
+  float delta = 0.f;
+  for (int d = lane; d < a.dim; d += 32) {
+    s_q[d] = to_f32(q[d]) * a.scale;
+    s_g[d] = to_f32(g[d]);
+    delta = fmaf(s_g[d], to_f32(o[d]), delta);
+  }
+  delta = warp_sum(delta);
+  if (TABLE && lane == 0) a.delta[h * a.n + p] = delta;
+  __syncwarp();
+  const float2 stats = a.stats[h * a.n + p];
+  const int exponent = TABLE && a.dtable ? dtable_exponent(a, h) : INT_MAX;
+  const double unit = exponent == INT_MAX ? 0.0 : ldexp(1.0, exponent);
+  float acc[ATTN_CH] = {};
+  for (int j0 = me.start; j0 < me.end; j0 += 32) {
+    const int j = j0 + lane;
+    float ds = 0.f;
+    int row = -1;
+    if (j < me.end) {
+      const PlanRow key = plan_at(a.plan, j);
+      row = key.row;
+      if (row >= 0) {
+        const int b = bucket_of(a, me, key);
+        const float s = dot_row(s_q, k + row * a.k_row, a.dim) + to_f32(table[b]);
+        const float dp = dot_row(s_g, v + row * a.v_row, a.dim);
+        ds = expf(s - stats.x) * stats.y * (dp - delta);
+        if constexpr (TABLE) {
+          if (a.dtable && !(fabsf(ds) < INFINITY))
+            atomicMax(a.norms + 2 * h, 0x7fffffffu);  // the head's table gradient is NaN
+          else if (exponent != INT_MAX)
+            atomicAdd(a.dtable + h * cells + b,
+                      (unsigned long long)__double2ll_rn((double)ds * unit));
+        }
+      }
+    }
+    const int count = min(32, me.end - j0);
+    for (int i = 0; i < count; ++i) {
+      const float w = __shfl_sync(0xffffffffu, ds, i);
+      const int r = __shfl_sync(0xffffffffu, row, i);
+      if (r < 0) continue;
+#pragma unroll
+      for (int c = 0; c < ATTN_CH; ++c) {
+        const int d = lane + 32 * c;
+        if (d < a.dim) acc[c] = fmaf(w, to_f32(k[r * a.k_row + d]), acc[c]);
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < ATTN_CH; ++c) {
+    const int d = lane + 32 * c;
+    if (d < a.dim) static_cast<T*>(a.dq)[own + d] = from_f32<T>(acc[c] * a.scale);
+  }
+  __syncwarp();
+}
+
+// dk and dv of a key. `scratch`: 2 * ATTN_MAX_DIM.
+template <typename T>
+__device__ void row_dkv(const AttnArgs& a, int64_t p, int h, float* scratch) {
+  const int lane = threadIdx.x & 31;
+  const PlanRow me = plan_at(a.plan, p);
+  if (me.row < 0) return;
+  float *s_k = scratch, *s_v = scratch + ATTN_MAX_DIM;
+  const T* q = static_cast<const T*>(a.q) + h * a.q_head;
+  const T* k = static_cast<const T*>(a.k) + me.row * a.k_row + h * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + me.row * a.v_row + h * a.v_head;
+  const T* g = static_cast<const T*>(a.dout) + (int64_t)h * a.dim;
+  const int64_t g_row = (int64_t)a.heads * a.dim;
+  const T* table = static_cast<const T*>(a.table) + (int64_t)h * a.nb * a.nb * a.nb;
+  for (int d = lane; d < a.dim; d += 32) {
+    s_k[d] = to_f32(k[d]) * a.scale;
+    s_v[d] = to_f32(v[d]);
+  }
+  __syncwarp();
+  float dk[ATTN_CH] = {}, dv[ATTN_CH] = {};
+  for (int i0 = me.start; i0 < me.end; i0 += 32) {
+    const int i = i0 + lane;
+    float w = 0.f, ds = 0.f;
+    int row = -1;
+    if (i < me.end) {
+      const PlanRow query = plan_at(a.plan, i);
+      row = query.row;
+      if (row >= 0) {
+        const float2 stats = a.stats[h * a.n + i];
+        const float s = dot_row(s_k, q + row * a.q_row, a.dim) +
+                        to_f32(table[bucket_of(a, query, me)]);
+        w = expf(s - stats.x) * stats.y;
+        ds = w * (dot_row(s_v, g + row * g_row, a.dim) - a.delta[h * a.n + i]);
+      }
+    }
+    const int count = min(32, me.end - i0);
+    for (int t = 0; t < count; ++t) {
+      const float pw = __shfl_sync(0xffffffffu, w, t);
+      const float dw = __shfl_sync(0xffffffffu, ds, t);
+      const int r = __shfl_sync(0xffffffffu, row, t);
+      if (r < 0) continue;
+#pragma unroll
+      for (int c = 0; c < ATTN_CH; ++c) {
+        const int d = lane + 32 * c;
+        if (d < a.dim) {
+          dv[c] = fmaf(pw, to_f32(g[r * g_row + d]), dv[c]);
+          dk[c] = fmaf(dw, to_f32(q[r * a.q_row + d]), dk[c]);
+        }
+      }
+    }
+  }
+  const int64_t own = (me.row * (int64_t)a.heads + h) * a.dim;
+#pragma unroll
+  for (int c = 0; c < ATTN_CH; ++c) {
+    const int d = lane + 32 * c;
+    if (d < a.dim) {
+      static_cast<T*>(a.dk)[own + d] = from_f32<T>(dk[c] * a.scale);
+      static_cast<T*>(a.dv)[own + d] = from_f32<T>(dv[c]);
+    }
+  }
+  __syncwarp();
 }
 #endif
 

@@ -36,32 +36,32 @@ def _strides(q, k, v):
                                 v.stride(1))
 
 
-def _forward(q, k, v, table, lut, plan, scale, keep_lse):
+def _forward(q, k, v, table, lut, plan, scale, keep_stats):
     n, heads, dim = q.shape
     dev = q.device
     out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
-    lse = torch.empty((heads, n), dtype=torch.float32, device=dev) if keep_lse else None
+    stats = torch.empty((heads, n, 2), dtype=torch.float32, device=dev) if keep_stats else None
     with N.on_device(dev):
         rc = N.load().sv_window_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), n, heads, dim,
             N.DTYPE_CODE[q.dtype], plan.data_ptr(), table.data_ptr(), table.shape[-1],
-            lut.data_ptr(), lut.numel() // 2, scale, out.data_ptr(), N.ptr(lse), N.stream(dev))
+            lut.data_ptr(), lut.numel() // 2, scale, out.data_ptr(), N.ptr(stats), N.stream(dev))
     N.check(rc, "sparse_self_attention")
-    return out, lse
+    return out, stats
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, lut, plan, scale):
-        out, lse = _forward(q, k, v, table, lut, plan, scale, True)
+        out, stats = _forward(q, k, v, table, lut, plan, scale, True)
         ctx.scale = scale
-        ctx.save_for_backward(q, k, v, table, lut, plan, out, lse)
+        ctx.save_for_backward(q, k, v, table, lut, plan, out, stats)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, lut, plan, out, lse = ctx.saved_tensors
+        q, k, v, table, lut, plan, out, stats = ctx.saved_tensors
         n, heads, dim = q.shape
         dev = q.device
         dout = dout.contiguous()
@@ -73,7 +73,7 @@ class _WindowAttention(torch.autograd.Function):
             ws = N.workspace(nbytes, dev)
             rc = lib.sv_window_attention_backward(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), out.data_ptr(),
-                dout.data_ptr(), lse.data_ptr(), n, heads, dim, N.DTYPE_CODE[q.dtype],
+                dout.data_ptr(), stats.data_ptr(), n, heads, dim, N.DTYPE_CODE[q.dtype],
                 plan.data_ptr(), table.data_ptr(), table.shape[-1], lut.data_ptr(),
                 lut.numel() // 2, ctx.scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                 N.ptr(dtable), ws.data_ptr(), nbytes, N.stream(dev))

@@ -4,7 +4,8 @@ window shapes from lone voxels to whole batch elements, head sizes, types, strid
 Bounds, with u = 2^-24 and e = eps / 2 of the type (a rounding is off by at most that): a score is
 off by ds <= (2 dim + 32) u (scale |q||k| + |s|) with exp and the running rescales in the 32; a weight
 p by p (2 ds + e), the e for the type it is multiplied in; sums of n products by 2 n u of their
-magnitudes."""
+magnitudes. Below the normal range these are absolute: exp may give zero for results under 2^-126,
+and a rounding to the type is off by half its smallest subnormal number."""
 
 from __future__ import annotations
 
@@ -79,7 +80,8 @@ def _reference(x, q, k, v, table, lut, window, shift, dout=None):
         ds_off = torch.where(torch.isfinite(ds_off), ds_off, torch.zeros_like(ds_off))
         p_rel = 2 * ds_off + 2 * ds_off.amax(-1, keepdim=True) + e + 8 * U
         o = p @ vs
-        o_off = (p * p_rel) @ vs.abs() + 2 * size * U * (p @ vs.abs())
+        low = max(torch.finfo(dtype).smallest_normal * e, 2.0**-126)
+        o_off = (p * p_rel + low) @ vs.abs() + 2 * size * U * (p @ vs.abs())
         val["out"][rows] = o.transpose(0, 1)
         off["out"][rows] = (o_off + e * (o.abs() + o_off)).transpose(0, 1)
         if g is None:
@@ -93,10 +95,11 @@ def _reference(x, q, k, v, table, lut, window, shift, dout=None):
             (gs.abs() * (o_off + e * (o.abs() + o_off)) + 2 * dim * U * gs.abs() * o.abs()
              ).sum(-1, keepdim=True)
         ds = p * w
-        ds32_off = p * (p_rel - e) * w.abs() + p * w_off  # before its own rounding to the type
-        ds_t_off = ds32_off + e * (ds.abs() + ds32_off)
+        # before its own rounding to the type, and with it
+        ds32_off = (p * (p_rel - e) + 2.0**-126) * w.abs() + p * w_off
+        ds_t_off = ds32_off + e * (ds.abs() + ds32_off) + low
         dv = p.transpose(1, 2) @ gs
-        dv_off = (p * p_rel).transpose(1, 2) @ gs.abs() + 2 * size * U * \
+        dv_off = (p * p_rel + low).transpose(1, 2) @ gs.abs() + 2 * size * U * \
             (p.transpose(1, 2) @ gs.abs())
         dq, dk = ds @ ks * scale, ds.transpose(1, 2) @ qs * scale
         dq_off = (ds_t_off + 2 * size * U * ds.abs()) @ ks.abs() * scale
@@ -108,8 +111,9 @@ def _reference(x, q, k, v, table, lut, window, shift, dout=None):
         off["dtable"].index_add_(1, b.flatten(), ds32_off.flatten(1))
         count.index_add_(0, b.flatten(), torch.ones_like(b.flatten(), dtype=F64))
     if g is not None:
-        # the fixed-point table: half a unit a pair, 2^-36 of a bound of one row's terms
-        unit = 2.0**-36 * 2 * g.norm(dim=2).amax(0) * v.norm(dim=2).amax(0)
+        # the fixed-point table: half a unit a pair, the unit 2^-41 (29 and 12 places) of up to twice
+        # the bound 2 |g| |v| of a row's terms times the 64 rows of a block: 2^-35 of it
+        unit = 2.0**-35 * 2 * g.norm(dim=2).amax(0) * v.norm(dim=2).amax(0)
         off["dtable"] += unit[:, None] * count
         off["dtable"] += e * (val["dtable"].abs() + off["dtable"])
     shape = (heads, nb, nb, nb)
@@ -208,18 +212,52 @@ def test_large_scores_keep_the_softmax_finite(dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_table_entries_that_mask(dtype):
-    """-inf and the type's lowest value in the table: pairs out of sight, and rows that see nothing."""
+    """-inf in the table: pairs out of sight, and rows that see nothing."""
     coords = _voxels(160, 8, 1, 4)
     lut = position_buckets(7, 7, device=DEV)
-    for low in (float("-inf"), torch.finfo(dtype).min):
-        table = _rand((2, 15, 15, 15), dtype, 30)
-        table[0, 8:] = low      # head 0 sees no key ahead of it along x
-        table[1] = low          # head 1 sees nothing, or everything alike
-        out, grads = _run(coords, 2, 32, dtype, 4, (0, 0, 0), 7, 7, lut=lut, table=table)
-        assert all(torch.isfinite(t).all() for t in (out, *grads))
-        if low == float("-inf"):
-            assert not out[:, 1].any() and not any(g[:, 1].any() for g in grads[:3])
-            assert not grads[3][1].any()
+    table = _rand((2, 15, 15, 15), dtype, 30)
+    table[0, 8:] = float("-inf")  # head 0 sees no key ahead of it along x
+    table[1] = float("-inf")      # head 1 sees nothing
+    out, grads = _run(coords, 2, 32, dtype, 4, (0, 0, 0), 7, 7, lut=lut, table=table)
+    assert all(torch.isfinite(t).all() for t in (out, *grads))
+    assert not out[:, 1].any() and not any(g[:, 1].any() for g in grads[:3])
+    assert not grads[3][1].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_table_entries_of_the_lowest_value(dtype):
+    """The type's lowest value masks like -inf beside ordinary entries; where a row has nothing else,
+    every score is that value in fp32 (the products vanish beside it), so the weights are equal."""
+    coords = _voxels(160, 8, 1, 4)
+    x = _tensor(coords)
+    lut = position_buckets(7, 7, device=DEV)
+    low = torch.finfo(dtype).min
+    table = _rand((2, 15, 15, 15), dtype, 30)
+    hidden = table.clone()
+    table[0, 8:], hidden[0, 8:] = low, float("-inf")
+    table[1] = low
+    q, k, v, dout = (_rand((160, 2, 32), dtype, 31 + i) for i in range(4))
+
+    def run(t, qq):
+        leaves = [a.clone().requires_grad_(True) for a in (qq, k, v, t)]
+        out = sparse_self_attention(x, *leaves[:3], window_size=4, position_bias=leaves[3],
+                                    position_buckets=lut)
+        return (out, *torch.autograd.grad(out, leaves, dout))
+
+    got, want = run(table, q), run(hidden, q)
+    for a, b in zip(got[:4], want[:4]):
+        assert torch.equal(a[:, 0], b[:, 0])
+    assert torch.equal(got[4][0], want[4][0])
+    flat = table.clone()
+    flat[1] = 0
+    zero = q.clone()
+    zero[:, 1] = 0
+    alike = run(flat, zero)  # equal scores of zero
+    for i in (0, 3):  # out and dv
+        assert torch.equal(got[i][:, 1], alike[i][:, 1])
+    assert torch.isfinite(got[2]).all()
+    assert torch.equal(got[1][:, 1], alike[1][:, 1])
+    assert torch.equal(got[4][1], alike[4][1])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -236,14 +274,18 @@ def test_not_finite_values_stay_in_their_window(dtype):
         return (out.detach(), *torch.autograd.grad(out, leaves, torch.ones_like(out)))
 
     clean = run(q, k, v)
+    val, off = _reference(x, q, k, v, table, lut, 4, (0, 0, 0), torch.ones_like(q))
     bad = 17
     near = (coords[:, 1:] // 4 == coords[bad, 1:] // 4).all(1)
     for which in range(3):
         args = [q.clone(), k.clone(), v.clone()]
         args[which][bad, 1, 5] = float("nan")
         got = run(*args)
-        for a, b in zip(got[:4], clean[:4]):
-            assert torch.equal(a[~near], b[~near]) and torch.equal(a[:, 0], b[:, 0])
+        for a, b, what in zip(got[:4], clean[:4], ("out", "dq", "dk", "dv")):
+            assert torch.equal(a[:, 0], b[:, 0])
+            # rows that shared a tile with the NaN are computed again without the tile's roundings,
+            # so they keep the bounds and not the bits
+            _close(a[~near], val[what][~near], off[what][~near], what)
         assert torch.isnan(got[0][bad, 1, 5 if which == 2 else 0])
         assert torch.equal(got[4][0], clean[4][0]) and torch.isnan(got[4][1]).any()
 
