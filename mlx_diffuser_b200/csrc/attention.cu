@@ -93,21 +93,21 @@ template <typename T>
 __global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_kernel(AttnArgs a) {
   __shared__ float scratch[ROW_WARPS][ATTN_MAX_DIM];
   const int64_t p = (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
-  if (p < a.n) row_forward<T>(a, p, blockIdx.y, scratch[threadIdx.x >> 5]);
+  if (p < a.n) row_forward<T, false>(a, p, blockIdx.y, scratch[threadIdx.x >> 5]);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(32 * ROW_WARPS) attn_dq_rows_kernel(AttnArgs a) {
   __shared__ float scratch[ROW_WARPS][2 * ATTN_MAX_DIM];
   const int64_t p = (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
-  if (p < a.n) row_dq<T, true>(a, p, blockIdx.y, scratch[threadIdx.x >> 5]);
+  if (p < a.n) row_dq<T, false, true>(a, p, blockIdx.y, scratch[threadIdx.x >> 5]);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(32 * ROW_WARPS) attn_dkv_rows_kernel(AttnArgs a) {
   __shared__ float scratch[ROW_WARPS][2 * ATTN_MAX_DIM];
   const int64_t p = (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
-  if (p < a.n) row_dkv<T>(a, p, blockIdx.y, scratch[threadIdx.x >> 5]);
+  if (p < a.n) row_dkv<T, false>(a, p, blockIdx.y, scratch[threadIdx.x >> 5]);
 }
 
 // norms[h] = bits of the largest |dout_i|^2 and |v_j|^2 of a head. Squares are not negative, so

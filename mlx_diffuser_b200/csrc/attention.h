@@ -38,7 +38,8 @@ struct AttnArgs {
   float2* stats;                     // [heads, n] by position: the softmax's maximum and 1 / sum
   float* delta;                      // [heads, n] by position: sum_d dout * o
   unsigned long long* dtable;        // [heads, nb^3] fixed point, or null
-  unsigned* norms;                   // [heads, 2]: bits of max |dout_i|^2 and max |v_j|^2
+  unsigned* norms;                   // [heads, 2]: bits of max |dout_i|^2 and max |v_j|^2 (fp32
+                                     // path), or of max |dS| (fp16 / bf16)
   int64_t n;
   int heads, dim, nb, reach;
   float scale;
@@ -127,8 +128,21 @@ constexpr int ATTN_CH = ATTN_MAX_DIM / 32;  // channels a lane sums
 // ---- one row of one head, by a warp: lanes along the other side's rows for the scores, along the
 // ---- head's channels for the sums, fp32 throughout
 
+// Scores as the kernel keeps them: natural (fp32 path), or times log2(e) for the fp16 / bf16 kernels,
+// whose statistics the rows computed again share.
+constexpr float ATTN_LOG2E = 1.4426950408889634f;
+// x log2(e), finite for every finite x: the type's lowest value stays a score like any other.
+__device__ __forceinline__ float times_log2e(float x) {
+  const float y = x * ATTN_LOG2E;
+  return fabsf(x) < INFINITY ? fminf(fmaxf(y, -3.402823466e38f), 3.402823466e38f) : y;
+}
+template <bool LOG2>
+__device__ __forceinline__ float score_of(float s) { return LOG2 ? times_log2e(s) : s; }
+template <bool LOG2>
+__device__ __forceinline__ float weight_of(float d) { return LOG2 ? exp2f(d) : expf(d); }
+
 // `s_q`: ATTN_MAX_DIM floats of the warp's own.
-template <typename T>
+template <typename T, bool LOG2>
 __device__ void row_forward(const AttnArgs& a, int64_t p, int h, float* s_q) {
   const int lane = threadIdx.x & 31;
   const PlanRow me = plan_at(a.plan, p);
@@ -148,12 +162,13 @@ __device__ void row_forward(const AttnArgs& a, int64_t p, int h, float* s_q) {
       const PlanRow key = plan_at(a.plan, j);
       row = key.row;
       if (row >= 0)
-        s = dot_row(s_q, k + row * a.k_row, a.dim) + to_f32(table[bucket_of(a, me, key)]);
+        s = score_of<LOG2>(dot_row(s_q, k + row * a.k_row, a.dim) +
+                           to_f32(table[bucket_of(a, me, key)]));
     }
     const float m = fmaxf(top, warp_max(s));
     const float base = m == -INFINITY ? 0.f : m;
-    const float keep = expf(top - base);
-    const float e = expf(s - base);
+    const float keep = weight_of<LOG2>(top - base);
+    const float e = weight_of<LOG2>(s - base);
     sum = sum * keep + warp_sum(e);
 #pragma unroll
     for (int c = 0; c < ATTN_CH; ++c) o[c] *= keep;
@@ -181,7 +196,7 @@ __device__ void row_forward(const AttnArgs& a, int64_t p, int h, float* s_q) {
 }
 
 // dq of a query, and with TABLE delta and the table's gradient too. `scratch`: 2 * ATTN_MAX_DIM.
-template <typename T, bool TABLE>
+template <typename T, bool LOG2, bool TABLE>
 __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
   const int lane = threadIdx.x & 31;
   const PlanRow me = plan_at(a.plan, p);
@@ -217,9 +232,9 @@ __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
       row = key.row;
       if (row >= 0) {
         const int b = bucket_of(a, me, key);
-        const float s = dot_row(s_q, k + row * a.k_row, a.dim) + to_f32(table[b]);
+        const float s = score_of<LOG2>(dot_row(s_q, k + row * a.k_row, a.dim) + to_f32(table[b]));
         const float dp = dot_row(s_g, v + row * a.v_row, a.dim);
-        ds = expf(s - stats.x) * stats.y * (dp - delta);
+        ds = weight_of<LOG2>(s - stats.x) * stats.y * (dp - delta);
         if constexpr (TABLE) {
           if (a.dtable && !(fabsf(ds) < INFINITY))
             atomicMax(a.norms + 2 * h, 0x7fffffffu);  // the head's table gradient is NaN
@@ -250,7 +265,7 @@ __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
 }
 
 // dk and dv of a key. `scratch`: 2 * ATTN_MAX_DIM.
-template <typename T>
+template <typename T, bool LOG2>
 __device__ void row_dkv(const AttnArgs& a, int64_t p, int h, float* scratch) {
   const int lane = threadIdx.x & 31;
   const PlanRow me = plan_at(a.plan, p);
@@ -277,9 +292,9 @@ __device__ void row_dkv(const AttnArgs& a, int64_t p, int h, float* scratch) {
       row = query.row;
       if (row >= 0) {
         const float2 stats = a.stats[h * a.n + i];
-        const float s = dot_row(s_k, q + row * a.q_row, a.dim) +
-                        to_f32(table[bucket_of(a, query, me)]);
-        w = expf(s - stats.x) * stats.y;
+        const float s = score_of<LOG2>(dot_row(s_k, q + row * a.q_row, a.dim) +
+                                       to_f32(table[bucket_of(a, query, me)]));
+        w = weight_of<LOG2>(s - stats.x) * stats.y;
         ds = w * (dot_row(s_v, g + row * g_row, a.dim) - a.delta[h * a.n + i]);
       }
     }

@@ -29,22 +29,12 @@ namespace sv {
 namespace {
 
 constexpr int BQ = 64;   // rows of a block
-constexpr int BKV = 64;  // positions of a tile
 constexpr int AT = 128;  // threads
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct KeyMeta {
-  int32_t x, y, z;
-  int32_t pos;  // INT_MAX: no row
-};
 
 // Tiles hold DP channels a row (the head's, padded with zeros) at a stride that is an odd multiple
 // of 16 bytes, so the 8 rows of a matrix fragment fall into different banks.
 template <int DP>
-struct Tile {
-  static constexpr int STRIDE = DP * 2 + 16;
-  static constexpr int BYTES = 64 * STRIDE;
-};
+constexpr int STRIDE = DP * 2 + 16;
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -96,29 +86,36 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// 64 gathered rows of one head into a tile; rows of -1 and channels past `dim` become zeros.
-template <typename T, int DP>
+// max that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+// R gathered rows of one head into a tile; rows of -1 and channels past `dim` become zeros.
+template <typename T, int DP, int R>
 __device__ __forceinline__ void load_tile(uint8_t* tile, const T* base, int64_t row_stride,
                                           const int32_t* rows, int dim, bool vec) {
   constexpr int CH = DP / 8;  // 16-byte chunks of a row
   if (vec) {
     const uint32_t at = smem_u32(tile);
 #pragma unroll
-    for (int i = 0; i < 64 * CH / AT; ++i) {
+    for (int i = 0; i < R * CH / AT; ++i) {
       const int c = threadIdx.x + AT * i;
       const int r = c / CH, col = c % CH;
       const int32_t row = rows[r];
       const bool in = row >= 0 && col * 8 < dim;
-      cp_async_16(at + r * Tile<DP>::STRIDE + col * 16,
+      cp_async_16(at + r * STRIDE<DP> + col * 16,
                   base + (in ? (int64_t)row * row_stride + col * 8 : 0), in ? 16u : 0u);
     }
   } else {
-    for (int c = threadIdx.x; c < 64 * DP; c += AT) {
+    for (int c = threadIdx.x; c < R * DP; c += AT) {
       const int r = c / DP, col = c % DP;
       const int32_t row = rows[r];
       T v = from_f32<T>(0.f);
       if (row >= 0 && col < dim) v = base[(int64_t)row * row_stride + col];
-      *reinterpret_cast<T*>(tile + r * Tile<DP>::STRIDE + col * 2) = v;
+      *reinterpret_cast<T*>(tile + r * STRIDE<DP> + col * 2) = v;
     }
   }
 }
@@ -131,13 +128,13 @@ __device__ __forceinline__ void store_rows(uint8_t* tile, const float (&o)[DP / 
                                            int head, int dim, bool vec) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c2 = 2 * (lane & 3);
-  uint8_t* mine = tile + warp * 16 * Tile<DP>::STRIDE;
+  uint8_t* mine = tile + warp * 16 * STRIDE<DP>;
   __syncwarp();
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) {
-    *reinterpret_cast<uint32_t*>(mine + g * Tile<DP>::STRIDE + (n * 8 + c2) * 2) =
+    *reinterpret_cast<uint32_t*>(mine + g * STRIDE<DP> + (n * 8 + c2) * 2) =
         pack2<T>(o[n][0] * s0, o[n][1] * s0);
-    *reinterpret_cast<uint32_t*>(mine + (g + 8) * Tile<DP>::STRIDE + (n * 8 + c2) * 2) =
+    *reinterpret_cast<uint32_t*>(mine + (g + 8) * STRIDE<DP> + (n * 8 + c2) * 2) =
         pack2<T>(o[n][2] * s1, o[n][3] * s1);
   }
   __syncwarp();
@@ -149,7 +146,7 @@ __device__ __forceinline__ void store_rows(uint8_t* tile, const float (&o)[DP / 
     const int32_t row = rows[warp * 16 + r];
     if (row < 0) continue;
     T* dst = out + ((int64_t)row * heads + head) * dim + col * 8;
-    const uint4 v = *reinterpret_cast<const uint4*>(mine + r * Tile<DP>::STRIDE + col * 16);
+    const uint4 v = *reinterpret_cast<const uint4*>(mine + r * STRIDE<DP> + col * 16);
     if (vec) {
       if (col * 8 < dim) *reinterpret_cast<uint4*>(dst) = v;
     } else {
@@ -161,47 +158,67 @@ __device__ __forceinline__ void store_rows(uint8_t* tile, const float (&o)[DP / 
   }
 }
 
-// What every kernel here keeps in shared memory besides its tiles.
+struct KeyMeta {
+  int32_t x, y, z, row;  // row -1: no row
+};
+
+// What every kernel here keeps in shared memory besides its tiles of KB positions.
+template <int KB>
 struct alignas(16) Shared {
-  KeyMeta key[3][BKV];    // ring of the other side's rows, two tiles ahead
-  int32_t key_lin[3][BKV];
-  int32_t key_row[3][BKV];
-  float2 key_stats[3][BKV];  // their softmax and delta (dk / dv)
-  float key_delta[3][BKV];
-  int32_t key_bad[3][2];  // a position without a row in either half
+  KeyMeta key[3][KB];      // ring of the other side's rows, two tiles ahead
+  int2 key_lin[3][KB];     // their linear coordinates: {of all axes, -}, or {of x and y, z}
+  int32_t key_row[3][KB];
+  float2 key_stats[3][KB]; // their softmax and delta (dk / dv)
+  float key_delta[3][KB];
+  int32_t key_bad[3];      // whether a position has no row
   PlanRow own[BQ];
   int32_t own_row[BQ];
   int32_t range[2];
 };
 
-template <typename T, int DP>
+// How a pair's bucket is found. LINEAR: the look-up is the identity and the windows are within the
+// table's reach, so the bucket is a difference of linear coordinates. JOINT: within the reach, and
+// the look-ups of x and y are joined in one table of all their offsets. GENERAL: any.
+enum { GENERAL = 0, JOINT = 1, LINEAR = 2 };
+constexpr int JOINT_MAX = 4096;
+
+template <typename T, int KB>
 struct Block {
   const AttnArgs& a;
-  Shared& s;
-  float* table;      // [nb^3] fp32
+  Shared<KB>& s;
+  float* table;      // [nb^3] times log2(e)
   int16_t* lut;      // [2 reach + 1]
+  int16_t* joint;    // [(2 reach + 1)^2], x and y buckets as the table's index, or null
   int head;
-  bool lut_linear;
+  bool identity;
+  float delta_top;   // largest |delta| staged by this thread
   // set per 64 rows
-  bool linear;
+  int mode;
   int j0, tiles;
 
   __device__ __forceinline__ int cells() const { return a.nb * a.nb * a.nb; }
+  __device__ __forceinline__ int width() const { return 2 * a.reach + 1; }
 
-  __device__ __forceinline__ int lin(const PlanRow& r) const {
-    return (int)(((unsigned)r.x * a.nb + (unsigned)r.y) * a.nb + (unsigned)r.z);
+  // Wrap-around is harmless: only differences inside a window are used.
+  __device__ __forceinline__ int2 lin(int x, int y, int z) const {
+    if (mode == LINEAR)
+      return make_int2((int)(((unsigned)x * a.nb + (unsigned)y) * a.nb + (unsigned)z), 0);
+    return make_int2((int)((unsigned)x * width() + (unsigned)y), z);
   }
 
   __device__ void stage_tables() {
     const T* src = static_cast<const T*>(a.table) + (int64_t)head * cells();
-    for (int i = threadIdx.x; i < cells(); i += AT) table[i] = to_f32(src[i]);
-    bool same = a.nb == 2 * a.reach + 1;
-    for (int i = threadIdx.x; i < 2 * a.reach + 1; i += AT) {
+    for (int i = threadIdx.x; i < cells(); i += AT) table[i] = times_log2e(to_f32(src[i]));
+    bool same = a.nb == width();
+    for (int i = threadIdx.x; i < width(); i += AT) {
       const int v = max(0, min(a.nb - 1, __ldg(a.lut + i)));
       lut[i] = (int16_t)v;
       same = same && v == i;
     }
-    lut_linear = __syncthreads_and(same);
+    identity = __syncthreads_and(same);
+    if (!identity && joint != nullptr)
+      for (int i = threadIdx.x; i < width() * width(); i += AT)
+        joint[i] = (int16_t)((lut[i / width()] * a.nb + lut[i % width()]) * a.nb);
   }
 
   // The block's rows and the positions their windows cover.
@@ -213,11 +230,7 @@ struct Block {
       const int64_t p = p0 + threadIdx.x;
       PlanRow r{};
       r.row = -1;
-      if (p < a.n) {
-        const int4* src = reinterpret_cast<const int4*>(a.plan + p);
-        *reinterpret_cast<int4*>(&r) = __ldg(src);
-        *(reinterpret_cast<int4*>(&r) + 1) = __ldg(src + 1);
-      }
+      if (p < a.n) r = plan_at(a.plan, p);
       if (r.row < 0) {
         r.start = r.end = 0;
       } else {
@@ -228,51 +241,42 @@ struct Block {
       s.own[threadIdx.x] = r;
       s.own_row[threadIdx.x] = r.row;
     }
-    linear = __syncthreads_and(narrow) && lut_linear;
+    narrow = __syncthreads_and(narrow);
+    mode = !narrow ? GENERAL : (identity ? LINEAR : (joint != nullptr ? JOINT : GENERAL));
     j0 = s.range[0];
-    tiles = s.range[1] > j0 ? (s.range[1] - j0 + BKV - 1) / BKV : 0;
+    tiles = s.range[1] > j0 ? (s.range[1] - j0 + KB - 1) / KB : 0;
   }
 
+  // By the first warp: a position a lane.
   template <bool STATS>
   __device__ void stage_meta(int t) {
+    static_assert(KB == 32, "a position a lane");
     const int slot = t % 3;
     const int i = threadIdx.x;
-    bool bad = false;
-    if (i < BKV) {
-      const int j = j0 + t * BKV + i;
-      KeyMeta m{0, 0, 0, INT_MAX};
-      int32_t row = -1, l = 0;
-      float2 x = make_float2(0.f, 0.f);
-      float y = 0.f;
-      if (j < s.range[1]) {
-        const int4* src = reinterpret_cast<const int4*>(a.plan + j);
-        const int4 c = __ldg(src);
-        row = c.w;
-        if (row >= 0) {
-          PlanRow r;
-          r.x = c.x; r.y = c.y; r.z = c.z;
-          l = lin(r);
-          m = KeyMeta{c.x, c.y, c.z, j};
-          if constexpr (STATS) {
-            x = a.stats[head * a.n + j];
-            y = a.delta[head * a.n + j];
-          }
-        }
-      }
-      bad = row < 0;
-      s.key[slot][i] = m;
-      s.key_lin[slot][i] = l;
-      s.key_row[slot][i] = row;
+    if (i < KB) {
+      const int j = j0 + t * KB + i;
+      KeyMeta m{0, 0, 0, -1};
+      if (j < s.range[1])
+        *reinterpret_cast<int4*>(&m) = __ldg(reinterpret_cast<const int4*>(a.plan + j));
       if constexpr (STATS) {
-        s.key_stats[slot][i] = x;
-        s.key_delta[slot][i] = y;
+        float2 st = make_float2(0.f, 0.f);
+        float d = 0.f;
+        if (m.row >= 0) {
+          st = a.stats[head * a.n + j];
+          d = a.delta[head * a.n + j];
+        }
+        s.key_stats[slot][i] = st;
+        s.key_delta[slot][i] = d;
+        delta_top = max_nan(delta_top, fabsf(d));
       }
-      const unsigned any = __ballot_sync(0xffffffffu, bad);
-      if ((i & 31) == 0) s.key_bad[slot][i >> 5] = any != 0;
+      const unsigned bad = __ballot_sync(0xffffffffu, j < s.range[1] && m.row < 0);
+      if (i == 0) s.key_bad[slot] = bad != 0;
+      s.key[slot][i] = m;
+      s.key_lin[slot][i] = lin(m.x, m.y, m.z);
+      s.key_row[slot][i] = m.row;
     }
   }
 
-  // Bucket of (query, key): `query` and `key` as linear coordinates, or by the look-up.
   __device__ __forceinline__ int bucket(int qx, int qy, int qz, int kx, int ky, int kz) const {
     const int R = a.reach;
     const int x = lut[max(-R, min(R, sub_sat(kx, qx))) + R];
@@ -282,96 +286,107 @@ struct Block {
   }
 };
 
-// Buckets of a thread's 32 pairs: rows g and g + 8 of the warp's 16, columns 8 n + 2 (lane % 4) + {0,
-// 1}. FLIP: the rows are keys and the columns queries.
-template <typename T, int DP, bool FLIP>
-__device__ __forceinline__ void buckets(const Block<T, DP>& b, int slot, const PlanRow (&own)[2],
-                                        int (&idx)[8][4]) {
+// Calls use(n, e, bucket) for a thread's pairs: element e of fragment n is row g + 8 (e / 2) of the
+// warp's 16 and column 8 n + 2 (lane % 4) + e % 2. FLIP: the rows are keys and the columns queries.
+// WHOLE: all pairs are inside a window; otherwise indexes of the others (masked) are clamped.
+template <bool FLIP, bool WHOLE, typename T, int KB, typename F>
+__device__ __forceinline__ void each_pair(const Block<T, KB>& b, int slot, const PlanRow (&own)[2],
+                                          F&& use) {
   const int c2 = 2 * (threadIdx.x & 3);
-  if (b.linear) {
-    // inside a window every index is in the table; across windows (masked later) it is clamped
+  auto within = [](int v, unsigned top) { return WHOLE ? v : (int)min((unsigned)v, top); };
+  if (b.mode == LINEAR) {
     const unsigned top = (unsigned)b.cells() - 1u;
-    const int mid = (int)(top / 2);
-    const int l0 = b.lin(own[0]), l1 = b.lin(own[1]);
+    const int mid = FLIP ? (int)(top / 2) : -(int)(top / 2);
+    const int l[2] = {b.lin(own[0].x, own[0].y, own[0].z).x + mid,
+                      b.lin(own[1].x, own[1].y, own[1].z).x + mid};
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const int2 l = *reinterpret_cast<const int2*>(&b.s.key_lin[slot][n * 8 + c2]);
-      const int d[4] = {l.x - l0, l.y - l0, l.x - l1, l.y - l1};
+    for (int n = 0; n < KB / 8; ++n) {
+      // the linear coordinates of two neighbours: .x and .z
+      const int4 k = *reinterpret_cast<const int4*>(&b.s.key_lin[slot][n * 8 + c2]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        idx[n][e] = (int)min((unsigned)((FLIP ? -d[e] : d[e]) + mid), top);
+      for (int e = 0; e < 4; ++e) {
+        const int c = e & 1 ? k.z : k.x;
+        use(n, e, within(FLIP ? l[e >> 1] - c : c - l[e >> 1], top));
+      }
+    }
+  } else if (b.mode == JOINT) {
+    const unsigned top = (unsigned)(b.width() * b.width()) - 1u, ztop = (unsigned)b.width() - 1u;
+    const int mid = FLIP ? (int)(top / 2) : -(int)(top / 2);
+    const int zmid = FLIP ? b.a.reach : -b.a.reach;
+    int2 l[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] = b.lin(own[r].x, own[r].y, own[r].z);
+      l[r].x += mid;
+      l[r].y += zmid;
+    }
+#pragma unroll
+    for (int n = 0; n < KB / 8; ++n) {
+      const int4 k = *reinterpret_cast<const int4*>(&b.s.key_lin[slot][n * 8 + c2]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = e & 1 ? k.z : k.x, z = e & 1 ? k.w : k.y;
+        const int xy = within(FLIP ? l[e >> 1].x - c : c - l[e >> 1].x, top);
+        const int dz = within(FLIP ? l[e >> 1].y - z : z - l[e >> 1].y, ztop);
+        use(n, e, b.joint[xy] + b.lut[dz]);
+      }
     }
   } else {
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
+    for (int n = 0; n < KB / 8; ++n) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const KeyMeta k = b.s.key[slot][n * 8 + c2 + c];
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          idx[n][2 * r + c] =
+          use(n, 2 * r + c,
               FLIP ? b.bucket(k.x, k.y, k.z, own[r].x, own[r].y, own[r].z)
-                   : b.bucket(own[r].x, own[r].y, own[r].z, k.x, k.y, k.z);
+                   : b.bucket(own[r].x, own[r].y, own[r].z, k.x, k.y, k.z));
       }
     }
   }
 }
 
-// acc[n] += rows (operand fragments in registers) x tile^T over DP channels: 16 x 64 products.
-template <typename T, int DP>
-__device__ __forceinline__ void mma_nt(float (&acc)[8][4], const uint32_t (&frag)[DP / 16][4],
-                                       uint32_t tile) {
+// acc += rows x tile^T over DP channels, 16 rows by KB columns; the rows' fragments come from `rows`
+// (the warp's 16 rows of a tile).
+template <typename T, int DP, int KB>
+__device__ __forceinline__ void mma_nt(float (&acc)[KB / 8][4], uint32_t rows, uint32_t tile) {
   const int lane = threadIdx.x & 31;
-  const uint32_t at = tile + ((lane & 7) + (lane >> 4) * 8) * Tile<DP>::STRIDE +
-                      ((lane >> 3) & 1) * 16;
+  const uint32_t from = rows + (lane & 15) * STRIDE<DP> + (lane >> 4) * 16;
+  const uint32_t at = tile + ((lane & 7) + (lane >> 4) * 8) * STRIDE<DP> + ((lane >> 3) & 1) * 16;
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k) {
+    uint32_t f[4];
+    ldsm4(from + k * 32, f);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+    for (int n = 0; n < KB / 16; ++n) {
       uint32_t b[4];
-      ldsm4(at + n * 16 * Tile<DP>::STRIDE + k * 32, b);
-      mma<T>(acc[2 * n], frag[k], b[0], b[1]);
-      mma<T>(acc[2 * n + 1], frag[k], b[2], b[3]);
+      ldsm4(at + n * 16 * STRIDE<DP> + k * 32, b);
+      mma<T>(acc[2 * n], f, b[0], b[1]);
+      mma<T>(acc[2 * n + 1], f, b[2], b[3]);
     }
   }
 }
 
-// out += w (16 x 64, packed as operand fragments) x tile (64 x DP).
-template <typename T, int DP>
-__device__ __forceinline__ void mma_nn(float (&out)[DP / 8][4], const uint32_t (&w)[4][4],
+// out += w (16 x KB sums, rounded to T as operand fragments) x tile (KB x DP).
+template <typename T, int DP, int KB>
+__device__ __forceinline__ void mma_nn(float (&out)[DP / 8][4], const float (&w)[KB / 8][4],
                                        uint32_t tile) {
   const int lane = threadIdx.x & 31;
-  const uint32_t at = tile + ((lane & 7) + ((lane >> 3) & 1) * 8) * Tile<DP>::STRIDE +
-                      (lane >> 4) * 16;
+  const uint32_t at = tile + ((lane & 7) + ((lane >> 3) & 1) * 8) * STRIDE<DP> + (lane >> 4) * 16;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < KB / 16; ++k) {
+    const uint32_t f[4] = {pack2<T>(w[2 * k][0], w[2 * k][1]), pack2<T>(w[2 * k][2], w[2 * k][3]),
+                           pack2<T>(w[2 * k + 1][0], w[2 * k + 1][1]),
+                           pack2<T>(w[2 * k + 1][2], w[2 * k + 1][3])};
 #pragma unroll
     for (int n = 0; n < DP / 16; ++n) {
       uint32_t b[4];
-      ldsm4_t(at + k * 16 * Tile<DP>::STRIDE + n * 32, b);
-      mma<T>(out[2 * n], w[k], b[0], b[1]);
-      mma<T>(out[2 * n + 1], w[k], b[2], b[3]);
+      ldsm4_t(at + k * 16 * STRIDE<DP> + n * 32, b);
+      mma<T>(out[2 * n], f, b[0], b[1]);
+      mma<T>(out[2 * n + 1], f, b[2], b[3]);
     }
   }
-}
-
-template <typename T>
-__device__ __forceinline__ void pack_rows(const float (&s)[8][4], uint32_t (&w)[4][4]) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    w[k][0] = pack2<T>(s[2 * k][0], s[2 * k][1]);
-    w[k][1] = pack2<T>(s[2 * k][2], s[2 * k][3]);
-    w[k][2] = pack2<T>(s[2 * k + 1][0], s[2 * k + 1][1]);
-    w[k][3] = pack2<T>(s[2 * k + 1][2], s[2 * k + 1][3]);
-  }
-}
-
-template <int DP>
-__device__ __forceinline__ void load_frags(uint32_t tile, uint32_t (&f)[DP / 16][4]) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t at = tile + (warp * 16 + (lane & 15)) * Tile<DP>::STRIDE + (lane >> 4) * 16;
-#pragma unroll
-  for (int k = 0; k < DP / 16; ++k) ldsm4(at + k * 32, f[k]);
 }
 
 template <int W>
@@ -380,11 +395,6 @@ __device__ __forceinline__ void zero(float (&x)[W][4]) {
   for (int i = 0; i < W; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
-}
-
-// Which of the warp's rows see column `pos`: both bounds of a row's window.
-__device__ __forceinline__ bool sees(const PlanRow& r, int pos) {
-  return pos >= r.start && pos < r.end;
 }
 
 // Positions that any of the warp's 16 rows sees, and those that all of them do.
@@ -407,6 +417,14 @@ __device__ __forceinline__ Reach warp_reach(const PlanRow (&own)[2]) {
   return w;
 }
 
+// Whether column `col` of a tile that begins at position p0 is outside the row's window, or has no
+// row (`bad`: some column has none).
+template <int KB>
+__device__ __forceinline__ bool hidden(const PlanRow& r, int p0, int col, bool bad,
+                                       const Shared<KB>& s, int slot) {
+  return col < r.start - p0 || col >= r.end - p0 || (bad && s.key_row[slot][col] < 0);
+}
+
 // A weight of zero does not hide a NaN or an infinity that another window's row brings into a tile,
 // and fp16 score gradients can overflow where their sums do not. So rows that come out not finite
 // are computed again, one at a time, from their own windows alone.
@@ -427,7 +445,7 @@ __device__ __forceinline__ uint32_t not_finite(const float (&o)[DP / 8][4]) {
   return rows;
 }
 
-template <typename T, typename F>
+template <typename F>
 __device__ __forceinline__ void again(uint32_t rows, int64_t p0, uint8_t* scratch, F&& row) {
   while (rows) {  // the same in all lanes
     const int r = __ffs(rows) - 1;
@@ -439,112 +457,139 @@ __device__ __forceinline__ void again(uint32_t rows, int64_t p0, uint8_t* scratc
 
 template <typename T>
 __device__ __noinline__ void again_forward(AttnArgs a, int64_t p, int h, float* s) {
-  row_forward<T>(a, p, h, s);
+  row_forward<T, true>(a, p, h, s);
 }
 template <typename T>
 __device__ __noinline__ void again_dq(AttnArgs a, int64_t p, int h, float* s) {
-  row_dq<T, false>(a, p, h, s);
+  row_dq<T, true, false>(a, p, h, s);
 }
 template <typename T>
 __device__ __noinline__ void again_dkv(AttnArgs a, int64_t p, int h, float* s) {
-  row_dkv<T>(a, p, h, s);
+  row_dkv<T, true>(a, p, h, s);
 }
 
-template <int DP, int TILES>
-struct SmemLayout {
-  static constexpr int SHARED = TILES * Tile<DP>::BYTES;
-  static constexpr int TABLE = (SHARED + (int)sizeof(Shared) + 15) / 16 * 16;
+// Shared memory: OWN tiles of the block's rows, two buffers of two tiles of KB positions, then the
+// tables.
+template <int DP, int KB, int OWN>
+struct Layout {
+  static constexpr int OWN_TILE = BQ * STRIDE<DP>;
+  static constexpr int TILE = KB * STRIDE<DP>;
+  static constexpr int RING = OWN * OWN_TILE;
+  static constexpr int SHARED = RING + 4 * TILE;
+  static constexpr int TABLE = (SHARED + (int)sizeof(Shared<KB>) + 15) / 16 * 16;
 };
 
-__host__ __device__ inline size_t table_bytes(int nb, int words) { return (size_t)nb * nb * nb * 4 * words; }
-inline size_t lut_bytes(int reach) { return align_up((size_t)(2 * reach + 1) * 2, 16); }
+struct Tables {
+  int grad, lut, joint, total;  // byte offsets behind Layout::TABLE; joint < 0: none
+};
+__host__ __device__ inline Tables tables(const AttnArgs& a, bool grad) {
+  const int cells = a.nb * a.nb * a.nb, width = 2 * a.reach + 1;
+  Tables t;
+  t.grad = cells * 4;
+  t.lut = t.grad + (grad ? cells * 4 : 0);
+  t.joint = -1;
+  t.total = t.lut + (width * 2 + 15) / 16 * 16;
+  if (width * width <= JOINT_MAX) {
+    t.joint = t.total;
+    t.total += width * width * 2;
+  }
+  return t;
+}
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(AT) attn_tc_kernel(AttnArgs a, int per_block, bool vec) {
-  using L = SmemLayout<DP, 5>;
+template <typename T, int KB>
+__device__ __forceinline__ Block<T, KB> make_block(const AttnArgs& a, uint8_t* smem, int shared,
+                                                   int table, bool grad) {
+  const Tables t = tables(a, grad);
+  return Block<T, KB>{a, *reinterpret_cast<Shared<KB>*>(smem + shared),
+                      reinterpret_cast<float*>(smem + table),
+                      reinterpret_cast<int16_t*>(smem + table + t.lut),
+                      t.joint < 0 ? nullptr : reinterpret_cast<int16_t*>(smem + table + t.joint),
+                      (int)blockIdx.y, false, 0.f};
+}
+
+// The tiles of one block: `own` loads the block's own rows, `load(buffer, rows)` a tile's, and
+// body(t, buffer) works on tile t. One barrier a tile: behind it the tile has landed, the other
+// buffer's readers are done, and the rows of the next tile are known. `flush` is asked at the
+// barrier, by any thread, and done before the tile.
+template <bool STATS, typename B, typename Load, typename Body, typename Ask, typename Flush>
+__device__ __forceinline__ void walk(B& b, Load&& load, Body&& body, Ask&& ask, Flush&& flush) {
+  b.template stage_meta<STATS>(0);
+  b.template stage_meta<STATS>(1);
+  __syncthreads();
+  if (b.tiles > 0) load(0, b.s.key_row[0]);
+  cp_commit();
+  for (int t = 0; t < b.tiles; ++t) {
+    cp_wait<0>();
+    if (__syncthreads_or(ask())) flush();
+    if (t + 1 < b.tiles) load((t + 1) & 1, b.s.key_row[(t + 1) % 3]);
+    cp_commit();
+    if (t + 2 < b.tiles) b.template stage_meta<STATS>(t + 2);
+    body(t, t & 1);
+  }
+  cp_wait<0>();
+  __syncthreads();
+}
+
+template <typename T, int DP, int KB>
+__global__ void __launch_bounds__(AT, DP <= 64 ? 4 : 2)
+    attn_tc_kernel(AttnArgs a, int per_block, bool vec) {
+  using L = Layout<DP, KB, 1>;
   extern __shared__ __align__(16) uint8_t smem[];
-  uint8_t* s_q = smem;
-  uint8_t* s_kv = smem + Tile<DP>::BYTES;  // two buffers of k and v
-  Shared& sh = *reinterpret_cast<Shared*>(smem + L::SHARED);
-  float* table = reinterpret_cast<float*>(smem + L::TABLE);
+  Block<T, KB> b = make_block<T, KB>(a, smem, L::SHARED, L::TABLE, false);
+  Shared<KB>& sh = b.s;
   const int head = blockIdx.y;
-  Block<T, DP> b{a, sh, table,
-                 reinterpret_cast<int16_t*>(smem + L::TABLE + table_bytes(a.nb, 1)), head};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c2 = 2 * (lane & 3);
+  uint8_t* mine = smem + warp * 16 * STRIDE<DP>;  // the warp's rows of q
   const T* q = static_cast<const T*>(a.q) + head * a.q_head;
   const T* k = static_cast<const T*>(a.k) + head * a.k_head;
   const T* v = static_cast<const T*>(a.v) + head * a.v_head;
+  const float scale = a.scale * ATTN_LOG2E;
   b.stage_tables();
   const int64_t first = (int64_t)blockIdx.x * per_block;
   for (int64_t t64 = first; t64 < first + per_block && t64 * BQ < a.n; ++t64) {
     b.begin(t64 * BQ);
-    load_tile<T, DP>(s_q, q, a.q_row, sh.own_row, a.dim, vec);
-    b.template stage_meta<false>(0);
-    __syncthreads();
-    if (b.tiles > 0) {
-      load_tile<T, DP>(s_kv, k, a.k_row, sh.key_row[0], a.dim, vec);
-      load_tile<T, DP>(s_kv + Tile<DP>::BYTES, v, a.v_row, sh.key_row[0], a.dim, vec);
-    }
-    cp_commit();
-    b.template stage_meta<false>(1);
+    load_tile<T, DP, BQ>(smem, q, a.q_row, sh.own_row, a.dim, vec);
     const PlanRow own[2] = {sh.own[warp * 16 + g], sh.own[warp * 16 + g + 8]};
     const Reach w = warp_reach(own);
-    uint32_t fq[DP / 16][4];
     float o[DP / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
     zero(o);
-    for (int t = 0; t < b.tiles; ++t) {
-      __syncthreads();  // the other buffer's readers are done; the next tile's rows are known
-      uint8_t* tile = s_kv + (t & 1) * 2 * Tile<DP>::BYTES;
-      if (t + 1 < b.tiles) {
-        uint8_t* next = s_kv + ((t + 1) & 1) * 2 * Tile<DP>::BYTES;
-        load_tile<T, DP>(next, k, a.k_row, sh.key_row[(t + 1) % 3], a.dim, vec);
-        load_tile<T, DP>(next + Tile<DP>::BYTES, v, a.v_row, sh.key_row[(t + 1) % 3], a.dim, vec);
-        cp_commit();
-        cp_wait<1>();
-      } else {
-        cp_wait<0>();
-      }
-      __syncthreads();
-      if (t + 2 < b.tiles) b.template stage_meta<false>(t + 2);
-      if (t == 0) load_frags<DP>(smem_u32(s_q), fq);
-      const int p0 = b.j0 + t * BKV;
-      if (p0 >= w.hi || p0 + BKV <= w.lo) continue;
-      float s[8][4];
-      zero(s);
-      mma_nt<T, DP>(s, fq, smem_u32(tile));
+    auto body = [&](int t, int buf) {
+      const int p0 = b.j0 + t * KB;
+      if (p0 >= w.hi || p0 + KB <= w.lo) return;
+      const uint32_t tile = smem_u32(smem + L::RING + buf * 2 * L::TILE);
       const int slot = t % 3;
-      int idx[8][4];
-      buckets<T, DP, false>(b, slot, own, idx);
-      const bool whole = p0 >= w.all_lo && p0 + BKV <= w.all_hi && !sh.key_bad[slot][0] && !sh.key_bad[slot][1];
-      float m[2] = {top[0], top[1]};
+      float s[KB / 8][4];
+      zero(s);
+      mma_nt<T, DP, KB>(s, smem_u32(mine), tile);
+      auto score = [&](int n, int e, int at) { s[n][e] = fmaf(s[n][e], scale, b.table[at]); };
+      const bool bad = sh.key_bad[slot];
+      if (p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad) {
+        each_pair<false, true>(b, slot, own, score);
+      } else {
+        each_pair<false, false>(b, slot, own, score);
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], a.scale, table[idx[n][e]]);
-        if (!whole) {
-          const int pos0 = sh.key[slot][n * 8 + c2].pos, pos1 = sh.key[slot][n * 8 + c2 + 1].pos;
+        for (int n = 0; n < KB / 8; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (!sees(own[e >> 1], e & 1 ? pos1 : pos0)) s[n][e] = -INFINITY;
-        }
-        m[0] = fmaxf(m[0], fmaxf(s[n][0], s[n][1]));
-        m[1] = fmaxf(m[1], fmaxf(s[n][2], s[n][3]));
+            if (hidden(own[e >> 1], p0, n * 8 + c2 + (e & 1), bad, sh, slot)) s[n][e] = -INFINITY;
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 1));
-        m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 2));
-        const float base = m[r] == -INFINITY ? 0.f : m[r];
-        const float keep = exp2_fast((top[r] - base) * LOG2E);
-        top[r] = m[r];
+        float m = top[r];
+#pragma unroll
+        for (int n = 0; n < KB / 8; ++n) m = fmaxf(m, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const float base = m == -INFINITY ? 0.f : m;
+        const float keep = exp2_fast(top[r] - base);
+        top[r] = m;
         sum[r] *= keep;
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
+        for (int n = 0; n < KB / 8; ++n) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            // subtracted before it is scaled: the type's lowest value times log2(e) overflows
-            const float e = exp2_fast((s[n][2 * r + c] - base) * LOG2E);
+            const float e = exp2_fast(s[n][2 * r + c] - base);
             s[n][2 * r + c] = e;
             sum[r] += e;
           }
@@ -555,10 +600,16 @@ __global__ void __launch_bounds__(AT) attn_tc_kernel(AttnArgs a, int per_block, 
           o[n][2 * r + 1] *= keep;
         }
       }
-      uint32_t p[4][4];
-      pack_rows<T>(s, p);
-      mma_nn<T, DP>(o, p, smem_u32(tile + Tile<DP>::BYTES));
-    }
+      mma_nn<T, DP, KB>(o, s, tile + L::TILE);
+    };
+    walk<false>(
+        b,
+        [&](int buf, const int32_t* rows) {
+          uint8_t* tile = smem + L::RING + buf * 2 * L::TILE;
+          load_tile<T, DP, KB>(tile, k, a.k_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile + L::TILE, v, a.v_row, rows, a.dim, vec);
+        },
+        body, [] { return false; }, [] {});
     float inv[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -569,128 +620,107 @@ __global__ void __launch_bounds__(AT) attn_tc_kernel(AttnArgs a, int per_block, 
       if (a.stats && c2 == 0 && own[r].row >= 0)
         a.stats[head * a.n + t64 * BQ + warp * 16 + g + 8 * r] = st;
     }
-    __syncthreads();
-    store_rows<T, DP>(s_q, o, inv[0], inv[1], sh.own_row, static_cast<T*>(a.out), a.heads, head,
+    store_rows<T, DP>(smem, o, inv[0], inv[1], sh.own_row, static_cast<T*>(a.out), a.heads, head,
                       a.dim, vec);
-    again<T>(not_finite<DP>(o), t64 * BQ + warp * 16, s_q + warp * 16 * Tile<DP>::STRIDE,
-             [&](int64_t p, float* f) { if (p < a.n) again_forward<T>(a, p, head, f); });
+    again(not_finite<DP>(o), t64 * BQ + warp * 16, mine,
+          [&](int64_t p, float* f) { if (p < a.n) again_forward<T>(a, p, head, f); });
     __syncthreads();
   }
 }
 
-// delta_i = dout_i . o_i by position, and the largest |dout_i|^2 and |v_j|^2 of a head (bits order
-// like the values of these non-negative numbers, a NaN above everything).
+// delta_i = dout_i . o_i by position: eight lanes a row and head.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_prepare_kernel(AttnArgs a) {
-  __shared__ unsigned s_top[2];
-  const int h = blockIdx.y;
-  if (threadIdx.x < 2) s_top[threadIdx.x] = 0u;
-  __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned g_top = 0u, v_top = 0u;
-  for (int64_t p = (int64_t)blockIdx.x * 8 + warp; p < a.n; p += (int64_t)gridDim.x * 8) {
+__global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a, bool vec) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 8;  // head * n + position
+  const int sub = threadIdx.x & 7;
+  float d = 0.f;
+  if (at < a.n * a.heads) {
+    const int64_t h = at / a.n, p = at - h * a.n;
     const int32_t row = __ldg(&a.plan[p].row);
-    if (row < 0) continue;
-    const int64_t at = ((int64_t)row * a.heads + h) * a.dim;
-    const T* g = static_cast<const T*>(a.dout) + at;
-    const T* o = static_cast<const T*>(a.o) + at;
-    const T* v = static_cast<const T*>(a.v) + row * a.v_row + h * a.v_head;
-    float g2 = 0.f, v2 = 0.f, d = 0.f;
-    for (int c = lane; c < a.dim; c += 32) {
-      const float x = to_f32(g[c]), y = to_f32(v[c]);
-      g2 = fmaf(x, x, g2);
-      v2 = fmaf(y, y, v2);
-      d = fmaf(x, to_f32(o[c]), d);
-    }
+    if (row >= 0) {
+      const int64_t from = ((int64_t)row * a.heads + h) * a.dim;
+      const T* g = static_cast<const T*>(a.dout) + from;
+      const T* o = static_cast<const T*>(a.o) + from;
+      if (vec) {
+        for (int c = sub * 8; c < a.dim; c += 64) {
+          const uint4 x = *reinterpret_cast<const uint4*>(g + c);
+          const uint4 y = *reinterpret_cast<const uint4*>(o + c);
+          const T* xe = reinterpret_cast<const T*>(&x);
+          const T* ye = reinterpret_cast<const T*>(&y);
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-      g2 += __shfl_xor_sync(0xffffffffu, g2, s);
-      v2 += __shfl_xor_sync(0xffffffffu, v2, s);
-      d += __shfl_xor_sync(0xffffffffu, d, s);
+          for (int k = 0; k < 8; ++k) d = fmaf(to_f32(xe[k]), to_f32(ye[k]), d);
+        }
+      } else {
+        for (int c = sub; c < a.dim; c += 8) d = fmaf(to_f32(g[c]), to_f32(o[c]), d);
+      }
     }
-    if (lane == 0) a.delta[h * a.n + p] = d;
-    g_top = max(g_top, __float_as_uint(g2) & 0x7fffffffu);
-    v_top = max(v_top, __float_as_uint(v2) & 0x7fffffffu);
   }
-  if (lane == 0) {
-    atomicMax(&s_top[0], g_top);
-    atomicMax(&s_top[1], v_top);
-  }
-  __syncthreads();
-  if (threadIdx.x < 2 && a.dtable) atomicMax(a.norms + 2 * h + threadIdx.x, s_top[threadIdx.x]);
+#pragma unroll
+  for (int s = 4; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
+  if (sub == 0 && at < a.n * a.heads) a.delta[at] = d;
 }
 
-// A block's share of the table's gradient sums in two 32-bit words a bucket: whole units, and the
-// rest in 2^-12 of one. |dS| over a row sums to at most 2 max|dout| max|v| (attention.h), so
-// `rows` of them stay below 2^30 units, and 2^19 remainders of at most half a unit fit the other
-// word (a block meets fewer pairs of one bucket: it empties the words every 2^19 / 64 positions).
-__device__ __forceinline__ int block_exponent(const AttnArgs& a, int head, int rows) {
-  const float g2 = __uint_as_float(a.norms[2 * head]), v2 = __uint_as_float(a.norms[2 * head + 1]);
-  const double bound = 2.0 * sqrt((double)g2) * sqrt((double)v2) * (double)rows;
-  if (!(bound < 1e300)) return INT_MAX;
-  if (bound == 0.0) return 0;
+// The table's gradient in fixed point: a score gradient is at most 2^18 units (the head's largest is
+// known from the dk / dv pass), and sums to a 32-bit word per bucket in shared memory. A thread
+// counts the units it has added; the block empties its words into the 64-bit sums in global memory
+// before any thread's count can pass 2^24, so 128 threads cannot overflow a word. INT_MAX when a
+// score gradient was not finite.
+constexpr int UNIT_BITS = 18;
+__device__ __forceinline__ int unit_exponent(const AttnArgs& a, int head) {
+  const float top = __uint_as_float(a.norms[2 * head]);
+  if (!(top < INFINITY)) return INT_MAX;
+  if (top == 0.f) return 0;
   int e;
-  frexp(bound, &e);
-  return max(-120, min(100, 29 - e));  // a factor of two left for the products' rounding
+  frexpf(top, &e);                      // top < 2^e
+  return min(UNIT_BITS - 1 - e, 120);   // the two passes round their products differently
 }
 
 // dq and the table's gradient.
-template <typename T, int DP, bool TABLE>
-__global__ void __launch_bounds__(AT) attn_dq_tc_kernel(AttnArgs a, int per_block, bool vec) {
-  using L = SmemLayout<DP, 6>;
+template <typename T, int DP, int KB, bool TABLE>
+__global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
+    attn_dq_tc_kernel(AttnArgs a, int per_block, bool vec) {
+  using L = Layout<DP, KB, 2>;
   extern __shared__ __align__(16) uint8_t smem[];
-  uint8_t* s_q = smem;
-  uint8_t* s_g = smem + Tile<DP>::BYTES;
-  uint8_t* s_kv = smem + 2 * Tile<DP>::BYTES;
-  Shared& sh = *reinterpret_cast<Shared*>(smem + L::SHARED);
-  float* table = reinterpret_cast<float*>(smem + L::TABLE);
-  const int cells = a.nb * a.nb * a.nb;
-  int* s_hi = reinterpret_cast<int*>(table + cells);
-  int* s_lo = s_hi + cells;
+  Block<T, KB> b = make_block<T, KB>(a, smem, L::SHARED, L::TABLE, TABLE);
+  Shared<KB>& sh = b.s;
+  int* s_grad = reinterpret_cast<int*>(smem + L::TABLE + tables(a, TABLE).grad);
+  const int cells = b.cells();
   const int head = blockIdx.y;
-  Block<T, DP> b{a, sh, table,
-                 reinterpret_cast<int16_t*>(smem + L::TABLE + table_bytes(a.nb, TABLE ? 3 : 1)),
-                 head};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c2 = 2 * (lane & 3);
+  uint8_t* mine = smem + warp * 16 * STRIDE<DP>;
   const T* q = static_cast<const T*>(a.q) + head * a.q_head;
   const T* k = static_cast<const T*>(a.k) + head * a.k_head;
   const T* v = static_cast<const T*>(a.v) + head * a.v_head;
   const T* dout = static_cast<const T*>(a.dout) + (int64_t)head * a.dim;
   const int64_t g_row = (int64_t)a.heads * a.dim;
-  const int exponent = TABLE ? block_exponent(a, head, per_block * BQ) : INT_MAX;
+  const float scale = a.scale * ATTN_LOG2E;
+  const int exponent = TABLE ? unit_exponent(a, head) : INT_MAX;
   const float unit = exponent == INT_MAX ? 0.f : ldexpf(1.f, exponent);
+  // a thread adds KB / 2 pairs a tile
+  constexpr float LIMIT = 16777216.f - (KB / 2) * (float)(1 << UNIT_BITS);
+  float spent = 0.f;  // sum of |dS| since the words were emptied
   if constexpr (TABLE) {
-    for (int i = threadIdx.x; i < 2 * cells; i += AT) s_hi[i] = 0;
+    for (int i = threadIdx.x; i < cells; i += AT) s_grad[i] = 0;
   }
   b.stage_tables();
   auto flush = [&] {
     if constexpr (TABLE) {
-      __syncthreads();
       for (int i = threadIdx.x; i < cells; i += AT) {
-        const long long add = ((long long)s_hi[i] << 12) + s_lo[i];
+        const int add = s_grad[i];
+        s_grad[i] = 0;
         if (add != 0)
-          atomicAdd(a.dtable + (int64_t)head * cells + i, (unsigned long long)add);
-        s_hi[i] = 0;
-        s_lo[i] = 0;
+          atomicAdd(a.dtable + (int64_t)head * cells + i, (unsigned long long)(long long)add);
       }
+      spent = 0.f;
       __syncthreads();
     }
   };
-  int since = 0;  // tiles of pairs since the words were emptied
   const int64_t first = (int64_t)blockIdx.x * per_block;
   for (int64_t t64 = first; t64 < first + per_block && t64 * BQ < a.n; ++t64) {
     b.begin(t64 * BQ);
-    load_tile<T, DP>(s_q, q, a.q_row, sh.own_row, a.dim, vec);
-    load_tile<T, DP>(s_g, dout, g_row, sh.own_row, a.dim, vec);
-    b.template stage_meta<false>(0);
-    __syncthreads();
-    if (b.tiles > 0) {
-      load_tile<T, DP>(s_kv, k, a.k_row, sh.key_row[0], a.dim, vec);
-      load_tile<T, DP>(s_kv + Tile<DP>::BYTES, v, a.v_row, sh.key_row[0], a.dim, vec);
-    }
-    cp_commit();
-    b.template stage_meta<false>(1);
+    load_tile<T, DP, BQ>(smem, q, a.q_row, sh.own_row, a.dim, vec);
+    load_tile<T, DP, BQ>(smem + L::OWN_TILE, dout, g_row, sh.own_row, a.dim, vec);
     const PlanRow own[2] = {sh.own[warp * 16 + g], sh.own[warp * 16 + g + 8]};
     const Reach w = warp_reach(own);
     float2 stats[2];
@@ -703,207 +733,170 @@ __global__ void __launch_bounds__(AT) attn_dq_tc_kernel(AttnArgs a, int per_bloc
     }
     float dq[DP / 8][4];
     zero(dq);
-    for (int t = 0; t < b.tiles; ++t) {
-      __syncthreads();
-      uint8_t* tile = s_kv + (t & 1) * 2 * Tile<DP>::BYTES;
-      if (t + 1 < b.tiles) {
-        uint8_t* next = s_kv + ((t + 1) & 1) * 2 * Tile<DP>::BYTES;
-        load_tile<T, DP>(next, k, a.k_row, sh.key_row[(t + 1) % 3], a.dim, vec);
-        load_tile<T, DP>(next + Tile<DP>::BYTES, v, a.v_row, sh.key_row[(t + 1) % 3], a.dim, vec);
-        cp_commit();
-        cp_wait<1>();
-      } else {
-        cp_wait<0>();
-      }
-      __syncthreads();
-      if (t + 2 < b.tiles) b.template stage_meta<false>(t + 2);
-      if constexpr (TABLE) {
-        if (++since > (1 << 19) / BKV / BQ) {  // 64 x 64 pairs a tile
-          flush();
-          since = 1;
-        }
-      }
-      const int p0 = b.j0 + t * BKV;
-      if (p0 >= w.hi || p0 + BKV <= w.lo) continue;
-      float s[8][4], dp[8][4];
-      zero(s);
-      zero(dp);
-      {
-        uint32_t f[DP / 16][4];
-        load_frags<DP>(smem_u32(s_q), f);
-        mma_nt<T, DP>(s, f, smem_u32(tile));
-        load_frags<DP>(smem_u32(s_g), f);
-        mma_nt<T, DP>(dp, f, smem_u32(tile + Tile<DP>::BYTES));
-      }
+    auto body = [&](int t, int buf) {
+      const int p0 = b.j0 + t * KB;
+      if (p0 >= w.hi || p0 + KB <= w.lo) return;
+      const uint32_t tile = smem_u32(smem + L::RING + buf * 2 * L::TILE);
       const int slot = t % 3;
-      int idx[8][4];
-      buckets<T, DP, false>(b, slot, own, idx);
-      const bool whole = p0 >= w.all_lo && p0 + BKV <= w.all_hi && !sh.key_bad[slot][0] && !sh.key_bad[slot][1];
+      float s[KB / 8][4], dp[KB / 8][4];
+      zero(s);
+      mma_nt<T, DP, KB>(s, smem_u32(mine), tile);
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const int pos0 = sh.key[slot][n * 8 + c2].pos, pos1 = sh.key[slot][n * 8 + c2 + 1].pos;
+      for (int n = 0; n < KB / 8; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = e >> 1;
-          const float x = fmaf(s[n][e], a.scale, table[idx[n][e]]);
-          float ds = exp2_fast((x - stats[r].x) * LOG2E) * stats[r].y * (dp[n][e] - delta[r]);
-          const bool in = whole || sees(own[r], e & 1 ? pos1 : pos0);
-          if (!in) ds = 0.f;
-          s[n][e] = ds;
-          if constexpr (TABLE) {
-            if (in && exponent != INT_MAX) {
-              if (fabsf(ds) < INFINITY) {
-                const float f = ds * unit;
-                const float whole_units = rintf(f);
-                atomicAdd(s_hi + idx[n][e], __float2int_rn(whole_units));
-                atomicAdd(s_lo + idx[n][e], __float2int_rn((f - whole_units) * 4096.f));
-              } else {
-                atomicMax(a.norms + 2 * head, 0x7fffffffu);  // the head's table gradient is NaN
-              }
-            }
+        for (int e = 0; e < 4; ++e) dp[n][e] = -delta[e >> 1];
+      mma_nt<T, DP, KB>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
+      const bool bad = sh.key_bad[slot];
+      auto grad = [&](int n, int e, int at, bool in) {
+        const int r = e >> 1;
+        const float x = fmaf(s[n][e], scale, b.table[at]);
+        const float ds = exp2_fast(x - stats[r].x) * stats[r].y * dp[n][e];
+        s[n][e] = in ? ds : 0.f;
+        if constexpr (TABLE) {
+          if (in) {
+            spent += fabsf(ds);
+            // 1.5 * 2^23: the sum's low bits are the rounded integer
+            const float f = fmaf(ds, unit, 12582912.f);
+            atomicAdd(s_grad + at, __float_as_int(f) - 0x4b400000);
           }
         }
+      };
+      if (p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad) {
+        each_pair<false, true>(b, slot, own, [&](int n, int e, int at) { grad(n, e, at, true); });
+      } else {
+        each_pair<false, false>(b, slot, own, [&](int n, int e, int at) {
+          grad(n, e, at, !hidden(own[e >> 1], p0, n * 8 + c2 + (e & 1), bad, sh, slot));
+        });
       }
-      uint32_t p[4][4];
-      pack_rows<T>(s, p);
-      mma_nn<T, DP>(dq, p, smem_u32(tile));
-    }
-    __syncthreads();
-    store_rows<T, DP>(s_q, dq, a.scale, a.scale, sh.own_row, static_cast<T*>(a.dq), a.heads, head,
+      mma_nn<T, DP, KB>(dq, s, tile);
+    };
+    walk<false>(
+        b,
+        [&](int buf, const int32_t* rows) {
+          uint8_t* tile = smem + L::RING + buf * 2 * L::TILE;
+          load_tile<T, DP, KB>(tile, k, a.k_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile + L::TILE, v, a.v_row, rows, a.dim, vec);
+        },
+        body, [&] { return TABLE && spent * unit > LIMIT; }, flush);
+    store_rows<T, DP>(smem, dq, a.scale, a.scale, sh.own_row, static_cast<T*>(a.dq), a.heads, head,
                       a.dim, vec);
-    again<T>(not_finite<DP>(dq), t64 * BQ + warp * 16, s_q + warp * 16 * Tile<DP>::STRIDE,
-             [&](int64_t p, float* f) { if (p < a.n) again_dq<T>(a, p, head, f); });
+    again(not_finite<DP>(dq), t64 * BQ + warp * 16, mine,
+          [&](int64_t p, float* f) { if (p < a.n) again_dq<T>(a, p, head, f); });
     __syncthreads();
   }
   flush();
 }
 
-// dk and dv: the block's rows are keys, the tiles queries.
-template <typename T, int DP>
-__global__ void __launch_bounds__(AT) attn_dkv_tc_kernel(AttnArgs a, int per_block, bool vec) {
-  using L = SmemLayout<DP, 6>;
+// dk and dv, and the largest |dS| of the head: the block's rows are keys, the tiles queries.
+template <typename T, int DP, int KB, bool TABLE>
+__global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
+    attn_dkv_tc_kernel(AttnArgs a, int per_block, bool vec) {
+  using L = Layout<DP, KB, 2>;
   extern __shared__ __align__(16) uint8_t smem[];
-  uint8_t* s_k = smem;
-  uint8_t* s_v = smem + Tile<DP>::BYTES;
-  uint8_t* s_qg = smem + 2 * Tile<DP>::BYTES;
-  Shared& sh = *reinterpret_cast<Shared*>(smem + L::SHARED);
-  float* table = reinterpret_cast<float*>(smem + L::TABLE);
+  Block<T, KB> b = make_block<T, KB>(a, smem, L::SHARED, L::TABLE, false);
+  Shared<KB>& sh = b.s;
   const int head = blockIdx.y;
-  Block<T, DP> b{a, sh, table,
-                 reinterpret_cast<int16_t*>(smem + L::TABLE + table_bytes(a.nb, 1)), head};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c2 = 2 * (lane & 3);
+  uint8_t* mine = smem + warp * 16 * STRIDE<DP>;
   const T* q = static_cast<const T*>(a.q) + head * a.q_head;
   const T* k = static_cast<const T*>(a.k) + head * a.k_head;
   const T* v = static_cast<const T*>(a.v) + head * a.v_head;
   const T* dout = static_cast<const T*>(a.dout) + (int64_t)head * a.dim;
   const int64_t g_row = (int64_t)a.heads * a.dim;
+  const float scale = a.scale * ATTN_LOG2E;
+  float most = 0.f;
   b.stage_tables();
   const int64_t first = (int64_t)blockIdx.x * per_block;
   for (int64_t t64 = first; t64 < first + per_block && t64 * BQ < a.n; ++t64) {
     b.begin(t64 * BQ);
-    load_tile<T, DP>(s_k, k, a.k_row, sh.own_row, a.dim, vec);
-    load_tile<T, DP>(s_v, v, a.v_row, sh.own_row, a.dim, vec);
-    b.template stage_meta<true>(0);
-    __syncthreads();
-    if (b.tiles > 0) {
-      load_tile<T, DP>(s_qg, q, a.q_row, sh.key_row[0], a.dim, vec);
-      load_tile<T, DP>(s_qg + Tile<DP>::BYTES, dout, g_row, sh.key_row[0], a.dim, vec);
-    }
-    cp_commit();
-    b.template stage_meta<true>(1);
+    load_tile<T, DP, BQ>(smem, k, a.k_row, sh.own_row, a.dim, vec);
+    load_tile<T, DP, BQ>(smem + L::OWN_TILE, v, a.v_row, sh.own_row, a.dim, vec);
     const PlanRow own[2] = {sh.own[warp * 16 + g], sh.own[warp * 16 + g + 8]};
     const Reach w = warp_reach(own);
     float dk[DP / 8][4], dv[DP / 8][4];
     zero(dk);
     zero(dv);
-    for (int t = 0; t < b.tiles; ++t) {
-      __syncthreads();
-      uint8_t* tile = s_qg + (t & 1) * 2 * Tile<DP>::BYTES;
-      if (t + 1 < b.tiles) {
-        uint8_t* next = s_qg + ((t + 1) & 1) * 2 * Tile<DP>::BYTES;
-        load_tile<T, DP>(next, q, a.q_row, sh.key_row[(t + 1) % 3], a.dim, vec);
-        load_tile<T, DP>(next + Tile<DP>::BYTES, dout, g_row, sh.key_row[(t + 1) % 3], a.dim, vec);
-        cp_commit();
-        cp_wait<1>();
-      } else {
-        cp_wait<0>();
-      }
-      __syncthreads();
-      if (t + 2 < b.tiles) b.template stage_meta<true>(t + 2);
-      const int p0 = b.j0 + t * BKV;
-      if (p0 >= w.hi || p0 + BKV <= w.lo) continue;
+    auto body = [&](int t, int buf) {
+      const int p0 = b.j0 + t * KB;
+      if (p0 >= w.hi || p0 + KB <= w.lo) return;
+      const uint32_t tile = smem_u32(smem + L::RING + buf * 2 * L::TILE);
       const int slot = t % 3;
-      float s[8][4], dp[8][4];
+      float s[KB / 8][4], dp[KB / 8][4];
       zero(s);
-      {
-        uint32_t f[DP / 16][4];
-        load_frags<DP>(smem_u32(s_k), f);
-        mma_nt<T, DP>(s, f, smem_u32(tile));
-      }
-      {
-        int idx[8][4];
-        buckets<T, DP, true>(b, slot, own, idx);
-        const bool whole = p0 >= w.all_lo && p0 + BKV <= w.all_hi && !sh.key_bad[slot][0] && !sh.key_bad[slot][1];
+      mma_nt<T, DP, KB>(s, smem_u32(mine), tile);
+      const bool bad = sh.key_bad[slot];
+      const bool whole = p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad;
+      auto weight = [&](int n, int e, int at) {
+        const float2 st = sh.key_stats[slot][n * 8 + c2 + (e & 1)];
+        s[n][e] = exp2_fast(fmaf(s[n][e], scale, b.table[at]) - st.x) * st.y;
+      };
+      if (whole) {
+        each_pair<true, true>(b, slot, own, weight);
+      } else {
+        each_pair<true, false>(b, slot, own, weight);
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const int pos0 = sh.key[slot][n * 8 + c2].pos, pos1 = sh.key[slot][n * 8 + c2 + 1].pos;
-          // {maximum, 1 / sum} of the two queries
-          const float4 st = *reinterpret_cast<const float4*>(&sh.key_stats[slot][n * 8 + c2]);
+        for (int n = 0; n < KB / 8; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = fmaf(s[n][e], a.scale, table[idx[n][e]]);
-            s[n][e] = exp2_fast((x - (e & 1 ? st.z : st.x)) * LOG2E) * (e & 1 ? st.w : st.y);
-            if (!whole && !sees(own[e >> 1], e & 1 ? pos1 : pos0)) s[n][e] = 0.f;
-          }
-        }
+          for (int e = 0; e < 4; ++e)
+            if (hidden(own[e >> 1], p0, n * 8 + c2 + (e & 1), bad, sh, slot)) s[n][e] = 0.f;
       }
-      {
-        uint32_t p[4][4];
-        pack_rows<T>(s, p);
-        mma_nn<T, DP>(dv, p, smem_u32(tile + Tile<DP>::BYTES));
-      }
-      zero(dp);
-      {
-        uint32_t f[DP / 16][4];
-        load_frags<DP>(smem_u32(s_v), f);
-        mma_nt<T, DP>(dp, f, smem_u32(tile + Tile<DP>::BYTES));
-      }
+      mma_nn<T, DP, KB>(dv, s, tile + L::TILE);
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
+      for (int n = 0; n < KB / 8; ++n) {
         const float2 delta = *reinterpret_cast<const float2*>(&sh.key_delta[slot][n * 8 + c2]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          // a weight of zero may stand for a row of another window, which may hold anything
-          dp[n][e] = s[n][e] == 0.f ? 0.f : s[n][e] * (dp[n][e] - (e & 1 ? delta.y : delta.x));
+        dp[n][0] = dp[n][2] = -delta.x;
+        dp[n][1] = dp[n][3] = -delta.y;
       }
-      uint32_t p[4][4];
-      pack_rows<T>(dp, p);
-      mma_nn<T, DP>(dk, p, smem_u32(tile));
-    }
-    __syncthreads();
-    store_rows<T, DP>(s_k, dk, a.scale, a.scale, sh.own_row, static_cast<T*>(a.dk), a.heads, head,
+      mma_nt<T, DP, KB>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
+#pragma unroll
+      for (int n = 0; n < KB / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float ds = s[n][e] * dp[n][e];
+          // a weight of zero may stand for a row of another window, which may hold anything
+          if (!whole && s[n][e] == 0.f) ds = 0.f;
+          dp[n][e] = ds;
+          if constexpr (TABLE) most = max_nan(most, fabsf(ds));
+        }
+      mma_nn<T, DP, KB>(dk, dp, tile);
+    };
+    walk<true>(
+        b,
+        [&](int buf, const int32_t* rows) {
+          uint8_t* tile = smem + L::RING + buf * 2 * L::TILE;
+          load_tile<T, DP, KB>(tile, q, a.q_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile + L::TILE, dout, g_row, rows, a.dim, vec);
+        },
+        body, [] { return false; }, [] {});
+    store_rows<T, DP>(smem, dk, a.scale, a.scale, sh.own_row, static_cast<T*>(a.dk), a.heads, head,
                       a.dim, vec);
-    store_rows<T, DP>(s_v, dv, 1.f, 1.f, sh.own_row, static_cast<T*>(a.dv), a.heads, head, a.dim,
-                      vec);
-    again<T>(not_finite<DP>(dk) | not_finite<DP>(dv), t64 * BQ + warp * 16,
-             s_k + warp * 16 * Tile<DP>::STRIDE,
-             [&](int64_t p, float* f) { if (p < a.n) again_dkv<T>(a, p, head, f); });
+    store_rows<T, DP>(smem + L::OWN_TILE, dv, 1.f, 1.f, sh.own_row, static_cast<T*>(a.dv), a.heads,
+                      head, a.dim, vec);
+    again(not_finite<DP>(dk) | not_finite<DP>(dv), t64 * BQ + warp * 16, mine,
+          [&](int64_t p, float* f) { if (p < a.n) again_dkv<T>(a, p, head, f); });
     __syncthreads();
+  }
+  if constexpr (TABLE) {
+    // The two passes round dp - delta differently, by up to 2^-17 |delta| or so; a head whose score
+    // gradients are nothing but that must not get a unit so small that the other pass overflows it.
+    most = max_nan(most, b.delta_top * 0x1p-14f);
+    // bits of non-negative numbers order like the numbers, a NaN's above all
+    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
+    if (lane == 0 && top) atomicMax(a.norms + 2 * head, top);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256)
-    dtable_tc_finish_kernel(AttnArgs a, int rows, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) dtable_tc_finish_kernel(AttnArgs a, T* __restrict__ out) {
   const int cells = a.nb * a.nb * a.nb;
   const int h = blockIdx.y;
-  const int exponent = block_exponent(a, h, rows);
+  const int exponent = unit_exponent(a, h);
   for (int b = blockIdx.x * 256 + threadIdx.x; b < cells; b += gridDim.x * 256) {
     const int64_t at = (int64_t)h * cells + b;
     const double v = exponent == INT_MAX
-                         ? __longlong_as_double(0x7ff8000000000000ll)  // the inputs were not finite
-                         : ldexp((double)(long long)a.dtable[at], -exponent - 12);
+                         ? __longlong_as_double(0x7ff8000000000000ll)  // something was not finite
+                         : ldexp((double)(long long)a.dtable[at], -exponent);
     out[at] = from_f32<T>((float)v);
   }
 }
@@ -936,51 +929,44 @@ int allow_smem(K kernel, size_t bytes) {
   return SV_OK;
 }
 
-template <int DP, int TILES>
-size_t smem_bytes(const AttnArgs& a, int words) {
-  return SmemLayout<DP, TILES>::TABLE + table_bytes(a.nb, words) + lut_bytes(a.reach);
-}
+constexpr int KB = 32;  // positions of a tile
 
 template <typename T, int DP>
 int forward(const AttnArgs& a, cudaStream_t s) {
-  const size_t bytes = smem_bytes<DP, 5>(a, 1);
-  const int rc = allow_smem(attn_tc_kernel<T, DP>, bytes);
+  const size_t bytes = Layout<DP, KB, 1>::TABLE + tables(a, false).total;
+  const int rc = allow_smem(attn_tc_kernel<T, DP, KB>, bytes);
   if (rc != SV_OK) return rc;
   const int per = tiles_per_block(a, 12);
   const int64_t blocks = ((a.n + BQ - 1) / BQ + per - 1) / per;
-  attn_tc_kernel<T, DP><<<dim3((unsigned)blocks, a.heads), AT, bytes, s>>>(a, per, wide_rows(a));
+  attn_tc_kernel<T, DP, KB><<<dim3((unsigned)blocks, a.heads), AT, bytes, s>>>(a, per,
+                                                                               wide_rows(a));
   SV_LAUNCH_CHECK();
   return SV_OK;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool TABLE>
 int backward(const AttnArgs& a, void* dtable, cudaStream_t s) {
-  const unsigned prep = (unsigned)((a.n + 63) / 64 < 512 ? (a.n + 63) / 64 : 512);
-  attn_prepare_kernel<T><<<dim3(prep, a.heads), 256, 0, s>>>(a);
-  SV_LAUNCH_CHECK();
   const bool vec = wide_rows(a);
+  attn_delta_kernel<T><<<(unsigned)((a.n * a.heads + 31) / 32), 256, 0, s>>>(
+      a, vec && aligned16(a.o));
+  SV_LAUNCH_CHECK();
   const int per = tiles_per_block(a, 6);
   const dim3 grid((unsigned)(((a.n + BQ - 1) / BQ + per - 1) / per), a.heads);
-  size_t bytes = smem_bytes<DP, 6>(a, dtable ? 3 : 1);
-  int rc = dtable ? allow_smem(attn_dq_tc_kernel<T, DP, true>, bytes)
-                  : allow_smem(attn_dq_tc_kernel<T, DP, false>, bytes);
+  size_t bytes = Layout<DP, KB, 2>::TABLE + tables(a, false).total;
+  int rc = allow_smem(attn_dkv_tc_kernel<T, DP, KB, TABLE>, bytes);
   if (rc != SV_OK) return rc;
-  if (dtable)
-    attn_dq_tc_kernel<T, DP, true><<<grid, AT, bytes, s>>>(a, per, vec);
-  else
-    attn_dq_tc_kernel<T, DP, false><<<grid, AT, bytes, s>>>(a, per, vec);
+  attn_dkv_tc_kernel<T, DP, KB, TABLE><<<grid, AT, bytes, s>>>(a, per, vec);
   SV_LAUNCH_CHECK();
-  if (dtable) {
+  bytes = Layout<DP, KB, 2>::TABLE + tables(a, TABLE).total;
+  rc = allow_smem(attn_dq_tc_kernel<T, DP, KB, TABLE>, bytes);
+  if (rc != SV_OK) return rc;
+  attn_dq_tc_kernel<T, DP, KB, TABLE><<<grid, AT, bytes, s>>>(a, per, vec);
+  SV_LAUNCH_CHECK();
+  if constexpr (TABLE) {
     const unsigned blocks = (unsigned)((a.nb * a.nb * a.nb + 255) / 256);
-    dtable_tc_finish_kernel<T><<<dim3(blocks, a.heads), 256, 0, s>>>(a, per * BQ,
-                                                                     static_cast<T*>(dtable));
+    dtable_tc_finish_kernel<T><<<dim3(blocks, a.heads), 256, 0, s>>>(a, static_cast<T*>(dtable));
     SV_LAUNCH_CHECK();
   }
-  bytes = smem_bytes<DP, 6>(a, 1);
-  rc = allow_smem(attn_dkv_tc_kernel<T, DP>, bytes);
-  if (rc != SV_OK) return rc;
-  attn_dkv_tc_kernel<T, DP><<<grid, AT, bytes, s>>>(a, per, vec);
-  SV_LAUNCH_CHECK();
   return SV_OK;
 }
 
@@ -993,9 +979,11 @@ int forward_typed(const AttnArgs& a, cudaStream_t s) {
 
 template <typename T>
 int backward_typed(const AttnArgs& a, void* dtable, cudaStream_t s) {
-  if (a.dim <= 32) return backward<T, 32>(a, dtable, s);
-  if (a.dim <= 64) return backward<T, 64>(a, dtable, s);
-  return backward<T, 128>(a, dtable, s);
+  if (a.dim <= 32)
+    return dtable ? backward<T, 32, true>(a, dtable, s) : backward<T, 32, false>(a, dtable, s);
+  if (a.dim <= 64)
+    return dtable ? backward<T, 64, true>(a, dtable, s) : backward<T, 64, false>(a, dtable, s);
+  return dtable ? backward<T, 128, true>(a, dtable, s) : backward<T, 128, false>(a, dtable, s);
 }
 
 }  // namespace

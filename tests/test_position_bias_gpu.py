@@ -63,6 +63,7 @@ def _reference(x, q, k, v, table, lut, window, shift, dout=None):
     flat = table.reshape(heads, -1)
     val["dtable"], off["dtable"] = torch.zeros_like(flat), torch.zeros_like(flat)
     count = torch.zeros(nb**3, dtype=F64, device=DEV)
+    top = torch.zeros(heads, dtype=F64, device=DEV)
     groups = attention_windows(_tensor(x.coords), window, shift)
     for rows in groups.as_list():
         rows = rows.long()
@@ -109,12 +110,17 @@ def _reference(x, q, k, v, table, lut, window, shift, dout=None):
             off[m][rows] = (bound + (e + 4 * U) * (value.abs() + bound)).transpose(0, 1)
         val["dtable"].index_add_(1, b.flatten(), ds.flatten(1))
         off["dtable"].index_add_(1, b.flatten(), ds32_off.flatten(1))
+        top = torch.maximum(top, torch.maximum(ds.abs().amax((1, 2)),
+                                               2.0**-14 * delta.abs().amax((1, 2))))
         count.index_add_(0, b.flatten(), torch.ones_like(b.flatten(), dtype=F64))
     if g is not None:
-        # the fixed-point table: half a unit a pair, the unit 2^-41 (29 and 12 places) of up to twice
-        # the bound 2 |g| |v| of a row's terms times the 64 rows of a block: 2^-35 of it
-        unit = 2.0**-35 * 2 * g.norm(dim=2).amax(0) * v.norm(dim=2).amax(0)
-        off["dtable"] += unit[:, None] * count
+        # the 16-bit kernels sum the table in fixed point: half a unit a pair, the unit 2^-17 of the
+        # power of two above the head's largest |ds| (at least 2^-14 of the largest |delta|)
+        # fp32: half of 2^-61 of the power of two above 2 n |g| |v|
+        half_unit = 2.0**-17 * top
+        if dtype == torch.float32:
+            half_unit = 2.0**-61 * 2 * n * g.norm(dim=2).amax(0) * v.norm(dim=2).amax(0)
+        off["dtable"] += half_unit[:, None] * count
         off["dtable"] += e * (val["dtable"].abs() + off["dtable"])
     shape = (heads, nb, nb, nb)
     val["dtable"], off["dtable"] = val["dtable"].view(shape), off["dtable"].view(shape)
