@@ -323,7 +323,9 @@ __global__ void __launch_bounds__(256)
       if (z) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float v = to_float(d[e]) * activate_slope(to_float(zz[e]), act);
+          const float zf = to_float(zz[e]);
+          const float v = to_float(d[e]) * (sizeof(T) == 2 ? activate_slope_half(zf, act)
+                                                           : activate_slope(zf, act));
           sum[e] += v;
           d[e] = from_f32<T>(v);
         }
@@ -410,7 +412,8 @@ enum class Path { kEmpty, kFew, kF32, kTensor };
 
 struct Plan {
   Path path;
-  int bn;       // tensor-core tile width, or 64 / 128 for the fp32 tiles
+  TcTile tile;  // tensor cores
+  bool small;   // fp32: 64 x 64 tiles
   int splits;
   size_t partial_bytes;
 };
@@ -431,6 +434,14 @@ size_t copy_bytes(const Extent& e, int dtype) {
   return align_up((size_t)e.rows * align_up((size_t)e.cols * elem_size(dtype), 16), COPY_ALIGN);
 }
 
+void set_splits(Plan* p, int64_t want, int64_t steps, int64_t m, int64_t n) {
+  if (want <= 1) return;
+  want = std::min<int64_t>(want, 64);
+  const int64_t part = (steps + want - 1) / want;
+  p->splits = (int)((steps + part - 1) / part);  // no part is empty
+  if (p->splits > 1) p->partial_bytes = align_up((size_t)p->splits * m * n * 4, COPY_ALIGN);
+}
+
 Plan plan_gemm(int64_t m, int64_t n, int64_t k, int dtype, bool a_mn, bool b_mn) {
   Plan p{};
   p.splits = 1;
@@ -443,35 +454,44 @@ Plan plan_gemm(int64_t m, int64_t n, int64_t k, int dtype, bool a_mn, bool b_mn)
     return p;
   }
   const int64_t sms = num_sms();
-  int64_t tiles, steps;  // tiles of the result, k blocks of a tile
   if (dtype == SV_FLOAT32) {
     p.path = Path::kF32;
-    tiles = ((m + 127) / 128) * ((n + 127) / 128);
-    p.bn = 128;
-    if (tiles < sms) {
-      p.bn = 64;
-      tiles = ((m + 63) / 64) * ((n + 63) / 64);
-    }
-    steps = (k + 4 * FK - 1) / (4 * FK);
-  } else {
-    p.path = Path::kTensor;
-    const int64_t rows = (m + 127) / 128;
-    // the widest tile that still gives every SM one: 256 columns re-read A least
-    p.bn = 256;
-    while (p.bn > 64 && (rows * ((n + p.bn - 1) / p.bn) < sms || n <= p.bn / 2)) p.bn /= 2;
-    tiles = rows * ((n + p.bn - 1) / p.bn);
-    steps = (k * elem_size(dtype) + 127) / 128;
+    int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128);
+    p.small = tiles < sms;
+    if (p.small) tiles = ((m + 63) / 64) * ((n + 63) / 64);
+    const int64_t steps = (k + 4 * FK - 1) / (4 * FK);
+    // split the k axis while tiles are fewer than SMs, each part at least 4 steps long
+    if (tiles < sms && steps >= 8) set_splits(&p, std::min(sms / tiles, steps / 4), steps, m, n);
+    return p;
   }
-  // Split the k axis while tiles are fewer than SMs, each part at least 4 blocks long: a part
-  // costs an fp32 tile written and read again.
-  if (tiles < sms && steps >= 8) {
-    const int64_t want = std::min(sms / tiles, steps / 4);
-    if (want > 1) {
-      const int64_t part = (steps + std::min<int64_t>(want, 64) - 1) / std::min<int64_t>(want, 64);
-      p.splits = (int)((steps + part - 1) / part);  // no part is empty
-      p.partial_bytes = align_up((size_t)p.splits * m * n * 4, COPY_ALIGN);
+  p.path = Path::kTensor;
+  // The tile and the split of the k axis with the least estimated time, in cycles: a 128-byte k step
+  // costs the stage's bytes at the 64 bytes a cycle that an SM draws from L2, a round of tiles
+  // its steps and about 1500 cycles to fill the pipeline and drain the accumulator, and a split
+  // its fp32 sums written and read at about 3 KB a cycle, plus a launch.
+  const int64_t steps = (k * elem_size(dtype) + 127) / 128;
+  struct { TcTile tile; int rows, cols, step_cycles; int64_t units; } const choices[] = {
+      {TcTile::kPair256, 256, 256, 512, sms / 2},
+      {TcTile::kPair128, 256, 128, 384, sms / 2},
+      {TcTile::kOne128, 128, 128, 512, sms},
+      {TcTile::kOne64, 128, 64, 384, sms},
+  };
+  int64_t best = INT64_MAX, splits = 1;
+  for (const auto& c : choices) {
+    const int64_t tiles = ((m + c.rows - 1) / c.rows) * ((n + c.cols - 1) / c.cols);
+    const int64_t most = tiles < c.units ? std::max<int64_t>(1, std::min(c.units / tiles, steps / 4)) : 1;
+    for (int64_t parts = 1; parts <= most; parts = parts < most && parts * 2 > most ? most : parts * 2) {
+      const int64_t rounds = (tiles * parts + c.units - 1) / c.units;
+      int64_t cost = rounds * ((steps + parts - 1) / parts * c.step_cycles + 1500);
+      if (parts > 1) cost += parts * m * n * 8 / 3000 + 4000;
+      if (cost < best) {
+        best = cost;
+        p.tile = c.tile;
+        splits = parts;
+      }
     }
   }
+  set_splits(&p, splits, steps, m, n);
   return p;
 }
 
@@ -520,13 +540,13 @@ int run_gemm(Gemm g, void* workspace, size_t workspace_bytes, int32_t* status, c
   }
   int rc;
   if (p.path == Path::kF32) {
-    rc = gemm_f32(g, p.bn == 64, s);
+    rc = gemm_f32(g, p.small, s);
   } else {
     if (copy_a && (rc = copy_operand(&g.a, extent(g.a.mn, g.m, g.k), g.dtype, &at, s)) != SV_OK)
       return rc;
     if (copy_b && (rc = copy_operand(&g.b, extent(g.b.mn, g.n, g.k), g.dtype, &at, s)) != SV_OK)
       return rc;
-    rc = gemm_tc(g, p.bn, status, s);
+    rc = gemm_tc(g, p.tile, status, s);
   }
   if (rc != SV_OK || p.splits == 1) return rc;
   return finish(g, partial, p.splits, s);

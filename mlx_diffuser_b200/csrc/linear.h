@@ -42,8 +42,12 @@ struct Gemm {
   Epilogue ep;
 };
 
-// linear_tc.cu. `bn`: the tile's width. Operands 16-byte aligned with row strides of a multiple of 16 bytes.
-int gemm_tc(const Gemm& g, int bn, int32_t* status, cudaStream_t s);
+// Tensor-core tiles: 256 rows by a pair of CTAs, or 128 by one, and their columns.
+enum class TcTile { kPair256, kPair128, kOne128, kOne64 };
+
+// linear_tc.cu. Operands 16-byte aligned with row strides of a multiple of 16 bytes; no split of the
+// k axis may be empty.
+int gemm_tc(const Gemm& g, TcTile tile, int32_t* status, cudaStream_t s);
 
 #ifdef __CUDACC__
 constexpr float SQRT_HALF = 0.70710678118654752f;
@@ -64,6 +68,22 @@ __device__ __forceinline__ float activate(float z, int act) {
   return z;
 }
 
+// Phi(z), the normal distribution's integral, by Abramowitz and Stegun's 7.1.26, off by at most
+// 7.5e-8: for the 16-bit types, whose rounding is far above that. `gauss`: exp(-z^2 / 2).
+__device__ __forceinline__ float normal_half(float z, float gauss) {
+  const float t = __fdividef(1.0f, fmaf(0.3275911f * SQRT_HALF, fabsf(z), 1.0f));
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f),
+                                   -0.284496736f), 0.254829592f);
+  const float tail = 0.5f * p * gauss;
+  return z < 0.0f ? tail : 1.0f - tail;
+}
+
+// The activation for results of 16 bits.
+__device__ __forceinline__ float activate_half(float z, int act) {
+  if (act == SV_ACT_GELU) return z * normal_half(z, __expf(-0.5f * z * z));
+  return activate(z, act);
+}
+
 // The activation's derivative.
 __device__ __forceinline__ float activate_slope(float z, int act) {
   if (act == SV_ACT_SILU) {
@@ -78,6 +98,14 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
     return g + z * g * (1.0f - g) * GELU_TANH_2C * (1.0f + 3.0f * GELU_CUBE * z * z);
   }
   return 1.0f;
+}
+
+__device__ __forceinline__ float activate_slope_half(float z, int act) {
+  if (act == SV_ACT_GELU) {
+    const float gauss = __expf(-0.5f * z * z);
+    return normal_half(z, gauss) + z * 0.39894228040143268f * gauss;
+  }
+  return activate_slope(z, act);
 }
 
 template <typename O>

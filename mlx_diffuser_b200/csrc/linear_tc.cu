@@ -2,20 +2,29 @@
 //
 //     C[i][j] = sum_l A(i, l) B(j, l), fp32 accumulation in TMEM, then the fused epilogue
 //
-// A tile is 128 rows by BN columns; a persistent CTA per SM takes tiles blockIdx.x, + gridDim.x,
-// ... in an order whose columns vary fastest, so the tiles that run together share rows of A and
-// the whole of B out of L2. Operands come by TMA in stages of 128 bytes of k (64 16-bit or 128
-// 8-bit elements), 128-byte swizzled:
-//   K-major (rows of the operand run along k): a box is 128 bytes of k by 128 / BN rows;
+// PAIR: two CTAs of a cluster form one 256-row tile (cta_group::2): each holds 128 rows of A, half of
+// the tile's rows of B and its own 128 rows of the sums, so a row of B crosses L2 once per 256 rows
+// of the result. Otherwise a CTA forms a 128-row tile by itself, for products too small to give every
+// pair a tile. What bounds the kernel is that traffic: single 128 x 256 tiles ran at 10.6 TB/s out of
+// L2 with the tensor pipe 56% busy (40,662 x 1024 -> 4096 bf16, 367 us).
+//
+// A persistent unit (CTA or pair) takes tiles unit, + units, ... in an order whose columns vary
+// fastest, so the tiles that run together share rows of A and the whole of B out of L2. Operands
+// come by TMA in stages of 128 bytes of k (64 16-bit or 128 8-bit elements), 128-byte swizzled:
+//   K-major (rows of the operand run along k): a box is 128 bytes of k by the CTA's rows;
 //   MN-major (the gradients' operands, transposed in place): a box is 64 rows by 64 k, laid out as
 //   8-k-row atoms; boxes follow each other 8 KB apart along the rows.
 // Warp roles (320 threads):
-//   warp 0      TMA producer;
-//   warp 1      TMEM allocator (two BN-column accumulators) and the tcgen05.mma issuer;
+//   warp 0      TMA producer, each CTA for its own rows; the bytes of both count on the first
+//               CTA's barrier;
+//   warp 1      TMEM allocator (two BN-column accumulators) and, in the first CTA, the tcgen05.mma
+//               issuer, whose commits free the stages of both CTAs;
 //   warps 2-9   epilogue: two warps per 32-lane quadrant, half of the columns each, overlapped
-//               with the next tile's products through the second accumulator.
-// Every wait is bounded (2 s, CTA abort flag); on expiry SV_DEVICE_WAIT_TIMEOUT is reported and the
-// copies and products in flight are waited for before the CTA ends.
+//               with the next tile's products through the second accumulator. Sums go through
+//               shared memory, 32 x 32 at a time, so that bias, residual and results are read and
+//               written in whole row segments.
+// Every wait on an mbarrier is bounded (2 s, CTA abort flag); on expiry SV_DEVICE_WAIT_TIMEOUT is
+// reported and the copies and products in flight are waited for before the CTA ends.
 #include <algorithm>
 
 #include "linear.h"
@@ -23,49 +32,124 @@
 namespace sv {
 namespace {
 
-constexpr int TM = 128;
+constexpr int TM = 128;  // rows of a CTA's tile
 constexpr int TC_THREADS = 320;
 constexpr int EPI_THREADS = 256;
+constexpr int EPI_WARPS = EPI_THREADS / 32;
 constexpr uint32_t ATOM = 1024;           // 8 rows of 128 bytes
 constexpr uint32_t MN_STRIDE = 8 * ATOM;  // next 64 rows of an MN-major operand
+constexpr int CHUNK_LD = 36;  // floats between staged rows: 16-byte rows in different banks
 
-template <int BN>
+template <int BN, bool PAIR>
 struct TcLayout {
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // of one CTA
   static constexpr int A_STAGE = TM * 128;
-  static constexpr int B_STAGE = BN * 128;
-  static constexpr int FIT = (192 * 1024) / (A_STAGE + B_STAGE);
-  static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+  static constexpr int B_STAGE = B_ROWS * 128;
+  static constexpr int FIT = (176 * 1024) / (A_STAGE + B_STAGE);
+  static constexpr int STAGES = FIT > 7 ? 7 : FIT;
   static constexpr int A_OFF = 0;
   static constexpr int B_OFF = STAGES * A_STAGE;
-  static constexpr int COL_OFF = B_OFF + STAGES * B_STAGE;  // float [2 buffers][2][BN]
+  static constexpr int CHUNK_OFF = B_OFF + STAGES * B_STAGE;  // float [8 warps][32][CHUNK_LD]
+  static constexpr int COL_OFF = CHUNK_OFF + EPI_WARPS * 32 * CHUNK_LD * 4;  // [2][bias, scale][BN]
   static constexpr int MISC_OFF = COL_OFF + 2 * 2 * BN * 4;
   static constexpr int BAR_OFF = MISC_OFF + 16;
   static constexpr int NUM_BARS = 2 * STAGES + 5;
   static constexpr int SMEM = BAR_OFF + NUM_BARS * 8 + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
+  static_assert(STAGES >= 4, "pipeline depth");
 };
 
 struct TcArgs {
   int64_t m, n;
   int32_t tiles_n, tiles;    // tiles of one split
   int32_t total;             // tiles * splits
+  int32_t units;             // CTAs, or pairs
   int32_t steps, part;       // 128-byte k steps in all, and of one split
   uint32_t idesc;
   bool e4m3, a_mn, b_mn, wide_io;
 };
 
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
 }
 
-__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                          uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The address of the first CTA's copy of a shared-memory object.
+__device__ __forceinline__ uint32_t in_first(uint32_t addr) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const void* tmap, uint32_t bar,
+                                              int32_t x, int32_t y) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(tmap), "r"(bar), "r"(x), "r"(y)
       : "memory");
+}
+
+template <bool PAIR, bool F8>
+__device__ __forceinline__ void issue_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t more) {
+#define SV_MMA(group, kind)                                                    \
+  asm volatile(                                                                \
+      "{\n\t.reg .pred p;\n\t"                                                 \
+      "setp.ne.b32 p, %4, 0;\n\t"                                              \
+      "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), \
+      "l"(a), "l"(b), "r"(idesc), "r"(more)                                    \
+      : "memory")
+  if constexpr (PAIR && F8) SV_MMA("2", "f8f6f4");
+  else if constexpr (PAIR) SV_MMA("2", "f16");
+  else if constexpr (F8) SV_MMA("1", "f8f6f4");
+  else SV_MMA("1", "f16");
+#undef SV_MMA
+}
+
+// Arrive, in both CTAs of a pair, when every product issued so far has completed.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    tc_commit(bar);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void alloc_tmem(uint32_t* dst, uint32_t cols) {
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(dst)),
+                 "r"(cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  } else {
+    tmem_alloc(dst, cols);
+    tmem_relinquish();
+  }
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void free_tmem(uint32_t addr, uint32_t cols) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+  else
+    tmem_dealloc(addr, cols);
 }
 
 __device__ __forceinline__ void epi_sync() {
@@ -73,91 +157,82 @@ __device__ __forceinline__ void epi_sync() {
 }
 
 struct Tile {
-  int32_t split, m0, n0, k0, k1;  // k in 128-byte steps
+  int32_t split, m0, n0, k0, k1;  // k in 128-byte steps; m0 of the whole tile
 };
 
-template <int BN>
+template <int BN, bool PAIR>
 __device__ __forceinline__ Tile tile_at(const TcArgs& a, int32_t t) {
   Tile o;
   o.split = t / a.tiles;
   const int32_t r = t - o.split * a.tiles;
   const int32_t row = r / a.tiles_n;
-  o.m0 = row * TM;
+  o.m0 = row * (PAIR ? 2 * TM : TM);
   o.n0 = (r - row * a.tiles_n) * BN;
   o.k0 = o.split * a.part;
   o.k1 = min(o.k0 + a.part, a.steps);
   return o;
 }
 
-// 32 consecutive columns of one row from fp32 sums to the output. `vec`: 16-byte accesses.
-template <typename O>
-__device__ __forceinline__ void finish_chunk(const Epilogue& ep, const float* s_bias,
-                                             const float* s_scale, int64_t row, int64_t col,
-                                             int64_t n, float row_scale, bool vec, bool scaled,
-                                             float (&v)[32]) {
+template <int ACT, int W>
+__device__ __forceinline__ void activate_all(float (&v)[W]) {
+#pragma unroll
+  for (int j = 0; j < W; ++j) v[j] = activate_half(v[j], ACT);
+}
+
+template <int W>
+__device__ __forceinline__ void activate_by(float (&v)[W], int act) {
+  if (act == SV_ACT_SILU) activate_all<SV_ACT_SILU>(v);
+  else if (act == SV_ACT_GELU) activate_all<SV_ACT_GELU>(v);
+  else if (act == SV_ACT_GELU_TANH) activate_all<SV_ACT_GELU_TANH>(v);
+}
+
+// W consecutive columns of one row: scale, bias, activation, residual, stores.
+template <typename O, int W>
+__device__ __forceinline__ void finish(const Epilogue& ep, float (&v)[W], const float* bias,
+                                       const float* scale, float row_scale, bool scaled,
+                                       int64_t at, int64_t at_res) {
   if (scaled) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= row_scale * s_scale[j];
+    for (int j = 0; j < W; ++j) v[j] *= row_scale * scale[j];
   }
   if (ep.bias) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += s_bias[j];
+    for (int j = 0; j < W; ++j) v[j] += bias[j];
   }
-  constexpr int E = 16 / sizeof(O);
-  const bool full = vec && col + 32 <= n;
   auto store = [&](void* base) {
-    O* dst = static_cast<O*>(base) + row * n + col;
-    if (full) {
+    O* dst = static_cast<O*>(base) + at;
+    if constexpr (W == 8) {
+      uint4 raw;
+      O* e = reinterpret_cast<O*>(&raw);
 #pragma unroll
-      for (int q = 0; q < 32 / E; ++q) {
-        uint4 raw;
-        O* e = reinterpret_cast<O*>(&raw);
-#pragma unroll
-        for (int j = 0; j < E; ++j) e[j] = from_f32<O>(v[q * E + j]);
-        reinterpret_cast<uint4*>(dst)[q] = raw;
-      }
+      for (int j = 0; j < 8; ++j) e[j] = from_f32<O>(v[j]);
+      *reinterpret_cast<uint4*>(dst) = raw;
     } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col + j < n) dst[j] = from_f32<O>(v[j]);
+      *dst = from_f32<O>(v[0]);
     }
   };
   if (ep.preact) store(ep.preact);
-  if (ep.act == SV_ACT_SILU) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = activate(v[j], SV_ACT_SILU);
-  } else if (ep.act == SV_ACT_GELU) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = activate(v[j], SV_ACT_GELU);
-  } else if (ep.act == SV_ACT_GELU_TANH) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = activate(v[j], SV_ACT_GELU_TANH);
-  }
+  activate_by(v, ep.act);
   if (ep.residual) {
-    const O* src = static_cast<const O*>(ep.residual) + row * ep.ld_res + col;
-    if (full) {
+    const O* src = static_cast<const O*>(ep.residual) + at_res;
+    if constexpr (W == 8) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src));
+      const O* e = reinterpret_cast<const O*>(&raw);
 #pragma unroll
-      for (int q = 0; q < 32 / E; ++q) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src) + q);
-        const O* e = reinterpret_cast<const O*>(&raw);
-#pragma unroll
-        for (int j = 0; j < E; ++j) v[q * E + j] += to_f32(e[j]);
-      }
+      for (int j = 0; j < 8; ++j) v[j] += to_f32(e[j]);
     } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col + j < n) v[j] += to_f32(src[j]);
+      v[0] += to_f32(*src);
     }
   }
   store(ep.out);
 }
 
-template <int BN, typename O>
+template <int BN, bool PAIR, typename O, bool F8>
 __global__ void __launch_bounds__(TC_THREADS, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a,
                    const __grid_constant__ CUtensorMap map_b, TcArgs a, Epilogue ep,
                    int32_t* status) {
-  using L = TcLayout<BN>;
+  using L = TcLayout<BN, PAIR>;
   constexpr int S = L::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -172,6 +247,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* drained = acc_empty + 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0u;
+  const int32_t unit = PAIR ? blockIdx.x >> 1 : blockIdx.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -180,7 +257,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], EPI_THREADS);
+      mbar_init(&acc_empty[b], (PAIR ? 2 : 1) * EPI_WARPS);
     }
     mbar_init(drained, 1);
     *s_abort = 0;
@@ -188,12 +265,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     prefetch_tmap(&map_a);
     prefetch_tmap(&map_b);
   }
-  if (warp == 1) {
-    tmem_alloc(s_tmem, 2 * BN);
-    tmem_relinquish();
-  }
+  if (warp == 1) alloc_tmem<PAIR>(s_tmem, 2 * BN);
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the other CTA's barriers are ready too
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
   bool ok = true;
@@ -201,32 +276,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if (warp == 0) {
     if (lane == 0) {
       int it = 0;
-      const int per = a.e4m3 ? 128 : 64;  // elements of a k step
-      for (int32_t t = blockIdx.x; t < a.total && ok; t += gridDim.x) {
-        const Tile w = tile_at<BN>(a, t);
+      constexpr int per = F8 ? 128 : 64;  // elements of a k step
+      for (int32_t t = unit; t < a.total && ok; t += a.units) {
+        const Tile w = tile_at<BN, PAIR>(a, t);
+        const int32_t m0 = w.m0 + (int32_t)rank * TM, n0 = w.n0 + (int32_t)rank * L::B_ROWS;
         for (int k = w.k0; k < w.k1; ++k, ++it) {
           const int slot = it % S;
           if (!mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, s_abort)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full[slot], L::A_STAGE + L::B_STAGE);
+          if (rank == 0)
+            mbar_arrive_expect_tx(&full[slot], (PAIR ? 2 : 1) * (L::A_STAGE + L::B_STAGE));
           const uint32_t sa = smem_u32(smem + L::A_OFF + slot * L::A_STAGE);
           const uint32_t sb = smem_u32(smem + L::B_OFF + slot * L::B_STAGE);
           const int kk = k * per;
-          if (a.a_mn) {
+          const uint32_t bar = PAIR ? in_first(smem_u32(&full[slot])) : 0u;
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+            if constexpr (PAIR) tma_load_pair(dst, map, bar, x, y);
+            else tma_load_2d(dst, map, &full[slot], x, y);
+          };
+          if (!F8 && a.a_mn) {
 #pragma unroll
-            for (int r = 0; r < TM / 64; ++r)
-              tma_load_2d(sa + r * MN_STRIDE, &map_a, &full[slot], w.m0 + 64 * r, kk);
+            for (int r = 0; r < TM / 64; ++r) load(sa + r * MN_STRIDE, &map_a, m0 + 64 * r, kk);
           } else {
-            tma_load_2d(sa, &map_a, &full[slot], kk, w.m0);
+            load(sa, &map_a, kk, m0);
           }
-          if (a.b_mn) {
+          if (!F8 && a.b_mn) {
 #pragma unroll
-            for (int r = 0; r < BN / 64; ++r)
-              tma_load_2d(sb + r * MN_STRIDE, &map_b, &full[slot], w.n0 + 64 * r, kk);
+            for (int r = 0; r < L::B_ROWS / 64; ++r)
+              load(sb + r * MN_STRIDE, &map_b, n0 + 64 * r, kk);
           } else {
-            tma_load_2d(sb, &map_b, &full[slot], kk, w.n0);
+            load(sb, &map_b, kk, n0);
           }
         }
       }
@@ -234,16 +315,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         report(status, SV_DEVICE_WAIT_TIMEOUT);
         // the copies in flight write this CTA's shared memory: let them land
         const uint64_t t0 = global_timer_ns();
-        for (int j = max(0, it - S); j < it; ++j)
-          while (!mbar_try_wait(&full[j % S], (j / S) & 1) && global_timer_ns() - t0 < 1000000000ull) {
-          }
+        while (global_timer_ns() - t0 < 10000000ull) {
+        }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       int it = 0, local = 0;
-      for (int32_t t = blockIdx.x; t < a.total && ok; t += gridDim.x, ++local) {
-        const Tile w = tile_at<BN>(a, t);
+      for (int32_t t = unit; t < a.total && ok; t += a.units, ++local) {
+        const Tile w = tile_at<BN, PAIR>(a, t);
         const int ab = local & 1;
         if (!mbar_wait_bounded(&acc_empty[ab], ((local >> 1) & 1) ^ 1, s_abort)) {
           ok = false;
@@ -262,23 +342,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           const uint32_t sb = smem_u32(smem + L::B_OFF + slot * L::B_STAGE);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {  // 32 bytes of k: one instruction
-            const uint64_t da = a.a_mn ? smem_desc_mn_sw128(sa + j * 2 * ATOM, MN_STRIDE, ATOM)
-                                       : smem_desc_sw128(sa + j * 32);
-            const uint64_t db = a.b_mn ? smem_desc_mn_sw128(sb + j * 2 * ATOM, MN_STRIDE, ATOM)
-                                       : smem_desc_sw128(sb + j * 32);
-            const uint32_t more = (k > w.k0 || j > 0) ? 1u : 0u;
-            if (a.e4m3)
-              tc_mma_f8(d, da, db, a.idesc, more);
-            else
-              tc_mma_f16(d, da, db, a.idesc, more);
+            const uint64_t da = !F8 && a.a_mn
+                                    ? smem_desc_mn_sw128(sa + j * 2 * ATOM, MN_STRIDE, ATOM)
+                                    : smem_desc_sw128(sa + j * 32);
+            const uint64_t db = !F8 && a.b_mn
+                                    ? smem_desc_mn_sw128(sb + j * 2 * ATOM, MN_STRIDE, ATOM)
+                                    : smem_desc_sw128(sb + j * 32);
+            issue_mma<PAIR, F8>(d, da, db, a.idesc, (k > w.k0 || j > 0) ? 1u : 0u);
           }
-          tc_commit(&empty[slot]);
+          commit<PAIR>(&empty[slot]);
         }
-        if (ok) tc_commit(&acc_full[ab]);
+        if (ok) commit<PAIR>(&acc_full[ab]);
       }
       if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
-      // the products in flight read this CTA's shared memory: let them finish
-      tc_commit(drained);
+      // the products in flight read both CTAs' shared memory: let them finish
+      commit<PAIR>(drained);
       const uint64_t t0 = global_timer_ns();
       while (!mbar_try_wait(drained, 0) && global_timer_ns() - t0 < 1000000000ull) {
       }
@@ -287,10 +365,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const int q = warp & 3;            // TMEM lanes 32 q .. 32 q + 31
     const int half = (warp - 2) >> 2;  // columns half * BN / 2 ..
     const int e = threadIdx.x - 64;
+    float* chunk = reinterpret_cast<float*>(smem + L::CHUNK_OFF) + (warp - 2) * 32 * CHUNK_LD;
     const bool scaled = ep.row_scale != nullptr || ep.col_scale != nullptr;
     int local = 0;
-    for (int32_t t = blockIdx.x; t < a.total; t += gridDim.x, ++local) {
-      const Tile w = tile_at<BN>(a, t);
+    for (int32_t t = unit; t < a.total; t += a.units, ++local) {
+      const Tile w = tile_at<BN, PAIR>(a, t);
       const int ab = local & 1;
       float* s_bias = s_cols + ab * 2 * BN;
       float* s_scale = s_bias + BN;
@@ -308,48 +387,90 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         break;
       }
       tc_fence_after();
-      const int64_t row = w.m0 + q * 32 + lane;
-      const bool live = row < a.m;
-      const float row_scale = live && ep.row_scale ? __ldg(ep.row_scale + row) : 1.f;
+      const int64_t row0 = (int64_t)w.m0 + rank * TM + q * 32;  // the warp's first row
+      const int rows = (int)max((int64_t)0, min((int64_t)32, a.m - row0));
       const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * BN);
 #pragma unroll 1
       for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
         uint32_t raw[32];
-        __syncwarp();  // lanes past the last row skip the rest of a round
         tmem_ld_32x32b_x32(t_row + c, raw);
         tc_wait_ld();
-        const int64_t col = w.n0 + c;
-        if (!live || col >= a.n) continue;
-        float v[32];
+        const int64_t col = (int64_t)w.n0 + c;
+        if (rows == 0 || col >= a.n) continue;  // the same in all lanes
+        __syncwarp();                           // the previous chunk has been read
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<uint4*>(chunk + lane * CHUNK_LD + j) =
+              make_uint4(raw[j], raw[j + 1], raw[j + 2], raw[j + 3]);
+        __syncwarp();
+        const int cols = (int)min((int64_t)32, a.n - col);
         if (ep.partial) {
-          float* dst = ep.partial + ((int64_t)w.split * a.m + row) * a.n + col;
-          if (a.n % 4 == 0 && col + 32 <= a.n) {
+          float* dst = ep.partial + ((int64_t)w.split * a.m + row0) * a.n + col;
+          if (a.n % 4 == 0 && cols == 32) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<float4*>(dst + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (col + j < a.n) dst[j] = v[j];
+            for (int i = 0; i < 8; ++i) {
+              const int r = i * 4 + (lane >> 3), j = (lane & 7) * 4;
+              if (r < rows)
+                *reinterpret_cast<float4*>(dst + r * a.n + j) =
+                    *reinterpret_cast<const float4*>(chunk + r * CHUNK_LD + j);
+            }
+          } else if (lane < cols) {
+            for (int r = 0; r < rows; ++r) dst[r * a.n + lane] = chunk[r * CHUNK_LD + lane];
           }
-        } else {
-          finish_chunk<O>(ep, s_bias + c, s_scale + c, row, col, a.n, row_scale, a.wide_io, scaled,
-                          v);
+        } else if (a.wide_io && cols == 32) {
+          const int j = (lane & 3) * 8;  // four lanes a row, eight rows at a time
+          float bias[8], scale[8];
+#pragma unroll
+          for (int x = 0; x < 8; x += 4) {
+            if (ep.bias)
+              *reinterpret_cast<float4*>(bias + x) =
+                  *reinterpret_cast<const float4*>(s_bias + c + j + x);
+            if (scaled)
+              *reinterpret_cast<float4*>(scale + x) =
+                  *reinterpret_cast<const float4*>(s_scale + c + j + x);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2);
+            if (r < rows) {
+              const int64_t row = row0 + r;
+              float v[8];
+              *reinterpret_cast<float4*>(v) =
+                  *reinterpret_cast<const float4*>(chunk + r * CHUNK_LD + j);
+              *reinterpret_cast<float4*>(v + 4) =
+                  *reinterpret_cast<const float4*>(chunk + r * CHUNK_LD + j + 4);
+              finish<O, 8>(ep, v, bias, scale, ep.row_scale ? __ldg(ep.row_scale + row) : 1.f,
+                           scaled, row * a.n + col + j, row * ep.ld_res + col + j);
+            }
+          }
+        } else if (lane < cols) {
+          const float bias[1] = {ep.bias ? s_bias[c + lane] : 0.f};
+          const float scale[1] = {scaled ? s_scale[c + lane] : 1.f};
+#pragma unroll 4
+          for (int r = 0; r < rows; ++r) {
+            const int64_t row = row0 + r;
+            float v[1] = {chunk[r * CHUNK_LD + lane]};
+            finish<O, 1>(ep, v, bias, scale, ep.row_scale ? __ldg(ep.row_scale + row) : 1.f, scaled,
+                         row * a.n + col + lane, row * ep.ld_res + col + lane);
+          }
         }
       }
       tc_fence_before();
-      mbar_arrive(&acc_empty[ab]);
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) arrive_at(in_first(smem_u32(&acc_empty[ab])));
+        else arrive_at(smem_u32(&acc_empty[ab]));
+      }
     }
     if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
   }
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // nothing of the pair still reads or signals this CTA
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * BN);
+    free_tmem<PAIR>(tmem, 2 * BN);
   }
 }
 
@@ -392,59 +513,85 @@ int operand_map(const Operand& o, int64_t outer, int64_t k, int dtype, int box_r
   return SV_OK;
 }
 
-template <int BN, typename O>
+template <int BN, bool PAIR, typename O, bool F8>
 int launch_tc(const Gemm& g, int32_t* status, cudaStream_t s) {
-  using L = TcLayout<BN>;
+  using L = TcLayout<BN, PAIR>;
+  auto kernel = gemm_tc_kernel<BN, PAIR, O, F8>;
   int dev = 0;
   SV_CUDA_TRY(cudaGetDevice(&dev));
-  static bool attr_done[256] = {};
-  if (dev >= 256 || !attr_done[dev]) {
-    SV_CUDA_TRY(cudaFuncSetAttribute(gemm_tc_kernel<BN, O>,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
-    if (dev < 256) attr_done[dev] = true;
+  cudaLaunchConfig_t config{};
+  config.blockDim = dim3(TC_THREADS);
+  config.dynamicSmemBytes = L::SMEM;
+  config.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = PAIR ? 2 : 1;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  // Units that run at the same time: one more would run after all the others.
+  static int units_of[256] = {};
+  int units = dev < 256 ? units_of[dev] : 0;
+  if (units == 0) {
+    SV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     L::SMEM));
+    units = num_sms();
+    if constexpr (PAIR) {
+      config.gridDim = dim3(num_sms() / 2 * 2);
+      SV_CUDA_TRY(cudaOccupancyMaxActiveClusters(&units, kernel, &config));
+      if (units < 1) SV_FAIL(SV_ERR_CUDA, "linear: no CTA pair fits this device");
+      units = std::min(units, num_sms() / 2);
+    }
+    if (dev < 256) units_of[dev] = units;
   }
   CUtensorMap map_a, map_b;
   int rc = operand_map(g.a, g.m, g.k, g.dtype, TM, &map_a);
-  if (rc == SV_OK) rc = operand_map(g.b, g.n, g.k, g.dtype, BN, &map_b);
+  if (rc == SV_OK) rc = operand_map(g.b, g.n, g.k, g.dtype, L::B_ROWS, &map_b);
   if (rc != SV_OK) return rc;
+  constexpr int ROWS = PAIR ? 2 * TM : TM;
   TcArgs a{};
   a.m = g.m;
   a.n = g.n;
   a.tiles_n = (int32_t)((g.n + BN - 1) / BN);
-  const int64_t tiles = (g.m + TM - 1) / TM * a.tiles_n;
+  const int64_t tiles = (g.m + ROWS - 1) / ROWS * a.tiles_n;
   if (tiles * g.splits > INT32_MAX / 2) SV_FAIL(SV_ERR_UNSUPPORTED, "linear: too many tiles");
   a.tiles = (int32_t)tiles;
   a.total = (int32_t)(tiles * g.splits);
+  a.units = std::min(a.total, units);
   const int per = 128 / elem_size(g.dtype);
   a.steps = (int32_t)((g.k + per - 1) / per);
   a.part = (a.steps + g.splits - 1) / g.splits;
-  a.e4m3 = g.dtype == SV_FLOAT8_E4M3;
   a.a_mn = g.a.mn;
   a.b_mn = g.b.mn;
-  a.idesc = a.e4m3 ? idesc_f16(false, TM, BN)  // the same fields; format 0 is e4m3
-                   : idesc_f16_major(g.dtype == SV_BFLOAT16, TM, BN, g.a.mn, g.b.mn);
+  a.idesc = F8 ? idesc_f16(false, ROWS, BN)  // the same fields; format 0 is e4m3
+               : idesc_f16_major(g.dtype == SV_BFLOAT16, ROWS, BN, g.a.mn, g.b.mn);
   const Epilogue& ep = g.ep;
-  const int e = 16 / elem_size(ep.out_dtype);
-  a.wide_io = g.n % e == 0 && aligned16(ep.out) && (!ep.preact || aligned16(ep.preact)) &&
-              (!ep.residual || (aligned16(ep.residual) && ep.ld_res % e == 0));
-  const int grid = (int)std::min<int64_t>(a.total, num_sms());
-  gemm_tc_kernel<BN, O><<<grid, TC_THREADS, L::SMEM, s>>>(map_a, map_b, a, ep, status);
-  SV_LAUNCH_CHECK();
+  a.wide_io = g.n % 8 == 0 && aligned16(ep.out) && (!ep.preact || aligned16(ep.preact)) &&
+              (!ep.residual || (aligned16(ep.residual) && ep.ld_res % 8 == 0));
+  config.gridDim = dim3((unsigned)(a.units * (PAIR ? 2 : 1)));
+  SV_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, map_a, map_b, a, ep, status));
   return SV_OK;
 }
 
-template <typename O>
-int launch_typed(const Gemm& g, int bn, int32_t* status, cudaStream_t s) {
-  if (bn == 256) return launch_tc<256, O>(g, status, s);
-  if (bn == 128) return launch_tc<128, O>(g, status, s);
-  return launch_tc<64, O>(g, status, s);
+template <typename O, bool F8>
+int launch_typed(const Gemm& g, TcTile tile, int32_t* status, cudaStream_t s) {
+  switch (tile) {
+    case TcTile::kPair256: return launch_tc<256, true, O, F8>(g, status, s);
+    case TcTile::kPair128: return launch_tc<128, true, O, F8>(g, status, s);
+    case TcTile::kOne128: return launch_tc<128, false, O, F8>(g, status, s);
+    default: return launch_tc<64, false, O, F8>(g, status, s);
+  }
 }
 
 }  // namespace
 
-int gemm_tc(const Gemm& g, int bn, int32_t* status, cudaStream_t s) {
-  return g.ep.out_dtype == SV_FLOAT16 ? launch_typed<__half>(g, bn, status, s)
-                                      : launch_typed<__nv_bfloat16>(g, bn, status, s);
+int gemm_tc(const Gemm& g, TcTile tile, int32_t* status, cudaStream_t s) {
+  const bool half = g.ep.out_dtype == SV_FLOAT16;
+  if (g.dtype == SV_FLOAT8_E4M3)
+    return half ? launch_typed<__half, true>(g, tile, status, s)
+                : launch_typed<__nv_bfloat16, true>(g, tile, status, s);
+  return half ? launch_typed<__half, false>(g, tile, status, s)
+              : launch_typed<__nv_bfloat16, false>(g, tile, status, s);
 }
 
 }  // namespace sv

@@ -168,6 +168,9 @@ __global__ void __launch_bounds__(kBlock<TPR>)
     const float scale = top == 0.f ? 1.f : top / E4M3_MAX;
     if (!live) return;
     if (sub == 0) a.scale[row] = scale;
+    // a product with the reciprocal: within 2^-23 of the quotient, a division an element cost 22 us
+    // of 88 at 40,662 x 1024
+    const float inv = 1.0f / scale;
     uint8_t* q = static_cast<uint8_t*>(out) + row * C;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -178,9 +181,9 @@ __global__ void __launch_bounds__(kBlock<TPR>)
 #pragma unroll
           for (int k = 0; k < V; k += 4) {
             const uint32_t lo = __nv_cvt_float2_to_fp8x2(
-                make_float2(v[j][k] / scale, v[j][k + 1] / scale), __NV_SATFINITE, __NV_E4M3);
+                make_float2(v[j][k] * inv, v[j][k + 1] * inv), __NV_SATFINITE, __NV_E4M3);
             const uint32_t hi = __nv_cvt_float2_to_fp8x2(
-                make_float2(v[j][k + 2] / scale, v[j][k + 3] / scale), __NV_SATFINITE, __NV_E4M3);
+                make_float2(v[j][k + 2] * inv, v[j][k + 3] * inv), __NV_SATFINITE, __NV_E4M3);
             packed[k / 4] = lo | hi << 16;
           }
           if constexpr (V == 8)
@@ -190,24 +193,26 @@ __global__ void __launch_bounds__(kBlock<TPR>)
         } else {
 #pragma unroll
           for (int k = 0; k < V; ++k)
-            q[c + k] = __nv_cvt_float_to_fp8(v[j][k] / scale, __NV_SATFINITE, __NV_E4M3);
+            q[c + k] = __nv_cvt_float_to_fp8(v[j][k] * inv, __NV_SATFINITE, __NV_E4M3);
         }
       }
     }
   }
 }
 
-// Gradients: each group of TPR threads takes rows group, group + groups, ... and keeps its
-// channels' share of dw in registers; a block adds its groups in order through shared memory and
-// writes one row of `partial` ([gridDim.x, C]), which column_sum_kernel adds in a fixed order.
-template <typename T, int V, int TPR, int J>
+// Gradients: each group of TPR threads takes R rows at a time (so that R rows' loads are in flight)
+// and keeps its channels' share of dw in registers; a block adds its groups in order through shared
+// memory and writes one row of `partial` ([gridDim.x, C]), which column_sum_kernel adds in a fixed
+// order.
+template <typename T, int V, int TPR, int J, int R>
 __global__ void __launch_bounds__(kBlock<TPR>)
     rms_backward_kernel(const T* __restrict__ h, const T* __restrict__ dy,
                         const T* __restrict__ dh, RmsArgs a, T* __restrict__ dx,
                         float* __restrict__ partial) {
-  constexpr int ROWS = kBlock<TPR> / TPR;
+  constexpr int GROUPS = kBlock<TPR> / TPR;
+  constexpr int W = TPR > 32 ? TPR / 32 : 1;
   extern __shared__ float s_dw[];  // [C] when dw is wanted
-  __shared__ float part[TPR > 32 ? TPR / 32 : 1];
+  __shared__ float part[2][R][W];
   const int sub = threadIdx.x % TPR;
   const int group = threadIdx.x / TPR;
   const int C = a.channels;
@@ -220,56 +225,85 @@ __global__ void __launch_bounds__(kBlock<TPR>)
     if (c < C) load_weight<V>(a.weight, c, w[j]);
   }
   const float inv_c = 1.0f / (float)C;
+  int flip = 0;
   // the block's groups take consecutive rows, so every group makes the same number of rounds
-  for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.n; base += (int64_t)gridDim.x * ROWS) {
-    const int64_t row = base + group;
-    const bool live = row < a.n;
-    float hv[J][V], g[J][V];
-    float dot = 0.f;
-    const float rstd = live ? __ldg(a.rstd + row) : 0.f;
+  for (int64_t base = (int64_t)blockIdx.x * GROUPS * R; base < a.n;
+       base += (int64_t)gridDim.x * GROUPS * R, flip ^= 1) {
+    const int64_t row0 = base + group * R;
+    float hv[R][J][V], g[R][J][V];
+    float dot[R], rstd[R];
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int c = (sub + TPR * j) * V;
-      if (live && c < C) {
-        load_row<T, V>(h + row * a.x_stride + c, hv[j]);
-        load_row<T, V>(dy + row * C + c, g[j]);
+    for (int r = 0; r < R; ++r) {
+      const bool live = row0 + r < a.n;
+      rstd[r] = live ? __ldg(a.rstd + row0 + r) : 0.f;
+      dot[r] = 0.f;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          dw[j][k] = fmaf(g[j][k], hv[j][k] * rstd, dw[j][k]);
-          g[j][k] *= w[j][k];
-          dot = fmaf(g[j][k], hv[j][k], dot);
+      for (int j = 0; j < J; ++j) {
+        const int c = (sub + TPR * j) * V;
+        if (live && c < C) {
+          load_row<T, V>(h + (row0 + r) * a.x_stride + c, hv[r][j]);
+          load_row<T, V>(dy + (row0 + r) * C + c, g[r][j]);
         }
       }
     }
-    dot = row_reduce<Sum, TPR>(dot, part);
-    const float pull = dot * rstd * rstd * inv_c;
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int c = (sub + TPR * j) * V;
-      if (live && c < C) {
-        float d[V];
+    for (int r = 0; r < R; ++r) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) d[k] = rstd * (g[j][k] - hv[j][k] * pull);
-        if (dh != nullptr) {
-          float e[V];
-          load_row<T, V>(dh + row * C + c, e);
+      for (int j = 0; j < J; ++j) {
+        if (row0 + r < a.n && (sub + TPR * j) * V < C) {
 #pragma unroll
-          for (int k = 0; k < V; ++k) d[k] += e[k];
+          for (int k = 0; k < V; ++k) {
+            dw[j][k] = fmaf(g[r][j][k], hv[r][j][k] * rstd[r], dw[j][k]);
+            g[r][j][k] *= w[j][k];
+            dot[r] = fmaf(g[r][j][k], hv[r][j][k], dot[r]);
+          }
         }
-        store_row<T, V>(dx + row * C + c, d);
+      }
+#pragma unroll
+      for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
+        dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], o);
+      if (TPR > 32 && (threadIdx.x & 31) == 0) part[flip][r][threadIdx.x >> 5] = dot[r];
+    }
+    if constexpr (TPR > 32) {
+      __syncthreads();  // two copies: the next round's writes do not meet this round's reads
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        dot[r] = part[flip][r][0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) dot[r] += part[flip][r][i];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float pull = dot[r] * rstd[r] * rstd[r] * inv_c;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int c = (sub + TPR * j) * V;
+        if (row0 + r < a.n && c < C) {
+          float d[V];
+#pragma unroll
+          for (int k = 0; k < V; ++k) d[k] = rstd[r] * (g[r][j][k] - hv[r][j][k] * pull);
+          if (dh != nullptr) {
+            float e[V];
+            load_row<T, V>(dh + (row0 + r) * C + c, e);
+#pragma unroll
+            for (int k = 0; k < V; ++k) d[k] += e[k];
+          }
+          store_row<T, V>(dx + (row0 + r) * C + c, d);
+        }
       }
     }
   }
   if (partial == nullptr) return;
-  for (int r = 0; r < ROWS; ++r) {
-    if (group == r) {
+  for (int q = 0; q < GROUPS; ++q) {
+    if (group == q) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int c = (sub + TPR * j) * V;
         if (c < C) {
 #pragma unroll
           for (int k = 0; k < V; ++k)
-            s_dw[c + k] = r == 0 ? dw[j][k] : s_dw[c + k] + dw[j][k];
+            s_dw[c + k] = q == 0 ? dw[j][k] : s_dw[c + k] + dw[j][k];
         }
       }
     }
@@ -299,23 +333,47 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict
   }
 }
 
-template <typename F>
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// Threads of a row and accesses of a thread for rows of nv accesses of V elements; widths that V
+// elements an access never reach are not compiled.
+template <int V, typename F>
 int by_width(int nv, F&& f) {
-  if (nv <= 8) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
-  if (nv <= 32) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
-  if (nv <= 64) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 2>{});
-  if (nv <= 128) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
-  if (nv <= 512) return f(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
-  if (nv <= 2048) return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
-  return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 16>{});
+  if (nv <= 8) return f(Int<8>{}, Int<1>{});
+  if (nv <= 32) return f(Int<32>{}, Int<1>{});
+  if (nv <= 64) return f(Int<32>{}, Int<2>{});
+  if (nv <= 128) return f(Int<32>{}, Int<4>{});
+  if (nv <= 512) return f(Int<128>{}, Int<4>{});
+  if constexpr (RMS_MAX_CHANNELS / V > 2048) {
+    if (nv > 2048) return f(Int<512>{}, Int<16>{});
+  }
+  return f(Int<512>{}, Int<4>{});
 }
 
-constexpr int BACKWARD_BLOCKS = 296;  // two per SM; also the rows of the dw partials
+// The backward pass holds more of a row (h, dy, w, dw), so it spreads one over more threads.
+template <int V, typename F>
+int by_width_backward(int nv, F&& f) {
+  if (nv <= 8) return f(Int<8>{}, Int<1>{}, Int<2>{});
+  if (nv <= 32) return f(Int<32>{}, Int<1>{}, Int<4>{});
+  if (nv <= 64) return f(Int<32>{}, Int<2>{}, Int<2>{});
+  if (nv <= 128) return f(Int<128>{}, Int<1>{}, Int<4>{});
+  if (nv <= 256) return f(Int<128>{}, Int<2>{}, Int<2>{});
+  if constexpr (RMS_MAX_CHANNELS / V > 1024) {
+    if constexpr (RMS_MAX_CHANNELS / V > 2048) {
+      if (nv > 2048) return f(Int<512>{}, Int<16>{}, Int<1>{});
+    }
+    if (nv > 1024) return f(Int<512>{}, Int<4>{}, Int<1>{});
+  }
+  return f(Int<512>{}, Int<2>{}, Int<1>{});
+}
+
+constexpr int BACKWARD_BLOCKS = 888;  // at most six per SM; also the rows of the dw partials
 
 template <typename T, int V>
 int launch_rms(const void* x, const void* res, const RmsArgs& a, void* h_out, void* out, bool q8,
                cudaStream_t s) {
-  return by_width((a.channels + V - 1) / V, [&](auto tpr, auto j) -> int {
+  return by_width<V>((a.channels + V - 1) / V, [&](auto tpr, auto j) -> int {
     constexpr int TPR = decltype(tpr)::value, J = decltype(j)::value;
     constexpr int ROWS = kBlock<TPR> / TPR;
     const int64_t blocks = (a.n + ROWS - 1) / ROWS;
@@ -330,12 +388,12 @@ int launch_rms(const void* x, const void* res, const RmsArgs& a, void* h_out, vo
 template <typename T, int V>
 int launch_rms_backward(const void* h, const void* dy, const void* dh, const RmsArgs& a, void* dx,
                         float* partial, float* dw, cudaStream_t s) {
-  return by_width((a.channels + V - 1) / V, [&](auto tpr, auto j) -> int {
-    constexpr int TPR = decltype(tpr)::value, J = decltype(j)::value;
-    constexpr int ROWS = kBlock<TPR> / TPR;
+  return by_width_backward<V>((a.channels + V - 1) / V, [&](auto tpr, auto j, auto r) -> int {
+    constexpr int TPR = decltype(tpr)::value, J = decltype(j)::value, R = decltype(r)::value;
+    constexpr int ROWS = kBlock<TPR> / TPR * R;
     const int64_t want = (a.n + ROWS - 1) / ROWS;
     const int blocks = (int)(want < BACKWARD_BLOCKS ? want : BACKWARD_BLOCKS);
-    rms_backward_kernel<T, V, TPR, J>
+    rms_backward_kernel<T, V, TPR, J, R>
         <<<blocks, kBlock<TPR>, dw ? a.channels * sizeof(float) : 0, s>>>(
             static_cast<const T*>(h), static_cast<const T*>(dy), static_cast<const T*>(dh), a,
             static_cast<T*>(dx), dw ? partial : nullptr);
