@@ -51,8 +51,20 @@ int gemm_tc(const Gemm& g, TcTile tile, int32_t* status, cudaStream_t s);
 
 #ifdef __CUDACC__
 constexpr float SQRT_HALF = 0.70710678118654752f;
+constexpr float LOG2_E = 1.4426950408889634f;
 constexpr float GELU_TANH_2C = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float GELU_CUBE = 0.044715f;
+
+__device__ __forceinline__ float exp2_half(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_half(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // exp and the quotient are the fast forms: within a few fp32 ulp of the value over the whole
 // range (x / (1 + inf) is 0), which is the error the fp32 path's tolerance counts.
@@ -71,17 +83,23 @@ __device__ __forceinline__ float activate(float z, int act) {
 // Phi(z), the normal distribution's integral, by Abramowitz and Stegun's 7.1.26, off by at most
 // 7.5e-8: for the 16-bit types, whose rounding is far above that. `gauss`: exp(-z^2 / 2).
 __device__ __forceinline__ float normal_half(float z, float gauss) {
-  const float t = __fdividef(1.0f, fmaf(0.3275911f * SQRT_HALF, fabsf(z), 1.0f));
+  const float t = rcp_half(fmaf(0.3275911f * SQRT_HALF, fabsf(z), 1.0f));
   const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f),
                                    -0.284496736f), 0.254829592f);
   const float tail = 0.5f * p * gauss;
   return z < 0.0f ? tail : 1.0f - tail;
 }
 
-// The activation for results of 16 bits.
+// The activation for results of 16 bits: the approximate reciprocal and exponential are off by an
+// fp32 ulp or two, and the factors of the exponent are folded.
 __device__ __forceinline__ float activate_half(float z, int act) {
-  if (act == SV_ACT_GELU) return z * normal_half(z, __expf(-0.5f * z * z));
-  return activate(z, act);
+  if (act == SV_ACT_SILU) return z * rcp_half(1.0f + exp2_half(-LOG2_E * z));
+  if (act == SV_ACT_GELU) return z * normal_half(z, exp2_half(-0.5f * LOG2_E * z * z));
+  if (act == SV_ACT_GELU_TANH) {
+    constexpr float A = -GELU_TANH_2C * LOG2_E;
+    return z * rcp_half(1.0f + exp2_half(z * fmaf(A * GELU_CUBE, z * z, A)));
+  }
+  return z;
 }
 
 // The activation's derivative.
@@ -102,7 +120,7 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
 
 __device__ __forceinline__ float activate_slope_half(float z, int act) {
   if (act == SV_ACT_GELU) {
-    const float gauss = __expf(-0.5f * z * z);
+    const float gauss = exp2_half(-0.5f * LOG2_E * z * z);
     return normal_half(z, gauss) + z * 0.39894228040143268f * gauss;
   }
   return activate_slope(z, act);

@@ -173,56 +173,73 @@ __device__ __forceinline__ Tile tile_at(const TcArgs& a, int32_t t) {
   return o;
 }
 
-template <int ACT, int W>
-__device__ __forceinline__ void activate_all(float (&v)[W]) {
+template <int ACT, int R, int W>
+__device__ __forceinline__ void activate_all(float (&v)[R][W]) {
 #pragma unroll
-  for (int j = 0; j < W; ++j) v[j] = activate_half(v[j], ACT);
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[i][j] = activate_half(v[i][j], ACT);
 }
 
-template <int W>
-__device__ __forceinline__ void activate_by(float (&v)[W], int act) {
-  if (act == SV_ACT_SILU) activate_all<SV_ACT_SILU>(v);
-  else if (act == SV_ACT_GELU) activate_all<SV_ACT_GELU>(v);
-  else if (act == SV_ACT_GELU_TANH) activate_all<SV_ACT_GELU_TANH>(v);
-}
-
-// W consecutive columns of one row: scale, bias, activation, residual, stores.
-template <typename O, int W>
-__device__ __forceinline__ void finish(const Epilogue& ep, float (&v)[W], const float* bias,
-                                       const float* scale, float row_scale, bool scaled,
-                                       int64_t at, int64_t at_res) {
+// R rows of W consecutive columns: scale, bias, activation, residual, stores. Step by step over all
+// of them, so that the rows' loads are in flight together. `at`, `at_res`: the first row's offsets.
+template <typename O, int R, int W>
+__device__ __forceinline__ void finish(const Epilogue& ep, float (&v)[R][W], const float* bias,
+                                       const float* scale, bool scaled, int64_t row, int step,
+                                       int rows, int64_t n, int64_t col) {
+  O res[R][W];
+  if (ep.residual) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (i * step < rows) {
+        const O* src = static_cast<const O*>(ep.residual) + (row + i * step) * ep.ld_res + col;
+        if constexpr (W == 8)
+          *reinterpret_cast<uint4*>(res[i]) = __ldg(reinterpret_cast<const uint4*>(src));
+        else
+          res[i][0] = *src;
+      }
+    }
+  }
   if (scaled) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) v[j] *= row_scale * scale[j];
+    for (int i = 0; i < R; ++i) {
+      const float by = ep.row_scale && i * step < rows ? __ldg(ep.row_scale + row + i * step) : 1.f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[i][j] *= by * scale[j];
+    }
   }
   if (ep.bias) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) v[j] += bias[j];
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[i][j] += bias[j];
   }
   auto store = [&](void* base) {
-    O* dst = static_cast<O*>(base) + at;
-    if constexpr (W == 8) {
-      uint4 raw;
-      O* e = reinterpret_cast<O*>(&raw);
+    O* dst = static_cast<O*>(base) + row * n + col;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = from_f32<O>(v[j]);
-      *reinterpret_cast<uint4*>(dst) = raw;
-    } else {
-      *dst = from_f32<O>(v[0]);
+    for (int i = 0; i < R; ++i) {
+      if (i * step < rows) {
+        if constexpr (W == 8) {
+          uint4 raw;
+          O* e = reinterpret_cast<O*>(&raw);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = from_f32<O>(v[i][j]);
+          *reinterpret_cast<uint4*>(dst + i * step * n) = raw;
+        } else {
+          dst[i * step * n] = from_f32<O>(v[i][0]);
+        }
+      }
     }
   };
   if (ep.preact) store(ep.preact);
-  activate_by(v, ep.act);
+  if (ep.act == SV_ACT_SILU) activate_all<SV_ACT_SILU>(v);
+  else if (ep.act == SV_ACT_GELU) activate_all<SV_ACT_GELU>(v);
+  else if (ep.act == SV_ACT_GELU_TANH) activate_all<SV_ACT_GELU_TANH>(v);
   if (ep.residual) {
-    const O* src = static_cast<const O*>(ep.residual) + at_res;
-    if constexpr (W == 8) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src));
-      const O* e = reinterpret_cast<const O*>(&raw);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += to_f32(e[j]);
-    } else {
-      v[0] += to_f32(*src);
-    }
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[i][j] += to_f32(res[i][j]);
   }
   store(ep.out);
 }
@@ -429,29 +446,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
               *reinterpret_cast<float4*>(scale + x) =
                   *reinterpret_cast<const float4*>(s_scale + c + j + x);
           }
+          float v[4][8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2);
-            if (r < rows) {
-              const int64_t row = row0 + r;
-              float v[8];
-              *reinterpret_cast<float4*>(v) =
-                  *reinterpret_cast<const float4*>(chunk + r * CHUNK_LD + j);
-              *reinterpret_cast<float4*>(v + 4) =
-                  *reinterpret_cast<const float4*>(chunk + r * CHUNK_LD + j + 4);
-              finish<O, 8>(ep, v, bias, scale, ep.row_scale ? __ldg(ep.row_scale + row) : 1.f,
-                           scaled, row * a.n + col + j, row * ep.ld_res + col + j);
-            }
+            const float* src = chunk + (i * 8 + (lane >> 2)) * CHUNK_LD + j;
+            *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(src);
+            *reinterpret_cast<float4*>(v[i] + 4) = *reinterpret_cast<const float4*>(src + 4);
           }
+          finish<O, 4, 8>(ep, v, bias, scale, scaled, row0 + (lane >> 2), 8, rows - (lane >> 2),
+                          a.n, col + j);
         } else if (lane < cols) {
           const float bias[1] = {ep.bias ? s_bias[c + lane] : 0.f};
           const float scale[1] = {scaled ? s_scale[c + lane] : 1.f};
-#pragma unroll 4
-          for (int r = 0; r < rows; ++r) {
-            const int64_t row = row0 + r;
-            float v[1] = {chunk[r * CHUNK_LD + lane]};
-            finish<O, 1>(ep, v, bias, scale, ep.row_scale ? __ldg(ep.row_scale + row) : 1.f, scaled,
-                         row * a.n + col + lane, row * ep.ld_res + col + lane);
+#pragma unroll 1
+          for (int r = 0; r < rows; r += 8) {
+            float v[8][1];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i][0] = chunk[(r + i) * CHUNK_LD + lane];
+            finish<O, 8, 1>(ep, v, bias, scale, scaled, row0 + r, 1, rows - r, a.n, col + lane);
           }
         }
       }
