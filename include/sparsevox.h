@@ -376,7 +376,7 @@ SV_API int sv_rownorm(const void* x, int64_t n, int channels, int dtype, float e
 SV_API int sv_rms_norm(const void* x, int64_t x_stride, const void* residual,
                        int64_t residual_stride, int64_t n, int channels, int dtype, float eps,
                        const float* weight, void* h, float* rstd, void* out, int out_dtype,
-                       float* scale, sv_stream_t stream);
+                       float* scale, int32_t* status, sv_stream_t stream);
 
 /* Gradients of y with respect to h, plus `dh` (the gradient that reaches h itself; may be null):
  * dx [n, channels] (also the residual's gradient) and dw fp32 [channels] (null: not wanted). The
@@ -385,7 +385,7 @@ SV_API size_t sv_rms_norm_backward_workspace_bytes(int channels);
 SV_API int sv_rms_norm_backward(const void* h, int64_t h_stride, const void* dy, const void* dh,
                                 int64_t n, int channels, int dtype, const float* weight,
                                 const float* rstd, void* dx, float* dw, void* workspace,
-                                size_t workspace_bytes, sv_stream_t stream);
+                                size_t workspace_bytes, int32_t* status, sv_stream_t stream);
 
 /* ---- linear projection with bias, activation and residual ------------------------------ */
 

@@ -101,11 +101,11 @@ _SIGNATURES = {
     ),
     "sv_rms_norm": (
         _I32,
-        [_P, _I64, _P, _I64, _I64, _I32, _I32, ctypes.c_float, _P, _P, _P, _P, _I32, _P, _P],
+        [_P, _I64, _P, _I64, _I64, _I32, _I32, ctypes.c_float, _P, _P, _P, _P, _I32, _P, _P, _P],
     ),
     "sv_rms_norm_backward_workspace_bytes": (_SZ, [_I32]),
     "sv_rms_norm_backward": (
-        _I32, [_P, _I64, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _SZ, _P]
+        _I32, [_P, _I64, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _SZ, _P, _P]
     ),
     "sv_linear_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64, _I32, _I32]),
     "sv_linear_forward": (

@@ -114,7 +114,8 @@ def _rms_forward(x, residual, weight, eps, quantize, keep_rstd):
             x.data_ptr(), max(x.stride(0), c), N.ptr(residual),
             max(residual.stride(0), c) if residual is not None else 0, n, c, code, eps,
             N.ptr(weight), N.ptr(h), N.ptr(rstd), out.data_ptr(),
-            N.SV_FLOAT8_E4M3 if quantize else code, N.ptr(scale), N.stream(dev))
+            N.SV_FLOAT8_E4M3 if quantize else code, N.ptr(scale), N.status_word(dev).data_ptr(),
+            N.stream(dev))
     N.check(rc, "rms_norm")
     return out, scale, h, rstd
 
@@ -152,7 +153,7 @@ class _RmsNorm(torch.autograd.Function):
             rc = lib.sv_rms_norm_backward(
                 h.data_ptr(), max(h.stride(0), c), dy.data_ptr(), N.ptr(dh), n, c,
                 N.DTYPE_CODE[h.dtype], N.ptr(w32), rstd.data_ptr(), dx.data_ptr(), N.ptr(dw),
-                N.ptr(ws), nbytes, N.stream(dev))
+                N.ptr(ws), nbytes, N.status_word(dev).data_ptr(), N.stream(dev))
         N.check(rc, "rms_norm (backward)")
         if dw is not None:
             dw = dw.to(ctx.weight_dtype)

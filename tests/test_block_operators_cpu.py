@@ -151,22 +151,22 @@ def test_c_entry_points_check_before_any_launch():
     lib = N.load()
     p = 256  # an aligned address that nothing reads: every call below ends before a launch
     assert lib.sv_rms_norm(None, 0, None, 0, 0, 8, 2, 1e-6, None, None, None, None, 2, None,
-                           None) == N.SV_OK
+                           None, None) == N.SV_OK
     assert lib.sv_rms_norm(p, 8, None, 0, 4, 8, 7, 1e-6, None, None, None, p, 2, None,
-                           None) == N.SV_ERR_BAD_DTYPE
+                           None, None) == N.SV_ERR_BAD_DTYPE
     assert lib.sv_rms_norm(p, 8, None, 0, 4, 8, 2, 1e-6, None, None, None, p, 0, None,
-                           None) == N.SV_ERR_BAD_DTYPE
+                           None, None) == N.SV_ERR_BAD_DTYPE
     assert lib.sv_rms_norm(p, 8, None, 0, 4, 8, 2, 1e-6, None, None, None, p, 3, None,
-                           None) == N.SV_ERR_INVALID_ARGUMENT  # e4m3 without a scale
+                           None, None) == N.SV_ERR_INVALID_ARGUMENT  # e4m3 without a scale
     assert lib.sv_rms_norm(p, 7, None, 0, 4, 8, 2, 1e-6, None, None, None, p, 2, None,
-                           None) == N.SV_ERR_INVALID_ARGUMENT
+                           None, None) == N.SV_ERR_INVALID_ARGUMENT
     assert lib.sv_rms_norm(p, 9000, None, 0, 4, 8193, 2, 1e-6, None, None, None, p, 2, None,
-                           None) == N.SV_ERR_UNSUPPORTED
+                           None, None) == N.SV_ERR_UNSUPPORTED
     assert lib.sv_rms_norm(p, 8, None, 0, 4, 8, 2, -1.0, None, None, None, p, 2, None,
-                           None) == N.SV_ERR_INVALID_ARGUMENT
+                           None, None) == N.SV_ERR_INVALID_ARGUMENT
     assert lib.sv_rms_norm_backward_workspace_bytes(1024) > 0
     assert lib.sv_rms_norm_backward(p, 8, p, None, 4, 8, 2, None, p, p, p, None, 0,
-                                    None) == N.SV_ERR_WORKSPACE
+                                    None, None) == N.SV_ERR_WORKSPACE
 
     def forward(m=20, k=64, n=64, dtype=2, out=2, act=0, ldx=64, ldw=64, x=p, ws=None, nbytes=0):
         return lib.sv_linear_forward(x, ldx, p, ldw, None, None, 0, None, None, m, k, n, dtype, out,

@@ -113,6 +113,54 @@ def test_gradients(c, dtype):
             assert (err <= (n * U + ROW) * terms.abs().sum(0) + 1e-30).all()
 
 
+@pytest.mark.parametrize("c", [264, 512, 516, 768, 1000, 1024])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_many_rows(c, dtype):
+    """Enough rows for the warps' pipelines, the last round not full, rows with a stride."""
+    n = 4 * 16 * torch.cuda.get_device_properties(DEV).multi_processor_count + 77
+    x, r, w = _inputs(n, c, dtype, c, True)
+    wide = torch.zeros((n, c + 8), dtype=dtype, device=DEV)
+    wide[:, :c] = x
+    x = wide[:, :c]
+    rh, rstd, u, ry = _reference(x, r, w)
+    y, h = rms_norm(x, w, residual=r)
+    assert torch.equal(h.to(F64), rh)
+    assert ((y.to(F64) - ry).abs() <= (_half(dtype) + ROW) * ry.abs()
+            + torch.finfo(dtype).tiny).all()
+    (q, s), h2 = rms_norm(x, w, residual=r, quantize=True)
+    top = ry.abs().amax(-1)
+    assert torch.equal(h2, h) and ((s.to(F64) - top / 448).abs() <= (ROW + U) * top / 448).all()
+    back = q.to(F64) * s.to(F64)[:, None]
+    assert ((back - ry).abs() <= (2.0**-4 + 2 * ROW) * ry.abs()
+            + (2.0**-10 + ROW) * (top / 448)[:, None]).all()
+    alone = rms_norm(x, w)
+    ra = _reference(x, None, w)[3]
+    assert ((alone.to(F64) - ra).abs() <= (_half(dtype) + ROW) * ra.abs()
+            + torch.finfo(dtype).tiny).all()
+    g = torch.Generator(device=DEV).manual_seed(c)
+    dy, dh = (torch.randn((n, c), device=DEV, generator=g).to(dtype) for _ in range(2))
+    for residual in (True, False):
+        leaves = [t.requires_grad_(True) for t in ((x.detach(), r, w) if residual
+                                                   else (x.detach(), w))]
+        out = rms_norm(leaves[0], w, residual=r if residual else None)
+        grads = torch.autograd.grad(out, leaves, (dy, dh) if residual else dy)
+        with torch.no_grad():
+            _, rstd, u, _ = _reference(x, r if residual else None, w)
+            gw = dy.to(F64) * w.to(F64)
+            gu = gw * u
+            want = rstd * (gw - u * gu.mean(-1, keepdim=True))
+            mag = rstd * (gw.abs() + u.abs() * gu.abs().mean(-1, keepdim=True))
+            if residual:
+                want, mag = want + dh.to(F64), mag + dh.to(F64).abs()
+            err = (grads[0].to(F64) - want).abs()
+            assert (err <= _half(dtype) * want.abs() + 4 * ROW * mag
+                    + torch.finfo(dtype).tiny).all()
+            terms = dy.to(F64) * u
+            err = (grads[-1].to(F64) - terms.sum(0)).abs()
+            assert (err <= (n * U + ROW) * terms.abs().sum(0)).all()
+    N.check_device_status(DEV)
+
+
 def test_gradient_against_differences():
     x, r, w = _inputs(5, 24, torch.float32, 9)
     x, r, w = (t.requires_grad_(True) for t in (x, r, w))
