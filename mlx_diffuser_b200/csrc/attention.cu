@@ -191,6 +191,13 @@ int check(int64_t n, int heads, int dim, int dtype, int nb, int reach, const cha
   return SV_OK;
 }
 
+int check_strides(const int64_t* strides, const char* what) {
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] < 0 || strides[i] > (1 << 30))
+      SV_FAIL(SV_ERR_UNSUPPORTED, std::string(what) + ": strides must be between 0 and 2^30");
+  return SV_OK;
+}
+
 // Workspace of the backward pass: fixed-point table, norms, delta.
 struct Layout {
   size_t table, norms, delta, total;
@@ -238,6 +245,8 @@ extern "C" int sv_window_attention(const void* q, const void* k, const void* v,
   if (n == 0 || heads == 0 || dim == 0) return SV_OK;
   if (!q || !k || !v || !strides || !plan || !table || !lut || !out || !aligned16(plan))
     SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_window_attention: null pointer");
+  const int bad = check_strides(strides, "sv_window_attention");
+  if (bad != SV_OK) return bad;
   AttnArgs a{};
   a.q = q; a.k = k; a.v = v; a.out = out;
   a.q_row = strides[0]; a.q_head = strides[1];
@@ -274,6 +283,8 @@ extern "C" int sv_window_attention_backward(
   if (!q || !k || !v || !strides || !o || !dout || !stats || !plan || !table || !lut || !dq || !dk ||
       !dv || !aligned16(plan))
     SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_window_attention_backward: null pointer");
+  const int bad = check_strides(strides, "sv_window_attention_backward");
+  if (bad != SV_OK) return bad;
   const Layout l = layout(n, heads, buckets);
   if (!workspace || workspace_bytes < l.total || !aligned16(workspace))
     SV_FAIL(SV_ERR_WORKSPACE, "sv_window_attention_backward: workspace too small or unaligned");

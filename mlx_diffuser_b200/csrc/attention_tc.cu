@@ -28,8 +28,8 @@
 namespace sv {
 namespace {
 
-constexpr int BQ = 64;   // rows of a block
-constexpr int AT = 128;  // threads
+constexpr int AT = 128;  // threads: four warps of 16 rows, or of 16 MR
+constexpr int KB = 32;   // positions of a tile
 
 // Tiles hold DP channels a row (the head's, padded with zeros) at a stride that is an odd multiple
 // of 16 bytes, so the 8 rows of a matrix fragment fall into different banks.
@@ -95,19 +95,20 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // R gathered rows of one head into a tile; rows of -1 and channels past `dim` become zeros.
 template <typename T, int DP, int R>
-__device__ __forceinline__ void load_tile(uint8_t* tile, const T* base, int64_t row_stride,
+__device__ __forceinline__ void load_tile(uint8_t* tile, const T* base, int row_stride,
                                           const int32_t* rows, int dim, bool vec) {
-  constexpr int CH = DP / 8;  // 16-byte chunks of a row
+  constexpr int CH = DP / 8;  // 16-byte chunks of a row; a thread copies the same one of every row
+  static_assert(AT % CH == 0 && R * CH % AT == 0, "whole rounds");
   if (vec) {
-    const uint32_t at = smem_u32(tile);
+    const int col = threadIdx.x % CH, r0 = threadIdx.x / CH;
+    const uint32_t at = smem_u32(tile) + r0 * STRIDE<DP> + col * 16;
+    const bool in_row = col * 8 < dim;
+    const T* from = base + (in_row ? col * 8 : 0);
 #pragma unroll
     for (int i = 0; i < R * CH / AT; ++i) {
-      const int c = threadIdx.x + AT * i;
-      const int r = c / CH, col = c % CH;
-      const int32_t row = rows[r];
-      const bool in = row >= 0 && col * 8 < dim;
-      cp_async_16(at + r * STRIDE<DP> + col * 16,
-                  base + (in ? (int64_t)row * row_stride + col * 8 : 0), in ? 16u : 0u);
+      const int32_t row = rows[r0 + i * (AT / CH)];
+      cp_async_16(at + i * (AT / CH) * STRIDE<DP>, from + (int64_t)max(row, 0) * row_stride,
+                  row >= 0 && in_row ? 16u : 0u);
     }
   } else {
     for (int c = threadIdx.x; c < R * DP; c += AT) {
@@ -120,15 +121,14 @@ __device__ __forceinline__ void load_tile(uint8_t* tile, const T* base, int64_t 
   }
 }
 
-// A 16-row accumulator (a warp's rows of the block) through the warp's own part of a tile to the
-// feature rows, in 16-byte stores.
+// A 16-row accumulator through the warp's own part of a tile (`mine`) to the feature rows `rows`, in
+// 16-byte stores.
 template <typename T, int DP>
-__device__ __forceinline__ void store_rows(uint8_t* tile, const float (&o)[DP / 8][4], float s0,
+__device__ __forceinline__ void store_rows(uint8_t* mine, const float (&o)[DP / 8][4], float s0,
                                            float s1, const int32_t* rows, T* out, int heads,
                                            int head, int dim, bool vec) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
   const int g = lane >> 2, c2 = 2 * (lane & 3);
-  uint8_t* mine = tile + warp * 16 * STRIDE<DP>;
   __syncwarp();
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) {
@@ -143,7 +143,7 @@ __device__ __forceinline__ void store_rows(uint8_t* tile, const float (&o)[DP / 
   for (int i = 0; i < 16 * CH / 32; ++i) {
     const int c = lane + 32 * i;
     const int r = c / CH, col = c % CH;
-    const int32_t row = rows[warp * 16 + r];
+    const int32_t row = rows[r];
     if (row < 0) continue;
     T* dst = out + ((int64_t)row * heads + head) * dim + col * 8;
     const uint4 v = *reinterpret_cast<const uint4*>(mine + r * STRIDE<DP> + col * 16);
@@ -162,15 +162,17 @@ struct KeyMeta {
   int32_t x, y, z, row;  // row -1: no row
 };
 
-// What every kernel here keeps in shared memory besides its tiles of KB positions.
-template <int KB>
+constexpr int SLOTS = 4;  // tiles whose rows are known: the one worked on and three ahead
+
+// What every kernel here keeps in shared memory besides its tiles; BQ rows of the block's own.
+template <int BQ>
 struct alignas(16) Shared {
-  KeyMeta key[3][KB];      // ring of the other side's rows, two tiles ahead
-  int2 key_lin[3][KB];     // their linear coordinates: {of all axes, -}, or {of x and y, z}
-  int32_t key_row[3][KB];
-  float2 key_stats[3][KB]; // their softmax and delta (dk / dv)
-  float key_delta[3][KB];
-  int32_t key_bad[3];      // whether a position has no row
+  KeyMeta key[SLOTS][KB];       // the other side's rows
+  int2 key_lin[SLOTS][KB];      // their linear coordinates (Block::lin)
+  int32_t key_row[SLOTS][KB];
+  float2 key_stats[SLOTS][KB];  // their softmax and delta (dk / dv)
+  float key_delta[SLOTS][KB];
+  int32_t key_bad[SLOTS];       // whether a position has no row
   PlanRow own[BQ];
   int32_t own_row[BQ];
   int32_t range[2];
@@ -178,47 +180,61 @@ struct alignas(16) Shared {
 
 // How a pair's bucket is found. LINEAR: the look-up is the identity and the windows are within the
 // table's reach, so the bucket is a difference of linear coordinates. JOINT: within the reach, and
-// the look-ups of x and y are joined in one table of all their offsets. GENERAL: any.
+// the look-ups of x and y are joined in one table of all their offsets. GENERAL: any. All indexes are
+// kept as byte offsets.
 enum { GENERAL = 0, JOINT = 1, LINEAR = 2 };
 constexpr int JOINT_MAX = 4096;
 
-template <typename T, int KB>
+__device__ __forceinline__ float lds_f32(uint32_t at) {
+  float v;
+  asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
+  uint16_t v;
+  asm("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+  return v;
+}
+
+template <typename T, int BQ>
 struct Block {
   const AttnArgs& a;
-  Shared<KB>& s;
+  Shared<BQ>& s;
   float* table;      // [nb^3] times log2(e)
-  int16_t* lut;      // [2 reach + 1]
-  int16_t* joint;    // [(2 reach + 1)^2], x and y buckets as the table's index, or null
+  uint16_t* lut;     // [2 reach + 1], times 4
+  uint16_t* joint;   // [(2 reach + 1)^2]: x and y buckets' offset in the table, or null
   int head;
   bool identity;
   float delta_top;   // largest |delta| staged by this thread
-  // set per 64 rows
+  // set per BQ rows
   int mode;
   int j0, tiles;
 
   __device__ __forceinline__ int cells() const { return a.nb * a.nb * a.nb; }
   __device__ __forceinline__ int width() const { return 2 * a.reach + 1; }
 
-  // Wrap-around is harmless: only differences inside a window are used.
+  // LINEAR: 4 ((x nb + y) nb + z); JOINT: 2 (x width + y) and 2 z. Wrap-around is harmless: only
+  // differences inside a window are used.
   __device__ __forceinline__ int2 lin(int x, int y, int z) const {
     if (mode == LINEAR)
-      return make_int2((int)(((unsigned)x * a.nb + (unsigned)y) * a.nb + (unsigned)z), 0);
-    return make_int2((int)((unsigned)x * width() + (unsigned)y), z);
+      return make_int2((int)((((unsigned)x * a.nb + (unsigned)y) * a.nb + (unsigned)z) * 4u), 0);
+    return make_int2((int)(((unsigned)x * width() + (unsigned)y) * 2u), (int)((unsigned)z * 2u));
   }
 
   __device__ void stage_tables() {
     const T* src = static_cast<const T*>(a.table) + (int64_t)head * cells();
+#pragma unroll 8
     for (int i = threadIdx.x; i < cells(); i += AT) table[i] = times_log2e(to_f32(src[i]));
     bool same = a.nb == width();
     for (int i = threadIdx.x; i < width(); i += AT) {
       const int v = max(0, min(a.nb - 1, __ldg(a.lut + i)));
-      lut[i] = (int16_t)v;
+      lut[i] = (uint16_t)(4 * v);
       same = same && v == i;
     }
     identity = __syncthreads_and(same);
     if (!identity && joint != nullptr)
       for (int i = threadIdx.x; i < width() * width(); i += AT)
-        joint[i] = (int16_t)((lut[i / width()] * a.nb + lut[i % width()]) * a.nb);
+        joint[i] = (uint16_t)((lut[i / width()] * a.nb + lut[i % width()]) * a.nb);
   }
 
   // The block's rows and the positions their windows cover.
@@ -247,58 +263,59 @@ struct Block {
     tiles = s.range[1] > j0 ? (s.range[1] - j0 + KB - 1) / KB : 0;
   }
 
-  // By the first warp: a position a lane.
+  // By one warp: a position a lane.
   template <bool STATS>
   __device__ void stage_meta(int t) {
     static_assert(KB == 32, "a position a lane");
-    const int slot = t % 3;
-    const int i = threadIdx.x;
-    if (i < KB) {
-      const int j = j0 + t * KB + i;
-      KeyMeta m{0, 0, 0, -1};
-      if (j < s.range[1])
-        *reinterpret_cast<int4*>(&m) = __ldg(reinterpret_cast<const int4*>(a.plan + j));
-      if constexpr (STATS) {
-        float2 st = make_float2(0.f, 0.f);
-        float d = 0.f;
-        if (m.row >= 0) {
-          st = a.stats[head * a.n + j];
-          d = a.delta[head * a.n + j];
-        }
-        s.key_stats[slot][i] = st;
-        s.key_delta[slot][i] = d;
-        delta_top = max_nan(delta_top, fabsf(d));
+    const int slot = t % SLOTS;
+    const int i = threadIdx.x & 31;
+    const int j = j0 + t * KB + i;
+    KeyMeta m{0, 0, 0, -1};
+    if (j < s.range[1])
+      *reinterpret_cast<int4*>(&m) = __ldg(reinterpret_cast<const int4*>(a.plan + j));
+    if constexpr (STATS) {
+      float2 st = make_float2(0.f, 0.f);
+      float d = 0.f;
+      if (m.row >= 0) {
+        st = a.stats[head * a.n + j];
+        d = a.delta[head * a.n + j];
       }
-      const unsigned bad = __ballot_sync(0xffffffffu, j < s.range[1] && m.row < 0);
-      if (i == 0) s.key_bad[slot] = bad != 0;
-      s.key[slot][i] = m;
-      s.key_lin[slot][i] = lin(m.x, m.y, m.z);
-      s.key_row[slot][i] = m.row;
+      s.key_stats[slot][i] = st;
+      s.key_delta[slot][i] = d;
+      delta_top = max_nan(delta_top, fabsf(d));
     }
+    const unsigned bad = __ballot_sync(0xffffffffu, j < s.range[1] && m.row < 0);
+    if (i == 0) s.key_bad[slot] = bad != 0;
+    s.key[slot][i] = m;
+    s.key_lin[slot][i] = lin(m.x, m.y, m.z);
+    s.key_row[slot][i] = m.row;
   }
 
-  __device__ __forceinline__ int bucket(int qx, int qy, int qz, int kx, int ky, int kz) const {
+  __device__ __forceinline__ uint32_t bucket(int qx, int qy, int qz, int kx, int ky, int kz) const {
     const int R = a.reach;
     const int x = lut[max(-R, min(R, sub_sat(kx, qx))) + R];
     const int y = lut[max(-R, min(R, sub_sat(ky, qy))) + R];
     const int z = lut[max(-R, min(R, sub_sat(kz, qz))) + R];
-    return (x * a.nb + y) * a.nb + z;
+    return (uint32_t)((x * a.nb + y) * a.nb + z);
   }
 };
 
-// Calls use(n, e, bucket) for a thread's pairs: element e of fragment n is row g + 8 (e / 2) of the
-// warp's 16 and column 8 n + 2 (lane % 4) + e % 2. FLIP: the rows are keys and the columns queries.
-// WHOLE: all pairs are inside a window; otherwise indexes of the others (masked) are clamped.
-template <bool FLIP, bool WHOLE, typename T, int KB, typename F>
-__device__ __forceinline__ void each_pair(const Block<T, KB>& b, int slot, const PlanRow (&own)[2],
+// Calls use(n, e, at) for a thread's pairs with the pair's byte offset in the table: element e of
+// fragment n is row g + 8 (e / 2) of 16 and column 8 n + 2 (lane % 4) + e % 2. FLIP: the rows are
+// keys and the columns queries. WHOLE: all pairs are inside a window; otherwise the offsets of the
+// others (masked) are clamped.
+template <bool FLIP, bool WHOLE, typename T, int BQ, typename F>
+__device__ __forceinline__ void each_pair(const Block<T, BQ>& b, int slot, const PlanRow* own,
                                           F&& use) {
   const int c2 = 2 * (threadIdx.x & 3);
-  auto within = [](int v, unsigned top) { return WHOLE ? v : (int)min((unsigned)v, top); };
+  auto within = [](int v, uint32_t top) -> uint32_t {
+    return WHOLE ? (uint32_t)v : min((uint32_t)v, top);
+  };
   if (b.mode == LINEAR) {
-    const unsigned top = (unsigned)b.cells() - 1u;
+    const uint32_t top = (uint32_t)b.cells() * 4u - 4u;
     const int mid = FLIP ? (int)(top / 2) : -(int)(top / 2);
     const int l[2] = {b.lin(own[0].x, own[0].y, own[0].z).x + mid,
-                      b.lin(own[1].x, own[1].y, own[1].z).x + mid};
+                      b.lin(own[8].x, own[8].y, own[8].z).x + mid};
 #pragma unroll
     for (int n = 0; n < KB / 8; ++n) {
       // the linear coordinates of two neighbours: .x and .z
@@ -310,13 +327,15 @@ __device__ __forceinline__ void each_pair(const Block<T, KB>& b, int slot, const
       }
     }
   } else if (b.mode == JOINT) {
-    const unsigned top = (unsigned)(b.width() * b.width()) - 1u, ztop = (unsigned)b.width() - 1u;
+    const uint32_t joint = smem_u32(b.joint), lut = smem_u32(b.lut);
+    const uint32_t top = (uint32_t)(b.width() * b.width()) * 2u - 2u;
+    const uint32_t ztop = (uint32_t)b.width() * 2u - 2u;
     const int mid = FLIP ? (int)(top / 2) : -(int)(top / 2);
-    const int zmid = FLIP ? b.a.reach : -b.a.reach;
+    const int zmid = FLIP ? 2 * b.a.reach : -2 * b.a.reach;
     int2 l[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      l[r] = b.lin(own[r].x, own[r].y, own[r].z);
+      l[r] = b.lin(own[8 * r].x, own[8 * r].y, own[8 * r].z);
       l[r].x += mid;
       l[r].y += zmid;
     }
@@ -326,9 +345,9 @@ __device__ __forceinline__ void each_pair(const Block<T, KB>& b, int slot, const
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int c = e & 1 ? k.z : k.x, z = e & 1 ? k.w : k.y;
-        const int xy = within(FLIP ? l[e >> 1].x - c : c - l[e >> 1].x, top);
-        const int dz = within(FLIP ? l[e >> 1].y - z : z - l[e >> 1].y, ztop);
-        use(n, e, b.joint[xy] + b.lut[dz]);
+        const uint32_t xy = within(FLIP ? l[e >> 1].x - c : c - l[e >> 1].x, top);
+        const uint32_t dz = within(FLIP ? l[e >> 1].y - z : z - l[e >> 1].y, ztop);
+        use(n, e, lds_u16(joint + xy) + lds_u16(lut + dz));
       }
     }
   } else {
@@ -338,53 +357,66 @@ __device__ __forceinline__ void each_pair(const Block<T, KB>& b, int slot, const
       for (int c = 0; c < 2; ++c) {
         const KeyMeta k = b.s.key[slot][n * 8 + c2 + c];
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-          use(n, 2 * r + c,
-              FLIP ? b.bucket(k.x, k.y, k.z, own[r].x, own[r].y, own[r].z)
-                   : b.bucket(own[r].x, own[r].y, own[r].z, k.x, k.y, k.z));
+        for (int r = 0; r < 2; ++r) {
+          const PlanRow& o = own[8 * r];
+          use(n, 2 * r + c, FLIP ? b.bucket(k.x, k.y, k.z, o.x, o.y, o.z)
+                                 : b.bucket(o.x, o.y, o.z, k.x, k.y, k.z));
+        }
       }
     }
   }
 }
 
-// acc += rows x tile^T over DP channels, 16 rows by KB columns; the rows' fragments come from `rows`
-// (the warp's 16 rows of a tile).
-template <typename T, int DP, int KB>
-__device__ __forceinline__ void mma_nt(float (&acc)[KB / 8][4], uint32_t rows, uint32_t tile) {
+// acc += rows x tile^T over DP channels, 16 MR rows by KB columns; the rows' fragments come from
+// `rows` (the warp's rows of a tile).
+template <typename T, int DP, int MR>
+__device__ __forceinline__ void mma_nt(float (&acc)[MR][KB / 8][4], uint32_t rows, uint32_t tile) {
   const int lane = threadIdx.x & 31;
   const uint32_t from = rows + (lane & 15) * STRIDE<DP> + (lane >> 4) * 16;
   const uint32_t at = tile + ((lane & 7) + (lane >> 4) * 8) * STRIDE<DP> + ((lane >> 3) & 1) * 16;
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k) {
-    uint32_t f[4];
-    ldsm4(from + k * 32, f);
+    uint32_t f[MR][4];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) ldsm4(from + m * 16 * STRIDE<DP> + k * 32, f[m]);
 #pragma unroll
     for (int n = 0; n < KB / 16; ++n) {
       uint32_t b[4];
       ldsm4(at + n * 16 * STRIDE<DP> + k * 32, b);
-      mma<T>(acc[2 * n], f, b[0], b[1]);
-      mma<T>(acc[2 * n + 1], f, b[2], b[3]);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        mma<T>(acc[m][2 * n], f[m], b[0], b[1]);
+        mma<T>(acc[m][2 * n + 1], f[m], b[2], b[3]);
+      }
     }
   }
 }
 
-// out += w (16 x KB sums, rounded to T as operand fragments) x tile (KB x DP).
-template <typename T, int DP, int KB>
-__device__ __forceinline__ void mma_nn(float (&out)[DP / 8][4], const float (&w)[KB / 8][4],
-                                       uint32_t tile) {
+// out += w (16 MR x KB sums, rounded to T as operand fragments) x tile (KB x DP).
+template <typename T, int DP, int MR>
+__device__ __forceinline__ void mma_nn(float (&out)[MR][DP / 8][4],
+                                       const float (&w)[MR][KB / 8][4], uint32_t tile) {
   const int lane = threadIdx.x & 31;
   const uint32_t at = tile + ((lane & 7) + ((lane >> 3) & 1) * 8) * STRIDE<DP> + (lane >> 4) * 16;
 #pragma unroll
   for (int k = 0; k < KB / 16; ++k) {
-    const uint32_t f[4] = {pack2<T>(w[2 * k][0], w[2 * k][1]), pack2<T>(w[2 * k][2], w[2 * k][3]),
-                           pack2<T>(w[2 * k + 1][0], w[2 * k + 1][1]),
-                           pack2<T>(w[2 * k + 1][2], w[2 * k + 1][3])};
+    uint32_t f[MR][4];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      f[m][0] = pack2<T>(w[m][2 * k][0], w[m][2 * k][1]);
+      f[m][1] = pack2<T>(w[m][2 * k][2], w[m][2 * k][3]);
+      f[m][2] = pack2<T>(w[m][2 * k + 1][0], w[m][2 * k + 1][1]);
+      f[m][3] = pack2<T>(w[m][2 * k + 1][2], w[m][2 * k + 1][3]);
+    }
 #pragma unroll
     for (int n = 0; n < DP / 16; ++n) {
       uint32_t b[4];
       ldsm4_t(at + k * 16 * STRIDE<DP> + n * 32, b);
-      mma<T>(out[2 * n], f, b[0], b[1]);
-      mma<T>(out[2 * n + 1], f, b[2], b[3]);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        mma<T>(out[m][2 * n], f[m], b[0], b[1]);
+        mma<T>(out[m][2 * n + 1], f[m], b[2], b[3]);
+      }
     }
   }
 }
@@ -397,32 +429,46 @@ __device__ __forceinline__ void zero(float (&x)[W][4]) {
     for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
 }
 
-// Positions that any of the warp's 16 rows sees, and those that all of them do.
+// Positions that any of a warp's ROWS rows sees, and those that all of them do.
 struct Reach {
   int lo, hi, all_lo, all_hi;
 };
-__device__ __forceinline__ Reach warp_reach(const PlanRow (&own)[2]) {
+template <int ROWS>
+__device__ __forceinline__ Reach warp_reach(const PlanRow* own) {
+  const int lane = threadIdx.x & 31;
+  const PlanRow& r = own[lane % ROWS];
+  const bool any = r.end > r.start;
   Reach w;
-  int lo = INT_MAX, hi = INT_MIN;
-#pragma unroll
-  for (int r = 0; r < 2; ++r)
-    if (own[r].end > own[r].start) {
-      lo = min(lo, own[r].start);
-      hi = max(hi, own[r].end);
-    }
-  w.lo = __reduce_min_sync(0xffffffffu, lo);
-  w.hi = __reduce_max_sync(0xffffffffu, hi);
-  w.all_lo = __reduce_max_sync(0xffffffffu, max(own[0].start, own[1].start));
-  w.all_hi = __reduce_min_sync(0xffffffffu, min(own[0].end, own[1].end));
+  w.lo = __reduce_min_sync(0xffffffffu, any ? r.start : INT_MAX);
+  w.hi = __reduce_max_sync(0xffffffffu, any ? r.end : INT_MIN);
+  w.all_lo = __reduce_max_sync(0xffffffffu, r.start);
+  w.all_hi = __reduce_min_sync(0xffffffffu, r.end);
   return w;
 }
 
-// Whether column `col` of a tile that begins at position p0 is outside the row's window, or has no
-// row (`bad`: some column has none).
-template <int KB>
-__device__ __forceinline__ bool hidden(const PlanRow& r, int p0, int col, bool bad,
-                                       const Shared<KB>& s, int slot) {
-  return col < r.start - p0 || col >= r.end - p0 || (bad && s.key_row[slot][col] < 0);
+// The columns of a thread's fragments that the rows g and g + 8 see, relative to its own first
+// column: element (n, e) is column 8 n + e % 2 of row e / 2.
+struct Sight {
+  int lo[2], hi[2];
+};
+__device__ __forceinline__ Sight sight(const PlanRow* own, int p0) {
+  const int c2 = 2 * (threadIdx.x & 3);
+  Sight v;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    v.lo[r] = own[8 * r].start - p0 - c2;
+    v.hi[r] = own[8 * r].end - p0 - c2;
+  }
+  return v;
+}
+// `bad`: some column has no row.
+template <int BQ>
+__device__ __forceinline__ bool hidden(const Sight& v, int n, int e, bool bad, const Shared<BQ>& s,
+                                       int slot) {
+  const int col = 8 * n + (e & 1);
+  bool out = (col < v.lo[e >> 1]) | (col >= v.hi[e >> 1]);
+  if (bad) out |= s.key_row[slot][col + 2 * (threadIdx.x & 3)] < 0;
+  return out;
 }
 
 // A weight of zero does not hide a NaN or an infinity that another window's row brings into a tile,
@@ -468,15 +514,15 @@ __device__ __noinline__ void again_dkv(AttnArgs a, int64_t p, int h, float* s) {
   row_dkv<T, true>(a, p, h, s);
 }
 
-// Shared memory: OWN tiles of the block's rows, two buffers of two tiles of KB positions, then the
-// tables.
-template <int DP, int KB, int OWN>
+// Shared memory: OWN tiles of the block's BQ rows, STAGES buffers of two tiles of KB positions, then
+// the tables.
+template <int DP, int BQ, int OWN, int STAGES>
 struct Layout {
   static constexpr int OWN_TILE = BQ * STRIDE<DP>;
   static constexpr int TILE = KB * STRIDE<DP>;
   static constexpr int RING = OWN * OWN_TILE;
-  static constexpr int SHARED = RING + 4 * TILE;
-  static constexpr int TABLE = (SHARED + (int)sizeof(Shared<KB>) + 15) / 16 * 16;
+  static constexpr int SHARED = RING + STAGES * 2 * TILE;
+  static constexpr int TABLE = (SHARED + (int)sizeof(Shared<BQ>) + 15) / 16 * 16;
 };
 
 struct Tables {
@@ -496,133 +542,186 @@ __host__ __device__ inline Tables tables(const AttnArgs& a, bool grad) {
   return t;
 }
 
-template <typename T, int KB>
-__device__ __forceinline__ Block<T, KB> make_block(const AttnArgs& a, uint8_t* smem, int shared,
+template <typename T, int BQ>
+__device__ __forceinline__ Block<T, BQ> make_block(const AttnArgs& a, uint8_t* smem, int shared,
                                                    int table, bool grad) {
   const Tables t = tables(a, grad);
-  return Block<T, KB>{a, *reinterpret_cast<Shared<KB>*>(smem + shared),
+  return Block<T, BQ>{a, *reinterpret_cast<Shared<BQ>*>(smem + shared),
                       reinterpret_cast<float*>(smem + table),
-                      reinterpret_cast<int16_t*>(smem + table + t.lut),
-                      t.joint < 0 ? nullptr : reinterpret_cast<int16_t*>(smem + table + t.joint),
+                      reinterpret_cast<uint16_t*>(smem + table + t.lut),
+                      t.joint < 0 ? nullptr : reinterpret_cast<uint16_t*>(smem + table + t.joint),
                       (int)blockIdx.y, false, 0.f};
 }
 
-// The tiles of one block: `own` loads the block's own rows, `load(buffer, rows)` a tile's, and
-// body(t, buffer) works on tile t. One barrier a tile: behind it the tile has landed, the other
-// buffer's readers are done, and the rows of the next tile are known. `flush` is asked at the
-// barrier, by any thread, and done before the tile.
-template <bool STATS, typename B, typename Load, typename Body, typename Ask, typename Flush>
+// The tiles of one block: load(buffer, rows) fetches a tile's rows, STAGES - 1 tiles ahead (the
+// block's own rows, loaded before, are in the first group), and body(t, buffer) works on tile t.
+// One barrier a tile: behind it the tile has landed, the readers of the buffer that is filled next
+// are done, and the rows of the tile that fills it are known. ask() is asked at the barrier, by
+// every thread, and flush() done before the tile if any said yes.
+template <bool STATS, int STAGES, typename B, typename Load, typename Body, typename Ask,
+          typename Flush>
 __device__ __forceinline__ void walk(B& b, Load&& load, Body&& body, Ask&& ask, Flush&& flush) {
-  b.template stage_meta<STATS>(0);
-  b.template stage_meta<STATS>(1);
+  static_assert(STAGES + 1 <= SLOTS, "rows known ahead");
+  const int warp = threadIdx.x >> 5;
+  if (warp < STAGES) b.template stage_meta<STATS>(warp);
   __syncthreads();
-  if (b.tiles > 0) load(0, b.s.key_row[0]);
-  cp_commit();
-  for (int t = 0; t < b.tiles; ++t) {
-    cp_wait<0>();
-    if (__syncthreads_or(ask())) flush();
-    if (t + 1 < b.tiles) load((t + 1) & 1, b.s.key_row[(t + 1) % 3]);
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t) {
+    if (t < b.tiles) load(t, b.s.key_row[t]);
     cp_commit();
-    if (t + 2 < b.tiles) b.template stage_meta<STATS>(t + 2);
-    body(t, t & 1);
+  }
+  int buf = 0, fill = STAGES - 1;
+  for (int t = 0; t < b.tiles; ++t) {
+    cp_wait<STAGES - 2>();
+    if (__syncthreads_or(ask())) flush();
+    if (t + STAGES - 1 < b.tiles) load(fill, b.s.key_row[(t + STAGES - 1) % SLOTS]);
+    cp_commit();
+    // by another warp each time
+    if (t + STAGES < b.tiles && warp == (t & 3)) b.template stage_meta<STATS>(t + STAGES);
+    body(t, buf);
+    buf = buf + 1 == STAGES ? 0 : buf + 1;
+    fill = fill + 1 == STAGES ? 0 : fill + 1;
   }
   cp_wait<0>();
   __syncthreads();
 }
 
-template <typename T, int DP, int KB>
-__global__ void __launch_bounds__(AT, DP <= 64 ? 4 : 2)
+// Scores may pass the running base by this much (in powers of two) before the sums are rescaled, so
+// most tiles skip it; weights then reach 2^8 at most, which neither type nor the fp32 sums notice.
+constexpr float SLACK = 8.f;
+
+// MR: 16-row parts of a warp, whose products share the tile's fragments.
+template <typename T, int DP, int MR, int STAGES>
+__global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
     attn_tc_kernel(AttnArgs a, int per_block, bool vec) {
-  using L = Layout<DP, KB, 1>;
+  constexpr int BQ = 64 * MR;
+  using L = Layout<DP, BQ, 1, STAGES>;
   extern __shared__ __align__(16) uint8_t smem[];
-  Block<T, KB> b = make_block<T, KB>(a, smem, L::SHARED, L::TABLE, false);
-  Shared<KB>& sh = b.s;
+  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, false);
+  Shared<BQ>& sh = b.s;
   const int head = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c2 = 2 * (lane & 3);
-  uint8_t* mine = smem + warp * 16 * STRIDE<DP>;  // the warp's rows of q
+  const int row0 = warp * 16 * MR;            // the warp's rows of the block
+  uint8_t* mine = smem + row0 * STRIDE<DP>;   // and of q
   const T* q = static_cast<const T*>(a.q) + head * a.q_head;
   const T* k = static_cast<const T*>(a.k) + head * a.k_head;
   const T* v = static_cast<const T*>(a.v) + head * a.v_head;
   const float scale = a.scale * ATTN_LOG2E;
+  const uint32_t table = smem_u32(b.table);
   b.stage_tables();
   const int64_t first = (int64_t)blockIdx.x * per_block;
-  for (int64_t t64 = first; t64 < first + per_block && t64 * BQ < a.n; ++t64) {
-    b.begin(t64 * BQ);
-    load_tile<T, DP, BQ>(smem, q, a.q_row, sh.own_row, a.dim, vec);
-    const PlanRow own[2] = {sh.own[warp * 16 + g], sh.own[warp * 16 + g + 8]};
-    const Reach w = warp_reach(own);
-    float o[DP / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-    zero(o);
+  for (int64_t block = first; block < first + per_block && block * BQ < a.n; ++block) {
+    b.begin(block * BQ);
+    load_tile<T, DP, BQ>(smem, q, (int)a.q_row, sh.own_row, a.dim, vec);
+    const PlanRow* own = sh.own + row0 + g;
+    const Reach w = warp_reach<16 * MR>(sh.own + row0);
+    float o[MR][DP / 8][4], base[MR][2], sum[MR][2];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      zero(o[m]);
+      base[m][0] = base[m][1] = -3.402823466e38f;
+      sum[m][0] = sum[m][1] = 0.f;
+    }
     auto body = [&](int t, int buf) {
       const int p0 = b.j0 + t * KB;
       if (p0 >= w.hi || p0 + KB <= w.lo) return;
       const uint32_t tile = smem_u32(smem + L::RING + buf * 2 * L::TILE);
-      const int slot = t % 3;
-      float s[KB / 8][4];
-      zero(s);
-      mma_nt<T, DP, KB>(s, smem_u32(mine), tile);
-      auto score = [&](int n, int e, int at) { s[n][e] = fmaf(s[n][e], scale, b.table[at]); };
+      const int slot = t % SLOTS;
       const bool bad = sh.key_bad[slot];
-      if (p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad) {
-        each_pair<false, true>(b, slot, own, score);
-      } else {
-        each_pair<false, false>(b, slot, own, score);
+      const bool whole = p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad;
+      float s[MR][KB / 8][4];
+#pragma unroll
+      for (int m = 0; m < MR; ++m) zero(s[m]);
+      mma_nt<T, DP, MR>(s, smem_u32(mine), tile);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        auto score = [&](int n, int e, uint32_t at) {
+          s[m][n][e] = fmaf(s[m][n][e], scale, lds_f32(table + at));
+        };
+        if (whole) {
+          each_pair<false, true>(b, slot, own + 16 * m, score);
+        } else {
+          each_pair<false, false>(b, slot, own + 16 * m, score);
+          const Sight seen = sight(own + 16 * m, p0);
+#pragma unroll
+          for (int n = 0; n < KB / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (hidden(seen, n, e, bad, sh, slot)) s[m][n][e] = -INFINITY;
+        }
+      }
+      float top[MR][2];
+      bool over = false;
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float x = fmaxf(s[m][0][2 * r], s[m][0][2 * r + 1]);
+#pragma unroll
+          for (int n = 1; n < KB / 8; ++n) x = fmaxf(x, fmaxf(s[m][n][2 * r], s[m][n][2 * r + 1]));
+          top[m][r] = x;
+          over = over || x > base[m][r] + SLACK;
+        }
+      }
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float x = top[m][r];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            x = fmaxf(x, base[m][r]);
+            const float keep = exp2_fast(base[m][r] - x);
+            base[m][r] = x;
+            sum[m][r] *= keep;
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n) {
+              o[m][n][2 * r] *= keep;
+              o[m][n][2 * r + 1] *= keep;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MR; ++m)
 #pragma unroll
         for (int n = 0; n < KB / 8; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (hidden(own[e >> 1], p0, n * 8 + c2 + (e & 1), bad, sh, slot)) s[n][e] = -INFINITY;
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float m = top[r];
-#pragma unroll
-        for (int n = 0; n < KB / 8; ++n) m = fmaxf(m, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float base = m == -INFINITY ? 0.f : m;
-        const float keep = exp2_fast(top[r] - base);
-        top[r] = m;
-        sum[r] *= keep;
-#pragma unroll
-        for (int n = 0; n < KB / 8; ++n) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float e = exp2_fast(s[n][2 * r + c] - base);
-            s[n][2 * r + c] = e;
-            sum[r] += e;
+          for (int e = 0; e < 4; ++e) {
+            s[m][n][e] = exp2_fast(s[m][n][e] - base[m][e >> 1]);
+            sum[m][e >> 1] += s[m][n][e];
           }
-        }
-#pragma unroll
-        for (int n = 0; n < DP / 8; ++n) {
-          o[n][2 * r] *= keep;
-          o[n][2 * r + 1] *= keep;
-        }
-      }
-      mma_nn<T, DP, KB>(o, s, tile + L::TILE);
+      mma_nn<T, DP, MR>(o, s, tile + L::TILE);
     };
-    walk<false>(
+    walk<false, STAGES>(
         b,
         [&](int buf, const int32_t* rows) {
           uint8_t* tile = smem + L::RING + buf * 2 * L::TILE;
-          load_tile<T, DP, KB>(tile, k, a.k_row, rows, a.dim, vec);
-          load_tile<T, DP, KB>(tile + L::TILE, v, a.v_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile, k, (int)a.k_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile + L::TILE, v, (int)a.v_row, rows, a.dim, vec);
         },
         body, [] { return false; }, [] {});
-    float inv[2];
+    uint32_t redo = 0;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-      const float2 st = row_stats(top[r], sum[r]);
-      inv[r] = st.y;
-      if (a.stats && c2 == 0 && own[r].row >= 0)
-        a.stats[head * a.n + t64 * BQ + warp * 16 + g + 8 * r] = st;
+    for (int m = 0; m < MR; ++m) {
+      float inv[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float x = sum[m][r];
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        const float2 st = row_stats(base[m][r], x);
+        inv[r] = st.y;
+        const int at = row0 + 16 * m + g + 8 * r;
+        if (a.stats && c2 == 0 && sh.own_row[at] >= 0) a.stats[head * a.n + block * BQ + at] = st;
+      }
+      store_rows<T, DP>(mine + 16 * m * STRIDE<DP>, o[m], inv[0], inv[1], sh.own_row + row0 + 16 * m,
+                        static_cast<T*>(a.out), a.heads, head, a.dim, vec);
+      redo |= not_finite<DP>(o[m]) << (16 * m);
     }
-    store_rows<T, DP>(smem, o, inv[0], inv[1], sh.own_row, static_cast<T*>(a.out), a.heads, head,
-                      a.dim, vec);
-    again(not_finite<DP>(o), t64 * BQ + warp * 16, mine,
+    again(redo, block * BQ + row0, mine,
           [&](int64_t p, float* f) { if (p < a.n) again_forward<T>(a, p, head, f); });
     __syncthreads();
   }
@@ -676,24 +775,26 @@ __device__ __forceinline__ int unit_exponent(const AttnArgs& a, int head) {
 }
 
 // dq and the table's gradient.
-template <typename T, int DP, int KB, bool TABLE>
+template <typename T, int DP, int STAGES, bool TABLE>
 __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
     attn_dq_tc_kernel(AttnArgs a, int per_block, bool vec) {
-  using L = Layout<DP, KB, 2>;
+  constexpr int BQ = 64;
+  using L = Layout<DP, BQ, 2, STAGES>;
   extern __shared__ __align__(16) uint8_t smem[];
-  Block<T, KB> b = make_block<T, KB>(a, smem, L::SHARED, L::TABLE, TABLE);
-  Shared<KB>& sh = b.s;
-  int* s_grad = reinterpret_cast<int*>(smem + L::TABLE + tables(a, TABLE).grad);
+  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, TABLE);
+  Shared<BQ>& sh = b.s;
   const int cells = b.cells();
+  int* s_grad = reinterpret_cast<int*>(smem + L::TABLE + tables(a, TABLE).grad);
+  const uint32_t table = smem_u32(b.table), grads = smem_u32(s_grad);
   const int head = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, c2 = 2 * (lane & 3);
+  const int g = lane >> 2;
   uint8_t* mine = smem + warp * 16 * STRIDE<DP>;
   const T* q = static_cast<const T*>(a.q) + head * a.q_head;
   const T* k = static_cast<const T*>(a.k) + head * a.k_head;
   const T* v = static_cast<const T*>(a.v) + head * a.v_head;
   const T* dout = static_cast<const T*>(a.dout) + (int64_t)head * a.dim;
-  const int64_t g_row = (int64_t)a.heads * a.dim;
+  const int g_row = a.heads * a.dim;
   const float scale = a.scale * ATTN_LOG2E;
   const int exponent = TABLE ? unit_exponent(a, head) : INT_MAX;
   const float unit = exponent == INT_MAX ? 0.f : ldexpf(1.f, exponent);
@@ -717,70 +818,76 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
     }
   };
   const int64_t first = (int64_t)blockIdx.x * per_block;
-  for (int64_t t64 = first; t64 < first + per_block && t64 * BQ < a.n; ++t64) {
-    b.begin(t64 * BQ);
-    load_tile<T, DP, BQ>(smem, q, a.q_row, sh.own_row, a.dim, vec);
+  for (int64_t block = first; block < first + per_block && block * BQ < a.n; ++block) {
+    b.begin(block * BQ);
+    load_tile<T, DP, BQ>(smem, q, (int)a.q_row, sh.own_row, a.dim, vec);
     load_tile<T, DP, BQ>(smem + L::OWN_TILE, dout, g_row, sh.own_row, a.dim, vec);
-    const PlanRow own[2] = {sh.own[warp * 16 + g], sh.own[warp * 16 + g + 8]};
-    const Reach w = warp_reach(own);
-    float2 stats[2];
-    float delta[2];
+    const PlanRow* own = sh.own + warp * 16 + g;
+    const Reach w = warp_reach<16>(sh.own + warp * 16);
+    float top[2], inv[2], delta[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int64_t p = t64 * BQ + warp * 16 + g + 8 * r;
-      stats[r] = own[r].row >= 0 ? a.stats[head * a.n + p] : make_float2(0.f, 0.f);
-      delta[r] = own[r].row >= 0 ? a.delta[head * a.n + p] : 0.f;
+      const bool live = own[8 * r].row >= 0;
+      const int64_t p = head * a.n + block * BQ + warp * 16 + g + 8 * r;
+      const float2 st = live ? a.stats[p] : make_float2(0.f, 0.f);
+      top[r] = st.x;
+      inv[r] = st.y;
+      delta[r] = live ? a.delta[p] : 0.f;
     }
-    float dq[DP / 8][4];
-    zero(dq);
+    float dq[1][DP / 8][4];
+    zero(dq[0]);
     auto body = [&](int t, int buf) {
       const int p0 = b.j0 + t * KB;
       if (p0 >= w.hi || p0 + KB <= w.lo) return;
       const uint32_t tile = smem_u32(smem + L::RING + buf * 2 * L::TILE);
-      const int slot = t % 3;
-      float s[KB / 8][4], dp[KB / 8][4];
-      zero(s);
-      mma_nt<T, DP, KB>(s, smem_u32(mine), tile);
+      const int slot = t % SLOTS;
+      float s[1][KB / 8][4], dp[1][KB / 8][4];
+      zero(s[0]);
+      mma_nt<T, DP, 1>(s, smem_u32(mine), tile);
 #pragma unroll
       for (int n = 0; n < KB / 8; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dp[n][e] = -delta[e >> 1];
-      mma_nt<T, DP, KB>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
+        for (int e = 0; e < 4; ++e) dp[0][n][e] = -delta[e >> 1];
+      mma_nt<T, DP, 1>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
       const bool bad = sh.key_bad[slot];
-      auto grad = [&](int n, int e, int at, bool in) {
+      auto grad = [&](int n, int e, uint32_t at, bool in) {
         const int r = e >> 1;
-        const float x = fmaf(s[n][e], scale, b.table[at]);
-        const float ds = exp2_fast(x - stats[r].x) * stats[r].y * dp[n][e];
-        s[n][e] = in ? ds : 0.f;
+        const float x = fmaf(s[0][n][e], scale, lds_f32(table + at));
+        const float ds = exp2_fast(x - top[r]) * (inv[r] * dp[0][n][e]);
+        s[0][n][e] = in ? ds : 0.f;
         if constexpr (TABLE) {
           if (in) {
             spent += fabsf(ds);
             // 1.5 * 2^23: the sum's low bits are the rounded integer
             const float f = fmaf(ds, unit, 12582912.f);
-            atomicAdd(s_grad + at, __float_as_int(f) - 0x4b400000);
+            asm volatile("red.shared.add.s32 [%0], %1;" ::"r"(grads + at),
+                         "r"(__float_as_int(f) - 0x4b400000)
+                         : "memory");
           }
         }
       };
       if (p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad) {
-        each_pair<false, true>(b, slot, own, [&](int n, int e, int at) { grad(n, e, at, true); });
+        each_pair<false, true>(b, slot, own,
+                               [&](int n, int e, uint32_t at) { grad(n, e, at, true); });
       } else {
-        each_pair<false, false>(b, slot, own, [&](int n, int e, int at) {
-          grad(n, e, at, !hidden(own[e >> 1], p0, n * 8 + c2 + (e & 1), bad, sh, slot));
+        const Sight seen = sight(own, p0);
+        each_pair<false, false>(b, slot, own, [&](int n, int e, uint32_t at) {
+          grad(n, e, at, !hidden(seen, n, e, bad, sh, slot));
         });
       }
-      mma_nn<T, DP, KB>(dq, s, tile);
+      mma_nn<T, DP, 1>(dq, s, tile);
     };
-    walk<false>(
+    walk<false, STAGES>(
         b,
         [&](int buf, const int32_t* rows) {
           uint8_t* tile = smem + L::RING + buf * 2 * L::TILE;
-          load_tile<T, DP, KB>(tile, k, a.k_row, rows, a.dim, vec);
-          load_tile<T, DP, KB>(tile + L::TILE, v, a.v_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile, k, (int)a.k_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile + L::TILE, v, (int)a.v_row, rows, a.dim, vec);
         },
         body, [&] { return TABLE && spent * unit > LIMIT; }, flush);
-    store_rows<T, DP>(smem, dq, a.scale, a.scale, sh.own_row, static_cast<T*>(a.dq), a.heads, head,
-                      a.dim, vec);
-    again(not_finite<DP>(dq), t64 * BQ + warp * 16, mine,
+    store_rows<T, DP>(mine, dq[0], a.scale, a.scale, sh.own_row + warp * 16, static_cast<T*>(a.dq),
+                      a.heads, head, a.dim, vec);
+    again(not_finite<DP>(dq[0]), block * BQ + warp * 16, mine,
           [&](int64_t p, float* f) { if (p < a.n) again_dq<T>(a, p, head, f); });
     __syncthreads();
   }
@@ -788,13 +895,15 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
 }
 
 // dk and dv, and the largest |dS| of the head: the block's rows are keys, the tiles queries.
-template <typename T, int DP, int KB, bool TABLE>
+template <typename T, int DP, int STAGES, bool TABLE>
 __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
     attn_dkv_tc_kernel(AttnArgs a, int per_block, bool vec) {
-  using L = Layout<DP, KB, 2>;
+  constexpr int BQ = 64;
+  using L = Layout<DP, BQ, 2, STAGES>;
   extern __shared__ __align__(16) uint8_t smem[];
-  Block<T, KB> b = make_block<T, KB>(a, smem, L::SHARED, L::TABLE, false);
-  Shared<KB>& sh = b.s;
+  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, false);
+  Shared<BQ>& sh = b.s;
+  const uint32_t table = smem_u32(b.table);
   const int head = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c2 = 2 * (lane & 3);
@@ -803,77 +912,78 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   const T* k = static_cast<const T*>(a.k) + head * a.k_head;
   const T* v = static_cast<const T*>(a.v) + head * a.v_head;
   const T* dout = static_cast<const T*>(a.dout) + (int64_t)head * a.dim;
-  const int64_t g_row = (int64_t)a.heads * a.dim;
+  const int g_row = a.heads * a.dim;
   const float scale = a.scale * ATTN_LOG2E;
   float most = 0.f;
   b.stage_tables();
   const int64_t first = (int64_t)blockIdx.x * per_block;
-  for (int64_t t64 = first; t64 < first + per_block && t64 * BQ < a.n; ++t64) {
-    b.begin(t64 * BQ);
-    load_tile<T, DP, BQ>(smem, k, a.k_row, sh.own_row, a.dim, vec);
-    load_tile<T, DP, BQ>(smem + L::OWN_TILE, v, a.v_row, sh.own_row, a.dim, vec);
-    const PlanRow own[2] = {sh.own[warp * 16 + g], sh.own[warp * 16 + g + 8]};
-    const Reach w = warp_reach(own);
-    float dk[DP / 8][4], dv[DP / 8][4];
-    zero(dk);
-    zero(dv);
+  for (int64_t block = first; block < first + per_block && block * BQ < a.n; ++block) {
+    b.begin(block * BQ);
+    load_tile<T, DP, BQ>(smem, k, (int)a.k_row, sh.own_row, a.dim, vec);
+    load_tile<T, DP, BQ>(smem + L::OWN_TILE, v, (int)a.v_row, sh.own_row, a.dim, vec);
+    const PlanRow* own = sh.own + warp * 16 + g;
+    const Reach w = warp_reach<16>(sh.own + warp * 16);
+    float dk[1][DP / 8][4], dv[1][DP / 8][4];
+    zero(dk[0]);
+    zero(dv[0]);
     auto body = [&](int t, int buf) {
       const int p0 = b.j0 + t * KB;
       if (p0 >= w.hi || p0 + KB <= w.lo) return;
       const uint32_t tile = smem_u32(smem + L::RING + buf * 2 * L::TILE);
-      const int slot = t % 3;
-      float s[KB / 8][4], dp[KB / 8][4];
-      zero(s);
-      mma_nt<T, DP, KB>(s, smem_u32(mine), tile);
+      const int slot = t % SLOTS;
+      float s[1][KB / 8][4], dp[1][KB / 8][4];
+      zero(s[0]);
+      mma_nt<T, DP, 1>(s, smem_u32(mine), tile);
       const bool bad = sh.key_bad[slot];
       const bool whole = p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad;
-      auto weight = [&](int n, int e, int at) {
+      auto weight = [&](int n, int e, uint32_t at) {
         const float2 st = sh.key_stats[slot][n * 8 + c2 + (e & 1)];
-        s[n][e] = exp2_fast(fmaf(s[n][e], scale, b.table[at]) - st.x) * st.y;
+        s[0][n][e] = exp2_fast(fmaf(s[0][n][e], scale, lds_f32(table + at)) - st.x) * st.y;
       };
       if (whole) {
         each_pair<true, true>(b, slot, own, weight);
       } else {
         each_pair<true, false>(b, slot, own, weight);
+        const Sight seen = sight(own, p0);
 #pragma unroll
         for (int n = 0; n < KB / 8; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (hidden(own[e >> 1], p0, n * 8 + c2 + (e & 1), bad, sh, slot)) s[n][e] = 0.f;
+            if (hidden(seen, n, e, bad, sh, slot)) s[0][n][e] = 0.f;
       }
-      mma_nn<T, DP, KB>(dv, s, tile + L::TILE);
+      mma_nn<T, DP, 1>(dv, s, tile + L::TILE);
 #pragma unroll
       for (int n = 0; n < KB / 8; ++n) {
         const float2 delta = *reinterpret_cast<const float2*>(&sh.key_delta[slot][n * 8 + c2]);
-        dp[n][0] = dp[n][2] = -delta.x;
-        dp[n][1] = dp[n][3] = -delta.y;
+        dp[0][n][0] = dp[0][n][2] = -delta.x;
+        dp[0][n][1] = dp[0][n][3] = -delta.y;
       }
-      mma_nt<T, DP, KB>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
+      mma_nt<T, DP, 1>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
 #pragma unroll
       for (int n = 0; n < KB / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float ds = s[n][e] * dp[n][e];
+          float ds = s[0][n][e] * dp[0][n][e];
           // a weight of zero may stand for a row of another window, which may hold anything
-          if (!whole && s[n][e] == 0.f) ds = 0.f;
-          dp[n][e] = ds;
+          if (!whole && s[0][n][e] == 0.f) ds = 0.f;
+          dp[0][n][e] = ds;
           if constexpr (TABLE) most = max_nan(most, fabsf(ds));
         }
-      mma_nn<T, DP, KB>(dk, dp, tile);
+      mma_nn<T, DP, 1>(dk, dp, tile);
     };
-    walk<true>(
+    walk<true, STAGES>(
         b,
         [&](int buf, const int32_t* rows) {
           uint8_t* tile = smem + L::RING + buf * 2 * L::TILE;
-          load_tile<T, DP, KB>(tile, q, a.q_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile, q, (int)a.q_row, rows, a.dim, vec);
           load_tile<T, DP, KB>(tile + L::TILE, dout, g_row, rows, a.dim, vec);
         },
         body, [] { return false; }, [] {});
-    store_rows<T, DP>(smem, dk, a.scale, a.scale, sh.own_row, static_cast<T*>(a.dk), a.heads, head,
-                      a.dim, vec);
-    store_rows<T, DP>(smem + L::OWN_TILE, dv, 1.f, 1.f, sh.own_row, static_cast<T*>(a.dv), a.heads,
-                      head, a.dim, vec);
-    again(not_finite<DP>(dk) | not_finite<DP>(dv), t64 * BQ + warp * 16, mine,
+    store_rows<T, DP>(mine, dk[0], a.scale, a.scale, sh.own_row + warp * 16, static_cast<T*>(a.dk),
+                      a.heads, head, a.dim, vec);
+    store_rows<T, DP>(mine + L::OWN_TILE, dv[0], 1.f, 1.f, sh.own_row + warp * 16,
+                      static_cast<T*>(a.dv), a.heads, head, a.dim, vec);
+    again(not_finite<DP>(dk[0]) | not_finite<DP>(dv[0]), block * BQ + warp * 16, mine,
           [&](int64_t p, float* f) { if (p < a.n) again_dkv<T>(a, p, head, f); });
     __syncthreads();
   }
@@ -914,11 +1024,11 @@ bool wide_rows(const AttnArgs& a) {
          wide(a.dq, row, head) && wide(a.dk, row, head) && wide(a.dv, row, head);
 }
 
-// 64-row tiles of one head that a block takes in turn, so that it stages the table (and adds up its
-// gradient) once: as many as still leave `waves` blocks for each of an SM's places.
-int tiles_per_block(const AttnArgs& a, int waves) {
-  const int64_t tiles = (a.n + BQ - 1) / BQ;
-  const int64_t per = tiles * a.heads / ((int64_t)num_sms() * waves);
+// Blocks of BQ rows of one head that a CTA takes in turn, so that it stages the table (and adds up its
+// gradient) once: as many as still leave `waves` CTAs for each SM.
+int blocks_per_cta(const AttnArgs& a, int bq, int waves) {
+  const int64_t blocks = (a.n + bq - 1) / bq;
+  const int64_t per = blocks * a.heads / ((int64_t)num_sms() * waves);
   return (int)(per < 1 ? 1 : (per > 16 ? 16 : per));
 }
 
@@ -929,38 +1039,40 @@ int allow_smem(K kernel, size_t bytes) {
   return SV_OK;
 }
 
-constexpr int KB = 32;  // positions of a tile
-
 template <typename T, int DP>
 int forward(const AttnArgs& a, cudaStream_t s) {
-  const size_t bytes = Layout<DP, KB, 1>::TABLE + tables(a, false).total;
-  const int rc = allow_smem(attn_tc_kernel<T, DP, KB>, bytes);
+  // two 16-row parts a warp where their sums fit the registers
+  constexpr int MR = DP <= 64 ? 2 : 1, STAGES = DP <= 64 ? 3 : 2;
+  const size_t bytes = Layout<DP, 64 * MR, 1, STAGES>::TABLE + tables(a, false).total;
+  const int rc = allow_smem(attn_tc_kernel<T, DP, MR, STAGES>, bytes);
   if (rc != SV_OK) return rc;
-  const int per = tiles_per_block(a, 12);
-  const int64_t blocks = ((a.n + BQ - 1) / BQ + per - 1) / per;
-  attn_tc_kernel<T, DP, KB><<<dim3((unsigned)blocks, a.heads), AT, bytes, s>>>(a, per,
-                                                                               wide_rows(a));
+  const int per = blocks_per_cta(a, 64 * MR, 9);
+  const int64_t ctas = ((a.n + 64 * MR - 1) / (64 * MR) + per - 1) / per;
+  attn_tc_kernel<T, DP, MR, STAGES>
+      <<<dim3((unsigned)ctas, a.heads), AT, bytes, s>>>(a, per, wide_rows(a));
   SV_LAUNCH_CHECK();
   return SV_OK;
 }
 
 template <typename T, int DP, bool TABLE>
 int backward(const AttnArgs& a, void* dtable, cudaStream_t s) {
+  constexpr int STAGES = 2;
+  using L = Layout<DP, 64, 2, STAGES>;
   const bool vec = wide_rows(a);
   attn_delta_kernel<T><<<(unsigned)((a.n * a.heads + 31) / 32), 256, 0, s>>>(
       a, vec && aligned16(a.o));
   SV_LAUNCH_CHECK();
-  const int per = tiles_per_block(a, 6);
-  const dim3 grid((unsigned)(((a.n + BQ - 1) / BQ + per - 1) / per), a.heads);
-  size_t bytes = Layout<DP, KB, 2>::TABLE + tables(a, false).total;
-  int rc = allow_smem(attn_dkv_tc_kernel<T, DP, KB, TABLE>, bytes);
+  const int per = blocks_per_cta(a, 64, 6);
+  const dim3 grid((unsigned)(((a.n + 63) / 64 + per - 1) / per), a.heads);
+  size_t bytes = L::TABLE + tables(a, false).total;
+  int rc = allow_smem(attn_dkv_tc_kernel<T, DP, STAGES, TABLE>, bytes);
   if (rc != SV_OK) return rc;
-  attn_dkv_tc_kernel<T, DP, KB, TABLE><<<grid, AT, bytes, s>>>(a, per, vec);
+  attn_dkv_tc_kernel<T, DP, STAGES, TABLE><<<grid, AT, bytes, s>>>(a, per, vec);
   SV_LAUNCH_CHECK();
-  bytes = Layout<DP, KB, 2>::TABLE + tables(a, TABLE).total;
-  rc = allow_smem(attn_dq_tc_kernel<T, DP, KB, TABLE>, bytes);
+  bytes = L::TABLE + tables(a, TABLE).total;
+  rc = allow_smem(attn_dq_tc_kernel<T, DP, STAGES, TABLE>, bytes);
   if (rc != SV_OK) return rc;
-  attn_dq_tc_kernel<T, DP, KB, TABLE><<<grid, AT, bytes, s>>>(a, per, vec);
+  attn_dq_tc_kernel<T, DP, STAGES, TABLE><<<grid, AT, bytes, s>>>(a, per, vec);
   SV_LAUNCH_CHECK();
   if constexpr (TABLE) {
     const unsigned blocks = (unsigned)((a.nb * a.nb * a.nb + 255) / 256);
