@@ -1062,7 +1062,7 @@ int backward(const AttnArgs& a, void* dtable, cudaStream_t s) {
   attn_delta_kernel<T><<<(unsigned)((a.n * a.heads + 31) / 32), 256, 0, s>>>(
       a, vec && aligned16(a.o));
   SV_LAUNCH_CHECK();
-  const int per = blocks_per_cta(a, 64, 6);
+  const int per = blocks_per_cta(a, 64, 9);
   const dim3 grid((unsigned)(((a.n + 63) / 64 + per - 1) / per), a.heads);
   size_t bytes = L::TABLE + tables(a, false).total;
   int rc = allow_smem(attn_dkv_tc_kernel<T, DP, STAGES, TABLE>, bytes);
