@@ -451,14 +451,14 @@ SV_API int sv_window_plan(const int32_t* coords, const int32_t* perm, const int3
  *   s_ij = scale q_i . k_j + table[h][lut[dx]][lut[dy]][lut[dz]], softmax over the window, o = p v.
  * dx, dy, dz: the key's coordinates minus the query's, clamped to +-reach (<= 1023); lut: int32
  * [2 reach + 1], values in [0, buckets) (others are clamped); table: [heads, buckets^3] in `dtype`,
- * buckets <= 23. `strides`: row and head strides of q, k, v in elements, channels contiguous.
+ * buckets <= 25. `strides`: row and head strides of q, k, v in elements, channels contiguous.
  * out: contiguous. stats (or null): fp32 [heads, n, 2] by position, 8-byte aligned: the softmax's
  * maximum and 1 / sum, for the backward pass. A row whose every score is -inf gives zeros. */
 SV_API int sv_window_attention(const void* q, const void* k, const void* v,
                                const int64_t* strides, int64_t n, int heads, int dim, int dtype,
                                const void* plan, const void* table, int buckets,
-                               const int32_t* lut, int reach, float scale, void* out, float* stats,
-                               int32_t* status, sv_stream_t stream);
+                               const int32_t* lut, int reach, float scale, void* out, float* lse,
+                               sv_stream_t stream);
 
 /* Its gradients, from the forward pass's out (`o`) and stats: dq, dk, dv contiguous, and dtable
  * [heads, buckets^3] (null: not wanted), whose sums do not depend on the order of execution. */
@@ -467,8 +467,7 @@ SV_API int sv_window_attention_backward(
     const void* q, const void* k, const void* v, const int64_t* strides, const void* o,
     const void* dout, const float* stats, int64_t n, int heads, int dim, int dtype, const void* plan,
     const void* table, int buckets, const int32_t* lut, int reach, float scale, void* dq, void* dk,
-    void* dv, void* dtable, void* workspace, size_t workspace_bytes, int32_t* status,
-    sv_stream_t stream);
+    void* dv, void* dtable, void* workspace, size_t workspace_bytes, sv_stream_t stream);
 
 /* ---- topology: occupancy -> coordinates, subdivision, attention windows --------------- */
 

@@ -186,7 +186,7 @@ int check(int64_t n, int heads, int dim, int dtype, int nb, int reach, const cha
       reach > ATTN_MAX_REACH)
     SV_FAIL(SV_ERR_UNSUPPORTED,
             std::string(what) +
-                ": at most 2^25 rows, 65535 heads, 128 channels a head, 23 buckets an axis and a "
+                ": at most 2^25 rows, 65535 heads, 128 channels a head, 25 buckets an axis and a "
                 "reach of 1023");
   return SV_OK;
 }
@@ -239,7 +239,7 @@ extern "C" int sv_window_attention(const void* q, const void* k, const void* v,
                                    const int64_t* strides, int64_t n, int heads, int dim,
                                    int dtype, const void* plan, const void* table, int buckets,
                                    const int32_t* lut, int reach, float scale, void* out,
-                                   float* stats, int32_t* status, sv_stream_t stream) {
+                                   float* stats, sv_stream_t stream) {
   const int rc = check(n, heads, dim, dtype, buckets, reach, "sv_window_attention");
   if (rc != SV_OK) return rc;
   if (n == 0 || heads == 0 || dim == 0) return SV_OK;
@@ -256,7 +256,7 @@ extern "C" int sv_window_attention(const void* q, const void* k, const void* v,
   a.table = table; a.lut = lut; a.stats = reinterpret_cast<float2*>(stats);
   a.n = n; a.heads = heads; a.dim = dim; a.nb = buckets; a.reach = reach; a.scale = scale;
   cudaStream_t s = to_stream(stream);
-  if (dtype != SV_FLOAT32) return attention_tc_forward(a, dtype == SV_BFLOAT16, status, s);
+  if (dtype != SV_FLOAT32) return attention_tc_forward(a, dtype == SV_BFLOAT16, s);
   attn_rows_kernel<float><<<row_grid(a), 32 * ROW_WARPS, 0, s>>>(a);
   SV_LAUNCH_CHECK();
   return SV_OK;
@@ -271,8 +271,7 @@ extern "C" int sv_window_attention_backward(
     const void* q, const void* k, const void* v, const int64_t* strides, const void* o,
     const void* dout, const float* stats, int64_t n, int heads, int dim, int dtype, const void* plan,
     const void* table, int buckets, const int32_t* lut, int reach, float scale, void* dq, void* dk,
-    void* dv, void* dtable, void* workspace, size_t workspace_bytes, int32_t* status,
-    sv_stream_t stream) {
+    void* dv, void* dtable, void* workspace, size_t workspace_bytes, sv_stream_t stream) {
   const int rc = check(n, heads, dim, dtype, buckets, reach, "sv_window_attention_backward");
   if (rc != SV_OK) return rc;
   cudaStream_t s = to_stream(stream);
@@ -307,5 +306,5 @@ extern "C" int sv_window_attention_backward(
     SV_CUDA_TRY(cudaMemsetAsync(ws, 0, l.delta, s));  // the table and the norms
   }
   if (dtype == SV_FLOAT32) return backward_rows(a, dtable, s);
-  return attention_tc_backward(a, dtype == SV_BFLOAT16, dtable, status, s);
+  return attention_tc_backward(a, dtype == SV_BFLOAT16, dtable, s);
 }

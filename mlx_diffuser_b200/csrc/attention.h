@@ -8,15 +8,14 @@
 namespace sv {
 
 constexpr int ATTN_MAX_DIM = 128;
-constexpr int ATTN_MAX_BUCKETS = 23;   // per axis
+constexpr int ATTN_MAX_BUCKETS = 25;   // per axis
 constexpr int ATTN_MAX_REACH = 1023;   // offsets beyond it share the outermost entries
 constexpr int ATTN_MAX_HEADS = 65535;
 
 // attention_tc.cu: the fp16 / bf16 kernels.
 struct AttnArgs;
-int attention_tc_forward(const AttnArgs& a, bool bf16, int32_t* status, cudaStream_t s);
-int attention_tc_backward(const AttnArgs& a, bool bf16, void* dtable, int32_t* status,
-                          cudaStream_t s);
+int attention_tc_forward(const AttnArgs& a, bool bf16, cudaStream_t s);
+int attention_tc_backward(const AttnArgs& a, bool bf16, void* dtable, cudaStream_t s);
 
 // One row of the attention plan, in window order: the coordinates, the window's range of
 // positions, and the feature row.

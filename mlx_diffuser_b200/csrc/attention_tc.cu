@@ -1,31 +1,20 @@
-// Windowed attention with a learned relative position bias in fp16 / bf16, on the 5th-generation
-// tensor cores.
+// Windowed attention with a learned relative position bias in fp16 / bf16, on the tensor cores.
 //
-// The formulas are attention.cu's. A CTA takes 128 rows in window order (queries, or keys for dk and
-// dv) of one head and walks the positions that any of their windows covers in tiles of KB: rows of
-// several small windows share a tile. The scores of a tile are one product into TMEM; a thread owns a row
-// of them, so the softmax needs no exchange between lanes, and writes the weights back to TMEM, where
-// they are the left operand of the second product:
-//   forward   S = Q K^T            o  += P V
-//   dq        S = Q K^T, D = dO V^T     dq += dS K, and the table's gradient
-//   dk, dv    S = K Q^T, D = V dO^T     dv += P dO, dk += dS Q   (transposed: rows are keys)
-// The right operands of the second products are the tiles of the first, read along the other axis.
+// The formulas are attention.cu's. A block takes 64 rows in window order (queries, or keys for dk and
+// dv) of one head, four warps of 16, and walks the positions that any of their windows covers in
+// tiles of 64: rows of several small windows share a tile, and a warp skips the tiles that none of
+// its own rows' windows reach. Scores stay in registers from the product to the softmax to the next
+// product (the accumulator's layout is the operand's), so the running maximum and sum are the only
+// state. The gathered rows arrive by cp.async, one tile ahead.
 //
-// What bounds it is the work a score needs besides the products: its bucket, the look-up, an
-// exponential, the running sums, about ten instructions; the products are a tenth of that time on
-// tcgen05. Fragments of warp-level mma.sync instead took 37 instructions a score for loads,
-// conversions and exchanges (40,662 voxels x 768 channels, 8^3 windows, bf16: 279 us).
+// Products are warp-level mma.sync: a window of a surface holds 100-300 rows, so a tile's two
+// products are a few hundred cycles, while each of its 4096 scores needs an exponential and a table
+// look-up of its own. The look-up, not the product, is what a faster matrix instruction would wait
+// for, and the register layout makes the bias and the softmax free of shared-memory round trips.
 //
 // The bucket of a pair: where the table is one entry per offset (the look-up is the identity) and
 // the windows are no wider than its reach, it is linear in the coordinates and costs a subtraction;
-// within the reach the look-ups of x and y are joined in one; otherwise three look-ups.
-//
-// Warp roles (224 threads, two CTAs an SM where shared memory and TMEM allow it):
-//   warps 0-3   a row a thread: scores, softmax, score gradients, results;
-//   warp 4      TMEM allocator and the tcgen05.mma issuer;
-//   warps 5, 6  gather the rows of the block and of the tiles by cp.async into 128-byte-swizzled
-//               panels of 64 channels, a few tiles ahead.
-// Every wait is bounded (2 s, CTA abort flag); on expiry SV_DEVICE_WAIT_TIMEOUT is reported.
+// otherwise three look-ups.
 //
 // Weights and score gradients are rounded to the feature type as operands of the second products
 // (half a step each, like the stored results); the softmax sums and the table's gradient use them
@@ -39,33 +28,39 @@
 namespace sv {
 namespace {
 
-constexpr int BQ = 128;        // rows of a block: the TMEM lanes
-constexpr int AT = 224;        // threads: with seven warps a CTA, two CTAs get 128 registers a thread
-constexpr int LOADERS = 64;    // of them, warps 5 and 6
-constexpr int PANEL = 128;     // bytes of a row in a panel: 64 channels
+constexpr int AT = 128;  // threads: four warps of 16 rows, or of 16 MR
+constexpr int KB = 32;   // positions of a tile
 
-enum { FWD = 0, DQ = 1, DKV = 2 };
+// Tiles hold DP channels a row (the head's, padded with zeros) at a stride that is an odd multiple
+// of 16 bytes, so the 8 rows of a matrix fragment fall into different banks.
+template <int DP>
+constexpr int STRIDE = DP * 2 + 16;
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
 }
-// max that keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float m;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-  return m;
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
 }
-__device__ __forceinline__ float lds_f32(uint32_t at) {
-  float v;
-  asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
-  uint16_t v;
-  asm("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
-  return v;
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 template <typename T>
@@ -79,174 +74,431 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
-__device__ __forceinline__ void arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// D[tmem] (+)= A[tmem] * B[smem]^T.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t more) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(more)
-      : "memory");
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// 32 lanes x 16 / 8 consecutive 32-bit columns from registers.
-__device__ __forceinline__ void tmem_st_x16(uint32_t at, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
-      " {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_x8(uint32_t at, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at),
-               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-               "r"(r[7])
-               : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+// max that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
 }
 
-constexpr int CH = 16;  // columns of scores a row thread works on at a time: code that stays in the
-                        // instruction cache, where whole tiles unrolled starved on fetches
-
-template <typename T>
-__device__ __forceinline__ void store_weights(uint32_t at, const float (&v)[CH]) {
-  uint32_t r[CH / 2];
+// R gathered rows of one head into a tile; rows of -1 and channels past `dim` become zeros.
+template <typename T, int DP, int R>
+__device__ __forceinline__ void load_tile(uint8_t* tile, const T* base, int row_stride,
+                                          const int32_t* rows, int dim, bool vec) {
+  constexpr int CH = DP / 8;  // 16-byte chunks of a row; a thread copies the same one of every row
+  static_assert(AT % CH == 0 && R * CH % AT == 0, "whole rounds");
+  if (vec) {
+    const int col = threadIdx.x % CH, r0 = threadIdx.x / CH;
+    const uint32_t at = smem_u32(tile) + r0 * STRIDE<DP> + col * 16;
+    const bool in_row = col * 8 < dim;
+    const T* from = base + (in_row ? col * 8 : 0);
 #pragma unroll
-  for (int i = 0; i < CH / 2; ++i) r[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-  tmem_st_x8(at, r);
+    for (int i = 0; i < R * CH / AT; ++i) {
+      const int32_t row = rows[r0 + i * (AT / CH)];
+      cp_async_16(at + i * (AT / CH) * STRIDE<DP>, from + (int64_t)max(row, 0) * row_stride,
+                  row >= 0 && in_row ? 16u : 0u);
+    }
+  } else {
+    for (int c = threadIdx.x; c < R * DP; c += AT) {
+      const int r = c / DP, col = c % DP;
+      const int32_t row = rows[r];
+      T v = from_f32<T>(0.f);
+      if (row >= 0 && col < dim) v = base[(int64_t)row * row_stride + col];
+      *reinterpret_cast<T*>(tile + r * STRIDE<DP> + col * 2) = v;
+    }
+  }
 }
 
-// The other side's rows of a tile, as the row threads read them.
-template <int KB>
-struct alignas(16) Meta {
-  int32_t lin[KB];     // LINEAR: 4 ((x nb + y) nb + z)
-  int2 joint[KB];      // JOINT: 2 (x width + y), 2 z
-  int4 xyzr[KB];       // coordinates and row (-1: none)
-  float top[KB], inv[KB], delta[KB];  // their softmax and delta (dk / dv)
-  uint32_t rows[KB / 32];              // bit c: position c of 32 has a row
+// A 16-row accumulator through the warp's own part of a tile (`mine`) to the feature rows `rows`, in
+// 16-byte stores.
+template <typename T, int DP>
+__device__ __forceinline__ void store_rows(uint8_t* mine, const float (&o)[DP / 8][4], float s0,
+                                           float s1, const int32_t* rows, T* out, int heads,
+                                           int head, int dim, bool vec) {
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2, c2 = 2 * (lane & 3);
+  __syncwarp();
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n) {
+    *reinterpret_cast<uint32_t*>(mine + g * STRIDE<DP> + (n * 8 + c2) * 2) =
+        pack2<T>(o[n][0] * s0, o[n][1] * s0);
+    *reinterpret_cast<uint32_t*>(mine + (g + 8) * STRIDE<DP> + (n * 8 + c2) * 2) =
+        pack2<T>(o[n][2] * s1, o[n][3] * s1);
+  }
+  __syncwarp();
+  constexpr int CH = DP / 8;
+#pragma unroll
+  for (int i = 0; i < 16 * CH / 32; ++i) {
+    const int c = lane + 32 * i;
+    const int r = c / CH, col = c % CH;
+    const int32_t row = rows[r];
+    if (row < 0) continue;
+    T* dst = out + ((int64_t)row * heads + head) * dim + col * 8;
+    const uint4 v = *reinterpret_cast<const uint4*>(mine + r * STRIDE<DP> + col * 16);
+    if (vec) {
+      if (col * 8 < dim) *reinterpret_cast<uint4*>(dst) = v;
+    } else {
+      const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (col * 8 + k < dim) dst[k] = e[k];
+    }
+  }
+}
+
+struct KeyMeta {
+  int32_t x, y, z, row;  // row -1: no row
 };
 
-// How a pair's bucket is found; all indexes are byte offsets.
+constexpr int SLOTS = 4;  // tiles whose rows are known: the one worked on and three ahead
+
+// What every kernel here keeps in shared memory besides its tiles; BQ rows of the block's own.
+template <int BQ>
+struct alignas(16) Shared {
+  KeyMeta key[SLOTS][KB];       // the other side's rows
+  int2 key_lin[SLOTS][KB];      // their linear coordinates (Block::lin)
+  int32_t key_row[SLOTS][KB];
+  float2 key_stats[SLOTS][KB];  // their softmax and delta (dk / dv)
+  float key_delta[SLOTS][KB];
+  int32_t key_bad[SLOTS];       // whether a position has no row
+  PlanRow own[BQ];
+  int32_t own_row[BQ];
+  int32_t range[2];
+};
+
+// How a pair's bucket is found. LINEAR: the look-up is the identity and the windows are within the
+// table's reach, so the bucket is a difference of linear coordinates. JOINT: within the reach, and
+// the look-ups of x and y are joined in one table of all their offsets. GENERAL: any. All indexes are
+// kept as byte offsets.
 enum { GENERAL = 0, JOINT = 1, LINEAR = 2 };
 constexpr int JOINT_MAX = 4096;
 
-struct Tables {
-  int grad, lut, joint, total;  // byte offsets behind the table; joint < 0: none
-};
-__host__ __device__ inline Tables tables(const AttnArgs& a, bool grad) {
-  const int cells = a.nb * a.nb * a.nb, width = 2 * a.reach + 1;
-  Tables t;
-  t.grad = cells * 4;
-  t.lut = t.grad + (grad ? cells * 4 : 0);
-  t.joint = -1;
-  t.total = t.lut + (width * 2 + 15) / 16 * 16;
-  if (width * width <= JOINT_MAX) {
-    t.joint = t.total;
-    t.total += width * width * 2;
+__device__ __forceinline__ float lds_f32(uint32_t at) {
+  float v;
+  asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
+  uint16_t v;
+  asm("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+  return v;
+}
+
+template <typename T, int BQ>
+struct Block {
+  const AttnArgs& a;
+  Shared<BQ>& s;
+  float* table;      // [nb^3] times log2(e)
+  uint16_t* lut;     // [2 reach + 1], times 4
+  uint16_t* joint;   // [(2 reach + 1)^2]: x and y buckets' offset in the table, or null
+  int head;
+  bool identity;
+  float delta_top;   // largest |delta| staged by this thread
+  // set per BQ rows
+  int mode;
+  int j0, tiles;
+
+  __device__ __forceinline__ int cells() const { return a.nb * a.nb * a.nb; }
+  __device__ __forceinline__ int width() const { return 2 * a.reach + 1; }
+
+  // LINEAR: 4 ((x nb + y) nb + z); JOINT: 2 (x width + y) and 2 z. Wrap-around is harmless: only
+  // differences inside a window are used.
+  __device__ __forceinline__ int2 lin(int x, int y, int z) const {
+    if (mode == LINEAR)
+      return make_int2((int)((((unsigned)x * a.nb + (unsigned)y) * a.nb + (unsigned)z) * 4u), 0);
+    return make_int2((int)(((unsigned)x * width() + (unsigned)y) * 2u), (int)((unsigned)z * 2u));
   }
-  return t;
-}
 
-// Shared memory and TMEM of one kernel. PANELS of 64 channels a row; TILES of the block's own rows.
-template <int MODE, int PANELS, int KB>
-struct Plan {
-  static constexpr int OWN = MODE == FWD ? 1 : 2;
-  static constexpr int STAGES = MODE == FWD && PANELS == 1 ? 3 : 2;
-  static constexpr int BUFS = MODE == FWD ? 2 : 1;  // score buffers in TMEM
-  static constexpr int OWN_PANEL = BQ * PANEL;
-  static constexpr int OWN_TILE = PANELS * OWN_PANEL;
-  static constexpr int TILE_PANEL = KB * PANEL;
-  static constexpr int TILE = PANELS * TILE_PANEL;
-  static constexpr int RING = OWN * OWN_TILE;
-  static constexpr int META = RING + STAGES * 2 * TILE;
-  static constexpr int SCRATCH = META + STAGES * (int)sizeof(Meta<KB>);
-  static constexpr int MISC = SCRATCH + 4 * 2 * ATTN_MAX_DIM * 4;
-  static constexpr int NUM_BARS = 2 * STAGES + 3 * BUFS + 3;
-  static constexpr int TABLE = (MISC + 32 + NUM_BARS * 8 + 15) / 16 * 16;
-  // TMEM columns: sums, then the score buffers
-  static constexpr int ACC = 64 * PANELS;
-  static constexpr int SCORES = (MODE == DKV ? 2 : 1) * ACC;
-  // A buffer: S and, forward, the weights beside it (a tile may be done again with another base);
-  // else S and D, whose weights and gradients take their place as they are read.
-  static constexpr int SCORE_COLS = MODE == FWD ? KB + KB / 2 : 2 * KB;
-  static constexpr int WEIGHTS = MODE == FWD ? KB : 0;
-  static constexpr int USED = SCORES + BUFS * SCORE_COLS;
-  static constexpr int COLS = USED <= 256 ? 256 : 512;
-  static_assert(USED <= 512, "TMEM columns");
-  static constexpr int CTAS = COLS == 256 ? 2 : 1;
-};
-
-// A row thread's own row and how it finds buckets.
-struct Own {
-  PlanRow p;
-  int lin, joint_xy, joint_z;
-};
-
-struct Look {
-  uint32_t table, lut, joint;  // shared-memory addresses
-  int nb, reach, mode;
-  uint32_t top, joint_top, z_top;  // largest byte offsets
-};
-
-__device__ __forceinline__ uint32_t bucket3(const Look& l, int qx, int qy, int qz, int kx, int ky,
-                                            int kz) {
-  const int R = l.reach;
-  const int x = lds_u16(l.lut + 2 * (max(-R, min(R, sub_sat(kx, qx))) + R));
-  const int y = lds_u16(l.lut + 2 * (max(-R, min(R, sub_sat(ky, qy))) + R));
-  const int z = lds_u16(l.lut + 2 * (max(-R, min(R, sub_sat(kz, qz))) + R));
-  return (uint32_t)((x * l.nb + y) * l.nb + z);
-}
-
-// The pairs' byte offsets in the table for the CH columns c0 .. of a tile. FLIP: the thread's row is
-// the key and the columns are queries. Outside a window (masked later) they are clamped; inside, the
-// clamp changes nothing.
-template <bool FLIP, int KB>
-__device__ __forceinline__ void buckets(const Look& l, const Meta<KB>& m, const Own& o, int c0,
-                                        uint32_t (&at)[CH]) {
-  if (l.mode == LINEAR) {
-#pragma unroll
-    for (int c = 0; c < CH; c += 4) {
-      const int4 k = *reinterpret_cast<const int4*>(&m.lin[c0 + c]);
-      const int v[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        at[c + e] = min((uint32_t)(FLIP ? o.lin - v[e] : v[e] - o.lin), l.top);
+  __device__ void stage_tables() {
+    const T* src = static_cast<const T*>(a.table) + (int64_t)head * cells();
+#pragma unroll 8
+    for (int i = threadIdx.x; i < cells(); i += AT) table[i] = times_log2e(to_f32(src[i]));
+    bool same = a.nb == width();
+    for (int i = threadIdx.x; i < width(); i += AT) {
+      const int v = max(0, min(a.nb - 1, __ldg(a.lut + i)));
+      lut[i] = (uint16_t)(4 * v);
+      same = same && v == i;
     }
-  } else if (l.mode == JOINT) {
+    identity = __syncthreads_and(same);
+    if (!identity && joint != nullptr)
+      for (int i = threadIdx.x; i < width() * width(); i += AT)
+        joint[i] = (uint16_t)((lut[i / width()] * a.nb + lut[i % width()]) * a.nb);
+  }
+
+  // The block's rows and the positions their windows cover.
+  __device__ void begin(int64_t p0) {
+    if (threadIdx.x < 2) s.range[threadIdx.x] = threadIdx.x ? INT_MIN : INT_MAX;
+    __syncthreads();
+    bool narrow = true;
+    if (threadIdx.x < BQ) {
+      const int64_t p = p0 + threadIdx.x;
+      PlanRow r{};
+      r.row = -1;
+      if (p < a.n) r = plan_at(a.plan, p);
+      if (r.row < 0) {
+        r.start = r.end = 0;
+      } else {
+        atomicMin(&s.range[0], r.start);
+        atomicMax(&s.range[1], r.end);
+        narrow = r.span <= a.reach;
+      }
+      s.own[threadIdx.x] = r;
+      s.own_row[threadIdx.x] = r.row;
+    }
+    narrow = __syncthreads_and(narrow);
+    mode = !narrow ? GENERAL : (identity ? LINEAR : (joint != nullptr ? JOINT : GENERAL));
+    j0 = s.range[0];
+    tiles = s.range[1] > j0 ? (s.range[1] - j0 + KB - 1) / KB : 0;
+  }
+
+  // By one warp: a position a lane.
+  template <bool STATS>
+  __device__ void stage_meta(int t) {
+    static_assert(KB == 32, "a position a lane");
+    const int slot = t % SLOTS;
+    const int i = threadIdx.x & 31;
+    const int j = j0 + t * KB + i;
+    KeyMeta m{0, 0, 0, -1};
+    if (j < s.range[1])
+      *reinterpret_cast<int4*>(&m) = __ldg(reinterpret_cast<const int4*>(a.plan + j));
+    if constexpr (STATS) {
+      float2 st = make_float2(0.f, 0.f);
+      float d = 0.f;
+      if (m.row >= 0) {
+        st = a.stats[head * a.n + j];
+        d = a.delta[head * a.n + j];
+      }
+      s.key_stats[slot][i] = st;
+      s.key_delta[slot][i] = d;
+      delta_top = max_nan(delta_top, fabsf(d));
+    }
+    const unsigned bad = __ballot_sync(0xffffffffu, j < s.range[1] && m.row < 0);
+    if (i == 0) s.key_bad[slot] = bad != 0;
+    s.key[slot][i] = m;
+    s.key_lin[slot][i] = lin(m.x, m.y, m.z);
+    s.key_row[slot][i] = m.row;
+  }
+
+  __device__ __forceinline__ uint32_t bucket(int qx, int qy, int qz, int kx, int ky, int kz) const {
+    const int R = a.reach;
+    const int x = lut[max(-R, min(R, sub_sat(kx, qx))) + R];
+    const int y = lut[max(-R, min(R, sub_sat(ky, qy))) + R];
+    const int z = lut[max(-R, min(R, sub_sat(kz, qz))) + R];
+    return (uint32_t)((x * a.nb + y) * a.nb + z);
+  }
+};
+
+// Calls use(n, e, at) for a thread's pairs with the pair's byte offset in the table: element e of
+// fragment n is row g + 8 (e / 2) of 16 and column 8 n + 2 (lane % 4) + e % 2. FLIP: the rows are
+// keys and the columns queries. WHOLE: all pairs are inside a window; otherwise the offsets of the
+// others (masked) are clamped.
+template <bool FLIP, bool WHOLE, typename T, int BQ, typename F>
+__device__ __forceinline__ void each_pair(const Block<T, BQ>& b, int slot, const PlanRow* own,
+                                          F&& use) {
+  const int c2 = 2 * (threadIdx.x & 3);
+  auto within = [](int v, uint32_t top) -> uint32_t {
+    return WHOLE ? (uint32_t)v : min((uint32_t)v, top);
+  };
+  if (b.mode == LINEAR) {
+    const uint32_t top = (uint32_t)b.cells() * 4u - 4u;
+    const int mid = FLIP ? (int)(top / 2) : -(int)(top / 2);
+    const int l[2] = {b.lin(own[0].x, own[0].y, own[0].z).x + mid,
+                      b.lin(own[8].x, own[8].y, own[8].z).x + mid};
 #pragma unroll
-    for (int c = 0; c < CH; c += 2) {
-      const int4 k = *reinterpret_cast<const int4*>(&m.joint[c0 + c]);
-      const int xy[2] = {k.x, k.z}, z[2] = {k.y, k.w};
+    for (int n = 0; n < KB / 8; ++n) {
+      // the linear coordinates of two neighbours: .x and .z
+      const int4 k = *reinterpret_cast<const int4*>(&b.s.key_lin[slot][n * 8 + c2]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t dxy = (uint32_t)(FLIP ? o.joint_xy - xy[e] : xy[e] - o.joint_xy);
-        const uint32_t dz = (uint32_t)(FLIP ? o.joint_z - z[e] : z[e] - o.joint_z);
-        at[c + e] = lds_u16(l.joint + min(dxy, l.joint_top)) + lds_u16(l.lut + min(dz, l.z_top));
+      for (int e = 0; e < 4; ++e) {
+        const int c = e & 1 ? k.z : k.x;
+        use(n, e, within(FLIP ? l[e >> 1] - c : c - l[e >> 1], top));
+      }
+    }
+  } else if (b.mode == JOINT) {
+    const uint32_t joint = smem_u32(b.joint), lut = smem_u32(b.lut);
+    const uint32_t top = (uint32_t)(b.width() * b.width()) * 2u - 2u;
+    const uint32_t ztop = (uint32_t)b.width() * 2u - 2u;
+    const int mid = FLIP ? (int)(top / 2) : -(int)(top / 2);
+    const int zmid = FLIP ? 2 * b.a.reach : -2 * b.a.reach;
+    int2 l[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] = b.lin(own[8 * r].x, own[8 * r].y, own[8 * r].z);
+      l[r].x += mid;
+      l[r].y += zmid;
+    }
+#pragma unroll
+    for (int n = 0; n < KB / 8; ++n) {
+      const int4 k = *reinterpret_cast<const int4*>(&b.s.key_lin[slot][n * 8 + c2]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = e & 1 ? k.z : k.x, z = e & 1 ? k.w : k.y;
+        const uint32_t xy = within(FLIP ? l[e >> 1].x - c : c - l[e >> 1].x, top);
+        const uint32_t dz = within(FLIP ? l[e >> 1].y - z : z - l[e >> 1].y, ztop);
+        use(n, e, lds_u16(joint + xy) + lds_u16(lut + dz));
       }
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int4 k = m.xyzr[c0 + c];
-      at[c] = FLIP ? bucket3(l, k.x, k.y, k.z, o.p.x, o.p.y, o.p.z)
-                   : bucket3(l, o.p.x, o.p.y, o.p.z, k.x, k.y, k.z);
+    for (int n = 0; n < KB / 8; ++n) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const KeyMeta k = b.s.key[slot][n * 8 + c2 + c];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const PlanRow& o = own[8 * r];
+          use(n, 2 * r + c, FLIP ? b.bucket(k.x, k.y, k.z, o.x, o.y, o.z)
+                                 : b.bucket(o.x, o.y, o.z, k.x, k.y, k.z));
+        }
+      }
     }
   }
 }
 
-// Bits of the CH columns c0 .. that a row with columns lo .. hi - 1 in its window sees.
-constexpr uint32_t ALL_SEEN = (1u << CH) - 1u;
-__device__ __forceinline__ uint32_t seen_bits(int lo, int hi, int c0) {
-  const int l = max(0, min(CH, lo - c0)), h = max(0, min(CH, hi - c0));
-  return ((1u << h) - 1u) & ~((1u << l) - 1u);
+// acc += rows x tile^T over DP channels, 16 MR rows by KB columns; the rows' fragments come from
+// `rows` (the warp's rows of a tile).
+template <typename T, int DP, int MR>
+__device__ __forceinline__ void mma_nt(float (&acc)[MR][KB / 8][4], uint32_t rows, uint32_t tile) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t from = rows + (lane & 15) * STRIDE<DP> + (lane >> 4) * 16;
+  const uint32_t at = tile + ((lane & 7) + (lane >> 4) * 8) * STRIDE<DP> + ((lane >> 3) & 1) * 16;
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    uint32_t f[MR][4];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) ldsm4(from + m * 16 * STRIDE<DP> + k * 32, f[m]);
+#pragma unroll
+    for (int n = 0; n < KB / 16; ++n) {
+      uint32_t b[4];
+      ldsm4(at + n * 16 * STRIDE<DP> + k * 32, b);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        mma<T>(acc[m][2 * n], f[m], b[0], b[1]);
+        mma<T>(acc[m][2 * n + 1], f[m], b[2], b[3]);
+      }
+    }
+  }
+}
+
+// out += w (16 MR x KB sums, rounded to T as operand fragments) x tile (KB x DP).
+template <typename T, int DP, int MR>
+__device__ __forceinline__ void mma_nn(float (&out)[MR][DP / 8][4],
+                                       const float (&w)[MR][KB / 8][4], uint32_t tile) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t at = tile + ((lane & 7) + ((lane >> 3) & 1) * 8) * STRIDE<DP> + (lane >> 4) * 16;
+#pragma unroll
+  for (int k = 0; k < KB / 16; ++k) {
+    uint32_t f[MR][4];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      f[m][0] = pack2<T>(w[m][2 * k][0], w[m][2 * k][1]);
+      f[m][1] = pack2<T>(w[m][2 * k][2], w[m][2 * k][3]);
+      f[m][2] = pack2<T>(w[m][2 * k + 1][0], w[m][2 * k + 1][1]);
+      f[m][3] = pack2<T>(w[m][2 * k + 1][2], w[m][2 * k + 1][3]);
+    }
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) {
+      uint32_t b[4];
+      ldsm4_t(at + k * 16 * STRIDE<DP> + n * 32, b);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        mma<T>(out[m][2 * n], f[m], b[0], b[1]);
+        mma<T>(out[m][2 * n + 1], f[m], b[2], b[3]);
+      }
+    }
+  }
+}
+
+template <int W>
+__device__ __forceinline__ void zero(float (&x)[W][4]) {
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
+}
+
+// Positions that any of a warp's ROWS rows sees, and those that all of them do.
+struct Reach {
+  int lo, hi, all_lo, all_hi;
+};
+template <int ROWS>
+__device__ __forceinline__ Reach warp_reach(const PlanRow* own) {
+  const int lane = threadIdx.x & 31;
+  const PlanRow& r = own[lane % ROWS];
+  const bool any = r.end > r.start;
+  Reach w;
+  w.lo = __reduce_min_sync(0xffffffffu, any ? r.start : INT_MAX);
+  w.hi = __reduce_max_sync(0xffffffffu, any ? r.end : INT_MIN);
+  w.all_lo = __reduce_max_sync(0xffffffffu, r.start);
+  w.all_hi = __reduce_min_sync(0xffffffffu, r.end);
+  return w;
+}
+
+// The columns of a thread's fragments that the rows g and g + 8 see, relative to its own first
+// column: element (n, e) is column 8 n + e % 2 of row e / 2.
+struct Sight {
+  int lo[2], hi[2];
+};
+__device__ __forceinline__ Sight sight(const PlanRow* own, int p0) {
+  const int c2 = 2 * (threadIdx.x & 3);
+  Sight v;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    v.lo[r] = own[8 * r].start - p0 - c2;
+    v.hi[r] = own[8 * r].end - p0 - c2;
+  }
+  return v;
+}
+// `bad`: some column has no row.
+template <int BQ>
+__device__ __forceinline__ bool hidden(const Sight& v, int n, int e, bool bad, const Shared<BQ>& s,
+                                       int slot) {
+  const int col = 8 * n + (e & 1);
+  bool out = (col < v.lo[e >> 1]) | (col >= v.hi[e >> 1]);
+  if (bad) out |= s.key_row[slot][col + 2 * (threadIdx.x & 3)] < 0;
+  return out;
+}
+
+// A weight of zero does not hide a NaN or an infinity that another window's row brings into a tile,
+// and fp16 score gradients can overflow where their sums do not. So rows that come out not finite
+// are computed again, one at a time, from their own windows alone.
+template <int DP>
+__device__ __forceinline__ uint32_t not_finite(const float (&o)[DP / 8][4]) {
+  bool bad[2] = {false, false};
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bad[e >> 1] = bad[e >> 1] || !(fabsf(o[n][e]) < INFINITY);
+  const unsigned b0 = __ballot_sync(0xffffffffu, bad[0]);
+  const unsigned b1 = __ballot_sync(0xffffffffu, bad[1]);
+  uint32_t rows = 0;  // bit r: row r of the warp's 16
+  for (int g = 0; g < 8; ++g) {
+    if (b0 >> (4 * g) & 15u) rows |= 1u << g;
+    if (b1 >> (4 * g) & 15u) rows |= 1u << (g + 8);
+  }
+  return rows;
+}
+
+template <typename F>
+__device__ __forceinline__ void again(uint32_t rows, int64_t p0, uint8_t* scratch, F&& row) {
+  while (rows) {  // the same in all lanes
+    const int r = __ffs(rows) - 1;
+    rows &= rows - 1;
+    __syncwarp();
+    row(p0 + r, reinterpret_cast<float*>(scratch));
+  }
 }
 
 template <typename T>
@@ -262,628 +514,216 @@ __device__ __noinline__ void again_dkv(AttnArgs a, int64_t p, int h, float* s) {
   row_dkv<T, true>(a, p, h, s);
 }
 
-// The table's gradient in fixed point: a score gradient is at most 2^17 units (the head's largest is
-// known from the dk / dv pass), and sums to a 32-bit word per bucket in shared memory. A thread
-// counts the units it has added; its warp moves the words into the 64-bit sums in global memory
-// before the count can pass 2^24, so the 128 threads cannot overflow a word. INT_MAX when a score
-// gradient was not finite.
-constexpr int UNIT_BITS = 17;
-__device__ __forceinline__ int unit_exponent(const AttnArgs& a, int head) {
-  const float top = __uint_as_float(a.norms[2 * head]);
-  if (!(top < INFINITY)) return INT_MAX;
-  if (top == 0.f) return 0;
-  int e;
-  frexpf(top, &e);                      // top < 2^e
-  return min(UNIT_BITS - 1 - e, 120);   // the two passes round their products differently
+// Shared memory: OWN tiles of the block's BQ rows, STAGES buffers of two tiles of KB positions, then
+// the tables.
+template <int DP, int BQ, int OWN, int STAGES>
+struct Layout {
+  static constexpr int OWN_TILE = BQ * STRIDE<DP>;
+  static constexpr int TILE = KB * STRIDE<DP>;
+  static constexpr int RING = OWN * OWN_TILE;
+  static constexpr int SHARED = RING + STAGES * 2 * TILE;
+  static constexpr int TABLE = (SHARED + (int)sizeof(Shared<BQ>) + 15) / 16 * 16;
+};
+
+struct Tables {
+  int grad, lut, joint, total;  // byte offsets behind Layout::TABLE; joint < 0: none
+};
+__host__ __device__ inline Tables tables(const AttnArgs& a, bool grad) {
+  const int cells = a.nb * a.nb * a.nb, width = 2 * a.reach + 1;
+  Tables t;
+  t.grad = cells * 4;
+  t.lut = t.grad + (grad ? cells * 4 : 0);
+  t.joint = -1;
+  t.total = t.lut + (width * 2 + 15) / 16 * 16;
+  if (width * width <= JOINT_MAX) {
+    t.joint = t.total;
+    t.total += width * width * 2;
+  }
+  return t;
 }
 
-// The running maximum of the softmax is only kept within this many powers of two: a row starts with
-// a base of 0, and its sums are rescaled (and the tile done again) when a score passes the base by
-// more, or when the first scores it sees are all that far below. Weights are then between 2^-8 and 2^8 of
-// the usual ones, which neither type nor the fp32 sums notice.
+template <typename T, int BQ>
+__device__ __forceinline__ Block<T, BQ> make_block(const AttnArgs& a, uint8_t* smem, int shared,
+                                                   int table, bool grad) {
+  const Tables t = tables(a, grad);
+  return Block<T, BQ>{a, *reinterpret_cast<Shared<BQ>*>(smem + shared),
+                      reinterpret_cast<float*>(smem + table),
+                      reinterpret_cast<uint16_t*>(smem + table + t.lut),
+                      t.joint < 0 ? nullptr : reinterpret_cast<uint16_t*>(smem + table + t.joint),
+                      (int)blockIdx.y, false, 0.f};
+}
+
+// The tiles of one block: load(buffer, rows) fetches a tile's rows, STAGES - 1 tiles ahead (the
+// block's own rows, loaded before, are in the first group), and body(t, buffer) works on tile t.
+// One barrier a tile: behind it the tile has landed, the readers of the buffer that is filled next
+// are done, and the rows of the tile that fills it are known. ask() is asked at the barrier, by
+// every thread, and flush() done before the tile if any said yes.
+template <bool STATS, int STAGES, typename B, typename Load, typename Body, typename Ask,
+          typename Flush>
+__device__ __forceinline__ void walk(B& b, Load&& load, Body&& body, Ask&& ask, Flush&& flush) {
+  static_assert(STAGES + 1 <= SLOTS, "rows known ahead");
+  const int warp = threadIdx.x >> 5;
+  if (warp < STAGES) b.template stage_meta<STATS>(warp);
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t) {
+    if (t < b.tiles) load(t, b.s.key_row[t]);
+    cp_commit();
+  }
+  int buf = 0, fill = STAGES - 1;
+  for (int t = 0; t < b.tiles; ++t) {
+    cp_wait<STAGES - 2>();
+    if (__syncthreads_or(ask())) flush();
+    if (t + STAGES - 1 < b.tiles) load(fill, b.s.key_row[(t + STAGES - 1) % SLOTS]);
+    cp_commit();
+    // by another warp each time
+    if (t + STAGES < b.tiles && warp == (t & 3)) b.template stage_meta<STATS>(t + STAGES);
+    body(t, buf);
+    buf = buf + 1 == STAGES ? 0 : buf + 1;
+    fill = fill + 1 == STAGES ? 0 : fill + 1;
+  }
+  cp_wait<0>();
+  __syncthreads();
+}
+
+// Scores may pass the running base by this much (in powers of two) before the sums are rescaled, so
+// most tiles skip it; weights then reach 2^8 at most, which neither type nor the fp32 sums notice.
 constexpr float SLACK = 8.f;
 
-// Range of positions that the block's rows see: by every warp for itself, from the plan.
-struct Range {
-  int lo, tiles;
-};
-template <int KB>
-__device__ __forceinline__ Range block_range(const AttnArgs& a, int64_t p0) {
-  const int lane = threadIdx.x & 31;
-  int lo = INT_MAX, hi = INT_MIN;
-#pragma unroll
-  for (int i = 0; i < BQ / 32; ++i) {
-    const int64_t p = p0 + lane + 32 * i;
-    if (p < a.n) {
-      const int4 r = __ldg(reinterpret_cast<const int4*>(a.plan + p) + 1);  // start, end, span
-      if (__ldg(&a.plan[p].row) >= 0) {
-        lo = min(lo, r.x);
-        hi = max(hi, r.y);
-      }
-    }
-  }
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  return Range{lo, hi > lo ? (hi - lo + KB - 1) / KB : 0};
-}
-
-template <typename T, int MODE, int PANELS, int KB, bool TABLE>
-__global__ void __launch_bounds__(AT, Plan<MODE, PANELS, KB>::CTAS)
-    attn_tc_kernel(AttnArgs a, int per_cta, bool vec, int32_t* status) {
-  using P = Plan<MODE, PANELS, KB>;
-  constexpr int ST = P::STAGES, NB = P::BUFS;
-  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~static_cast<uintptr_t>(1023));
-  Meta<KB>* metas = reinterpret_cast<Meta<KB>*>(smem + P::META);
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + P::MISC);
-  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + P::MISC + 4);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + P::MISC + 32);  // a tile has landed
-  uint64_t* empty = full + ST;        // a tile's products are done
-  uint64_t* s_full = empty + ST;      // scores are in TMEM
-  uint64_t* p_full = s_full + NB;     // weights are in TMEM
-  uint64_t* acc_done = p_full + NB;   // a tile's second products are done (one a buffer: a wait by
-                                      // parity tells a phase from the next only)
-  uint64_t* acc_free = acc_done + NB;  // the block's results have been read
-  uint64_t* own_full = acc_free + 1;
-  uint64_t* own_empty = own_full + 1;
-  const Tables tb = tables(a, TABLE && MODE == DQ);
-  float* table = reinterpret_cast<float*>(smem + P::TABLE);
-  int* s_grad = reinterpret_cast<int*>(smem + P::TABLE + tb.grad);
-  uint16_t* lut = reinterpret_cast<uint16_t*>(smem + P::TABLE + tb.lut);
-  uint16_t* joint =
-      tb.joint < 0 ? nullptr : reinterpret_cast<uint16_t*>(smem + P::TABLE + tb.joint);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// MR: 16-row parts of a warp, whose products share the tile's fragments.
+template <typename T, int DP, int MR, int STAGES>
+__global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
+    attn_tc_kernel(AttnArgs a, int per_block, bool vec) {
+  constexpr int BQ = 64 * MR;
+  using L = Layout<DP, BQ, 1, STAGES>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, false);
+  Shared<BQ>& sh = b.s;
   const int head = blockIdx.y;
-  const int cells = a.nb * a.nb * a.nb, width = 2 * a.reach + 1;
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < ST; ++s) {
-      mbar_init(&full[s], 2 * LOADERS);  // each loader: its copies, and its plain stores
-      mbar_init(&empty[s], 1);
-    }
-    for (int s = 0; s < NB; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
-      mbar_init(&acc_done[s], 1);
-    }
-    mbar_init(acc_free, 4);
-    mbar_init(own_full, 2 * LOADERS);
-    mbar_init(own_empty, 1);
-    *s_abort = 0;
-    fence_mbar_init();
-  }
-  if (warp == 4) {
-    tmem_alloc(s_tmem, P::COLS);
-    tmem_relinquish();
-  }
-  {
-    const T* src = static_cast<const T*>(a.table) + (int64_t)head * cells;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < cells; i += AT) table[i] = times_log2e(to_f32(src[i]));
-    if constexpr (TABLE && MODE == DQ)
-      for (int i = threadIdx.x; i < cells; i += AT) s_grad[i] = 0;
-  }
-  bool same = a.nb == width;
-  for (int i = threadIdx.x; i < width; i += AT) {
-    const int v = max(0, min(a.nb - 1, __ldg(a.lut + i)));
-    lut[i] = (uint16_t)(4 * v);
-    same = same && v == i;
-  }
-  tc_fence_before();
-  const bool identity = __syncthreads_and(same);
-  tc_fence_after();
-  if (!identity && joint != nullptr) {
-    for (int i = threadIdx.x; i < width * width; i += AT)
-      joint[i] = (uint16_t)((lut[i / width] * a.nb + lut[i % width]) * a.nb);
-    __syncthreads();
-  }
-  const uint32_t tmem = *s_tmem;
-  const int64_t blocks = (a.n + BQ - 1) / BQ;
-  const int64_t first = (int64_t)blockIdx.x * per_cta;
-  const int64_t last = first + per_cta < blocks ? first + per_cta : blocks;
-  const int ksteps = (a.dim + 15) / 16;  // of 16 channels
-  bool ok = true;
-
-  if (warp >= 5) {
-    // ---- loaders ----
-    const int tid = threadIdx.x - 160;
-    const T* q = static_cast<const T*>(a.q) + head * a.q_head;
-    const T* k = static_cast<const T*>(a.k) + head * a.k_head;
-    const T* v = static_cast<const T*>(a.v) + head * a.v_head;
-    const T* g = static_cast<const T*>(a.dout) + (int64_t)head * a.dim;
-    const int g_row = a.heads * a.dim;
-    const T* own0 = MODE == DKV ? k : q;
-    const T* own1 = MODE == DKV ? v : g;
-    const int own0_row = (int)(MODE == DKV ? a.k_row : a.q_row);
-    const int own1_row = MODE == DKV ? (int)a.v_row : g_row;
-    const T* tile0 = MODE == DKV ? q : k;
-    const T* tile1 = MODE == DKV ? g : v;
-    const int tile0_row = (int)(MODE == DKV ? a.q_row : a.k_row);
-    const int tile1_row = MODE == DKV ? g_row : (int)a.v_row;
-    const int chunks = 2 * ksteps;  // 16-byte pieces of a row that the products read
-    // Rows p .. p + ROWS - 1 (positions below `end`) of one or two tensors. A thread takes one piece
-    // of every (128 / PIECES)th row.
-    constexpr int PIECES = 8 * PANELS;
-    auto gather = [&](uint8_t* dst0, uint8_t* dst1, const T* src0, const T* src1, int row0, int row1,
-                      int64_t p, int64_t end, auto rows_c) {
-      constexpr int ROWS = decltype(rows_c)::value;
-      constexpr int STEP = LOADERS / PIECES;
-      const int c = tid % PIECES;
-      const uint32_t panel = (uint32_t)(c / 8) * (ROWS * PANEL);
-      int32_t idx[ROWS / STEP];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c2 = 2 * (lane & 3);
+  const int row0 = warp * 16 * MR;            // the warp's rows of the block
+  uint8_t* mine = smem + row0 * STRIDE<DP>;   // and of q
+  const T* q = static_cast<const T*>(a.q) + head * a.q_head;
+  const T* k = static_cast<const T*>(a.k) + head * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + head * a.v_head;
+  const float scale = a.scale * ATTN_LOG2E;
+  const uint32_t table = smem_u32(b.table);
+  b.stage_tables();
+  const int64_t first = (int64_t)blockIdx.x * per_block;
+  for (int64_t block = first; block < first + per_block && block * BQ < a.n; ++block) {
+    b.begin(block * BQ);
+    load_tile<T, DP, BQ>(smem, q, (int)a.q_row, sh.own_row, a.dim, vec);
+    const PlanRow* own = sh.own + row0 + g;
+    const Reach w = warp_reach<16 * MR>(sh.own + row0);
+    float o[MR][DP / 8][4], base[MR][2], sum[MR][2];
 #pragma unroll
-      for (int i = 0; i < ROWS / STEP; ++i) {
-        const int64_t at = p + tid / PIECES + i * STEP;
-        idx[i] = at < end ? __ldg(&a.plan[at].row) : -1;
-      }
-      if (c < chunks) {
-#pragma unroll
-        for (int i = 0; i < ROWS / STEP; ++i) {
-          const int r = tid / PIECES + i * STEP;
-          const uint32_t at = panel + r * PANEL + (((c & 7) ^ (r & 7)) << 4);
-          const int64_t row = max(idx[i], 0);
-          if (vec) {
-            const bool in = idx[i] >= 0 && c * 8 < a.dim;
-            const int from = in ? c * 8 : 0;
-            cp_async_16(smem_u32(dst0) + at, src0 + row * row0 + from, in ? 16u : 0u);
-            if (dst1) cp_async_16(smem_u32(dst1) + at, src1 + row * row1 + from, in ? 16u : 0u);
-          } else {
-            for (int d = 0; d < (dst1 ? 2 : 1); ++d) {
-              T e[8];
-#pragma unroll
-              for (int x = 0; x < 8; ++x) {
-                e[x] = from_f32<T>(0.f);
-                if (idx[i] >= 0 && c * 8 + x < a.dim)
-                  e[x] = d ? src1[row * row1 + c * 8 + x] : src0[row * row0 + c * 8 + x];
-              }
-              *reinterpret_cast<uint4*>((d ? dst1 : dst0) + at) = *reinterpret_cast<uint4*>(e);
-            }
-          }
-        }
-      }
-    };
-    // Arrives for the copies when they land, and for the plain stores now.
-    auto landed = [](uint64_t* bar) {
-      fence_proxy_async_smem();
-      cp_async_arrive_noinc(bar);
-      arrive(bar);
-    };
-    int it = 0, local = 0;
-    float delta_top = 0.f;
-    for (int64_t block = first; block < last && ok; ++block, ++local) {
-      const Range range = block_range<KB>(a, block * BQ);
-      if (!mbar_wait_bounded(own_empty, (local & 1) ^ 1, s_abort)) {
-        ok = false;
-        break;
-      }
-      gather(smem, P::OWN == 2 ? smem + P::OWN_TILE : nullptr, own0, own1, own0_row, own1_row,
-             block * BQ, a.n, std::integral_constant<int, BQ>{});
-      landed(own_full);
-      for (int t = 0; t < range.tiles; ++t, ++it) {
-        const int s = it % ST;
-        const int64_t p0 = (int64_t)range.lo + t * KB;
-        const int64_t end = min(a.n, p0 + KB);
-        if (!mbar_wait_bounded(&empty[s], ((it / ST) & 1) ^ 1, s_abort)) {
-          ok = false;
-          break;
-        }
-        uint8_t* dst = smem + P::RING + s * 2 * P::TILE;
-        gather(dst, dst + P::TILE, tile0, tile1, tile0_row, tile1_row, p0, end,
-               std::integral_constant<int, KB>{});
-        if (tid < KB) {
-          Meta<KB>& m = metas[s];
-          int4 r = make_int4(0, 0, 0, -1);
-          if (p0 + tid < end) r = __ldg(reinterpret_cast<const int4*>(a.plan + p0 + tid));
-          m.xyzr[tid] = r;
-          m.lin[tid] = (int)((((unsigned)r.x * a.nb + (unsigned)r.y) * a.nb + (unsigned)r.z) * 4u);
-          m.joint[tid] = make_int2((int)(((unsigned)r.x * width + (unsigned)r.y) * 2u),
-                                   (int)((unsigned)r.z * 2u));
-          if constexpr (MODE == DKV) {
-            float2 st = make_float2(0.f, 0.f);
-            float d = 0.f;
-            if (r.w >= 0) {
-              st = a.stats[head * a.n + p0 + tid];
-              d = a.delta[head * a.n + p0 + tid];
-            }
-            m.top[tid] = st.x;
-            m.inv[tid] = st.y;
-            m.delta[tid] = d;
-            delta_top = max_nan(delta_top, fabsf(d));
-          }
-          const unsigned rows = __ballot_sync(0xffffffffu, r.w >= 0);
-          if (lane == 0) m.rows[tid / 32] = rows;
-        }
-        landed(&full[s]);
-      }
+    for (int m = 0; m < MR; ++m) {
+      zero(o[m]);
+      base[m][0] = base[m][1] = -3.402823466e38f;
+      sum[m][0] = sum[m][1] = 0.f;
     }
-    if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
-    cp_async_wait_all();
-    if constexpr (MODE == DKV && TABLE) {
-      // The two passes round dp - delta differently, by up to 2^-17 |delta| or so; a head whose score
-      // gradients are nothing but that must not get a unit so small that the other pass overflows it.
-      const unsigned top =
-          __reduce_max_sync(0xffffffffu, __float_as_uint(delta_top * 0x1p-14f) & 0x7fffffffu);
-      if (lane == 0 && top) atomicMax(a.norms + 2 * head, top);
-    }
-  } else if (warp == 4) {
-    // ---- products ----
-    const uint32_t id_nt = idesc_f16(kBF16, BQ, KB);
-    const uint32_t id_nn = idesc_f16_major(kBF16, BQ, 16 * ksteps, false, true);
-    int it = 0, local = 0;
-    for (int64_t block = first; block < last && ok; ++block, ++local) {
-      const Range range = block_range<KB>(a, block * BQ);
-      if (lane == 0) {
-        const uint32_t own = smem_u32(smem);
-        auto stage = [&](int i) { return smem_u32(smem + P::RING + (i % ST) * 2 * P::TILE); };
-        // Scores of tile i: A = the block's rows, B = the tile's, both along the channels. `after`:
-        // the tile of the block whose weights were in the buffer, to be multiplied first (-1: none).
-        auto scores = [&](int i, int after) {
-          if (!mbar_wait_bounded(&full[i % ST], (i / ST) & 1, s_abort)) return false;
-          if (after >= 0 &&
-              !mbar_wait_bounded(&acc_done[after % NB], (after / NB) & 1, s_abort))
-            return false;
-          tc_fence_after();
-          fence_proxy_async_smem();
-          const uint32_t d = tmem + P::SCORES + (i % NB) * P::SCORE_COLS;
-          for (int x = 0; x < (MODE == FWD ? 1 : 2); ++x) {
-            for (int j = 0; j < ksteps; ++j) {
-              const uint32_t at = (j % 4) * 32;
-              tc_mma_f16(d + x * KB,
-                         smem_desc_sw128(own + x * P::OWN_TILE + (j / 4) * P::OWN_PANEL + at),
-                         smem_desc_sw128(stage(i) + x * P::TILE + (j / 4) * P::TILE_PANEL + at),
-                         id_nt, j > 0);
-            }
-          }
-          tc_commit(&s_full[i % NB]);
-          return true;
+    auto body = [&](int t, int buf) {
+      const int p0 = b.j0 + t * KB;
+      if (p0 >= w.hi || p0 + KB <= w.lo) return;
+      const uint32_t tile = smem_u32(smem + L::RING + buf * 2 * L::TILE);
+      const int slot = t % SLOTS;
+      const bool bad = sh.key_bad[slot];
+      const bool whole = p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad;
+      float s[MR][KB / 8][4];
+#pragma unroll
+      for (int m = 0; m < MR; ++m) zero(s[m]);
+      mma_nt<T, DP, MR>(s, smem_u32(mine), tile);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        auto score = [&](int n, int e, uint32_t at) {
+          s[m][n][e] = fmaf(s[m][n][e], scale, lds_f32(table + at));
         };
-        if (range.tiles > 0) {
-          ok = mbar_wait_bounded(own_full, local & 1, s_abort) &&
-               (local == 0 || mbar_wait_bounded(acc_free, (local - 1) & 1, s_abort));
-          if (ok) ok = scores(it, -1);
-        }
-        for (int t = 0; t < range.tiles && ok; ++t) {
-          const int i = it + t;
-          if (NB == 2 && t + 1 < range.tiles && !(ok = scores(i + 1, t > 0 ? i - 1 : -1))) break;
-          if (!(ok = mbar_wait_bounded(&p_full[i % NB], (i / NB) & 1, s_abort))) break;
-          tc_fence_after();
-          const uint32_t s = tmem + P::SCORES + (i % NB) * P::SCORE_COLS;
-          // sums += weights x tile, the tile read along its rows
-          for (int j = 0; j < KB / 16; ++j) {
-            auto tile = [&](int x) {
-              return smem_desc_mn_sw128(stage(i) + x * P::TILE + j * 16 * PANEL, P::TILE_PANEL,
-                                        8 * PANEL);
-            };
-            const uint32_t more = t > 0 || j > 0;
-            if constexpr (MODE == FWD) mma_ts(tmem, s + P::WEIGHTS + j * 8, tile(1), id_nn, more);
-            if constexpr (MODE == DQ) mma_ts(tmem, s + j * 8, tile(0), id_nn, more);
-            if constexpr (MODE == DKV) {
-              mma_ts(tmem, s + KB + j * 8, tile(0), id_nn, more);      // dk += dS Q
-              mma_ts(tmem + P::ACC, s + j * 8, tile(1), id_nn, more);  // dv += P dO
-            }
-          }
-          tc_commit(&empty[i % ST]);
-          tc_commit(&acc_done[i % NB]);
-          if (t + 1 == range.tiles) tc_commit(own_empty);
-          if (NB == 1 && t + 1 < range.tiles && !(ok = scores(i + 1, i))) break;
-        }
-        if (range.tiles == 0) {
-          // nothing reads the block's rows; keep the barriers' phases in step
-          ok = mbar_wait_bounded(own_full, local & 1, s_abort) &&
-               (local == 0 || mbar_wait_bounded(acc_free, (local - 1) & 1, s_abort));
-          arrive(own_empty);
-        }
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      it += range.tiles;
-    }
-    if (lane == 0) {
-      // The last commit's arrival, and after a wait that ran out the products in flight, use this
-      // CTA's shared memory and TMEM: let them finish.
-      if (ok) ok = mbar_wait_bounded(own_empty, (local - 1) & 1, s_abort);
-      if (!ok) {
-        report(status, SV_DEVICE_WAIT_TIMEOUT);
-        const uint64_t t0 = global_timer_ns();
-        while (global_timer_ns() - t0 < 10000000ull) {
-        }
-      }
-    }
-  } else {
-    // ---- a row a thread ----
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    float* scratch = reinterpret_cast<float*>(smem + P::SCRATCH) + warp * 2 * ATTN_MAX_DIM;
-    const float scale = a.scale * ATTN_LOG2E;
-    Look look{smem_u32(table), smem_u32(lut), joint ? smem_u32(joint) : 0u, a.nb, a.reach, GENERAL,
-              (uint32_t)cells * 4u - 4u, (uint32_t)(width * width) * 2u - 2u,
-              (uint32_t)width * 2u - 2u};
-    const uint32_t grads = smem_u32(s_grad);
-    const int exponent = TABLE && MODE == DQ ? unit_exponent(a, head) : INT_MAX;
-    const float unit = exponent == INT_MAX ? 0.f : ldexpf(1.f, exponent);
-    constexpr float LIMIT = 16777216.f - CH * (float)(1 << UNIT_BITS);  // CH pairs between checks
-    float spent = 0.f;  // sum of |dS| since this warp emptied the words
-    float most = 0.f;
-    auto flush = [&] {
-      for (int i = lane; i < cells; i += 32) {
-        const int add = atomicExch(s_grad + i, 0);
-        if (add != 0)
-          atomicAdd(a.dtable + (int64_t)head * cells + i, (unsigned long long)(long long)add);
-      }
-      spent = 0.f;
-    };
-    auto wait = [&](uint64_t* bar, int phase) {
-      return (bool)__all_sync(0xffffffffu, mbar_wait_bounded(bar, phase & 1, s_abort));
-    };
-    int it = 0;
-    for (int64_t block = first; block < last && ok; ++block) {
-      const Range range = block_range<KB>(a, block * BQ);
-      const int64_t pos = block * BQ + warp * 32 + lane;
-      Own own;
-      own.p = PlanRow{};
-      own.p.row = -1;
-      if (pos < a.n) own.p = plan_at(a.plan, pos);
-      const bool live = own.p.row >= 0;
-      if (!live) own.p.start = own.p.end = 0;
-      const bool narrow = __all_sync(0xffffffffu, !live || own.p.span <= a.reach);
-      look.mode = !narrow ? GENERAL : (identity ? LINEAR : (joint ? JOINT : GENERAL));
-      // the middle of the tables is folded into the row's side
-      const int sign = MODE == DKV ? 1 : -1;
-      own.lin = (int)((((unsigned)own.p.x * a.nb + (unsigned)own.p.y) * a.nb + (unsigned)own.p.z) *
-                      4u) + sign * (int)(look.top / 2);
-      own.joint_xy = (int)(((unsigned)own.p.x * width + (unsigned)own.p.y) * 2u) +
-                     sign * (int)(look.joint_top / 2);
-      own.joint_z = (int)((unsigned)own.p.z * 2u) + sign * 2 * a.reach;
-      float base = 0.f, sum = 0.f;                     // forward
-      bool fresh = true;                               // no score seen yet
-      float top = 0.f, inv = 0.f, shift = 0.f;         // dq
-      if constexpr (MODE == DQ) {
-        if (live) {
-          const float2 st = a.stats[head * a.n + pos];
-          top = st.x;
-          inv = st.y;
-          shift = -st.y * a.delta[head * a.n + pos];
-        }
-      }
-      for (int t = 0; t < range.tiles && ok; ++t, ++it) {
-        const int p0 = range.lo + t * KB;
-        const int buf = it % NB;
-        const Meta<KB>& m = metas[it % ST];
-        const uint32_t at = lanes + P::SCORES + buf * P::SCORE_COLS;
-        if (!wait(&full[it % ST], it / ST) || !wait(&s_full[buf], it / NB)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const int lo = own.p.start - p0, hi = own.p.end - p0;
-        // Bits of the columns c0 .. that the row sees.
-        auto seen_at = [&](int c0) {
-          return seen_bits(lo, hi, c0) & (m.rows[c0 / 32] >> (c0 % 32));
-        };
-        if constexpr (MODE == FWD) {
-          for (bool again = false;; again = true) {
-            float high = -INFINITY, part = 0.f;
-#pragma unroll 1
-            for (int c0 = 0; c0 < KB; c0 += CH) {
-              const uint32_t seen = seen_at(c0);
-              float v[CH];
-              if (!__any_sync(0xffffffffu, seen)) {
-#pragma unroll
-                for (int c = 0; c < CH; ++c) v[c] = 0.f;
-              } else {
-                uint32_t r[CH], off[CH];
-                tmem_ld_32x32b_x16(at + c0, r);
-                buckets<false>(look, m, own, c0, off);
-                tc_wait_ld();
-#pragma unroll
-                for (int c = 0; c < CH; ++c)
-                  v[c] = fmaf(__uint_as_float(r[c]), scale, lds_f32(look.table + off[c]));
-                if (!__all_sync(0xffffffffu, seen == ALL_SEEN)) {
-#pragma unroll
-                  for (int c = 0; c < CH; ++c)
-                    if (!(seen & (1u << c))) v[c] = -INFINITY;
-                }
-#pragma unroll
-                for (int c = 0; c < CH; c += 2) high = fmaxf(high, fmaxf(v[c], v[c + 1]));
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                  v[c] = exp2_fast(v[c] - base);
-                  part += v[c];
-                }
-              }
-              __syncwarp();
-              store_weights<T>(at + P::WEIGHTS + c0 / 2, v);
-            }
-            const bool off_base =
-                high > base + SLACK || (fresh && high > -INFINITY && high < base - SLACK);
-            if (again || !__any_sync(0xffffffffu, off_base)) {
-              sum += part;
-              fresh = fresh && high == -INFINITY;
-              break;
-            }
-            // lanes whose base stays keep it: their weights come out the same again
-            const float keep = off_base ? exp2_fast(base - high) : 1.f;
-            if (off_base) base = high;
-            sum = fresh ? 0.f : sum * keep;
-            if (t > 0) {
-              if (!wait(&acc_done[(it - 1) % NB], (it - 1) / NB)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              for (int c = 0; c < 16 * ksteps; c += 16) {
-                uint32_t r[16];
-                tmem_ld_32x32b_x16(lanes + c, r);
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  r[i] = fresh ? 0u : __float_as_uint(__uint_as_float(r[i]) * keep);
-                tmem_st_x16(lanes + c, r);
-              }
-            }
-            tmem_wait_st();
-          }
-          if (!ok) break;
+        if (whole) {
+          each_pair<false, true>(b, slot, own + 16 * m, score);
         } else {
-#pragma unroll 1
-          for (int c0 = 0; c0 < KB; c0 += CH) {
-            const uint32_t seen = seen_at(c0);
-            float s[CH], d[CH];
-            if (!__any_sync(0xffffffffu, seen)) {
+          each_pair<false, false>(b, slot, own + 16 * m, score);
+          const Sight seen = sight(own + 16 * m, p0);
 #pragma unroll
-              for (int c = 0; c < CH; ++c) s[c] = d[c] = 0.f;
-            } else {
-              uint32_t rs[CH], rd[CH], off[CH];
-              tmem_ld_32x32b_x16(at + c0, rs);
-              tmem_ld_32x32b_x16(at + KB + c0, rd);
-              buckets<MODE == DKV>(look, m, own, c0, off);
-              tc_wait_ld();
+          for (int n = 0; n < KB / 8; ++n)
 #pragma unroll
-              for (int c = 0; c < CH; ++c) {
-                s[c] = fmaf(__uint_as_float(rs[c]), scale, lds_f32(look.table + off[c]));
-                d[c] = __uint_as_float(rd[c]);
-              }
-              const bool whole = __all_sync(0xffffffffu, seen == ALL_SEEN);
-              if constexpr (MODE == DQ) {
+            for (int e = 0; e < 4; ++e)
+              if (hidden(seen, n, e, bad, sh, slot)) s[m][n][e] = -INFINITY;
+        }
+      }
+      float top[MR][2];
+      bool over = false;
 #pragma unroll
-                for (int c = 0; c < CH; ++c)
-                  s[c] = exp2_fast(s[c] - top) * fmaf(d[c], inv, shift);
-                if (!whole) {
+      for (int m = 0; m < MR; ++m) {
 #pragma unroll
-                  for (int c = 0; c < CH; ++c)
-                    if (!(seen & (1u << c))) s[c] = 0.f;
-                }
-                if constexpr (TABLE) {
+        for (int r = 0; r < 2; ++r) {
+          float x = fmaxf(s[m][0][2 * r], s[m][0][2 * r + 1]);
 #pragma unroll
-                  for (int c = 0; c < CH; ++c) {
-                    spent += fabsf(s[c]);
-                    // 1.5 * 2^23: the sum's low bits are the rounded integer
-                    const float f = fmaf(s[c], unit, 12582912.f);
-                    const int add = __float_as_int(f) - 0x4b400000;
-                    if (add != 0)
-                      asm volatile("red.shared.add.s32 [%0], %1;" ::"r"(grads + off[c]), "r"(add)
-                                   : "memory");
-                  }
-                }
-              } else {
+          for (int n = 1; n < KB / 8; ++n) x = fmaxf(x, fmaxf(s[m][n][2 * r], s[m][n][2 * r + 1]));
+          top[m][r] = x;
+          over = over || x > base[m][r] + SLACK;
+        }
+      }
+      if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-                for (int c = 0; c < CH; c += 4) {
-                  const float4 tp = *reinterpret_cast<const float4*>(&m.top[c0 + c]);
-                  const float4 iv = *reinterpret_cast<const float4*>(&m.inv[c0 + c]);
-                  const float4 dl = *reinterpret_cast<const float4*>(&m.delta[c0 + c]);
-                  const float tops[4] = {tp.x, tp.y, tp.z, tp.w}, invs[4] = {iv.x, iv.y, iv.z, iv.w},
-                              dels[4] = {dl.x, dl.y, dl.z, dl.w};
+        for (int m = 0; m < MR; ++m) {
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    s[c + e] = exp2_fast(s[c + e] - tops[e]) * invs[e];
-                    d[c + e] -= dels[e];
-                  }
-                }
-                if (!whole) {  // another window's row may hold anything
+          for (int r = 0; r < 2; ++r) {
+            float x = top[m][r];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            x = fmaxf(x, base[m][r]);
+            const float keep = exp2_fast(base[m][r] - x);
+            base[m][r] = x;
+            sum[m][r] *= keep;
 #pragma unroll
-                  for (int c = 0; c < CH; ++c)
-                    if (!(seen & (1u << c))) s[c] = d[c] = 0.f;
-                }
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                  d[c] *= s[c];
-                  if constexpr (TABLE) most = max_nan(most, fabsf(d[c]));
-                }
-              }
-            }
-            __syncwarp();
-            store_weights<T>(at + c0 / 2, s);
-            if constexpr (MODE == DKV) store_weights<T>(at + KB + c0 / 2, d);
-            if constexpr (TABLE && MODE == DQ) {
-              if (__any_sync(0xffffffffu, spent * unit > LIMIT)) flush();
+            for (int n = 0; n < DP / 8; ++n) {
+              o[m][n][2 * r] *= keep;
+              o[m][n][2 * r + 1] *= keep;
             }
           }
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive(&p_full[buf]);
       }
-      if (!ok) break;
-      // ---- results ----
-      if (range.tiles > 0) {
-        if (!wait(&acc_done[(it - 1) % NB], (it - 1) / NB)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-      }
-      float by = a.scale;  // dq, dk
-      if constexpr (MODE == FWD) {
-        const float2 st = row_stats(base, sum);
-        by = st.y;
-        if (a.stats && live) a.stats[head * a.n + pos] = st;
-      }
-      bool finite = true;
-      const int64_t out_row = ((int64_t)max(own.p.row, 0) * a.heads + head) * a.dim;
-#pragma unroll 1
-      for (int x = 0; x < (MODE == DKV ? 2 : 1); ++x) {
-        T* out = static_cast<T*>(MODE == FWD ? a.out : MODE == DQ ? a.dq : x ? a.dv : a.dk);
-        const float f = MODE == DKV && x ? 1.f : by;
-#pragma unroll 1
-        for (int c = 0; c < 16 * ksteps && range.tiles > 0; c += 16) {
-          uint32_t r[16];
-          __syncwarp();  // lanes without a row skip the rest of a round
-          tmem_ld_32x32b_x16(lanes + x * P::ACC + c, r);
-          tc_wait_ld();
-          if (!live) continue;
-          float o[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            o[i] = __uint_as_float(r[i]) * f;
-            finite = finite && fabsf(o[i]) < INFINITY;
+      for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int n = 0; n < KB / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[m][n][e] = exp2_fast(s[m][n][e] - base[m][e >> 1]);
+            sum[m][e >> 1] += s[m][n][e];
           }
-          T* dst = out + out_row + c;
-          if (vec) {
+      mma_nn<T, DP, MR>(o, s, tile + L::TILE);
+    };
+    walk<false, STAGES>(
+        b,
+        [&](int buf, const int32_t* rows) {
+          uint8_t* tile = smem + L::RING + buf * 2 * L::TILE;
+          load_tile<T, DP, KB>(tile, k, (int)a.k_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile + L::TILE, v, (int)a.v_row, rows, a.dim, vec);
+        },
+        body, [] { return false; }, [] {});
+    uint32_t redo = 0;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (c + 8 * i < a.dim)
-                reinterpret_cast<uint4*>(dst)[i] =
-                    make_uint4(pack2<T>(o[8 * i], o[8 * i + 1]), pack2<T>(o[8 * i + 2], o[8 * i + 3]),
-                               pack2<T>(o[8 * i + 4], o[8 * i + 5]),
-                               pack2<T>(o[8 * i + 6], o[8 * i + 7]));
-          } else {
+    for (int m = 0; m < MR; ++m) {
+      float inv[2];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (c + i < a.dim) dst[i] = from_f32<T>(o[i]);
-          }
-        }
+      for (int r = 0; r < 2; ++r) {
+        float x = sum[m][r];
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        const float2 st = row_stats(base[m][r], x);
+        inv[r] = st.y;
+        const int at = row0 + 16 * m + g + 8 * r;
+        if (a.stats && c2 == 0 && sh.own_row[at] >= 0) a.stats[head * a.n + block * BQ + at] = st;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive(acc_free);
-      // A weight of zero does not hide a NaN or an infinity that another window's row brings into a
-      // tile, and fp16 score gradients can overflow where their sums do not. So rows that come out
-      // not finite are computed again, one at a time, from their own windows alone.
-      unsigned redo = __ballot_sync(0xffffffffu, live && !finite);
-      while (redo) {  // the same in all lanes
-        const int64_t p = block * BQ + warp * 32 + __ffs(redo) - 1;
-        redo &= redo - 1;
-        __syncwarp();
-        if constexpr (MODE == FWD) again_forward<T>(a, p, head, scratch);
-        if constexpr (MODE == DQ) again_dq<T>(a, p, head, scratch);
-        if constexpr (MODE == DKV) again_dkv<T>(a, p, head, scratch);
-      }
+      store_rows<T, DP>(mine + 16 * m * STRIDE<DP>, o[m], inv[0], inv[1], sh.own_row + row0 + 16 * m,
+                        static_cast<T*>(a.out), a.heads, head, a.dim, vec);
+      redo |= not_finite<DP>(o[m]) << (16 * m);
     }
-    if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
-    if constexpr (TABLE && MODE == DKV) {
-      // bits of non-negative numbers order like the numbers, a NaN's above all
-      const unsigned high = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
-      if (lane == 0 && high) atomicMax(a.norms + 2 * head, high);
-    }
-    if constexpr (TABLE && MODE == DQ) flush();
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 4) {
-    tc_fence_after();
-    tmem_dealloc(tmem, P::COLS);
+    again(redo, block * BQ + row0, mine,
+          [&](int64_t p, float* f) { if (p < a.n) again_forward<T>(a, p, head, f); });
+    __syncthreads();
   }
 }
 
@@ -919,6 +759,244 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a, bool vec) {
   if (sub == 0 && at < a.n * a.heads) a.delta[at] = d;
 }
 
+// The table's gradient in fixed point: a score gradient is at most 2^18 units (the head's largest is
+// known from the dk / dv pass), and sums to a 32-bit word per bucket in shared memory. A thread
+// counts the units it has added; the block empties its words into the 64-bit sums in global memory
+// before any thread's count can pass 2^24, so 128 threads cannot overflow a word. INT_MAX when a
+// score gradient was not finite.
+constexpr int UNIT_BITS = 18;
+__device__ __forceinline__ int unit_exponent(const AttnArgs& a, int head) {
+  const float top = __uint_as_float(a.norms[2 * head]);
+  if (!(top < INFINITY)) return INT_MAX;
+  if (top == 0.f) return 0;
+  int e;
+  frexpf(top, &e);                      // top < 2^e
+  return min(UNIT_BITS - 1 - e, 120);   // the two passes round their products differently
+}
+
+// dq and the table's gradient.
+template <typename T, int DP, int STAGES, bool TABLE>
+__global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
+    attn_dq_tc_kernel(AttnArgs a, int per_block, bool vec) {
+  constexpr int BQ = 64;
+  using L = Layout<DP, BQ, 2, STAGES>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, TABLE);
+  Shared<BQ>& sh = b.s;
+  const int cells = b.cells();
+  int* s_grad = reinterpret_cast<int*>(smem + L::TABLE + tables(a, TABLE).grad);
+  const uint32_t table = smem_u32(b.table), grads = smem_u32(s_grad);
+  const int head = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2;
+  uint8_t* mine = smem + warp * 16 * STRIDE<DP>;
+  const T* q = static_cast<const T*>(a.q) + head * a.q_head;
+  const T* k = static_cast<const T*>(a.k) + head * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + head * a.v_head;
+  const T* dout = static_cast<const T*>(a.dout) + (int64_t)head * a.dim;
+  const int g_row = a.heads * a.dim;
+  const float scale = a.scale * ATTN_LOG2E;
+  const int exponent = TABLE ? unit_exponent(a, head) : INT_MAX;
+  const float unit = exponent == INT_MAX ? 0.f : ldexpf(1.f, exponent);
+  // a thread adds KB / 2 pairs a tile
+  constexpr float LIMIT = 16777216.f - (KB / 2) * (float)(1 << UNIT_BITS);
+  float spent = 0.f;  // sum of |dS| since the words were emptied
+  if constexpr (TABLE) {
+    for (int i = threadIdx.x; i < cells; i += AT) s_grad[i] = 0;
+  }
+  b.stage_tables();
+  auto flush = [&] {
+    if constexpr (TABLE) {
+      for (int i = threadIdx.x; i < cells; i += AT) {
+        const int add = s_grad[i];
+        s_grad[i] = 0;
+        if (add != 0)
+          atomicAdd(a.dtable + (int64_t)head * cells + i, (unsigned long long)(long long)add);
+      }
+      spent = 0.f;
+      __syncthreads();
+    }
+  };
+  const int64_t first = (int64_t)blockIdx.x * per_block;
+  for (int64_t block = first; block < first + per_block && block * BQ < a.n; ++block) {
+    b.begin(block * BQ);
+    load_tile<T, DP, BQ>(smem, q, (int)a.q_row, sh.own_row, a.dim, vec);
+    load_tile<T, DP, BQ>(smem + L::OWN_TILE, dout, g_row, sh.own_row, a.dim, vec);
+    const PlanRow* own = sh.own + warp * 16 + g;
+    const Reach w = warp_reach<16>(sh.own + warp * 16);
+    float top[2], inv[2], delta[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const bool live = own[8 * r].row >= 0;
+      const int64_t p = head * a.n + block * BQ + warp * 16 + g + 8 * r;
+      const float2 st = live ? a.stats[p] : make_float2(0.f, 0.f);
+      top[r] = st.x;
+      inv[r] = st.y;
+      delta[r] = live ? a.delta[p] : 0.f;
+    }
+    float dq[1][DP / 8][4];
+    zero(dq[0]);
+    auto body = [&](int t, int buf) {
+      const int p0 = b.j0 + t * KB;
+      if (p0 >= w.hi || p0 + KB <= w.lo) return;
+      const uint32_t tile = smem_u32(smem + L::RING + buf * 2 * L::TILE);
+      const int slot = t % SLOTS;
+      float s[1][KB / 8][4], dp[1][KB / 8][4];
+      zero(s[0]);
+      mma_nt<T, DP, 1>(s, smem_u32(mine), tile);
+#pragma unroll
+      for (int n = 0; n < KB / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[0][n][e] = -delta[e >> 1];
+      mma_nt<T, DP, 1>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
+      const bool bad = sh.key_bad[slot];
+      auto grad = [&](int n, int e, uint32_t at, bool in) {
+        const int r = e >> 1;
+        const float x = fmaf(s[0][n][e], scale, lds_f32(table + at));
+        const float ds = exp2_fast(x - top[r]) * (inv[r] * dp[0][n][e]);
+        s[0][n][e] = in ? ds : 0.f;
+        if constexpr (TABLE) {
+          if (in) {
+            spent += fabsf(ds);
+            // 1.5 * 2^23: the sum's low bits are the rounded integer
+            const float f = fmaf(ds, unit, 12582912.f);
+            asm volatile("red.shared.add.s32 [%0], %1;" ::"r"(grads + at),
+                         "r"(__float_as_int(f) - 0x4b400000)
+                         : "memory");
+          }
+        }
+      };
+      if (p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad) {
+        each_pair<false, true>(b, slot, own,
+                               [&](int n, int e, uint32_t at) { grad(n, e, at, true); });
+      } else {
+        const Sight seen = sight(own, p0);
+        each_pair<false, false>(b, slot, own, [&](int n, int e, uint32_t at) {
+          grad(n, e, at, !hidden(seen, n, e, bad, sh, slot));
+        });
+      }
+      mma_nn<T, DP, 1>(dq, s, tile);
+    };
+    walk<false, STAGES>(
+        b,
+        [&](int buf, const int32_t* rows) {
+          uint8_t* tile = smem + L::RING + buf * 2 * L::TILE;
+          load_tile<T, DP, KB>(tile, k, (int)a.k_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile + L::TILE, v, (int)a.v_row, rows, a.dim, vec);
+        },
+        body, [&] { return TABLE && spent * unit > LIMIT; }, flush);
+    store_rows<T, DP>(mine, dq[0], a.scale, a.scale, sh.own_row + warp * 16, static_cast<T*>(a.dq),
+                      a.heads, head, a.dim, vec);
+    again(not_finite<DP>(dq[0]), block * BQ + warp * 16, mine,
+          [&](int64_t p, float* f) { if (p < a.n) again_dq<T>(a, p, head, f); });
+    __syncthreads();
+  }
+  flush();
+}
+
+// dk and dv, and the largest |dS| of the head: the block's rows are keys, the tiles queries.
+template <typename T, int DP, int STAGES, bool TABLE>
+__global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
+    attn_dkv_tc_kernel(AttnArgs a, int per_block, bool vec) {
+  constexpr int BQ = 64;
+  using L = Layout<DP, BQ, 2, STAGES>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, false);
+  Shared<BQ>& sh = b.s;
+  const uint32_t table = smem_u32(b.table);
+  const int head = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c2 = 2 * (lane & 3);
+  uint8_t* mine = smem + warp * 16 * STRIDE<DP>;
+  const T* q = static_cast<const T*>(a.q) + head * a.q_head;
+  const T* k = static_cast<const T*>(a.k) + head * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + head * a.v_head;
+  const T* dout = static_cast<const T*>(a.dout) + (int64_t)head * a.dim;
+  const int g_row = a.heads * a.dim;
+  const float scale = a.scale * ATTN_LOG2E;
+  float most = 0.f;
+  b.stage_tables();
+  const int64_t first = (int64_t)blockIdx.x * per_block;
+  for (int64_t block = first; block < first + per_block && block * BQ < a.n; ++block) {
+    b.begin(block * BQ);
+    load_tile<T, DP, BQ>(smem, k, (int)a.k_row, sh.own_row, a.dim, vec);
+    load_tile<T, DP, BQ>(smem + L::OWN_TILE, v, (int)a.v_row, sh.own_row, a.dim, vec);
+    const PlanRow* own = sh.own + warp * 16 + g;
+    const Reach w = warp_reach<16>(sh.own + warp * 16);
+    float dk[1][DP / 8][4], dv[1][DP / 8][4];
+    zero(dk[0]);
+    zero(dv[0]);
+    auto body = [&](int t, int buf) {
+      const int p0 = b.j0 + t * KB;
+      if (p0 >= w.hi || p0 + KB <= w.lo) return;
+      const uint32_t tile = smem_u32(smem + L::RING + buf * 2 * L::TILE);
+      const int slot = t % SLOTS;
+      float s[1][KB / 8][4], dp[1][KB / 8][4];
+      zero(s[0]);
+      mma_nt<T, DP, 1>(s, smem_u32(mine), tile);
+      const bool bad = sh.key_bad[slot];
+      const bool whole = p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad;
+      auto weight = [&](int n, int e, uint32_t at) {
+        const float2 st = sh.key_stats[slot][n * 8 + c2 + (e & 1)];
+        s[0][n][e] = exp2_fast(fmaf(s[0][n][e], scale, lds_f32(table + at)) - st.x) * st.y;
+      };
+      if (whole) {
+        each_pair<true, true>(b, slot, own, weight);
+      } else {
+        each_pair<true, false>(b, slot, own, weight);
+        const Sight seen = sight(own, p0);
+#pragma unroll
+        for (int n = 0; n < KB / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (hidden(seen, n, e, bad, sh, slot)) s[0][n][e] = 0.f;
+      }
+      mma_nn<T, DP, 1>(dv, s, tile + L::TILE);
+#pragma unroll
+      for (int n = 0; n < KB / 8; ++n) {
+        const float2 delta = *reinterpret_cast<const float2*>(&sh.key_delta[slot][n * 8 + c2]);
+        dp[0][n][0] = dp[0][n][2] = -delta.x;
+        dp[0][n][1] = dp[0][n][3] = -delta.y;
+      }
+      mma_nt<T, DP, 1>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
+#pragma unroll
+      for (int n = 0; n < KB / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float ds = s[0][n][e] * dp[0][n][e];
+          // a weight of zero may stand for a row of another window, which may hold anything
+          if (!whole && s[0][n][e] == 0.f) ds = 0.f;
+          dp[0][n][e] = ds;
+          if constexpr (TABLE) most = max_nan(most, fabsf(ds));
+        }
+      mma_nn<T, DP, 1>(dk, dp, tile);
+    };
+    walk<true, STAGES>(
+        b,
+        [&](int buf, const int32_t* rows) {
+          uint8_t* tile = smem + L::RING + buf * 2 * L::TILE;
+          load_tile<T, DP, KB>(tile, q, (int)a.q_row, rows, a.dim, vec);
+          load_tile<T, DP, KB>(tile + L::TILE, dout, g_row, rows, a.dim, vec);
+        },
+        body, [] { return false; }, [] {});
+    store_rows<T, DP>(mine, dk[0], a.scale, a.scale, sh.own_row + warp * 16, static_cast<T*>(a.dk),
+                      a.heads, head, a.dim, vec);
+    store_rows<T, DP>(mine + L::OWN_TILE, dv[0], 1.f, 1.f, sh.own_row + warp * 16,
+                      static_cast<T*>(a.dv), a.heads, head, a.dim, vec);
+    again(not_finite<DP>(dk[0]) | not_finite<DP>(dv[0]), block * BQ + warp * 16, mine,
+          [&](int64_t p, float* f) { if (p < a.n) again_dkv<T>(a, p, head, f); });
+    __syncthreads();
+  }
+  if constexpr (TABLE) {
+    // The two passes round dp - delta differently, by up to 2^-17 |delta| or so; a head whose score
+    // gradients are nothing but that must not get a unit so small that the other pass overflows it.
+    most = max_nan(most, b.delta_top * 0x1p-14f);
+    // bits of non-negative numbers order like the numbers, a NaN's above all
+    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
+    if (lane == 0 && top) atomicMax(a.norms + 2 * head, top);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) dtable_tc_finish_kernel(AttnArgs a, T* __restrict__ out) {
   const int cells = a.nb * a.nb * a.nb;
@@ -946,10 +1024,10 @@ bool wide_rows(const AttnArgs& a) {
          wide(a.dq, row, head) && wide(a.dk, row, head) && wide(a.dv, row, head);
 }
 
-// Blocks of one head that a CTA takes in turn, so that it stages the table (and adds up its gradient)
-// once: as many as still leave `waves` CTAs for each SM.
-int blocks_per_cta(const AttnArgs& a, int waves) {
-  const int64_t blocks = (a.n + BQ - 1) / BQ;
+// Blocks of BQ rows of one head that a CTA takes in turn, so that it stages the table (and adds up its
+// gradient) once: as many as still leave `waves` CTAs for each SM.
+int blocks_per_cta(const AttnArgs& a, int bq, int waves) {
+  const int64_t blocks = (a.n + bq - 1) / bq;
   const int64_t per = blocks * a.heads / ((int64_t)num_sms() * waves);
   return (int)(per < 1 ? 1 : (per > 16 ? 16 : per));
 }
@@ -961,29 +1039,41 @@ int allow_smem(K kernel, size_t bytes) {
   return SV_OK;
 }
 
-template <typename T, int MODE, int PANELS, bool TABLE>
-int launch(const AttnArgs& a, int32_t* status, cudaStream_t s) {
-  constexpr int KB = PANELS == 1 ? 64 : 32;  // positions of a tile: two CTAs fit an SM
-  auto kernel = attn_tc_kernel<T, MODE, PANELS, KB, TABLE>;
-  const size_t bytes =
-      Plan<MODE, PANELS, KB>::TABLE + tables(a, TABLE && MODE == DQ).total + 1024;
-  const int rc = allow_smem(kernel, bytes);
+template <typename T, int DP>
+int forward(const AttnArgs& a, cudaStream_t s) {
+  // two 16-row parts a warp where their sums fit the registers
+  constexpr int MR = DP <= 64 ? 2 : 1, STAGES = DP <= 64 ? 3 : 2;
+  const size_t bytes = Layout<DP, 64 * MR, 1, STAGES>::TABLE + tables(a, false).total;
+  const int rc = allow_smem(attn_tc_kernel<T, DP, MR, STAGES>, bytes);
   if (rc != SV_OK) return rc;
-  const int per = blocks_per_cta(a, MODE == FWD ? 8 : 8);
-  const int64_t ctas = ((a.n + BQ - 1) / BQ + per - 1) / per;
-  kernel<<<dim3((unsigned)ctas, a.heads), AT, bytes, s>>>(a, per, wide_rows(a), status);
+  const int per = blocks_per_cta(a, 64 * MR, 9);
+  const int64_t ctas = ((a.n + 64 * MR - 1) / (64 * MR) + per - 1) / per;
+  attn_tc_kernel<T, DP, MR, STAGES>
+      <<<dim3((unsigned)ctas, a.heads), AT, bytes, s>>>(a, per, wide_rows(a));
   SV_LAUNCH_CHECK();
   return SV_OK;
 }
 
-template <typename T, int PANELS, bool TABLE>
-int backward(const AttnArgs& a, void* dtable, int32_t* status, cudaStream_t s) {
+template <typename T, int DP, bool TABLE>
+int backward(const AttnArgs& a, void* dtable, cudaStream_t s) {
+  constexpr int STAGES = 2;
+  using L = Layout<DP, 64, 2, STAGES>;
+  const bool vec = wide_rows(a);
   attn_delta_kernel<T><<<(unsigned)((a.n * a.heads + 31) / 32), 256, 0, s>>>(
-      a, wide_rows(a) && aligned16(a.o));
+      a, vec && aligned16(a.o));
   SV_LAUNCH_CHECK();
-  int rc = launch<T, DKV, PANELS, TABLE>(a, status, s);
-  if (rc == SV_OK) rc = launch<T, DQ, PANELS, TABLE>(a, status, s);
+  const int per = blocks_per_cta(a, 64, 9);
+  const dim3 grid((unsigned)(((a.n + 63) / 64 + per - 1) / per), a.heads);
+  size_t bytes = L::TABLE + tables(a, false).total;
+  int rc = allow_smem(attn_dkv_tc_kernel<T, DP, STAGES, TABLE>, bytes);
   if (rc != SV_OK) return rc;
+  attn_dkv_tc_kernel<T, DP, STAGES, TABLE><<<grid, AT, bytes, s>>>(a, per, vec);
+  SV_LAUNCH_CHECK();
+  bytes = L::TABLE + tables(a, TABLE).total;
+  rc = allow_smem(attn_dq_tc_kernel<T, DP, STAGES, TABLE>, bytes);
+  if (rc != SV_OK) return rc;
+  attn_dq_tc_kernel<T, DP, STAGES, TABLE><<<grid, AT, bytes, s>>>(a, per, vec);
+  SV_LAUNCH_CHECK();
   if constexpr (TABLE) {
     const unsigned blocks = (unsigned)((a.nb * a.nb * a.nb + 255) / 256);
     dtable_tc_finish_kernel<T><<<dim3(blocks, a.heads), 256, 0, s>>>(a, static_cast<T*>(dtable));
@@ -993,30 +1083,29 @@ int backward(const AttnArgs& a, void* dtable, int32_t* status, cudaStream_t s) {
 }
 
 template <typename T>
-int forward_typed(const AttnArgs& a, int32_t* status, cudaStream_t s) {
-  return a.dim <= 64 ? launch<T, FWD, 1, false>(a, status, s)
-                     : launch<T, FWD, 2, false>(a, status, s);
+int forward_typed(const AttnArgs& a, cudaStream_t s) {
+  if (a.dim <= 32) return forward<T, 32>(a, s);
+  if (a.dim <= 64) return forward<T, 64>(a, s);
+  return forward<T, 128>(a, s);
 }
 
 template <typename T>
-int backward_typed(const AttnArgs& a, void* dtable, int32_t* status, cudaStream_t s) {
+int backward_typed(const AttnArgs& a, void* dtable, cudaStream_t s) {
+  if (a.dim <= 32)
+    return dtable ? backward<T, 32, true>(a, dtable, s) : backward<T, 32, false>(a, dtable, s);
   if (a.dim <= 64)
-    return dtable ? backward<T, 1, true>(a, dtable, status, s)
-                  : backward<T, 1, false>(a, dtable, status, s);
-  return dtable ? backward<T, 2, true>(a, dtable, status, s)
-                : backward<T, 2, false>(a, dtable, status, s);
+    return dtable ? backward<T, 64, true>(a, dtable, s) : backward<T, 64, false>(a, dtable, s);
+  return dtable ? backward<T, 128, true>(a, dtable, s) : backward<T, 128, false>(a, dtable, s);
 }
 
 }  // namespace
 
-int attention_tc_forward(const AttnArgs& a, bool bf16, int32_t* status, cudaStream_t s) {
-  return bf16 ? forward_typed<__nv_bfloat16>(a, status, s) : forward_typed<__half>(a, status, s);
+int attention_tc_forward(const AttnArgs& a, bool bf16, cudaStream_t s) {
+  return bf16 ? forward_typed<__nv_bfloat16>(a, s) : forward_typed<__half>(a, s);
 }
 
-int attention_tc_backward(const AttnArgs& a, bool bf16, void* dtable, int32_t* status,
-                          cudaStream_t s) {
-  return bf16 ? backward_typed<__nv_bfloat16>(a, dtable, status, s)
-              : backward_typed<__half>(a, dtable, status, s);
+int attention_tc_backward(const AttnArgs& a, bool bf16, void* dtable, cudaStream_t s) {
+  return bf16 ? backward_typed<__nv_bfloat16>(a, dtable, s) : backward_typed<__half>(a, dtable, s);
 }
 
 }  // namespace sv

@@ -11,7 +11,7 @@ from torch.autograd.function import once_differentiable
 from .. import _native as N
 
 MAX_DIM = 128
-MAX_BUCKETS = 23
+MAX_BUCKETS = 25
 MAX_REACH = 1023
 
 
@@ -45,8 +45,7 @@ def _forward(q, k, v, table, lut, plan, scale, keep_stats):
         rc = N.load().sv_window_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), n, heads, dim,
             N.DTYPE_CODE[q.dtype], plan.data_ptr(), table.data_ptr(), table.shape[-1],
-            lut.data_ptr(), lut.numel() // 2, scale, out.data_ptr(), N.ptr(stats),
-            N.status_word(dev).data_ptr(), N.stream(dev))
+            lut.data_ptr(), lut.numel() // 2, scale, out.data_ptr(), N.ptr(stats), N.stream(dev))
     N.check(rc, "sparse_self_attention")
     return out, stats
 
@@ -77,7 +76,7 @@ class _WindowAttention(torch.autograd.Function):
                 dout.data_ptr(), stats.data_ptr(), n, heads, dim, N.DTYPE_CODE[q.dtype],
                 plan.data_ptr(), table.data_ptr(), table.shape[-1], lut.data_ptr(),
                 lut.numel() // 2, ctx.scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                N.ptr(dtable), ws.data_ptr(), nbytes, N.status_word(dev).data_ptr(), N.stream(dev))
+                N.ptr(dtable), ws.data_ptr(), nbytes, N.stream(dev))
         N.check(rc, "sparse_self_attention (backward)")
         return dq, dk, dv, dtable, None, None, None
 

@@ -732,7 +732,7 @@ def sparse_self_attention(
     coordinates minus the query's and ``L`` the int32 ``position_buckets`` ``(2 * reach + 1,)`` at
     the difference clamped to ``-reach..reach`` (:func:`position_buckets` makes one). Scores, bias,
     softmax and sums then run in one kernel over all windows, with gradients for ``q``, ``k``, ``v``
-    and the table that do not depend on the order of execution. head_dim up to 128, B up to 23,
+    and the table that do not depend on the order of execution. head_dim up to 128, B up to 25,
     reach up to 1023. A row whose every score is -inf gives zeros."""
 
     if q.shape != k.shape or q.shape != v.shape or q.shape[0] != x.num_points:

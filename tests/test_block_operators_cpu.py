@@ -117,7 +117,7 @@ def test_biased_attention_refusals():
     with pytest.raises(ValueError, match="head_dim"):
         run(wide, wide, wide)
     with pytest.raises(ValueError, match="head_dim"):
-        run(table=torch.zeros((2, 24, 24, 24)))
+        run(table=torch.zeros((2, 26, 26, 26)))
     with pytest.raises(ValueError, match="reach"):
         run(lut=torch.zeros(2 * 1024 + 1, dtype=torch.int32))
     with pytest.raises(RuntimeError, match="CUDA device"):
@@ -196,13 +196,13 @@ def test_c_entry_points_check_before_any_launch():
 
     def attend(n=4, heads=2, dim=16, dtype=2, buckets=3, reach=1, q=p):
         return lib.sv_window_attention(q, p, p, six, n, heads, dim, dtype, p, p, buckets, p, reach,
-                                       0.25, p, None, None, None)
+                                       0.25, p, None, None)
 
     assert attend(n=0, q=None) == N.SV_OK
     assert attend(dtype=3) == N.SV_ERR_BAD_DTYPE
     assert attend(q=None) == N.SV_ERR_INVALID_ARGUMENT
     assert attend(buckets=0) == N.SV_ERR_INVALID_ARGUMENT
-    for bad in ({"dim": 129}, {"buckets": 24}, {"reach": 1024}, {"n": 2**25 + 1},
+    for bad in ({"dim": 129}, {"buckets": 26}, {"reach": 1024}, {"n": 2**25 + 1},
                 {"heads": 65536}):
         assert attend(**bad) == N.SV_ERR_UNSUPPORTED
     assert lib.sv_window_plan_bytes(10) == 320
@@ -212,4 +212,4 @@ def test_c_entry_points_check_before_any_launch():
     assert nbytes >= 2 * 27 * 8 + 2 * 100 * 4
     assert lib.sv_window_attention_backward(p, p, p, six, p, p, p, 100, 2, 16, 2, p, p, 3, p, 1,
                                             0.25, p, p, p, p, p, nbytes - 1,
-                                            None, None) == N.SV_ERR_WORKSPACE
+                                            None) == N.SV_ERR_WORKSPACE

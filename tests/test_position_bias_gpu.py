@@ -114,10 +114,10 @@ def _reference(x, q, k, v, table, lut, window, shift, dout=None):
                                                2.0**-14 * delta.abs().amax((1, 2))))
         count.index_add_(0, b.flatten(), torch.ones_like(b.flatten(), dtype=F64))
     if g is not None:
-        # the 16-bit kernels sum the table in fixed point: half a unit a pair, the unit 2^-16 of the
+        # the 16-bit kernels sum the table in fixed point: half a unit a pair, the unit 2^-17 of the
         # power of two above the head's largest |ds| (at least 2^-14 of the largest |delta|)
         # fp32: half of 2^-61 of the power of two above 2 n |g| |v|
-        half_unit = 2.0**-16 * top
+        half_unit = 2.0**-17 * top
         if dtype == torch.float32:
             half_unit = 2.0**-61 * 2 * n * g.norm(dim=2).amax(0) * v.norm(dim=2).amax(0)
         off["dtable"] += half_unit[:, None] * count
@@ -178,7 +178,7 @@ def test_large_window(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("reach,side", [(1, 1), (7, 7), (11, 11), (31, 5), (1023, 11)])
+@pytest.mark.parametrize("reach,side", [(1, 1), (7, 7), (12, 12), (31, 5), (1023, 12)])
 def test_tables(reach, side, dtype):
     _run(_voxels(220, 10, 1, reach), 2, 32, dtype, 8, (4, 4, 4), reach, side, seed=reach)
 
@@ -250,13 +250,10 @@ def test_table_entries_of_the_lowest_value(dtype):
                                     position_buckets=lut)
         return (out, *torch.autograd.grad(out, leaves, dout))
 
-    # head 0 keeps the bounds of the table with -inf (the softmax's running base, which may differ,
-    # changes roundings only)
-    got = run(table, q)
-    val, off = _reference(x, q, k, v, hidden, lut, 4, (0, 0, 0), dout)
-    for a, what in zip(got[:4], ("out", "dq", "dk", "dv")):
-        _close(a[:, 0], val[what][:, 0], off[what][:, 0], what)
-    _close(got[4][0], val["dtable"][0], off["dtable"][0], "dtable")
+    got, want = run(table, q), run(hidden, q)
+    for a, b in zip(got[:4], want[:4]):
+        assert torch.equal(a[:, 0], b[:, 0])
+    assert torch.equal(got[4][0], want[4][0])
     flat = table.clone()
     flat[1] = 0
     zero = q.clone()
