@@ -412,19 +412,19 @@ SV_API size_t sv_linear_workspace_bytes(int pass, int64_t m, int64_t k, int64_t 
 
 /* out = act(x weight^T * x_scale[i] * w_scale[j] + bias[j]) + residual, [m, n] contiguous in
  * `out_dtype`; bias, residual (rows `ld_res` apart, `out_dtype`) and the fp32 scales may be null.
- * `preact` (or null) receives the activation's argument, [m, n] in `out_dtype`. fp32 accumulation,
+ * `preact` (or null) receives the activation's argument, [m, n] in fp32. fp32 accumulation,
  * one rounding. dtype fp32 / fp16 / bf16 (out_dtype the same) or e4m3 (out_dtype fp16 / bf16).
  * fp16, bf16 and e4m3 run on the tensor cores; out must not overlap an operand. */
 SV_API int sv_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw,
                              const void* bias, const void* residual, int64_t ld_res,
                              const float* x_scale, const float* w_scale, int64_t m, int64_t k,
                              int64_t n, int dtype, int out_dtype, int activation, void* out,
-                             void* preact, void* workspace, size_t workspace_bytes,
+                             float* preact, void* workspace, size_t workspace_bytes,
                              int32_t* status, sv_stream_t stream);
 
 /* dz = dout * act'(preact), [m, n]; dbias = its column sums in a fixed order (null: not wanted).
  * Without an activation dz is dout: preact and dz are not used. */
-SV_API int sv_linear_backward_z(const void* dout, const void* preact, int64_t m, int64_t n,
+SV_API int sv_linear_backward_z(const void* dout, const float* preact, int64_t m, int64_t n,
                                 int dtype, int activation, void* dz, void* dbias, void* workspace,
                                 size_t workspace_bytes, sv_stream_t stream);
 
@@ -452,22 +452,24 @@ SV_API int sv_window_plan(const int32_t* coords, const int32_t* perm, const int3
  * dx, dy, dz: the key's coordinates minus the query's, clamped to +-reach (<= 1023); lut: int32
  * [2 reach + 1], values in [0, buckets) (others are clamped); table: [heads, buckets^3] in `dtype`,
  * buckets <= 25. `strides`: row and head strides of q, k, v in elements, channels contiguous.
- * out: contiguous. stats (or null): fp32 [heads, n, 2] by position, 8-byte aligned: the softmax's
- * maximum and 1 / sum, for the backward pass. A row whose every score is -inf gives zeros. */
+ * out: contiguous. For the backward pass, or null: stats, fp32 [heads, n, 2] by position, 8-byte
+ * aligned: the softmax's maximum and 1 / sum; out_rest, like out: what its rounding to fp16 / bf16
+ * left out (not written for fp32). A row whose every score is -inf gives zeros. */
 SV_API int sv_window_attention(const void* q, const void* k, const void* v,
                                const int64_t* strides, int64_t n, int heads, int dim, int dtype,
                                const void* plan, const void* table, int buckets,
-                               const int32_t* lut, int reach, float scale, void* out, float* lse,
-                               sv_stream_t stream);
+                               const int32_t* lut, int reach, float scale, void* out,
+                               void* out_rest, float* stats, sv_stream_t stream);
 
 /* Its gradients, from the forward pass's out (`o`) and stats: dq, dk, dv contiguous, and dtable
- * [heads, buckets^3] (null: not wanted), whose sums do not depend on the order of execution. */
+ * [heads, buckets^3] (null: not wanted), whose sums do not depend on the order of execution.
+ * o_rest: the forward pass's out_rest (null: taken as zeros, at half a step of `o` in dS). */
 SV_API size_t sv_window_attention_backward_workspace_bytes(int64_t n, int heads, int buckets);
 SV_API int sv_window_attention_backward(
     const void* q, const void* k, const void* v, const int64_t* strides, const void* o,
-    const void* dout, const float* stats, int64_t n, int heads, int dim, int dtype, const void* plan,
-    const void* table, int buckets, const int32_t* lut, int reach, float scale, void* dq, void* dk,
-    void* dv, void* dtable, void* workspace, size_t workspace_bytes, sv_stream_t stream);
+    const void* o_rest, const void* dout, const float* stats, int64_t n, int heads, int dim,
+    int dtype, const void* plan, const void* table, int buckets, const int32_t* lut, int reach,
+    float scale, void* dq, void* dk, void* dv, void* dtable, void* workspace, size_t workspace_bytes, sv_stream_t stream);
 
 /* ---- topology: occupancy -> coordinates, subdivision, attention windows --------------- */
 

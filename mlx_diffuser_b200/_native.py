@@ -123,12 +123,12 @@ _SIGNATURES = {
     "sv_window_attention": (
         _I32,
         [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _I32, _P, _I32, ctypes.c_float, _P, _P,
-         _P],
+         _P, _P],
     ),
     "sv_window_attention_backward_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
     "sv_window_attention_backward": (
         _I32,
-        [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _I32, _P, _I32,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _I32, _P, _I32,
          ctypes.c_float, _P, _P, _P, _P, _P, _SZ, _P],
     ),
     "sv_downsample_workspace_bytes": (_SZ, [_I64]),

@@ -239,7 +239,7 @@ extern "C" int sv_window_attention(const void* q, const void* k, const void* v,
                                    const int64_t* strides, int64_t n, int heads, int dim,
                                    int dtype, const void* plan, const void* table, int buckets,
                                    const int32_t* lut, int reach, float scale, void* out,
-                                   float* stats, sv_stream_t stream) {
+                                   void* out_rest, float* stats, sv_stream_t stream) {
   const int rc = check(n, heads, dim, dtype, buckets, reach, "sv_window_attention");
   if (rc != SV_OK) return rc;
   if (n == 0 || heads == 0 || dim == 0) return SV_OK;
@@ -248,7 +248,7 @@ extern "C" int sv_window_attention(const void* q, const void* k, const void* v,
   const int bad = check_strides(strides, "sv_window_attention");
   if (bad != SV_OK) return bad;
   AttnArgs a{};
-  a.q = q; a.k = k; a.v = v; a.out = out;
+  a.q = q; a.k = k; a.v = v; a.out = out; a.out_rest = dtype == SV_FLOAT32 ? nullptr : out_rest;
   a.q_row = strides[0]; a.q_head = strides[1];
   a.k_row = strides[2]; a.k_head = strides[3];
   a.v_row = strides[4]; a.v_head = strides[5];
@@ -269,7 +269,7 @@ extern "C" size_t sv_window_attention_backward_workspace_bytes(int64_t n, int he
 
 extern "C" int sv_window_attention_backward(
     const void* q, const void* k, const void* v, const int64_t* strides, const void* o,
-    const void* dout, const float* stats, int64_t n, int heads, int dim, int dtype, const void* plan,
+    const void* o_rest, const void* dout, const float* stats, int64_t n, int heads, int dim, int dtype, const void* plan,
     const void* table, int buckets, const int32_t* lut, int reach, float scale, void* dq, void* dk,
     void* dv, void* dtable, void* workspace, size_t workspace_bytes, sv_stream_t stream) {
   const int rc = check(n, heads, dim, dtype, buckets, reach, "sv_window_attention_backward");
@@ -291,6 +291,7 @@ extern "C" int sv_window_attention_backward(
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   AttnArgs a{};
   a.q = q; a.k = k; a.v = v; a.o = o; a.dout = dout;
+  a.o_rest = dtype == SV_FLOAT32 ? nullptr : o_rest;
   a.q_row = strides[0]; a.q_head = strides[1];
   a.k_row = strides[2]; a.k_head = strides[3];
   a.v_row = strides[4]; a.v_head = strides[5];

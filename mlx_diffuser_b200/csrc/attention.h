@@ -29,9 +29,9 @@ struct alignas(16) PlanRow {
 static_assert(sizeof(PlanRow) == 32, "sv_window_plan writes 32 bytes a row");
 
 struct AttnArgs {
-  const void *q, *k, *v, *o, *dout;  // [n, heads, dim], the last axis contiguous
+  const void *q, *k, *v, *o, *o_rest, *dout;  // [n, heads, dim], the last axis contiguous
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements
-  void *out, *dq, *dk, *dv;          // contiguous [n, heads, dim]
+  void *out, *out_rest, *dq, *dk, *dv;        // contiguous [n, heads, dim]
   const PlanRow* plan;               // [n]
   const void* table;                 // [heads, nb, nb, nb]
   const int32_t* lut;                // [2 * reach + 1]
@@ -125,6 +125,13 @@ __device__ __forceinline__ PlanRow plan_at(const PlanRow* plan, int64_t p) {
 
 constexpr int ATTN_CH = ATTN_MAX_DIM / 32;  // channels a lane sums
 
+// What rounding `x` to T left out, itself rounded: nothing for fp32, nor next to an overflow.
+template <typename T>
+__device__ __forceinline__ float rest_of(float x) {
+  const float r = x - to_f32(from_f32<T>(x));
+  return fabsf(r) < INFINITY ? r : 0.f;
+}
+
 // ---- one row of one head, by a warp: lanes along the other side's rows for the scores, along the
 // ---- head's channels for the sums, fp32 throughout
 
@@ -185,11 +192,15 @@ __device__ void row_forward(const AttnArgs& a, int64_t p, int h, float* s_q) {
     }
     top = m;
   }
-  T* out = static_cast<T*>(a.out) + (me.row * (int64_t)a.heads + h) * a.dim;
+  const int64_t own = (me.row * (int64_t)a.heads + h) * a.dim;
+  T* out = static_cast<T*>(a.out) + own;
 #pragma unroll
   for (int c = 0; c < ATTN_CH; ++c) {
     const int d = lane + 32 * c;
-    if (d < a.dim) out[d] = from_f32<T>(sum == 0.f ? 0.f : o[c] / sum);
+    const float x = sum == 0.f ? 0.f : o[c] / sum;
+    if (d < a.dim) out[d] = from_f32<T>(x);
+    if (d < a.dim && a.out_rest)
+      static_cast<T*>(a.out_rest)[own + d] = from_f32<T>(rest_of<T>(x));
   }
   if (lane == 0 && a.stats) a.stats[h * a.n + p] = row_stats(top, sum);
   __syncwarp();
@@ -208,13 +219,14 @@ __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
   const T* v = static_cast<const T*>(a.v) + h * a.v_head;
   const T* g = static_cast<const T*>(a.dout) + own;
   const T* o = static_cast<const T*>(a.o) + own;
+  const T* o_rest = a.o_rest ? static_cast<const T*>(a.o_rest) + own : nullptr;
   const int64_t cells = (int64_t)a.nb * a.nb * a.nb;
   const T* table = static_cast<const T*>(a.table) + h * cells;
   float delta = 0.f;
   for (int d = lane; d < a.dim; d += 32) {
     s_q[d] = to_f32(q[d]) * a.scale;
     s_g[d] = to_f32(g[d]);
-    delta = fmaf(s_g[d], to_f32(o[d]), delta);
+    delta = fmaf(s_g[d], to_f32(o[d]) + (o_rest ? to_f32(o_rest[d]) : 0.f), delta);
   }
   delta = warp_sum(delta);
   if (TABLE && lane == 0) a.delta[h * a.n + p] = delta;

@@ -121,24 +121,31 @@ __device__ __forceinline__ void load_tile(uint8_t* tile, const T* base, int row_
   }
 }
 
-// A 16-row accumulator through the warp's own part of a tile (`mine`) to the feature rows `rows`, in
-// 16-byte stores.
-template <typename T, int DP>
-__device__ __forceinline__ void store_rows(uint8_t* mine, const float (&o)[DP / 8][4], float s0,
-                                           float s1, const int32_t* rows, T* out, int heads,
-                                           int head, int dim, bool vec) {
+// A 16-row accumulator into the warp's own part of a tile (`mine`), rounded to T, or with REST what
+// that rounding leaves out.
+template <typename T, int DP, bool REST = false>
+__device__ __forceinline__ void put_rows(uint8_t* mine, const float (&o)[DP / 8][4], float s0,
+                                         float s1) {
   const int lane = threadIdx.x & 31;
   const int g = lane >> 2, c2 = 2 * (lane & 3);
-  __syncwarp();
+  auto pack = [](float x, float y) {
+    return REST ? pack2<T>(rest_of<T>(x), rest_of<T>(y)) : pack2<T>(x, y);
+  };
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) {
     *reinterpret_cast<uint32_t*>(mine + g * STRIDE<DP> + (n * 8 + c2) * 2) =
-        pack2<T>(o[n][0] * s0, o[n][1] * s0);
+        pack(o[n][0] * s0, o[n][1] * s0);
     *reinterpret_cast<uint32_t*>(mine + (g + 8) * STRIDE<DP> + (n * 8 + c2) * 2) =
-        pack2<T>(o[n][2] * s1, o[n][3] * s1);
+        pack(o[n][2] * s1, o[n][3] * s1);
   }
-  __syncwarp();
+}
+
+// Those 16 rows to the feature rows `rows`, in 16-byte stores.
+template <typename T, int DP>
+__device__ __forceinline__ void send_rows(const uint8_t* mine, const int32_t* rows, T* out,
+                                          int heads, int head, int dim, bool vec) {
   constexpr int CH = DP / 8;
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int i = 0; i < 16 * CH / 32; ++i) {
     const int c = lane + 32 * i;
@@ -156,6 +163,16 @@ __device__ __forceinline__ void store_rows(uint8_t* mine, const float (&o)[DP / 
         if (col * 8 + k < dim) dst[k] = e[k];
     }
   }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_rows(uint8_t* mine, const float (&o)[DP / 8][4], float s0,
+                                           float s1, const int32_t* rows, T* out, int heads,
+                                           int head, int dim, bool vec) {
+  __syncwarp();
+  put_rows<T, DP>(mine, o, s0, s1);
+  __syncwarp();
+  send_rows<T, DP>(mine, rows, out, heads, head, dim, vec);
 }
 
 struct KeyMeta {
@@ -590,8 +607,9 @@ __device__ __forceinline__ void walk(B& b, Load&& load, Body&& body, Ask&& ask, 
 // most tiles skip it; weights then reach 2^8 at most, which neither type nor the fp32 sums notice.
 constexpr float SLACK = 8.f;
 
-// MR: 16-row parts of a warp, whose products share the tile's fragments.
-template <typename T, int DP, int MR, int STAGES>
+// MR: 16-row parts of a warp, whose products share the tile's fragments. TRAIN: the backward pass's
+// inputs are kept too.
+template <typename T, int DP, int MR, int STAGES, bool TRAIN>
 __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
     attn_tc_kernel(AttnArgs a, int per_block, bool vec) {
   constexpr int BQ = 64 * MR;
@@ -703,6 +721,9 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
           load_tile<T, DP, KB>(tile + L::TILE, v, (int)a.v_row, rows, a.dim, vec);
         },
         body, [] { return false; }, [] {});
+    // the ring is free: the rests go there, a stretch a warp
+    static_assert(4 * MR * 16 * STRIDE<DP> <= STAGES * 2 * L::TILE, "room for the rests");
+    uint8_t* rest = smem + L::RING + row0 * STRIDE<DP>;
     uint32_t redo = 0;
 #pragma unroll
     for (int m = 0; m < MR; ++m) {
@@ -715,11 +736,23 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
         const float2 st = row_stats(base[m][r], x);
         inv[r] = st.y;
         const int at = row0 + 16 * m + g + 8 * r;
-        if (a.stats && c2 == 0 && sh.own_row[at] >= 0) a.stats[head * a.n + block * BQ + at] = st;
+        if (TRAIN && a.stats && c2 == 0 && sh.own_row[at] >= 0)
+          a.stats[head * a.n + block * BQ + at] = st;
       }
-      store_rows<T, DP>(mine + 16 * m * STRIDE<DP>, o[m], inv[0], inv[1], sh.own_row + row0 + 16 * m,
-                        static_cast<T*>(a.out), a.heads, head, a.dim, vec);
+      put_rows<T, DP>(mine + 16 * m * STRIDE<DP>, o[m], inv[0], inv[1]);
+      if constexpr (TRAIN)
+        put_rows<T, DP, true>(rest + 16 * m * STRIDE<DP>, o[m], inv[0], inv[1]);
       redo |= not_finite<DP>(o[m]) << (16 * m);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      const int32_t* rows = sh.own_row + row0 + 16 * m;
+      send_rows<T, DP>(mine + 16 * m * STRIDE<DP>, rows, static_cast<T*>(a.out), a.heads, head,
+                       a.dim, vec);
+      if (TRAIN && a.out_rest)
+        send_rows<T, DP>(rest + 16 * m * STRIDE<DP>, rows, static_cast<T*>(a.out_rest), a.heads,
+                         head, a.dim, vec);
     }
     again(redo, block * BQ + row0, mine,
           [&](int64_t p, float* f) { if (p < a.n) again_forward<T>(a, p, head, f); });
@@ -727,36 +760,44 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   }
 }
 
-// delta_i = dout_i . o_i by position: eight lanes a row and head.
+// delta_i = dout_i . o_i by position: eight lanes a row and head, a warp four heads of a row, a block
+// eight positions. o is taken with what its rounding left out: dS = P (dP - delta) is small next to
+// delta where a window has few rows, so half a step of o would be several of dS.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a, bool vec) {
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 8;  // head * n + position
   const int sub = threadIdx.x & 7;
+  const int64_t p = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int h = blockIdx.y * 4 + ((threadIdx.x >> 3) & 3);
+  const bool live = p < a.n && h < a.heads;
+  const int32_t row = live ? __ldg(&a.plan[p].row) : -1;
   float d = 0.f;
-  if (at < a.n * a.heads) {
-    const int64_t h = at / a.n, p = at - h * a.n;
-    const int32_t row = __ldg(&a.plan[p].row);
-    if (row >= 0) {
-      const int64_t from = ((int64_t)row * a.heads + h) * a.dim;
-      const T* g = static_cast<const T*>(a.dout) + from;
-      const T* o = static_cast<const T*>(a.o) + from;
-      if (vec) {
-        for (int c = sub * 8; c < a.dim; c += 64) {
-          const uint4 x = *reinterpret_cast<const uint4*>(g + c);
-          const uint4 y = *reinterpret_cast<const uint4*>(o + c);
-          const T* xe = reinterpret_cast<const T*>(&x);
-          const T* ye = reinterpret_cast<const T*>(&y);
+  if (row >= 0) {
+    const int64_t from = ((int64_t)row * a.heads + h) * a.dim;
+    const T* g = static_cast<const T*>(a.dout) + from;
+    const T* o = static_cast<const T*>(a.o) + from;
+    const T* rest = a.o_rest ? static_cast<const T*>(a.o_rest) + from : nullptr;
+    if (vec) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) d = fmaf(to_f32(xe[k]), to_f32(ye[k]), d);
-        }
-      } else {
-        for (int c = sub; c < a.dim; c += 8) d = fmaf(to_f32(g[c]), to_f32(o[c]), d);
+      for (int i = 0; i < ATTN_MAX_DIM / 64; ++i) {
+        const int c = sub * 8 + i * 64;
+        if (c >= a.dim) break;
+        const uint4 x = *reinterpret_cast<const uint4*>(g + c);
+        const uint4 y = *reinterpret_cast<const uint4*>(o + c);
+        const uint4 z = rest ? *reinterpret_cast<const uint4*>(rest + c) : make_uint4(0, 0, 0, 0);
+        const T* xe = reinterpret_cast<const T*>(&x);
+        const T* ye = reinterpret_cast<const T*>(&y);
+        const T* ze = reinterpret_cast<const T*>(&z);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d = fmaf(to_f32(xe[k]), to_f32(ye[k]) + to_f32(ze[k]), d);
       }
+    } else {
+      for (int c = sub; c < a.dim; c += 8)
+        d = fmaf(to_f32(g[c]), to_f32(o[c]) + (rest ? to_f32(rest[c]) : 0.f), d);
     }
   }
 #pragma unroll
   for (int s = 4; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-  if (sub == 0 && at < a.n * a.heads) a.delta[at] = d;
+  if (sub == 0 && live) a.delta[h * a.n + p] = d;
 }
 
 // The table's gradient in fixed point: a score gradient is at most 2^18 units (the head's largest is
@@ -1020,7 +1061,8 @@ bool wide(const void* p, int64_t row, int64_t head) {
 bool wide_rows(const AttnArgs& a) {
   const int64_t head = a.dim, row = (int64_t)a.heads * a.dim;
   return a.dim % 8 == 0 && wide(a.q, a.q_row, a.q_head) && wide(a.k, a.k_row, a.k_head) &&
-         wide(a.v, a.v_row, a.v_head) && wide(a.out, row, head) && wide(a.dout, row, head) &&
+         wide(a.v, a.v_row, a.v_head) && wide(a.out, row, head) && wide(a.out_rest, row, head) &&
+         wide(a.o, row, head) && wide(a.o_rest, row, head) && wide(a.dout, row, head) &&
          wide(a.dq, row, head) && wide(a.dk, row, head) && wide(a.dv, row, head);
 }
 
@@ -1039,16 +1081,16 @@ int allow_smem(K kernel, size_t bytes) {
   return SV_OK;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool TRAIN>
 int forward(const AttnArgs& a, cudaStream_t s) {
   // two 16-row parts a warp where their sums fit the registers
   constexpr int MR = DP <= 64 ? 2 : 1, STAGES = DP <= 64 ? 3 : 2;
   const size_t bytes = Layout<DP, 64 * MR, 1, STAGES>::TABLE + tables(a, false).total;
-  const int rc = allow_smem(attn_tc_kernel<T, DP, MR, STAGES>, bytes);
+  const int rc = allow_smem(attn_tc_kernel<T, DP, MR, STAGES, TRAIN>, bytes);
   if (rc != SV_OK) return rc;
   const int per = blocks_per_cta(a, 64 * MR, 9);
   const int64_t ctas = ((a.n + 64 * MR - 1) / (64 * MR) + per - 1) / per;
-  attn_tc_kernel<T, DP, MR, STAGES>
+  attn_tc_kernel<T, DP, MR, STAGES, TRAIN>
       <<<dim3((unsigned)ctas, a.heads), AT, bytes, s>>>(a, per, wide_rows(a));
   SV_LAUNCH_CHECK();
   return SV_OK;
@@ -1059,8 +1101,8 @@ int backward(const AttnArgs& a, void* dtable, cudaStream_t s) {
   constexpr int STAGES = 2;
   using L = Layout<DP, 64, 2, STAGES>;
   const bool vec = wide_rows(a);
-  attn_delta_kernel<T><<<(unsigned)((a.n * a.heads + 31) / 32), 256, 0, s>>>(
-      a, vec && aligned16(a.o));
+  attn_delta_kernel<T>
+      <<<dim3((unsigned)((a.n + 7) / 8), (unsigned)((a.heads + 3) / 4)), 256, 0, s>>>(a, vec);
   SV_LAUNCH_CHECK();
   const int per = blocks_per_cta(a, 64, 9);
   const dim3 grid((unsigned)(((a.n + 63) / 64 + per - 1) / per), a.heads);
@@ -1082,11 +1124,16 @@ int backward(const AttnArgs& a, void* dtable, cudaStream_t s) {
   return SV_OK;
 }
 
+template <typename T, bool TRAIN>
+int forward_dim(const AttnArgs& a, cudaStream_t s) {
+  if (a.dim <= 32) return forward<T, 32, TRAIN>(a, s);
+  if (a.dim <= 64) return forward<T, 64, TRAIN>(a, s);
+  return forward<T, 128, TRAIN>(a, s);
+}
+
 template <typename T>
 int forward_typed(const AttnArgs& a, cudaStream_t s) {
-  if (a.dim <= 32) return forward<T, 32>(a, s);
-  if (a.dim <= 64) return forward<T, 64>(a, s);
-  return forward<T, 128>(a, s);
+  return a.stats || a.out_rest ? forward_dim<T, true>(a, s) : forward_dim<T, false>(a, s);
 }
 
 template <typename T>

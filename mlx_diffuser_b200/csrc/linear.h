@@ -19,7 +19,8 @@ struct Operand {
 };
 
 // y = act(acc * row_scale[i] * col_scale[j] + bias[j]) + residual[i][j], every pointer optional;
-// `preact` receives the activation's argument. With `partial` set the kernel stores its raw fp32
+// `preact` receives the activation's argument in fp32: rounded to 16 bits it would put a third of a
+// step into every gradient, next to the step that rounding dz costs. With `partial` set the kernel stores its raw fp32
 // sums there ([splits][M][N]) and a second pass applies the rest.
 struct Epilogue {
   const void* bias;      // [N], out_dtype
@@ -28,7 +29,7 @@ struct Epilogue {
   const float* row_scale;
   const float* col_scale;
   void* out;     // [M][N] contiguous, out_dtype
-  void* preact;  // [M][N] contiguous, out_dtype
+  float* preact;  // [M][N] contiguous
   float* partial;
   int out_dtype;
   int act;
@@ -132,7 +133,7 @@ __device__ __forceinline__ void epilogue_store(const Epilogue& ep, int64_t i, in
   if (ep.row_scale) acc *= __ldg(ep.row_scale + i);
   if (ep.col_scale) acc *= __ldg(ep.col_scale + j);
   if (ep.bias) acc += to_f32(static_cast<const O*>(ep.bias)[j]);
-  if (ep.preact) static_cast<O*>(ep.preact)[i * n + j] = from_f32<O>(acc);
+  if (ep.preact) ep.preact[i * n + j] = acc;
   acc = activate(acc, ep.act);
   if (ep.residual) acc += to_f32(static_cast<const O*>(ep.residual)[i * ep.ld_res + j]);
   static_cast<O*>(ep.out)[i * n + j] = from_f32<O>(acc);

@@ -214,24 +214,20 @@ __device__ __forceinline__ void finish(const Epilogue& ep, float (&v)[R][W], con
 #pragma unroll
       for (int j = 0; j < W; ++j) v[i][j] += bias[j];
   }
-  auto store = [&](void* base) {
-    O* dst = static_cast<O*>(base) + row * n + col;
+  if (ep.preact) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (i * step < rows) {
+        float* dst = ep.preact + (row + i * step) * n + col;
         if constexpr (W == 8) {
-          uint4 raw;
-          O* e = reinterpret_cast<O*>(&raw);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) e[j] = from_f32<O>(v[i][j]);
-          *reinterpret_cast<uint4*>(dst + i * step * n) = raw;
+          *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(v[i]);
+          *reinterpret_cast<float4*>(dst + 4) = *reinterpret_cast<const float4*>(v[i] + 4);
         } else {
-          dst[i * step * n] = from_f32<O>(v[i][0]);
+          *dst = v[i][0];
         }
       }
     }
-  };
-  if (ep.preact) store(ep.preact);
+  }
   if (ep.act == SV_ACT_SILU) activate_all<SV_ACT_SILU>(v);
   else if (ep.act == SV_ACT_GELU) activate_all<SV_ACT_GELU>(v);
   else if (ep.act == SV_ACT_GELU_TANH) activate_all<SV_ACT_GELU_TANH>(v);
@@ -241,7 +237,21 @@ __device__ __forceinline__ void finish(const Epilogue& ep, float (&v)[R][W], con
 #pragma unroll
       for (int j = 0; j < W; ++j) v[i][j] += to_f32(res[i][j]);
   }
-  store(ep.out);
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (i * step < rows) {
+      O* dst = static_cast<O*>(ep.out) + (row + i * step) * n + col;
+      if constexpr (W == 8) {
+        uint4 raw;
+        O* e = reinterpret_cast<O*>(&raw);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = from_f32<O>(v[i][j]);
+        *reinterpret_cast<uint4*>(dst) = raw;
+      } else {
+        *dst = from_f32<O>(v[i][0]);
+      }
+    }
+  }
 }
 
 template <int BN, bool PAIR, typename O, bool F8>

@@ -36,32 +36,35 @@ def _strides(q, k, v):
                                 v.stride(1))
 
 
-def _forward(q, k, v, table, lut, plan, scale, keep_stats):
+def _forward(q, k, v, table, lut, plan, scale, train):
     n, heads, dim = q.shape
     dev = q.device
     out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
-    stats = torch.empty((heads, n, 2), dtype=torch.float32, device=dev) if keep_stats else None
+    stats = torch.empty((heads, n, 2), dtype=torch.float32, device=dev) if train else None
+    # what rounding `out` left out: the backward pass takes dS from a difference with dout . out
+    rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
     with N.on_device(dev):
         rc = N.load().sv_window_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), n, heads, dim,
             N.DTYPE_CODE[q.dtype], plan.data_ptr(), table.data_ptr(), table.shape[-1],
-            lut.data_ptr(), lut.numel() // 2, scale, out.data_ptr(), N.ptr(stats), N.stream(dev))
+            lut.data_ptr(), lut.numel() // 2, scale, out.data_ptr(), N.ptr(rest), N.ptr(stats),
+            N.stream(dev))
     N.check(rc, "sparse_self_attention")
-    return out, stats
+    return out, rest, stats
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, lut, plan, scale):
-        out, stats = _forward(q, k, v, table, lut, plan, scale, True)
+        out, rest, stats = _forward(q, k, v, table, lut, plan, scale, True)
         ctx.scale = scale
-        ctx.save_for_backward(q, k, v, table, lut, plan, out, stats)
+        ctx.save_for_backward(q, k, v, table, lut, plan, out, rest, stats)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, lut, plan, out, stats = ctx.saved_tensors
+        q, k, v, table, lut, plan, out, rest, stats = ctx.saved_tensors
         n, heads, dim = q.shape
         dev = q.device
         dout = dout.contiguous()
@@ -73,9 +76,9 @@ class _WindowAttention(torch.autograd.Function):
             ws = N.workspace(nbytes, dev)
             rc = lib.sv_window_attention_backward(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), out.data_ptr(),
-                dout.data_ptr(), stats.data_ptr(), n, heads, dim, N.DTYPE_CODE[q.dtype],
-                plan.data_ptr(), table.data_ptr(), table.shape[-1], lut.data_ptr(),
-                lut.numel() // 2, ctx.scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                N.ptr(rest), dout.data_ptr(), stats.data_ptr(), n, heads, dim,
+                N.DTYPE_CODE[q.dtype], plan.data_ptr(), table.data_ptr(), table.shape[-1],
+                lut.data_ptr(), lut.numel() // 2, ctx.scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                 N.ptr(dtable), ws.data_ptr(), nbytes, N.stream(dev))
         N.check(rc, "sparse_self_attention (backward)")
         return dq, dk, dv, dtable, None, None, None

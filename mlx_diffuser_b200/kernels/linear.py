@@ -41,7 +41,7 @@ def _forward(x, weight, bias, residual, activation, x_scale, w_scale, out_dtype,
     n = weight.shape[0]
     dev = x.device
     out = torch.empty((m, n), dtype=out_dtype, device=dev)
-    preact = torch.empty_like(out) if keep_preact else None
+    preact = torch.empty((m, n), dtype=torch.float32, device=dev) if keep_preact else None
     if out.numel() == 0:
         return out, preact
     code = N.DTYPE_CODE.get(x.dtype, N.SV_FLOAT8_E4M3)

@@ -196,7 +196,7 @@ def test_c_entry_points_check_before_any_launch():
 
     def attend(n=4, heads=2, dim=16, dtype=2, buckets=3, reach=1, q=p):
         return lib.sv_window_attention(q, p, p, six, n, heads, dim, dtype, p, p, buckets, p, reach,
-                                       0.25, p, None, None)
+                                       0.25, p, None, None, None)
 
     assert attend(n=0, q=None) == N.SV_OK
     assert attend(dtype=3) == N.SV_ERR_BAD_DTYPE
@@ -210,6 +210,6 @@ def test_c_entry_points_check_before_any_launch():
     assert lib.sv_window_plan(p, p, p, 0, 5, p, None, None) == N.SV_ERR_INVALID_ARGUMENT
     nbytes = lib.sv_window_attention_backward_workspace_bytes(100, 2, 3)
     assert nbytes >= 2 * 27 * 8 + 2 * 100 * 4
-    assert lib.sv_window_attention_backward(p, p, p, six, p, p, p, 100, 2, 16, 2, p, p, 3, p, 1,
-                                            0.25, p, p, p, p, p, nbytes - 1,
+    assert lib.sv_window_attention_backward(p, p, p, six, p, None, p, p, 100, 2, 16, 2, p, p, 3, p,
+                                            1, 0.25, p, p, p, p, p, nbytes - 1,
                                             None) == N.SV_ERR_WORKSPACE
