@@ -396,17 +396,11 @@ typedef enum sv_activation {
   SV_ACT_GELU_TANH = 3 /* the tanh form */
 } sv_activation;
 
-/* The product a workspace is for. */
-typedef enum sv_linear_pass {
-  SV_LINEAR_FORWARD = 0,
-  SV_LINEAR_DZ = 1,
-  SV_LINEAR_DX = 2,
-  SV_LINEAR_DW = 3
-} sv_linear_pass;
+typedef enum sv_linear_pass { SV_LINEAR_FORWARD = 0, SV_LINEAR_BACKWARD = 1 } sv_linear_pass;
 
-/* Workspace of one pass over x [m, k] and weight [n, k]. `copies`: bit 0 / bit 1 set when the
- * product's first / second operand (x, weight; dz, weight; dz, x) is not 16-byte aligned or its
- * row stride is not a multiple of 16 bytes; it is then copied into padded rows. */
+/* Workspace of one pass over x [m, k] and weight [n, k]. `copies`: bit 0 / bit 1 set when x / weight
+ * is not 16-byte aligned or its row stride is not a multiple of 16 bytes (it is then copied into
+ * padded rows); bit 2, of the backward pass, when it has an activation or dout is not so aligned. */
 SV_API size_t sv_linear_workspace_bytes(int pass, int64_t m, int64_t k, int64_t n, int dtype,
                                         int copies);
 
@@ -422,19 +416,15 @@ SV_API int sv_linear_forward(const void* x, int64_t ldx, const void* weight, int
                              float* preact, void* workspace, size_t workspace_bytes,
                              int32_t* status, sv_stream_t stream);
 
-/* dz = dout * act'(preact), [m, n]; dbias = its column sums in a fixed order (null: not wanted).
- * Without an activation dz is dout: preact and dz are not used. */
-SV_API int sv_linear_backward_z(const void* dout, const float* preact, int64_t m, int64_t n,
-                                int dtype, int activation, void* dz, void* dbias, void* workspace,
-                                size_t workspace_bytes, sv_stream_t stream);
-
-/* dx [m, k] = dz [m, n] weight [n, k]; dw [n, k] = dz^T x. dz and the results contiguous. */
-SV_API int sv_linear_dx(const void* dz, const void* weight, int64_t ldw, int64_t m, int64_t k,
-                        int64_t n, int dtype, void* dx, void* workspace, size_t workspace_bytes,
-                        int32_t* status, sv_stream_t stream);
-SV_API int sv_linear_dw(const void* dz, const void* x, int64_t ldx, int64_t m, int64_t k,
-                        int64_t n, int dtype, void* dw, void* workspace, size_t workspace_bytes,
-                        int32_t* status, sv_stream_t stream);
+/* Its gradients for x, weight and bias (each null where it is not wanted), contiguous, in `dtype`
+ * (fp32 / fp16 / bf16): with dz = dout * act'(preact) rounded to `dtype` (dout itself without an
+ * activation), dx = dz weight, dw = dz^T x, dbias = the column sums of the unrounded dz. Every sum has
+ * a fixed order. dout: [m, n] contiguous; preact: the forward pass's. */
+SV_API int sv_linear_backward(const void* dout, const float* preact, const void* x, int64_t ldx,
+                              const void* weight, int64_t ldw, int64_t m, int64_t k, int64_t n,
+                              int dtype, int activation, void* dx, void* dw, void* dbias,
+                              void* workspace, size_t workspace_bytes, int32_t* status,
+                              sv_stream_t stream);
 
 /* ---- windowed attention with a learned relative position bias --------------------------- */
 

@@ -44,7 +44,7 @@ SV_FLOAT8_E4M3 = 3  # operands of the projection, output of the root-mean-square
 
 # sv_activation / sv_linear_pass
 ACTIVATION_CODE = {None: 0, "none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
-SV_LINEAR_FORWARD, SV_LINEAR_DZ, SV_LINEAR_DX, SV_LINEAR_DW = range(4)
+SV_LINEAR_FORWARD, SV_LINEAR_BACKWARD = range(2)
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -113,11 +113,10 @@ _SIGNATURES = {
         [_P, _I64, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _P,
          _SZ, _P, _P],
     ),
-    "sv_linear_backward_z": (
-        _I32, [_P, _P, _I64, _I64, _I32, _I32, _P, _P, _P, _SZ, _P]
+    "sv_linear_backward": (
+        _I32,
+        [_P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I32, _I32, _P, _P, _P, _P, _SZ, _P, _P],
     ),
-    "sv_linear_dx": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _SZ, _P, _P]),
-    "sv_linear_dw": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _SZ, _P, _P]),
     "sv_window_plan_bytes": (_SZ, [_I64]),
     "sv_window_plan": (_I32, [_P, _P, _P, _I64, _I64, _P, _P, _P]),
     "sv_window_attention": (

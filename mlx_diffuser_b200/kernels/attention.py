@@ -39,8 +39,8 @@ def _strides(q, k, v):
 def _forward(q, k, v, table, lut, plan, scale, train):
     n, heads, dim = q.shape
     dev = q.device
-    out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
-    stats = torch.empty((heads, n, 2), dtype=torch.float32, device=dev) if train else None
+    out = q.new_empty((n, heads, dim))
+    stats = q.new_empty((heads, n, 2), dtype=torch.float32) if train else None
     # what rounding `out` left out: the backward pass takes dS from a difference with dout . out
     rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
     with N.on_device(dev):
@@ -68,7 +68,7 @@ class _WindowAttention(torch.autograd.Function):
         n, heads, dim = q.shape
         dev = q.device
         dout = dout.contiguous()
-        dq, dk, dv = (torch.empty((n, heads, dim), dtype=q.dtype, device=dev) for _ in range(3))
+        dq, dk, dv = (q.new_empty((n, heads, dim)) for _ in range(3))
         dtable = torch.empty_like(table) if ctx.needs_input_grad[3] else None
         lib = N.load()
         nbytes = lib.sv_window_attention_backward_workspace_bytes(n, heads, table.shape[-1])
@@ -90,7 +90,8 @@ def biased_window_attention(q, k, v, table, lut, plan, scale: float) -> torch.Te
 
     q, k, v = (t if t.stride(2) == 1 or t.shape[2] <= 1 else t.contiguous() for t in (q, k, v))
     table, lut = table.contiguous(), lut.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, table)):
+    if torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
         return _WindowAttention.apply(q, k, v, table, lut, plan, scale)
     return _forward(q, k, v, table, lut, plan, scale, False)[0]
 

@@ -5,6 +5,8 @@ it is given an activation or a residual."""
 
 from __future__ import annotations
 
+import math
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -26,30 +28,28 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _unaligned(t: torch.Tensor) -> bool:
-    return t.data_ptr() % 16 != 0 or _ld(t) * t.element_size() % 16 != 0
-
-
-def _workspace(which: int, m: int, k: int, n: int, code: int, a: torch.Tensor, b: torch.Tensor):
-    nbytes = N.load().sv_linear_workspace_bytes(which, m, k, n, code,
-                                                _unaligned(a) + 2 * _unaligned(b))
-    return (N.workspace(nbytes, a.device) if nbytes else None), nbytes
+def _unaligned(address: int, ld: int, t: torch.Tensor) -> bool:
+    return (address | ld * t.element_size()) & 15 != 0
 
 
 def _forward(x, weight, bias, residual, activation, x_scale, w_scale, out_dtype, keep_preact):
     m, k = x.shape
     n = weight.shape[0]
     dev = x.device
-    out = torch.empty((m, n), dtype=out_dtype, device=dev)
-    preact = torch.empty((m, n), dtype=torch.float32, device=dev) if keep_preact else None
-    if out.numel() == 0:
+    out = weight.new_empty((m, n), dtype=out_dtype)
+    preact = weight.new_empty((m, n), dtype=torch.float32) if keep_preact else None
+    if m == 0 or n == 0:
         return out, preact
     code = N.DTYPE_CODE.get(x.dtype, N.SV_FLOAT8_E4M3)
+    px, ldx, pw, ldw = x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight)
+    copies = _unaligned(px, ldx, x) + 2 * _unaligned(pw, ldw, weight)
+    lib = N.load()
     with N.on_device(dev):
-        ws, nbytes = _workspace(N.SV_LINEAR_FORWARD, m, k, n, code, x, weight)
-        rc = N.load().sv_linear_forward(
-            x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight), N.ptr(bias), N.ptr(residual),
-            _ld(residual) if residual is not None else 0, N.ptr(x_scale), N.ptr(w_scale), m, k, n,
+        nbytes = lib.sv_linear_workspace_bytes(N.SV_LINEAR_FORWARD, m, k, n, code, copies)
+        ws = N.workspace(nbytes, dev) if nbytes else None
+        rc = lib.sv_linear_forward(
+            px, ldx, pw, ldw, N.ptr(bias), N.ptr(residual),
+            0 if residual is None else _ld(residual), N.ptr(x_scale), N.ptr(w_scale), m, k, n,
             code, N.DTYPE_CODE[out_dtype], N.ACTIVATION_CODE[activation], out.data_ptr(),
             N.ptr(preact), N.ptr(ws), nbytes, N.status_word(dev).data_ptr(), N.stream(dev))
     N.check(rc, "linear")
@@ -69,40 +69,29 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         x, weight, preact = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         dout = dout.contiguous()
         m, k = x.shape
         n = weight.shape[0]
-        dev, dtype = x.device, x.dtype
-        code = N.DTYPE_CODE[dtype]
-        lib = N.load()
-        dx = dw = db = None
-        dz = dout
-        with N.on_device(dev):
-            status, stream = N.status_word(dev).data_ptr(), N.stream(dev)
-            if need_b or (preact is not None and (need_x or need_w)):
-                if preact is not None:
-                    dz = torch.empty_like(dout)
-                db = torch.empty(n, dtype=dtype, device=dev) if need_b else None
-                nbytes = lib.sv_linear_workspace_bytes(N.SV_LINEAR_DZ, m, k, n, code, 0)
-                ws = N.workspace(nbytes, dev) if need_b else None
-                rc = lib.sv_linear_backward_z(
-                    dout.data_ptr(), N.ptr(preact), m, n, code,
-                    N.ACTIVATION_CODE[ctx.activation], dz.data_ptr(), N.ptr(db), N.ptr(ws),
-                    nbytes, stream)
-                N.check(rc, "linear (backward)")
-            if need_x:
-                dx = torch.empty((m, k), dtype=dtype, device=dev)
-                ws, nbytes = _workspace(N.SV_LINEAR_DX, m, k, n, code, dz, weight)
-                rc = lib.sv_linear_dx(dz.data_ptr(), weight.data_ptr(), _ld(weight), m, k, n, code,
-                                      dx.data_ptr(), N.ptr(ws), nbytes, status, stream)
-                N.check(rc, "linear (input gradient)")
-            if need_w:
-                dw = torch.empty((n, k), dtype=dtype, device=dev)
-                ws, nbytes = _workspace(N.SV_LINEAR_DW, m, k, n, code, dz, x)
-                rc = lib.sv_linear_dw(dz.data_ptr(), x.data_ptr(), _ld(x), m, k, n, code,
-                                      dw.data_ptr(), N.ptr(ws), nbytes, status, stream)
-                N.check(rc, "linear (weight gradient)")
+        dev = x.device
+        code = N.DTYPE_CODE[x.dtype]
+        dx = x.new_empty((m, k)) if need_x else None
+        dw = x.new_empty((n, k)) if need_w else None
+        db = x.new_empty((n,)) if need_b else None
+        if need_x or need_w or need_b:
+            px, pw, pd = x.data_ptr(), weight.data_ptr(), dout.data_ptr()
+            ldx, ldw = _ld(x), _ld(weight)
+            copies = (_unaligned(px, ldx, x) + 2 * _unaligned(pw, ldw, weight)
+                      + 4 * (preact is not None or _unaligned(pd, n, dout)))
+            lib = N.load()
+            with N.on_device(dev):
+                nbytes = lib.sv_linear_workspace_bytes(N.SV_LINEAR_BACKWARD, m, k, n, code, copies)
+                rc = lib.sv_linear_backward(
+                    pd, N.ptr(preact), px, ldx, pw, ldw, m, k, n, code,
+                    N.ACTIVATION_CODE[ctx.activation], N.ptr(dx), N.ptr(dw), N.ptr(db),
+                    N.workspace(nbytes, dev).data_ptr(), nbytes, N.status_word(dev).data_ptr(),
+                    N.stream(dev))
+            N.check(rc, "linear (backward)")
         return dx, dw, db, dout if need_r else None, None
 
 
@@ -153,30 +142,33 @@ def linear(
         if out_dtype not in (None, x.dtype):
             raise ValueError(f"linear: the result has the operands' type {x.dtype}")
         out_dtype = x.dtype
-    shape = (*x.shape[:-1], n)
+    dev = x.device
+    rows = x.shape[:-1]
     for name, t, want, dtype in (
+        ("weight", weight, weight.shape, x.dtype),
         ("bias", bias, (n,), out_dtype),
-        ("residual", residual, shape, out_dtype),
-        ("x_scale", x_scale, x.shape[:-1], torch.float32),
+        ("residual", residual, (*rows, n), out_dtype),
+        ("x_scale", x_scale, rows, torch.float32),
         ("weight_scale", weight_scale, (n,), torch.float32),
     ):
-        if t is not None and (tuple(t.shape) != tuple(want) or t.dtype != dtype):
+        if t is None:
+            continue
+        if t.shape != want or t.dtype != dtype:
             raise ValueError(f"linear: {name} must be a {tuple(want)} {dtype} tensor, got "
                              f"{tuple(t.shape)} {t.dtype}")
-    for name, t in (("weight", weight), ("bias", bias), ("residual", residual),
-                    ("x_scale", x_scale), ("weight_scale", weight_scale)):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"linear: {name} is on {t.device}, x on {x.device}")
-    grads = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, weight, bias, residual))
+        if t.device != dev:
+            raise ValueError(f"linear: {name} is on {t.device}, x on {dev}")
+    grads = torch.is_grad_enabled() and (
+        x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+        or (residual is not None and residual.requires_grad))
     if grads and e4m3:
         raise ValueError("linear: 8-bit operands have no gradients")
     N.require_cuda(x, "x")
-    x2 = _row_major(x.reshape(-1, x.shape[-1]) if x.ndim != 2 else x)
+    x2 = _row_major(x if x.ndim == 2 else x.reshape(math.prod(rows), x.shape[-1]))
     w2 = _row_major(weight)
     r2 = None
     if residual is not None:
-        r2 = _row_major(residual.reshape(-1, n) if residual.ndim != 2 else residual)
+        r2 = _row_major(residual if x.ndim == 2 else residual.reshape(x2.shape[0], n))
     b2 = None if bias is None else bias.contiguous()
     if grads:
         out = _Linear.apply(x2, w2, b2, r2, activation)
@@ -184,7 +176,7 @@ def linear(
         xs = None if x_scale is None else x_scale.reshape(-1).contiguous()
         ws = None if weight_scale is None else weight_scale.contiguous()
         out, _ = _forward(x2, w2, b2, r2, activation, xs, ws, out_dtype, False)
-    return out if x.ndim == 2 else out.reshape(shape)
+    return out if x.ndim == 2 else out.reshape(*rows, n)
 
 
 __all__ = ["linear"]

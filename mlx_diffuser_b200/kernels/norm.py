@@ -104,10 +104,10 @@ def _rms_forward(x, residual, weight, eps, quantize, keep_rstd):
     n, c = x.shape
     dev = x.device
     lib = N.load()
-    h = torch.empty((n, c), dtype=x.dtype, device=dev) if residual is not None else None
-    rstd = torch.empty(n, dtype=torch.float32, device=dev) if keep_rstd else None
-    scale = torch.empty(n, dtype=torch.float32, device=dev) if quantize else None
-    out = torch.empty((n, c), dtype=torch.float8_e4m3fn if quantize else x.dtype, device=dev)
+    h = x.new_empty((n, c)) if residual is not None else None
+    rstd = x.new_empty((n,), dtype=torch.float32) if keep_rstd else None
+    scale = x.new_empty((n,), dtype=torch.float32) if quantize else None
+    out = x.new_empty((n, c), dtype=torch.float8_e4m3fn) if quantize else x.new_empty((n, c))
     code = N.DTYPE_CODE[x.dtype]
     with N.on_device(dev):
         rc = lib.sv_rms_norm(
@@ -145,8 +145,8 @@ class _RmsNorm(torch.autograd.Function):
         lib = N.load()
         dy = dy.contiguous()
         dh = None if dh is None else dh.contiguous()
-        dx = torch.empty((n, c), dtype=h.dtype, device=dev)
-        dw = torch.empty(c, dtype=torch.float32, device=dev) if need_w else None
+        dx = h.new_empty((n, c))
+        dw = h.new_empty((c,), dtype=torch.float32) if need_w else None
         with N.on_device(dev):
             nbytes = lib.sv_rms_norm_backward_workspace_bytes(c) if need_w else 0
             ws = N.workspace(nbytes, dev) if need_w else None
@@ -188,15 +188,16 @@ def rms_norm(
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"rms_norm: residual must be a {tuple(x.shape)} {x.dtype} tensor, got "
                          f"{tuple(residual.shape)} {residual.dtype}")
-    if weight is not None and (tuple(weight.shape) != (c,) or not weight.is_floating_point()):
+    if weight is not None and (weight.shape != (c,) or not weight.is_floating_point()):
         raise ValueError(f"rms_norm: weight must be a float tensor of shape ({c},)")
     for name, t in (("residual", residual), ("weight", weight)):
         if t is not None and t.device != x.device:
             raise ValueError(f"rms_norm: {name} is on {t.device}, x on {x.device}")
     if not eps >= 0:
         raise ValueError("rms_norm: eps must not be negative")
-    grads = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, residual, weight))
+    grads = torch.is_grad_enabled() and (
+        x.requires_grad or (residual is not None and residual.requires_grad)
+        or (weight is not None and weight.requires_grad))
     if grads and quantize:
         raise ValueError("rms_norm: the 8-bit output has no gradients")
     N.require_cuda(x, "x")

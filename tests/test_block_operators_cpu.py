@@ -184,13 +184,23 @@ def test_c_entry_points_check_before_any_launch():
     # an operand that TMA cannot read needs its padded copy
     assert lib.sv_linear_workspace_bytes(N.SV_LINEAR_FORWARD, 20, 63, 64, 2, 3) >= 84 * 128
     assert forward(k=63, ldx=63, ldw=63) == N.SV_ERR_WORKSPACE
-    assert lib.sv_linear_backward_z(p, p, 4, 8, 2, 1, p, p, None, 0, None) == N.SV_ERR_WORKSPACE
-    assert lib.sv_linear_backward_z(p, None, 4, 8, 2, 1, p, None, None, 0,
-                                    None) == N.SV_ERR_INVALID_ARGUMENT
-    assert lib.sv_linear_backward_z(p, None, 4, 8, 2, 0, None, None, None, 0, None) == N.SV_OK
-    assert lib.sv_linear_dx(p, p, 7, 20, 8, 8, 2, p, None, 0, None,
-                            None) == N.SV_ERR_INVALID_ARGUMENT
-    assert lib.sv_linear_dw(p, p, 8, 20, 8, 8, 5, p, None, 0, None, None) == N.SV_ERR_BAD_DTYPE
+    def backward(m=4, k=8, n=8, dtype=2, act=1, z=p, ldx=8, ldw=8, dx=p, dw=p, db=p, ws=None,
+                 nbytes=0):
+        return lib.sv_linear_backward(p, z, p, ldx, p, ldw, m, k, n, dtype, act, dx, dw, db, ws,
+                                      nbytes, None, None)
+
+    assert backward() == N.SV_ERR_WORKSPACE
+    need = lib.sv_linear_workspace_bytes(N.SV_LINEAR_BACKWARD, 4, 8, 8, 2, 4)
+    assert need >= 4 * 16 + 4 * 8
+    assert backward(ws=p, nbytes=need - 1) == N.SV_ERR_WORKSPACE
+    assert backward(z=None) == N.SV_ERR_INVALID_ARGUMENT
+    assert backward(dx=None, dw=None, db=None) == N.SV_OK
+    assert backward(n=0, dx=None) == backward(m=0, dw=None, db=None) == N.SV_OK
+    assert backward(ldw=7) == backward(ldx=7) == N.SV_ERR_INVALID_ARGUMENT
+    assert backward(act=4) == N.SV_ERR_INVALID_ARGUMENT
+    assert backward(dtype=5) == backward(dtype=3) == N.SV_ERR_BAD_DTYPE
+    assert backward(k=-1) == N.SV_ERR_INVALID_ARGUMENT
+    assert backward(k=2**31) == N.SV_ERR_UNSUPPORTED
 
     six = (ctypes.c_int64 * 6)(*[64] * 6)
 
