@@ -88,6 +88,48 @@ __global__ void __launch_bounds__(256)
   plan[p] = r;
 }
 
+// The blocks of the plan: a thread per window, blockIdx.y for the two sizes.
+__global__ void __launch_bounds__(128)
+    window_blocks_kernel(const int32_t* __restrict__ offsets, int64_t groups, int64_t n,
+                         uint8_t* __restrict__ plan, int32_t* status) {
+  const int64_t g = (int64_t)blockIdx.x * 128 + threadIdx.x;
+  if (g >= groups) return;
+  const int which = blockIdx.y, size = which ? 128 : 64, half = size / 2;
+  const PlanBlocks at = plan_blocks(n);
+  int2* blocks = reinterpret_cast<int2*>(plan + at.block[which]);
+  auto bound = [&](int64_t i) { return max(0, min((int)n, __ldg(offsets + i))); };
+  const int start = bound(g), end = bound(g + 1), rows = end - start;
+  if (rows <= 0) return;
+  int stop = end;
+  if (rows <= half) {
+    // The first small window of its stretch takes the others along. Empty windows between them are
+    // passed over, though not without end; both loops go by the same rule.
+    constexpr int GAP = 64;
+    for (int64_t i = g - 1, gap = 0; i >= 0 && gap <= GAP; --i, ++gap) {
+      const int s = bound(i), e = bound(i + 1);
+      if (e <= s) continue;
+      if (e == start && e - s <= half && s / half == start / half) return;
+      break;
+    }
+    for (int64_t i = g + 1, gap = 0; i < groups && gap <= GAP; ++i, ++gap) {
+      const int s = bound(i), e = bound(i + 1);
+      if (e <= s) continue;
+      if (s != stop || e - s > half || s / half != start / half) break;
+      stop = e;
+      gap = -1;
+    }
+  }
+  const int pieces = (stop - start + size - 1) / size;
+  const int first = atomicAdd(reinterpret_cast<int*>(plan + at.count) + which, pieces);
+  for (int i = 0; i < pieces; ++i) {
+    if (first + i >= at.cap[which]) {  // windows that overlap
+      report(status, SV_DEVICE_BAD_INDEX);
+      return;
+    }
+    const int p = start + i * size;
+    blocks[first + i] = make_int2(p, min(size, stop - p));
+  }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_kernel(AttnArgs a) {
@@ -216,7 +258,9 @@ Layout layout(int64_t n, int heads, int nb) {
 
 using namespace sv;
 
-extern "C" size_t sv_window_plan_bytes(int64_t n) { return n > 0 ? (size_t)n * sizeof(PlanRow) : 0; }
+extern "C" size_t sv_window_plan_bytes(int64_t n) {
+  return n > 0 && n <= (1 << 25) ? (size_t)plan_blocks(n).total : 0;
+}
 
 extern "C" int sv_window_plan(const int32_t* coords, const int32_t* perm, const int32_t* offsets,
                               int64_t groups, int64_t n, void* plan, int32_t* status,
@@ -224,13 +268,20 @@ extern "C" int sv_window_plan(const int32_t* coords, const int32_t* perm, const 
   if (n < 0 || groups < 0) SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_window_plan: negative size");
   if (n > (1 << 25)) SV_FAIL(SV_ERR_UNSUPPORTED, "sv_window_plan: at most 2^25 rows");
   if (n == 0) return SV_OK;
-  if (!coords || !perm || !offsets || !plan || groups < 1 || groups > n || !aligned16(coords) || !aligned16(plan))
-    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_window_plan: null or misaligned pointer, or not 1 to n groups");
+  if (!coords || !perm || !offsets || !plan || groups < 1 || groups > n || !aligned16(coords) ||
+      !aligned16(plan))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT,
+            "sv_window_plan: null or misaligned pointer, or not 1 to n groups");
+  uint8_t* bytes = static_cast<uint8_t*>(plan);
+  SV_CUDA_TRY(cudaMemsetAsync(bytes + plan_blocks(n).count, 0, 16, to_stream(stream)));
   window_plan_kernel<<<(unsigned)((n + 255) / 256), 256, 0, to_stream(stream)>>>(
       coords, perm, offsets, groups, n, static_cast<PlanRow*>(plan), status);
   SV_LAUNCH_CHECK();
   window_span_kernel<<<(unsigned)groups, 128, 0, to_stream(stream)>>>(
       offsets, groups, n, static_cast<PlanRow*>(plan));
+  SV_LAUNCH_CHECK();
+  window_blocks_kernel<<<dim3((unsigned)((groups + 127) / 128), 2), 128, 0, to_stream(stream)>>>(
+      offsets, groups, n, bytes, status);
   SV_LAUNCH_CHECK();
   return SV_OK;
 }

@@ -28,6 +28,27 @@ struct alignas(16) PlanRow {
 };
 static_assert(sizeof(PlanRow) == 32, "sv_window_plan writes 32 bytes a row");
 
+// Behind the rows: the blocks of at most 64 and at most 128 positions that the fp16 / bf16 kernels
+// take, each {first position, positions} and in no particular order. A window of more than half a
+// block has blocks of its own; smaller ones that start in the same stretch of half a block share one.
+// So all rows of a block of a large window see the same positions: against blocks of 64 or 128
+// consecutive positions, whichever windows those cut, 84% instead of 60% of the tiles need no mask,
+// and no warp waits for another window's tiles.
+struct PlanBlocks {
+  int64_t count, block[2], cap[2], total;  // byte offsets of int32 [2] and int2 [cap]; 64, 128
+};
+__host__ __device__ inline PlanBlocks plan_blocks(int64_t n) {
+  PlanBlocks b;
+  b.count = n * (int64_t)sizeof(PlanRow);
+  // at most 2 n / B blocks of large windows, and one of small ones per stretch of B / 2
+  b.cap[0] = n / 16 + 2;
+  b.cap[1] = n / 32 + 2;
+  b.block[0] = b.count + 16;
+  b.block[1] = b.block[0] + (b.cap[0] + 1) / 2 * 16;
+  b.total = b.block[1] + (b.cap[1] + 1) / 2 * 16;
+  return b;
+}
+
 struct AttnArgs {
   const void *q, *k, *v, *o, *o_rest, *dout;  // [n, heads, dim], the last axis contiguous
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements

@@ -21,6 +21,7 @@
 // unrounded.
 #include <limits.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "attention.h"
@@ -28,6 +29,7 @@
 namespace sv {
 namespace {
 
+constexpr int WAVES = 9;  // CTAs an SM over a call's course (three run at a time)
 constexpr int AT = 128;  // threads: four warps of 16 rows, or of 16 MR
 constexpr int KB = 32;   // positions of a tile
 
@@ -254,22 +256,26 @@ struct Block {
         joint[i] = (uint16_t)((lut[i / width()] * a.nb + lut[i % width()]) * a.nb);
   }
 
-  // The block's rows and the positions their windows cover.
-  __device__ void begin(int64_t p0) {
+  // The block's rows, `count` from position p0 on, and the positions their windows cover. Rows behind
+  // them stand in for the first one, so that they need no mask of their own; nothing of theirs is
+  // stored.
+  __device__ void begin(int p0, int count) {
     if (threadIdx.x < 2) s.range[threadIdx.x] = threadIdx.x ? INT_MIN : INT_MAX;
     __syncthreads();
     bool narrow = true;
     if (threadIdx.x < BQ) {
-      const int64_t p = p0 + threadIdx.x;
-      PlanRow r{};
-      r.row = -1;
-      if (p < a.n) r = plan_at(a.plan, p);
+      const bool in = (int)threadIdx.x < count;
+      PlanRow r = plan_at(a.plan, in ? p0 + threadIdx.x : p0);
       if (r.row < 0) {
         r.start = r.end = 0;
       } else {
-        atomicMin(&s.range[0], r.start);
-        atomicMax(&s.range[1], r.end);
         narrow = r.span <= a.reach;
+        if (in) {
+          atomicMin(&s.range[0], r.start);
+          atomicMax(&s.range[1], r.end);
+        } else {
+          r.row = -1;
+        }
       }
       s.own[threadIdx.x] = r;
       s.own_row[threadIdx.x] = r.row;
@@ -454,7 +460,7 @@ template <int ROWS>
 __device__ __forceinline__ Reach warp_reach(const PlanRow* own) {
   const int lane = threadIdx.x & 31;
   const PlanRow& r = own[lane % ROWS];
-  const bool any = r.end > r.start;
+  const bool any = r.row >= 0;
   Reach w;
   w.lo = __reduce_min_sync(0xffffffffu, any ? r.start : INT_MAX);
   w.hi = __reduce_max_sync(0xffffffffu, any ? r.end : INT_MIN);
@@ -509,12 +515,12 @@ __device__ __forceinline__ uint32_t not_finite(const float (&o)[DP / 8][4]) {
 }
 
 template <typename F>
-__device__ __forceinline__ void again(uint32_t rows, int64_t p0, uint8_t* scratch, F&& row) {
+__device__ __forceinline__ void again(uint32_t rows, int first, uint8_t* scratch, F&& row) {
   while (rows) {  // the same in all lanes
     const int r = __ffs(rows) - 1;
     rows &= rows - 1;
     __syncwarp();
-    row(p0 + r, reinterpret_cast<float*>(scratch));
+    row(first + r, reinterpret_cast<float*>(scratch));
   }
 }
 
@@ -557,6 +563,21 @@ __host__ __device__ inline Tables tables(const AttnArgs& a, bool grad) {
     t.total += width * width * 2;
   }
   return t;
+}
+
+// The plan's list of blocks of BQ positions.
+struct BlockList {
+  const int2* at;
+  int count;
+};
+template <int BQ>
+__device__ __forceinline__ BlockList block_list(const AttnArgs& a) {
+  static_assert(BQ == 64 || BQ == 128, "the plan's sizes");
+  constexpr int which = BQ == 128;
+  const PlanBlocks b = plan_blocks(a.n);
+  const uint8_t* plan = reinterpret_cast<const uint8_t*>(a.plan);
+  const int count = __ldg(reinterpret_cast<const int*>(plan + b.count) + which);
+  return {reinterpret_cast<const int2*>(plan + b.block[which]), (int)min((int64_t)count, b.cap[which])};
 }
 
 template <typename T, int BQ>
@@ -611,10 +632,12 @@ constexpr float SLACK = 8.f;
 // inputs are kept too.
 template <typename T, int DP, int MR, int STAGES, bool TRAIN>
 __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
-    attn_tc_kernel(AttnArgs a, int per_block, bool vec) {
+    attn_tc_kernel(AttnArgs a, bool vec) {
   constexpr int BQ = 64 * MR;
   using L = Layout<DP, BQ, 1, STAGES>;
   extern __shared__ __align__(16) uint8_t smem[];
+  const BlockList list = block_list<BQ>(a);
+  if ((int)blockIdx.x >= list.count) return;
   Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, false);
   Shared<BQ>& sh = b.s;
   const int head = blockIdx.y;
@@ -628,9 +651,9 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   const float scale = a.scale * ATTN_LOG2E;
   const uint32_t table = smem_u32(b.table);
   b.stage_tables();
-  const int64_t first = (int64_t)blockIdx.x * per_block;
-  for (int64_t block = first; block < first + per_block && block * BQ < a.n; ++block) {
-    b.begin(block * BQ);
+  for (int block = blockIdx.x; block < list.count; block += gridDim.x) {
+    const int2 at = __ldg(list.at + block);
+    b.begin(at.x, at.y);
     load_tile<T, DP, BQ>(smem, q, (int)a.q_row, sh.own_row, a.dim, vec);
     const PlanRow* own = sh.own + row0 + g;
     const Reach w = warp_reach<16 * MR>(sh.own + row0);
@@ -735,9 +758,9 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
         x += __shfl_xor_sync(0xffffffffu, x, 2);
         const float2 st = row_stats(base[m][r], x);
         inv[r] = st.y;
-        const int at = row0 + 16 * m + g + 8 * r;
-        if (TRAIN && a.stats && c2 == 0 && sh.own_row[at] >= 0)
-          a.stats[head * a.n + block * BQ + at] = st;
+        const int i = row0 + 16 * m + g + 8 * r;
+        if (TRAIN && a.stats && c2 == 0 && sh.own_row[i] >= 0)
+          a.stats[head * a.n + at.x + i] = st;
       }
       put_rows<T, DP>(mine + 16 * m * STRIDE<DP>, o[m], inv[0], inv[1]);
       if constexpr (TRAIN)
@@ -754,8 +777,9 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
         send_rows<T, DP>(rest + 16 * m * STRIDE<DP>, rows, static_cast<T*>(a.out_rest), a.heads,
                          head, a.dim, vec);
     }
-    again(redo, block * BQ + row0, mine,
-          [&](int64_t p, float* f) { if (p < a.n) again_forward<T>(a, p, head, f); });
+    again(redo, row0, mine, [&](int i, float* f) {
+      if (sh.own_row[i] >= 0) again_forward<T>(a, at.x + i, head, f);
+    });
     __syncthreads();
   }
 }
@@ -818,10 +842,12 @@ __device__ __forceinline__ int unit_exponent(const AttnArgs& a, int head) {
 // dq and the table's gradient.
 template <typename T, int DP, int STAGES, bool TABLE>
 __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
-    attn_dq_tc_kernel(AttnArgs a, int per_block, bool vec) {
+    attn_dq_tc_kernel(AttnArgs a, bool vec) {
   constexpr int BQ = 64;
   using L = Layout<DP, BQ, 2, STAGES>;
   extern __shared__ __align__(16) uint8_t smem[];
+  const BlockList list = block_list<BQ>(a);
+  if ((int)blockIdx.x >= list.count) return;
   Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, TABLE);
   Shared<BQ>& sh = b.s;
   const int cells = b.cells();
@@ -858,9 +884,9 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
       __syncthreads();
     }
   };
-  const int64_t first = (int64_t)blockIdx.x * per_block;
-  for (int64_t block = first; block < first + per_block && block * BQ < a.n; ++block) {
-    b.begin(block * BQ);
+  for (int block = blockIdx.x; block < list.count; block += gridDim.x) {
+    const int2 at = __ldg(list.at + block);
+    b.begin(at.x, at.y);
     load_tile<T, DP, BQ>(smem, q, (int)a.q_row, sh.own_row, a.dim, vec);
     load_tile<T, DP, BQ>(smem + L::OWN_TILE, dout, g_row, sh.own_row, a.dim, vec);
     const PlanRow* own = sh.own + warp * 16 + g;
@@ -869,7 +895,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const bool live = own[8 * r].row >= 0;
-      const int64_t p = head * a.n + block * BQ + warp * 16 + g + 8 * r;
+      const int64_t p = head * a.n + at.x + warp * 16 + g + 8 * r;
       const float2 st = live ? a.stats[p] : make_float2(0.f, 0.f);
       top[r] = st.x;
       inv[r] = st.y;
@@ -928,8 +954,9 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
         body, [&] { return TABLE && spent * unit > LIMIT; }, flush);
     store_rows<T, DP>(mine, dq[0], a.scale, a.scale, sh.own_row + warp * 16, static_cast<T*>(a.dq),
                       a.heads, head, a.dim, vec);
-    again(not_finite<DP>(dq[0]), block * BQ + warp * 16, mine,
-          [&](int64_t p, float* f) { if (p < a.n) again_dq<T>(a, p, head, f); });
+    again(not_finite<DP>(dq[0]), warp * 16, mine, [&](int i, float* f) {
+      if (sh.own_row[i] >= 0) again_dq<T>(a, at.x + i, head, f);
+    });
     __syncthreads();
   }
   flush();
@@ -938,10 +965,12 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
 // dk and dv, and the largest |dS| of the head: the block's rows are keys, the tiles queries.
 template <typename T, int DP, int STAGES, bool TABLE>
 __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
-    attn_dkv_tc_kernel(AttnArgs a, int per_block, bool vec) {
+    attn_dkv_tc_kernel(AttnArgs a, bool vec) {
   constexpr int BQ = 64;
   using L = Layout<DP, BQ, 2, STAGES>;
   extern __shared__ __align__(16) uint8_t smem[];
+  const BlockList list = block_list<BQ>(a);
+  if ((int)blockIdx.x >= list.count) return;
   Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, false);
   Shared<BQ>& sh = b.s;
   const uint32_t table = smem_u32(b.table);
@@ -957,9 +986,9 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   const float scale = a.scale * ATTN_LOG2E;
   float most = 0.f;
   b.stage_tables();
-  const int64_t first = (int64_t)blockIdx.x * per_block;
-  for (int64_t block = first; block < first + per_block && block * BQ < a.n; ++block) {
-    b.begin(block * BQ);
+  for (int block = blockIdx.x; block < list.count; block += gridDim.x) {
+    const int2 at = __ldg(list.at + block);
+    b.begin(at.x, at.y);
     load_tile<T, DP, BQ>(smem, k, (int)a.k_row, sh.own_row, a.dim, vec);
     load_tile<T, DP, BQ>(smem + L::OWN_TILE, v, (int)a.v_row, sh.own_row, a.dim, vec);
     const PlanRow* own = sh.own + warp * 16 + g;
@@ -1024,8 +1053,9 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
                       a.heads, head, a.dim, vec);
     store_rows<T, DP>(mine + L::OWN_TILE, dv[0], 1.f, 1.f, sh.own_row + warp * 16,
                       static_cast<T*>(a.dv), a.heads, head, a.dim, vec);
-    again(not_finite<DP>(dk[0]) | not_finite<DP>(dv[0]), block * BQ + warp * 16, mine,
-          [&](int64_t p, float* f) { if (p < a.n) again_dkv<T>(a, p, head, f); });
+    again(not_finite<DP>(dk[0]) | not_finite<DP>(dv[0]), warp * 16, mine, [&](int i, float* f) {
+      if (sh.own_row[i] >= 0) again_dkv<T>(a, at.x + i, head, f);
+    });
     __syncthreads();
   }
   if constexpr (TABLE) {
@@ -1066,12 +1096,11 @@ bool wide_rows(const AttnArgs& a) {
          wide(a.dq, row, head) && wide(a.dk, row, head) && wide(a.dv, row, head);
 }
 
-// Blocks of BQ rows of one head that a CTA takes in turn, so that it stages the table (and adds up its
-// gradient) once: as many as still leave `waves` CTAs for each SM.
-int blocks_per_cta(const AttnArgs& a, int bq, int waves) {
-  const int64_t blocks = (a.n + bq - 1) / bq;
-  const int64_t per = blocks * a.heads / ((int64_t)num_sms() * waves);
-  return (int)(per < 1 ? 1 : (per > 16 ? 16 : per));
+// CTAs of one head: each takes every that-many-th block, so that it stages the table (and adds up its
+// gradient) once. `waves` for each SM over all heads; the list is at most `cap` long.
+unsigned ctas_of(const AttnArgs& a, int bq, int waves) {
+  const int64_t want = ((int64_t)num_sms() * waves + a.heads - 1) / a.heads;
+  return (unsigned)std::min(want, plan_blocks(a.n).cap[bq == 128]);
 }
 
 template <typename K>
@@ -1088,10 +1117,8 @@ int forward(const AttnArgs& a, cudaStream_t s) {
   const size_t bytes = Layout<DP, 64 * MR, 1, STAGES>::TABLE + tables(a, false).total;
   const int rc = allow_smem(attn_tc_kernel<T, DP, MR, STAGES, TRAIN>, bytes);
   if (rc != SV_OK) return rc;
-  const int per = blocks_per_cta(a, 64 * MR, 9);
-  const int64_t ctas = ((a.n + 64 * MR - 1) / (64 * MR) + per - 1) / per;
   attn_tc_kernel<T, DP, MR, STAGES, TRAIN>
-      <<<dim3((unsigned)ctas, a.heads), AT, bytes, s>>>(a, per, wide_rows(a));
+      <<<dim3(ctas_of(a, 64 * MR, WAVES), a.heads), AT, bytes, s>>>(a, wide_rows(a));
   SV_LAUNCH_CHECK();
   return SV_OK;
 }
@@ -1104,17 +1131,16 @@ int backward(const AttnArgs& a, void* dtable, cudaStream_t s) {
   attn_delta_kernel<T>
       <<<dim3((unsigned)((a.n + 7) / 8), (unsigned)((a.heads + 3) / 4)), 256, 0, s>>>(a, vec);
   SV_LAUNCH_CHECK();
-  const int per = blocks_per_cta(a, 64, 9);
-  const dim3 grid((unsigned)(((a.n + 63) / 64 + per - 1) / per), a.heads);
+  const dim3 grid(ctas_of(a, 64, WAVES), a.heads);
   size_t bytes = L::TABLE + tables(a, false).total;
   int rc = allow_smem(attn_dkv_tc_kernel<T, DP, STAGES, TABLE>, bytes);
   if (rc != SV_OK) return rc;
-  attn_dkv_tc_kernel<T, DP, STAGES, TABLE><<<grid, AT, bytes, s>>>(a, per, vec);
+  attn_dkv_tc_kernel<T, DP, STAGES, TABLE><<<grid, AT, bytes, s>>>(a, vec);
   SV_LAUNCH_CHECK();
   bytes = L::TABLE + tables(a, TABLE).total;
   rc = allow_smem(attn_dq_tc_kernel<T, DP, STAGES, TABLE>, bytes);
   if (rc != SV_OK) return rc;
-  attn_dq_tc_kernel<T, DP, STAGES, TABLE><<<grid, AT, bytes, s>>>(a, per, vec);
+  attn_dq_tc_kernel<T, DP, STAGES, TABLE><<<grid, AT, bytes, s>>>(a, vec);
   SV_LAUNCH_CHECK();
   if constexpr (TABLE) {
     const unsigned blocks = (unsigned)((a.nb * a.nb * a.nb + 255) / 256);

@@ -215,7 +215,7 @@ def test_c_entry_points_check_before_any_launch():
     for bad in ({"dim": 129}, {"buckets": 26}, {"reach": 1024}, {"n": 2**25 + 1},
                 {"heads": 65536}):
         assert attend(**bad) == N.SV_ERR_UNSUPPORTED
-    assert lib.sv_window_plan_bytes(10) == 320
+    assert lib.sv_window_plan_bytes(10) >= 10 * 32 and lib.sv_window_plan_bytes(0) == 0
     assert lib.sv_window_plan(None, None, None, 0, 0, None, None, None) == N.SV_OK
     assert lib.sv_window_plan(p, p, p, 0, 5, p, None, None) == N.SV_ERR_INVALID_ARGUMENT
     nbytes = lib.sv_window_attention_backward_workspace_bytes(100, 2, 3)
