@@ -444,12 +444,17 @@ SV_API int sv_window_plan(const int32_t* coords, const int32_t* perm, const int3
  * buckets <= 25. `strides`: row and head strides of q, k, v in elements, channels contiguous.
  * out: contiguous. For the backward pass, or null: stats, fp32 [heads, n, 2] by position, 8-byte
  * aligned: the softmax's maximum and 1 / sum; out_rest, like out: what its rounding to fp16 / bf16
- * left out (not written for fp32). A row whose every score is -inf gives zeros. */
+ * left out (not written for fp32). A row whose every score is -inf gives zeros. `windows`: how many the
+ * plan has; from their mean length it is decided whether the walk over a window's rows is split, with
+ * the parts' sums in the workspace (0 bytes: not split). */
+SV_API size_t sv_window_attention_workspace_bytes(int64_t n, int heads, int dim, int dtype,
+                                                  int64_t windows);
 SV_API int sv_window_attention(const void* q, const void* k, const void* v,
                                const int64_t* strides, int64_t n, int heads, int dim, int dtype,
-                               const void* plan, const void* table, int buckets,
+                               const void* plan, int64_t windows, const void* table, int buckets,
                                const int32_t* lut, int reach, float scale, void* out,
-                               void* out_rest, float* stats, sv_stream_t stream);
+                               void* out_rest, float* stats, void* workspace,
+                               size_t workspace_bytes, sv_stream_t stream);
 
 /* Its gradients, from the forward pass's out (`o`) and stats: dq, dk, dv contiguous, and dtable
  * [heads, buckets^3] (null: not wanted), whose sums do not depend on the order of execution.

@@ -119,10 +119,11 @@ _SIGNATURES = {
     ),
     "sv_window_plan_bytes": (_SZ, [_I64]),
     "sv_window_plan": (_I32, [_P, _P, _P, _I64, _I64, _P, _P, _P]),
+    "sv_window_attention_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I64]),
     "sv_window_attention": (
         _I32,
-        [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _I32, _P, _I32, ctypes.c_float, _P, _P,
-         _P, _P],
+        [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _I64, _P, _I32, _P, _I32, ctypes.c_float, _P,
+         _P, _P, _P, _SZ, _P],
     ),
     "sv_window_attention_backward_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
     "sv_window_attention_backward": (

@@ -219,8 +219,10 @@ int backward_rows(const AttnArgs& a, void* dtable, cudaStream_t s) {
   return SV_OK;
 }
 
+bool float_type(int d) { return d == SV_FLOAT32 || d == SV_FLOAT16 || d == SV_BFLOAT16; }
+
 int check(int64_t n, int heads, int dim, int dtype, int nb, int reach, const char* what) {
-  if (dtype != SV_FLOAT32 && dtype != SV_FLOAT16 && dtype != SV_BFLOAT16)
+  if (!float_type(dtype))
     SV_FAIL(SV_ERR_BAD_DTYPE, std::string(what) + ": unknown dtype");
   if (n < 0 || heads < 0 || dim < 0 || nb < 1 || reach < 0)
     SV_FAIL(SV_ERR_INVALID_ARGUMENT, std::string(what) + ": negative size");
@@ -238,6 +240,21 @@ int check_strides(const int64_t* strides, const char* what) {
     if (strides[i] < 0 || strides[i] > (1 << 30))
       SV_FAIL(SV_ERR_UNSUPPORTED, std::string(what) + ": strides must be between 0 and 2^30");
   return SV_OK;
+}
+
+// Workspace of a split forward pass: the parts' sums.
+struct PartLayout {
+  int parts;
+  size_t stats, total;  // the sums are at the start
+};
+PartLayout part_layout(int64_t n, int heads, int dim, int dtype, int64_t windows) {
+  PartLayout l{1, 0, 0};
+  if (dtype != SV_FLOAT32) l.parts = attention_tc_parts(n, heads, dim, windows);
+  if (l.parts == 1) return l;
+  const size_t rows = (size_t)l.parts * heads * n;
+  l.stats = align_up(rows * dim * 4, 256);
+  l.total = l.stats + align_up(rows * 8, 256);
+  return l;
 }
 
 // Workspace of the backward pass: fixed-point table, norms, delta.
@@ -286,11 +303,18 @@ extern "C" int sv_window_plan(const int32_t* coords, const int32_t* perm, const 
   return SV_OK;
 }
 
+extern "C" size_t sv_window_attention_workspace_bytes(int64_t n, int heads, int dim, int dtype,
+                                                      int64_t windows) {
+  if (n < 0 || heads < 0 || dim < 0 || dim > ATTN_MAX_DIM || !float_type(dtype)) return 0;
+  return part_layout(n, heads, dim, dtype, windows).total;
+}
+
 extern "C" int sv_window_attention(const void* q, const void* k, const void* v,
                                    const int64_t* strides, int64_t n, int heads, int dim,
-                                   int dtype, const void* plan, const void* table, int buckets,
-                                   const int32_t* lut, int reach, float scale, void* out,
-                                   void* out_rest, float* stats, sv_stream_t stream) {
+                                   int dtype, const void* plan, int64_t windows,
+                                   const void* table, int buckets, const int32_t* lut, int reach,
+                                   float scale, void* out, void* out_rest, float* stats,
+                                   void* workspace, size_t workspace_bytes, sv_stream_t stream) {
   const int rc = check(n, heads, dim, dtype, buckets, reach, "sv_window_attention");
   if (rc != SV_OK) return rc;
   if (n == 0 || heads == 0 || dim == 0) return SV_OK;
@@ -307,6 +331,14 @@ extern "C" int sv_window_attention(const void* q, const void* k, const void* v,
   a.table = table; a.lut = lut; a.stats = reinterpret_cast<float2*>(stats);
   a.n = n; a.heads = heads; a.dim = dim; a.nb = buckets; a.reach = reach; a.scale = scale;
   cudaStream_t s = to_stream(stream);
+  const PartLayout l = part_layout(n, heads, dim, dtype, windows);
+  a.parts = l.parts;
+  if (l.parts > 1) {
+    if (!workspace || workspace_bytes < l.total || !aligned16(workspace))
+      SV_FAIL(SV_ERR_WORKSPACE, "sv_window_attention: workspace too small or unaligned");
+    a.part_out = static_cast<float*>(workspace);
+    a.part_stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + l.stats);
+  }
   if (dtype != SV_FLOAT32) return attention_tc_forward(a, dtype == SV_BFLOAT16, s);
   attn_rows_kernel<float><<<row_grid(a), 32 * ROW_WARPS, 0, s>>>(a);
   SV_LAUNCH_CHECK();

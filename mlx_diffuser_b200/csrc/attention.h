@@ -15,6 +15,7 @@ constexpr int ATTN_MAX_HEADS = 65535;
 // attention_tc.cu: the fp16 / bf16 kernels.
 struct AttnArgs;
 int attention_tc_forward(const AttnArgs& a, bool bf16, cudaStream_t s);
+int attention_tc_parts(int64_t n, int heads, int dim, int64_t windows);
 int attention_tc_backward(const AttnArgs& a, bool bf16, void* dtable, cudaStream_t s);
 
 // One row of the attention plan, in window order: the coordinates, the window's range of
@@ -61,8 +62,11 @@ struct AttnArgs {
   unsigned long long* dtable;        // [heads, nb^3] fixed point, or null
   unsigned* norms;                   // [heads, 2]: bits of max |dout_i|^2 and max |v_j|^2 (fp32
                                      // path), or of max |dS| (fp16 / bf16)
+  float2* part_stats;                // parts > 1: [parts, heads, n] by position, base and sum
+  float* part_out;                   // and [parts, heads, n, dim], not yet divided by the sum
   int64_t n;
   int heads, dim, nb, reach;
+  int parts;                         // of every block's positions (fp16 / bf16 forward pass)
   float scale;
 };
 

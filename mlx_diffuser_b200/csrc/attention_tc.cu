@@ -32,6 +32,9 @@ namespace {
 constexpr int WAVES = 9;  // CTAs an SM over a call's course (three run at a time)
 constexpr int AT = 128;  // threads: four warps of 16 rows, or of 16 MR
 constexpr int KB = 32;   // positions of a tile
+// Rows of a block in the forward pass: two 16-row parts a warp, whose products share the tile's
+// fragments (8,192 x 6 x 128 fp16: 678 us with one, 651 with two).
+constexpr int FORWARD_ROWS = 128;
 
 // Tiles hold DP channels a row (the head's, padded with zeros) at a stride that is an odd multiple
 // of 16 bytes, so the 8 rows of a matrix fragment fall into different banks.
@@ -256,10 +259,12 @@ struct Block {
         joint[i] = (uint16_t)((lut[i / width()] * a.nb + lut[i % width()]) * a.nb);
   }
 
-  // The block's rows, `count` from position p0 on, and the positions their windows cover. Rows behind
-  // them stand in for the first one, so that they need no mask of their own; nothing of theirs is
-  // stored.
-  __device__ void begin(int p0, int count) {
+  // The block's rows, `count` from position p0 on, and the positions their windows cover, of which part
+  // `part` of `parts` is walked. STAND_IN: rows behind the last see what the first one does, so that
+  // they cost no mask; nothing of theirs is stored. Without it they see nothing, as the backward
+  // pass needs them to, which takes sums and maxima over all of a warp's pairs.
+  template <bool STAND_IN>
+  __device__ void begin(int p0, int count, int part = 0, int parts = 1) {
     if (threadIdx.x < 2) s.range[threadIdx.x] = threadIdx.x ? INT_MIN : INT_MAX;
     __syncthreads();
     bool narrow = true;
@@ -275,6 +280,7 @@ struct Block {
           atomicMax(&s.range[1], r.end);
         } else {
           r.row = -1;
+          if (!STAND_IN) r.start = r.end = 0;
         }
       }
       s.own[threadIdx.x] = r;
@@ -284,6 +290,11 @@ struct Block {
     mode = !narrow ? GENERAL : (identity ? LINEAR : (joint != nullptr ? JOINT : GENERAL));
     j0 = s.range[0];
     tiles = s.range[1] > j0 ? (s.range[1] - j0 + KB - 1) / KB : 0;
+    if (parts > 1) {
+      const int per = (tiles + parts - 1) / parts;
+      j0 += part * per * KB;
+      tiles = max(0, min(per, tiles - part * per));
+    }
   }
 
   // By one warp: a position a lane.
@@ -653,7 +664,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   b.stage_tables();
   for (int block = blockIdx.x; block < list.count; block += gridDim.x) {
     const int2 at = __ldg(list.at + block);
-    b.begin(at.x, at.y);
+    b.template begin<true>(at.x, at.y, blockIdx.z, a.parts);
     load_tile<T, DP, BQ>(smem, q, (int)a.q_row, sh.own_row, a.dim, vec);
     const PlanRow* own = sh.own + row0 + g;
     const Reach w = warp_reach<16 * MR>(sh.own + row0);
@@ -744,6 +755,29 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
           load_tile<T, DP, KB>(tile + L::TILE, v, (int)a.v_row, rows, a.dim, vec);
         },
         body, [] { return false; }, [] {});
+    if (a.parts > 1) {
+      const int64_t first = ((int64_t)blockIdx.z * a.heads + head) * a.n + at.x;
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float x = sum[m][r];
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          const int i = row0 + 16 * m + g + 8 * r;
+          if (sh.own_row[i] < 0) continue;
+          if (c2 == 0) a.part_stats[first + i] = make_float2(base[m][r], x);
+          float* dst = a.part_out + (first + i) * a.dim;
+#pragma unroll
+          for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (n * 8 + c2 + e < a.dim) dst[n * 8 + c2 + e] = o[m][n][2 * r + e];
+        }
+      }
+      __syncthreads();
+      continue;
+    }
     // the ring is free: the rests go there, a stretch a warp
     static_assert(4 * MR * 16 * STRIDE<DP> <= STAGES * 2 * L::TILE, "room for the rests");
     uint8_t* rest = smem + L::RING + row0 * STRIDE<DP>;
@@ -782,6 +816,49 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
     });
     __syncthreads();
   }
+}
+
+// The parts of a split walk, joined in order: a warp per row and head. Rows that come out not finite
+// are computed again, as in the kernel above.
+constexpr int JOIN_WARPS = 8;
+template <typename T>
+__global__ void __launch_bounds__(32 * JOIN_WARPS) attn_join_kernel(AttnArgs a) {
+  __shared__ float scratch[JOIN_WARPS][ATTN_MAX_DIM];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y;
+  const int64_t p = (int64_t)blockIdx.x * JOIN_WARPS + warp;
+  if (p >= a.n) return;
+  const int32_t row = __ldg(&a.plan[p].row);
+  if (row < 0) return;
+  float top = -3.402823466e38f, sum = 0.f, o[ATTN_CH] = {};
+  for (int z = 0; z < a.parts; ++z)
+    top = fmaxf(top, a.part_stats[((int64_t)z * a.heads + h) * a.n + p].x);
+  for (int z = 0; z < a.parts; ++z) {
+    const int64_t at = ((int64_t)z * a.heads + h) * a.n + p;
+    const float2 st = a.part_stats[at];
+    const float w = exp2f(st.x - top);
+    sum = fmaf(w, st.y, sum);
+#pragma unroll
+    for (int c = 0; c < ATTN_CH; ++c)
+      if (lane + 32 * c < a.dim) o[c] = fmaf(w, a.part_out[at * a.dim + lane + 32 * c], o[c]);
+  }
+  bool finite = true;
+#pragma unroll
+  for (int c = 0; c < ATTN_CH; ++c) finite = finite && fabsf(o[c]) < INFINITY;
+  if (!__all_sync(0xffffffffu, finite)) {
+    again_forward<T>(a, p, h, scratch[warp]);
+    return;
+  }
+  const float2 st = row_stats(top, sum);
+  const int64_t own = ((int64_t)row * a.heads + h) * a.dim;
+#pragma unroll
+  for (int c = 0; c < ATTN_CH; ++c) {
+    const int d = lane + 32 * c;
+    if (d >= a.dim) continue;
+    const float x = o[c] * st.y;
+    static_cast<T*>(a.out)[own + d] = from_f32<T>(x);
+    if (a.out_rest) static_cast<T*>(a.out_rest)[own + d] = from_f32<T>(rest_of<T>(x));
+  }
+  if (lane == 0 && a.stats) a.stats[h * a.n + p] = st;
 }
 
 // delta_i = dout_i . o_i by position: eight lanes a row and head, a warp four heads of a row, a block
@@ -886,7 +963,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   };
   for (int block = blockIdx.x; block < list.count; block += gridDim.x) {
     const int2 at = __ldg(list.at + block);
-    b.begin(at.x, at.y);
+    b.template begin<false>(at.x, at.y);
     load_tile<T, DP, BQ>(smem, q, (int)a.q_row, sh.own_row, a.dim, vec);
     load_tile<T, DP, BQ>(smem + L::OWN_TILE, dout, g_row, sh.own_row, a.dim, vec);
     const PlanRow* own = sh.own + warp * 16 + g;
@@ -988,7 +1065,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   b.stage_tables();
   for (int block = blockIdx.x; block < list.count; block += gridDim.x) {
     const int2 at = __ldg(list.at + block);
-    b.begin(at.x, at.y);
+    b.template begin<false>(at.x, at.y);
     load_tile<T, DP, BQ>(smem, k, (int)a.k_row, sh.own_row, a.dim, vec);
     load_tile<T, DP, BQ>(smem + L::OWN_TILE, v, (int)a.v_row, sh.own_row, a.dim, vec);
     const PlanRow* own = sh.own + warp * 16 + g;
@@ -1112,14 +1189,18 @@ int allow_smem(K kernel, size_t bytes) {
 
 template <typename T, int DP, bool TRAIN>
 int forward(const AttnArgs& a, cudaStream_t s) {
-  // two 16-row parts a warp where their sums fit the registers
-  constexpr int MR = DP <= 64 ? 2 : 1, STAGES = DP <= 64 ? 3 : 2;
+  constexpr int MR = FORWARD_ROWS / 64, STAGES = DP <= 64 ? 3 : 2;
   const size_t bytes = Layout<DP, 64 * MR, 1, STAGES>::TABLE + tables(a, false).total;
   const int rc = allow_smem(attn_tc_kernel<T, DP, MR, STAGES, TRAIN>, bytes);
   if (rc != SV_OK) return rc;
   attn_tc_kernel<T, DP, MR, STAGES, TRAIN>
-      <<<dim3(ctas_of(a, 64 * MR, WAVES), a.heads), AT, bytes, s>>>(a, wide_rows(a));
+      <<<dim3(ctas_of(a, 64 * MR, WAVES), a.heads, a.parts), AT, bytes, s>>>(a, wide_rows(a));
   SV_LAUNCH_CHECK();
+  if (a.parts > 1) {
+    attn_join_kernel<T><<<dim3((unsigned)((a.n + JOIN_WARPS - 1) / JOIN_WARPS), a.heads),
+                          32 * JOIN_WARPS, 0, s>>>(a);
+    SV_LAUNCH_CHECK();
+  }
   return SV_OK;
 }
 
@@ -1172,6 +1253,30 @@ int backward_typed(const AttnArgs& a, void* dtable, cudaStream_t s) {
 }
 
 }  // namespace
+
+// Parts of every block's positions in the forward pass. Few blocks of long windows leave CTAs idle (8,192
+// rows of 6 heads x 128 in two windows are 384 blocks for 296 resident CTAs: two rounds, the second a
+// third full), so the walk is split where that shortens the estimated time: rounds of CTAs, each as
+// many tiles long, against a pass that joins the parts' fp32 sums. Windows of a few tiles are left
+// whole. Estimates in us: a tile of 32 positions 1 + dim / 85, the join 4 and 4 MB of sums a us.
+int attention_tc_parts(int64_t n, int heads, int dim, int64_t windows) {
+  if (n <= 0 || heads <= 0 || windows <= 0) return 1;
+  const int64_t tiles = n / windows / KB, blocks = (n / FORWARD_ROWS + 1) * heads;
+  const int64_t slots = (int64_t)num_sms() * (dim <= 64 ? 3 : 2);
+  const double tile_us = 1.0 + dim / 85.0, mb = 8e-6 * n * heads * dim;
+  int best = 1;
+  double least = 0;
+  for (int parts = 1; parts <= 16 && (parts == 1 || tiles / parts >= 4); ++parts) {
+    const int64_t rounds = (blocks * parts + slots - 1) / slots;
+    double us = tile_us * rounds * ((tiles + parts - 1) / parts + 2);
+    if (parts > 1) us += 4 + mb * parts / 4;
+    if (parts == 1 || us < least) {
+      least = us;
+      best = parts;
+    }
+  }
+  return mb * best > 1024 ? 1 : best;
+}
 
 int attention_tc_forward(const AttnArgs& a, bool bf16, cudaStream_t s) {
   return bf16 ? forward_typed<__nv_bfloat16>(a, s) : forward_typed<__half>(a, s);

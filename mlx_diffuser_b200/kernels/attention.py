@@ -36,18 +36,22 @@ def _strides(q, k, v):
                                 v.stride(1))
 
 
-def _forward(q, k, v, table, lut, plan, scale, train):
+def _forward(q, k, v, table, lut, plan, windows, scale, train):
     n, heads, dim = q.shape
     dev = q.device
     out = q.new_empty((n, heads, dim))
     stats = q.new_empty((heads, n, 2), dtype=torch.float32) if train else None
     # what rounding `out` left out: the backward pass takes dS from a difference with dout . out
     rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
+    lib = N.load()
+    code = N.DTYPE_CODE[q.dtype]
     with N.on_device(dev):
-        rc = N.load().sv_window_attention(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), n, heads, dim,
-            N.DTYPE_CODE[q.dtype], plan.data_ptr(), table.data_ptr(), table.shape[-1],
-            lut.data_ptr(), lut.numel() // 2, scale, out.data_ptr(), N.ptr(rest), N.ptr(stats),
+        nbytes = lib.sv_window_attention_workspace_bytes(n, heads, dim, code, windows)
+        ws = N.workspace(nbytes, dev) if nbytes else None
+        rc = lib.sv_window_attention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), n, heads, dim, code,
+            plan.data_ptr(), windows, table.data_ptr(), table.shape[-1], lut.data_ptr(),
+            lut.numel() // 2, scale, out.data_ptr(), N.ptr(rest), N.ptr(stats), N.ptr(ws), nbytes,
             N.stream(dev))
     N.check(rc, "sparse_self_attention")
     return out, rest, stats
@@ -55,8 +59,8 @@ def _forward(q, k, v, table, lut, plan, scale, train):
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, lut, plan, scale):
-        out, rest, stats = _forward(q, k, v, table, lut, plan, scale, True)
+    def forward(ctx, q, k, v, table, lut, plan, windows, scale):
+        out, rest, stats = _forward(q, k, v, table, lut, plan, windows, scale, True)
         ctx.scale = scale
         ctx.save_for_backward(q, k, v, table, lut, plan, out, rest, stats)
         return out
@@ -78,22 +82,22 @@ class _WindowAttention(torch.autograd.Function):
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), out.data_ptr(),
                 N.ptr(rest), dout.data_ptr(), stats.data_ptr(), n, heads, dim,
                 N.DTYPE_CODE[q.dtype], plan.data_ptr(), table.data_ptr(), table.shape[-1],
-                lut.data_ptr(), lut.numel() // 2, ctx.scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                N.ptr(dtable), ws.data_ptr(), nbytes, N.stream(dev))
+                lut.data_ptr(), lut.numel() // 2, ctx.scale, dq.data_ptr(), dk.data_ptr(),
+                dv.data_ptr(), N.ptr(dtable), ws.data_ptr(), nbytes, N.stream(dev))
         N.check(rc, "sparse_self_attention (backward)")
-        return dq, dk, dv, dtable, None, None, None
+        return dq, dk, dv, dtable, None, None, None, None
 
 
-def biased_window_attention(q, k, v, table, lut, plan, scale: float) -> torch.Tensor:
-    """Attention inside the plan's windows: ``q``, ``k``, ``v`` (N, heads, dim) of one type,
+def biased_window_attention(q, k, v, table, lut, plan, windows: int, scale: float) -> torch.Tensor:
+    """Attention inside the plan's ``windows`` windows: ``q``, ``k``, ``v`` (N, heads, dim) of one type,
     ``table`` (heads, B, B, B) of the same type, ``lut`` int32 (2 * reach + 1,)."""
 
     q, k, v = (t if t.stride(2) == 1 or t.shape[2] <= 1 else t.contiguous() for t in (q, k, v))
     table, lut = table.contiguous(), lut.contiguous()
     if torch.is_grad_enabled() and (
             q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
-        return _WindowAttention.apply(q, k, v, table, lut, plan, scale)
-    return _forward(q, k, v, table, lut, plan, scale, False)[0]
+        return _WindowAttention.apply(q, k, v, table, lut, plan, windows, scale)
+    return _forward(q, k, v, table, lut, plan, windows, scale, False)[0]
 
 
 __all__ = ["biased_window_attention", "window_plan"]

@@ -779,7 +779,7 @@ def _biased_self_attention(x, q, k, v, window_size, shift_window, table, lut) ->
         if groups.perm.numel() != q.shape[0]:
             raise ValueError("the cached attention windows belong to other coordinates")
         plan = groups.plan_rows(x.coords)
-    return biased_window_attention(q, k, v, table, lut, plan, dim**-0.5)
+    return biased_window_attention(q, k, v, table, lut, plan, groups.num_groups, dim**-0.5)
 
 
 def position_buckets(reach: int, side: int, *, exact: int | None = None, device=None):

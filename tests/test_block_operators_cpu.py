@@ -205,8 +205,8 @@ def test_c_entry_points_check_before_any_launch():
     six = (ctypes.c_int64 * 6)(*[64] * 6)
 
     def attend(n=4, heads=2, dim=16, dtype=2, buckets=3, reach=1, q=p):
-        return lib.sv_window_attention(q, p, p, six, n, heads, dim, dtype, p, p, buckets, p, reach,
-                                       0.25, p, None, None, None)
+        return lib.sv_window_attention(q, p, p, six, n, heads, dim, dtype, p, 1, p, buckets, p,
+                                       reach, 0.25, p, None, None, None, 0, None)
 
     assert attend(n=0, q=None) == N.SV_OK
     assert attend(dtype=3) == N.SV_ERR_BAD_DTYPE

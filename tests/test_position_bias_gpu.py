@@ -177,6 +177,73 @@ def test_large_window(dtype):
     _run(_voxels(1500, 16, 1, 5), 1, 64, dtype, None, (0, 0, 0), 15, 4, seed=5)
 
 
+def _parts_bytes(n, heads, dim, dtype, windows):
+    return N.load().sv_window_attention_workspace_bytes(n, heads, dim, N.DTYPE_CODE[dtype], windows)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [24, 64, 100, 128])
+def test_long_windows_in_parts(dim, dtype):
+    """Few rows of long windows: the walk over the keys is split and joined."""
+    coords = _voxels(1100, 16, 2, dim)
+    if dtype != torch.float32:
+        assert _parts_bytes(2200, 2, dim, dtype, 2) > 0
+    _run(coords, 2, dim, dtype, None, (0, 0, 0), 15, 3, seed=dim)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_parts_with_masks_and_not_finite_values(dtype):
+    """A head that sees nothing, one whose keys lie in one direction (so that some parts of a row hold
+    none), and a NaN and an infinity in one of two windows."""
+    coords = _voxels(1000, 16, 2, 3)
+    x = _tensor(coords)
+    lut = position_buckets(15, 2, device=DEV)
+    table = _rand((2, 5, 5, 5), dtype, 5)
+    table[0, 2:] = float("-inf")
+    table[1] = float("-inf")
+    q, k, v = (_rand((2000, 2, 64), dtype, 6 + i) for i in range(3))
+    assert _parts_bytes(2000, 2, 64, dtype, 2) > 0
+
+    def run():
+        return sparse_self_attention(x, q, k, v, window_size=None, position_bias=table,
+                                     position_buckets=lut)
+
+    val, off = _reference(x, q, k, v, table, lut, None, (0, 0, 0))
+    out = run()
+    _close(out, val["out"], off["out"], "out")
+    assert not out[:, 1].any()
+    table[1] = 0
+    val, off = _reference(x, q, k, v, table, lut, None, (0, 0, 0))
+    first = torch.nonzero(coords[:, 0] == 0).flatten()
+    rest = coords[:, 0] == 1
+    k[first[3], 1, 4] = float("inf")
+    v[first[9], 1, 7] = float("nan")
+    got = run()
+    _close(got[rest], val["out"][rest], off["out"][rest], "out")
+    assert torch.isnan(got[~rest, 1, 7]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_windows_of_every_length(dtype):
+    """Windows of 1 to 140 rows in a row, so that blocks hold several, one, and a part of one."""
+    sizes = [1, 2, 31, 32, 33, 1, 63, 64, 65, 5, 127, 128, 129, 1, 1, 1, 140, 30, 3]
+    rows = []
+    for i, n in enumerate(sizes):
+        at = np.arange(n)
+        rows.append(np.stack([np.zeros(n, int), 6 * i + at // 36, at // 6 % 6, at % 6], 1))
+    coords = torch.from_numpy(np.concatenate(rows).astype(np.int32)).to(DEV)
+    for seed in range(2):
+        order = torch.randperm(len(coords), generator=torch.Generator().manual_seed(seed)).to(DEV)
+        _run(coords[order].contiguous() if seed else coords, 2, 32, dtype, 6, (0, 0, 0), 5, 5,
+             seed=seed)
+    # scores around -68, far below the zero that a row of zeros would score
+    n = len(coords)
+    base = torch.ones((1, 2, 32), device=DEV)
+    q = (-12 * base + _rand((n, 2, 32), torch.float32, 8, 0.1)).to(dtype)
+    k = (base + _rand((n, 2, 32), torch.float32, 9, 0.1)).to(dtype)
+    _run(coords, 2, 32, dtype, 6, (0, 0, 0), 5, 5, qkv=[q, k, _rand((n, 2, 32), dtype, 10)])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reach,side", [(1, 1), (7, 7), (12, 12), (31, 5), (1023, 12)])
 def test_tables(reach, side, dtype):
