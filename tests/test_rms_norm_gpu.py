@@ -59,6 +59,24 @@ def test_forward(c, dtype):
             assert (err <= (_half(dtype) + ROW) * ry.abs() + torch.finfo(dtype).tiny).all()
 
 
+@pytest.mark.parametrize("n,c", [(5, 72), (5, 331), (9600, 512)])
+def test_eight_bit_output_of_the_smallest_numbers(n, c):
+    """Rows whose scale is a subnormal number, or would be zero. The scale is then off by half of the
+    smallest number, 2^-150, and the value it stands for by at most 448 times that, next to half a
+    step of e4m3 (2^-4 of the value, or 2^-10 scales below its normal range)."""
+    x, _, _ = _inputs(n, c, torch.bfloat16, 9, False)
+    for size in (1e-36, 1e-40, 3e-44):
+        w = torch.full((c,), size, device=DEV)
+        w[::3] = 0
+        q, scale = rms_norm(x, w, quantize=True)
+        _, _, _, y = _reference(x, None, w)
+        got, s = q.float().to(F64), scale.to(F64)[:, None]
+        assert torch.isfinite(got).all() and (scale > 0).all() and not got[:, ::3].any()
+        # y is a multiple of 2^-149 too
+        off = (2.0**-4 + ROW) * y.abs() + 2.0**-10 * s + 450 * 2.0**-149
+        assert ((got * s - y).abs() <= off).all()
+
+
 @pytest.mark.parametrize("c", [1, 7, 64, 72, 331, 1024, 2048, 8192])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_eight_bit_output(c, dtype):
