@@ -641,6 +641,10 @@ class WindowGroups:
         if (self.plan is None or self.plan[0] is not coords
                 or self.plan[1] != coords._version):
             rows = window_plan(coords.contiguous(), self.perm, self.offsets)
+            if torch.cuda.is_current_stream_capturing():
+                return rows  # written by the graph's replays alone: not for others
+            # like the grouping, whole for whatever stream uses it next
+            torch.cuda.current_stream(coords.device).synchronize()
             self.plan = (coords, coords._version, rows)
         return self.plan[2]
 

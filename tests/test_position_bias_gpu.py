@@ -438,6 +438,36 @@ def test_empty_tensor_and_partial_gradients():
             assert torch.equal(got, want[i])
 
 
+def test_plan_of_a_captured_call_is_not_for_others():
+    """Windows known, their plan not: the capture lays out its own, which holds nothing until a replay;
+    a call outside lays out another."""
+    coords = _voxels(500, 12, 1, 14)
+    x = _tensor(coords)
+    q, k, v = (_rand((500, 2, 32), torch.bfloat16, 90 + i) for i in range(3))
+    table, lut = _rand((2, 9, 9, 9), torch.bfloat16, 93), position_buckets(4, 4, device=DEV)
+
+    def run(t):
+        return sparse_self_attention(t, q, k, v, window_size=5, position_bias=table,
+                                     position_buckets=lut)
+
+    want = run(_tensor(coords))
+    attention_windows(x, 5, (0, 0, 0))
+    N.status_word(DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = run(x)
+    outside = run(x)
+    assert torch.equal(outside, want)
+    graph.replay()
+    assert torch.equal(inside, want)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        again = run(x)
+    side.synchronize()
+    assert torch.equal(again, want)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_streams_graph_and_cached_windows(dtype):
     coords = _voxels(500, 12, 1, 13)
