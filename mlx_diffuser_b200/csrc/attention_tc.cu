@@ -1,16 +1,29 @@
 // Windowed attention with a learned relative position bias in fp16 / bf16, on the tensor cores.
 //
-// The formulas are attention.cu's. A block takes 64 rows in window order (queries, or keys for dk and
-// dv) of one head, four warps of 16, and walks the positions that any of their windows covers in
-// tiles of 64: rows of several small windows share a tile, and a warp skips the tiles that none of
-// its own rows' windows reach. Scores stay in registers from the product to the softmax to the next
-// product (the accumulator's layout is the operand's), so the running maximum and sum are the only
-// state. The gathered rows arrive by cp.async, one tile ahead.
+// The formulas are attention.cu's. A block takes up to 128 rows (queries; 64 in the backward pass, keys
+// for dk and dv) of one head out of the plan's list, four warps of 32 or 16, and walks the positions
+// that any of their windows covers in tiles of 32: rows of several small windows share a tile, and a
+// warp skips the tiles that none of its own rows' windows reach. Scores stay in registers from the
+// product to the softmax to the next product (the accumulator's layout is the operand's), so the
+// running maximum and sum are the only state. The gathered rows arrive by cp.async, one or two tiles
+// ahead.
 //
 // Products are warp-level mma.sync: a window of a surface holds 100-300 rows, so a tile's two
-// products are a few hundred cycles, while each of its 4096 scores needs an exponential and a table
-// look-up of its own. The look-up, not the product, is what a faster matrix instruction would wait
-// for, and the register layout makes the bias and the softmax free of shared-memory round trips.
+// products are a few hundred cycles, while each of its scores needs an exponential and a table
+// look-up of its own. The register layout makes the bias and the softmax free of shared-memory round
+// trips. A form with the scores in TMEM (tcgen05, four row warps a block) was slower: 332 against
+// 279 us forward, 398 + 305 against 308 + 276 us backward, its warps waiting for each other between
+// tiles that short; it won only for windows of 4,096 rows (590 against 678 us, before that walk was
+// split).
+//
+// Latency bounds these kernels: with the 168 registers of a thread three blocks fit an SM, 2.8 warps a
+// scheduler that issue an instruction every 2.6 cycles (a quarter of the stalls at the tile's barrier,
+// a fifth fixed latencies). bf16, 64 channels:
+//   forward   40,662 x 12 heads, windows of 8^3 (95 M pairs): 239 us; 20,331 x 16 (63 M): 202 us with
+//             what training keeps, 41 MB of it the rests
+//   backward  20,331 x 16: delta 25 us, dk and dv 267 us, dq and the table's gradient 284 us
+//   forward   8,192 x 6 x 128 in two windows (201 M pairs), three parts: 495 us and 28 us to join
+// Two row parts a warp in the dk / dv pass halve its fragment loads but leave two blocks an SM: 328 us.
 //
 // The bucket of a pair: where the table is one entry per offset (the look-up is the identity) and
 // the windows are no wider than its reach, it is linear in the coordinates and costs a subtraction;
@@ -29,8 +42,10 @@
 namespace sv {
 namespace {
 
-constexpr int WAVES = 9;  // CTAs an SM over a call's course (three run at a time)
-constexpr int AT = 128;  // threads: four warps of 16 rows, or of 16 MR
+// CTAs an SM over a call's course (three run at a time). 5: 265 us forward and 308 + 289 us backward; 9:
+// 238 and 284 + 266; 16: 233 and 288 + 269, whose staging of the table counts in the backward pass.
+constexpr int WAVES = 9;
+constexpr int AT = 128;   // threads: four warps of 16 rows, or of 32
 constexpr int KB = 32;   // positions of a tile
 // Rows of a block in the forward pass: two 16-row parts a warp, whose products share the tile's
 // fragments (8,192 x 6 x 128 fp16: 678 us with one, 651 with two).

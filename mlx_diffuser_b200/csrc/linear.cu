@@ -34,7 +34,9 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162f
 // ---- few rows ----------------------------------------------------------------------------------
 
 // W warps per output column (1: eight columns a block, 8: one), lanes along k in accesses of V
-// elements. Every lane holds the partial sums of all rows; x comes out of L1.
+// elements. Every lane holds the partial sums of all rows; x comes out of L1, all rows' accesses in
+// flight together (rows past the last read it again: behind a branch each waited for the one
+// before, 8 x 2048 -> 2048 bf16 19 us).
 template <typename T, typename O, int ROWS, int V, int W>
 __global__ void __launch_bounds__(256)
     few_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
@@ -55,19 +57,19 @@ __global__ void __launch_bounds__(256)
         *reinterpret_cast<uint4*>(we) = __ldg(reinterpret_cast<const uint4*>(wr + c));
       else
         we[0] = wr[c];
+      alignas(16) T xe[ROWS][V];
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
-        if (r < m) {
-          T xe[V];
-          if constexpr (V * sizeof(T) == 16)
-            *reinterpret_cast<uint4*>(xe) =
-                __ldg(reinterpret_cast<const uint4*>(x + r * ldx + c));
-          else
-            xe[0] = x[r * ldx + c];
-#pragma unroll
-          for (int e = 0; e < V; ++e) acc[r] = fmaf(to_float(xe[e]), to_float(we[e]), acc[r]);
-        }
+        const T* from = x + min(r, m - 1) * ldx + c;
+        if constexpr (V * sizeof(T) == 16)
+          *reinterpret_cast<uint4*>(xe[r]) = __ldg(reinterpret_cast<const uint4*>(from));
+        else
+          xe[r][0] = *from;
       }
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[r] = fmaf(to_float(xe[r][e]), to_float(we[e]), acc[r]);
     }
   }
 #pragma unroll

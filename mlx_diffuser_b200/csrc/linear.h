@@ -20,8 +20,8 @@ struct Operand {
 
 // y = act(acc * row_scale[i] * col_scale[j] + bias[j]) + residual[i][j], every pointer optional;
 // `preact` receives the activation's argument in fp32: rounded to 16 bits it would put a third of a
-// step into every gradient, next to the step that rounding dz costs. With `partial` set the kernel stores its raw fp32
-// sums there ([splits][M][N]) and a second pass applies the rest.
+// step into every gradient, next to the step that rounding dz costs. With `partial` set the kernel
+// stores its raw fp32 sums there ([splits][M][N]) and a second pass applies the rest.
 struct Epilogue {
   const void* bias;      // [N], out_dtype
   const void* residual;  // out_dtype, rows ld_res apart
