@@ -9,17 +9,12 @@
 // L maps an offset along an axis, clamped to the table's reach, to a bucket. The windows come as a
 // plan: rows in window order with each window's range of positions (sv_window_plan).
 //
-// fp32 runs on the kernels here, a warp per row and head (attention.h), with exact fp32 products and
-// sums; fp16 and bf16 on attention_tc.cu.
-//
-// The table's gradient sums in 64-bit fixed point, so that neither the order of the atomics nor
-// the number of blocks changes it.
+// fp32 runs on attention_f32.cu, fp16 and bf16 on attention_tc.cu; the plan and the entry points are
+// here.
 #include "attention.h"
 
 namespace sv {
 namespace {
-
-constexpr int ROW_WARPS = 8;
 
 // Every row's window extent: a block per window.
 __global__ void __launch_bounds__(128)
@@ -129,94 +124,6 @@ __global__ void __launch_bounds__(128)
     const int p = start + i * size;
     blocks[first + i] = make_int2(p, min(size, stop - p));
   }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_kernel(AttnArgs a) {
-  __shared__ float scratch[ROW_WARPS][ATTN_MAX_DIM];
-  const int64_t p = (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
-  if (p < a.n) row_forward<T, false>(a, p, blockIdx.y, scratch[threadIdx.x >> 5]);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * ROW_WARPS) attn_dq_rows_kernel(AttnArgs a) {
-  __shared__ float scratch[ROW_WARPS][2 * ATTN_MAX_DIM];
-  const int64_t p = (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
-  if (p < a.n) row_dq<T, false, true>(a, p, blockIdx.y, scratch[threadIdx.x >> 5]);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * ROW_WARPS) attn_dkv_rows_kernel(AttnArgs a) {
-  __shared__ float scratch[ROW_WARPS][2 * ATTN_MAX_DIM];
-  const int64_t p = (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
-  if (p < a.n) row_dkv<T, false>(a, p, blockIdx.y, scratch[threadIdx.x >> 5]);
-}
-
-// norms[h] = bits of the largest |dout_i|^2 and |v_j|^2 of a head. Squares are not negative, so
-// their bits order like the values, and a NaN stays above everything.
-template <typename T>
-__global__ void __launch_bounds__(256) attn_norms_kernel(AttnArgs a, unsigned* norms) {
-  __shared__ unsigned s_top[2];
-  const int h = blockIdx.y;
-  if (threadIdx.x < 2) s_top[threadIdx.x] = 0u;
-  __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + warp; r < a.n; r += (int64_t)gridDim.x * 8) {
-    const T* g = static_cast<const T*>(a.dout) + (r * a.heads + h) * a.dim;
-    const T* v = static_cast<const T*>(a.v) + r * a.v_row + h * a.v_head;
-    float g2 = 0.f, v2 = 0.f;
-    for (int d = lane; d < a.dim; d += 32) {
-      const float x = to_f32(g[d]), y = to_f32(v[d]);
-      g2 = fmaf(x, x, g2);
-      v2 = fmaf(y, y, v2);
-    }
-    g2 = warp_sum(g2);
-    v2 = warp_sum(v2);
-    if (lane == 0) {
-      atomicMax(&s_top[0], __float_as_uint(g2) & 0x7fffffffu);
-      atomicMax(&s_top[1], __float_as_uint(v2) & 0x7fffffffu);
-    }
-  }
-  __syncthreads();
-  if (threadIdx.x < 2) atomicMax(norms + 2 * h + threadIdx.x, s_top[threadIdx.x]);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256)
-    dtable_finish_kernel(AttnArgs a, T* __restrict__ out) {
-  const int64_t cells = (int64_t)a.nb * a.nb * a.nb;
-  const int h = blockIdx.y;
-  const int exponent = dtable_exponent(a, h);
-  for (int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x; b < cells;
-       b += (int64_t)gridDim.x * 256) {
-    const double v = exponent == INT_MAX
-                         ? __longlong_as_double(0x7ff8000000000000ll)  // the inputs were not finite
-                         : ldexp((double)(long long)a.dtable[h * cells + b], -exponent);
-    out[h * cells + b] = from_f32<T>((float)v);
-  }
-}
-
-dim3 row_grid(const AttnArgs& a) {
-  return dim3((unsigned)((a.n + ROW_WARPS - 1) / ROW_WARPS), (unsigned)a.heads);
-}
-
-int backward_rows(const AttnArgs& a, void* dtable, cudaStream_t s) {
-  if (dtable) {
-    const unsigned blocks = (unsigned)((a.n + 63) / 64 < 512 ? (a.n + 63) / 64 : 512);
-    attn_norms_kernel<float><<<dim3(blocks, a.heads), 256, 0, s>>>(a, a.norms);
-    SV_LAUNCH_CHECK();
-  }
-  attn_dq_rows_kernel<float><<<row_grid(a), 32 * ROW_WARPS, 0, s>>>(a);
-  SV_LAUNCH_CHECK();
-  attn_dkv_rows_kernel<float><<<row_grid(a), 32 * ROW_WARPS, 0, s>>>(a);
-  SV_LAUNCH_CHECK();
-  if (dtable) {
-    const unsigned blocks = (unsigned)((a.nb * a.nb * a.nb + 255) / 256);
-    dtable_finish_kernel<float><<<dim3(blocks, a.heads), 256, 0, s>>>(a,
-                                                                      static_cast<float*>(dtable));
-    SV_LAUNCH_CHECK();
-  }
-  return SV_OK;
 }
 
 bool float_type(int d) { return d == SV_FLOAT32 || d == SV_FLOAT16 || d == SV_BFLOAT16; }
@@ -340,9 +247,7 @@ extern "C" int sv_window_attention(const void* q, const void* k, const void* v,
     a.part_stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + l.stats);
   }
   if (dtype != SV_FLOAT32) return attention_tc_forward(a, dtype == SV_BFLOAT16, s);
-  attn_rows_kernel<float><<<row_grid(a), 32 * ROW_WARPS, 0, s>>>(a);
-  SV_LAUNCH_CHECK();
-  return SV_OK;
+  return attention_f32_forward(a, s);
 }
 
 extern "C" size_t sv_window_attention_backward_workspace_bytes(int64_t n, int heads, int buckets) {
@@ -352,9 +257,10 @@ extern "C" size_t sv_window_attention_backward_workspace_bytes(int64_t n, int he
 
 extern "C" int sv_window_attention_backward(
     const void* q, const void* k, const void* v, const int64_t* strides, const void* o,
-    const void* o_rest, const void* dout, const float* stats, int64_t n, int heads, int dim, int dtype, const void* plan,
-    const void* table, int buckets, const int32_t* lut, int reach, float scale, void* dq, void* dk,
-    void* dv, void* dtable, void* workspace, size_t workspace_bytes, sv_stream_t stream) {
+    const void* o_rest, const void* dout, const float* stats, int64_t n, int heads, int dim,
+    int dtype, const void* plan, const void* table, int buckets, const int32_t* lut, int reach,
+    float scale, void* dq, void* dk, void* dv, void* dtable, void* workspace,
+    size_t workspace_bytes, sv_stream_t stream) {
   const int rc = check(n, heads, dim, dtype, buckets, reach, "sv_window_attention_backward");
   if (rc != SV_OK) return rc;
   cudaStream_t s = to_stream(stream);
@@ -389,6 +295,6 @@ extern "C" int sv_window_attention_backward(
     a.dtable = reinterpret_cast<unsigned long long*>(ws + l.table);
     SV_CUDA_TRY(cudaMemsetAsync(ws, 0, l.delta, s));  // the table and the norms
   }
-  if (dtype == SV_FLOAT32) return backward_rows(a, dtable, s);
+  if (dtype == SV_FLOAT32) return attention_f32_backward(a, dtable, s);
   return attention_tc_backward(a, dtype == SV_BFLOAT16, dtable, s);
 }

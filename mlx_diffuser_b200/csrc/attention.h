@@ -16,6 +16,9 @@ constexpr int ATTN_MAX_HEADS = 65535;
 struct AttnArgs;
 int attention_tc_forward(const AttnArgs& a, bool bf16, cudaStream_t s);
 int attention_tc_parts(int64_t n, int heads, int dim, int64_t windows);
+// attention_f32.cu: the fp32 ones.
+int attention_f32_forward(const AttnArgs& a, cudaStream_t s);
+int attention_f32_backward(const AttnArgs& a, void* dtable, cudaStream_t s);
 int attention_tc_backward(const AttnArgs& a, bool bf16, void* dtable, cudaStream_t s);
 
 // One row of the attention plan, in window order: the coordinates, the window's range of

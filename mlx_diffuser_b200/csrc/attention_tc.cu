@@ -603,7 +603,8 @@ __device__ __forceinline__ BlockList block_list(const AttnArgs& a) {
   const PlanBlocks b = plan_blocks(a.n);
   const uint8_t* plan = reinterpret_cast<const uint8_t*>(a.plan);
   const int count = __ldg(reinterpret_cast<const int*>(plan + b.count) + which);
-  return {reinterpret_cast<const int2*>(plan + b.block[which]), (int)min((int64_t)count, b.cap[which])};
+  return {reinterpret_cast<const int2*>(plan + b.block[which]),
+          (int)min((int64_t)count, b.cap[which])};
 }
 
 template <typename T, int BQ>
