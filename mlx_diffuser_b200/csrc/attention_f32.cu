@@ -7,8 +7,9 @@
 // the tile and eight of the rows for 32 fused multiply-adds); the weights then go through shared
 // memory, and for the sums the lanes lie along the channels. So a row of the other side leaves HBM or
 // L2 once per 64 rows and shared memory once per eight. Shared-memory reads bound it, at about one per
-// three multiply-adds. A warp per row straight from global memory, one position a lane, was bound by
-// L1 instead (32 lines an access).
+// three multiply-adds. 10,000 rows x 8 heads x 64, windows of 8^3: forward 204 us, dq and the table 293,
+// dk and dv 275; a warp per row straight from global memory, one position a lane, was bound by L1 (32
+// lines an access) and took 1,137, 1,311 and 1,461 us.
 //
 // The table's gradient sums in 64-bit fixed point, so that neither the order of the atomics nor
 // the number of blocks changes it.

@@ -137,16 +137,71 @@ int gemm_few(const Gemm& g, cudaStream_t s) {
 
 constexpr int FK = 16;  // k per shared-memory stage
 
+// One operand's T rows x FK steps of a stage, by 256 threads in accesses of V elements: from global
+// memory into registers, and from there into shared memory, steps outermost.
+template <int T, int V>
+struct Stage {
+  static constexpr int PER = T * FK / 256;  // elements a thread
+  // The e-th access's row r and step l, along one of which its elements lie.
+  static __device__ __forceinline__ void place(bool mn, int e, int* r, int* l) {
+    const int at = threadIdx.x + 256 * e;
+    *r = mn ? at % (T / V) * V : at / (FK / V);
+    *l = mn ? at / (T / V) : at % (FK / V) * V;
+  }
+  static __device__ __forceinline__ void fetch(const Operand& o, int64_t r0, int64_t rows,
+                                               int64_t l0, int64_t l1, float (&v)[PER]) {
+    const float* p = static_cast<const float*>(o.p);
+#pragma unroll
+    for (int e = 0; e < PER / V; ++e) {
+      int r, l;
+      place(o.mn, e, &r, &l);
+      const int64_t i = r0 + r, ll = l0 + l;
+      const float* from = p + (o.mn ? ll * o.ld + i : i * o.ld + ll);
+      const int64_t left = i < rows && ll < l1 ? (o.mn ? rows - i : l1 - ll) : 0;
+      if (V == 4 && left >= 4) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(from));
+        v[V * e] = x.x;
+        v[V * e + 1 % V] = x.y;
+        v[V * e + 2 % V] = x.z;
+        v[V * e + 3 % V] = x.w;
+      } else {
+#pragma unroll
+        for (int x = 0; x < V; ++x) v[V * e + x] = x < left ? __ldg(from + x) : 0.f;
+      }
+    }
+  }
+  static __device__ __forceinline__ void put(bool mn, float (*s)[T + 4], const float (&v)[PER]) {
+#pragma unroll
+    for (int e = 0; e < PER / V; ++e) {
+      int r, l;
+      place(mn, e, &r, &l);
+      if (V == 4 && mn) {
+        *reinterpret_cast<float4*>(&s[l][r]) =
+            make_float4(v[V * e], v[V * e + 1 % V], v[V * e + 2 % V], v[V * e + 3 % V]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < V; ++x) {
+          if (mn) s[l][r + x] = v[V * e + x];
+          else s[l + x][r] = v[V * e + x];
+        }
+      }
+    }
+  }
+};
+
 // C tile of 16 R x 16 R, 256 threads with R x R sums each (R / 4 groups of four rows and columns,
-// 64 apart, so that the shared-memory reads are 16-byte and conflict-free).
-template <int R>
-__global__ void __launch_bounds__(256)
+// 64 apart, so that the shared-memory reads are 16-byte and conflict-free). VA, VB: elements of an
+// access to each operand. 12,001 x 1024 x 1024: 729 us (34.5 TFLOP/s, two blocks an SM in 2.5 rounds);
+// element by element with one block an SM it took 1,078 us.
+template <int R, int VA, int VB>
+__global__ void __launch_bounds__(256, 2)
     gemm_f32_kernel(Operand a, Operand b, int64_t m, int64_t n, int64_t k, int64_t k_part,
                     Epilogue ep) {
   constexpr int T = 16 * R;
-  constexpr int PER = T * FK / 256;  // elements of each operand a thread stages
-  __shared__ float sa[2][FK][T + 4];
-  __shared__ float sb[2][FK][T + 4];
+  using SA = Stage<T, VA>;
+  using SB = Stage<T, VB>;
+  __shared__ __align__(16) float sa[2][FK][T + 4];
+  __shared__ __align__(16) float sb[2][FK][T + 4];
   const int tid = threadIdx.x;
   const int tx = tid % 16, ty = tid / 16;
   // columns vary fastest: blocks that run together share the rows of A
@@ -154,41 +209,23 @@ __global__ void __launch_bounds__(256)
   const int64_t i0 = (int64_t)(blockIdx.x / across) * T, j0 = (int64_t)(blockIdx.x % across) * T;
   const int64_t k0 = (int64_t)blockIdx.y * k_part;
   const int64_t k1 = k0 + k_part < k ? k0 + k_part : k;
-  float ra[PER], rb[PER];
-  auto fetch = [&](const Operand& o, int64_t r0, int64_t rows, int64_t l0, float (&v)[PER]) {
-    const float* p = static_cast<const float*>(o.p);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int at = tid + 256 * e;
-      const int r = o.mn ? at % T : at / FK, l = o.mn ? at / T : at % FK;
-      const int64_t i = r0 + r, ll = l0 + l;
-      v[e] = i < rows && ll < k1 ? __ldg(p + (o.mn ? ll * o.ld + i : i * o.ld + ll)) : 0.f;
-    }
-  };
-  auto put = [&](const Operand& o, float (&s)[FK][T + 4], const float (&v)[PER]) {
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int at = tid + 256 * e;
-      const int r = o.mn ? at % T : at / FK, l = o.mn ? at / T : at % FK;
-      s[l][r] = v[e];
-    }
-  };
+  float ra[SA::PER], rb[SB::PER];
   float acc[R][R];
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int j = 0; j < R; ++j) acc[i][j] = 0.f;
-  fetch(a, i0, m, k0, ra);
-  fetch(b, j0, n, k0, rb);
-  put(a, sa[0], ra);
-  put(b, sb[0], rb);
+  SA::fetch(a, i0, m, k0, k1, ra);
+  SB::fetch(b, j0, n, k0, k1, rb);
+  SA::put(a.mn, sa[0], ra);
+  SB::put(b.mn, sb[0], rb);
   __syncthreads();
   int buf = 0;
   for (int64_t l0 = k0; l0 < k1; l0 += FK, buf ^= 1) {
     const bool more = l0 + FK < k1;
     if (more) {
-      fetch(a, i0, m, l0 + FK, ra);
-      fetch(b, j0, n, l0 + FK, rb);
+      SA::fetch(a, i0, m, l0 + FK, k1, ra);
+      SB::fetch(b, j0, n, l0 + FK, k1, rb);
     }
 #pragma unroll
     for (int l = 0; l < FK; ++l) {
@@ -206,8 +243,8 @@ __global__ void __launch_bounds__(256)
         for (int j = 0; j < R; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
     }
     if (more) {
-      put(a, sa[buf ^ 1], ra);
-      put(b, sb[buf ^ 1], rb);
+      SA::put(a.mn, sa[buf ^ 1], ra);
+      SB::put(b.mn, sb[buf ^ 1], rb);
       __syncthreads();
     }
   }
@@ -227,6 +264,14 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+template <int R>
+void launch_f32(const Gemm& g, dim3 grid, int64_t k_part, cudaStream_t s) {
+  const bool va = aligned16(g.a.p) && g.a.ld % 4 == 0, vb = aligned16(g.b.p) && g.b.ld % 4 == 0;
+  auto kernel = va ? (vb ? gemm_f32_kernel<R, 4, 4> : gemm_f32_kernel<R, 4, 1>)
+                   : (vb ? gemm_f32_kernel<R, 1, 4> : gemm_f32_kernel<R, 1, 1>);
+  kernel<<<grid, 256, 0, s>>>(g.a, g.b, g.m, g.n, g.k, k_part, g.ep);
+}
+
 int gemm_f32(const Gemm& g, bool small, cudaStream_t s) {
   const int tile = small ? 64 : 128;
   const int64_t k_part = (((g.k + g.splits - 1) / g.splits + FK - 1) / FK) * FK;
@@ -234,9 +279,9 @@ int gemm_f32(const Gemm& g, bool small, cudaStream_t s) {
   if (tiles > INT32_MAX) SV_FAIL(SV_ERR_UNSUPPORTED, "linear: too many tiles");
   const dim3 grid((unsigned)tiles, (unsigned)g.splits);
   if (small)
-    gemm_f32_kernel<4><<<grid, 256, 0, s>>>(g.a, g.b, g.m, g.n, g.k, k_part, g.ep);
+    launch_f32<4>(g, grid, k_part, s);
   else
-    gemm_f32_kernel<8><<<grid, 256, 0, s>>>(g.a, g.b, g.m, g.n, g.k, k_part, g.ep);
+    launch_f32<8>(g, grid, k_part, s);
   SV_LAUNCH_CHECK();
   return SV_OK;
 }
@@ -536,12 +581,14 @@ Plan plan_gemm(int64_t m, int64_t n, int64_t k, int dtype, bool a_mn, bool b_mn)
   const int64_t sms = num_sms();
   if (dtype == SV_FLOAT32) {
     p.path = Path::kF32;
+    // Tiles of 128 x 128 where they and the parts of a split k axis, each at least 4 steps of 64 long,
+    // give every SM one; of 64 x 64 otherwise. 12,001 x 1024 x 1024: dW in parts takes 812 us, in
+    // small tiles 855 us.
+    const int64_t steps = (k + 4 * FK - 1) / (4 * FK), most = std::max<int64_t>(1, steps / 4);
     int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128);
-    p.small = tiles < sms;
+    p.small = tiles * most < sms;
     if (p.small) tiles = ((m + 63) / 64) * ((n + 63) / 64);
-    const int64_t steps = (k + 4 * FK - 1) / (4 * FK);
-    // split the k axis while tiles are fewer than SMs, each part at least 4 steps long
-    if (tiles < sms && steps >= 8) set_splits(&p, std::min(sms / tiles, steps / 4), steps, m, n);
+    if (tiles < sms) set_splits(&p, std::min((2 * sms + tiles - 1) / tiles, most), steps, m, n);
     return p;
   }
   p.path = Path::kTensor;
