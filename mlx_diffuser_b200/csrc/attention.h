@@ -151,6 +151,10 @@ __device__ __forceinline__ PlanRow plan_at(const PlanRow* plan, int64_t p) {
   return r;
 }
 
+// A row that sees one position has a weight of one whatever its score, so its score gradient is zero;
+// dP - delta, which the passes round differently, would leave a trace of rounding errors.
+__device__ __forceinline__ bool lone(const PlanRow& r) { return r.end - r.start == 1; }
+
 constexpr int ATTN_CH = ATTN_MAX_DIM / 32;  // channels a lane sums
 
 // What rounding `x` to T left out, itself rounded: nothing for fp32, nor next to an overflow.
@@ -263,11 +267,12 @@ __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
   const int exponent = TABLE && a.dtable ? dtable_exponent(a, h) : INT_MAX;
   const double unit = exponent == INT_MAX ? 0.0 : ldexp(1.0, exponent);
   float acc[ATTN_CH] = {};
-  for (int j0 = me.start; j0 < me.end; j0 += 32) {
+  const int end = lone(me) ? me.start : me.end;
+  for (int j0 = me.start; j0 < end; j0 += 32) {
     const int j = j0 + lane;
     float ds = 0.f;
     int row = -1;
-    if (j < me.end) {
+    if (j < end) {
       const PlanRow key = plan_at(a.plan, j);
       row = key.row;
       if (row >= 0) {
@@ -284,7 +289,7 @@ __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
         }
       }
     }
-    const int count = min(32, me.end - j0);
+    const int count = min(32, end - j0);
     for (int i = 0; i < count; ++i) {
       const float w = __shfl_sync(0xffffffffu, ds, i);
       const int r = __shfl_sync(0xffffffffu, row, i);
@@ -335,7 +340,7 @@ __device__ void row_dkv(const AttnArgs& a, int64_t p, int h, float* scratch) {
         const float s = score_of<LOG2>(dot_row(s_k, q + row * a.q_row, a.dim) +
                                        to_f32(table[bucket_of(a, query, me)]));
         w = weight_of<LOG2>(s - stats.x) * stats.y;
-        ds = w * (dot_row(s_v, g + row * g_row, a.dim) - a.delta[h * a.n + i]);
+        if (!lone(me)) ds = w * (dot_row(s_v, g + row * g_row, a.dim) - a.delta[h * a.n + i]);
       }
     }
     const int count = min(32, me.end - i0);

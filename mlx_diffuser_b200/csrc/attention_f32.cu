@@ -263,9 +263,11 @@ __global__ void __launch_bounds__(F_THREADS) attn_f32_kernel(AttnArgs a, bool ve
           second[r] += e;
           w0[r * FT + lane] = e;
         } else if constexpr (PASS == DQ) {
-          const float ds = in ? expf(x - stats[r].x) * stats[r].y * (dp[r] - first[r]) : 0.f;
+          const bool counts = in && !lone(me);
+          const float ds =
+              counts ? expf(x - stats[r].x) * stats[r].y * (dp[r] - first[r]) : 0.f;
           w0[r * FT + lane] = ds;
-          if (in && a.dtable) {
+          if (counts && a.dtable) {
             if (!(fabsf(ds) < INFINITY))
               atomicMax(a.norms + 2 * h, 0x7fffffffu);  // the head's table gradient is NaN
             else if (exponent != INT_MAX)
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(F_THREADS) attn_f32_kernel(AttnArgs a, bool ve
           const float2 st = sh.stats[buf][lane];
           const float e = in ? expf(x - st.x) * st.y : 0.f;
           w0[r * FT + lane] = e;
-          w1[r * FT + lane] = in ? e * (dp[r] - sh.delta[buf][lane]) : 0.f;
+          w1[r * FT + lane] = in && !lone(me) ? e * (dp[r] - sh.delta[buf][lane]) : 0.f;
         }
       }
       __syncwarp();

@@ -278,7 +278,8 @@ struct Block {
   // `part` of `parts` is walked. STAND_IN: rows behind the last see what the first one does, so that
   // they cost no mask; nothing of theirs is stored. Without it they see nothing, as the backward
   // pass needs them to, which takes sums and maxima over all of a warp's pairs.
-  template <bool STAND_IN>
+  // LONE: rows that see one position see nothing (dq).
+  template <bool STAND_IN, bool LONE = false>
   __device__ void begin(int p0, int count, int part = 0, int parts = 1) {
     if (threadIdx.x < 2) s.range[threadIdx.x] = threadIdx.x ? INT_MIN : INT_MAX;
     __syncthreads();
@@ -286,8 +287,9 @@ struct Block {
     if (threadIdx.x < BQ) {
       const bool in = (int)threadIdx.x < count;
       PlanRow r = plan_at(a.plan, in ? p0 + threadIdx.x : p0);
-      if (r.row < 0) {
+      if (r.row < 0 || (LONE && lone(r))) {
         r.start = r.end = 0;
+        if (!in) r.row = -1;
       } else {
         narrow = r.span <= a.reach;
         if (in) {
@@ -486,7 +488,7 @@ template <int ROWS>
 __device__ __forceinline__ Reach warp_reach(const PlanRow* own) {
   const int lane = threadIdx.x & 31;
   const PlanRow& r = own[lane % ROWS];
-  const bool any = r.row >= 0;
+  const bool any = r.row >= 0 && r.end > r.start;
   Reach w;
   w.lo = __reduce_min_sync(0xffffffffu, any ? r.start : INT_MAX);
   w.hi = __reduce_max_sync(0xffffffffu, any ? r.end : INT_MIN);
@@ -979,7 +981,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   };
   for (int block = blockIdx.x; block < list.count; block += gridDim.x) {
     const int2 at = __ldg(list.at + block);
-    b.template begin<false>(at.x, at.y);
+    b.template begin<false, true>(at.x, at.y);
     load_tile<T, DP, BQ>(smem, q, (int)a.q_row, sh.own_row, a.dim, vec);
     load_tile<T, DP, BQ>(smem + L::OWN_TILE, dout, g_row, sh.own_row, a.dim, vec);
     const PlanRow* own = sh.own + warp * 16 + g;
@@ -1142,8 +1144,8 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
           load_tile<T, DP, KB>(tile + L::TILE, dout, g_row, rows, a.dim, vec);
         },
         body, [] { return false; }, [] {});
-    store_rows<T, DP>(mine, dk[0], a.scale, a.scale, sh.own_row + warp * 16, static_cast<T*>(a.dk),
-                      a.heads, head, a.dim, vec);
+    store_rows<T, DP>(mine, dk[0], lone(own[0]) ? 0.f : a.scale, lone(own[8]) ? 0.f : a.scale,
+                      sh.own_row + warp * 16, static_cast<T*>(a.dk), a.heads, head, a.dim, vec);
     store_rows<T, DP>(mine + L::OWN_TILE, dv[0], 1.f, 1.f, sh.own_row + warp * 16,
                       static_cast<T*>(a.dv), a.heads, head, a.dim, vec);
     again(not_finite<DP>(dk[0]) | not_finite<DP>(dv[0]), warp * 16, mine, [&](int i, float* f) {

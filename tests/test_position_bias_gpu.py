@@ -177,6 +177,24 @@ def test_large_window(dtype):
     _run(_voxels(1500, 16, 1, 5), 1, 64, dtype, None, (0, 0, 0), 15, 4, seed=5)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,dim", [(1, 8), (2, 64), (300, 24), (300, 128)])
+def test_lone_rows(n, dim, dtype):
+    """Windows of one row: the output is v, dv is dout, and the score, which changes nothing, has a
+    gradient of exactly zero."""
+    coords = torch.zeros((n, 4), dtype=torch.int32, device=DEV)
+    coords[:, 1] = 4 * torch.arange(n, device=DEV)
+    x = _tensor(coords)
+    leaves = [_rand((n, 2, dim), dtype, i).requires_grad_(True) for i in range(3)]
+    leaves.append(_rand((2, 7, 7, 7), dtype, 3).requires_grad_(True))
+    dout = _rand((n, 2, dim), dtype, 4)
+    out = sparse_self_attention(x, *leaves[:3], window_size=4, position_bias=leaves[3],
+                                position_buckets=position_buckets(3, 3, device=DEV))
+    dq, dk, dv, dtable = torch.autograd.grad(out, leaves, dout)
+    assert torch.equal(out, leaves[2]) and torch.equal(dv, dout)
+    assert not dq.any() and not dk.any() and not dtable.any()
+
+
 def _parts_bytes(n, heads, dim, dtype, windows):
     return N.load().sv_window_attention_workspace_bytes(n, heads, dim, N.DTYPE_CODE[dtype], windows)
 
