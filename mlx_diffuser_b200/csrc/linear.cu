@@ -137,6 +137,15 @@ int gemm_few(const Gemm& g, cudaStream_t s) {
 
 constexpr int FK = 16;  // k per shared-memory stage
 
+// Two fp32 multiply-adds in one instruction, each rounded like fmaf's.
+__device__ __forceinline__ void fma_pair(uint64_t& c, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ uint64_t twice(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return (uint64_t)u << 32 | u;
+}
+
 // One operand's T rows x FK steps of a stage, by 256 threads in accesses of V elements: from global
 // memory into registers, and from there into shared memory, steps outermost.
 template <int T, int V>
@@ -191,8 +200,9 @@ struct Stage {
 
 // C tile of 16 R x 16 R, 256 threads with R x R sums each (R / 4 groups of four rows and columns,
 // 64 apart, so that the shared-memory reads are 16-byte and conflict-free). VA, VB: elements of an
-// access to each operand. 12,001 x 1024 x 1024: 729 us (34.5 TFLOP/s, two blocks an SM in 2.5 rounds);
-// element by element with one block an SM it took 1,078 us.
+// access to each operand. 12,001 x 1024 x 1024, the three products of a training step: 668 us on
+// average (37.7 TFLOP/s; two blocks an SM, 2.5 rounds of tiles), 755 us with one multiply-add an
+// instruction, and 1,127 us element by element with one block an SM. The library's fp32 product: 455.
 template <int R, int VA, int VB>
 __global__ void __launch_bounds__(256, 2)
     gemm_f32_kernel(Operand a, Operand b, int64_t m, int64_t n, int64_t k, int64_t k_part,
@@ -210,11 +220,11 @@ __global__ void __launch_bounds__(256, 2)
   const int64_t k0 = (int64_t)blockIdx.y * k_part;
   const int64_t k1 = k0 + k_part < k ? k0 + k_part : k;
   float ra[SA::PER], rb[SB::PER];
-  float acc[R][R];
+  uint64_t acc[R][R / 2];  // two neighbouring columns each
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < R; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < R / 2; ++j) acc[i][j] = 0;
   SA::fetch(a, i0, m, k0, k1, ra);
   SB::fetch(b, j0, n, k0, k1, rb);
   SA::put(a.mn, sa[0], ra);
@@ -229,18 +239,23 @@ __global__ void __launch_bounds__(256, 2)
     }
 #pragma unroll
     for (int l = 0; l < FK; ++l) {
-      float av[R], bv[R];
+      uint64_t av[R], bv[R / 2];
 #pragma unroll
       for (int q = 0; q < R / 4; ++q) {
-        *reinterpret_cast<float4*>(av + 4 * q) =
-            *reinterpret_cast<const float4*>(&sa[buf][l][64 * q + 4 * ty]);
-        *reinterpret_cast<float4*>(bv + 4 * q) =
-            *reinterpret_cast<const float4*>(&sb[buf][l][64 * q + 4 * tx]);
+        const float4 x = *reinterpret_cast<const float4*>(&sa[buf][l][64 * q + 4 * ty]);
+        av[4 * q] = twice(x.x);
+        av[4 * q + 1] = twice(x.y);
+        av[4 * q + 2] = twice(x.z);
+        av[4 * q + 3] = twice(x.w);
+        const ulonglong2 y =
+            *reinterpret_cast<const ulonglong2*>(&sb[buf][l][64 * q + 4 * tx]);
+        bv[2 * q] = y.x;
+        bv[2 * q + 1] = y.y;
       }
 #pragma unroll
       for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < R; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+        for (int j = 0; j < R / 2; ++j) fma_pair(acc[i][j], av[i], bv[j]);
     }
     if (more) {
       SA::put(a.mn, sa[buf ^ 1], ra);
@@ -256,10 +271,11 @@ __global__ void __launch_bounds__(256, 2)
     for (int j = 0; j < R; ++j) {
       const int64_t col = j0 + 64 * (j / 4) + 4 * tx + j % 4;
       if (col >= n) continue;
+      const float v = __uint_as_float((uint32_t)(acc[i][j / 2] >> (j % 2 * 32)));
       if (ep.partial)
-        ep.partial[((int64_t)blockIdx.y * m + row) * n + col] = acc[i][j];
+        ep.partial[((int64_t)blockIdx.y * m + row) * n + col] = v;
       else
-        epilogue_store<float>(ep, row, col, n, acc[i][j]);
+        epilogue_store<float>(ep, row, col, n, v);
     }
   }
 }
@@ -582,8 +598,8 @@ Plan plan_gemm(int64_t m, int64_t n, int64_t k, int dtype, bool a_mn, bool b_mn)
   if (dtype == SV_FLOAT32) {
     p.path = Path::kF32;
     // Tiles of 128 x 128 where they and the parts of a split k axis, each at least 4 steps of 64 long,
-    // give every SM one; of 64 x 64 otherwise. 12,001 x 1024 x 1024: dW in parts takes 812 us, in
-    // small tiles 855 us.
+    // give every SM one; of 64 x 64 otherwise. 12,001 x 1024 x 1024, before the paired
+    // multiply-adds: dW in parts took 812 us, in small tiles 855 us.
     const int64_t steps = (k + 4 * FK - 1) / (4 * FK), most = std::max<int64_t>(1, steps / 4);
     int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128);
     p.small = tiles * most < sms;
