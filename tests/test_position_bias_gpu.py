@@ -605,3 +605,57 @@ def test_transformer_block(dtype):
         rel = float((a.to(F64) - b).norm() / b.norm())
         assert rel <= tol, (name, rel, tol)
     N.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("window", [5, None])
+def test_training_step_in_a_graph_and_on_two_streams(window):
+    """Forward and backward of norm, projection and attention captured together (their workspaces come
+    from the graph's pool), replayed on other inputs, and two eager steps at once on two streams."""
+    coords = _voxels(1200, 12, 1, 15)
+    x = _tensor(coords)
+    lut = position_buckets(4, 2, device=DEV)
+    dtype = torch.bfloat16
+
+    def inputs(seed):
+        shapes = [(1200, 64), (64,), (192, 64), (192,), (2, 5, 5, 5)]
+        return [_rand(s, dtype, seed + i, 0.3) for i, s in enumerate(shapes)]
+
+    dout = _rand((1200, 2, 32), dtype, 99)
+
+    def step(args):
+        f, w, p, b, table = args
+        h = rms_norm(f, w)
+        q, k, v = linear(h, p, b, activation="silu").view(1200, 3, 2, 32).unbind(1)
+        out = sparse_self_attention(x, q, k, v, window_size=window, position_bias=table,
+                                    position_buckets=lut)
+        return [out.detach(), *torch.autograd.grad(out, args, dout)]
+
+    def eager(seed):
+        return step([t.requires_grad_(True) for t in inputs(seed)])
+
+    want = {seed: eager(seed) for seed in (100, 200)}
+    static = [t.requires_grad_(True) for t in inputs(100)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(static)
+    for seed in (200, 100):
+        with torch.no_grad():
+            for t, new in zip(static, inputs(seed)):
+                t.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[seed]))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for s, seed in zip(streams, (100, 200)):
+        with torch.cuda.stream(s):
+            results.append(eager(seed))
+    torch.cuda.synchronize()
+    for seed, res in zip((100, 200), results):
+        assert all(torch.equal(a, b) for a, b in zip(res, want[seed]))
+    N.check_device_status(DEV)
