@@ -19,8 +19,8 @@
 // Latency bounds these kernels: with the 168 registers of a thread three blocks fit an SM, 2.8 warps a
 // scheduler that issue an instruction every 2.6 cycles (a quarter of the stalls at the tile's barrier,
 // a fifth fixed latencies). bf16, 64 channels:
-//   forward   40,662 x 12 heads, windows of 8^3 (95 M pairs): 239 us; 20,331 x 16 (63 M): 202 us with
-//             what training keeps, 41 MB of it the rests
+//   forward   40,662 x 12 heads, windows of 8^3 (95 M pairs): 239 us; 20,331 x 16 (63 M): 225 us with
+//             what training adds, 41 MB of rests and a second product
 //   backward  20,331 x 16: delta 25 us, dk and dv 267 us, dq and the table's gradient 284 us
 //   forward   8,192 x 6 x 128 in two windows (201 M pairs), three parts: 495 us and 28 us to join
 // Two row parts a warp in the dk / dv pass halve its fragment loads but leave two blocks an SM: 328 us.
@@ -31,7 +31,9 @@
 //
 // Weights and score gradients are rounded to the feature type as operands of the second products
 // (half a step each, like the stored results); the softmax sums and the table's gradient use them
-// unrounded.
+// unrounded. The forward pass of training adds a second product for what rounding the weights leaves
+// out: delta, which dS is a small difference with, comes from its output (dq and dk off by 1.42 times
+// the plain form's error instead of up to 1.55, for 22 us of 225 at 20,331 x 16 x 64).
 #include <limits.h>
 
 #include <algorithm>
@@ -91,6 +93,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   } else {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// What pack2 left out of two numbers, rounded in turn.
+template <typename T>
+__device__ __forceinline__ uint32_t rest2(uint32_t packed, float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return pack2<T>(lo - __uint_as_float(packed << 16), hi - __uint_as_float(packed & 0xffff0000u));
+  } else {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&packed));
+    return pack2<T>(lo - v.x, hi - v.y);
   }
 }
 
@@ -443,8 +456,9 @@ __device__ __forceinline__ void mma_nt(float (&acc)[MR][KB / 8][4], uint32_t row
   }
 }
 
-// out += w (16 MR x KB sums, rounded to T as operand fragments) x tile (KB x DP).
-template <typename T, int DP, int MR>
+// out += w (16 MR x KB sums, rounded to T as operand fragments) x tile (KB x DP). SPLIT: with a second
+// product for what the rounding leaves out.
+template <typename T, int DP, int MR, bool SPLIT = false>
 __device__ __forceinline__ void mma_nn(float (&out)[MR][DP / 8][4],
                                        const float (&w)[MR][KB / 8][4], uint32_t tile) {
   const int lane = threadIdx.x & 31;
@@ -459,6 +473,15 @@ __device__ __forceinline__ void mma_nn(float (&out)[MR][DP / 8][4],
       f[m][2] = pack2<T>(w[m][2 * k + 1][0], w[m][2 * k + 1][1]);
       f[m][3] = pack2<T>(w[m][2 * k + 1][2], w[m][2 * k + 1][3]);
     }
+    uint32_t low[MR][4];
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          low[m][i] = rest2<T>(f[m][i], w[m][2 * k + i / 2][i % 2 * 2],
+                               w[m][2 * k + i / 2][i % 2 * 2 + 1]);
+    }
 #pragma unroll
     for (int n = 0; n < DP / 16; ++n) {
       uint32_t b[4];
@@ -467,6 +490,10 @@ __device__ __forceinline__ void mma_nn(float (&out)[MR][DP / 8][4],
       for (int m = 0; m < MR; ++m) {
         mma<T>(out[m][2 * n], f[m], b[0], b[1]);
         mma<T>(out[m][2 * n + 1], f[m], b[2], b[3]);
+        if constexpr (SPLIT) {
+          mma<T>(out[m][2 * n], low[m], b[0], b[1]);
+          mma<T>(out[m][2 * n + 1], low[m], b[2], b[3]);
+        }
       }
     }
   }
@@ -763,7 +790,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
             s[m][n][e] = exp2_fast(s[m][n][e] - base[m][e >> 1]);
             sum[m][e >> 1] += s[m][n][e];
           }
-      mma_nn<T, DP, MR>(o, s, tile + L::TILE);
+      mma_nn<T, DP, MR, TRAIN>(o, s, tile + L::TILE);
     };
     walk<false, STAGES>(
         b,
