@@ -164,8 +164,8 @@ __device__ __forceinline__ float rest_of(float x) {
   return fabsf(r) < INFINITY ? r : 0.f;
 }
 
-// ---- one row of one head, by a warp: lanes along the other side's rows for the scores, along the
-// ---- head's channels for the sums, fp32 throughout
+// ---- one row of one head computed again, by a warp: lanes along the other side's rows for the
+// ---- scores, along the head's channels for the sums, fp32 throughout
 
 // Scores as the kernel keeps them: natural (fp32 path), or times log2(e) for the fp16 / bf16 kernels,
 // whose statistics the rows computed again share.
@@ -238,8 +238,8 @@ __device__ void row_forward(const AttnArgs& a, int64_t p, int h, float* s_q) {
   __syncwarp();
 }
 
-// dq of a query, and with TABLE delta and the table's gradient too. `scratch`: 2 * ATTN_MAX_DIM.
-template <typename T, bool LOG2, bool TABLE>
+// dq of a query. `scratch`: 2 * ATTN_MAX_DIM.
+template <typename T, bool LOG2>
 __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
   const int lane = threadIdx.x & 31;
   const PlanRow me = plan_at(a.plan, p);
@@ -252,8 +252,7 @@ __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
   const T* g = static_cast<const T*>(a.dout) + own;
   const T* o = static_cast<const T*>(a.o) + own;
   const T* o_rest = a.o_rest ? static_cast<const T*>(a.o_rest) + own : nullptr;
-  const int64_t cells = (int64_t)a.nb * a.nb * a.nb;
-  const T* table = static_cast<const T*>(a.table) + h * cells;
+  const T* table = static_cast<const T*>(a.table) + (int64_t)h * a.nb * a.nb * a.nb;
   float delta = 0.f;
   for (int d = lane; d < a.dim; d += 32) {
     s_q[d] = to_f32(q[d]) * a.scale;
@@ -261,11 +260,8 @@ __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
     delta = fmaf(s_g[d], to_f32(o[d]) + (o_rest ? to_f32(o_rest[d]) : 0.f), delta);
   }
   delta = warp_sum(delta);
-  if (TABLE && lane == 0) a.delta[h * a.n + p] = delta;
   __syncwarp();
   const float2 stats = a.stats[h * a.n + p];
-  const int exponent = TABLE && a.dtable ? dtable_exponent(a, h) : INT_MAX;
-  const double unit = exponent == INT_MAX ? 0.0 : ldexp(1.0, exponent);
   float acc[ATTN_CH] = {};
   const int end = lone(me) ? me.start : me.end;
   for (int j0 = me.start; j0 < end; j0 += 32) {
@@ -276,17 +272,10 @@ __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
       const PlanRow key = plan_at(a.plan, j);
       row = key.row;
       if (row >= 0) {
-        const int b = bucket_of(a, me, key);
-        const float s = score_of<LOG2>(dot_row(s_q, k + row * a.k_row, a.dim) + to_f32(table[b]));
+        const float s = score_of<LOG2>(dot_row(s_q, k + row * a.k_row, a.dim) +
+                                       to_f32(table[bucket_of(a, me, key)]));
         const float dp = dot_row(s_g, v + row * a.v_row, a.dim);
         ds = weight_of<LOG2>(s - stats.x) * stats.y * (dp - delta);
-        if constexpr (TABLE) {
-          if (a.dtable && !(fabsf(ds) < INFINITY))
-            atomicMax(a.norms + 2 * h, 0x7fffffffu);  // the head's table gradient is NaN
-          else if (exponent != INT_MAX)
-            atomicAdd(a.dtable + h * cells + b,
-                      (unsigned long long)__double2ll_rn((double)ds * unit));
-        }
       }
     }
     const int count = min(32, end - j0);

@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(F_THREADS) attn_f32_kernel(AttnArgs a, bool ve
       // are the scratch.
       if (!__all_sync(0xffffffffu, finite)) {
         if constexpr (PASS == FORWARD) row_forward<float, false>(a, p, h, w0);
-        if constexpr (PASS == DQ) row_dq<float, false, false>(a, p, h, w0);
+        if constexpr (PASS == DQ) row_dq<float, false>(a, p, h, w0);
         if constexpr (PASS == DKV) row_dkv<float, false>(a, p, h, w0);
       }
     }

@@ -585,7 +585,7 @@ __device__ __noinline__ void again_forward(AttnArgs a, int64_t p, int h, float* 
 }
 template <typename T>
 __device__ __noinline__ void again_dq(AttnArgs a, int64_t p, int h, float* s) {
-  row_dq<T, true, false>(a, p, h, s);
+  row_dq<T, true>(a, p, h, s);
 }
 template <typename T>
 __device__ __noinline__ void again_dkv(AttnArgs a, int64_t p, int h, float* s) {

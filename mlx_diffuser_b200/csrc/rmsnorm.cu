@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, 2)
         sq = row_reduce<Sum, 32>(sq, nullptr);
         const float rstd = 1.0f / sqrtf(sq / (float)C + a.eps);
         if (lane == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
-        float top = 0.f;
+        [[maybe_unused]] float top = 0.f;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const int c = (lane + 32 * j) * V;
