@@ -659,3 +659,10 @@ def test_training_step_in_a_graph_and_on_two_streams(window):
     for seed, res in zip((100, 200), results):
         assert all(torch.equal(a, b) for a, b in zip(res, want[seed]))
     N.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reach", [12, 31, 1023])
+def test_largest_table_with_the_widest_heads(reach, dtype):
+    """25 buckets an axis and 128 channels: the most shared memory that any call takes."""
+    _run(_voxels(220, 10, 1, reach), 2, 128, dtype, 8, (4, 4, 4), reach, 12, seed=reach)
