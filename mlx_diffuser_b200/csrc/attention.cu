@@ -164,15 +164,16 @@ PartLayout part_layout(int64_t n, int heads, int dim, int dtype, int64_t windows
   return l;
 }
 
-// Workspace of the backward pass: fixed-point table, norms, delta.
+// Workspace of the backward pass: fixed-point table, norms, the buckets' largest terms, delta.
 struct Layout {
-  size_t table, norms, delta, total;
+  size_t table, norms, tops, delta, total;
 };
 Layout layout(int64_t n, int heads, int nb) {
   Layout l;
   l.table = 0;
   l.norms = l.table + align_up((size_t)heads * nb * nb * nb * 8, 256);
-  l.delta = l.norms + align_up((size_t)heads * 8, 256);
+  l.tops = l.norms + align_up((size_t)heads * 8, 256);
+  l.delta = l.tops + align_up((size_t)heads * nb * nb * nb * 4, 256);
   l.total = l.delta + align_up((size_t)heads * n * 4, 256);
   return l;
 }
@@ -291,9 +292,10 @@ extern "C" int sv_window_attention_backward(
   a.delta = reinterpret_cast<float*>(ws + l.delta);
   a.n = n; a.heads = heads; a.dim = dim; a.nb = buckets; a.reach = reach; a.scale = scale;
   a.norms = reinterpret_cast<unsigned*>(ws + l.norms);
+  a.tops = reinterpret_cast<unsigned*>(ws + l.tops);
   if (dtable) {
     a.dtable = reinterpret_cast<unsigned long long*>(ws + l.table);
-    SV_CUDA_TRY(cudaMemsetAsync(ws, 0, l.delta, s));  // the table and the norms
+    SV_CUDA_TRY(cudaMemsetAsync(ws, 0, l.delta, s));  // the table, the norms and the buckets' largest terms
   }
   if (dtype == SV_FLOAT32) return attention_f32_backward(a, dtable, s);
   return attention_tc_backward(a, dtype == SV_BFLOAT16, dtable, s);

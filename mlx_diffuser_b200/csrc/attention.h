@@ -63,8 +63,8 @@ struct AttnArgs {
   float2* stats;                     // [heads, n] by position: the softmax's maximum and 1 / sum
   float* delta;                      // [heads, n] by position: sum_d dout * o
   unsigned long long* dtable;        // [heads, nb^3] fixed point, or null
-  unsigned* norms;                   // [heads, 2]: bits of max |dout_i|^2 and max |v_j|^2 (fp32
-                                     // path), or of max |dS| (fp16 / bf16)
+  unsigned* norms;                   // [heads, 2]: bits of max |dout_i|^2 and max |v_j|^2 (fp32)
+  unsigned* tops;                    // [heads, nb^3]: bits of each bucket's max |dS| (fp16 / bf16)
   float2* part_stats;                // parts > 1: [parts, heads, n] by position, base and sum
   float* part_out;                   // and [parts, heads, n, dim], not yet divided by the sum
   int64_t n;

@@ -21,7 +21,8 @@
 // a fifth fixed latencies). bf16, 64 channels:
 //   forward   40,662 x 12 heads, windows of 8^3 (95 M pairs): 239 us; 20,331 x 16 (63 M): 225 us with
 //             what training adds, 41 MB of rests and a second product
-//   backward  20,331 x 16: delta 25 us, dk and dv 267 us, dq and the table's gradient 284 us
+//   backward  20,331 x 16: delta 26 us, dk and dv with each bucket's largest term 371 us (296 where no
+//             table gradient is wanted), dq and the table's gradient 328 us
 //   forward   8,192 x 6 x 128 in two windows (201 M pairs), three parts: 495 us and 28 us to join
 // Two row parts a warp in the dk / dv pass halve its fragment loads but leave two blocks an SM: 328 us.
 //
@@ -240,6 +241,11 @@ __device__ __forceinline__ float lds_f32(uint32_t at) {
   asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
   return v;
 }
+__device__ __forceinline__ uint32_t lds_u8(uint32_t at) {
+  uint32_t v;
+  asm("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at));
+  return v;
+}
 __device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
   uint16_t v;
   asm("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
@@ -255,7 +261,6 @@ struct Block {
   uint16_t* joint;   // [(2 reach + 1)^2]: x and y buckets' offset in the table, or null
   int head;
   bool identity;
-  float delta_top;   // largest |delta| staged by this thread
   // set per BQ rows
   int mode;
   int j0, tiles;
@@ -346,7 +351,6 @@ struct Block {
       }
       s.key_stats[slot][i] = st;
       s.key_delta[slot][i] = d;
-      delta_top = max_nan(delta_top, fabsf(d));
     }
     const unsigned bad = __ballot_sync(0xffffffffu, j < s.range[1] && m.row < 0);
     if (i == 0) s.key_bad[slot] = bad != 0;
@@ -604,13 +608,15 @@ struct Layout {
 };
 
 struct Tables {
-  int grad, lut, joint, total;  // byte offsets behind Layout::TABLE; joint < 0: none
+  int words, units, lut, joint, total;  // byte offsets behind Layout::TABLE; joint < 0: none
 };
-__host__ __device__ inline Tables tables(const AttnArgs& a, bool grad) {
+// `words`: one 32-bit word a bucket beside the bias; `units`: and one byte.
+__host__ __device__ inline Tables tables(const AttnArgs& a, bool words, bool units) {
   const int cells = a.nb * a.nb * a.nb, width = 2 * a.reach + 1;
   Tables t;
-  t.grad = cells * 4;
-  t.lut = t.grad + (grad ? cells * 4 : 0);
+  t.words = cells * 4;
+  t.units = t.words + (words ? cells * 4 : 0);
+  t.lut = (t.units + (units ? cells : 0) + 15) / 16 * 16;
   t.joint = -1;
   t.total = t.lut + (width * 2 + 15) / 16 * 16;
   if (width * width <= JOINT_MAX) {
@@ -638,13 +644,13 @@ __device__ __forceinline__ BlockList block_list(const AttnArgs& a) {
 
 template <typename T, int BQ>
 __device__ __forceinline__ Block<T, BQ> make_block(const AttnArgs& a, uint8_t* smem, int shared,
-                                                   int table, bool grad) {
-  const Tables t = tables(a, grad);
+                                                   int table, bool words, bool units) {
+  const Tables t = tables(a, words, units);
   return Block<T, BQ>{a, *reinterpret_cast<Shared<BQ>*>(smem + shared),
                       reinterpret_cast<float*>(smem + table),
                       reinterpret_cast<uint16_t*>(smem + table + t.lut),
                       t.joint < 0 ? nullptr : reinterpret_cast<uint16_t*>(smem + table + t.joint),
-                      (int)blockIdx.y, false, 0.f};
+                      (int)blockIdx.y, false};
 }
 
 // The tiles of one block: load(buffer, rows) fetches a tile's rows, STAGES - 1 tiles ahead (the
@@ -694,7 +700,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   extern __shared__ __align__(16) uint8_t smem[];
   const BlockList list = block_list<BQ>(a);
   if ((int)blockIdx.x >= list.count) return;
-  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, false);
+  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, false, false);
   Shared<BQ>& sh = b.s;
   const int head = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -946,16 +952,20 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a, bool vec) {
   if (sub == 0 && live) a.delta[h * a.n + p] = d;
 }
 
-// The table's gradient in fixed point: a score gradient is at most 2^18 units (the head's largest is
-// known from the dk / dv pass), and sums to a 32-bit word per bucket in shared memory. A thread
-// counts the units it has added; the block empties its words into the 64-bit sums in global memory
-// before any thread's count can pass 2^24, so 128 threads cannot overflow a word. INT_MAX when a
-// score gradient was not finite.
+// The table's gradient in fixed point, with a unit for each bucket: a score gradient is at most 2^18 of
+// its bucket's units (the bucket's largest is known from the dk / dv pass), so every pair keeps 2^-18 of
+// its own bucket's largest however far another bucket's or row's lie above it. (One unit for a head
+// left exact zeros in 62% of the buckets of a table that falls by 1.5 a voxel.) The pairs sum to a
+// 32-bit word per bucket in shared memory. A thread counts the units it has added; the block empties its
+// words into the 64-bit sums in global memory before any thread's count can pass 2^24, so 128 threads
+// cannot overflow a word.
 constexpr int UNIT_BITS = 18;
-__device__ __forceinline__ int unit_exponent(const AttnArgs& a, int head) {
-  const float top = __uint_as_float(a.norms[2 * head]);
+constexpr float UNIT_TOP = (float)(1 << UNIT_BITS);
+// Exponent of a bucket's reciprocal unit; INT_MAX when a score gradient of the bucket was not finite.
+__device__ __forceinline__ int unit_exponent(unsigned bits) {
+  const float top = __uint_as_float(bits);
   if (!(top < INFINITY)) return INT_MAX;
-  if (top == 0.f) return 0;
+  if (top == 0.f) return 120;
   int e;
   frexpf(top, &e);                      // top < 2^e
   return min(UNIT_BITS - 1 - e, 120);   // the two passes round their products differently
@@ -970,11 +980,13 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   extern __shared__ __align__(16) uint8_t smem[];
   const BlockList list = block_list<BQ>(a);
   if ((int)blockIdx.x >= list.count) return;
-  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, TABLE);
+  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, TABLE, TABLE);
   Shared<BQ>& sh = b.s;
   const int cells = b.cells();
-  int* s_grad = reinterpret_cast<int*>(smem + L::TABLE + tables(a, TABLE).grad);
-  const uint32_t table = smem_u32(b.table), grads = smem_u32(s_grad);
+  const Tables extra = tables(a, TABLE, TABLE);
+  int* s_grad = reinterpret_cast<int*>(smem + L::TABLE + extra.words);
+  uint8_t* s_unit = smem + L::TABLE + extra.units;  // the units' reciprocals: their exponent fields
+  const uint32_t table = smem_u32(b.table), grads = smem_u32(s_grad), units = smem_u32(s_unit);
   const int head = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2;
@@ -985,13 +997,17 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   const T* dout = static_cast<const T*>(a.dout) + (int64_t)head * a.dim;
   const int g_row = a.heads * a.dim;
   const float scale = a.scale * ATTN_LOG2E;
-  const int exponent = TABLE ? unit_exponent(a, head) : INT_MAX;
-  const float unit = exponent == INT_MAX ? 0.f : ldexpf(1.f, exponent);
-  // a thread adds KB / 2 pairs a tile
-  constexpr float LIMIT = 16777216.f - (KB / 2) * (float)(1 << UNIT_BITS);
-  float spent = 0.f;  // sum of |dS| since the words were emptied
+  // a thread adds KB / 2 pairs a tile; half a unit each for rounding to an integer and as much for
+  // rounding the count itself
+  constexpr float LIMIT = 16777216.f - 2 * KB - (KB / 2) * UNIT_TOP;
+  float spent = 0.f;  // units added since the words were emptied
   if constexpr (TABLE) {
-    for (int i = threadIdx.x; i < cells; i += AT) s_grad[i] = 0;
+    const unsigned* tops = a.tops + (int64_t)head * cells;
+    for (int i = threadIdx.x; i < cells; i += AT) {
+      const int e = unit_exponent(__ldg(tops + i));
+      s_grad[i] = 0;
+      s_unit[i] = (uint8_t)(e == INT_MAX ? 0 : 127 + e);  // 0: nothing of the bucket counts
+    }
   }
   b.stage_tables();
   auto flush = [&] {
@@ -1039,6 +1055,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
         for (int e = 0; e < 4; ++e) dp[0][n][e] = -delta[e >> 1];
       mma_nt<T, DP, 1>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
       const bool bad = sh.key_bad[slot];
+      if constexpr (TABLE) spent += KB / 2;
       auto grad = [&](int n, int e, uint32_t at, bool in) {
         const int r = e >> 1;
         const float x = fmaf(s[0][n][e], scale, lds_f32(table + at));
@@ -1046,12 +1063,14 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
         s[0][n][e] = in ? ds : 0.f;
         if constexpr (TABLE) {
           if (in) {
-            spent += fabsf(ds);
+            // The two passes round dp - delta differently: where that is all a bucket's terms are, this
+            // one may find a larger term. A NaN counts as a number, and its bucket ends as NaN.
+            const float unit = __uint_as_float(lds_u8(units + (at >> 2)) << 23);
+            const float u = fminf(fmaxf(ds * unit, -UNIT_TOP), UNIT_TOP);
+            spent += fabsf(u);
             // 1.5 * 2^23: the sum's low bits are the rounded integer
-            const float f = fmaf(ds, unit, 12582912.f);
             asm volatile("red.shared.add.s32 [%0], %1;" ::"r"(grads + at),
-                         "r"(__float_as_int(f) - 0x4b400000)
-                         : "memory");
+                         "r"(__float_as_int(u + 12582912.f) - 0x4b400000));
           }
         }
       };
@@ -1073,7 +1092,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
           load_tile<T, DP, KB>(tile, k, (int)a.k_row, rows, a.dim, vec);
           load_tile<T, DP, KB>(tile + L::TILE, v, (int)a.v_row, rows, a.dim, vec);
         },
-        body, [&] { return TABLE && spent * unit > LIMIT; }, flush);
+        body, [&] { return TABLE && spent > LIMIT; }, flush);
     store_rows<T, DP>(mine, dq[0], a.scale, a.scale, sh.own_row + warp * 16, static_cast<T*>(a.dq),
                       a.heads, head, a.dim, vec);
     again(not_finite<DP>(dq[0]), warp * 16, mine, [&](int i, float* f) {
@@ -1084,7 +1103,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   flush();
 }
 
-// dk and dv, and the largest |dS| of the head: the block's rows are keys, the tiles queries.
+// dk and dv, and the largest |dS| of every bucket: the block's rows are keys, the tiles queries.
 template <typename T, int DP, int STAGES, bool TABLE>
 __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
     attn_dkv_tc_kernel(AttnArgs a, bool vec) {
@@ -1093,9 +1112,11 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   extern __shared__ __align__(16) uint8_t smem[];
   const BlockList list = block_list<BQ>(a);
   if ((int)blockIdx.x >= list.count) return;
-  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, false);
+  Block<T, BQ> b = make_block<T, BQ>(a, smem, L::SHARED, L::TABLE, TABLE, false);
   Shared<BQ>& sh = b.s;
-  const uint32_t table = smem_u32(b.table);
+  const int cells = b.cells();
+  unsigned* s_top = reinterpret_cast<unsigned*>(smem + L::TABLE + tables(a, TABLE, false).words);
+  const uint32_t table = smem_u32(b.table), tops = smem_u32(s_top);
   const int head = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c2 = 2 * (lane & 3);
@@ -1106,7 +1127,9 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   const T* dout = static_cast<const T*>(a.dout) + (int64_t)head * a.dim;
   const int g_row = a.heads * a.dim;
   const float scale = a.scale * ATTN_LOG2E;
-  float most = 0.f;
+  if constexpr (TABLE) {
+    for (int i = threadIdx.x; i < cells; i += AT) s_top[i] = 0u;
+  }
   b.stage_tables();
   for (int block = blockIdx.x; block < list.count; block += gridDim.x) {
     const int2 at = __ldg(list.at + block);
@@ -1115,6 +1138,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
     load_tile<T, DP, BQ>(smem + L::OWN_TILE, v, (int)a.v_row, sh.own_row, a.dim, vec);
     const PlanRow* own = sh.own + warp * 16 + g;
     const Reach w = warp_reach<16>(sh.own + warp * 16);
+    const bool solo[2] = {lone(own[0]), lone(own[8])};
     float dk[1][DP / 8][4], dv[1][DP / 8][4];
     zero(dk[0]);
     zero(dv[0]);
@@ -1123,27 +1147,11 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
       if (p0 >= w.hi || p0 + KB <= w.lo) return;
       const uint32_t tile = smem_u32(smem + L::RING + buf * 2 * L::TILE);
       const int slot = t % SLOTS;
+      const bool bad = sh.key_bad[slot];
+      const bool whole = p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad;
       float s[1][KB / 8][4], dp[1][KB / 8][4];
       zero(s[0]);
       mma_nt<T, DP, 1>(s, smem_u32(mine), tile);
-      const bool bad = sh.key_bad[slot];
-      const bool whole = p0 >= w.all_lo && p0 + KB <= w.all_hi && !bad;
-      auto weight = [&](int n, int e, uint32_t at) {
-        const float2 st = sh.key_stats[slot][n * 8 + c2 + (e & 1)];
-        s[0][n][e] = exp2_fast(fmaf(s[0][n][e], scale, lds_f32(table + at)) - st.x) * st.y;
-      };
-      if (whole) {
-        each_pair<true, true>(b, slot, own, weight);
-      } else {
-        each_pair<true, false>(b, slot, own, weight);
-        const Sight seen = sight(own, p0);
-#pragma unroll
-        for (int n = 0; n < KB / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (hidden(seen, n, e, bad, sh, slot)) s[0][n][e] = 0.f;
-      }
-      mma_nn<T, DP, 1>(dv, s, tile + L::TILE);
 #pragma unroll
       for (int n = 0; n < KB / 8; ++n) {
         const float2 delta = *reinterpret_cast<const float2*>(&sh.key_delta[slot][n * 8 + c2]);
@@ -1151,16 +1159,27 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
         dp[0][n][1] = dp[0][n][3] = -delta.y;
       }
       mma_nt<T, DP, 1>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
-#pragma unroll
-      for (int n = 0; n < KB / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float ds = s[0][n][e] * dp[0][n][e];
-          // a weight of zero may stand for a row of another window, which may hold anything
-          if (!whole && s[0][n][e] == 0.f) ds = 0.f;
-          dp[0][n][e] = ds;
-          if constexpr (TABLE) most = max_nan(most, fabsf(ds));
-        }
+      // a pair out of sight may be with a row that holds anything
+      auto grad = [&](int n, int e, uint32_t at, bool in, bool counts) {
+        const float2 st = sh.key_stats[slot][n * 8 + c2 + (e & 1)];
+        const float w = exp2_fast(fmaf(s[0][n][e], scale, lds_f32(table + at)) - st.x) * st.y;
+        s[0][n][e] = in ? w : 0.f;
+        dp[0][n][e] = in ? w * dp[0][n][e] : 0.f;
+        // bits of numbers that are not negative order like the numbers, a NaN's above all
+        if constexpr (TABLE)
+          asm volatile("red.shared.max.u32 [%0], %1;" ::"r"(tops + at),
+                       "r"(counts ? __float_as_uint(dp[0][n][e]) & 0x7fffffffu : 0u));
+      };
+      if (whole) {
+        each_pair<true, true>(b, slot, own,
+                              [&](int n, int e, uint32_t at) { grad(n, e, at, true, true); });
+      } else {
+        const Sight seen = sight(own, p0);
+        each_pair<true, false>(b, slot, own, [&](int n, int e, uint32_t at) {
+          grad(n, e, at, !hidden(seen, n, e, bad, sh, slot), !solo[e >> 1]);
+        });
+      }
+      mma_nn<T, DP, 1>(dv, s, tile + L::TILE);
       mma_nn<T, DP, 1>(dk, dp, tile);
     };
     walk<true, STAGES>(
@@ -1180,13 +1199,10 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
     });
     __syncthreads();
   }
-  if constexpr (TABLE) {
-    // The two passes round dp - delta differently, by up to 2^-17 |delta| or so; a head whose score
-    // gradients are nothing but that must not get a unit so small that the other pass overflows it.
-    most = max_nan(most, b.delta_top * 0x1p-14f);
-    // bits of non-negative numbers order like the numbers, a NaN's above all
-    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
-    if (lane == 0 && top) atomicMax(a.norms + 2 * head, top);
+  if constexpr (TABLE) {  // behind the last block's barrier
+    unsigned* to = a.tops + (int64_t)head * cells;
+    for (int i = threadIdx.x; i < cells; i += AT)
+      if (s_top[i] != 0u) atomicMax(to + i, s_top[i]);
   }
 }
 
@@ -1194,9 +1210,9 @@ template <typename T>
 __global__ void __launch_bounds__(256) dtable_tc_finish_kernel(AttnArgs a, T* __restrict__ out) {
   const int cells = a.nb * a.nb * a.nb;
   const int h = blockIdx.y;
-  const int exponent = unit_exponent(a, h);
   for (int b = blockIdx.x * 256 + threadIdx.x; b < cells; b += gridDim.x * 256) {
     const int64_t at = (int64_t)h * cells + b;
+    const int exponent = unit_exponent(a.tops[at]);
     const double v = exponent == INT_MAX
                          ? __longlong_as_double(0x7ff8000000000000ll)  // something was not finite
                          : ldexp((double)(long long)a.dtable[at], -exponent);
@@ -1235,7 +1251,7 @@ int allow_smem(K kernel, size_t bytes) {
 template <typename T, int DP, bool TRAIN>
 int forward(const AttnArgs& a, cudaStream_t s) {
   constexpr int MR = FORWARD_ROWS / 64, STAGES = DP <= 64 ? 3 : 2;
-  const size_t bytes = Layout<DP, 64 * MR, 1, STAGES>::TABLE + tables(a, false).total;
+  const size_t bytes = Layout<DP, 64 * MR, 1, STAGES>::TABLE + tables(a, false, false).total;
   const int rc = allow_smem(attn_tc_kernel<T, DP, MR, STAGES, TRAIN>, bytes);
   if (rc != SV_OK) return rc;
   attn_tc_kernel<T, DP, MR, STAGES, TRAIN>
@@ -1258,12 +1274,12 @@ int backward(const AttnArgs& a, void* dtable, cudaStream_t s) {
       <<<dim3((unsigned)((a.n + 7) / 8), (unsigned)((a.heads + 3) / 4)), 256, 0, s>>>(a, vec);
   SV_LAUNCH_CHECK();
   const dim3 grid(ctas_of(a, 64, WAVES), a.heads);
-  size_t bytes = L::TABLE + tables(a, false).total;
+  size_t bytes = L::TABLE + tables(a, TABLE, false).total;
   int rc = allow_smem(attn_dkv_tc_kernel<T, DP, STAGES, TABLE>, bytes);
   if (rc != SV_OK) return rc;
   attn_dkv_tc_kernel<T, DP, STAGES, TABLE><<<grid, AT, bytes, s>>>(a, vec);
   SV_LAUNCH_CHECK();
-  bytes = L::TABLE + tables(a, TABLE).total;
+  bytes = L::TABLE + tables(a, TABLE, TABLE).total;
   rc = allow_smem(attn_dq_tc_kernel<T, DP, STAGES, TABLE>, bytes);
   if (rc != SV_OK) return rc;
   attn_dq_tc_kernel<T, DP, STAGES, TABLE><<<grid, AT, bytes, s>>>(a, vec);
