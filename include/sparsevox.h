@@ -443,8 +443,9 @@ SV_API int sv_window_plan(const int32_t* coords, const int32_t* perm, const int3
  * [2 reach + 1], values in [0, buckets) (others are clamped); table: [heads, buckets^3] in `dtype`,
  * buckets <= 25. `strides`: row and head strides of q, k, v in elements, channels contiguous.
  * out: contiguous. For the backward pass, or null: stats, fp32 [heads, n, 2] by position, 8-byte
- * aligned: the softmax's maximum and 1 / sum; out_rest, like out: what its rounding to fp16 / bf16
- * left out (not written for fp32). A row whose every score is -inf gives zeros. `windows`: how many the
+ * aligned: a row's base (its largest score, or near it) and 1 / sum of its weights over that base;
+ * out_rest, like out: what its rounding to bf16 left out, or 2^11 times that for fp16 (not written for
+ * fp32). A row whose every score is -inf gives zeros. `windows`: how many the
  * plan has; from their mean length it is decided whether the walk over a window's rows is split, with
  * the parts' sums in the workspace (0 bytes: not split). */
 SV_API size_t sv_window_attention_workspace_bytes(int64_t n, int heads, int dim, int dtype,

@@ -3,6 +3,8 @@
 
 #include <limits.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace sv {
@@ -157,11 +159,20 @@ __device__ __forceinline__ bool lone(const PlanRow& r) { return r.end - r.start 
 
 constexpr int ATTN_CH = ATTN_MAX_DIM / 32;  // channels a lane sums
 
-// What rounding `x` to T left out, itself rounded: nothing for fp32, nor next to an overflow.
+// What rounding `x` to T left out, to be rounded itself: nothing for fp32, nor next to an overflow. For
+// fp16 it is 2^11 times that, no larger than x: as it is, it would be lost below the type's smallest
+// numbers wherever |x| is below 2^-14.
+template <typename T>
+constexpr float REST_RAISE = std::is_same<T, __half>::value ? 2048.f : 1.f;
 template <typename T>
 __device__ __forceinline__ float rest_of(float x) {
   const float r = x - to_f32(from_f32<T>(x));
-  return fabsf(r) < INFINITY ? r : 0.f;
+  return fabsf(r) < INFINITY ? r * REST_RAISE<T> : 0.f;
+}
+// x again, from its rounded value and a stored rest.
+template <typename T>
+__device__ __forceinline__ float whole_of(T x, T rest) {
+  return fmaf(to_f32(rest), 1.f / REST_RAISE<T>, to_f32(x));
 }
 
 // ---- one row of one head computed again, by a warp: lanes along the other side's rows for the
@@ -257,7 +268,7 @@ __device__ void row_dq(const AttnArgs& a, int64_t p, int h, float* scratch) {
   for (int d = lane; d < a.dim; d += 32) {
     s_q[d] = to_f32(q[d]) * a.scale;
     s_g[d] = to_f32(g[d]);
-    delta = fmaf(s_g[d], to_f32(o[d]) + (o_rest ? to_f32(o_rest[d]) : 0.f), delta);
+    delta = fmaf(s_g[d], o_rest ? whole_of(o[d], o_rest[d]) : to_f32(o[d]), delta);
   }
   delta = warp_sum(delta);
   __syncwarp();

@@ -35,6 +35,12 @@
 // unrounded. The forward pass of training adds a second product for what rounding the weights leaves
 // out: delta, which dS is a small difference with, comes from its output (dq and dk off by 1.42 times
 // the plain form's error instead of up to 1.55, for 22 us of 225 at 20,331 x 16 x 64).
+//
+// In fp16 these operands, and what rounding the output leaves out, are raised by powers of two that the
+// result's factor takes back: below 2^-14 a half has no 11 bits, below 2^-25 it is zero, and the weights
+// of long windows and the score gradients of a mean loss lie there (unraised, dq of 4,096 rows was off by
+// 8 times the result's rounding at output gradients of 1e-3). Weights by fixed powers, score gradients by
+// one for each row, lowered when a larger one comes.
 #include <limits.h>
 
 #include <algorithm>
@@ -53,6 +59,12 @@ constexpr int KB = 32;   // positions of a tile
 // Rows of a block in the forward pass: two 16-row parts a warp, whose products share the tile's
 // fragments (8,192 x 6 x 128 fp16: 678 us with one, 651 with two).
 constexpr int FORWARD_ROWS = 128;
+
+template <typename T>
+constexpr bool IS_HALF = std::is_same<T, __half>::value;
+// The dk / dv pass's weights, at most 1, as operands: raised by this.
+template <typename T>
+constexpr float RAISE = IS_HALF<T> ? 32768.f : 1.f;
 
 // Tiles hold DP channels a row (the head's, padded with zeros) at a stride that is an odd multiple
 // of 16 bytes, so the 8 rows of a matrix fragment fall into different banks.
@@ -221,7 +233,7 @@ struct alignas(16) Shared {
   KeyMeta key[SLOTS][KB];       // the other side's rows
   int2 key_lin[SLOTS][KB];      // their linear coordinates (Block::lin)
   int32_t key_row[SLOTS][KB];
-  float2 key_stats[SLOTS][KB];  // their softmax and delta (dk / dv)
+  float2 key_stats[SLOTS][KB];  // their softmax, the weights raised by RAISE, and delta (dk / dv)
   float key_delta[SLOTS][KB];
   int32_t key_bad[SLOTS];       // whether a position has no row
   PlanRow own[BQ];
@@ -347,6 +359,7 @@ struct Block {
       float d = 0.f;
       if (m.row >= 0) {
         st = a.stats[head * a.n + j];
+        st.y *= RAISE<T>;
         d = a.delta[head * a.n + j];
       }
       s.key_stats[slot][i] = st;
@@ -686,9 +699,14 @@ __device__ __forceinline__ void walk(B& b, Load&& load, Body&& body, Ask&& ask, 
   __syncthreads();
 }
 
-// Scores may pass the running base by this much (in powers of two) before the sums are rescaled, so
-// most tiles skip it; weights then reach 2^8 at most, which neither type nor the fp32 sums notice.
-constexpr float SLACK = 8.f;
+// The running base lies LIFT below the largest score that it was set by, so that weights start at
+// 2^LIFT, and scores may pass that by SLACK (all in powers of two) before the sums are rescaled, so most
+// tiles skip it. bf16: weights of 1 to 2^8, which neither the type nor the fp32 sums notice. fp16: up
+// to 2^15, so that weights 2^-27 of the largest still have all their bits.
+template <typename T>
+constexpr float LIFT = IS_HALF<T> ? 13.f : 0.f;
+template <typename T>
+constexpr float SLACK = IS_HALF<T> ? 2.f : 8.f;
 
 // MR: 16-row parts of a warp, whose products share the tile's fragments. TRAIN: the backward pass's
 // inputs are kept too.
@@ -764,7 +782,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
 #pragma unroll
           for (int n = 1; n < KB / 8; ++n) x = fmaxf(x, fmaxf(s[m][n][2 * r], s[m][n][2 * r + 1]));
           top[m][r] = x;
-          over = over || x > base[m][r] + SLACK;
+          over = over || x > base[m][r] + (LIFT<T> + SLACK<T>);
         }
       }
       if (__any_sync(0xffffffffu, over)) {
@@ -775,7 +793,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
             float x = top[m][r];
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-            x = fmaxf(x, base[m][r]);
+            x = fmaxf(x - LIFT<T>, base[m][r]);
             const float keep = exp2_fast(base[m][r] - x);
             base[m][r] = x;
             sum[m][r] *= keep;
@@ -940,16 +958,54 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a, bool vec) {
         const T* ye = reinterpret_cast<const T*>(&y);
         const T* ze = reinterpret_cast<const T*>(&z);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) d = fmaf(to_f32(xe[k]), to_f32(ye[k]) + to_f32(ze[k]), d);
+        for (int k = 0; k < 8; ++k) d = fmaf(to_f32(xe[k]), whole_of(ye[k], ze[k]), d);
       }
     } else {
       for (int c = sub; c < a.dim; c += 8)
-        d = fmaf(to_f32(g[c]), to_f32(o[c]) + (rest ? to_f32(rest[c]) : 0.f), d);
+        d = fmaf(to_f32(g[c]), rest ? whole_of(o[c], rest[c]) : to_f32(o[c]), d);
     }
   }
 #pragma unroll
   for (int s = 4; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
   if (sub == 0 && live) a.delta[h * a.n + p] = d;
+}
+
+// Raises score gradients `ds` of a thread's two rows (g and g + 8; the four lanes of a row agree) so that
+// their largest lies below 2^15, and lowers the sums formed so far with them: `by` is a power of two
+// for each row, no larger than it was.
+constexpr float RAISE_START = 0x1p100f;
+template <int DP>
+__device__ __forceinline__ void raise_rows(float (&ds)[KB / 8][4], float (&by)[2],
+                                           float (&sums)[DP / 8][4]) {
+  float top[2] = {0.f, 0.f};
+#pragma unroll
+  for (int n = 0; n < KB / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], fabsf(ds[n][e]));
+  constexpr float LIMIT = 32768.f;
+  if (__any_sync(0xffffffffu, top[0] * by[0] > LIMIT || top[1] * by[1] > LIMIT)) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float x = top[r];
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      // an infinity stays one, and its row is computed again
+      if (x * by[r] > LIMIT && x < INFINITY) {
+        const float to = __uint_as_float((268u - (__float_as_uint(x) >> 23)) << 23);  // x to = 2^14 ..
+        const float keep = to / by[r];
+        by[r] = to;
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n) {
+          sums[n][2 * r] *= keep;
+          sums[n][2 * r + 1] *= keep;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < KB / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ds[n][e] *= by[e >> 1];
 }
 
 // The table's gradient in fixed point, with a unit for each bucket: a score gradient is at most 2^18 of
@@ -1039,8 +1095,9 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
       inv[r] = st.y;
       delta[r] = live ? a.delta[p] : 0.f;
     }
-    float dq[1][DP / 8][4];
+    float dq[1][DP / 8][4], by[2] = {1.f, 1.f};
     zero(dq[0]);
+    if constexpr (IS_HALF<T>) by[0] = by[1] = RAISE_START;
     auto body = [&](int t, int buf) {
       const int p0 = b.j0 + t * KB;
       if (p0 >= w.hi || p0 + KB <= w.lo) return;
@@ -1083,6 +1140,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
           grad(n, e, at, !hidden(seen, n, e, bad, sh, slot));
         });
       }
+      if constexpr (IS_HALF<T>) raise_rows<DP>(s[0], by, dq[0]);
       mma_nn<T, DP, 1>(dq, s, tile);
     };
     walk<false, STAGES>(
@@ -1093,8 +1151,8 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
           load_tile<T, DP, KB>(tile + L::TILE, v, (int)a.v_row, rows, a.dim, vec);
         },
         body, [&] { return TABLE && spent > LIMIT; }, flush);
-    store_rows<T, DP>(mine, dq[0], a.scale, a.scale, sh.own_row + warp * 16, static_cast<T*>(a.dq),
-                      a.heads, head, a.dim, vec);
+    store_rows<T, DP>(mine, dq[0], a.scale / by[0], a.scale / by[1], sh.own_row + warp * 16,
+                      static_cast<T*>(a.dq), a.heads, head, a.dim, vec);
     again(not_finite<DP>(dq[0]), warp * 16, mine, [&](int i, float* f) {
       if (sh.own_row[i] >= 0) again_dq<T>(a, at.x + i, head, f);
     });
@@ -1139,7 +1197,8 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
     const PlanRow* own = sh.own + warp * 16 + g;
     const Reach w = warp_reach<16>(sh.own + warp * 16);
     const bool solo[2] = {lone(own[0]), lone(own[8])};
-    float dk[1][DP / 8][4], dv[1][DP / 8][4];
+    float dk[1][DP / 8][4], dv[1][DP / 8][4], by[2] = {1.f, 1.f};
+    if constexpr (IS_HALF<T>) by[0] = by[1] = RAISE_START;
     zero(dk[0]);
     zero(dv[0]);
     auto body = [&](int t, int buf) {
@@ -1180,6 +1239,7 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
         });
       }
       mma_nn<T, DP, 1>(dv, s, tile + L::TILE);
+      if constexpr (IS_HALF<T>) raise_rows<DP>(dp[0], by, dk[0]);
       mma_nn<T, DP, 1>(dk, dp, tile);
     };
     walk<true, STAGES>(
@@ -1190,9 +1250,10 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
           load_tile<T, DP, KB>(tile + L::TILE, dout, g_row, rows, a.dim, vec);
         },
         body, [] { return false; }, [] {});
-    store_rows<T, DP>(mine, dk[0], lone(own[0]) ? 0.f : a.scale, lone(own[8]) ? 0.f : a.scale,
-                      sh.own_row + warp * 16, static_cast<T*>(a.dk), a.heads, head, a.dim, vec);
-    store_rows<T, DP>(mine + L::OWN_TILE, dv[0], 1.f, 1.f, sh.own_row + warp * 16,
+    // a power of two, and the quotient exact
+    const float down[2] = {a.scale / RAISE<T> / by[0], a.scale / RAISE<T> / by[1]};
+    store_rows<T, DP>(mine, dk[0], solo[0] ? 0.f : down[0], solo[1] ? 0.f : down[1], sh.own_row + warp * 16, static_cast<T*>(a.dk), a.heads, head, a.dim, vec);
+    store_rows<T, DP>(mine + L::OWN_TILE, dv[0], 1.f / RAISE<T>, 1.f / RAISE<T>, sh.own_row + warp * 16,
                       static_cast<T*>(a.dv), a.heads, head, a.dim, vec);
     again(not_finite<DP>(dk[0]) | not_finite<DP>(dv[0]), warp * 16, mine, [&](int i, float* f) {
       if (sh.own_row[i] >= 0) again_dkv<T>(a, at.x + i, head, f);
@@ -1202,7 +1263,8 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
   if constexpr (TABLE) {  // behind the last block's barrier
     unsigned* to = a.tops + (int64_t)head * cells;
     for (int i = threadIdx.x; i < cells; i += AT)
-      if (s_top[i] != 0u) atomicMax(to + i, s_top[i]);
+      if (s_top[i] != 0u)
+        atomicMax(to + i, __float_as_uint(__uint_as_float(s_top[i]) / RAISE<T>));
   }
 }
 

@@ -1,16 +1,21 @@
-"""Gradients of the biased attention in fp16 / bf16 where their magnitudes span many powers of two:
-tables that fall steeply, rows whose output gradient lies far above the others'. Every entry is held
-to what its own terms allow, not to the largest of the head.
+"""The biased attention in fp16 / bf16 where magnitudes span many powers of two: tables that fall steeply,
+rows whose output gradient lies far above the others', small output gradients and weights. Every
+entry is held to what its own terms allow, not to the largest of the head.
 
 Bounds, with u = 2^-24 and e = eps / 2 of the type: a score is off by (2 dim + 32) u of the magnitudes in
 it, so a weight p by twice that (and its row's largest) of itself; dP by (2 dim + 16) u of |dout||v|; delta, a
 mean of dP over rows, by as much of the row's mean of |dout||v| and by what the output keeps of the
-forward pass, at most e^2 of |dout||out| twice over. So a score gradient is off by
+forward pass, at most e^2 of |dout||out| twice over and half of the rest's smallest number (2^-25 of
+2^-11 in fp16). So a score gradient is off by
 
     ds_off = |ds| (p's) + p (dP's + delta's),
 
 none of it rounded to the type. A bucket of the table sums its terms in units of at most 2^-16 of its own
-largest term, half a unit a pair, and is rounded once."""
+largest term, half a unit a pair, and is rounded once.
+
+As operands of the second products weights and score gradients are rounded to the type, by e of
+themselves. In fp16 they are raised first: below 2^-27 of a row's (or, for dv, of 1) a weight is off by 2^-38
+of that at most, a score gradient below 2^-28 of its row's largest by 2^-39 of that."""
 
 from __future__ import annotations
 
@@ -60,6 +65,7 @@ def _falling_table(heads, side, step, dtype):
 def _terms(coords, q, k, v, table, lut, window, dout):
     """Per window: its rows, the buckets [L, L], and p, ds and ds_off [heads, L, L]."""
     e = _half(q.dtype)
+    small = 2.0**-36 if q.dtype == torch.float16 else 2.0**-126
     q, k, v, flat, dout = (t.detach().to(F64) for t in (q, k, v, table.flatten(1), dout))
     reach, nb, dim = lut.numel() // 2, table.shape[-1], q.shape[-1]
     x = SparseTensor(torch.zeros((len(coords), 1), device=DEV), coords)
@@ -80,7 +86,7 @@ def _terms(coords, q, k, v, table, lut, window, dout):
         out = p @ vs
         ds = p * (dp - delta)
         p_rel = 2 * s_off + 2 * s_off.amax(-1, keepdim=True) + 8 * U
-        kept = 2 * e * e * (gs.abs() * (p @ vs.abs())).sum(-1, keepdim=True)
+        kept = (2 * e * e * gs.abs() * (p @ vs.abs()) + small * gs.abs()).sum(-1, keepdim=True)
         d_off = ((p * p_rel) @ vs.abs() * gs.abs()).sum(-1, keepdim=True) + kept + \
             (2 * dim + 2 * len(rows)) * U * (p * mag).sum(-1, keepdim=True) + \
             2 * dim * U * (gs.abs() * out.abs()).sum(-1, keepdim=True)
@@ -163,3 +169,74 @@ def test_table_beside_a_value_that_is_not_finite(dtype):
     touched[1, 6:8, 7, 7] = True  # from it to the other row and to itself: -1 and 0 along x
     assert torch.equal(got[~touched], clean[~touched])
     assert not torch.isfinite(got[touched]).any()
+
+
+def _check_rows(coords, q, k, v, table, lut, window, dout, got):
+    """out, dq, dk and dv against the formula, entry by entry, and (the errors of single operands being
+    independent) as a whole: an operand's rounding and the result's, each half a step, give 2^0.5 of the
+    result's alone; 2 leaves room for ds_off and the sums. The result's is taken as what rounding the
+    exact value to the type leaves."""
+    dtype = q.dtype
+    e, scale = _half(dtype), q.shape[-1] ** -0.5
+    wants = [torch.zeros(q.shape, dtype=F64, device=DEV) for _ in range(4)]
+    offs = [torch.zeros(q.shape, dtype=F64, device=DEV) for _ in range(4)]
+    small_p, small_ds = (2.0**-38, 2.0**-39) if dtype == torch.float16 else (2.0**-126,) * 2
+    for rows, _, p, ds, ds_off in _terms(coords, q, k, v, table, lut, window, dout):
+        n = len(rows)
+        qs, ks, vs, gs = (t.detach().to(F64)[rows].transpose(0, 1) for t in (q, k, v, dout))
+        s_off = (2 * q.shape[-1] + 32) * U * (
+            qs.abs() @ ks.abs().transpose(1, 2) * scale + table.abs().max().double())
+        p_off = p * (2 * s_off + 2 * s_off.amax(-1, keepdim=True) + 8 * U + e + 2 * n * U)
+        t_off = ds_off + (e + 2 * n * U) * ds.abs()
+        by_query = t_off + small_ds * ds.abs().amax(-1, keepdim=True)
+        by_key = t_off + small_ds * ds.abs().amax(-2, keepdim=True)
+        for i, (value, off) in enumerate((
+                (p @ vs, (p_off + small_p) @ vs.abs()),
+                (ds @ ks * scale, by_query @ ks.abs() * scale),
+                (ds.transpose(1, 2) @ qs * scale, by_key.transpose(1, 2) @ qs.abs() * scale),
+                (p.transpose(1, 2) @ gs, (p_off + small_p).transpose(1, 2) @ gs.abs()))):
+            wants[i][rows] = value.transpose(0, 1)
+            offs[i][rows] = (off + e * (value.abs() + off)).transpose(0, 1) + _least(dtype)
+    for name, a, want, off in zip(("out", "dq", "dk", "dv"), got, wants, offs):
+        err = (a.to(F64) - want).abs()
+        assert (err <= off).all(), (name, float((err / off).max()))
+        alone = (want.to(dtype).to(F64) - want).norm()
+        assert err.norm() <= 2 * alone, (name, float(err.norm() / alone))
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4])
+def test_small_output_gradients_in_half_precision(size):
+    """4,096 rows that all see each other: score gradients around 2^-12 of the output's, which for a mean
+    loss is below the smallest numbers of the type."""
+    coords = _voxels(4096, 16, 4)
+    lut = position_buckets(15, 8, device=DEV)
+    q, k, v = (_rand((4096, 2, 64), torch.float16, 30 + i) for i in range(3))
+    dout = _rand((4096, 2, 64), torch.float16, 33, size)
+    table = _rand((2, 17, 17, 17), torch.float16, 34)
+    got = _attend(coords, q, k, v, table, lut, None, dout)
+    _check_rows(coords, q, k, v, table, lut, None, dout, got[:4])
+    _check_table(coords, q, k, v, table, lut, None, dout, got[4])
+
+
+@pytest.mark.parametrize("window", [8, None])
+@pytest.mark.parametrize("dtype", HALVES)
+def test_weights_far_below_the_largest(dtype, window):
+    """Every row sees itself e^17 times as much as any other, and half of the rows hold nothing: their
+    outputs are sums of weights around 2^-24."""
+    n = 2500 if window else 3000
+    coords = _voxels(n, 16, 5)
+    reach = 7 if window else 15
+    lut = position_buckets(reach, 3, device=DEV)
+    q, k = (_rand((n, 2, 32), dtype, 40 + i, 0.1) for i in range(2))
+    v = 1 + _rand((n, 2, 32), dtype, 42, 0.25)
+    v[::2] = 0
+    dout = _rand((n, 2, 32), dtype, 43)
+    dout[1::2] = 0
+    table = torch.zeros((2, 7, 7, 7), dtype=dtype, device=DEV)
+    table[:, 3, 3, 3] = 17
+    got = _attend(coords, q, k, v, table, lut, window, dout)
+    _check_rows(coords, q, k, v, table, lut, window, dout, got[:4])
+    x = SparseTensor(torch.zeros((n, 1), device=DEV), coords)
+    serving = sparse_self_attention(x, q, k, v, window_size=window, position_bias=table,
+                                    position_buckets=lut)
+    _check_rows(coords, q, k, v, table, lut, window, dout, (serving,))
