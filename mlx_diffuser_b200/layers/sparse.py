@@ -622,6 +622,12 @@ def sparse_subdivide(x: SparseTensor) -> SparseTensor:
                         spatial_shape, scale, {})
 
 
+def _version(coords: torch.Tensor) -> int | None:
+    """The coordinates' version counter; None for an inference tensor, which has none."""
+
+    return None if coords.is_inference() else coords._version
+
+
 @dataclasses.dataclass
 class WindowGroups:
     """Attention windows of a sparse tensor as one device permutation: group g is
@@ -630,22 +636,23 @@ class WindowGroups:
     ``buckets`` maps a group length L to the [groups, L] row-index matrix of all groups of that
     length (built on first use; one host read of the lengths). ``plan`` holds the rows in window
     order with their coordinates and window bounds, for the biased attention kernels, next to the
-    coordinates it was built from (held, version-checked)."""
+    coordinates it was built from (held, version-checked where the tensor has a version: those of
+    inference mode do not)."""
 
     perm: torch.Tensor
     offsets: torch.Tensor
     buckets: dict[int, torch.Tensor] | None = None
-    plan: tuple[torch.Tensor, int, torch.Tensor] | None = None
+    plan: tuple[torch.Tensor, int | None, torch.Tensor] | None = None
 
     def plan_rows(self, coords: torch.Tensor) -> torch.Tensor:
         if (self.plan is None or self.plan[0] is not coords
-                or self.plan[1] != coords._version):
+                or self.plan[1] != _version(coords)):
             rows = window_plan(coords.contiguous(), self.perm, self.offsets)
             if torch.cuda.is_current_stream_capturing():
                 return rows  # written by the graph's replays alone: not for others
             # like the grouping, whole for whatever stream uses it next
             torch.cuda.current_stream(coords.device).synchronize()
-            self.plan = (coords, coords._version, rows)
+            self.plan = (coords, _version(coords), rows)
         return self.plan[2]
 
     @property

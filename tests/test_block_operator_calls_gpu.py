@@ -1,0 +1,68 @@
+"""How ``rms_norm``, ``linear`` and the biased attention may be called: autograd modes, coordinates that
+change, streams and graphs that share a tensor's cache."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from mlx_diffuser_b200 import SparseTensor, _native as N
+from mlx_diffuser_b200 import linear, position_buckets, rms_norm, sparse_self_attention
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+
+
+def _rand(shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(shape, device=DEV, generator=g) * scale).to(dtype)
+
+
+def _voxels(n, grid, seed):
+    cells = np.random.default_rng(seed).choice(grid**3, n, replace=False)
+    rows = np.stack([np.zeros(n, np.int64), *np.unravel_index(cells, (grid,) * 3)], 1)
+    return torch.from_numpy(rows.astype(np.int32)).to(DEV)
+
+
+def _tensor(coords):
+    return SparseTensor(torch.zeros((len(coords), 1), device=DEV), coords)
+
+
+def _attention(n=400, dtype=torch.bfloat16, seed=0):
+    """A call of the biased attention on a tensor of n rows."""
+    q, k, v = (_rand((n, 2, 32), dtype, seed + i) for i in range(3))
+    table, lut = _rand((2, 9, 9, 9), dtype, seed + 3), position_buckets(4, 4, device=DEV)
+
+    def run(x, window=5):
+        return sparse_self_attention(x, q, k, v, window_size=window, position_bias=table,
+                                     position_buckets=lut)
+
+    return run
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_inference_mode(dtype):
+    """Tensors made under inference mode have no version counter; inside and outside of it the operators
+    give what they give elsewhere."""
+    coords = _voxels(400, 12, 1)
+    run = _attention(dtype=dtype)
+    want = run(_tensor(coords))
+    f, g, w = (_rand(s, dtype, 10 + i) for i, s in enumerate([(90, 64), (64,), (32, 64)]))
+    want_y, want_z = rms_norm(f, g), linear(f, w, activation="silu")
+    with torch.inference_mode():
+        x = _tensor(coords.clone())
+        assert x.coords.is_inference()
+        first, again = run(x), run(x)
+        assert torch.equal(first, want) and torch.equal(again, want)
+        assert torch.equal(rms_norm(f.clone(), g), want_y)
+        assert torch.equal(linear(f, w.clone(), activation="silu"), want_z)
+        (q8, s8), h = rms_norm(f, g, residual=f.clone(), quantize=True)
+    (q8_, s8_), h_ = rms_norm(f, g, residual=f, quantize=True)
+    assert torch.equal(q8.view(torch.uint8), q8_.view(torch.uint8))
+    assert torch.equal(s8, s8_) and torch.equal(h, h_)
+    assert torch.equal(run(x), want)  # the tensor used after the mode has ended
+    with torch.inference_mode():
+        assert torch.equal(run(_tensor(coords)), want)  # an ordinary tensor inside it
+    N.check_device_status(DEV)
