@@ -62,13 +62,15 @@ class _WindowAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, table, lut, plan, windows, scale):
         out, rest, stats = _forward(q, k, v, table, lut, plan, windows, scale, True)
         ctx.scale = scale
-        ctx.save_for_backward(q, k, v, table, lut, plan, out, rest, stats)
+        # not a saved tensor: one laid out under inference mode could not be, and nothing changes it
+        ctx.plan = plan
+        ctx.save_for_backward(q, k, v, table, lut, out, rest, stats)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, lut, plan, out, rest, stats = ctx.saved_tensors
+        q, k, v, table, lut, out, rest, stats = ctx.saved_tensors
         n, heads, dim = q.shape
         dev = q.device
         dout = dout.contiguous()
@@ -81,7 +83,7 @@ class _WindowAttention(torch.autograd.Function):
             rc = lib.sv_window_attention_backward(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), out.data_ptr(),
                 N.ptr(rest), dout.data_ptr(), stats.data_ptr(), n, heads, dim,
-                N.DTYPE_CODE[q.dtype], plan.data_ptr(), table.data_ptr(), table.shape[-1],
+                N.DTYPE_CODE[q.dtype], ctx.plan.data_ptr(), table.data_ptr(), table.shape[-1],
                 lut.data_ptr(), lut.numel() // 2, ctx.scale, dq.data_ptr(), dk.data_ptr(),
                 dv.data_ptr(), N.ptr(dtable), ws.data_ptr(), nbytes, N.stream(dev))
         N.check(rc, "sparse_self_attention (backward)")

@@ -66,3 +66,23 @@ def test_inference_mode(dtype):
     with torch.inference_mode():
         assert torch.equal(run(_tensor(coords)), want)  # an ordinary tensor inside it
     N.check_device_status(DEV)
+
+
+def test_training_on_windows_laid_out_under_inference_mode():
+    """A tensor whose first call was under inference mode is trained on later."""
+    coords = _voxels(400, 12, 2)
+    lut = position_buckets(4, 4, device=DEV)
+    leaves = [_rand((400, 2, 32), torch.bfloat16, i).requires_grad_(True) for i in range(3)]
+    leaves.append(_rand((2, 9, 9, 9), torch.bfloat16, 3).requires_grad_(True))
+    dout = _rand((400, 2, 32), torch.bfloat16, 4)
+
+    def step(x):
+        out = sparse_self_attention(x, *leaves[:3], window_size=5, position_bias=leaves[3],
+                                    position_buckets=lut)
+        return (out, *torch.autograd.grad(out, leaves, dout))
+
+    want = step(_tensor(coords))
+    x = _tensor(coords)
+    with torch.inference_mode():
+        _attention()(x)
+    assert all(torch.equal(a, b) for a, b in zip(step(x), want))
