@@ -633,27 +633,31 @@ class WindowGroups:
     """Attention windows of a sparse tensor as one device permutation: group g is
     ``perm[offsets[g]:offsets[g + 1]]``. Groups are in the order of their first row and rows
     ascend inside a group, the order of the reference's ``_attention_groups`` lists.
-    ``buckets`` maps a group length L to the [groups, L] row-index matrix of all groups of that
-    length (built on first use; one host read of the lengths). ``plan`` holds the rows in window
-    order with their coordinates and window bounds, for the biased attention kernels, next to the
-    coordinates it was built from (held, version-checked where the tensor has a version: those of
-    inference mode do not)."""
+    ``coords`` are the coordinates it was made from, with their version (None for those of
+    inference mode, which have none): it serves no others. ``buckets`` maps a group length L to the
+    [groups, L] row-index matrix of all groups of that length (built on first use; one host read of
+    the lengths). ``plan`` holds the rows in window order with their coordinates and window bounds,
+    for the biased attention kernels."""
 
     perm: torch.Tensor
     offsets: torch.Tensor
+    coords: torch.Tensor
+    version: int | None
     buckets: dict[int, torch.Tensor] | None = None
-    plan: tuple[torch.Tensor, int | None, torch.Tensor] | None = None
+    plan: torch.Tensor | None = None
 
-    def plan_rows(self, coords: torch.Tensor) -> torch.Tensor:
-        if (self.plan is None or self.plan[0] is not coords
-                or self.plan[1] != _version(coords)):
-            rows = window_plan(coords.contiguous(), self.perm, self.offsets)
+    def serves(self, coords: torch.Tensor) -> bool:
+        return self.coords is coords and self.version == _version(coords)
+
+    def plan_rows(self) -> torch.Tensor:
+        if self.plan is None:
+            rows = window_plan(self.coords.contiguous(), self.perm, self.offsets)
             if torch.cuda.is_current_stream_capturing():
                 return rows  # written by the graph's replays alone: not for others
             # like the grouping, whole for whatever stream uses it next
-            torch.cuda.current_stream(coords.device).synchronize()
-            self.plan = (coords, _version(coords), rows)
-        return self.plan[2]
+            torch.cuda.current_stream(self.coords.device).synchronize()
+            self.plan = rows
+        return self.plan
 
     @property
     def num_groups(self) -> int:
@@ -682,12 +686,13 @@ def attention_windows(
 ) -> WindowGroups:
     """Group rows by batch, or by batch and ``(coords + shift) // window_size``, on the GPU
     (``_attention_groups``, ``src/mlx_diffuser/layers/sparse.py:321-342``), cached under the
-    reference's key ``attention_groups_{window_size}_{shift}_{scale}``."""
+    reference's key ``attention_groups_{window_size}_{shift}_{scale}`` and made again for other
+    coordinates than the cached ones (another tensor, or changed in place)."""
 
     shift = tuple(int(v) for v in shift_window)
     key = f"attention_groups_{window_size}_{shift}_{x.scale}"
     cached = x.cache.get(key)
-    if cached is not None:
+    if cached is not None and cached.serves(x.coords):
         return cached
     if window_size is not None and int(window_size) < 1:
         raise ValueError("window_size must be a positive integer or None")
@@ -709,7 +714,7 @@ def attention_windows(
         ws.data_ptr(), ws_bytes, N.stream(dev),
     )
     N.check(rc, "attention groups")
-    result = WindowGroups(perm, offsets[: int(groups.value) + 1])
+    result = WindowGroups(perm, offsets[: int(groups.value) + 1], x.coords, _version(x.coords))
     x.cache[key] = result
     return result
 
@@ -788,8 +793,8 @@ def _biased_self_attention(x, q, k, v, window_size, shift_window, table, lut) ->
     with N.on_device(q.device):
         groups = attention_windows(x, window_size, shift_window)
         if groups.perm.numel() != q.shape[0]:
-            raise ValueError("the cached attention windows belong to other coordinates")
-        plan = groups.plan_rows(x.coords)
+            raise ValueError("coords must have one row per feature row")
+        plan = groups.plan_rows()
     return biased_window_attention(q, k, v, table, lut, plan, groups.num_groups, dim**-0.5)
 
 

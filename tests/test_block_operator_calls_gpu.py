@@ -86,3 +86,38 @@ def test_training_on_windows_laid_out_under_inference_mode():
     with torch.inference_mode():
         _attention()(x)
     assert all(torch.equal(a, b) for a, b in zip(step(x), want))
+
+
+@pytest.mark.parametrize("window", [5, None])
+def test_changed_coordinates(window):
+    """Windows and biases belong to the coordinates that the tensor holds now: changed in place, or
+    another tensor's beside the same cache."""
+    coords = _voxels(400, 12, 3)
+    other = _voxels(400, 12, 4)
+    other[200:, 0] = 1
+    run = _attention()
+    want, want_other = run(_tensor(coords), window), run(_tensor(other), window)
+    assert not torch.equal(want, want_other)
+    x = _tensor(coords.clone())
+    assert torch.equal(run(x, window), want)
+    y = x.replace(x.features, other)  # shares the cache
+    assert y.cache is x.cache
+    assert torch.equal(run(y, window), want_other)
+    assert torch.equal(run(x, window), want)
+    x.coords.copy_(other)
+    assert torch.equal(run(x, window), want_other)
+    # the same windows without a bias
+    q = _rand((400, 2, 32), torch.bfloat16, 50)
+    z = _tensor(coords.clone())
+    sparse_self_attention(z, q, q, q, window_size=window)
+    z.coords.copy_(other)
+    assert torch.equal(sparse_self_attention(z, q, q, q, window_size=window),
+                       sparse_self_attention(_tensor(other), q, q, q, window_size=window))
+    N.check_device_status(DEV)
+
+
+def test_fewer_coordinates_than_features_are_refused():
+    x = _tensor(_voxels(400, 12, 5))
+    x.coords = x.coords[:300]
+    with pytest.raises(ValueError, match="one row per feature row"):
+        _attention()(x)
