@@ -637,7 +637,7 @@ class WindowGroups:
     inference mode, which have none): it serves no others. ``buckets`` maps a group length L to the
     [groups, L] row-index matrix of all groups of that length (built on first use; one host read of
     the lengths). ``plan`` holds the rows in window order with their coordinates and window bounds,
-    for the biased attention kernels."""
+    for the biased attention kernels; ``stream`` is the one it was laid out on."""
 
     perm: torch.Tensor
     offsets: torch.Tensor
@@ -645,18 +645,31 @@ class WindowGroups:
     version: int | None
     buckets: dict[int, torch.Tensor] | None = None
     plan: torch.Tensor | None = None
+    stream: int | None = None
 
     def serves(self, coords: torch.Tensor) -> bool:
         return self.coords is coords and self.version == _version(coords)
 
-    def plan_rows(self) -> torch.Tensor:
+    def plan_rows(self, cache: dict) -> torch.Tensor:
+        """The plan, for a call on the current stream. What a graph's replays will read stays in the
+        tensor's ``cache`` when the coordinates change and another grouping takes this one's place."""
+
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
+            captured = cache.setdefault("attention_groups_captured", [])
+            if not any(g is self for g in captured):
+                captured.append(self)
+        stream = torch.cuda.current_stream(self.coords.device)
         if self.plan is None:
             rows = window_plan(self.coords.contiguous(), self.perm, self.offsets)
-            if torch.cuda.is_current_stream_capturing():
+            if capturing:
                 return rows  # written by the graph's replays alone: not for others
             # like the grouping, whole for whatever stream uses it next
-            torch.cuda.current_stream(self.coords.device).synchronize()
-            self.plan = rows
+            stream.synchronize()
+            self.plan, self.stream = rows, stream.cuda_stream
+        elif not capturing and stream.cuda_stream != self.stream:
+            # its memory is not handed on before this stream's calls have read it
+            self.plan.record_stream(stream)
         return self.plan
 
     @property
@@ -749,7 +762,9 @@ def sparse_self_attention(
     the difference clamped to ``-reach..reach`` (:func:`position_buckets` makes one). Scores, bias,
     softmax and sums then run in one kernel over all windows, with gradients for ``q``, ``k``, ``v``
     and the table that do not depend on the order of execution. head_dim up to 128, B up to 25,
-    reach up to 1023. A row whose every score is -inf gives zeros."""
+    reach up to 1023. A row whose every score is -inf gives zeros. A call captured into a CUDA graph
+    reads the windows that ``x``'s cache holds then: keep ``x`` as long as the graph, and capture
+    again after its coordinates have changed."""
 
     if q.shape != k.shape or q.shape != v.shape or q.shape[0] != x.num_points:
         raise ValueError("q, k, and v must share shape (N, heads, head_dim)")
@@ -794,7 +809,7 @@ def _biased_self_attention(x, q, k, v, window_size, shift_window, table, lut) ->
         groups = attention_windows(x, window_size, shift_window)
         if groups.perm.numel() != q.shape[0]:
             raise ValueError("coords must have one row per feature row")
-        plan = groups.plan_rows()
+        plan = groups.plan_rows(x.cache)
     return biased_window_attention(q, k, v, table, lut, plan, groups.num_groups, dim**-0.5)
 
 

@@ -121,3 +121,49 @@ def test_fewer_coordinates_than_features_are_refused():
     x.coords = x.coords[:300]
     with pytest.raises(ValueError, match="one row per feature row"):
         _attention()(x)
+
+
+def test_plan_read_on_another_stream_is_not_handed_on():
+    """A plan laid out on one stream and read on another, dropped while that one still works: its memory
+    stays out of the first stream's reach until the reading is done."""
+    coords = _voxels(3000, 16, 6)
+    run = _attention(3000)
+    x = _tensor(coords)
+    want = run(x)
+    plan = next(g for k, g in x.cache.items() if k.startswith("attention_groups_5")).plan
+    address, size = plan.data_ptr(), plan.numel()
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        got = run(x)
+    busy = not side.query()
+    del plan, x
+    taken = [torch.empty(size, dtype=torch.uint8, device=DEV) for _ in range(8)]
+    still = busy and not side.query()
+    inside = [t for t in taken if t.data_ptr() < address + size and address < t.data_ptr() + size]
+    side.synchronize()
+    assert still and not inside
+    assert torch.equal(got, want)
+
+
+def test_captured_call_and_changed_coordinates():
+    """A graph that read the cached plan replays what it captured, though another has taken the plan's
+    place since."""
+    coords = _voxels(400, 12, 7)
+    run = _attention()
+    x = _tensor(coords.clone())
+    want = run(x)
+    N.status_word(DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = run(x)
+    x.coords.copy_(_voxels(400, 12, 8))
+    changed = run(x)
+    assert torch.equal(changed, run(_tensor(x.coords))) and not torch.equal(changed, want)
+    junk = [torch.full((1 << 16,), 255, dtype=torch.uint8, device=DEV) for _ in range(64)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(inside, want)
+    assert len(junk) == 64 and len(x.cache["attention_groups_captured"]) == 1
