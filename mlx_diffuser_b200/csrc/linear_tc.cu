@@ -28,7 +28,9 @@
 //               shared memory, 32 x 32 at a time, so that bias, residual and results are read and
 //               written in whole row segments.
 // Every wait on an mbarrier is bounded (2 s, CTA abort flag); on expiry SV_DEVICE_WAIT_TIMEOUT is
-// reported and the copies and products in flight are waited for before the CTA ends.
+// reported and the copies and products in flight are waited for before the CTA ends. An epilogue warp
+// that has given up still walks its remaining tiles, without waiting, reading sums or storing: the warps
+// decide one by one, and the others' named barrier counts it.
 #include <algorithm>
 
 #include "linear.h"
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     float* chunk = reinterpret_cast<float*>(smem + L::CHUNK_OFF) + (warp - 2) * 32 * CHUNK_LD;
     const bool scaled = ep.row_scale != nullptr || ep.col_scale != nullptr;
     int local = 0;
-    for (int32_t t = unit; t < a.total; t += a.units, ++local) {
+    for (int32_t t = unit; t < a.total; t += a.units, ++local) {  // left by all warps alike
       const Tile w = tile_at<BN, PAIR>(a, t);
       const int ab = local & 1;
       float* s_bias = s_cols + ab * 2 * BN;
@@ -417,6 +419,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         epi_sync();
       }
+      if (!ok) continue;
       const int64_t row0 = (int64_t)w.m0 + rank * TM + q * 32;  // the warp's first row
       const int rows = (int)max((int64_t)0, min((int64_t)32, a.m - row0));
       if (ep.residual && lane < rows) {
@@ -427,7 +430,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       }
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[ab], (local >> 1) & 1, s_abort))) {
         ok = false;
-        break;
+        continue;
       }
       tc_fence_after();
       const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * BN);
