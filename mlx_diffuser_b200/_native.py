@@ -13,6 +13,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libsparsevox.so")
 
@@ -222,6 +223,15 @@ def on_device(device: torch.device):
     if device.index is None or device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(device)
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raise where a tensor carries a forward-mode tangent: kernels write through pointers, and the
+    result would come back without one."""
+
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: no forward-mode derivatives")
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

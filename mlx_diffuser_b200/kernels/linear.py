@@ -163,6 +163,7 @@ def linear(
         or (residual is not None and residual.requires_grad))
     if grads and e4m3:
         raise ValueError("linear: 8-bit operands have no gradients")
+    N.refuse_tangents("linear", x, weight, bias, residual, x_scale, weight_scale)
     N.require_cuda(x, "x")
     x2 = _row_major(x if x.ndim == 2 else x.reshape(math.prod(rows), x.shape[-1]))
     w2 = _row_major(weight)

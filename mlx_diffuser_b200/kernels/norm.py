@@ -200,6 +200,7 @@ def rms_norm(
         or (weight is not None and weight.requires_grad))
     if grads and quantize:
         raise ValueError("rms_norm: the 8-bit output has no gradients")
+    N.refuse_tangents("rms_norm", x, residual, weight)
     N.require_cuda(x, "x")
     x2 = _rows(x, c) if c else x.reshape(math.prod(x.shape[:-1]), 0)
     r2 = None

@@ -800,6 +800,7 @@ def _biased_self_attention(x, q, k, v, window_size, shift_window, table, lut) ->
     if dim > MAX_DIM or not 1 <= table.shape[-1] <= MAX_BUCKETS or lut.numel() // 2 > MAX_REACH:
         raise ValueError(f"position_bias needs head_dim <= {MAX_DIM}, 1 <= B <= {MAX_BUCKETS} and "
                          f"reach <= {MAX_REACH}")
+    N.refuse_tangents("sparse_self_attention with position_bias", q, k, v, table)
     N.require_cuda(q, "q")
     for name, t in (("k", k), ("v", v), ("position_bias", table), ("position_buckets", lut),
                     ("coords", x.coords)):
