@@ -114,7 +114,8 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
            z * 0.39894228040143268f * __expf(-0.5f * z * z);
   if (act == SV_ACT_GELU_TANH) {
     const float g = sigmoid_f(GELU_TANH_2C * (z + GELU_CUBE * z * z * z));
-    return g + z * g * (1.0f - g) * GELU_TANH_2C * (1.0f + 3.0f * GELU_CUBE * z * z);
+    // 1 - g is zero long before z^2 overflows
+    return g + z * g * (1.0f - g) * GELU_TANH_2C * (1.0f + 3.0f * GELU_CUBE * fminf(z * z, 1e30f));
   }
   return 1.0f;
 }
