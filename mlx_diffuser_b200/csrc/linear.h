@@ -67,17 +67,28 @@ __device__ __forceinline__ float rcp_half(float x) {
   return y;
 }
 
-// exp and the quotient are the fast forms: within a few fp32 ulp of the value over the whole
-// range (x / (1 + inf) is 0), which is the error the fp32 path's tolerance counts.
-__device__ __forceinline__ float sigmoid_f(float x) {
-  return __fdividef(1.0f, 1.0f + __expf(-x));
+// The logistic function and its slope, from exp(-|x|): neither overflows, and neither is a difference
+// of nearly equal numbers, so both are within a few fp32 ulp down to the subnormal numbers.
+struct Sigmoid {
+  float value, slope;
+};
+__device__ __forceinline__ Sigmoid sigmoid_f(float x) {
+  const float e = expf(-fabsf(x));
+  const float inv = 1.0f / (1.0f + e);
+  return {x < 0.0f ? e * inv : inv, e * inv * inv};
 }
 
+// For fp32 results. The fast exponential is off by 2 + 1.16 |x| ulp, which the tails would show. Phi(z)
+// is half of erfc(-z / sqrt 2): 1 + erf cancels for negative z. What is left in the tails is the rounding of
+// the argument, which the function multiplies: by |u| for the tanh form's u, by z^2 for Phi.
+__device__ __forceinline__ float tanh_argument(float z) {
+  return GELU_TANH_2C * (z + GELU_CUBE * z * z * z);
+}
 __device__ __forceinline__ float activate(float z, int act) {
-  if (act == SV_ACT_SILU) return z * sigmoid_f(z);
-  if (act == SV_ACT_GELU) return 0.5f * z * (1.0f + erff(z * SQRT_HALF));
+  if (act == SV_ACT_SILU) return z * sigmoid_f(z).value;
+  if (act == SV_ACT_GELU) return 0.5f * z * erfcf(-z * SQRT_HALF);
   // 0.5 (1 + tanh(u)) = sigmoid(2u): no cancellation for negative z
-  if (act == SV_ACT_GELU_TANH) return z * sigmoid_f(GELU_TANH_2C * (z + GELU_CUBE * z * z * z));
+  if (act == SV_ACT_GELU_TANH) return z * sigmoid_f(tanh_argument(z)).value;
   return z;
 }
 
@@ -106,26 +117,39 @@ __device__ __forceinline__ float activate_half(float z, int act) {
 // The activation's derivative.
 __device__ __forceinline__ float activate_slope(float z, int act) {
   if (act == SV_ACT_SILU) {
-    const float g = sigmoid_f(z);
-    return g * (1.0f + z * (1.0f - g));
+    const Sigmoid g = sigmoid_f(z);
+    return g.value + z * g.slope;
   }
   if (act == SV_ACT_GELU)
-    return 0.5f * (1.0f + erff(z * SQRT_HALF)) +
-           z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    return 0.5f * erfcf(-z * SQRT_HALF) + z * 0.39894228040143268f * expf(-0.5f * z * z);
   if (act == SV_ACT_GELU_TANH) {
-    const float g = sigmoid_f(GELU_TANH_2C * (z + GELU_CUBE * z * z * z));
-    // 1 - g is zero long before z^2 overflows
-    return g + z * g * (1.0f - g) * GELU_TANH_2C * (1.0f + 3.0f * GELU_CUBE * fminf(z * z, 1e30f));
+    const Sigmoid g = sigmoid_f(tanh_argument(z));
+    // g.slope is zero long before z^2 overflows
+    return g.value + z * g.slope * GELU_TANH_2C * (1.0f + 3.0f * GELU_CUBE * fminf(z * z, 1e30f));
   }
   return 1.0f;
 }
 
+// And for 16 bits, by the approximate exponential and reciprocal.
+__device__ __forceinline__ Sigmoid sigmoid_half(float x) {
+  const float e = exp2_half(-LOG2_E * fabsf(x));
+  const float inv = rcp_half(1.0f + e);
+  return {x < 0.0f ? e * inv : inv, e * inv * inv};
+}
 __device__ __forceinline__ float activate_slope_half(float z, int act) {
+  if (act == SV_ACT_SILU) {
+    const Sigmoid g = sigmoid_half(z);
+    return g.value + z * g.slope;
+  }
   if (act == SV_ACT_GELU) {
     const float gauss = exp2_half(-0.5f * LOG2_E * z * z);
     return normal_half(z, gauss) + z * 0.39894228040143268f * gauss;
   }
-  return activate_slope(z, act);
+  if (act == SV_ACT_GELU_TANH) {
+    const Sigmoid g = sigmoid_half(tanh_argument(z));
+    return g.value + z * g.slope * GELU_TANH_2C * (1.0f + 3.0f * GELU_CUBE * fminf(z * z, 1e30f));
+  }
+  return 1.0f;
 }
 
 template <typename O>
