@@ -417,8 +417,8 @@ SV_API int sv_linear_forward(const void* x, int64_t ldx, const void* weight, int
                              int32_t* status, sv_stream_t stream);
 
 /* Its gradients for x, weight and bias (each null where it is not wanted), contiguous, in `dtype`
- * (fp32 / fp16 / bf16): with dz = dout * act'(preact) rounded to `dtype` (dout itself without an
- * activation), dx = dz weight, dw = dz^T x, dbias = the column sums of the unrounded dz. Every sum has
+ * (fp32 / fp16 / bf16): with dz = dout * act'(preact) rounded to `dtype` (in fp16 after a power of two
+ * that brings the largest |dout| near the type's; dout itself without an activation), dx = dz weight, dw = dz^T x, dbias = the column sums of the unrounded dz. Every sum has
  * a fixed order. dout: [m, n] contiguous; preact: the forward pass's. */
 SV_API int sv_linear_backward(const void* dout, const float* preact, const void* x, int64_t ldx,
                               const void* weight, int64_t ldw, int64_t m, int64_t k, int64_t n,

@@ -17,6 +17,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "linear.h"
 
@@ -420,6 +421,46 @@ int pad_rows(const Pad* pads, int count, int es, cudaStream_t s) {
   return SV_OK;
 }
 
+// fp16's dz is raised by a power of two before it is rounded, and the products' column scales take it
+// back: below 2^-14 a half has no 11 bits, and the gradients of a mean loss lie there. The power puts the
+// largest |dy| below 2^15 (the activations' slopes are below 1.13), so values down to 2^-28 of it keep
+// all their bits. It costs a pass over dy: 12,001 x 1024 in 7 us.
+struct Raise {
+  unsigned* top;  // bits of the largest |dy|, as a half; null: dz is not raised
+  float* down;    // [k]: what the products are multiplied by
+  int64_t k;
+};
+__device__ __forceinline__ float raise_of(unsigned top) {
+  if (top == 0u || top >= 0x7c00u) return 1.0f;  // nothing, or not a number
+  const float x = __half2float(__ushort_as_half((unsigned short)top));
+  return __uint_as_float((268u - (__float_as_uint(x) >> 23)) << 23);  // 2^14 <= x * this < 2^15
+}
+
+template <int V>
+__global__ void __launch_bounds__(256)
+    top_kernel(const unsigned short* __restrict__ x, int64_t cells, unsigned* __restrict__ top) {
+  unsigned most = 0u;  // of both halves of a word
+  const int64_t step = (int64_t)gridDim.x * 256 * V;
+#pragma unroll 4
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < cells; i += step) {
+    if constexpr (V == 8) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + i));
+      most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                     __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+    } else {
+      most = __vmaxu2(most, x[i] & 0x7fffu);
+    }
+  }
+  __shared__ unsigned s_top[8];
+  const unsigned one = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = one;
+  __syncthreads();
+  if (threadIdx.x < 32) {  // one atomic a block: one a warp took 11 us
+    const unsigned all = __reduce_max_sync(0xffffffffu, threadIdx.x < 8 ? s_top[threadIdx.x] : 0u);
+    if (threadIdx.x == 0 && all) atomicMax(top, all);
+  }
+}
+
 // dz = dy * act'(z), rows `ld` apart, and the column sums of dz: a block takes 32 V columns (V to a
 // thread) of a strip of rows, eight rows at a time, and writes one row of `partial` for its strip.
 // dz and partial may be null. A pass over 8 bytes of bf16 and fp32 an element (12,001 x 1024: 18 us,
@@ -427,7 +468,8 @@ int pad_rows(const Pad* pads, int count, int es, cudaStream_t s) {
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256, 6)
     dz_kernel(const T* __restrict__ dy, const float* __restrict__ z, int64_t m, int64_t n,
-              int64_t rows_per_strip, T* __restrict__ dz, int64_t ld, float* __restrict__ partial) {
+              int64_t rows_per_strip, T* __restrict__ dz, int64_t ld, float* __restrict__ partial,
+              Raise raise) {
   __shared__ float s_sum[8][32 * V + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * V;
@@ -436,6 +478,14 @@ __global__ void __launch_bounds__(256, 6)
   float sum[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) sum[e] = 0.f;
+  float up = 1.0f;
+  if constexpr (std::is_same<T, __half>::value) {
+    if (raise.top != nullptr) {
+      up = raise_of(__ldg(raise.top));
+      if (blockIdx.x == 0 && blockIdx.y == 0)
+        for (int64_t i = threadIdx.x; i < raise.k; i += 256) raise.down[i] = 1.0f / up;
+    }
+  }
   if (c < n) {
 #pragma unroll 2
     for (int64_t r = r0 + warp; r < r1; r += 8) {
@@ -463,7 +513,7 @@ __global__ void __launch_bounds__(256, 6)
           const float v = to_float(d[e]) * (sizeof(T) == 2 ? activate_slope_half(zz[e], ACT)
                                                            : activate_slope(zz[e], ACT));
           sum[e] += v;
-          d[e] = from_f32<T>(v);
+          d[e] = from_f32<T>(v * up);
         }
       }
       if (dz) {
@@ -520,7 +570,7 @@ int strips_for(int64_t m, int64_t n, int v) {
 
 template <typename T, int V>
 int launch_dz(const T* dy, const float* z, int64_t m, int64_t n, int act, T* dz, int64_t ld, T* db,
-              float* partial, cudaStream_t s) {
+              float* partial, const Raise& raise, cudaStream_t s) {
   const int strips = strips_for(m, n, V);
   const int64_t per = (m + strips - 1) / strips;
   const dim3 grid((unsigned)((n + 32 * V - 1) / (32 * V)), (unsigned)strips);
@@ -528,7 +578,7 @@ int launch_dz(const T* dy, const float* z, int64_t m, int64_t n, int act, T* dz,
                 : act == SV_ACT_GELU      ? dz_kernel<T, V, SV_ACT_GELU>
                 : act == SV_ACT_GELU_TANH ? dz_kernel<T, V, SV_ACT_GELU_TANH>
                                           : dz_kernel<T, V, SV_ACT_NONE>;
-  kernel<<<grid, 256, 0, s>>>(dy, z, m, n, per, dz, ld, db ? partial : nullptr);
+  kernel<<<grid, 256, 0, s>>>(dy, z, m, n, per, dz, ld, db ? partial : nullptr, raise);
   SV_LAUNCH_CHECK();
   if (db) {
     dbias_kernel<T><<<(unsigned)((n + 31) / 32), 256, 0, s>>>(partial, strips, n, db);
@@ -539,12 +589,23 @@ int launch_dz(const T* dy, const float* z, int64_t m, int64_t n, int act, T* dz,
 
 template <typename T>
 int dz_typed(const void* dy, const float* z, int64_t m, int64_t n, int act, void* dz, int64_t ld,
-             void* db, float* partial, cudaStream_t s) {
+             void* db, float* partial, const Raise& raise, cudaStream_t s) {
+  if (raise.top) {
+    SV_CUDA_TRY(cudaMemsetAsync(raise.top, 0, sizeof(unsigned), s));
+    const unsigned short* x = static_cast<const unsigned short*>(dy);
+    const int64_t cells = m * n;
+    const bool wide = cells % 8 == 0 && aligned16(dy);
+    const unsigned blocks = (unsigned)std::min<int64_t>(
+        (cells / (wide ? 8 : 1) + 255) / 256, (int64_t)num_sms() * 8);
+    if (wide) top_kernel<8><<<blocks, 256, 0, s>>>(x, cells, raise.top);
+    else top_kernel<1><<<blocks, 256, 0, s>>>(x, cells, raise.top);
+    SV_LAUNCH_CHECK();
+  }
   const bool vec = n % 4 == 0 && aligned16(dy) && aligned16(z) && aligned16(dz);
   const T* g = static_cast<const T*>(dy);
   T *d = static_cast<T*>(dz), *b = static_cast<T*>(db);
-  return vec ? launch_dz<T, 4>(g, z, m, n, act, d, ld, b, partial, s)
-             : launch_dz<T, 1>(g, z, m, n, act, d, ld, b, partial, s);
+  return vec ? launch_dz<T, 4>(g, z, m, n, act, d, ld, b, partial, raise, s)
+             : launch_dz<T, 1>(g, z, m, n, act, d, ld, b, partial, raise, s);
 }
 
 // ---- the plan of one product -------------------------------------------------------------------
@@ -692,10 +753,10 @@ int run_gemm(Gemm g, void* workspace, size_t workspace_bytes, int32_t* status, c
   return finish(g, partial, p.splits, s);
 }
 
-// The backward pass's workspace: dz in rows of a multiple of 16 bytes, where it is not dout itself;
-// the bias's partial sums; and what the larger of the two products needs.
+// The backward pass's workspace: dz in rows of a multiple of 16 bytes, where it is not dout itself; the
+// bias's partial sums; what raises fp16's dz; and what the larger of the two products needs.
 struct BackLayout {
-  size_t bias, scratch, total;  // dz is at the start
+  size_t bias, raise, scratch, total;  // dz is at the start
   int64_t ld;
 };
 BackLayout back_layout(int64_t m, int64_t k, int64_t n, int dtype, bool copy_x, bool copy_w,
@@ -704,7 +765,9 @@ BackLayout back_layout(int64_t m, int64_t k, int64_t n, int dtype, bool copy_x, 
   const size_t row = align_up((size_t)n * elem_size(dtype), 16);
   l.ld = hold ? (int64_t)(row / elem_size(dtype)) : n;
   l.bias = hold ? align_up(m * row, COPY_ALIGN) : 0;
-  l.scratch = l.bias + align_up((size_t)MAX_STRIPS * n * sizeof(float), COPY_ALIGN);
+  l.raise = l.bias + align_up((size_t)MAX_STRIPS * n * sizeof(float), COPY_ALIGN);
+  l.scratch = l.raise;
+  if (hold && dtype == SV_FLOAT16) l.scratch += COPY_ALIGN + align_up(k * sizeof(float), COPY_ALIGN);
   l.total = l.scratch +
             std::max(plan_bytes(plan_gemm(m, k, n, dtype, false, true), m, k, n, dtype, false, true,
                                 false, copy_w),
@@ -793,28 +856,33 @@ extern "C" int sv_linear_backward(const void* dout, const float* preact, const v
     SV_FAIL(SV_ERR_WORKSPACE, "sv_linear_backward: workspace too small or unaligned");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const void* dz = hold ? ws : dout;
+  Raise raise{};
   if (!terms) {
     if (dbias) SV_CUDA_TRY(cudaMemsetAsync(dbias, 0, n * elem_size(dtype), s));
   } else if (dbias || (hold && (dx || dw))) {
     void* to = hold && (dx || dw) ? ws : nullptr;
     float* partial = reinterpret_cast<float*>(ws + l.bias);
+    if (to && act && dtype == SV_FLOAT16)
+      raise = {reinterpret_cast<unsigned*>(ws + l.raise),
+               reinterpret_cast<float*>(ws + l.raise + COPY_ALIGN), k};
     const int bad =
         dtype == SV_FLOAT32
-            ? dz_typed<float>(dout, preact, m, n, activation, to, l.ld, dbias, partial, s)
+            ? dz_typed<float>(dout, preact, m, n, activation, to, l.ld, dbias, partial, raise, s)
         : dtype == SV_FLOAT16
-            ? dz_typed<__half>(dout, preact, m, n, activation, to, l.ld, dbias, partial, s)
-            : dz_typed<__nv_bfloat16>(dout, preact, m, n, activation, to, l.ld, dbias, partial, s);
+            ? dz_typed<__half>(dout, preact, m, n, activation, to, l.ld, dbias, partial, raise, s)
+            : dz_typed<__nv_bfloat16>(dout, preact, m, n, activation, to, l.ld, dbias, partial, raise,
+                                      s);
     if (bad != SV_OK) return bad;
   }
   const size_t left = workspace_bytes - l.scratch;
   if (dx) {
     const Gemm g{{dz, l.ld, false}, wo, m, k, n, dtype, 1,
-                 {nullptr, nullptr, 0, nullptr, nullptr, dx, nullptr, nullptr, dtype, SV_ACT_NONE}};
+                 {nullptr, nullptr, 0, nullptr, raise.down, dx, nullptr, nullptr, dtype, SV_ACT_NONE}};
     const int bad = run_gemm(g, ws + l.scratch, left, status, s, "sv_linear_backward (dx)");
     if (bad != SV_OK) return bad;
   }
   if (!dw) return SV_OK;
   const Gemm g{{dz, l.ld, true}, xo, n, k, m, dtype, 1,
-               {nullptr, nullptr, 0, nullptr, nullptr, dw, nullptr, nullptr, dtype, SV_ACT_NONE}};
+               {nullptr, nullptr, 0, nullptr, raise.down, dw, nullptr, nullptr, dtype, SV_ACT_NONE}};
   return run_gemm(g, ws + l.scratch, left, status, s, "sv_linear_backward (dw)");
 }

@@ -5,7 +5,13 @@ Bounds, with u = 2^-24: exp, erfc, the divisions and the products around them ar
 together. The argument's own rounding is multiplied by the function: at most 8 u of t = 2 sqrt(2 / pi)
 (z + 0.044715 z^3) by |t| for the tanh form, 2 u of z by z^2 for the normal integral. A factor below 2^-126 (the
 logistic function, its slope, the integral, its density) is off by 2^-149, times what it is multiplied by: z,
-and in the tanh form's slope z dt/dz."""
+and in the tanh form's slope z dt/dz.
+
+Gradients of 16-bit types: dz is rounded by half a step e of itself, in fp16 after it is raised, so that below
+2^-28 of the largest |dy| it is off by 2^-39 of that at most; its slope by (2 k + 16) u of |x||w| + |b| through
+z (the slopes' own slopes are below 1.2) and 32 u (1 + |z|) by the approximate exponential; a sum of t
+products by 2 t u. The two roundings of dx and dw, dz's and the result's, are independent and of half a step each:
+2^0.5 of the result's alone as a whole, and 2 with room for the rest."""
 
 from __future__ import annotations
 
@@ -80,3 +86,61 @@ def test_largest_arguments(act, dtype):
         assert torch.equal(y[:, 0][up], z[:n][up]) and not y[:, 0][~up].any()
         assert (dx[:n, 0][up] == 1).all() and not dx[:n, 0][~up].any()
     N.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-6])
+@pytest.mark.parametrize("shape", [(2048, 128, 192), (2047, 72, 331), (300, 40, 24)], ids=str)
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_small_output_gradients(shape, act, size, dtype):
+    """A mean loss's output gradients, down to fp16's smallest numbers."""
+    m, k, n = shape
+    gen = torch.Generator(device=DEV).manual_seed(m + k)
+
+    def rand(*s, scale=1.0):
+        return (torch.randn(s, device=DEV, generator=gen) * scale).to(dtype)
+
+    x, w, b, dy = rand(m, k), rand(n, k, scale=k**-0.5), rand(n), rand(m, n, scale=size)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    grads = torch.autograd.grad(linear(x, w, b, activation=act), leaves, dy)
+    N.check_device_status(DEV)
+    e = torch.finfo(dtype).eps / 2
+    least = torch.finfo(dtype).smallest_normal * e
+    with torch.no_grad():
+        x64, w64, b64, g = (t.to(F64) for t in (x, w, b, dy))
+        z = x64 @ w64.T + b64
+        dz = g * _parts(z, act)[1]
+        small = 2.0**-39 * float(g.abs().max()) if dtype == torch.float16 else 2.0**-126
+        off = e * dz.abs() + small + (1 + e) * g.abs() * (
+            1.2 * (2 * k + 16) * U * (x64.abs() @ w64.abs().T + b64.abs())
+            + 32 * U * (1 + z.abs()))
+        for name, got, want, o, mag, terms in (
+            ("dx", grads[0], dz @ w64, off @ w64.abs(), dz.abs() @ w64.abs(), n),
+            ("dw", grads[1], dz.T @ x64, off.T @ x64.abs(), dz.abs().T @ x64.abs(), m),
+            ("db", grads[2], dz.sum(0), off.sum(0), dz.abs().sum(0), m),
+        ):
+            total = o + (2 * terms + 16) * U * (mag + o)
+            bound = total + e * (want.abs() + total) + least
+            err = (got.to(F64) - want).abs()
+            assert (err <= bound).all(), (name, float((err / bound).max()))
+            alone = (want.to(dtype).to(F64) - want).norm()
+            assert err.norm() <= 2 * alone, (name, float(err.norm() / alone))
+
+
+@pytest.mark.parametrize("shape", [(300, 40, 24), (64, 8, 7)], ids=str)
+def test_output_gradients_that_are_zero_large_or_not_finite(shape):
+    m, k, n = shape
+    x = torch.ones((m, k), device=DEV, dtype=torch.float16, requires_grad=True)
+    w = torch.full((n, k), 1 / k, device=DEV, dtype=torch.float16, requires_grad=True)
+    y = linear(x, w, activation="gelu_tanh")
+    dx, dw = torch.autograd.grad(y, (x, w), torch.zeros_like(y), retain_graph=True)
+    assert not dx.any() and not dw.any()
+    dy = torch.zeros_like(y)
+    dy[3, 2] = 60000.0  # slope 1.083: more than the type holds, though not its products with w
+    dx, = torch.autograd.grad(y, x, dy, retain_graph=True)
+    want = 60000 * float(_parts(torch.ones(1, dtype=F64), "gelu_tanh")[1]) * float(w[2, 0].detach())
+    assert (dx[3].to(F64) - want).abs().max() <= 2.0**-9 * want and not dx[:3].any()
+    dy[3, 2] = float("inf")
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert torch.isinf(dx[3]).all() and not dx[4:].any() and not dx[:3].any()
+    assert torch.isinf(dw[2]).all() and not dw[3:].any() and not dw[:2].any()
