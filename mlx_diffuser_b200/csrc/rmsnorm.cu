@@ -757,8 +757,8 @@ extern "C" int sv_rms_norm(const void* x, int64_t x_stride, const void* residual
   const bool q8 = out_dtype == SV_FLOAT8_E4M3;
   if (!q8 && out_dtype != dtype)
     SV_FAIL(SV_ERR_BAD_DTYPE, "sv_rms_norm: the output has the input's type or is e4m3");
-  if (n == 0 || channels == 0) return SV_OK;
-  if (!x || !out || (q8 && !scale))
+  if (n == 0 || (channels == 0 && !q8)) return SV_OK;  // rows of nothing still have scales
+  if ((channels > 0 && (!x || !out)) || (q8 && !scale))
     SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_rms_norm: null pointer");
   if (x_stride < channels || (residual && residual_stride < channels))
     SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_rms_norm: row stride below the channel count");

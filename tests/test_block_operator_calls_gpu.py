@@ -167,3 +167,17 @@ def test_captured_call_and_changed_coordinates():
     torch.cuda.synchronize()
     assert torch.equal(inside, want)
     assert len(junk) == 64 and len(x.cache["attention_groups_captured"]) == 1
+
+
+def test_eight_bit_rows_without_channels_have_scales():
+    """A row of nothing is a row of zeros: its scale is 1, not what was in memory before."""
+    for shape in ((5, 0), (3, 4, 0), (4096, 0)):
+        x = torch.zeros(shape, dtype=torch.bfloat16, device=DEV)
+        dirt = [torch.full(shape[:-1], float("nan"), device=DEV) for _ in range(4)]
+        del dirt
+        for r in (None, x):
+            out = rms_norm(x, residual=r, quantize=True)
+            q, s = out if r is None else out[0]
+            assert q.shape == shape and s.shape == shape[:-1]
+            assert torch.equal(s, torch.ones(shape[:-1], device=DEV))
+    N.check_device_status(DEV)
