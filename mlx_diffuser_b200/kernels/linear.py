@@ -86,11 +86,12 @@ class _Linear(torch.autograd.Function):
             lib = N.load()
             with N.on_device(dev):
                 nbytes = lib.sv_linear_workspace_bytes(N.SV_LINEAR_BACKWARD, m, k, n, code, copies)
+                # held over the call: another thread's launches on this stream could take it meanwhile
+                ws = N.workspace(nbytes, dev)
                 rc = lib.sv_linear_backward(
                     pd, N.ptr(preact), px, ldx, pw, ldw, m, k, n, code,
                     N.ACTIVATION_CODE[ctx.activation], N.ptr(dx), N.ptr(dw), N.ptr(db),
-                    N.workspace(nbytes, dev).data_ptr(), nbytes, N.status_word(dev).data_ptr(),
-                    N.stream(dev))
+                    ws.data_ptr(), nbytes, N.status_word(dev).data_ptr(), N.stream(dev))
             N.check(rc, "linear (backward)")
         return dx, dw, db, dout if need_r else None, None
 

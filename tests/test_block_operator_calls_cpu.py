@@ -1,11 +1,15 @@
-"""Calls that ``rms_norm``, ``linear`` and the biased attention refuse before anything runs: no GPU."""
+"""Calls that ``rms_norm``, ``linear`` and the biased attention refuse before anything runs, and what their
+bindings hold on to: no GPU."""
 
 from __future__ import annotations
+
+import weakref
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from mlx_diffuser_b200 import _native as N
 from mlx_diffuser_b200 import (
     SparseTensor,
     linear,
@@ -44,3 +48,54 @@ def test_forward_mode_derivatives_are_refused():
         a = forward_ad.make_dual(norm[0], torch.ones_like(norm[0]))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             rms_norm(a, quantize=True)
+
+
+class _Library:
+    """In the library's place: sizes are 4096, and every other call finds its workspaces alive."""
+
+    def __init__(self):
+        self.held = []
+        self.calls = []
+
+    def __getattr__(self, name):
+        if not name.startswith("sv_"):
+            raise AttributeError(name)
+        if name.endswith("_bytes"):
+            return lambda *a: 4096
+
+        def call(*args):
+            self.calls.append(name)
+            assert all(r() is not None for r in self.held), f"{name}: a workspace is gone"
+            self.held.clear()
+            return N.SV_OK
+
+        return call
+
+
+def test_workspaces_live_until_their_call_returns(monkeypatch):
+    """The library is called without the interpreter's lock: memory that is dropped before the call goes to
+    whatever another thread launches on the same stream in the meantime."""
+    lib = _Library()
+
+    def workspace(nbytes, device):
+        t = torch.empty(nbytes, dtype=torch.uint8)
+        lib.held.append(weakref.ref(t))
+        return t
+
+    monkeypatch.setattr(N, "load", lambda: lib)
+    monkeypatch.setattr(N, "workspace", workspace)
+    monkeypatch.setattr(N, "require_cuda", lambda *a: None)
+    monkeypatch.setattr(N, "status_word", lambda device: torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(N, "stream", lambda device: 0)
+    x, w, b = (torch.zeros(s, requires_grad=True) for s in ((20, 8), (6, 8), (6,)))
+    linear(x, w, b, activation="gelu").sum().backward()
+    rms_norm(x, w[0].detach().requires_grad_(True)).sum().backward()
+    from mlx_diffuser_b200.kernels.attention import biased_window_attention
+
+    q, k, v = (torch.zeros((5, 2, 8), requires_grad=True) for _ in range(3))
+    table = torch.zeros((2, 3, 3, 3), requires_grad=True)
+    plan = torch.zeros(4096, dtype=torch.uint8)
+    biased_window_attention(q, k, v, table, position_buckets(1, 1), plan, 1, 0.5).sum().backward()
+    assert lib.calls == ["sv_linear_forward", "sv_linear_backward", "sv_rms_norm",
+                         "sv_rms_norm_backward", "sv_window_attention",
+                         "sv_window_attention_backward"]
