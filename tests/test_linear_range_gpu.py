@@ -144,3 +144,31 @@ def test_output_gradients_that_are_zero_large_or_not_finite(shape):
     dx, dw = torch.autograd.grad(y, (x, w), dy)
     assert torch.isinf(dx[3]).all() and not dx[4:].any() and not dx[:3].any()
     assert torch.isinf(dw[2]).all() and not dw[3:].any() and not dw[:2].any()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gradients_are_taken_at_the_unrounded_argument(act, dtype):
+    """Around the slope's zero an argument rounded to the type would show: half a step of z, times a second
+    derivative near one, where dz and its own rounding all but vanish."""
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    root = {"silu": -1.2784645, "gelu": -0.7517916, "gelu_tanh": -0.7524614}[act]
+    x = (root + 0.02 * torch.randn((4096, 1), device=DEV, generator=gen)).to(dtype)
+    w = torch.full((1, 1), 1.0234375, dtype=dtype, device=DEV)  # products need twice the type's bits
+    x.requires_grad_(True)
+    y = linear(x, w, activation=act)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    e = torch.finfo(dtype).eps / 2
+    with torch.no_grad():
+        z, w64 = x.to(F64) * w.to(F64), w.to(F64)
+        dz = _parts(z, act)[1]
+        off = e * dz.abs() + (1 + e) * (1.2 * 18 * U * z.abs() + 32 * U * (1 + z.abs()))
+        if dtype == torch.float16:
+            off += 2.0**-39  # the least of what it was raised to
+        want = dz * w64
+        err = (dx.to(F64) - want).abs()
+        bound = off * w64 + e * (want.abs() + off * w64) + 2.0**-25
+        assert (err <= bound).all(), float((err / bound).max())
+        # and this would not pass at the rounded argument
+        rounded = _parts(z.to(dtype).to(F64), act)[1] * w64
+        assert ((rounded - want).abs() > bound).double().mean() > 0.25
