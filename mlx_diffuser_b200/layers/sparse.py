@@ -659,17 +659,18 @@ class WindowGroups:
             captured = cache.setdefault("attention_groups_captured", [])
             if not any(g is self for g in captured):
                 captured.append(self)
-        stream = torch.cuda.current_stream(self.coords.device)
+        dev = self.coords.device
+        stream = N.stream(dev)
         if self.plan is None:
             rows = window_plan(self.coords.contiguous(), self.perm, self.offsets)
             if capturing:
                 return rows  # written by the graph's replays alone: not for others
             # like the grouping, whole for whatever stream uses it next
-            stream.synchronize()
-            self.plan, self.stream = rows, stream.cuda_stream
-        elif not capturing and stream.cuda_stream != self.stream:
+            torch.cuda.current_stream(dev).synchronize()
+            self.plan, self.stream = rows, stream
+        elif not capturing and stream != self.stream:
             # its memory is not handed on before this stream's calls have read it
-            self.plan.record_stream(stream)
+            self.plan.record_stream(torch.cuda.current_stream(dev))
         return self.plan
 
     @property
@@ -761,7 +762,9 @@ def sparse_self_attention(
     coordinates minus the query's and ``L`` the int32 ``position_buckets`` ``(2 * reach + 1,)`` at
     the difference clamped to ``-reach..reach`` (:func:`position_buckets` makes one). Scores, bias,
     softmax and sums then run in one kernel over all windows, with gradients for ``q``, ``k``, ``v``
-    and the table that do not depend on the order of execution. head_dim up to 128, B up to 25,
+    and the table that do not depend on the order of execution (the table's terms are summed as whole
+    multiples of 2^-16, or less, of their bucket's largest; in fp32 of 2^-61 of a bound for the whole
+    sum). head_dim up to 128, B up to 25,
     reach up to 1023. A row whose every score is -inf gives zeros. A call captured into a CUDA graph
     reads the windows that ``x``'s cache holds then: keep ``x`` as long as the graph, and capture
     again after its coordinates have changed."""
