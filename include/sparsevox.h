@@ -372,7 +372,8 @@ SV_API int sv_rownorm(const void* x, int64_t n, int channels, int dtype, float e
  *   h: receives the sum, [n, channels] in `dtype`, or null. rstd: fp32 [n] or null.
  *   out: [n, channels] in `out_dtype`, which is `dtype`, or SV_FLOAT8_E4M3: then
  *     scale[r] = max|y| / 448 (1 for a row of zeros) and out = e4m3(y / scale), y = out * scale.
- * A row that holds a NaN or an infinity gives NaNs, its scale among them. */
+ * A row that holds a NaN gives NaNs. One that holds an infinity has an rstd of zero: NaN at the infinity,
+ * zeros elsewhere. In 8 bits either is NaN throughout, its scale too. */
 SV_API int sv_rms_norm(const void* x, int64_t x_stride, const void* residual,
                        int64_t residual_stride, int64_t n, int channels, int dtype, float eps,
                        const float* weight, void* h, float* rstd, void* out, int out_dtype,
@@ -458,14 +459,17 @@ SV_API int sv_window_attention(const void* q, const void* k, const void* v,
                                size_t workspace_bytes, sv_stream_t stream);
 
 /* Its gradients, from the forward pass's out (`o`) and stats: dq, dk, dv contiguous, and dtable
- * [heads, buckets^3] (null: not wanted), whose sums do not depend on the order of execution.
+ * [heads, buckets^3] (null: not wanted), whose sums do not depend on the order of execution: fp32 terms
+ * are rounded to 2^-61 of twice n times the head's largest |dout| |v|, those of fp16 and bf16 to 2^-16
+ * (or finer) of their own bucket's largest.
  * o_rest: the forward pass's out_rest (null: taken as zeros, at half a step of `o` in dS). */
 SV_API size_t sv_window_attention_backward_workspace_bytes(int64_t n, int heads, int buckets);
 SV_API int sv_window_attention_backward(
     const void* q, const void* k, const void* v, const int64_t* strides, const void* o,
     const void* o_rest, const void* dout, const float* stats, int64_t n, int heads, int dim,
     int dtype, const void* plan, const void* table, int buckets, const int32_t* lut, int reach,
-    float scale, void* dq, void* dk, void* dv, void* dtable, void* workspace, size_t workspace_bytes, sv_stream_t stream);
+    float scale, void* dq, void* dk, void* dv, void* dtable, void* workspace,
+    size_t workspace_bytes, sv_stream_t stream);
 
 /* ---- topology: occupancy -> coordinates, subdivision, attention windows --------------- */
 

@@ -421,8 +421,9 @@ int pad_rows(const Pad* pads, int count, int es, cudaStream_t s) {
   return SV_OK;
 }
 
-// fp16's dz is raised by a power of two before it is rounded, and the products' column scales take it
-// back: below 2^-14 a half has no 11 bits, and the gradients of a mean loss lie there. The power puts the
+// dz is rounded to the feature type, since the tensor cores take it as an operand of both products: half
+// a step more beside the result's own (0.0023 against 0.0017 over the gradients of 12,001 x 1024 x 1024
+// bf16). fp16's is raised by a power of two first, and the products' column scales take that back: below 2^-14 a half has no 11 bits, and the gradients of a mean loss lie there. The power puts the
 // largest |dy| below 2^15 (the activations' slopes are below 1.13), so values down to 2^-28 of it keep
 // all their bits. It costs a pass over dy: 12,001 x 1024 in 7 us.
 struct Raise {

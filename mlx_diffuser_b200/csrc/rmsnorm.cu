@@ -637,6 +637,10 @@ constexpr int BACKWARD_BLOCKS = 888;  // at most six per SM; also the rows of th
 
 // Whether rows go through the warps' pipelines: rows of 33 to 128 16-byte accesses, and enough of them
 // that every warp gets four (below that the direct kernels start sooner: 8 x 1024 bf16 2.1 against 3 us).
+// Wider rows do not fit a warp's registers beside the weight and dw, and keep the direct kernels. 20,331
+// rows, launch included, with residual / backward: 1024 channels of bf16 33 / 33 us (the direct kernel's
+// backward pass took 72 at that width), 1280 57 / 88, 2048 72 / 102, 4096 127 / 211, 8192 322 / 272 us;
+// 512 of fp32 33 / 29, 1024 57 / 51, 2048 107 / 121, 4096 201 / 172 us.
 constexpr int ROW_BLOCKS_PER_SM = 2;
 bool pipelined(int64_t n, int nv) {
   return nv > 32 && nv <= 128 && n >= (int64_t)4 * ROW_WARPS * ROW_BLOCKS_PER_SM * num_sms();

@@ -173,7 +173,7 @@ def rms_norm(
 
     ``h`` is rounded to ``x.dtype`` before it is normed: it is the residual stream that goes on to
     the next block, returned beside the result. ``weight``: (C,), any float type, used in fp32.
-    ``residual``: like ``x``.
+    ``residual``: like ``x``. At most 8192 channels.
 
     Returns ``y`` in ``x.dtype``, or ``(y, h)`` with a residual. With ``quantize``, ``y`` is a pair
     ``(q, scale)``: ``q`` in ``torch.float8_e4m3fn`` and one fp32 scale per row (``x.shape[:-1]``),
