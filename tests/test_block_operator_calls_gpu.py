@@ -181,3 +181,70 @@ def test_eight_bit_rows_without_channels_have_scales():
             assert q.shape == shape and s.shape == shape[:-1]
             assert torch.equal(s, torch.ones(shape[:-1], device=DEV))
     N.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_training_step_with_small_gradients_in_a_graph(dtype):
+    """Norm, projection and attention, forward and backward, captured and replayed on other inputs whose
+    gradients are 2^-10 of the captured ones: what fp16's gradients are raised by is found at replay."""
+    coords = _voxels(900, 12, 9)
+    x = _tensor(coords)
+    lut = position_buckets(4, 4, device=DEV)
+    shapes = [(900, 64), (64,), (192, 64), (192,), (2, 9, 9, 9)]
+
+    def inputs(seed):
+        return [_rand(s, dtype, seed + i, 0.3) for i, s in enumerate(shapes)]
+
+    def step(args, dout):
+        f, g, w, b, table = args
+        q, k, v = linear(rms_norm(f, g), w, b, activation="gelu").view(900, 3, 2, 32).unbind(1)
+        out = sparse_self_attention(x, q, k, v, window_size=5, position_bias=table,
+                                    position_buckets=lut)
+        return [out.detach(), *torch.autograd.grad(out, args, dout)]
+
+    douts = {100: _rand((900, 2, 32), dtype, 98), 200: _rand((900, 2, 32), dtype, 99, 2.0**-10)}
+    want = {}
+    for seed, dout in douts.items():
+        want[seed] = step([t.requires_grad_(True) for t in inputs(seed)], dout)
+    static, sdout = [t.requires_grad_(True) for t in inputs(100)], douts[100].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static, sdout)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(static, sdout)
+    for seed in (200, 100, 200):
+        with torch.no_grad():
+            for t, new in zip(static, inputs(seed)):
+                t.copy_(new)
+            sdout.copy_(douts[seed])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[seed]))
+    N.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(300, 40, 24), (300, 41, 23), (5, 64, 24)], ids=str)
+def test_some_of_the_projections_gradients(shape, dtype):
+    """Any subset of the gradients is what all of them together are, with an activation and without,
+    and through an output gradient off a 16-byte boundary."""
+    m, k, n = shape
+    x, w, b = _rand((m, k), dtype, 1), _rand((n, k), dtype, 2, 0.2), _rand((n,), dtype, 3)
+    r = _rand((m, n), dtype, 4)
+    odd = _rand((m * n + 1,), dtype, 5, 1e-3)[1:].view(m, n)
+    for act in (None, "silu"):
+        for dy in (odd, odd.clone()):
+            want = None
+            for wanted in range(15, 0, -1):
+                leaves = [t.clone().requires_grad_(bool(wanted >> i & 1))
+                          for i, t in enumerate((x, w, b, r))]
+                y = linear(*leaves[:3], activation=act, residual=leaves[3])
+                some = [t for t in leaves if t.requires_grad]
+                got = iter(torch.autograd.grad(y, some, dy))
+                got = [next(got) if t.requires_grad else None for t in leaves]
+                want = got if want is None else want
+                assert all(a is None or torch.equal(a, c) for a, c in zip(got, want))
+    N.check_device_status(DEV)
