@@ -641,9 +641,9 @@ class WindowGroups:
 
     perm: torch.Tensor
     offsets: torch.Tensor
-    coords: torch.Tensor
-    version: int | None
     buckets: dict[int, torch.Tensor] | None = None
+    coords: torch.Tensor | None = None
+    version: int | None = None
     plan: torch.Tensor | None = None
     stream: int | None = None
 
@@ -728,7 +728,8 @@ def attention_windows(
         ws.data_ptr(), ws_bytes, N.stream(dev),
     )
     N.check(rc, "attention groups")
-    result = WindowGroups(perm, offsets[: int(groups.value) + 1], x.coords, _version(x.coords))
+    result = WindowGroups(perm, offsets[: int(groups.value) + 1], coords=x.coords,
+                          version=_version(x.coords))
     x.cache[key] = result
     return result
 
