@@ -21,8 +21,9 @@
 // a fifth fixed latencies). bf16, 64 channels:
 //   forward   40,662 x 12 heads, windows of 8^3 (95 M pairs): 239 us; 20,331 x 16 (63 M): 225 us with
 //             what training adds, 41 MB of rests and a second product
-//   backward  20,331 x 16: delta 26 us, dk and dv with each bucket's largest term 371 us (296 where no
-//             table gradient is wanted), dq and the table's gradient 328 us
+//   backward  20,331 x 16: delta 26 us, dk and dv with each bucket's largest term 371 us, dq and the
+//             table's gradient 328 us; 282 and 226 where no table gradient is wanted (fp16, whose score
+//             gradients are raised row by row, 306 and 246)
 //   forward   8,192 x 6 x 128 in two windows (201 M pairs), three parts: 495 us and 28 us to join
 // Two row parts a warp in the dk / dv pass halve its fragment loads but leave two blocks an SM: 328 us
 // where one took 268.
@@ -1213,23 +1214,29 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
       float s[1][KB / 8][4], dp[1][KB / 8][4];
       zero(s[0]);
       mma_nt<T, DP, 1>(s, smem_u32(mine), tile);
+      auto form_dp = [&] {
 #pragma unroll
-      for (int n = 0; n < KB / 8; ++n) {
-        const float2 delta = *reinterpret_cast<const float2*>(&sh.key_delta[slot][n * 8 + c2]);
-        dp[0][n][0] = dp[0][n][2] = -delta.x;
-        dp[0][n][1] = dp[0][n][3] = -delta.y;
-      }
-      mma_nt<T, DP, 1>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
-      // a pair out of sight may be with a row that holds anything
+        for (int n = 0; n < KB / 8; ++n) {
+          const float2 delta = *reinterpret_cast<const float2*>(&sh.key_delta[slot][n * 8 + c2]);
+          dp[0][n][0] = dp[0][n][2] = -delta.x;
+          dp[0][n][1] = dp[0][n][3] = -delta.y;
+        }
+        mma_nt<T, DP, 1>(dp, smem_u32(mine + L::OWN_TILE), tile + L::TILE);
+      };
+      // A bucket's largest term wants dP while its word is known; without a table gradient dP comes after
+      // dv's product, which spares its registers there (282 against 291 us).
+      if constexpr (TABLE) form_dp();
       auto grad = [&](int n, int e, uint32_t at, bool in, bool counts) {
         const float2 st = sh.key_stats[slot][n * 8 + c2 + (e & 1)];
         const float w = exp2_fast(fmaf(s[0][n][e], scale, lds_f32(table + at)) - st.x) * st.y;
         s[0][n][e] = in ? w : 0.f;
-        dp[0][n][e] = in ? w * dp[0][n][e] : 0.f;
-        // bits of numbers that are not negative order like the numbers, a NaN's above all
-        if constexpr (TABLE)
+        if constexpr (TABLE) {
+          // a pair out of sight may be with a row that holds anything
+          dp[0][n][e] = in ? w * dp[0][n][e] : 0.f;
+          // bits of numbers that are not negative order like the numbers, a NaN's above all
           asm volatile("red.shared.max.u32 [%0], %1;" ::"r"(tops + at),
                        "r"(counts ? __float_as_uint(dp[0][n][e]) & 0x7fffffffu : 0u));
+        }
       };
       if (whole) {
         each_pair<true, true>(b, slot, own,
@@ -1241,6 +1248,15 @@ __global__ void __launch_bounds__(AT, DP <= 64 ? 3 : 2)
         });
       }
       mma_nn<T, DP, 1>(dv, s, tile + L::TILE);
+      if constexpr (!TABLE) {
+        form_dp();
+#pragma unroll
+        for (int n = 0; n < KB / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            // here a weight of zero stands for a pair out of sight
+            dp[0][n][e] = !whole && s[0][n][e] == 0.f ? 0.f : s[0][n][e] * dp[0][n][e];
+      }
       if constexpr (IS_HALF<T>) raise_rows<DP>(dp[0], by, dk[0]);
       mma_nn<T, DP, 1>(dk, dp, tile);
     };
