@@ -373,7 +373,8 @@ SV_API int sv_rownorm(const void* x, int64_t n, int channels, int dtype, float e
  *   out: [n, channels] in `out_dtype`, which is `dtype`, or SV_FLOAT8_E4M3: then
  *     scale[r] = max|y| / 448 (1 for a row of zeros) and out = e4m3(y / scale), y = out * scale.
  * A row that holds a NaN gives NaNs. One that holds an infinity has an rstd of zero: NaN at the infinity,
- * zeros elsewhere. In 8 bits either is NaN throughout, its scale too. */
+ * zeros elsewhere. In 8 bits either is NaN throughout, its scale too. A row whose sum of squares passes
+ * fp32's range has an rstd of zero as well. */
 SV_API int sv_rms_norm(const void* x, int64_t x_stride, const void* residual,
                        int64_t residual_stride, int64_t n, int channels, int dtype, float eps,
                        const float* weight, void* h, float* rstd, void* out, int out_dtype,
