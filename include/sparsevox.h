@@ -389,6 +389,76 @@ SV_API int sv_rms_norm_backward(const void* h, int64_t h_stride, const void* dy,
                                 const float* rstd, void* dx, float* dw, void* workspace,
                                 size_t workspace_bytes, int32_t* status, sv_stream_t stream);
 
+/* ---- the border between two blocks: gate, residual, norm, modulation --------------------- */
+
+/* Rows of coefficients, one per batch element `stride` elements apart (stride 0: one row for all), in
+ * any of fp32 / fp16 / bf16; data null: none. */
+typedef struct sv_rows {
+  const void* data;
+  int64_t stride;
+  int dtype;
+} sv_rows;
+
+/*   d = drop(branch) (sv_dropout's, element row * channels + channel), u = N(d) * branch_weight where
+ *   branch_norm is set, else d;
+ *   h = round(x + residual_scale * gate[b] * u), y = (N(h) * weight + bias) * (1 + scale[b]) + shift[b].
+ * N: LayerNorm without its weights where `layer` is set, else the root-mean-square norm. x, branch, h, y:
+ * [n, channels] of `dtype`, h and y contiguous; channels <= 8192. weight, bias, branch_weight: one row
+ * (their stride is not read). b = coords[row, 0] (coords [n, 4]) where gate, scale or shift has a
+ * stride; a row whose b is outside [0, batch <= 8191) is left without all three and ORs
+ * SV_DEVICE_BAD_INDEX into `status`. stats: fp32 [n, 4], 16-byte aligned, for the backward pass, or null:
+ * mean and rstd of h, then of d. A row whose sum of squares passes fp32's range has an rstd of zero. */
+typedef struct sv_block_norm_args {
+  int64_t n;
+  int64_t batch;
+  const void* x;
+  int64_t x_stride;
+  const void* branch;
+  int64_t branch_stride;
+  void* h;
+  float* stats;
+  const int32_t* coords;
+  sv_rows weight, bias, branch_weight, gate, scale, shift;
+  double dropout;
+  uint64_t seed;
+  const void* seed_at;
+  uint64_t subsequence;
+  int channels;
+  int dtype;
+  int layer;
+  int branch_norm;
+  float residual_scale;
+  float eps;
+} sv_block_norm_args;
+
+SV_API int sv_block_norm(const sv_block_norm_args* args, void* y, int32_t* status,
+                         sv_stream_t stream);
+
+/* Its gradients, from the forward pass's h and stats and the gradients of y and h (one of them may be
+ * null): dx and dbranch contiguous, and the coefficients' (data null: not wanted), with strides that are
+ * zero where the coefficients' are. Every sum has a fixed order. x is not read. Workspace:
+ * sv_block_norm_backward_workspace_bytes(n, channels, batch), batch 0 where no coefficients have a
+ * stride. */
+typedef struct sv_block_norm_grads {
+  sv_rows weight, bias, branch_weight, gate, scale, shift;
+} sv_block_norm_grads;
+
+SV_API size_t sv_block_norm_backward_workspace_bytes(int64_t n, int channels, int64_t batch);
+SV_API int sv_block_norm_backward(const sv_block_norm_args* args, const void* dy, const void* dh,
+                                  void* dx, void* dbranch, const sv_block_norm_grads* grads,
+                                  void* workspace, size_t workspace_bytes, sv_stream_t stream);
+
+/* ---- dropout with counter-based random numbers ------------------------------------------ */
+
+/* out = x * 2^16 / (2^16 - cut) where the element's random number is at least cut = round(p 2^16), else
+ * zero, plus residual (or null): `cells` elements of `dtype` (fp32 / fp16 / bf16), contiguous; out may be
+ * x or residual. Element i has the 16-bit half i % 8 (low halves first) of Philox4x32-10 at the counter
+ * (i / 8, subsequence), two 32-bit words each, keyed by `seed`, or by the 8-byte aligned word
+ * `seed_at` on the device where that is not null. The gradient of x is the same call on dout. */
+SV_API int sv_dropout(const void* x, const void* residual, int64_t cells, int dtype, double p,
+                      uint64_t seed, const void* seed_at, uint64_t subsequence, void* out,
+                      sv_stream_t stream);
+
 /* ---- linear projection with bias, activation and residual ------------------------------ */
 
 typedef enum sv_activation {

@@ -5,6 +5,8 @@ transformer block over the same rows: ``rms_norm``, ``linear`` and ``sparse_self
 learned relative position bias."""
 
 from ._native import check_device_status
+from .kernels.block_norm import block_norm
+from .kernels.dropout import dropout
 from .kernels.linear import linear
 from .kernels.norm import rms_norm
 from .kernels.sparse import sparse_conv3d
@@ -21,8 +23,10 @@ from .layers.sparse import (
 __all__ = [
     "SparseConv3D",
     "SparseTensor",
+    "block_norm",
     "build_neighbor_map",
     "check_device_status",
+    "dropout",
     "linear",
     "position_buckets",
     "rms_norm",

@@ -49,8 +49,35 @@ SV_LINEAR_FORWARD, SV_LINEAR_BACKWARD = range(2)
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
+_U64 = ctypes.c_uint64
 _I32 = ctypes.c_int
 _SZ = ctypes.c_size_t
+
+
+class Rows(ctypes.Structure):
+    """sv_rows: rows of coefficients in any float type."""
+
+    _fields_ = [("data", _P), ("stride", _I64), ("dtype", _I32)]
+
+
+class BlockNormArgs(ctypes.Structure):
+    """sv_block_norm_args."""
+
+    _fields_ = [
+        ("n", _I64), ("batch", _I64), ("x", _P), ("x_stride", _I64), ("branch", _P),
+        ("branch_stride", _I64), ("h", _P), ("stats", _P), ("coords", _P), ("weight", Rows),
+        ("bias", Rows), ("branch_weight", Rows), ("gate", Rows), ("scale", Rows), ("shift", Rows),
+        ("dropout", ctypes.c_double), ("seed", _U64), ("seed_at", _P), ("subsequence", _U64),
+        ("channels", _I32), ("dtype", _I32), ("layer", _I32), ("branch_norm", _I32),
+        ("residual_scale", ctypes.c_float), ("eps", ctypes.c_float),
+    ]
+
+
+class BlockNormGrads(ctypes.Structure):
+    """sv_block_norm_grads."""
+
+    _fields_ = [(name, Rows) for name in ("weight", "bias", "branch_weight", "gate", "scale", "shift")]
+
 
 _SIGNATURES = {
     "sv_last_error": (ctypes.c_char_p, []),
@@ -107,6 +134,16 @@ _SIGNATURES = {
     "sv_rms_norm_backward_workspace_bytes": (_SZ, [_I32]),
     "sv_rms_norm_backward": (
         _I32, [_P, _I64, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _SZ, _P, _P]
+    ),
+    "sv_block_norm": (_I32, [ctypes.POINTER(BlockNormArgs), _P, _P, _P]),
+    "sv_block_norm_backward_workspace_bytes": (_SZ, [_I64, _I32, _I64]),
+    "sv_block_norm_backward": (
+        _I32,
+        [ctypes.POINTER(BlockNormArgs), _P, _P, _P, _P, ctypes.POINTER(BlockNormGrads), _P, _SZ,
+         _P],
+    ),
+    "sv_dropout": (
+        _I32, [_P, _P, _I64, _I32, ctypes.c_double, _U64, _P, _U64, _P, _P]
     ),
     "sv_linear_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64, _I32, _I32]),
     "sv_linear_forward": (

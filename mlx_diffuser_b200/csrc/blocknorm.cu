@@ -1,0 +1,818 @@
+// The border between two blocks of a transformer, one pass over the rows in each direction.
+//
+//     d = drop(branch),  u = N(d) * wb  (d itself without a norm behind the branch)
+//     h = round(x + alpha * gate[b] * u)
+//     y = (N(h) * w + beta) * (1 + scale[b]) + shift[b]
+//     N(v) = (v - mean) * rstd (layer) or v * rstd (rms), rstd = 1 / sqrt(mean square + eps)
+//
+// h is the residual stream that goes on, rounded to the feature type before it is normed. With n = N(h),
+// a = w (1 + scale) and gg = alpha gate wb, the gradients are
+//     D  = dh + rstd (dy a - mean(dy a) - n mean(dy a n))      the gradient of h, and of x
+//     dd = rstd_d (gg D - mean(gg D) - N(d) mean(gg D N(d))),  dbranch = drop(dd)
+// (without the means of the first order for rms), and three sums over the rows of each batch element,
+//     A = sum dy n,  B = sum dy,  E = sum D N(d),
+// give all the others: dshift = B, dscale = w A + beta B, dgate = alpha wb E, and over the batch elements
+// dw = sum (1 + scale) A, dbeta = sum (1 + scale) B, dwb = sum alpha gate E.
+//
+// The passes move 4 and 6 values an element and do 14 and 30 operations, so HBM bounds them. A row
+// lives in the registers of TPR threads, J accesses of V elements each. The sums have a fixed order:
+// the backward pass walks the rows by batch element (a stable counting sort of their indices), cut into
+// pieces; a block holds the three sums of its piece in registers and writes them out once.
+#include <algorithm>
+
+#include "dropout.cuh"
+#include "group.h"
+
+namespace sv {
+namespace {
+
+constexpr int BN_MAX_CHANNELS = 8192;
+constexpr int BN_PIECES_PER_SM = 4;
+
+// A row or rows of coefficients in any float type; null: the neutral value.
+struct Coef {
+  const void* p;
+  int64_t stride;  // elements between batch elements; 0: one row for all
+  int dtype;
+};
+
+struct BlockArgs {
+  int64_t n;
+  int channels;
+  const void* x;
+  int64_t x_stride;
+  const void* branch;
+  int64_t branch_stride;
+  bool layer, branch_norm;
+  float alpha, eps;
+  Coef weight, bias, branch_weight, gate, scale, shift;
+  bool per_batch;         // otherwise every row is batch element 0
+  const int32_t* coords;  // [n][4]
+  int64_t batch;
+  Dropout drop;
+  void* h;
+  void* y;
+  float4* stats;  // of h and of d: mean, rstd; or null
+  int32_t* status;
+};
+
+struct BackArgs {
+  BlockArgs f;  // h is read; x, y and status are not used
+  const void* dy;
+  const void* dh;
+  void* dx;
+  void* dbranch;
+  const int32_t* perm;     // rows by batch element, or null: as they are
+  const int32_t* offsets;  // [batch + 1], or null: one group
+  int piece;               // rows of a piece
+  float* partial;          // [pieces][3][C], or null: no sums are wanted
+  bool want_e;
+};
+
+template <int V>
+__device__ __forceinline__ void load_coef(const Coef& c, int64_t b, int col, float neutral,
+                                          float (&v)[V]) {
+  if (c.p == nullptr) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = neutral;
+    return;
+  }
+  const int64_t at = b * c.stride + col;
+  if (c.dtype == SV_FLOAT32) {
+    const float* p = static_cast<const float*>(c.p) + at;
+    if constexpr (V == 8) {
+      const float4 lo = __ldg(reinterpret_cast<const float4*>(p));
+      const float4 hi = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+      v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+    } else {
+      v[0] = __ldg(p);
+    }
+    return;
+  }
+  const uint16_t* p = static_cast<const uint16_t*>(c.p) + at;
+  alignas(16) uint16_t e[V];
+  if constexpr (V == 8)
+    *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(p));
+  else
+    e[0] = __ldg(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    v[i] = c.dtype == SV_FLOAT16 ? __half2float(__ushort_as_half(e[i]))
+                                 : __uint_as_float((uint32_t)e[i] << 16);
+}
+
+__device__ __forceinline__ float coef_at(const Coef& c, int64_t b, int col, float neutral) {
+  float v[1];
+  load_coef<1>(c, b, col, neutral, v);
+  return v[0];
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load_row(const T* p, float (&v)[V]) {
+  if constexpr (V == 8) {
+    alignas(16) T e[8];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(e) / 16; ++i)
+      reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+  } else {
+    v[0] = to_f32(*p);
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_row(T* p, const float (&v)[V]) {
+  if constexpr (V == 8) {
+    alignas(16) T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(e) / 16; ++i)
+      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
+  } else {
+    *p = from_f32<T>(v[0]);
+  }
+}
+
+template <int TPR>
+constexpr int kThreads = TPR > 128 ? TPR : 128;
+
+// Sums over the TPR threads of a row, the same in all of them. Rows of more than a warp meet in
+// `part`, two buffers in turn: the next sum but one writes a buffer again only after every thread has
+// passed the barrier in between, so one barrier a sum is enough.
+template <int TPR>
+struct RowSum {
+  float2* part;  // [2][warps of the block]
+  int turn;
+  __device__ __forceinline__ float2 operator()(float a, float b) {
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    if constexpr (TPR > 32) {
+      constexpr int ALL = kThreads<TPR> / 32, W = TPR / 32;
+      float2* to = part + turn * ALL;
+      turn ^= 1;
+      const int warp = threadIdx.x >> 5;
+      if ((threadIdx.x & 31) == 0) to[warp] = make_float2(a, b);
+      __syncthreads();
+      const int first = warp / W * W;
+      a = b = 0.0f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        a += to[first + i].x;
+        b += to[first + i].y;
+      }
+    }
+    return make_float2(a, b);
+  }
+};
+
+// The row's channel of a thread's access j.
+template <int V, int TPR>
+__device__ __forceinline__ int column(int j, int t) {
+  return (j * TPR + t) * V;
+}
+
+template <typename T, int V, int J>
+__device__ __forceinline__ void drop_row(float (&v)[J][V], int64_t row, int channels, int t, int tpr,
+                                         uint64_t seed, const Dropout& d) {
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int c = (j * tpr + t) * V;
+    if (c >= channels) continue;
+    const uint64_t at = (uint64_t)row * channels + c;
+    if constexpr (V == 8)
+      drop_eight(v[j], philox(at >> 3, d.subsequence, seed), d);
+    else
+      v[j][0] = drop_one(v[j][0], at, seed, d);
+  }
+}
+
+// mean and rstd of a row in registers (zeros behind the last channel).
+template <int V, int J, int TPR>
+__device__ __forceinline__ float2 row_stats(const float (&v)[J][V], int t, int channels, bool layer,
+                                            float eps, RowSum<TPR>& sum) {
+  const float inv = 1.0f / (float)channels;
+  float mean = 0.0f;
+  if (layer) {
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += v[j][i];
+    mean = sum(s, 0.0f).x * inv;
+  }
+  float q = 0.0f;
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (column<V, TPR>(j, t) < channels) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) q = fmaf(v[j][i] - mean, v[j][i] - mean, q);
+    }
+  return make_float2(mean, rsqrtf(fmaf(sum(q, 0.0f).x, inv, eps)));
+}
+
+__device__ __forceinline__ int64_t batch_of(const BlockArgs& a, int64_t row) {
+  if (!a.per_batch) return 0;
+  const int64_t b = __ldg(a.coords + row * 4);
+  return b >= 0 && b < a.batch ? b : -1;
+}
+
+template <typename T, int V, int J, int TPR>
+__global__ void __launch_bounds__(kThreads<TPR>)
+    block_norm_kernel(const __grid_constant__ BlockArgs a) {
+  constexpr int ROWS = kThreads<TPR> / TPR;
+  constexpr bool KEEP = J == 1;  // the coefficients of a batch element stay in registers
+  __shared__ float2 part[2 * kThreads<TPR> / 32];
+  RowSum<TPR> sum{part, 0};
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int C = a.channels;
+  const uint64_t seed = a.drop.cut ? seed_of(a.drop) : 0;
+  float gg[J][V], mul[J][V], add[J][V];
+  int64_t held = -2;
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.n; r0 += (int64_t)gridDim.x * ROWS) {
+    const int64_t row = r0 + group;
+    const bool in = row < a.n;
+    float x[J][V], d[J][V];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = column<V, TPR>(j, t);
+      if (in && c < C) {
+        load_row<T, V>(static_cast<const T*>(a.x) + row * a.x_stride + c, x[j]);
+        load_row<T, V>(static_cast<const T*>(a.branch) + row * a.branch_stride + c, d[j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[j][i] = d[j][i] = 0.0f;
+      }
+    }
+    const int64_t b = in ? batch_of(a, row) : held;
+    if (b == -1 && in && t == 0) report(a.status, SV_DEVICE_BAD_INDEX);
+    // a row without a batch element is not modulated
+    auto coefs = [&](int j, float (&g)[V], float (&m)[V], float (&s)[V]) {
+      const int c = column<V, TPR>(j, t);
+      if (c >= C) return;
+      float w[V], beta[V], wb[V];
+      load_coef(a.weight, 0, c, 1.0f, w);
+      load_coef(a.bias, 0, c, 0.0f, beta);
+      load_coef(a.branch_weight, 0, c, 1.0f, wb);
+      if (b >= 0) {
+        load_coef(a.gate, b, c, 1.0f, g);
+        load_coef(a.scale, b, c, 0.0f, m);
+        load_coef(a.shift, b, c, 0.0f, s);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (b < 0) g[i] = 1.0f, m[i] = s[i] = 0.0f;
+        g[i] *= a.alpha * wb[i];
+        s[i] = fmaf(beta[i], 1.0f + m[i], s[i]);
+        m[i] = w[i] * (1.0f + m[i]);
+      }
+    };
+    if (KEEP && b != held) {
+      held = b;
+#pragma unroll
+      for (int j = 0; j < J; ++j) coefs(j, gg[j], mul[j], add[j]);
+    }
+    if (a.drop.cut && in) drop_row<T, V, J>(d, row, C, t, TPR, seed, a.drop);
+    float2 sd = make_float2(0.0f, 1.0f);
+    if (a.branch_norm) sd = row_stats<V, J, TPR>(d, t, C, a.layer, a.eps, sum);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = column<V, TPR>(j, t);
+      if constexpr (!KEEP) coefs(j, gg[0], mul[0], add[0]);
+      if (c < C) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float u = (d[j][i] - sd.x) * sd.y;
+          x[j][i] = to_f32(from_f32<T>(fmaf(gg[KEEP ? j : 0][i], u, x[j][i])));
+        }
+        if (in) store_row<T, V>(static_cast<T*>(a.h) + row * C + c, x[j]);
+      }
+    }
+    const float2 sh = row_stats<V, J, TPR>(x, t, C, a.layer, a.eps, sum);
+    if (a.stats && in && t == 0) a.stats[row] = make_float4(sh.x, sh.y, sd.x, sd.y);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = column<V, TPR>(j, t);
+      if constexpr (!KEEP) coefs(j, gg[0], mul[0], add[0]);
+      if (in && c < C) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          x[j][i] = fmaf((x[j][i] - sh.x) * sh.y, mul[KEEP ? j : 0][i], add[KEEP ? j : 0][i]);
+        store_row<T, V>(static_cast<T*>(a.y) + row * C + c, x[j]);
+      }
+    }
+  }
+}
+
+template <typename T, int V, int J, int TPR>
+__global__ void __launch_bounds__(kThreads<TPR>)
+    block_norm_backward_kernel(const __grid_constant__ BackArgs a) {
+  constexpr int THREADS = kThreads<TPR>, ROWS = THREADS / TPR;
+  constexpr bool KEEP = J == 1;
+  __shared__ float2 part[2 * THREADS / 32];
+  __shared__ float joined[ROWS > 1 ? THREADS * V * J : 1];
+  RowSum<TPR> sum{part, 0};
+  const BlockArgs& f = a.f;
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int C = f.channels;
+  Piece p{0, 0, 0};
+  if (a.offsets) {
+    p = find_piece<true>(a.offsets, (int)f.batch, (int)f.n, a.piece, blockIdx.x);
+  } else {
+    p.first = (int)min((int64_t)blockIdx.x * a.piece, f.n);
+    p.last = (int)min((int64_t)p.first + a.piece, f.n);
+    if (p.first >= p.last) p.group = -1;
+  }
+  if (p.group < 0) return;  // the whole block
+  const int64_t b = p.group < f.batch ? p.group : -1;
+  const uint64_t seed = f.drop.cut ? seed_of(f.drop) : 0;
+  float gg[J][V], mul[J][V];
+  auto coefs = [&](int j, float (&g)[V], float (&m)[V]) {
+    const int c = column<V, TPR>(j, t);
+    if (c >= C) return;
+    float w[V], wb[V];
+    load_coef(f.weight, 0, c, 1.0f, w);
+    load_coef(f.branch_weight, 0, c, 1.0f, wb);
+    if (b >= 0) {
+      load_coef(f.gate, b, c, 1.0f, g);
+      load_coef(f.scale, b, c, 0.0f, m);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (b < 0) g[i] = 1.0f, m[i] = 0.0f;
+      g[i] *= f.alpha * wb[i];
+      m[i] = w[i] * (1.0f + m[i]);
+    }
+  };
+  if constexpr (KEEP) coefs(0, gg[0], mul[0]);
+  float sum_a[J][V], sum_b[J][V], sum_e[J][V];
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum_a[j][i] = sum_b[j][i] = sum_e[j][i] = 0.0f;
+  const float inv = 1.0f / (float)C;
+  const bool with_d = f.branch_norm || a.want_e;
+  for (int r0 = p.first; r0 < p.last; r0 += ROWS) {
+    const bool in = r0 + group < p.last;
+    int64_t row = in ? r0 + group : r0;
+    if (a.perm) row = __ldg(a.perm + row);
+    float4 st = make_float4(0.0f, 0.0f, 0.0f, 1.0f);
+    if (in) st = __ldg(f.stats + row);
+    float dy[J][V], n[J][V], d[J][V], D[J][V];
+    auto get = [&](const void* from, int64_t stride, float (&v)[J][V]) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int c = column<V, TPR>(j, t);
+        if (in && c < C && from) {
+          load_row<T, V>(static_cast<const T*>(from) + row * stride + c, v[j]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[j][i] = 0.0f;
+        }
+      }
+    };
+    get(a.dy, C, dy);
+    get(f.h, C, n);
+    get(with_d ? f.branch : nullptr, f.branch_stride, d);
+    get(a.dh, C, D);
+    if (f.drop.cut && in && with_d) drop_row<T, V, J>(d, row, C, t, TPR, seed, f.drop);
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (column<V, TPR>(j, t) >= C) continue;
+      if constexpr (!KEEP) coefs(j, gg[0], mul[0]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        n[j][i] = (n[j][i] - st.x) * st.y;
+        sum_a[j][i] = fmaf(dy[j][i], in ? n[j][i] : 0.0f, sum_a[j][i]);
+        sum_b[j][i] += dy[j][i];
+        dy[j][i] *= mul[KEEP ? j : 0][i];
+        s1 += dy[j][i];
+        s2 = fmaf(dy[j][i], n[j][i], s2);
+      }
+    }
+    const float2 m = sum(s1, s2);
+    const float m1 = f.layer ? m.x * inv : 0.0f, m2 = m.y * inv;
+    s1 = s2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = column<V, TPR>(j, t);
+      if (c >= C) continue;
+      if constexpr (!KEEP) coefs(j, gg[0], mul[0]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        D[j][i] = fmaf(st.y, dy[j][i] - m1 - n[j][i] * m2, D[j][i]);
+        d[j][i] = (d[j][i] - st.z) * st.w;
+        if (in) sum_e[j][i] = fmaf(D[j][i], d[j][i], sum_e[j][i]);
+      }
+      if (in && a.dx) store_row<T, V>(static_cast<T*>(a.dx) + row * C + c, D[j]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        D[j][i] *= gg[KEEP ? j : 0][i];
+        s1 += D[j][i];
+        s2 = fmaf(D[j][i], d[j][i], s2);
+      }
+    }
+    if (f.branch_norm) {
+      const float2 e = sum(s1, s2);
+      const float e1 = f.layer ? e.x * inv : 0.0f, e2 = e.y * inv;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) D[j][i] = st.w * (D[j][i] - e1 - d[j][i] * e2);
+    }
+    if (in && a.dbranch) {
+      if (f.drop.cut) drop_row<T, V, J>(D, row, C, t, TPR, seed, f.drop);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int c = column<V, TPR>(j, t);
+        if (c < C) store_row<T, V>(static_cast<T*>(a.dbranch) + row * C + c, D[j]);
+      }
+    }
+  }
+  if (a.partial == nullptr) return;
+  float* to = a.partial + (int64_t)blockIdx.x * 3 * C;
+  auto join = [&](const float (&v)[J][V], float* out) {
+    if constexpr (ROWS == 1) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (column<V, TPR>(j, t) < C) out[column<V, TPR>(j, t) + i] = v[j][i];
+    } else {
+      __syncthreads();  // the previous sums have been read
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) joined[group * TPR * V * J + column<V, TPR>(j, t) + i] = v[j][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < C; c += THREADS) {
+        float all = joined[c];
+#pragma unroll
+        for (int g = 1; g < ROWS; ++g) all += joined[g * TPR * V * J + c];
+        out[c] = all;
+      }
+    }
+  };
+  join(sum_a, to);
+  join(sum_b, to + C);
+  join(sum_e, to + 2 * C);
+}
+
+// ---- the coefficients' gradients from the pieces' sums -------------------------------------------
+
+struct Grad {
+  void* p;
+  int64_t stride;  // between batch elements; 0: summed over them
+  int dtype;
+};
+struct SumArgs {
+  BlockArgs f;
+  const int32_t* offsets;
+  int piece;
+  const float* partial;
+  Grad weight, bias, branch_weight, gate, scale, shift;
+};
+
+__device__ __forceinline__ void store_grad(const Grad& g, int64_t b, int c, float v) {
+  const int64_t at = b * g.stride + c;
+  if (g.dtype == SV_FLOAT32) static_cast<float*>(g.p)[at] = v;
+  else if (g.dtype == SV_FLOAT16) static_cast<__half*>(g.p)[at] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(g.p)[at] = __float2bfloat16_rn(v);
+}
+
+// 32 channels a block; its 32 warps share a batch element's pieces and are joined in order.
+__global__ void __launch_bounds__(1024)
+    block_norm_sums_kernel(const __grid_constant__ SumArgs a) {
+  __shared__ float s[3][32][33];
+  const BlockArgs& f = a.f;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane, C = f.channels;
+  const bool in = c < C;
+  float dw = 0.0f, dbeta = 0.0f, dwb = 0.0f, dgate = 0.0f, dscale = 0.0f, dshift = 0.0f;
+  const float w = in ? coef_at(f.weight, 0, c, 1.0f) : 0.0f;
+  const float beta = in ? coef_at(f.bias, 0, c, 0.0f) : 0.0f;
+  const float wb = in ? coef_at(f.branch_weight, 0, c, 1.0f) : 0.0f;
+  int64_t first = 0;
+  const int groups = a.offsets ? (int)f.batch + 1 : 1;
+  for (int g = 0; g < groups; ++g) {
+    int64_t rows = f.n;
+    if (a.offsets)
+      rows = (g < f.batch ? (int64_t)a.offsets[g + 1] : f.n) - a.offsets[g];
+    const int64_t pieces = (rows + a.piece - 1) / a.piece;
+    float v0 = 0.0f, v1 = 0.0f, v2 = 0.0f;
+    if (in)
+      for (int64_t p = first + warp; p < first + pieces; p += 32) {
+        const float* from = a.partial + p * 3 * C + c;
+        v0 += __ldg(from);
+        v1 += __ldg(from + C);
+        v2 += __ldg(from + 2 * C);
+      }
+    first += pieces;
+    __syncthreads();  // the previous element's sums have been read
+    s[0][warp][lane] = v0;
+    s[1][warp][lane] = v1;
+    s[2][warp][lane] = v2;
+    __syncthreads();
+    if (warp != 0 || !in) continue;
+    float A = 0.0f, B = 0.0f, E = 0.0f;
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i) {
+      A += s[0][i][lane];
+      B += s[1][i][lane];
+      E += s[2][i][lane];
+    }
+    const bool mod = !a.offsets || g < f.batch;  // rows without a batch element are not modulated
+    const float one = 1.0f + (mod ? coef_at(f.scale, g, c, 0.0f) : 0.0f);
+    const float gate = mod ? coef_at(f.gate, g, c, 1.0f) : 1.0f;
+    dw = fmaf(one, A, dw);
+    dbeta = fmaf(one, B, dbeta);
+    dwb = fmaf(f.alpha * gate, E, dwb);
+    if (!mod) continue;
+    const float eg = f.alpha * wb * E, es = fmaf(w, A, beta * B);
+    if (a.gate.p && a.gate.stride) store_grad(a.gate, g, c, eg);
+    if (a.scale.p && a.scale.stride) store_grad(a.scale, g, c, es);
+    if (a.shift.p && a.shift.stride) store_grad(a.shift, g, c, B);
+    dgate += eg;
+    dscale += es;
+    dshift += B;
+  }
+  if (warp != 0 || !in) return;
+  if (a.weight.p) store_grad(a.weight, 0, c, dw);
+  if (a.bias.p) store_grad(a.bias, 0, c, dbeta);
+  if (a.branch_weight.p) store_grad(a.branch_weight, 0, c, dwb);
+  if (a.gate.p && !a.gate.stride) store_grad(a.gate, 0, c, dgate);
+  if (a.scale.p && !a.scale.stride) store_grad(a.scale, 0, c, dscale);
+  if (a.shift.p && !a.shift.stride) store_grad(a.shift, 0, c, dshift);
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+bool float_type(int d) { return d == SV_FLOAT32 || d == SV_FLOAT16 || d == SV_BFLOAT16; }
+
+bool wide_coef(const Coef& c) { return !c.p || (aligned16(c.p) && c.stride % 8 == 0); }
+
+// 16-byte accesses: rows of a multiple of eight elements on 16-byte boundaries.
+bool wide_rows(const BlockArgs& a) {
+  return a.channels % 8 == 0 && a.x_stride % 8 == 0 && a.branch_stride % 8 == 0 && aligned16(a.x) &&
+         aligned16(a.branch) && aligned16(a.h) && aligned16(a.y) && wide_coef(a.weight) &&
+         wide_coef(a.bias) && wide_coef(a.branch_weight) && wide_coef(a.gate) &&
+         wide_coef(a.scale) && wide_coef(a.shift);
+}
+
+template <typename T, int V, int J, int TPR>
+int launch_forward(const BlockArgs& a, cudaStream_t s) {
+  constexpr int ROWS = kThreads<TPR> / TPR;
+  const unsigned blocks = (unsigned)std::min<int64_t>((a.n + ROWS - 1) / ROWS,
+                                                      (int64_t)num_sms() * 16);
+  block_norm_kernel<T, V, J, TPR><<<blocks, kThreads<TPR>, 0, s>>>(a);
+  SV_LAUNCH_CHECK();
+  return SV_OK;
+}
+
+template <typename T, int V, int J, int TPR>
+int launch_backward(const BackArgs& a, unsigned blocks, cudaStream_t s) {
+  block_norm_backward_kernel<T, V, J, TPR><<<blocks, kThreads<TPR>, 0, s>>>(a);
+  SV_LAUNCH_CHECK();
+  return SV_OK;
+}
+
+// A row's threads: as few as hold it with eight elements each, so that more rows share a block.
+#define SV_BLOCK_NORM_PICK(call, C, wide)                                          \
+  if (wide) {                                                                      \
+    if ((C) <= 64) return call(8, 1, 8);                                           \
+    if ((C) <= 128) return call(8, 1, 16);                                         \
+    if ((C) <= 256) return call(8, 1, 32);                                         \
+    if ((C) <= 512) return call(8, 1, 64);                                         \
+    if ((C) <= 1024) return call(8, 1, 128);                                       \
+    if ((C) <= 2048) return call(8, 1, 256);                                       \
+    if ((C) <= 4096) return call(8, 2, 256);                                       \
+    return call(8, 4, 256);                                                        \
+  }                                                                                \
+  if ((C) <= 256) return call(1, 8, 32);                                           \
+  if ((C) <= 1024) return call(1, 8, 128);                                         \
+  if ((C) <= 2048) return call(1, 8, 256);                                         \
+  return call(1, 32, 256)
+
+template <typename T>
+int forward_typed(const BlockArgs& a, cudaStream_t s) {
+#define SV_CALL(V, J, TPR) launch_forward<T, V, J, TPR>(a, s)
+  SV_BLOCK_NORM_PICK(SV_CALL, a.channels, wide_rows(a));
+#undef SV_CALL
+}
+
+template <typename T>
+int backward_typed(const BackArgs& a, bool wide, unsigned blocks, cudaStream_t s) {
+#define SV_CALL(V, J, TPR) launch_backward<T, V, J, TPR>(a, blocks, s)
+  SV_BLOCK_NORM_PICK(SV_CALL, a.f.channels, wide);
+#undef SV_CALL
+}
+
+// Rows of a piece, and how many pieces there can be (each batch element's last one is ragged).
+struct Pieces {
+  int rows;
+  int64_t most;
+};
+Pieces pieces_of(int64_t n, int64_t groups) {
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>((n + 15) / 16, (int64_t)num_sms() * BN_PIECES_PER_SM));
+  Pieces p;
+  p.rows = (int)std::max<int64_t>(1, (n + want - 1) / want);
+  p.most = (n + p.rows - 1) / p.rows + groups;
+  return p;
+}
+
+struct BackPlan {
+  Pieces pieces;
+  size_t perm, offsets, scratch, total;  // `partial` is at the start
+};
+BackPlan back_plan(int64_t n, int channels, int64_t groups) {  // groups 0: rows are not sorted
+  BackPlan p;
+  p.pieces = pieces_of(n, groups ? groups + 1 : 0);
+  p.perm = align_up((size_t)p.pieces.most * 3 * channels * sizeof(float), 256);
+  p.offsets = p.perm + (groups ? align_up((size_t)n * sizeof(int32_t), 256) : 0);
+  p.scratch = p.offsets + (groups ? align_up((size_t)(groups + 1) * sizeof(int32_t), 256) : 0);
+  p.total = p.scratch + (groups ? group_rows_bytes(n, (int)groups) : 0);
+  return p;
+}
+
+Coef to_coef(const sv_rows& r) { return {r.data, r.stride, r.dtype}; }
+Grad to_grad(const sv_rows& r) { return {const_cast<void*>(r.data), r.stride, r.dtype}; }
+
+int check_rows(const sv_rows& r, const char* name, const char* what) {
+  if (!r.data) return SV_OK;
+  if (!float_type(r.dtype)) SV_FAIL(SV_ERR_BAD_DTYPE, std::string(what) + ": unknown dtype of " + name);
+  if (r.stride < 0) SV_FAIL(SV_ERR_INVALID_ARGUMENT, std::string(what) + ": negative stride of " + name);
+  return SV_OK;
+}
+
+int fill(const sv_block_norm_args* g, const char* what, BlockArgs* a) {
+  const std::string at = what;
+  if (!g) SV_FAIL(SV_ERR_INVALID_ARGUMENT, at + ": null arguments");
+  if (g->n < 0 || g->channels < 0 || g->batch < 0)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, at + ": negative size");
+  if (!float_type(g->dtype)) SV_FAIL(SV_ERR_BAD_DTYPE, at + ": unknown dtype");
+  if (g->channels > BN_MAX_CHANNELS)
+    SV_FAIL(SV_ERR_UNSUPPORTED, at + ": more than " + std::to_string(BN_MAX_CHANNELS) + " channels");
+  if (g->n > INT32_MAX - 1024) SV_FAIL(SV_ERR_UNSUPPORTED, at + ": too many rows");
+  if (!(g->dropout >= 0.0 && g->dropout <= 1.0))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, at + ": dropout outside [0, 1]");
+  if (!(g->eps >= 0.0f)) SV_FAIL(SV_ERR_INVALID_ARGUMENT, at + ": eps must not be negative");
+  const struct { const sv_rows* r; const char* name; } rows[] = {
+      {&g->weight, "weight"}, {&g->bias, "bias"}, {&g->branch_weight, "branch_weight"},
+      {&g->gate, "gate"}, {&g->scale, "scale"}, {&g->shift, "shift"}};
+  for (const auto& r : rows) {
+    const int rc = check_rows(*r.r, r.name, what);
+    if (rc != SV_OK) return rc;
+  }
+  if (g->branch_weight.data && !g->branch_norm)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, at + ": a branch weight goes with the branch's norm");
+  const bool per_batch = (g->gate.data && g->gate.stride) || (g->scale.data && g->scale.stride) ||
+                         (g->shift.data && g->shift.stride);
+  if (per_batch && g->n > 0 && !g->coords)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, at + ": rows of coefficients per batch element need coords");
+  if (per_batch && g->batch > GROUP_MAX_BINS - 1)
+    SV_FAIL(SV_ERR_UNSUPPORTED, at + ": more than " + std::to_string(GROUP_MAX_BINS - 1) + " batch elements");
+  *a = BlockArgs{};
+  a->n = g->n;
+  a->channels = g->channels;
+  a->x = g->x;
+  a->x_stride = g->x_stride;
+  a->branch = g->branch;
+  a->branch_stride = g->branch_stride;
+  a->layer = g->layer != 0;
+  a->branch_norm = g->branch_norm != 0;
+  a->alpha = g->residual_scale;
+  a->eps = g->eps;
+  a->weight = to_coef(g->weight);
+  a->bias = to_coef(g->bias);
+  a->branch_weight = to_coef(g->branch_weight);
+  a->gate = to_coef(g->gate);
+  a->scale = to_coef(g->scale);
+  a->shift = to_coef(g->shift);
+  a->weight.stride = a->bias.stride = a->branch_weight.stride = 0;
+  a->per_batch = per_batch;
+  a->coords = g->coords;
+  a->batch = per_batch ? g->batch : 1;
+  a->drop = make_dropout(g->dropout, g->seed, g->seed_at, g->subsequence);
+  a->h = g->h;
+  a->stats = reinterpret_cast<float4*>(g->stats);
+  return SV_OK;
+}
+
+}  // namespace
+}  // namespace sv
+
+using namespace sv;
+
+extern "C" int sv_block_norm(const sv_block_norm_args* args, void* y, int32_t* status,
+                             sv_stream_t stream) {
+  BlockArgs a;
+  const int rc = fill(args, "sv_block_norm", &a);
+  if (rc != SV_OK) return rc;
+  if (a.n == 0 || a.channels == 0) return SV_OK;
+  if (!a.x || !a.branch || !a.h || !y)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_block_norm: null pointer");
+  if (a.x_stride < a.channels || a.branch_stride < a.channels)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_block_norm: row stride below the row length");
+  if (a.stats && !aligned16(a.stats))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_block_norm: stats must be 16-byte aligned");
+  a.y = y;
+  a.status = status;
+  switch (args->dtype) {
+    case SV_FLOAT32: return forward_typed<float>(a, to_stream(stream));
+    case SV_FLOAT16: return forward_typed<__half>(a, to_stream(stream));
+    default: return forward_typed<__nv_bfloat16>(a, to_stream(stream));
+  }
+}
+
+extern "C" size_t sv_block_norm_backward_workspace_bytes(int64_t n, int channels, int64_t batch) {
+  if (n < 0 || channels < 0 || batch < 0 || batch > GROUP_MAX_BINS - 1) return 0;
+  return back_plan(n, channels, batch).total;
+}
+
+extern "C" int sv_block_norm_backward(const sv_block_norm_args* args, const void* dy, const void* dh,
+                                      void* dx, void* dbranch, const sv_block_norm_grads* grads,
+                                      void* workspace, size_t workspace_bytes, sv_stream_t stream) {
+  BlockArgs f;
+  const int rc = fill(args, "sv_block_norm_backward", &f);
+  if (rc != SV_OK) return rc;
+  if (!grads) SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_block_norm_backward: null arguments");
+  const struct { const sv_rows* r; const Coef* c; const char* name; } rows[] = {
+      {&grads->weight, &f.weight, "dweight"}, {&grads->bias, &f.bias, "dbias"},
+      {&grads->branch_weight, &f.branch_weight, "dbranch_weight"}, {&grads->gate, &f.gate, "dgate"},
+      {&grads->scale, &f.scale, "dscale"}, {&grads->shift, &f.shift, "dshift"}};
+  bool sums = false;
+  for (const auto& r : rows) {
+    const int bad = check_rows(*r.r, r.name, "sv_block_norm_backward");
+    if (bad != SV_OK) return bad;
+    if (r.r->data && (!r.c->p || (r.r->stride != 0) != (r.c->stride != 0)))
+      SV_FAIL(SV_ERR_INVALID_ARGUMENT,
+              std::string("sv_block_norm_backward: ") + r.name + " has no coefficients of its shape");
+    sums |= r.r->data != nullptr;
+  }
+  if (f.channels == 0 || !(sums || dx || dbranch)) return SV_OK;
+  if (f.n > 0 && (!f.h || !f.stats || !f.branch || !(dy || dh)))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_block_norm_backward: null pointer");
+  if (f.branch_stride < f.channels)
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_block_norm_backward: row stride below the row length");
+  if (!aligned16(f.stats))
+    SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_block_norm_backward: stats must be 16-byte aligned");
+  // Rows are sorted where coefficients differ by batch element: the pieces then have one element each.
+  const int64_t groups = f.per_batch ? f.batch : 0;
+  const BackPlan plan = back_plan(f.n, f.channels, groups);
+  if ((sums || groups) && (!workspace || workspace_bytes < plan.total || !aligned16(workspace)))
+    SV_FAIL(SV_ERR_WORKSPACE, "sv_block_norm_backward: workspace too small or unaligned");
+  cudaStream_t s = to_stream(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  BackArgs a{};
+  a.f = f;
+  a.dy = dy;
+  a.dh = dh;
+  a.dx = dx;
+  a.dbranch = dbranch;
+  a.piece = plan.pieces.rows;
+  a.partial = sums ? reinterpret_cast<float*>(ws) : nullptr;
+  a.want_e = grads->gate.data || grads->branch_weight.data;
+  if (groups) {
+    int32_t* perm = reinterpret_cast<int32_t*>(ws + plan.perm);
+    int32_t* offsets = reinterpret_cast<int32_t*>(ws + plan.offsets);
+    const int bad = group_rows(f.coords, 4, f.n, (int)groups, perm, offsets, nullptr,
+                               ws + plan.scratch, s);
+    if (bad != SV_OK) return bad;
+    a.perm = perm;
+    a.offsets = offsets;
+  }
+  if (f.n > 0) {
+    BlockArgs ready = f;  // what the backward pass reads has to be aligned; x and y are not there
+    ready.x = nullptr;
+    ready.x_stride = 0;
+    const bool wide = wide_rows(ready) && aligned16(dy) && aligned16(dh) && aligned16(dx) &&
+                      aligned16(dbranch);
+    const unsigned blocks = (unsigned)plan.pieces.most;
+    const int bad = args->dtype == SV_FLOAT32   ? backward_typed<float>(a, wide, blocks, s)
+                    : args->dtype == SV_FLOAT16 ? backward_typed<__half>(a, wide, blocks, s)
+                                                : backward_typed<__nv_bfloat16>(a, wide, blocks, s);
+    if (bad != SV_OK) return bad;
+  }
+  if (!sums) return SV_OK;
+  SumArgs g{};
+  g.f = f;
+  g.offsets = a.offsets;
+  g.piece = a.piece;
+  g.partial = a.partial;
+  g.weight = to_grad(grads->weight);
+  g.bias = to_grad(grads->bias);
+  g.branch_weight = to_grad(grads->branch_weight);
+  g.gate = to_grad(grads->gate);
+  g.scale = to_grad(grads->scale);
+  g.shift = to_grad(grads->shift);
+  g.weight.stride = g.bias.stride = g.branch_weight.stride = 0;
+  block_norm_sums_kernel<<<(unsigned)((f.channels + 31) / 32), 1024, 0, s>>>(g);
+  SV_LAUNCH_CHECK();
+  return SV_OK;
+}

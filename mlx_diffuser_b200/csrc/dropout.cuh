@@ -1,0 +1,75 @@
+// Dropout whose mask is a function of the element's number: counter-based random numbers, formed again
+// wherever they are wanted, so that no mask is stored between the passes.
+//
+// Philox4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as
+// 1, 2, 3", 2011): key = the seed's two words, counter = (g, subsequence) as two words each. One counter
+// gives eight 16-bit numbers, those of the elements 8 g .. 8 g + 7 in row-major order, the low half of
+// a word first. An element is dropped when its number is below `cut` = p 2^16 rounded, and kept
+// ones are multiplied by 2^16 / (2^16 - cut), which keeps the mean exactly. 16 bits an element, since
+// with 32 the generator's integer products would bound the pass and not HBM.
+#pragma once
+
+#include "common.cuh"
+
+namespace sv {
+
+struct Dropout {
+  uint32_t cut;      // 0: nothing is dropped; 65536: everything
+  float scale;       // of what is kept
+  uint64_t seed;
+  const uint64_t* seed_at;  // on the device, read instead of `seed`; or null
+  uint64_t subsequence;
+};
+
+inline Dropout make_dropout(double p, uint64_t seed, const void* seed_at, uint64_t subsequence) {
+  Dropout d;
+  d.cut = (uint32_t)(p * 65536.0 + 0.5);
+  d.scale = d.cut >= 65536u ? 0.0f : (float)(65536.0 / (65536.0 - d.cut));
+  d.seed = seed;
+  d.seed_at = static_cast<const uint64_t*>(seed_at);
+  d.subsequence = subsequence;
+  return d;
+}
+
+#ifdef __CUDACC__
+__device__ __forceinline__ uint64_t seed_of(const Dropout& d) {
+  return d.seed_at ? __ldg(reinterpret_cast<const unsigned long long*>(d.seed_at)) : d.seed;
+}
+
+__device__ __forceinline__ uint4 philox(uint64_t group, uint64_t subsequence, uint64_t seed) {
+  uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32);
+  uint32_t c2 = (uint32_t)subsequence, c3 = (uint32_t)(subsequence >> 32);
+  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// v[0..7], the elements of one counter: scaled, or zero whatever they were.
+__device__ __forceinline__ void drop_eight(float (&v)[8], const uint4& r, const Dropout& d) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = (w[i] & 0xffffu) >= d.cut ? v[2 * i] * d.scale : 0.0f;
+    v[2 * i + 1] = (w[i] >> 16) >= d.cut ? v[2 * i + 1] * d.scale : 0.0f;
+  }
+}
+
+// One element by itself, number `at`.
+__device__ __forceinline__ float drop_one(float v, uint64_t at, uint64_t seed, const Dropout& d) {
+  const uint4 r = philox(at >> 3, d.subsequence, seed);
+  const uint32_t half = (uint32_t)at & 7u;
+  const uint32_t w = half < 2 ? r.x : half < 4 ? r.y : half < 6 ? r.z : r.w;
+  return (half & 1u ? w >> 16 : w & 0xffffu) >= d.cut ? v * d.scale : 0.0f;
+}
+#endif
+
+}  // namespace sv
