@@ -498,6 +498,72 @@ SV_API int sv_linear_backward(const void* dout, const float* preact, const void*
                               void* workspace, size_t workspace_bytes, int32_t* status,
                               sv_stream_t stream);
 
+/* ---- mixture of experts: the router and the products grouped by expert -------------------- */
+
+/* Each row's k largest logits ([n, experts] of `dtype`, rows `stride` apart), by falling value and the
+ * lower index first among equals: chosen [n, k], -1 where the logit is -inf; weights fp32 [n, k], the
+ * softmax over the chosen logits (`normalize`) or over all, 0 for -1. The slots (row * k + choice) sorted by
+ * expert, ascending within one, those of -1 last: order [n k], offsets [experts + 1], and place [n, k],
+ * the slot's position in order or -1. experts <= 1024, k <= min(experts, 32). A NaN counts as the
+ * largest and makes the row's weights NaN. */
+SV_API size_t sv_route_workspace_bytes(int64_t n, int experts, int k);
+SV_API int sv_route(const void* logits, int64_t stride, int64_t n, int experts, int k, int dtype,
+                    int normalize, int32_t* chosen, float* weights, int32_t* order,
+                    int32_t* offsets, int32_t* place, void* workspace, size_t workspace_bytes,
+                    sv_stream_t stream);
+
+/* The gradient of the weights: dlogits [n, experts] of `dtype`, contiguous. */
+SV_API int sv_route_backward(const void* logits, int64_t stride, int64_t n, int experts, int k,
+                             int dtype, int normalize, const int32_t* chosen, const float* weights,
+                             const float* dweights, void* dlogits, sv_stream_t stream);
+
+/* Projections grouped by expert over the slots of sv_route. Position p of expert e (offsets[e] <= p <
+ * offsets[e + 1]) has r_p = act(x_p weight_e^T + bias_e), x_p = x[order[p] / k] with `gather` (x [n,
+ * inputs]), else x[p] (x [n k, inputs]); rows `ldx` apart. weight: rows `ldw` apart, experts `w_expert`
+ * elements apart; bias [experts, outputs] or null. The result is r [n k, outputs], zeros behind the
+ * last expert's position, or with `combine` sum_j weights[n, j] r[place[n, j]], [n, outputs]; then
+ * `rows` [n k, outputs] holds r in fp32. preact: receives the activation's argument in fp32, or null. dtype fp32 / fp16 / bf16,
+ * fp32 sums; 16-bit types run on the tensor cores. An entry of order that is no slot counts as a row of
+ * zeros (SV_DEVICE_BAD_INDEX), one of place as none. */
+typedef struct sv_expert_args {
+  int64_t n;
+  const void* x;
+  int64_t ldx;
+  const void* weight;
+  int64_t ldw;
+  int64_t w_expert;
+  const void* bias;
+  const int32_t* order;
+  const int32_t* offsets;
+  const int32_t* place;
+  const float* weights;
+  float* preact;
+  float* rows;
+  int64_t inputs;
+  int64_t outputs;
+  int k;
+  int experts;
+  int dtype;
+  int activation;
+  int gather;
+  int combine;
+} sv_expert_args;
+
+/* Workspace of one pass (an sv_linear_pass); the last three are of the backward pass: which gradients are
+ * wanted, and dout. */
+SV_API size_t sv_expert_linear_workspace_bytes(const sv_expert_args* args, int pass, int want_dx,
+                                               int want_dw, const void* dout);
+SV_API int sv_expert_linear(const sv_expert_args* args, void* out, void* workspace,
+                            size_t workspace_bytes, int32_t* status, sv_stream_t stream);
+
+/* The gradients of x, weight, bias (contiguous, of `dtype`) and of the routing's weights (fp32 [n, k];
+ * with `combine` only), each null where it is not wanted, from dout (contiguous, like the result) and the
+ * forward pass's preact and rows. dz is rounded to `dtype` before the products (sv_linear_backward).
+ * Every sum has a fixed order. workspace: 128-byte aligned. */
+SV_API int sv_expert_linear_backward(const sv_expert_args* args, const void* dout, void* dx,
+                                     void* dweight, void* dbias, float* dweights, void* workspace,
+                                     size_t workspace_bytes, int32_t* status, sv_stream_t stream);
+
 /* ---- windowed attention with a learned relative position bias --------------------------- */
 
 /* The rows of a window grouping (sv_window_groups' perm [n] and offsets [groups + 1]) in window

@@ -7,6 +7,7 @@ learned relative position bias."""
 from ._native import check_device_status
 from .kernels.block_norm import block_norm
 from .kernels.dropout import dropout
+from .kernels.expert import ExpertRoutes, expert_linear, route
 from .kernels.linear import linear
 from .kernels.norm import rms_norm
 from .kernels.sparse import sparse_conv3d
@@ -21,15 +22,18 @@ from .layers.sparse import (
 )
 
 __all__ = [
+    "ExpertRoutes",
     "SparseConv3D",
     "SparseTensor",
     "block_norm",
     "build_neighbor_map",
     "check_device_status",
     "dropout",
+    "expert_linear",
     "linear",
     "position_buckets",
     "rms_norm",
+    "route",
     "sparse_conv3d",
     "sparse_downsample",
     "sparse_self_attention",

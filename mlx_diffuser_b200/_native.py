@@ -79,6 +79,18 @@ class BlockNormGrads(ctypes.Structure):
     _fields_ = [(name, Rows) for name in ("weight", "bias", "branch_weight", "gate", "scale", "shift")]
 
 
+class ExpertArgs(ctypes.Structure):
+    """sv_expert_args."""
+
+    _fields_ = [
+        ("n", _I64), ("x", _P), ("ldx", _I64), ("weight", _P), ("ldw", _I64), ("w_expert", _I64),
+        ("bias", _P), ("order", _P), ("offsets", _P), ("place", _P), ("weights", _P),
+        ("preact", _P), ("rows", _P), ("inputs", _I64), ("outputs", _I64), ("k", _I32),
+        ("experts", _I32), ("dtype", _I32), ("activation", _I32), ("gather", _I32),
+        ("combine", _I32),
+    ]
+
+
 _SIGNATURES = {
     "sv_last_error": (ctypes.c_char_p, []),
     "sv_abi_version": (_I32, []),
@@ -154,6 +166,20 @@ _SIGNATURES = {
     "sv_linear_backward": (
         _I32,
         [_P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I32, _I32, _P, _P, _P, _P, _SZ, _P, _P],
+    ),
+    "sv_route_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
+    "sv_route": (
+        _I32, [_P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _SZ, _P]
+    ),
+    "sv_route_backward": (
+        _I32, [_P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P]
+    ),
+    "sv_expert_linear_workspace_bytes": (
+        _SZ, [ctypes.POINTER(ExpertArgs), _I32, _I32, _I32, _P]
+    ),
+    "sv_expert_linear": (_I32, [ctypes.POINTER(ExpertArgs), _P, _P, _SZ, _P, _P]),
+    "sv_expert_linear_backward": (
+        _I32, [ctypes.POINTER(ExpertArgs), _P, _P, _P, _P, _P, _P, _SZ, _P, _P]
     ),
     "sv_window_plan_bytes": (_SZ, [_I64]),
     "sv_window_plan": (_I32, [_P, _P, _P, _I64, _I64, _P, _P, _P]),

@@ -1,0 +1,594 @@
+// The products grouped by expert on the 5th-generation tensor cores (fp16, bf16).
+//
+// The tiles, stages and warp roles are those of linear_tc.cu: persistent CTAs, or pairs of them
+// (cta_group::2) on tiles of 256 rows, operands by TMA into 128-byte swizzled stages, one issuing
+// thread, two accumulators in TMEM, and eight epilogue warps that work on one tile while the next is
+// formed. What differs is where the tiles are:
+//
+//   kRows      Every expert's positions are cut into tiles of their own, so that a tile has one weight.
+//              The CTAs count the tiles of all experts on the device (a scan over the offsets in
+//              shared memory) and look a tile's expert up by bisection. A tile's last rows may be the
+//              next expert's: they are formed and not stored. Weights are read through a
+//              three-dimensional map, so that what lies past an expert's matrix is zeros and not
+//              its neighbour.
+//   kWeights   The sum runs over an expert's positions, from any first row to any last. The steps of 64
+//              positions start at the first; the rows past the last one have to be zeros in both
+//              operands (0 times a neighbour's infinity is not 0), which a TMA load gives past the end of
+//              its map: every expert has a copy of the two maps whose extent ends with its last
+//              position, written by expert_maps_kernel.
+//
+// Every wait on an mbarrier is bounded, and unwinds as in linear_tc.cu.
+#include <algorithm>
+
+#include "expert.h"
+#include "gemm_tc.cuh"
+
+namespace sv {
+namespace {
+
+constexpr int EX_MAX = 1024;  // experts
+
+template <int BN, bool PAIR>
+struct ExLayout {
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // of one CTA
+  static constexpr int A_STAGE = TM * 128;
+  static constexpr int B_STAGE = B_ROWS * 128;
+  static constexpr int FIT = (176 * 1024) / (A_STAGE + B_STAGE);
+  static constexpr int STAGES = FIT > 7 ? 7 : FIT;
+  static constexpr int A_OFF = 0;
+  static constexpr int B_OFF = STAGES * A_STAGE;
+  static constexpr int CHUNK_OFF = B_OFF + STAGES * B_STAGE;  // float [8 warps][32][CHUNK_LD]
+  static constexpr int COL_OFF = CHUNK_OFF + EPI_WARPS * 32 * CHUNK_LD * 4;  // [2][bias, scale][BN]
+  static constexpr int FIRST_OFF = COL_OFF + 2 * 2 * BN * 4;  // int [experts + 1]
+  static constexpr int MISC_OFF = FIRST_OFF + (EX_MAX + 4) * 4;
+  static constexpr int BAR_OFF = MISC_OFF + 16;
+  static constexpr int NUM_BARS = 2 * STAGES + 5;
+  static constexpr int SMEM = BAR_OFF + NUM_BARS * 8 + 1024;
+  static_assert(SMEM <= 227 * 1024, "shared memory budget");
+  static_assert(STAGES >= 4, "pipeline depth");
+};
+
+struct ExArgs {
+  const int32_t* offsets;
+  int32_t experts, slots;
+  int64_t m, n;            // m: kWeights
+  int32_t tiles_m, tiles_n;  // tiles_m: kWeights
+  int32_t steps;           // kRows
+  uint32_t idesc;
+  bool b_mn, wide_io, zero_tail;
+  const CUtensorMap* maps;  // kWeights: [experts][2]
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint64_t* bar, int32_t x,
+                                            int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap, uint32_t bar,
+                                                 int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// The segment of an expert, whatever the offsets are.
+__device__ __forceinline__ int2 segment(const ExArgs& a, int e) {
+  const int first = min(max(__ldg(a.offsets + e), 0), a.slots);
+  return make_int2(first, max(min(__ldg(a.offsets + e + 1), a.slots), first));
+}
+
+struct ExTile {
+  int32_t e, row, last, n0, k1;  // row: first position (kRows), or row of the expert's result
+  int32_t base;                  // kWeights: the expert's first position
+};
+
+template <int BN, bool PAIR, bool WEIGHTS>
+__device__ __forceinline__ ExTile ex_tile(const ExArgs& a, const int32_t* first, int32_t t) {
+  constexpr int ROWS = PAIR ? 2 * TM : TM;
+  ExTile o;
+  const int32_t piece = t / a.tiles_n;
+  o.n0 = (t - piece * a.tiles_n) * BN;
+  if constexpr (WEIGHTS) {
+    o.e = piece / a.tiles_m;
+    o.row = (piece - o.e * a.tiles_m) * ROWS;
+    o.last = (int32_t)a.m;
+    const int2 s = segment(a, o.e);
+    o.base = s.x;
+    o.k1 = (s.y - s.x + 63) / 64;
+  } else {
+    int lo = 0, hi = a.experts;  // first[lo] <= piece < first[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] <= piece) lo = mid;
+      else hi = mid;
+    }
+    const int2 s = segment(a, lo);
+    o.e = lo;
+    o.row = s.x + (piece - first[lo]) * ROWS;
+    o.last = s.y;
+    o.base = 0;
+    o.k1 = a.steps;
+  }
+  return o;
+}
+
+// finish() of gemm_tc.cuh for what the experts' epilogue has: scale, bias, argument kept, activation, and
+// results in O or, WIDE, in fp32.
+template <typename O, bool WIDE, int R, int W>
+__device__ __forceinline__ void ex_finish(const Epilogue& ep, float (&v)[R][W], const float* bias,
+                                          const float* scale, int64_t row, int step, int rows,
+                                          int64_t n, int64_t col) {
+  if constexpr (!WIDE) {
+    finish<O, R, W>(ep, v, bias, scale, ep.col_scale != nullptr, row, step, rows, n, col);
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        if (ep.col_scale) v[i][j] *= scale[j];
+        if (ep.bias) v[i][j] += bias[j];
+      }
+    auto store = [&](float* to) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (i * step >= rows) continue;
+        float* dst = to + (row + i * step) * n + col;
+        if constexpr (W == 8) {
+          *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(v[i]);
+          *reinterpret_cast<float4*>(dst + 4) = *reinterpret_cast<const float4*>(v[i] + 4);
+        } else {
+          *dst = v[i][0];
+        }
+      }
+    };
+    if (ep.preact) store(ep.preact);
+    if (ep.act == SV_ACT_SILU) activate_all<SV_ACT_SILU>(v);
+    else if (ep.act == SV_ACT_GELU) activate_all<SV_ACT_GELU>(v);
+    else if (ep.act == SV_ACT_GELU_TANH) activate_all<SV_ACT_GELU_TANH>(v);
+    store(static_cast<float*>(ep.out));
+  }
+}
+
+template <int BN, bool PAIR, typename O, bool WEIGHTS, bool WIDE>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+    expert_tc_kernel(const __grid_constant__ CUtensorMap map_a,
+                     const __grid_constant__ CUtensorMap map_b, ExArgs a, Epilogue ep,
+                     int32_t* status) {
+  using L = ExLayout<BN, PAIR>;
+  constexpr int S = L::STAGES;
+  constexpr int ROWS = PAIR ? 2 * TM : TM;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  float* s_cols = reinterpret_cast<float*>(smem + L::COL_OFF);
+  int32_t* s_first = reinterpret_cast<int32_t*>(smem + L::FIRST_OFF);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + S;
+  uint64_t* acc_full = bars + 2 * S;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drained = acc_empty + 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0u;
+  const int32_t unit = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+  const int32_t units = PAIR ? gridDim.x >> 1 : gridDim.x;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], (PAIR ? 2 : 1) * EPI_WARPS);
+    }
+    mbar_init(drained, 1);
+    *s_abort = 0;
+    fence_mbar_init();
+    if constexpr (!WEIGHTS) {
+      prefetch_tmap(&map_a);
+      prefetch_tmap(&map_b);
+    }
+  }
+  if (warp == 1) alloc_tmem<PAIR>(s_tmem, 2 * BN);
+  if constexpr (!WEIGHTS) {
+    for (int e = threadIdx.x; e < a.experts; e += TC_THREADS) {
+      const int2 s = segment(a, e);
+      s_first[e + 1] = (s.y - s.x + ROWS - 1) / ROWS;
+    }
+  }
+  __syncthreads();
+  if (!WEIGHTS && warp == 2) {  // tiles of the experts before each
+    int before = 0;
+    for (int e0 = 0; e0 < a.experts; e0 += 32) {
+      int v = e0 + lane < a.experts ? s_first[e0 + lane + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      v += before;
+      if (e0 + lane < a.experts) s_first[e0 + lane + 1] = v;
+      before = __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) s_first[0] = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the other CTA's barriers are ready too
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  const int32_t total = (WEIGHTS ? a.experts * a.tiles_m : s_first[a.experts]) * a.tiles_n;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0, seen = -1;
+      for (int32_t t = unit; t < total && ok; t += units) {
+        const ExTile w = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, t);
+        const CUtensorMap* ma = &map_a;
+        const CUtensorMap* mb = &map_b;
+        if constexpr (WEIGHTS) {
+          ma = a.maps + 2 * w.e;
+          mb = ma + 1;
+          if (w.e != seen) {  // written by another kernel through the generic proxy
+            asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(ma) : "memory");
+            asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(mb) : "memory");
+            seen = w.e;
+          }
+        }
+        const int32_t m0 = w.row + (int32_t)rank * TM, n0 = w.n0 + (int32_t)rank * L::B_ROWS;
+        for (int k = 0; k < w.k1; ++k, ++it) {
+          const int slot = it % S;
+          if (!mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, s_abort)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0)
+            mbar_arrive_expect_tx(&full[slot], (PAIR ? 2 : 1) * (L::A_STAGE + L::B_STAGE));
+          const uint32_t sa = smem_u32(smem + L::A_OFF + slot * L::A_STAGE);
+          const uint32_t sb = smem_u32(smem + L::B_OFF + slot * L::B_STAGE);
+          const int kk = k * 64;
+          const uint32_t bar = PAIR ? in_first(smem_u32(&full[slot])) : 0u;
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+            if constexpr (PAIR) tma_load_pair(dst, map, bar, x, y);
+            else tma_load_2d(dst, map, &full[slot], x, y);
+          };
+          auto load3 = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+            if constexpr (PAIR) tma_load_3d_pair(dst, map, bar, x, y, w.e);
+            else tma_load_3d(dst, map, &full[slot], x, y, w.e);
+          };
+          if constexpr (WEIGHTS) {
+#pragma unroll
+            for (int r = 0; r < TM / 64; ++r) load(sa + r * MN_STRIDE, ma, m0 + 64 * r, w.base + kk);
+#pragma unroll
+            for (int r = 0; r < L::B_ROWS / 64; ++r)
+              load(sb + r * MN_STRIDE, mb, n0 + 64 * r, w.base + kk);
+          } else {
+            load(sa, ma, kk, m0);
+            if (a.b_mn) {
+#pragma unroll
+              for (int r = 0; r < L::B_ROWS / 64; ++r)
+                load3(sb + r * MN_STRIDE, mb, n0 + 64 * r, kk);
+            } else {
+              load3(sb, mb, kk, n0);
+            }
+          }
+        }
+      }
+      if (!ok) {
+        report(status, SV_DEVICE_WAIT_TIMEOUT);
+        // the copies in flight write this CTA's shared memory: let them land
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 10000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int it = 0, local = 0;
+      for (int32_t t = unit; t < total && ok; t += units, ++local) {
+        const ExTile w = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, t);
+        const int ab = local & 1;
+        if (!mbar_wait_bounded(&acc_empty[ab], ((local >> 1) & 1) ^ 1, s_abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(ab * BN);
+        for (int k = 0; k < w.k1; ++k, ++it) {
+          const int slot = it % S;
+          if (!mbar_wait_bounded(&full[slot], (it / S) & 1, s_abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + L::A_OFF + slot * L::A_STAGE);
+          const uint32_t sb = smem_u32(smem + L::B_OFF + slot * L::B_STAGE);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {  // 16 of k: one instruction
+            const uint64_t da = WEIGHTS ? smem_desc_mn_sw128(sa + j * 2 * ATOM, MN_STRIDE, ATOM)
+                                        : smem_desc_sw128(sa + j * 32);
+            const uint64_t db = WEIGHTS || a.b_mn
+                                    ? smem_desc_mn_sw128(sb + j * 2 * ATOM, MN_STRIDE, ATOM)
+                                    : smem_desc_sw128(sb + j * 32);
+            issue_mma<PAIR, false>(d, da, db, a.idesc, (k > 0 || j > 0) ? 1u : 0u);
+          }
+          commit<PAIR>(&empty[slot]);
+        }
+        if (ok) commit<PAIR>(&acc_full[ab]);
+      }
+      if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
+      // the products in flight read both CTAs' shared memory: let them finish
+      commit<PAIR>(drained);
+      const uint64_t t0 = global_timer_ns();
+      while (!mbar_try_wait(drained, 0) && global_timer_ns() - t0 < 1000000000ull) {
+      }
+    }
+  } else {
+    const int q = warp & 3;            // TMEM lanes 32 q .. 32 q + 31
+    const int half = (warp - 2) >> 2;  // columns half * BN / 2 ..
+    const int e = threadIdx.x - 64;
+    float* chunk = reinterpret_cast<float*>(smem + L::CHUNK_OFF) + (warp - 2) * 32 * CHUNK_LD;
+    const bool scaled = ep.col_scale != nullptr;
+    int local = 0;
+    for (int32_t t = unit; t < total; t += units, ++local) {  // left by all warps alike
+      const ExTile w = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, t);
+      const int ab = local & 1;
+      float* s_bias = s_cols + ab * 2 * BN;
+      float* s_scale = s_bias + BN;
+      Epilogue out = ep;
+      if constexpr (WEIGHTS) out.out = static_cast<O*>(ep.out) + (int64_t)w.e * a.m * a.n;
+      // this buffer's last readers were two tiles ago, before the previous epi_sync
+      for (int c = e; c < BN; c += EPI_THREADS) {
+        const bool in = w.n0 + c < a.n;
+        if (ep.bias)
+          s_bias[c] = in ? to_f32(static_cast<const O*>(ep.bias)[w.e * a.n + w.n0 + c]) : 0.f;
+        if (scaled) s_scale[c] = in ? __ldg(ep.col_scale + w.n0 + c) : 1.f;
+      }
+      epi_sync();
+      if (!ok) continue;
+      const int64_t row0 = (int64_t)w.row + rank * TM + q * 32;  // the warp's first row
+      const int rows = (int)max((int64_t)0, min((int64_t)32, w.last - row0));
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[ab], (local >> 1) & 1, s_abort))) {
+        ok = false;
+        continue;
+      }
+      tc_fence_after();
+      const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * BN);
+#pragma unroll 1
+      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+        uint32_t raw[32];
+        tmem_ld_32x32b_x32(t_row + c, raw);
+        tc_wait_ld();
+        const int64_t col = (int64_t)w.n0 + c;
+        if (rows == 0 || col >= a.n) continue;  // the same in all lanes
+        if (w.k1 == 0) {  // an expert without positions: nothing was formed
+#pragma unroll
+          for (int j = 0; j < 32; ++j) raw[j] = 0u;
+        }
+        __syncwarp();  // the previous chunk has been read
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<uint4*>(chunk + lane * CHUNK_LD + j) =
+              make_uint4(raw[j], raw[j + 1], raw[j + 2], raw[j + 3]);
+        __syncwarp();
+        const int cols = (int)min((int64_t)32, a.n - col);
+        if (a.wide_io && cols == 32) {
+          const int j = (lane & 3) * 8;  // four lanes a row, eight rows at a time
+          float bias[8], scale[8];
+#pragma unroll
+          for (int x = 0; x < 8; x += 4) {
+            if (ep.bias)
+              *reinterpret_cast<float4*>(bias + x) =
+                  *reinterpret_cast<const float4*>(s_bias + c + j + x);
+            if (scaled)
+              *reinterpret_cast<float4*>(scale + x) =
+                  *reinterpret_cast<const float4*>(s_scale + c + j + x);
+          }
+          float v[4][8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float* src = chunk + (i * 8 + (lane >> 2)) * CHUNK_LD + j;
+            *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(src);
+            *reinterpret_cast<float4*>(v[i] + 4) = *reinterpret_cast<const float4*>(src + 4);
+          }
+          ex_finish<O, WIDE, 4, 8>(out, v, bias, scale, row0 + (lane >> 2), 8, rows - (lane >> 2), a.n,
+                                   col + j);
+        } else if (lane < cols) {
+          const float bias[1] = {ep.bias ? s_bias[c + lane] : 0.f};
+          const float scale[1] = {scaled ? s_scale[c + lane] : 1.f};
+#pragma unroll 1
+          for (int r = 0; r < rows; r += 16) {
+            float v[16][1];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i][0] = chunk[(r + i) * CHUNK_LD + lane];
+            ex_finish<O, WIDE, 16, 1>(out, v, bias, scale, row0 + r, 1, rows - r, a.n, col + lane);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) arrive_at(in_first(smem_u32(&acc_empty[ab])));
+        else arrive_at(smem_u32(&acc_empty[ab]));
+      }
+    }
+    if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
+    if (!WEIGHTS && a.zero_tail) {
+      const int64_t end = a.slots * a.n;
+      for (int64_t i = (int64_t)segment(a, a.experts - 1).y * a.n + (int64_t)blockIdx.x * EPI_THREADS + e;
+           i < end; i += (int64_t)gridDim.x * EPI_THREADS)
+        static_cast<O*>(ep.out)[i] = from_f32<O>(0.f);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // nothing of the pair still reads or signals this CTA
+  if (warp == 1) {
+    tc_fence_after();
+    free_tmem<PAIR>(tmem, 2 * BN);
+  }
+}
+
+// Copies of the operands' maps whose rows end with each expert's last position.
+__global__ void __launch_bounds__(32)
+    expert_maps_kernel(const __grid_constant__ CUtensorMap map_a,
+                       const __grid_constant__ CUtensorMap map_b, const int32_t* offsets, int slots,
+                       CUtensorMap* maps) {
+  __shared__ alignas(128) uint32_t held[2][32];
+  const int e = blockIdx.x, lane = threadIdx.x;
+  held[0][lane] = reinterpret_cast<const uint32_t*>(&map_a)[lane];
+  held[1][lane] = reinterpret_cast<const uint32_t*>(&map_b)[lane];
+  __syncwarp();
+  if (lane < 2) {
+    // an expert without positions is not loaded; an extent is at least one
+    const uint32_t rows = (uint32_t)max(1, min(__ldg(offsets + e + 1), slots));
+    asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;" ::"r"(
+                     smem_u32(held[lane])),
+                 "r"(rows)
+                 : "memory");
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    asm volatile(
+        "tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned"
+        " [%0], [%1], 128;" ::"l"(maps + 2 * e + i),
+        "r"(smem_u32(held[i]))
+        : "memory");
+}
+
+// A map over `dims` elements (innermost first), with boxes of 128 bytes by `box_rows`. What is past
+// the end of a dimension is filled with zeros.
+int expert_map(const void* p, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+               int dtype, int box_rows, CUtensorMap* map) {
+  EncodeFn encode = encode_fn();
+  if (encode == nullptr) SV_FAIL(SV_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  const cuuint32_t steps[3] = {1, 1, 1};
+  const CUtensorMapDataType type = dtype == SV_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (encode(map, type, rank, const_cast<void*>(p), dims, strides, box, steps,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    SV_FAIL(SV_ERR_CUDA, "cuTensorMapEncodeTiled failed for an operand of the experts");
+  return SV_OK;
+}
+
+template <int BN, bool PAIR, typename O, bool WEIGHTS, bool WIDE>
+int launch_expert(const ExpertGemm& g, CUtensorMap* maps, int32_t* status, cudaStream_t s) {
+  using L = ExLayout<BN, PAIR>;
+  auto kernel = expert_tc_kernel<BN, PAIR, O, WEIGHTS, WIDE>;
+  constexpr int ROWS = PAIR ? 2 * TM : TM;
+  int dev = 0;
+  SV_CUDA_TRY(cudaGetDevice(&dev));
+  cudaLaunchConfig_t config{};
+  config.blockDim = dim3(TC_THREADS);
+  config.dynamicSmemBytes = L::SMEM;
+  config.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = PAIR ? 2 : 1;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  // Units that run at the same time: one more would run after all the others.
+  static int units_of[256] = {};
+  int units = dev < 256 ? units_of[dev] : 0;
+  if (units == 0) {
+    SV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
+    units = num_sms();
+    if constexpr (PAIR) {
+      config.gridDim = dim3(num_sms() / 2 * 2);
+      SV_CUDA_TRY(cudaOccupancyMaxActiveClusters(&units, kernel, &config));
+      if (units < 1) SV_FAIL(SV_ERR_CUDA, "expert_linear: no CTA pair fits this device");
+      units = std::min(units, num_sms() / 2);
+    }
+    if (dev < 256) units_of[dev] = units;
+  }
+  constexpr int ES = 2;
+  CUtensorMap map_a, map_b;
+  const cuuint64_t slots = (cuuint64_t)g.slots;
+  int rc;
+  if constexpr (WEIGHTS) {
+    const cuuint64_t da[2] = {(cuuint64_t)g.m, slots}, db[2] = {(cuuint64_t)g.n, slots};
+    const cuuint64_t sa = (cuuint64_t)g.a.ld * ES, sb = (cuuint64_t)g.b.ld * ES;
+    rc = expert_map(g.a.p, 2, da, &sa, g.dtype, 64, &map_a);
+    if (rc == SV_OK) rc = expert_map(g.b.p, 2, db, &sb, g.dtype, 64, &map_b);
+    if (rc != SV_OK) return rc;
+    expert_maps_kernel<<<g.experts, 32, 0, s>>>(map_a, map_b, g.offsets, (int)g.slots, maps);
+    SV_LAUNCH_CHECK();
+  } else {
+    const cuuint64_t da[2] = {(cuuint64_t)g.k, slots};
+    const cuuint64_t sa = (cuuint64_t)g.a.ld * ES;
+    rc = expert_map(g.a.p, 2, da, &sa, g.dtype, TM, &map_a);
+    const cuuint64_t db[3] = {(cuuint64_t)(g.b.mn ? g.n : g.k), (cuuint64_t)(g.b.mn ? g.k : g.n),
+                              (cuuint64_t)g.experts};
+    const cuuint64_t sb[2] = {(cuuint64_t)g.b.ld * ES, (cuuint64_t)g.b_expert * ES};
+    if (rc == SV_OK) rc = expert_map(g.b.p, 3, db, sb, g.dtype, g.b.mn ? 64 : L::B_ROWS, &map_b);
+    if (rc != SV_OK) return rc;
+  }
+  ExArgs a{};
+  a.offsets = g.offsets;
+  a.experts = g.experts;
+  a.slots = (int32_t)g.slots;
+  a.m = g.m;
+  a.n = g.n;
+  a.tiles_n = (int32_t)((g.n + BN - 1) / BN);
+  a.tiles_m = (int32_t)((g.m + ROWS - 1) / ROWS);
+  a.steps = (int32_t)((g.k + 63) / 64);
+  a.b_mn = g.b.mn;
+  a.zero_tail = g.zero_tail;
+  a.maps = maps;
+  a.idesc = idesc_f16_major(g.dtype == SV_BFLOAT16, ROWS, BN, WEIGHTS, WEIGHTS || g.b.mn);
+  const int64_t pieces = WEIGHTS ? (int64_t)g.experts * a.tiles_m : g.slots / ROWS + g.experts;
+  if (pieces * a.tiles_n > INT32_MAX / 2) SV_FAIL(SV_ERR_UNSUPPORTED, "expert_linear: too many tiles");
+  const Epilogue& ep = g.ep;
+  a.wide_io = g.n % 8 == 0 && aligned16(ep.out) && (!ep.preact || aligned16(ep.preact));
+  units = (int)std::min<int64_t>(pieces * a.tiles_n, units);
+  config.gridDim = dim3((unsigned)(units * (PAIR ? 2 : 1)));
+  SV_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, map_a, map_b, a, ep, status));
+  return SV_OK;
+}
+
+template <typename O, bool WEIGHTS, bool WIDE>
+int launch_form(const ExpertGemm& g, ExpertTile tile, CUtensorMap* maps, int32_t* status,
+                cudaStream_t s) {
+  switch (tile) {
+    case ExpertTile::kPair256: return launch_expert<256, true, O, WEIGHTS, WIDE>(g, maps, status, s);
+    case ExpertTile::kPair128: return launch_expert<128, true, O, WEIGHTS, WIDE>(g, maps, status, s);
+    case ExpertTile::kOne128: return launch_expert<128, false, O, WEIGHTS, WIDE>(g, maps, status, s);
+    default: return launch_expert<64, false, O, WEIGHTS, WIDE>(g, maps, status, s);
+  }
+}
+
+}  // namespace
+
+size_t expert_maps_bytes(int experts) { return (size_t)experts * 2 * sizeof(CUtensorMap); }
+
+int expert_gemm_tc(const ExpertGemm& g, ExpertTile tile, void* maps, int32_t* status,
+                   cudaStream_t s) {
+  CUtensorMap* at = static_cast<CUtensorMap*>(maps);
+  const bool half = g.dtype == SV_FLOAT16;
+  if (g.form == ExpertForm::kWeights)
+    return half ? launch_form<__half, true, false>(g, tile, at, status, s)
+                : launch_form<__nv_bfloat16, true, false>(g, tile, at, status, s);
+  if (g.ep.out_dtype == SV_FLOAT32)
+    return half ? launch_form<__half, false, true>(g, tile, at, status, s)
+                : launch_form<__nv_bfloat16, false, true>(g, tile, at, status, s);
+  return half ? launch_form<__half, false, false>(g, tile, at, status, s)
+              : launch_form<__nv_bfloat16, false, false>(g, tile, at, status, s);
+}
+
+}  // namespace sv

@@ -19,7 +19,8 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "linear.h"
+#include "gemm_f32.cuh"
+#include "raise.cuh"
 
 namespace sv {
 namespace {
@@ -136,69 +137,6 @@ int gemm_few(const Gemm& g, cudaStream_t s) {
 
 // ---- fp32 tiles --------------------------------------------------------------------------------
 
-constexpr int FK = 16;  // k per shared-memory stage
-
-// Two fp32 multiply-adds in one instruction, each rounded like fmaf's.
-__device__ __forceinline__ void fma_pair(uint64_t& c, uint64_t a, uint64_t b) {
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
-}
-__device__ __forceinline__ uint64_t twice(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return (uint64_t)u << 32 | u;
-}
-
-// One operand's T rows x FK steps of a stage, by 256 threads in accesses of V elements: from global
-// memory into registers, and from there into shared memory, steps outermost.
-template <int T, int V>
-struct Stage {
-  static constexpr int PER = T * FK / 256;  // elements a thread
-  // The e-th access's row r and step l, along one of which its elements lie.
-  static __device__ __forceinline__ void place(bool mn, int e, int* r, int* l) {
-    const int at = threadIdx.x + 256 * e;
-    *r = mn ? at % (T / V) * V : at / (FK / V);
-    *l = mn ? at / (T / V) : at % (FK / V) * V;
-  }
-  static __device__ __forceinline__ void fetch(const Operand& o, int64_t r0, int64_t rows,
-                                               int64_t l0, int64_t l1, float (&v)[PER]) {
-    const float* p = static_cast<const float*>(o.p);
-#pragma unroll
-    for (int e = 0; e < PER / V; ++e) {
-      int r, l;
-      place(o.mn, e, &r, &l);
-      const int64_t i = r0 + r, ll = l0 + l;
-      const float* from = p + (o.mn ? ll * o.ld + i : i * o.ld + ll);
-      const int64_t left = i < rows && ll < l1 ? (o.mn ? rows - i : l1 - ll) : 0;
-      if (V == 4 && left >= 4) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(from));
-        v[V * e] = x.x;
-        v[V * e + 1 % V] = x.y;
-        v[V * e + 2 % V] = x.z;
-        v[V * e + 3 % V] = x.w;
-      } else {
-#pragma unroll
-        for (int x = 0; x < V; ++x) v[V * e + x] = x < left ? __ldg(from + x) : 0.f;
-      }
-    }
-  }
-  static __device__ __forceinline__ void put(bool mn, float (*s)[T + 4], const float (&v)[PER]) {
-#pragma unroll
-    for (int e = 0; e < PER / V; ++e) {
-      int r, l;
-      place(mn, e, &r, &l);
-      if (V == 4 && mn) {
-        *reinterpret_cast<float4*>(&s[l][r]) =
-            make_float4(v[V * e], v[V * e + 1 % V], v[V * e + 2 % V], v[V * e + 3 % V]);
-      } else {
-#pragma unroll
-        for (int x = 0; x < V; ++x) {
-          if (mn) s[l][r + x] = v[V * e + x];
-          else s[l + x][r] = v[V * e + x];
-        }
-      }
-    }
-  }
-};
-
 // C tile of 16 R x 16 R, 256 threads with R x R sums each (R / 4 groups of four rows and columns,
 // 64 apart, so that the shared-memory reads are 16-byte and conflict-free). VA, VB: elements of an
 // access to each operand. 12,001 x 1024 x 1024, the three products of a training step: 668 us on
@@ -209,8 +147,6 @@ __global__ void __launch_bounds__(256, 2)
     gemm_f32_kernel(Operand a, Operand b, int64_t m, int64_t n, int64_t k, int64_t k_part,
                     Epilogue ep) {
   constexpr int T = 16 * R;
-  using SA = Stage<T, VA>;
-  using SB = Stage<T, VB>;
   __shared__ __align__(16) float sa[2][FK][T + 4];
   __shared__ __align__(16) float sb[2][FK][T + 4];
   const int tid = threadIdx.x;
@@ -220,50 +156,8 @@ __global__ void __launch_bounds__(256, 2)
   const int64_t i0 = (int64_t)(blockIdx.x / across) * T, j0 = (int64_t)(blockIdx.x % across) * T;
   const int64_t k0 = (int64_t)blockIdx.y * k_part;
   const int64_t k1 = k0 + k_part < k ? k0 + k_part : k;
-  float ra[SA::PER], rb[SB::PER];
-  uint64_t acc[R][R / 2];  // two neighbouring columns each
-#pragma unroll
-  for (int i = 0; i < R; ++i)
-#pragma unroll
-    for (int j = 0; j < R / 2; ++j) acc[i][j] = 0;
-  SA::fetch(a, i0, m, k0, k1, ra);
-  SB::fetch(b, j0, n, k0, k1, rb);
-  SA::put(a.mn, sa[0], ra);
-  SB::put(b.mn, sb[0], rb);
-  __syncthreads();
-  int buf = 0;
-  for (int64_t l0 = k0; l0 < k1; l0 += FK, buf ^= 1) {
-    const bool more = l0 + FK < k1;
-    if (more) {
-      SA::fetch(a, i0, m, l0 + FK, k1, ra);
-      SB::fetch(b, j0, n, l0 + FK, k1, rb);
-    }
-#pragma unroll
-    for (int l = 0; l < FK; ++l) {
-      uint64_t av[R], bv[R / 2];
-#pragma unroll
-      for (int q = 0; q < R / 4; ++q) {
-        const float4 x = *reinterpret_cast<const float4*>(&sa[buf][l][64 * q + 4 * ty]);
-        av[4 * q] = twice(x.x);
-        av[4 * q + 1] = twice(x.y);
-        av[4 * q + 2] = twice(x.z);
-        av[4 * q + 3] = twice(x.w);
-        const ulonglong2 y =
-            *reinterpret_cast<const ulonglong2*>(&sb[buf][l][64 * q + 4 * tx]);
-        bv[2 * q] = y.x;
-        bv[2 * q + 1] = y.y;
-      }
-#pragma unroll
-      for (int i = 0; i < R; ++i)
-#pragma unroll
-        for (int j = 0; j < R / 2; ++j) fma_pair(acc[i][j], av[i], bv[j]);
-    }
-    if (more) {
-      SA::put(a.mn, sa[buf ^ 1], ra);
-      SB::put(b.mn, sb[buf ^ 1], rb);
-      __syncthreads();
-    }
-  }
+  uint64_t acc[R][R / 2];
+  tile_f32<R, VA, VB>(a, i0, m, b, j0, n, k0, k1, sa, sb, acc);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int64_t row = i0 + 64 * (i / 4) + 4 * ty + i % 4;
@@ -421,47 +315,6 @@ int pad_rows(const Pad* pads, int count, int es, cudaStream_t s) {
   return SV_OK;
 }
 
-// dz is rounded to the feature type, since the tensor cores take it as an operand of both products: half
-// a step more beside the result's own (0.0023 against 0.0017 over the gradients of 12,001 x 1024 x 1024
-// bf16). fp16's is raised by a power of two first, and the products' column scales take that back: below 2^-14 a half has no 11 bits, and the gradients of a mean loss lie there. The power puts the
-// largest |dy| below 2^15 (the activations' slopes are below 1.13), so values down to 2^-28 of it keep
-// all their bits. It costs a pass over dy: 12,001 x 1024 in 7 us.
-struct Raise {
-  unsigned* top;  // bits of the largest |dy|, as a half; null: dz is not raised
-  float* down;    // [k]: what the products are multiplied by
-  int64_t k;
-};
-__device__ __forceinline__ float raise_of(unsigned top) {
-  if (top == 0u || top >= 0x7c00u) return 1.0f;  // nothing, or not a number
-  const float x = __half2float(__ushort_as_half((unsigned short)top));
-  return __uint_as_float((268u - (__float_as_uint(x) >> 23)) << 23);  // 2^14 <= x * this < 2^15
-}
-
-template <int V>
-__global__ void __launch_bounds__(256)
-    top_kernel(const unsigned short* __restrict__ x, int64_t cells, unsigned* __restrict__ top) {
-  unsigned most = 0u;  // of both halves of a word
-  const int64_t step = (int64_t)gridDim.x * 256 * V;
-#pragma unroll 4
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < cells; i += step) {
-    if constexpr (V == 8) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + i));
-      most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
-                                     __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
-    } else {
-      most = __vmaxu2(most, x[i] & 0x7fffu);
-    }
-  }
-  __shared__ unsigned s_top[8];
-  const unsigned one = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
-  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = one;
-  __syncthreads();
-  if (threadIdx.x < 32) {  // one atomic a block: one a warp took 11 us
-    const unsigned all = __reduce_max_sync(0xffffffffu, threadIdx.x < 8 ? s_top[threadIdx.x] : 0u);
-    if (threadIdx.x == 0 && all) atomicMax(top, all);
-  }
-}
-
 // dz = dy * act'(z), rows `ld` apart, and the column sums of dz: a block takes 32 V columns (V to a
 // thread) of a strip of rows, eight rows at a time, and writes one row of `partial` for its strip.
 // dz and partial may be null. A pass over 8 bytes of bf16 and fp32 an element (12,001 x 1024: 18 us,
@@ -592,15 +445,8 @@ template <typename T>
 int dz_typed(const void* dy, const float* z, int64_t m, int64_t n, int act, void* dz, int64_t ld,
              void* db, float* partial, const Raise& raise, cudaStream_t s) {
   if (raise.top) {
-    SV_CUDA_TRY(cudaMemsetAsync(raise.top, 0, sizeof(unsigned), s));
-    const unsigned short* x = static_cast<const unsigned short*>(dy);
-    const int64_t cells = m * n;
-    const bool wide = cells % 8 == 0 && aligned16(dy);
-    const unsigned blocks = (unsigned)std::min<int64_t>(
-        (cells / (wide ? 8 : 1) + 255) / 256, (int64_t)num_sms() * 8);
-    if (wide) top_kernel<8><<<blocks, 256, 0, s>>>(x, cells, raise.top);
-    else top_kernel<1><<<blocks, 256, 0, s>>>(x, cells, raise.top);
-    SV_LAUNCH_CHECK();
+    const int rc = find_top<false>(dy, m * n, raise.top, s);
+    if (rc != SV_OK) return rc;
   }
   const bool vec = n % 4 == 0 && aligned16(dy) && aligned16(z) && aligned16(dz);
   const T* g = static_cast<const T*>(dy);
