@@ -405,7 +405,7 @@ typedef struct sv_rows {
  * N: LayerNorm without its weights where `layer` is set, else the root-mean-square norm. x, branch, h, y:
  * [n, channels] of `dtype`, h and y contiguous; channels <= 8192. weight, bias, branch_weight: one row
  * (their stride is not read). b = coords[row, 0] (coords [n, 4]) where gate, scale or shift has a
- * stride; a row whose b is outside [0, batch <= 8191) is left without all three and ORs
+ * stride; a row whose b is outside [0, batch <= 4095) is left without all three and ORs
  * SV_DEVICE_BAD_INDEX into `status`. stats: fp32 [n, 4], 16-byte aligned, for the backward pass, or null:
  * mean and rstd of h, then of d. A row whose sum of squares passes fp32's range has an rstd of zero. */
 typedef struct sv_block_norm_args {

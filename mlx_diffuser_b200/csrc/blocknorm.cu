@@ -108,18 +108,49 @@ __device__ __forceinline__ float coef_at(const Coef& c, int64_t b, int col, floa
   return v[0];
 }
 
+// V elements of a row as they are in memory, so that the next row's can be on their way while this one's
+// are worked on.
 template <typename T, int V>
-__device__ __forceinline__ void load_row(const T* p, float (&v)[V]) {
-  if constexpr (V == 8) {
-    alignas(16) T e[8];
+struct Raw {
+  alignas(V == 8 ? 16 : sizeof(T)) T e[V];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (V == 8) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(e) / 16; ++i)
-      reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
-  } else {
-    v[0] = to_f32(*p);
+      for (int i = 0; i < (int)sizeof(e) / 16; ++i)
+        reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+      e[0] = __ldg(p);
+    }
   }
+  __device__ __forceinline__ void clear() {
+    if constexpr (V == 8) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(e) / 16; ++i)
+        reinterpret_cast<uint4*>(e)[i] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      e[0] = from_f32<T>(0.0f);
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f32(e[i]);
+  }
+};
+
+template <typename T, int V, int J, int TPR>
+__device__ __forceinline__ void load_row(Raw<T, V> (&raw)[J], const void* p, int64_t at, bool in,
+                                         int channels, int t) {
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int c = (j * TPR + t) * V;
+    if (in && c < channels) raw[j].load(static_cast<const T*>(p) + at + c);
+    else raw[j].clear();
+  }
+}
+template <typename T, int V, int J>
+__device__ __forceinline__ void unpack_row(const Raw<T, V> (&raw)[J], float (&v)[J][V]) {
+#pragma unroll
+  for (int j = 0; j < J; ++j) raw[j].unpack(v[j]);
 }
 
 template <typename T, int V>
@@ -139,35 +170,46 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[V]) {
 template <int TPR>
 constexpr int kThreads = TPR > 128 ? TPR : 128;
 
-// Sums over the TPR threads of a row, the same in all of them. Rows of more than a warp meet in
-// `part`, two buffers in turn: the next sum but one writes a buffer again only after every thread has
+// Sums of W values over the TPR threads of a row, the same in all of them. Rows of more than a warp meet
+// in `part`, two buffers in turn: the next sum but one writes a buffer again only after every thread has
 // passed the barrier in between, so one barrier a sum is enough.
 template <int TPR>
 struct RowSum {
   float2* part;  // [2][warps of the block]
   int turn;
-  __device__ __forceinline__ float2 operator()(float a, float b) {
+  template <int W>
+  __device__ __forceinline__ void add(float (&v)[W]) {
 #pragma unroll
-    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int w = 0; w < W; ++w) v[w] += __shfl_xor_sync(0xffffffffu, v[w], o);
     if constexpr (TPR > 32) {
-      constexpr int ALL = kThreads<TPR> / 32, W = TPR / 32;
+      constexpr int ALL = kThreads<TPR> / 32, WARPS = TPR / 32;
       float2* to = part + turn * ALL;
       turn ^= 1;
       const int warp = threadIdx.x >> 5;
-      if ((threadIdx.x & 31) == 0) to[warp] = make_float2(a, b);
+      if ((threadIdx.x & 31) == 0) to[warp] = make_float2(v[0], v[W - 1]);
       __syncthreads();
-      const int first = warp / W * W;
-      a = b = 0.0f;
+      const int first = warp / WARPS * WARPS;
+      float2 all = to[first];
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        a += to[first + i].x;
-        b += to[first + i].y;
+      for (int i = 1; i < WARPS; ++i) {
+        all.x += to[first + i].x;
+        all.y += to[first + i].y;
       }
+      v[W - 1] = all.y;
+      v[0] = all.x;
     }
-    return make_float2(a, b);
+  }
+  __device__ __forceinline__ float one(float a) {
+    float v[1] = {a};
+    add(v);
+    return v[0];
+  }
+  __device__ __forceinline__ float2 two(float a, float b) {
+    float v[2] = {a, b};
+    add(v);
+    return make_float2(v[0], v[1]);
   }
 };
 
@@ -177,19 +219,25 @@ __device__ __forceinline__ int column(int j, int t) {
   return (j * TPR + t) * V;
 }
 
-template <typename T, int V, int J>
-__device__ __forceinline__ void drop_row(float (&v)[J][V], int64_t row, int channels, int t, int tpr,
+// Which of a thread's elements are kept, bit i of word j: the V elements of access j.
+template <int V, int J, int TPR>
+__device__ __forceinline__ void kept_row(uint32_t (&kept)[J], int64_t row, int channels, int t,
                                          uint64_t seed, const Dropout& d) {
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    const int c = (j * tpr + t) * V;
+    const int c = (j * TPR + t) * V;
+    kept[j] = 0u;
     if (c >= channels) continue;
     const uint64_t at = (uint64_t)row * channels + c;
-    if constexpr (V == 8)
-      drop_eight(v[j], philox(at >> 3, d.subsequence, seed), d);
-    else
-      v[j][0] = drop_one(v[j][0], at, seed, d);
+    kept[j] = V == 8 ? kept_eight(philox(at >> 3, d.subsequence, seed), d) : kept_one(at, seed, d);
   }
+}
+template <int V, int J>
+__device__ __forceinline__ void drop_row(float (&v)[J][V], const uint32_t (&kept)[J], float scale) {
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[j][i] = kept[j] >> i & 1u ? v[j][i] * scale : 0.0f;
 }
 
 // mean and rstd of a row in registers (zeros behind the last channel).
@@ -204,7 +252,7 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[J][V], int t, int c
     for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) s += v[j][i];
-    mean = sum(s, 0.0f).x * inv;
+    mean = sum.one(s) * inv;
   }
   float q = 0.0f;
 #pragma unroll
@@ -213,7 +261,7 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[J][V], int t, int c
 #pragma unroll
       for (int i = 0; i < V; ++i) q = fmaf(v[j][i] - mean, v[j][i] - mean, q);
     }
-  return make_float2(mean, rsqrtf(fmaf(sum(q, 0.0f).x, inv, eps)));
+  return make_float2(mean, rsqrtf(fmaf(sum.one(q), inv, eps)));
 }
 
 __device__ __forceinline__ int64_t batch_of(const BlockArgs& a, int64_t row) {
@@ -226,30 +274,34 @@ template <typename T, int V, int J, int TPR>
 __global__ void __launch_bounds__(kThreads<TPR>)
     block_norm_kernel(const __grid_constant__ BlockArgs a) {
   constexpr int ROWS = kThreads<TPR> / TPR;
-  constexpr bool KEEP = J == 1;  // the coefficients of a batch element stay in registers
+  // up to two accesses a thread: the coefficients of a batch element stay in registers, and the next row
+  // is loaded while this one is worked on
+  constexpr bool KEEP = J <= 2;
   __shared__ float2 part[2 * kThreads<TPR> / 32];
   RowSum<TPR> sum{part, 0};
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int C = a.channels;
   const uint64_t seed = a.drop.cut ? seed_of(a.drop) : 0;
   float gg[J][V], mul[J][V], add[J][V];
-  int64_t held = -2;
-  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.n; r0 += (int64_t)gridDim.x * ROWS) {
+  int64_t held = -2, b_next = -2;
+  Raw<T, V> raw_x[J], raw_d[J];
+  auto fetch = [&](int64_t row) {
+    const bool in = row < a.n;
+    load_row<T, V, J, TPR>(raw_x, a.x, row * a.x_stride, in, C, t);
+    load_row<T, V, J, TPR>(raw_d, a.branch, row * a.branch_stride, in, C, t);
+    if (in) b_next = batch_of(a, row);
+  };
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  if constexpr (KEEP) fetch((int64_t)blockIdx.x * ROWS + group);
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.n; r0 += step) {
     const int64_t row = r0 + group;
     const bool in = row < a.n;
     float x[J][V], d[J][V];
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int c = column<V, TPR>(j, t);
-      if (in && c < C) {
-        load_row<T, V>(static_cast<const T*>(a.x) + row * a.x_stride + c, x[j]);
-        load_row<T, V>(static_cast<const T*>(a.branch) + row * a.branch_stride + c, d[j]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[j][i] = d[j][i] = 0.0f;
-      }
-    }
-    const int64_t b = in ? batch_of(a, row) : held;
+    if constexpr (!KEEP) fetch(row);
+    unpack_row(raw_x, x);
+    unpack_row(raw_d, d);
+    const int64_t b = in ? b_next : held;
+    if constexpr (KEEP) fetch(row + step);
     if (b == -1 && in && t == 0) report(a.status, SV_DEVICE_BAD_INDEX);
     // a row without a batch element is not modulated
     auto coefs = [&](int j, float (&g)[V], float (&m)[V], float (&s)[V]) {
@@ -277,7 +329,11 @@ __global__ void __launch_bounds__(kThreads<TPR>)
 #pragma unroll
       for (int j = 0; j < J; ++j) coefs(j, gg[j], mul[j], add[j]);
     }
-    if (a.drop.cut && in) drop_row<T, V, J>(d, row, C, t, TPR, seed, a.drop);
+    if (a.drop.cut) {
+      uint32_t kept[J];
+      kept_row<V, J, TPR>(kept, row, C, t, seed, a.drop);
+      drop_row<V, J>(d, kept, a.drop.scale);
+    }
     float2 sd = make_float2(0.0f, 1.0f);
     if (a.branch_norm) sd = row_stats<V, J, TPR>(d, t, C, a.layer, a.eps, sum);
 #pragma unroll
@@ -313,7 +369,7 @@ template <typename T, int V, int J, int TPR>
 __global__ void __launch_bounds__(kThreads<TPR>)
     block_norm_backward_kernel(const __grid_constant__ BackArgs a) {
   constexpr int THREADS = kThreads<TPR>, ROWS = THREADS / TPR;
-  constexpr bool KEEP = J == 1;
+  constexpr bool KEEP = J <= 2;
   __shared__ float2 part[2 * THREADS / 32];
   __shared__ float joined[ROWS > 1 ? THREADS * V * J : 1];
   RowSum<TPR> sum{part, 0};
@@ -349,7 +405,10 @@ __global__ void __launch_bounds__(kThreads<TPR>)
       m[i] = w[i] * (1.0f + m[i]);
     }
   };
-  if constexpr (KEEP) coefs(0, gg[0], mul[0]);
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) coefs(j, gg[j], mul[j]);
+  }
   float sum_a[J][V], sum_b[J][V], sum_e[J][V];
 #pragma unroll
   for (int j = 0; j < J; ++j)
@@ -357,30 +416,47 @@ __global__ void __launch_bounds__(kThreads<TPR>)
     for (int i = 0; i < V; ++i) sum_a[j][i] = sum_b[j][i] = sum_e[j][i] = 0.0f;
   const float inv = 1.0f / (float)C;
   const bool with_d = f.branch_norm || a.want_e;
+  Raw<T, V> raw_y[J], raw_h[J], raw_d[J], raw_D[J];
+  float4 st_next = make_float4(0.0f, 0.0f, 0.0f, 1.0f);
+  auto row_at = [&](int at) {
+    const int64_t i = min(at, p.last - 1);
+    return a.perm ? (int64_t)__ldg(a.perm + i) : i;
+  };
+  auto fetch = [&](int64_t row, bool in) {
+    load_row<T, V, J, TPR>(raw_y, a.dy, row * C, in && a.dy, C, t);
+    load_row<T, V, J, TPR>(raw_h, f.h, row * C, in, C, t);
+    load_row<T, V, J, TPR>(raw_d, f.branch, row * f.branch_stride, in && with_d, C, t);
+    load_row<T, V, J, TPR>(raw_D, a.dh, row * C, in && a.dh, C, t);
+    st_next = in ? __ldg(f.stats + row) : make_float4(0.0f, 0.0f, 0.0f, 1.0f);
+  };
+  int64_t row_next = row_at(p.first + group), row_after = 0;
+  if constexpr (KEEP) {
+    row_after = row_at(p.first + ROWS + group);
+    fetch(row_next, p.first + group < p.last);
+  }
   for (int r0 = p.first; r0 < p.last; r0 += ROWS) {
     const bool in = r0 + group < p.last;
-    int64_t row = in ? r0 + group : r0;
-    if (a.perm) row = __ldg(a.perm + row);
-    float4 st = make_float4(0.0f, 0.0f, 0.0f, 1.0f);
-    if (in) st = __ldg(f.stats + row);
+    if constexpr (!KEEP) {
+      row_next = row_at(r0 + group);
+      fetch(row_next, in);
+    }
+    const int64_t row = row_next;
+    const float4 st = st_next;
     float dy[J][V], n[J][V], d[J][V], D[J][V];
-    auto get = [&](const void* from, int64_t stride, float (&v)[J][V]) {
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int c = column<V, TPR>(j, t);
-        if (in && c < C && from) {
-          load_row<T, V>(static_cast<const T*>(from) + row * stride + c, v[j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[j][i] = 0.0f;
-        }
-      }
-    };
-    get(a.dy, C, dy);
-    get(f.h, C, n);
-    get(with_d ? f.branch : nullptr, f.branch_stride, d);
-    get(a.dh, C, D);
-    if (f.drop.cut && in && with_d) drop_row<T, V, J>(d, row, C, t, TPR, seed, f.drop);
+    unpack_row(raw_y, dy);
+    unpack_row(raw_h, n);
+    unpack_row(raw_d, d);
+    unpack_row(raw_D, D);
+    if constexpr (KEEP) {
+      row_next = row_after;
+      fetch(row_next, r0 + ROWS + group < p.last);
+      row_after = row_at(r0 + 2 * ROWS + group);
+    }
+    uint32_t kept[J];  // for the branch and for its gradient
+    if (f.drop.cut) {
+      kept_row<V, J, TPR>(kept, row, C, t, seed, f.drop);
+      drop_row<V, J>(d, kept, f.drop.scale);
+    }
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -396,8 +472,8 @@ __global__ void __launch_bounds__(kThreads<TPR>)
         s2 = fmaf(dy[j][i], n[j][i], s2);
       }
     }
-    const float2 m = sum(s1, s2);
-    const float m1 = f.layer ? m.x * inv : 0.0f, m2 = m.y * inv;
+    const float2 m = f.layer ? sum.two(s1, s2) : make_float2(0.0f, sum.one(s2));
+    const float m1 = m.x * inv, m2 = m.y * inv;
     s1 = s2 = 0.0f;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -414,20 +490,22 @@ __global__ void __launch_bounds__(kThreads<TPR>)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         D[j][i] *= gg[KEEP ? j : 0][i];
-        s1 += D[j][i];
-        s2 = fmaf(D[j][i], d[j][i], s2);
+        if (f.branch_norm) {
+          s1 += D[j][i];
+          s2 = fmaf(D[j][i], d[j][i], s2);
+        }
       }
     }
     if (f.branch_norm) {
-      const float2 e = sum(s1, s2);
-      const float e1 = f.layer ? e.x * inv : 0.0f, e2 = e.y * inv;
+      const float2 e = f.layer ? sum.two(s1, s2) : make_float2(0.0f, sum.one(s2));
+      const float e1 = e.x * inv, e2 = e.y * inv;
 #pragma unroll
       for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) D[j][i] = st.w * (D[j][i] - e1 - d[j][i] * e2);
     }
     if (in && a.dbranch) {
-      if (f.drop.cut) drop_row<T, V, J>(D, row, C, t, TPR, seed, f.drop);
+      if (f.drop.cut) drop_row<V, J>(D, kept, f.drop.scale);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int c = column<V, TPR>(j, t);
@@ -473,9 +551,8 @@ struct Grad {
 };
 struct SumArgs {
   BlockArgs f;
-  const int32_t* offsets;
-  int piece;
-  const float* partial;
+  int groups;         // batch elements, and one for the rows without
+  const float* sums;  // [groups][3][C]
   Grad weight, bias, branch_weight, gate, scale, shift;
 };
 
@@ -486,48 +563,54 @@ __device__ __forceinline__ void store_grad(const Grad& g, int64_t b, int c, floa
   else static_cast<__nv_bfloat16*>(g.p)[at] = __float2bfloat16_rn(v);
 }
 
-// 32 channels a block; its 32 warps share a batch element's pieces and are joined in order.
+// The sums of a batch element's pieces (blockIdx.y), 32 of the 3 C columns a block: its 32 warps share the
+// pieces and are joined in order.
 __global__ void __launch_bounds__(1024)
-    block_norm_sums_kernel(const __grid_constant__ SumArgs a) {
-  __shared__ float s[3][32][33];
-  const BlockArgs& f = a.f;
+    block_norm_join_kernel(const float* partial, const int32_t* offsets, int64_t n, int batch,
+                           int piece, int64_t cols, float* out) {
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane, C = f.channels;
-  const bool in = c < C;
-  float dw = 0.0f, dbeta = 0.0f, dwb = 0.0f, dgate = 0.0f, dscale = 0.0f, dshift = 0.0f;
-  const float w = in ? coef_at(f.weight, 0, c, 1.0f) : 0.0f;
-  const float beta = in ? coef_at(f.bias, 0, c, 0.0f) : 0.0f;
-  const float wb = in ? coef_at(f.branch_weight, 0, c, 1.0f) : 0.0f;
-  int64_t first = 0;
-  const int groups = a.offsets ? (int)f.batch + 1 : 1;
-  for (int g = 0; g < groups; ++g) {
-    int64_t rows = f.n;
-    if (a.offsets)
-      rows = (g < f.batch ? (int64_t)a.offsets[g + 1] : f.n) - a.offsets[g];
-    const int64_t pieces = (rows + a.piece - 1) / a.piece;
-    float v0 = 0.0f, v1 = 0.0f, v2 = 0.0f;
-    if (in)
-      for (int64_t p = first + warp; p < first + pieces; p += 32) {
-        const float* from = a.partial + p * 3 * C + c;
-        v0 += __ldg(from);
-        v1 += __ldg(from + C);
-        v2 += __ldg(from + 2 * C);
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  int64_t first = 0, pieces = (n + piece - 1) / piece;
+  if (offsets) {
+    for (int g0 = 0; g0 <= (int)blockIdx.y; g0 += 32) {
+      const int g = g0 + lane;
+      int mine = 0;
+      if (g <= (int)blockIdx.y) {
+        const int rows = (g < batch ? __ldg(offsets + g + 1) : (int)n) - __ldg(offsets + g);
+        mine = (rows + piece - 1) / piece;
       }
-    first += pieces;
-    __syncthreads();  // the previous element's sums have been read
-    s[0][warp][lane] = v0;
-    s[1][warp][lane] = v1;
-    s[2][warp][lane] = v2;
-    __syncthreads();
-    if (warp != 0 || !in) continue;
-    float A = 0.0f, B = 0.0f, E = 0.0f;
-#pragma unroll 8
-    for (int i = 0; i < 32; ++i) {
-      A += s[0][i][lane];
-      B += s[1][i][lane];
-      E += s[2][i][lane];
+      const int all = __reduce_add_sync(0xffffffffu, g < (int)blockIdx.y ? mine : 0);
+      first += all;
+      pieces = __reduce_add_sync(0xffffffffu, g == (int)blockIdx.y ? mine : 0);
     }
-    const bool mod = !a.offsets || g < f.batch;  // rows without a batch element are not modulated
+  }
+  float v = 0.0f;
+  if (c < cols) {
+    const float* from = partial + (first + warp) * cols + c;
+#pragma unroll 8
+    for (int64_t p = warp; p < pieces; p += 32, from += 32 * cols) v += __ldg(from);
+  }
+  s[warp][lane] = v;
+  __syncthreads();
+  if (warp != 0 || c >= cols) return;
+#pragma unroll
+  for (int i = 1; i < 32; ++i) v += s[i][lane];
+  out[blockIdx.y * cols + c] = v;
+}
+
+// A channel a thread, the batch elements in order.
+__global__ void __launch_bounds__(64) block_norm_sums_kernel(const __grid_constant__ SumArgs a) {
+  const BlockArgs& f = a.f;
+  const int c = blockIdx.x * 64 + threadIdx.x, C = f.channels;
+  if (c >= C) return;
+  float dw = 0.0f, dbeta = 0.0f, dwb = 0.0f, dgate = 0.0f, dscale = 0.0f, dshift = 0.0f;
+  const float w = coef_at(f.weight, 0, c, 1.0f), beta = coef_at(f.bias, 0, c, 0.0f);
+  const float wb = coef_at(f.branch_weight, 0, c, 1.0f);
+  for (int g = 0; g < a.groups; ++g) {
+    const float* from = a.sums + (int64_t)g * 3 * C + c;
+    const float A = __ldg(from), B = __ldg(from + C), E = __ldg(from + 2 * C);
+    const bool mod = !f.per_batch || g < f.batch;  // rows without a batch element are not modulated
     const float one = 1.0f + (mod ? coef_at(f.scale, g, c, 0.0f) : 0.0f);
     const float gate = mod ? coef_at(f.gate, g, c, 1.0f) : 1.0f;
     dw = fmaf(one, A, dw);
@@ -542,7 +625,6 @@ __global__ void __launch_bounds__(1024)
     dscale += es;
     dshift += B;
   }
-  if (warp != 0 || !in) return;
   if (a.weight.p) store_grad(a.weight, 0, c, dw);
   if (a.bias.p) store_grad(a.bias, 0, c, dbeta);
   if (a.branch_weight.p) store_grad(a.branch_weight, 0, c, dwb);
@@ -582,15 +664,16 @@ int launch_backward(const BackArgs& a, unsigned blocks, cudaStream_t s) {
   return SV_OK;
 }
 
-// A row's threads: as few as hold it with eight elements each, so that more rows share a block.
+// A row's threads: as few as hold it with 16 elements each. What a thread does once a row (addresses, the
+// steps of the sums, the loop) is as much as the work on 8 elements.
 #define SV_BLOCK_NORM_PICK(call, C, wide)                                          \
   if (wide) {                                                                      \
     if ((C) <= 64) return call(8, 1, 8);                                           \
-    if ((C) <= 128) return call(8, 1, 16);                                         \
-    if ((C) <= 256) return call(8, 1, 32);                                         \
-    if ((C) <= 512) return call(8, 1, 64);                                         \
-    if ((C) <= 1024) return call(8, 1, 128);                                       \
-    if ((C) <= 2048) return call(8, 1, 256);                                       \
+    if ((C) <= 128) return call(8, 2, 8);                                          \
+    if ((C) <= 256) return call(8, 2, 16);                                         \
+    if ((C) <= 512) return call(8, 2, 32);                                         \
+    if ((C) <= 1024) return call(8, 2, 64);                                        \
+    if ((C) <= 2048) return call(8, 2, 128);                                       \
     if ((C) <= 4096) return call(8, 2, 256);                                       \
     return call(8, 4, 256);                                                        \
   }                                                                                \
@@ -628,12 +711,13 @@ Pieces pieces_of(int64_t n, int64_t groups) {
 
 struct BackPlan {
   Pieces pieces;
-  size_t perm, offsets, scratch, total;  // `partial` is at the start
+  size_t joined, perm, offsets, scratch, total;  // `partial` is at the start
 };
 BackPlan back_plan(int64_t n, int channels, int64_t groups) {  // groups 0: rows are not sorted
   BackPlan p;
   p.pieces = pieces_of(n, groups ? groups + 1 : 0);
-  p.perm = align_up((size_t)p.pieces.most * 3 * channels * sizeof(float), 256);
+  p.joined = align_up((size_t)p.pieces.most * 3 * channels * sizeof(float), 256);
+  p.perm = p.joined + align_up((size_t)(groups + 1) * 3 * channels * sizeof(float), 256);
   p.offsets = p.perm + (groups ? align_up((size_t)n * sizeof(int32_t), 256) : 0);
   p.scratch = p.offsets + (groups ? align_up((size_t)(groups + 1) * sizeof(int32_t), 256) : 0);
   p.total = p.scratch + (groups ? group_rows_bytes(n, (int)groups) : 0);
@@ -800,11 +884,15 @@ extern "C" int sv_block_norm_backward(const sv_block_norm_args* args, const void
     if (bad != SV_OK) return bad;
   }
   if (!sums) return SV_OK;
+  const int64_t cols = 3 * (int64_t)f.channels;
   SumArgs g{};
   g.f = f;
-  g.offsets = a.offsets;
-  g.piece = a.piece;
-  g.partial = a.partial;
+  g.groups = f.per_batch ? (int)f.batch + 1 : 1;
+  float* joined = reinterpret_cast<float*>(ws + plan.joined);
+  g.sums = joined;
+  block_norm_join_kernel<<<dim3((unsigned)((cols + 31) / 32), (unsigned)g.groups), 1024, 0, s>>>(
+      a.partial, a.offsets, f.n, (int)f.batch, a.piece, cols, joined);
+  SV_LAUNCH_CHECK();
   g.weight = to_grad(grads->weight);
   g.bias = to_grad(grads->bias);
   g.branch_weight = to_grad(grads->branch_weight);
@@ -812,7 +900,7 @@ extern "C" int sv_block_norm_backward(const sv_block_norm_args* args, const void
   g.scale = to_grad(grads->scale);
   g.shift = to_grad(grads->shift);
   g.weight.stride = g.bias.stride = g.branch_weight.stride = 0;
-  block_norm_sums_kernel<<<(unsigned)((f.channels + 31) / 32), 1024, 0, s>>>(g);
+  block_norm_sums_kernel<<<(unsigned)((f.channels + 63) / 64), 64, 0, s>>>(g);
   SV_LAUNCH_CHECK();
   return SV_OK;
 }

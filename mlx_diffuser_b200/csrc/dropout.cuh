@@ -53,22 +53,34 @@ __device__ __forceinline__ uint4 philox(uint64_t group, uint64_t subsequence, ui
   return make_uint4(c0, c1, c2, c3);
 }
 
-// v[0..7], the elements of one counter: scaled, or zero whatever they were.
-__device__ __forceinline__ void drop_eight(float (&v)[8], const uint4& r, const Dropout& d) {
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+// Bit i: element i of the counter's eight is kept. A half is compared where it stands, in a word's upper
+// half: the lower bits of the word cannot change the comparison with cut 2^16.
+__device__ __forceinline__ uint32_t kept_eight(const uint4& r, const Dropout& d) {
+  if (d.cut >= 65536u) return 0u;
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w}, cut = d.cut << 16;
+  uint32_t kept = 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[2 * i] = (w[i] & 0xffffu) >= d.cut ? v[2 * i] * d.scale : 0.0f;
-    v[2 * i + 1] = (w[i] >> 16) >= d.cut ? v[2 * i + 1] * d.scale : 0.0f;
+    kept |= (w[i] << 16) >= cut ? 1u << 2 * i : 0u;
+    kept |= w[i] >= cut ? 2u << 2 * i : 0u;
+  }
+  return kept;
+}
+
+// v[0..7], the elements of one counter: scaled, or zero whatever they were.
+__device__ __forceinline__ void drop_eight(float (&v)[8], const uint4& r, const Dropout& d) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w}, cut = d.cut << 16;
+  const bool none = d.cut >= 65536u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = (w[i] << 16) >= cut && !none ? v[2 * i] * d.scale : 0.0f;
+    v[2 * i + 1] = w[i] >= cut && !none ? v[2 * i + 1] * d.scale : 0.0f;
   }
 }
 
-// One element by itself, number `at`.
-__device__ __forceinline__ float drop_one(float v, uint64_t at, uint64_t seed, const Dropout& d) {
-  const uint4 r = philox(at >> 3, d.subsequence, seed);
-  const uint32_t half = (uint32_t)at & 7u;
-  const uint32_t w = half < 2 ? r.x : half < 4 ? r.y : half < 6 ? r.z : r.w;
-  return (half & 1u ? w >> 16 : w & 0xffffu) >= d.cut ? v * d.scale : 0.0f;
+// Whether element `at` by itself is kept.
+__device__ __forceinline__ uint32_t kept_one(uint64_t at, uint64_t seed, const Dropout& d) {
+  return kept_eight(philox(at >> 3, d.subsequence, seed), d) >> ((uint32_t)at & 7u) & 1u;
 }
 #endif
 

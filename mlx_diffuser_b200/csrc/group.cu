@@ -1,8 +1,7 @@
 // Stable counting sort of rows by a small key.
 //
 // Every warp takes a contiguous run of rows ("part"). Three steps: a histogram per part, an exclusive
-// scan over the histograms with the bins outermost (so that a bin's parts follow each other in the rows'
-// order), and the scatter, in which a warp ranks 32 rows at a time among those with the same key.
+// scan over each bin's parts (a bin's parts follow each other in the rows' order), and the scatter, in which a warp ranks 32 rows at a time among those with the same key.
 // Nothing depends on the order of execution. Few rows take one launch of one block, more take three:
 // the launches are what bounds the small ones (8 to 16 thousand rows: the block of 32 warps walks 512
 // rows a warp at about 0.1 us for 32).
@@ -14,7 +13,7 @@ namespace sv {
 namespace {
 
 constexpr int GROUP_WARPS = 8;
-constexpr int SMEM_COUNTS = 11 * 1024;  // counters of a block: 44 KB of shared memory
+constexpr int SMEM_COUNTS = 12 * 1024;  // counters of a block: 48 KB of shared memory
 
 __device__ __forceinline__ int bin_of(int32_t key, int groups) {
   return key >= 0 && key < groups ? key : groups;
@@ -127,21 +126,64 @@ __global__ void __launch_bounds__(GROUP_WARPS * 32)
   }
 }
 
-__global__ void __launch_bounds__(1024) group_scan_kernel(int32_t* counts, int total, int parts,
-                                                          int groups, int32_t* offsets) {
-  __shared__ int32_t part[32];
-  scan_block(counts, total, part);
-  for (int g = threadIdx.x; g <= groups; g += 1024) offsets[g] = counts[(int64_t)g * parts];
+// Exclusive sums over a bin's parts in place, a block a bin, and the bin's total.
+__global__ void __launch_bounds__(256) group_scan_kernel(int32_t* counts, int parts, int32_t* totals) {
+  __shared__ int32_t part[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int32_t* mine = counts + (int64_t)blockIdx.x * parts;
+  int before = 0;
+  for (int i0 = 0; i0 < parts; i0 += 256) {
+    const int i = i0 + tid;
+    const int c = i < parts ? mine[i] : 0;
+    int upto = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    __syncthreads();  // the previous round's sums have been read
+    if (lane == 31) part[warp] = upto;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if (w == warp) upto += all;
+      all += part[w];
+    }
+    if (i < parts) mine[i] = before + upto - c;
+    before += all;
+  }
+  if (tid == 0) totals[blockIdx.x] = before;
 }
 
 __global__ void __launch_bounds__(GROUP_WARPS * 32)
     group_place_kernel(const int32_t* keys, int64_t stride, int64_t n, int64_t per, int groups,
-                       int parts, const int32_t* counts, int32_t* perm, int32_t* place) {
+                       int parts, const int32_t* counts, const int32_t* totals, int32_t* offsets,
+                       int32_t* perm, int32_t* place) {
   extern __shared__ int32_t mine[];
   const int bins = groups + 1, warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
+  int32_t* base = mine + bins * warps;  // where each bin starts
+  if (warp == 0) {
+    int before = 0;
+    for (int b0 = 0; b0 < bins; b0 += 32) {
+      const int b = b0 + (int)threadIdx.x, c = b < bins ? __ldg(totals + b) : 0;
+      int upto = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if ((int)threadIdx.x >= o) upto += v;
+      }
+      if (b < bins) {
+        base[b] = before + upto - c;
+        if (blockIdx.x == 0) offsets[b] = before + upto - c;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  __syncthreads();
   for (int i = threadIdx.x; i < bins * warps; i += blockDim.x) {
     const int bin = i / warps, w = i - bin * warps;
-    mine[w * bins + bin] = counts[(int64_t)bin * parts + blockIdx.x * warps + w];
+    mine[w * bins + bin] = base[bin] + counts[(int64_t)bin * parts + blockIdx.x * warps + w];
   }
   __syncthreads();
   const int64_t p = (int64_t)blockIdx.x * warps + warp;
@@ -158,12 +200,13 @@ struct GroupPlan {
 GroupPlan group_plan(int64_t n, int groups) {
   const int bins = groups + 1;
   GroupPlan p{};
-  p.small = n <= 16384 && bins * 64 <= SMEM_COUNTS;
+  p.small = n <= 16384 && bins * 64 + 32 <= SMEM_COUNTS;
   if (p.small) return p;
-  p.warps = std::max(1, std::min(GROUP_WARPS, SMEM_COUNTS / bins));
-  // parts of 64 rows at least, no more than two blocks an SM, and a scan of 128 Ki counters at most
-  int64_t parts = std::min<int64_t>((n + 63) / 64, (int64_t)num_sms() * 2 * p.warps);
-  parts = std::max<int64_t>(1, std::min<int64_t>(parts, (128 * 1024) / bins));
+  // a block holds a counter a warp and bin, and a base a bin
+  p.warps = std::max(1, std::min(GROUP_WARPS, SMEM_COUNTS / bins - 1));
+  // parts of 64 rows at least, no more than a block an SM, and a megabyte of counters at most
+  int64_t parts = std::min<int64_t>((n + 63) / 64, (int64_t)num_sms() * p.warps);
+  parts = std::max<int64_t>(1, std::min<int64_t>(parts, (256 * 1024) / bins));
   p.blocks = (int)((parts + p.warps - 1) / p.warps);
   parts = (int64_t)p.blocks * p.warps;
   p.per = ((n + parts - 1) / parts + 31) / 32 * 32;
@@ -174,7 +217,7 @@ GroupPlan group_plan(int64_t n, int groups) {
 
 size_t group_rows_bytes(int64_t n, int groups) {
   const GroupPlan p = group_plan(n, groups);
-  return p.small ? 0 : align_up((size_t)(groups + 1) * p.blocks * p.warps * sizeof(int32_t), 256);
+  return p.small ? 0 : align_up((size_t)(groups + 1) * (p.blocks * p.warps + 1) * sizeof(int32_t), 256);
 }
 
 int group_rows(const int32_t* keys, int64_t stride, int64_t n, int groups, int32_t* perm,
@@ -190,15 +233,16 @@ int group_rows(const int32_t* keys, int64_t stride, int64_t n, int groups, int32
     return SV_OK;
   }
   int32_t* counts = static_cast<int32_t*>(workspace);
-  const size_t bytes = bins * p.warps * sizeof(int32_t);
   const int parts = p.blocks * p.warps;
+  int32_t* totals = counts + bins * parts;
+  const size_t bytes = bins * p.warps * sizeof(int32_t);
   group_count_kernel<<<p.blocks, p.warps * 32, bytes, s>>>(keys, stride, n, p.per, groups, parts,
                                                            counts);
   SV_LAUNCH_CHECK();
-  group_scan_kernel<<<1, 1024, 0, s>>>(counts, (int)(bins * parts), parts, groups, offsets);
+  group_scan_kernel<<<(unsigned)bins, 256, 0, s>>>(counts, parts, totals);
   SV_LAUNCH_CHECK();
-  group_place_kernel<<<p.blocks, p.warps * 32, bytes, s>>>(keys, stride, n, p.per, groups, parts,
-                                                           counts, perm, place);
+  group_place_kernel<<<p.blocks, p.warps * 32, bytes + bins * sizeof(int32_t), s>>>(
+      keys, stride, n, p.per, groups, parts, counts, totals, offsets, perm, place);
   SV_LAUNCH_CHECK();
   return SV_OK;
 }

@@ -6,7 +6,7 @@
 
 namespace sv {
 
-constexpr int GROUP_MAX_BINS = 8192;  // groups, and one more for the rows without one
+constexpr int GROUP_MAX_BINS = 4096;  // groups, and one more for the rows without one
 
 // Bytes that group_rows needs for n rows and `groups` groups.
 size_t group_rows_bytes(int64_t n, int groups);

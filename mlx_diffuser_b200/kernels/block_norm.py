@@ -128,7 +128,7 @@ def block_norm(
     ``bias``, ``branch_weight``: (C,). ``gate``, ``scale``, ``shift``: (B, C) with the row picked by
     ``coords[:, 0]`` of the (rows, 4) int32 coordinates, or (C,) / (1, C) for every row; any of the
     three float types. A row whose batch index is outside ``batch_size`` (by default the largest B, at most
-    8191) is left without gate, scale and shift, and :func:`check_device_status` reports it.
+    4095) is left without gate, scale and shift, and :func:`check_device_status` reports it.
     ``dropout``, ``seed`` and ``subsequence`` are those of :func:`~mlx_diffuser_b200.dropout`.
 
     Gradients for everything but the coordinates and the seed, in fixed orders of summation.

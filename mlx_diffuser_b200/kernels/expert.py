@@ -70,11 +70,14 @@ class _Route(torch.autograd.Function):
         ctx.save_for_backward(logits, experts, weights)
         ctx.normalize = normalize
         ctx.mark_non_differentiable(experts, order, offsets, place)
+        ctx.set_materialize_grads(False)
         return experts, weights, order, offsets, place
 
     @staticmethod
     @once_differentiable
     def backward(ctx, _experts, dweights, *_):
+        if dweights is None:
+            return None, None, None
         logits, experts, weights = ctx.saved_tensors
         n, e = logits.shape
         dev = logits.device
