@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -54,42 +55,11 @@ _I32 = ctypes.c_int
 _SZ = ctypes.c_size_t
 
 
-class Rows(ctypes.Structure):
-    """sv_rows: rows of coefficients in any float type."""
-
-    _fields_ = [("data", _P), ("stride", _I64), ("dtype", _I32)]
-
-
-class BlockNormArgs(ctypes.Structure):
-    """sv_block_norm_args."""
-
-    _fields_ = [
-        ("n", _I64), ("batch", _I64), ("x", _P), ("x_stride", _I64), ("branch", _P),
-        ("branch_stride", _I64), ("h", _P), ("stats", _P), ("coords", _P), ("weight", Rows),
-        ("bias", Rows), ("branch_weight", Rows), ("gate", Rows), ("scale", Rows), ("shift", Rows),
-        ("dropout", ctypes.c_double), ("seed", _U64), ("seed_at", _P), ("subsequence", _U64),
-        ("channels", _I32), ("dtype", _I32), ("layer", _I32), ("branch_norm", _I32),
-        ("residual_scale", ctypes.c_float), ("eps", ctypes.c_float),
-    ]
-
-
-class BlockNormGrads(ctypes.Structure):
-    """sv_block_norm_grads."""
-
-    _fields_ = [(name, Rows) for name in ("weight", "bias", "branch_weight", "gate", "scale", "shift")]
-
-
-class ExpertArgs(ctypes.Structure):
-    """sv_expert_args."""
-
-    _fields_ = [
-        ("n", _I64), ("x", _P), ("ldx", _I64), ("weight", _P), ("ldw", _I64), ("w_expert", _I64),
-        ("bias", _P), ("order", _P), ("offsets", _P), ("place", _P), ("weights", _P),
-        ("preact", _P), ("rows", _P), ("inputs", _I64), ("outputs", _I64), ("k", _I32),
-        ("experts", _I32), ("dtype", _I32), ("activation", _I32), ("gather", _I32),
-        ("combine", _I32),
-    ]
-
+# Structures that entry points take by pointer, packed in one step: sv_rows is data, stride and dtype.
+_ROWS = "Qqi4x"
+BLOCK_NORM_ARGS = struct.Struct("qqQqQqQQQ" + 6 * _ROWS + "dQQQiiiiff")
+BLOCK_NORM_GRADS = struct.Struct(6 * _ROWS)
+EXPERT_ARGS = struct.Struct("qQqQqqQQQQQQQqqiiiiii")
 
 _SIGNATURES = {
     "sv_last_error": (ctypes.c_char_p, []),
@@ -147,11 +117,11 @@ _SIGNATURES = {
     "sv_rms_norm_backward": (
         _I32, [_P, _I64, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _SZ, _P, _P]
     ),
-    "sv_block_norm": (_I32, [ctypes.POINTER(BlockNormArgs), _P, _P, _P]),
+    "sv_block_norm": (_I32, [ctypes.c_char_p, _P, _P, _P]),
     "sv_block_norm_backward_workspace_bytes": (_SZ, [_I64, _I32, _I64]),
     "sv_block_norm_backward": (
         _I32,
-        [ctypes.POINTER(BlockNormArgs), _P, _P, _P, _P, ctypes.POINTER(BlockNormGrads), _P, _SZ,
+        [ctypes.c_char_p, _P, _P, _P, _P, ctypes.c_char_p, _P, _SZ,
          _P],
     ),
     "sv_dropout": (
@@ -175,11 +145,11 @@ _SIGNATURES = {
         _I32, [_P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P]
     ),
     "sv_expert_linear_workspace_bytes": (
-        _SZ, [ctypes.POINTER(ExpertArgs), _I32, _I32, _I32, _P]
+        _SZ, [ctypes.c_char_p, _I32, _I32, _I32, _P]
     ),
-    "sv_expert_linear": (_I32, [ctypes.POINTER(ExpertArgs), _P, _P, _SZ, _P, _P]),
+    "sv_expert_linear": (_I32, [ctypes.c_char_p, _P, _P, _SZ, _P, _P]),
     "sv_expert_linear_backward": (
-        _I32, [ctypes.POINTER(ExpertArgs), _P, _P, _P, _P, _P, _P, _SZ, _P, _P]
+        _I32, [ctypes.c_char_p, _P, _P, _P, _P, _P, _P, _SZ, _P, _P]
     ),
     "sv_window_plan_bytes": (_SZ, [_I64]),
     "sv_window_plan": (_I32, [_P, _P, _P, _I64, _I64, _P, _P, _P]),
@@ -286,6 +256,15 @@ def on_device(device: torch.device):
     if device.index is None or device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(device)
+
+
+def call(device: torch.device, fn, *args) -> int:
+    """``fn(*args)`` with ``device`` as the current CUDA device."""
+
+    if device.index == torch.cuda.current_device():
+        return fn(*args)
+    with on_device(device):
+        return fn(*args)
 
 
 def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:

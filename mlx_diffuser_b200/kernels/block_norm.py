@@ -4,7 +4,6 @@ block's result, gate, residual scale and addition, then the next block's norm wi
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -14,49 +13,47 @@ from .. import _native as N
 from .dropout import check_share, seed_argument
 from .norm import _rows
 
-_COEFS = ("weight", "bias", "branch_weight", "gate", "scale", "shift")
+_NONE = (0, 0, 0)  # an sv_rows without data
 
 
-def _row(t: torch.Tensor | None) -> N.Rows:
-    if t is None:
-        return N.Rows(None, 0, 0)
+def _row(t: torch.Tensor) -> tuple[int, int, int]:
+    """``t`` (C,), (1, C) or (B, C), rows contiguous, as an sv_rows."""
+
     per_batch = t.ndim == 2 and t.shape[0] > 1
-    return N.Rows(t.data_ptr(), t.stride(0) if per_batch else 0, N.DTYPE_CODE[t.dtype])
+    return t.data_ptr(), t.stride(0) if per_batch else 0, N.DTYPE_CODE[t.dtype]
 
 
-def _per_batch(coefs) -> bool:
-    return any(t is not None and t.ndim == 2 and t.shape[0] > 1 for t in coefs)
+class _Call:
+    """What both passes hand to the library beside the tensors of their own."""
+
+    __slots__ = ("n", "c", "code", "batch", "per_batch", "branch_stride", "rows", "p", "seed",
+                 "subsequence", "layer", "branch_norm", "residual_scale", "eps")
+
+    def pack(self, x, x_stride, branch, h, stats, coords, seed_at) -> bytes:
+        return N.BLOCK_NORM_ARGS.pack(
+            self.n, self.batch, x, x_stride, branch.data_ptr(), self.branch_stride, h.data_ptr(),
+            0 if stats is None else stats.data_ptr(), 0 if coords is None else coords.data_ptr(),
+            *self.rows, self.p, self.seed, 0 if seed_at is None else seed_at.data_ptr(),
+            self.subsequence, self.c, self.code, self.layer, self.branch_norm,
+            self.residual_scale, self.eps)
 
 
-def _arguments(branch, h, stats, coords, coefs, o) -> N.BlockNormArgs:
-    n, c = h.shape
-    a = N.BlockNormArgs(
-        n=n, batch=o["batch"], branch=branch.data_ptr(), branch_stride=max(branch.stride(0), c),
-        h=h.data_ptr(), stats=N.ptr(stats), coords=N.ptr(coords), dropout=o["p"], seed=o["seed"],
-        subsequence=o["subsequence"], channels=c, dtype=N.DTYPE_CODE[h.dtype], layer=o["layer"],
-        branch_norm=o["branch_norm"], residual_scale=o["residual_scale"], eps=o["eps"])
-    for name, t in zip(_COEFS, coefs):
-        setattr(a, name, _row(t))
-    return a
-
-
-def _forward(x, branch, coords, seed_at, coefs, o, keep):
-    n, c = x.shape
+def _forward(x, branch, coords, seed_at, o, keep):
+    n, c, dev = o.n, o.c, x.device
     h, y = x.new_empty((n, c)), x.new_empty((n, c))
-    stats = x.new_empty((n, 4), dtype=torch.float32) if keep else None
-    a = _arguments(branch, h, stats, coords, coefs, o)
-    a.x, a.x_stride, a.seed_at = x.data_ptr(), max(x.stride(0), c), N.ptr(seed_at)
-    with N.on_device(x.device):
-        rc = N.load().sv_block_norm(ctypes.byref(a), y.data_ptr(),
-                                    N.status_word(x.device).data_ptr(), N.stream(x.device))
-    N.check(rc, "block_norm")
+    stats = torch.empty((n, 4), dtype=torch.float32, device=dev) if keep else None
+    args = o.pack(x.data_ptr(), max(x.stride(0), c), branch, h, stats, coords, seed_at)
+    rc = N.call(dev, N.load().sv_block_norm, args, y.data_ptr(), N.status_word(dev).data_ptr(),
+                N.stream(dev))
+    if rc:
+        N.check(rc, "block_norm")
     return y, h, stats
 
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, branch, coords, seed_at, o, *coefs):
-        y, h, stats = _forward(x, branch, coords, seed_at, coefs, o, True)
+        y, h, stats = _forward(x, branch, coords, seed_at, o, True)
         ctx.save_for_backward(branch, h, stats, coords, seed_at, *coefs)
         ctx.options = o
         ctx.set_materialize_grads(False)
@@ -68,28 +65,27 @@ class _BlockNorm(torch.autograd.Function):
         branch, h, stats, coords, seed_at, *coefs = ctx.saved_tensors
         need_x, need_branch, _, _, _, *need = ctx.needs_input_grad
         if dy is None and dh is None:
-            return (None,) * len(ctx.needs_input_grad)
-        n, c = h.shape
-        dev = h.device
-        o = ctx.options
+            return (None,) * (5 + len(need))
+        o, dev = ctx.options, h.device
         dy = None if dy is None else dy.contiguous()
         dh = None if dh is None else dh.contiguous()
-        dx = h.new_empty((n, c)) if need_x else None
-        dbranch = h.new_empty((n, c)) if need_branch else None
+        dx = torch.empty_like(h) if need_x else None
+        dbranch = torch.empty_like(h) if need_branch else None
         grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if want else None
                  for t, want in zip(coefs, need)]
-        a = _arguments(branch, h, stats, coords, coefs, o)
-        a.seed_at = N.ptr(seed_at)
-        g = N.BlockNormGrads(*(_row(t) for t in grads))
+        rows = []
+        for t in grads:
+            rows += _NONE if t is None else _row(t)
         lib = N.load()
-        with N.on_device(dev):
-            batch = o["batch"] if _per_batch(coefs) else 0
-            nbytes = lib.sv_block_norm_backward_workspace_bytes(n, c, batch)
-            ws = N.workspace(nbytes, dev) if batch or any(need) else None
-            rc = lib.sv_block_norm_backward(
-                ctypes.byref(a), N.ptr(dy), N.ptr(dh), N.ptr(dx), N.ptr(dbranch), ctypes.byref(g),
-                N.ptr(ws), nbytes, N.stream(dev))
-        N.check(rc, "block_norm (backward)")
+        nbytes, ws = 0, None
+        if o.per_batch or any(need):
+            nbytes = lib.sv_block_norm_backward_workspace_bytes(o.n, o.c, o.batch if o.per_batch else 0)
+            ws = N.workspace(nbytes, dev)
+        rc = N.call(dev, lib.sv_block_norm_backward, o.pack(0, 0, branch, h, stats, coords, seed_at),
+                    N.ptr(dy), N.ptr(dh), N.ptr(dx), N.ptr(dbranch), N.BLOCK_NORM_GRADS.pack(*rows),
+                    N.ptr(ws), nbytes, N.stream(dev))
+        if rc:
+            N.check(rc, "block_norm (backward)")
         return dx, dbranch, None, None, None, *grads
 
 
@@ -135,75 +131,87 @@ def block_norm(
     """
 
     x, branch = N.as_tensor(x), N.as_tensor(branch)
-    if x.ndim < 1 or x.dtype not in N.DTYPE_CODE:
-        raise ValueError(f"block_norm: unsupported input, shape {tuple(x.shape)}, dtype {x.dtype}")
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    if not shape or dtype not in N.DTYPE_CODE:
+        raise ValueError(f"block_norm: unsupported input, shape {tuple(shape)}, dtype {dtype}")
     if norm not in ("layer", "rms"):
         raise ValueError(f"block_norm: unknown norm {norm!r}")
-    c = x.shape[-1]
-    rows = math.prod(x.shape[:-1])
-    if branch.shape != x.shape or branch.dtype != x.dtype:
-        raise ValueError(f"block_norm: branch must be a {tuple(x.shape)} {x.dtype} tensor, got "
+    c = shape[-1]
+    rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+    if branch.shape != shape or branch.dtype != dtype:
+        raise ValueError(f"block_norm: branch must be a {tuple(shape)} {dtype} tensor, got "
                          f"{tuple(branch.shape)} {branch.dtype}")
     if branch_weight is not None and not branch_norm:
         raise ValueError("block_norm: branch_weight goes with branch_norm")
-    for name, t in (("weight", weight), ("bias", bias), ("branch_weight", branch_weight)):
-        if t is not None and (t.shape != (c,) or t.dtype not in N.DTYPE_CODE):
-            raise ValueError(f"block_norm: {name} must be a float tensor of shape ({c},)")
-    largest = 1
-    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+    grads = torch.is_grad_enabled()
+    some = grads and (x.requires_grad or branch.requires_grad)
+    o = _Call()
+    packed, coefs, largest = [], [], 1
+    for name, t, rank in (("weight", weight, 1), ("bias", bias, 1),
+                          ("branch_weight", branch_weight, 1), ("gate", gate, 2),
+                          ("scale", scale, 2), ("shift", shift, 2)):
         if t is None:
+            packed += _NONE
+            coefs.append(None)
             continue
-        if t.ndim not in (1, 2) or t.shape[-1] != c or t.dtype not in N.DTYPE_CODE:
-            raise ValueError(f"block_norm: {name} must be a float tensor of shape (B, {c})")
-        largest = max(largest, t.shape[0] if t.ndim == 2 else 1)
+        size = t.shape
+        if not 1 <= len(size) <= rank or size[-1] != c or t.dtype not in N.DTYPE_CODE:
+            raise ValueError(f"block_norm: {name} must be a float tensor of shape "
+                             + (f"(B, {c})" if rank == 2 else f"({c},)"))
+        if t.device != dev:
+            raise ValueError(f"block_norm: {name} is on {t.device}, x on {dev}")
+        if len(size) == 2 and size[0] != 1:
+            if largest not in (1, size[0]):
+                raise ValueError(f"block_norm: {name} has {size[0]} rows, others {largest}")
+            largest = size[0]
+        if not t.is_contiguous() and not (
+                (t.stride(-1) == 1 or c <= 1) and (len(size) == 1 or t.stride(0) >= c)):
+            t = t.contiguous()
+        some = some or (grads and t.requires_grad)
+        coefs.append(t)
+        packed += _row(t)
     batch = largest if batch_size is None else int(batch_size)
-    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
-        if t is not None and t.ndim == 2 and t.shape[0] not in (1, batch):
-            raise ValueError(f"block_norm: {name} has {t.shape[0]} rows for batch {batch}")
-    if largest > 1:
+    if largest not in (1, batch):
+        raise ValueError(f"block_norm: {largest} rows of coefficients for batch {batch}")
+    if largest != 1:
         if coords is None:
             raise ValueError("block_norm: rows per batch element need the coordinates")
         if coords.shape != (rows, 4) or coords.dtype != torch.int32:
             raise ValueError(f"block_norm: coords must be an int32 tensor of shape ({rows}, 4)")
+        if coords.device != dev:
+            raise ValueError(f"block_norm: coords is on {coords.device}, x on {dev}")
+        coords = coords.contiguous()
     else:
         coords = None
-    for name, t in (("branch", branch), ("weight", weight), ("bias", bias), ("gate", gate),
-                    ("branch_weight", branch_weight), ("scale", scale), ("shift", shift),
-                    ("coords", coords)):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"block_norm: {name} is on {t.device}, x on {x.device}")
+    if branch.device != dev:
+        raise ValueError(f"block_norm: branch is on {branch.device}, x on {dev}")
     if not eps >= 0:
         raise ValueError("block_norm: eps must not be negative")
-    p = check_share("block_norm", dropout)
-    seed_value, seed_at = 0, None
-    if p > 0:
+    p, seed_value, seed_at = 0.0, 0, None
+    if dropout != 0:
+        p = check_share("block_norm", dropout)
         if seed is None:
             raise ValueError("block_norm: dropout needs a seed")
-        seed_value, seed_at, subsequence = seed_argument("block_norm", seed, subsequence, x.device)
+        seed_value, seed_at, subsequence = seed_argument("block_norm", seed, subsequence, dev)
     else:
         subsequence = 0
-    N.refuse_tangents("block_norm", x, branch, weight, bias, branch_weight, gate, scale, shift)
+    N.refuse_tangents("block_norm", x, branch, *coefs)
     N.require_cuda(x, "x")
-    x2, branch2 = (_rows(t, c) if c else t.reshape(rows, 0) for t in (x, branch))
-    if coords is not None:
-        coords = coords.contiguous()
-
-    def dense(t):
-        if t is None or ((t.stride(-1) == 1 or c <= 1)
-                         and (t.ndim == 1 or t.shape[0] <= 1 or t.stride(0) >= c)):
-            return t
-        return t.contiguous()
-
-    coefs = [dense(t) for t in (weight, bias, branch_weight, gate, scale, shift)]
-    o = {"batch": batch, "p": p, "seed": seed_value, "subsequence": subsequence,
-         "layer": int(norm == "layer"), "branch_norm": int(bool(branch_norm)),
-         "residual_scale": float(residual_scale), "eps": float(eps)}
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, branch, *coefs)):
-        y, h = _BlockNorm.apply(x2, branch2, coords, seed_at, o, *coefs)
+    flat = len(shape) == 2
+    if not (flat and x.is_contiguous()):
+        x = _rows(x, c) if c else x.reshape(rows, 0)
+    if not (flat and branch.is_contiguous()):
+        branch = _rows(branch, c) if c else branch.reshape(rows, 0)
+    o.n, o.c, o.code, o.batch, o.per_batch, o.rows = rows, c, N.DTYPE_CODE[dtype], batch, largest != 1, packed
+    o.branch_stride = max(branch.stride(0), c)
+    o.p, o.seed, o.subsequence = p, seed_value, subsequence
+    o.layer, o.branch_norm = int(norm == "layer"), int(bool(branch_norm))
+    o.residual_scale, o.eps = float(residual_scale), float(eps)
+    if some:
+        y, h = _BlockNorm.apply(x, branch, coords, seed_at, o, *coefs)
     else:
-        y, h, _ = _forward(x2, branch2, coords, seed_at, coefs, o, False)
-    return (y, h) if x.ndim == 2 else (y.reshape(x.shape), h.reshape(x.shape))
+        y, h, _ = _forward(x, branch, coords, seed_at, o, False)
+    return (y, h) if flat else (y.reshape(shape), h.reshape(shape))
 
 
 __all__ = ["block_norm"]

@@ -33,12 +33,13 @@ def check_share(what: str, p) -> float:
 
 
 def _forward(x, residual, p, seed, seed_at, subsequence):
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with N.on_device(x.device):
-        rc = N.load().sv_dropout(x.data_ptr(), N.ptr(residual), x.numel(), N.DTYPE_CODE[x.dtype],
-                                 p, seed, N.ptr(seed_at), subsequence, out.data_ptr(),
-                                 N.stream(x.device))
-    N.check(rc, "dropout")
+    out = torch.empty_like(x)
+    dev = x.device
+    rc = N.call(dev, N.load().sv_dropout, x.data_ptr(), N.ptr(residual), x.numel(),
+                N.DTYPE_CODE[x.dtype], p, seed, N.ptr(seed_at), subsequence, out.data_ptr(),
+                N.stream(dev))
+    if rc:
+        N.check(rc, "dropout")
     return out
 
 

@@ -3,7 +3,6 @@ expert (``sv_expert_linear``), with gradients."""
 
 from __future__ import annotations
 
-import ctypes
 import dataclasses
 
 import torch
@@ -45,51 +44,51 @@ class ExpertRoutes:
 
 
 def _route(logits, k, normalize):
+    """(weights, experts, order, offsets, place)."""
+
     n, e = logits.shape
     dev = logits.device
     lib = N.load()
-    experts, place = (torch.empty((n, k), dtype=torch.int32, device=dev) for _ in range(2))
     weights = torch.empty((n, k), dtype=torch.float32, device=dev)
-    order = torch.empty((n * k,), dtype=torch.int32, device=dev)
-    offsets = torch.empty((e + 1,), dtype=torch.int32, device=dev)
-    with N.on_device(dev):
-        nbytes = lib.sv_route_workspace_bytes(n, e, k)
-        ws = N.workspace(nbytes, dev) if nbytes else None
-        rc = lib.sv_route(
-            logits.data_ptr(), max(logits.stride(0), e), n, e, k, N.DTYPE_CODE[logits.dtype],
-            int(normalize), experts.data_ptr(), weights.data_ptr(), order.data_ptr(),
-            offsets.data_ptr(), place.data_ptr(), N.ptr(ws), nbytes, N.stream(dev))
-    N.check(rc, "route")
-    return experts, weights, order, offsets, place
+    # one allocation for what is integer: a call of few rows is bound by its host steps
+    slots = n * k
+    words = torch.empty((3 * slots + e + 1,), dtype=torch.int32, device=dev)
+    experts, place, order, offsets = words.split((slots, slots, slots, e + 1))
+    nbytes = lib.sv_route_workspace_bytes(n, e, k)
+    ws = N.workspace(nbytes, dev) if nbytes else None
+    at = words.data_ptr()
+    rc = N.call(dev, lib.sv_route, logits.data_ptr(), max(logits.stride(0), e), n, e, k,
+                N.DTYPE_CODE[logits.dtype], normalize, at, weights.data_ptr(), at + 8 * slots,
+                at + 12 * slots, at + 4 * slots, N.ptr(ws), nbytes, N.stream(dev))
+    if rc:
+        N.check(rc, "route")
+    return weights, experts.view(n, k), order, offsets, place.view(n, k)
 
 
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, k, normalize):
-        experts, weights, order, offsets, place = _route(logits, k, normalize)
+    def forward(ctx, logits, k, normalize, found):
+        weights, experts, *rest = _route(logits, k, normalize)
+        found += experts, *rest
         ctx.save_for_backward(logits, experts, weights)
         ctx.normalize = normalize
-        ctx.mark_non_differentiable(experts, order, offsets, place)
-        ctx.set_materialize_grads(False)
-        return experts, weights, order, offsets, place
+        return weights
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, _experts, dweights, *_):
-        if dweights is None:
-            return None, None, None
+    def backward(ctx, dweights):
         logits, experts, weights = ctx.saved_tensors
         n, e = logits.shape
         dev = logits.device
         dweights = dweights.contiguous()
         dlogits = torch.empty((n, e), dtype=logits.dtype, device=dev)
-        with N.on_device(dev):
-            rc = N.load().sv_route_backward(
-                logits.data_ptr(), max(logits.stride(0), e), n, e, experts.shape[1],
-                N.DTYPE_CODE[logits.dtype], int(ctx.normalize), experts.data_ptr(),
-                weights.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), N.stream(dev))
-        N.check(rc, "route (backward)")
-        return dlogits, None, None
+        rc = N.call(dev, N.load().sv_route_backward, logits.data_ptr(), max(logits.stride(0), e),
+                    n, e, experts.shape[1], N.DTYPE_CODE[logits.dtype], ctx.normalize,
+                    experts.data_ptr(), weights.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(),
+                    N.stream(dev))
+        if rc:
+            N.check(rc, "route (backward)")
+        return dlogits, None, None, None
 
 
 def route(logits: torch.Tensor, k: int, *, normalize: bool = True) -> ExpertRoutes:
@@ -117,39 +116,44 @@ def route(logits: torch.Tensor, k: int, *, normalize: bool = True) -> ExpertRout
     N.require_cuda(logits, "logits")
     logits = _row_major(logits)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return ExpertRoutes(*_Route.apply(logits, k, bool(normalize)))
-    return ExpertRoutes(*_route(logits, k, bool(normalize)))
+        found: list[torch.Tensor] = []
+        weights = _Route.apply(logits, k, int(bool(normalize)), found)
+        experts, order, offsets, place = found
+    else:
+        weights, experts, order, offsets, place = _route(logits, k, int(bool(normalize)))
+    return ExpertRoutes(experts, weights, order, offsets, place)
 
 
-def _arguments(x, weight, bias, p, order, offsets, place, preact, rows, o) -> N.ExpertArgs:
+def _pack(x, weight, bias, p, order, offsets, place, preact, rows, o) -> bytes:
     experts, outputs, inputs = weight.shape
-    return N.ExpertArgs(
-        n=p.shape[0], x=x.data_ptr(), ldx=_ld(x), weight=weight.data_ptr(),
-        ldw=max(weight.stride(1), inputs), w_expert=weight.stride(0), bias=N.ptr(bias),
-        order=order.data_ptr(), offsets=offsets.data_ptr(), place=place.data_ptr(),
-        weights=p.data_ptr(), preact=N.ptr(preact), rows=N.ptr(rows), inputs=inputs,
-        outputs=outputs, k=p.shape[1], experts=experts, dtype=N.DTYPE_CODE[x.dtype],
-        activation=N.ACTIVATION_CODE[o["activation"]], gather=o["gather"], combine=o["combine"])
+    n, k = p.shape
+    return N.EXPERT_ARGS.pack(
+        n, x.data_ptr(), _ld(x), weight.data_ptr(), max(weight.stride(1), inputs),
+        weight.stride(0), 0 if bias is None else bias.data_ptr(), order.data_ptr(),
+        offsets.data_ptr(), place.data_ptr(), p.data_ptr(), 0 if preact is None else preact.data_ptr(),
+        0 if rows is None else rows.data_ptr(), inputs, outputs, k, experts, N.DTYPE_CODE[x.dtype],
+        *o)
 
 
 def _forward(x, weight, bias, p, order, offsets, place, o, keep):
+    act, _, combine = o
     n, k = p.shape
-    outputs = weight.shape[1]
+    slots, outputs = n * k, weight.shape[1]
     dev = x.device
-    out = torch.empty((n if o["combine"] else n * k, outputs), dtype=x.dtype, device=dev)
+    out = x.new_empty((n if combine else slots, outputs))
     rows = preact = None
-    if o["combine"]:
-        rows = torch.empty((n * k, outputs), dtype=torch.float32, device=dev)
-    if keep and N.ACTIVATION_CODE[o["activation"]]:
-        preact = torch.empty((n * k, outputs), dtype=torch.float32, device=dev)
-    a = _arguments(x, weight, bias, p, order, offsets, place, preact, rows, o)
+    if combine:
+        rows = torch.empty((slots, outputs), dtype=torch.float32, device=dev)
+    if keep and act:
+        preact = torch.empty((slots, outputs), dtype=torch.float32, device=dev)
+    a = _pack(x, weight, bias, p, order, offsets, place, preact, rows, o)
     lib = N.load()
-    with N.on_device(dev):
-        nbytes = lib.sv_expert_linear_workspace_bytes(ctypes.byref(a), N.SV_LINEAR_FORWARD, 0, 0, None)
-        ws = N.workspace(nbytes, dev) if nbytes else None
-        rc = lib.sv_expert_linear(ctypes.byref(a), out.data_ptr(), N.ptr(ws), nbytes,
-                                  N.status_word(dev).data_ptr(), N.stream(dev))
-    N.check(rc, "expert_linear")
+    nbytes = lib.sv_expert_linear_workspace_bytes(a, N.SV_LINEAR_FORWARD, 0, 0, None)
+    ws = N.workspace(nbytes, dev) if nbytes else None
+    rc = N.call(dev, lib.sv_expert_linear, a, out.data_ptr(), N.ptr(ws), nbytes,
+                N.status_word(dev).data_ptr(), N.stream(dev))
+    if rc:
+        N.check(rc, "expert_linear")
     return out, preact, rows
 
 
@@ -167,25 +171,23 @@ class _ExpertLinear(torch.autograd.Function):
     def backward(ctx, dout):
         x, weight, p, order, offsets, place, preact, rows = ctx.saved_tensors
         need_x, need_w, need_b, need_p, *_ = ctx.needs_input_grad
-        dev = x.device
+        o, dev = ctx.options, x.device
         dout = dout.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_w else None
-        db = torch.empty(ctx.bias_shape, dtype=x.dtype, device=dev) if need_b else None
+        dx = x.new_empty(x.shape) if need_x else None
+        dw = x.new_empty(weight.shape) if need_w else None
+        db = x.new_empty(ctx.bias_shape) if need_b else None
         dp = None
-        if need_p:
-            dp = (torch.empty if ctx.options["combine"] else torch.zeros)(
-                p.shape, dtype=torch.float32, device=dev)
-        a = _arguments(x, weight, None, p, order, offsets, place, preact, rows, ctx.options)
+        if need_p:  # without the weighted sum nothing reaches the weights
+            dp = torch.empty_like(p) if o[2] else torch.zeros_like(p)
+        a = _pack(x, weight, None, p, order, offsets, place, preact, rows, o)
         lib = N.load()
-        with N.on_device(dev):
-            nbytes = lib.sv_expert_linear_workspace_bytes(
-                ctypes.byref(a), N.SV_LINEAR_BACKWARD, int(need_x), int(need_w), dout.data_ptr())
-            ws = N.workspace(nbytes, dev)
-            rc = lib.sv_expert_linear_backward(
-                ctypes.byref(a), dout.data_ptr(), N.ptr(dx), N.ptr(dw), N.ptr(db), N.ptr(dp),
-                ws.data_ptr(), nbytes, N.status_word(dev).data_ptr(), N.stream(dev))
-        N.check(rc, "expert_linear (backward)")
+        at = dout.data_ptr()
+        nbytes = lib.sv_expert_linear_workspace_bytes(a, N.SV_LINEAR_BACKWARD, need_x, need_w, at)
+        ws = N.workspace(nbytes, dev)
+        rc = N.call(dev, lib.sv_expert_linear_backward, a, at, N.ptr(dx), N.ptr(dw), N.ptr(db),
+                    N.ptr(dp), ws.data_ptr(), nbytes, N.status_word(dev).data_ptr(), N.stream(dev))
+        if rc:
+            N.check(rc, "expert_linear (backward)")
         return dx, dw, db, dp, None, None, None, None
 
 
@@ -222,47 +224,49 @@ def expert_linear(
         raise ValueError(f"expert_linear: unknown activation {activation!r}")
     if not isinstance(routes, ExpertRoutes):
         raise ValueError("expert_linear: routes must be an ExpertRoutes")
-    if x.ndim != 2 or weight.ndim != 3 or weight.shape[2] != x.shape[1]:
+    shape, dtype, dev = weight.shape, x.dtype, x.device
+    if x.ndim != 2 or len(shape) != 3 or shape[2] != x.shape[1]:
         raise ValueError(f"expert_linear: x must have shape (rows, K) and weight (experts, N, K), got "
-                         f"{tuple(x.shape)} and {tuple(weight.shape)}")
-    if x.dtype not in N.DTYPE_CODE:
-        raise ValueError(f"expert_linear: unsupported dtype {x.dtype}")
-    e, outputs, inputs = weight.shape
+                         f"{tuple(x.shape)} and {tuple(shape)}")
+    if dtype not in N.DTYPE_CODE:
+        raise ValueError(f"expert_linear: unsupported dtype {dtype}")
+    e, outputs, inputs = shape
+    p = routes.weights
     n, k = routes.experts.shape
-    dev = x.device
     want_rows = n if gather else n * k
     if x.shape[0] != want_rows:
         raise ValueError(f"expert_linear: x has {x.shape[0]} rows, the routes ask for {want_rows}")
     if not 1 <= e <= MAX_EXPERTS or routes.num_experts != e:
         raise ValueError(f"expert_linear: weight has {e} experts, the routes {routes.num_experts}")
-    for name, t, want, dtype in (
-        ("weight", weight, (e, outputs, inputs), x.dtype),
-        ("bias", bias, (e, outputs), x.dtype),
-        ("routes.weights", routes.weights, (n, k), torch.float32),
+    for name, t, want, kind in (
+        ("weight", weight, shape, dtype),
+        ("bias", bias, (e, outputs), dtype),
+        ("routes.weights", p, (n, k), torch.float32),
         ("routes.order", routes.order, (n * k,), torch.int32),
         ("routes.offsets", routes.offsets, (e + 1,), torch.int32),
         ("routes.place", routes.place, (n, k), torch.int32),
     ):
         if t is None:
             continue
-        if t.shape != want or t.dtype != dtype:
-            raise ValueError(f"expert_linear: {name} must be a {tuple(want)} {dtype} tensor, got "
+        if t.shape != want or t.dtype != kind:
+            raise ValueError(f"expert_linear: {name} must be a {tuple(want)} {kind} tensor, got "
                              f"{tuple(t.shape)} {t.dtype}")
         if t.device != dev:
             raise ValueError(f"expert_linear: {name} is on {t.device}, x on {dev}")
-    N.refuse_tangents("expert_linear", x, weight, bias, routes.weights)
+    N.refuse_tangents("expert_linear", x, weight, bias, p)
     N.require_cuda(x, "x")
     x = _row_major(x)
-    if not (weight.stride(2) == 1 or inputs <= 1) or weight.stride(1) < inputs or \
-            weight.stride(0) < outputs * inputs:
+    if not weight.is_contiguous() and (
+            not (weight.stride(2) == 1 or inputs <= 1) or weight.stride(1) < inputs
+            or weight.stride(0) < outputs * inputs):
         weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    p, order, offsets, place = (t.contiguous() for t in (
-        routes.weights, routes.order, routes.offsets, routes.place))
-    o = {"activation": activation, "gather": int(bool(gather)), "combine": int(bool(combine))}
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias)) or (
-            torch.is_grad_enabled() and combine and p.requires_grad):
+    order, offsets, place = routes.order.contiguous(), routes.offsets.contiguous(), routes.place.contiguous()
+    p = p.contiguous()
+    o = N.ACTIVATION_CODE[activation], int(bool(gather)), int(bool(combine))
+    if torch.is_grad_enabled() and (
+            x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+            or (combine and p.requires_grad)):
         return _ExpertLinear.apply(x, weight, bias, p, order, offsets, place, o)
     return _forward(x, weight, bias, p, order, offsets, place, o, False)[0]
 
