@@ -446,7 +446,8 @@ typedef struct sv_block_norm_grads {
 SV_API size_t sv_block_norm_backward_workspace_bytes(int64_t n, int channels, int64_t batch);
 SV_API int sv_block_norm_backward(const sv_block_norm_args* args, const void* dy, const void* dh,
                                   void* dx, void* dbranch, const sv_block_norm_grads* grads,
-                                  void* workspace, size_t workspace_bytes, sv_stream_t stream);
+                                  void* workspace, size_t workspace_bytes, int32_t* status,
+                                  sv_stream_t stream);
 
 /* ---- dropout with counter-based random numbers ------------------------------------------ */
 

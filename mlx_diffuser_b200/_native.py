@@ -121,8 +121,7 @@ _SIGNATURES = {
     "sv_block_norm_backward_workspace_bytes": (_SZ, [_I64, _I32, _I64]),
     "sv_block_norm_backward": (
         _I32,
-        [ctypes.c_char_p, _P, _P, _P, _P, ctypes.c_char_p, _P, _SZ,
-         _P],
+        [ctypes.c_char_p, _P, _P, _P, _P, ctypes.c_char_p, _P, _SZ, _P, _P],
     ),
     "sv_dropout": (
         _I32, [_P, _P, _I64, _I32, ctypes.c_double, _U64, _P, _U64, _P, _P]

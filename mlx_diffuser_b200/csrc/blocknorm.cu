@@ -22,12 +22,12 @@
 
 #include "dropout.cuh"
 #include "group.h"
+#include "rows.cuh"
 
 namespace sv {
 namespace {
 
 constexpr int BN_MAX_CHANNELS = 8192;
-constexpr int BN_PIECES_PER_SM = 4;
 
 // A row or rows of coefficients in any float type; null: the neutral value.
 struct Coef {
@@ -57,7 +57,7 @@ struct BlockArgs {
 };
 
 struct BackArgs {
-  BlockArgs f;  // h is read; x, y and status are not used
+  BlockArgs f;  // h is read; x and y are not used
   const void* dy;
   const void* dh;
   void* dx;
@@ -542,6 +542,408 @@ __global__ void __launch_bounds__(kThreads<TPR>)
   join(sum_e, to + 2 * C);
 }
 
+// ---- long runs of rows: a pipeline per warp ------------------------------------------------------
+//
+// A warp has a row to itself (the sums need no barrier), 2 to 4 times 8 elements a lane, and keeps the next
+// rows in flight by bulk copies (rows.cuh). The coefficients of one batch element stand in shared
+// memory, folded: what differs from row to row is added up in registers, and HBM is not waited for.
+
+// Folded coefficients, planes of four: element c of plane k is at [(k * 2 + c / 4 % 2) * 4 * Q + c / 8 * 4
+// + c % 4], so that the lanes' 16-byte accesses of neighbouring eights do not meet in a bank.
+template <int J>
+struct Folded {
+  static constexpr int Q = 32 * J;  // eights of a row
+  static constexpr int PLANE = 8 * Q;
+  float* at;
+  __device__ __forceinline__ void load(int k, int q, float (&v)[8]) const {
+    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(at + (k * 2) * 4 * Q + q * 4);
+    *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(at + (k * 2 + 1) * 4 * Q + q * 4);
+  }
+  __device__ __forceinline__ void store(int k, int q, const float (&v)[8]) const {
+    *reinterpret_cast<float4*>(at + (k * 2) * 4 * Q + q * 4) = *reinterpret_cast<const float4*>(v);
+    *reinterpret_cast<float4*>(at + (k * 2 + 1) * 4 * Q + q * 4) = *reinterpret_cast<const float4*>(v + 4);
+  }
+};
+
+// gate alpha wb; w (1 + scale); beta (1 + scale) + shift: for eight channels of batch element b, b < 0: a
+// row without one.
+__device__ __forceinline__ void fold(const BlockArgs& a, int64_t b, int c, float (&g)[8], float (&m)[8],
+                                     float (&s)[8]) {
+  float w[8], beta[8], wb[8];
+  load_coef(a.weight, 0, c, 1.0f, w);
+  load_coef(a.bias, 0, c, 0.0f, beta);
+  load_coef(a.branch_weight, 0, c, 1.0f, wb);
+  if (b >= 0) {
+    load_coef(a.gate, b, c, 1.0f, g);
+    load_coef(a.scale, b, c, 0.0f, m);
+    load_coef(a.shift, b, c, 0.0f, s);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (b < 0) g[i] = 1.0f, m[i] = s[i] = 0.0f;
+    g[i] *= a.alpha * wb[i];
+    s[i] = fmaf(beta[i], 1.0f + m[i], s[i]);
+    m[i] = w[i] * (1.0f + m[i]);
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_eight(const uint8_t* stage, int q, float (&v)[8]) {
+  alignas(16) T e[8];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(e) / 16; ++i)
+    reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(stage)[q * (sizeof(e) / 16) + i];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+}
+
+// Stages that fit two blocks an SM of 16-bit rows, or one of fp32 rows.
+template <typename T, int J, int TENSORS, int PLANES>
+struct RowsLayout {
+  using Ring = RowRing<T, J * (int)sizeof(T) / 2>;  // 32 J eights: as many 16-byte accesses, twice for fp32
+  static constexpr int STAGES = 2;
+  static constexpr int TABLE = Ring::SMEM(TENSORS, STAGES);
+  static constexpr int SMEM = TABLE + PLANES * Folded<J>::PLANE * 4;
+  static_assert(SMEM <= 227 * 1024, "shared memory budget");
+};
+
+template <typename T, int J, bool LAYER, bool BRANCH>
+__global__ void __launch_bounds__(32 * ROW_WARPS, sizeof(T) == 2 ? 2 : 1)
+    block_norm_rows_kernel(const __grid_constant__ BlockArgs a) {
+  using L = RowsLayout<T, J, 2, 6>;
+  using Ring = typename L::Ring;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int C = a.channels;
+  const Folded<J> tables{reinterpret_cast<float*>(smem + L::TABLE)};
+  if (threadIdx.x == 0) s_abort = 0;
+  // The block's rows are neighbours, of one batch element or of two: those of its first and last row have
+  // tables. Rows of others fold their coefficients again, waiting for L2: one block that did so for half
+  // of its rows took as long as the others' whole pass.
+  const int64_t per = (a.n + gridDim.x - 1) / gridDim.x;
+  const int64_t first = min(blockIdx.x * per, a.n), last = min(first + per, a.n);
+  const int64_t held0 = first < last ? batch_of(a, first) : 0;
+  const int64_t held1 = first < last ? batch_of(a, last - 1) : 0;
+  for (int q = threadIdx.x; q * 8 < C; q += 32 * ROW_WARPS) {
+    float g[8], m[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (i == 1 && held1 == held0) break;
+      fold(a, i ? held1 : held0, q * 8, g, m, s);
+      tables.store(3 * i, q, g);
+      tables.store(3 * i + 1, q, m);
+      tables.store(3 * i + 2, q, s);
+    }
+  }
+  __syncthreads();
+  int b_lane = 0;  // the batch elements of the warp's next 32 rows, a lane each
+  const uint64_t seed = a.drop.cut ? seed_of(a.drop) : 0;
+  const float inv = 1.0f / (float)C;
+  const bool ok = run_rows<T, J * (int)sizeof(T) / 2, 2, L::STAGES>(
+      smem, first + warp, ROW_WARPS, last, C * (int)sizeof(T), 2, &s_abort,
+      [](int64_t r, int64_t) { return r; },
+      [&](int t, int64_t r) -> const void* {
+        return t == 0 ? static_cast<const T*>(a.x) + r * a.x_stride
+                      : static_cast<const T*>(a.branch) + r * a.branch_stride;
+      },
+      [&](int64_t row, int64_t k, const uint8_t* stage, auto&& release) {
+        if (a.per_batch && (k & 31) == 0) {
+          const int64_t mine = row + lane * ROW_WARPS;
+          b_lane = mine < last ? (int)batch_of(a, mine) : 0;
+        }
+        const int64_t b = __shfl_sync(0xffffffffu, b_lane, (int)(k & 31));
+        if (b < 0 && lane == 0) report(a.status, SV_DEVICE_BAD_INDEX);
+        const int table = b == held0 ? 0 : b == held1 ? 3 : -1;
+        float x[J][8], d[J][8];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int q = lane + 32 * j;
+          if (q * 8 < C) {
+            load_eight<T>(stage, q, x[j]);
+            load_eight<T>(stage + Ring::ROW, q, d[j]);
+            if (a.drop.cut)
+              drop_eight(d[j], philox(((uint64_t)row * C >> 3) + q, a.drop.subsequence, seed), a.drop);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[j][i] = d[j][i] = 0.0f;
+          }
+        }
+        release();
+        float dm = 0.0f, dr = 1.0f;
+        if constexpr (BRANCH) {
+          if constexpr (LAYER) {
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) s += d[j][i];
+            dm = warp_sum(s) * inv;
+          }
+          float s = 0.0f;
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            if ((lane + 32 * j) * 8 < C) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                if constexpr (LAYER) d[j][i] -= dm;
+                s = fmaf(d[j][i], d[j][i], s);
+              }
+            }
+          dr = rsqrtf(fmaf(warp_sum(s), inv, a.eps));
+        }
+        float hm = 0.0f, s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int q = lane + 32 * j;
+          if (q * 8 >= C) continue;
+          float g[8], unused[8], other[8];
+          if (table >= 0) tables.load(table, q, g);
+          else fold(a, b, q * 8, g, unused, other);
+          alignas(16) T e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float u = BRANCH ? d[j][i] * dr : d[j][i];
+            e[i] = from_f32<T>(fmaf(g[i], u, x[j][i]));
+            x[j][i] = to_f32(e[i]);
+            if constexpr (LAYER) s += x[j][i];
+            else s = fmaf(x[j][i], x[j][i], s);
+          }
+          uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.h) + row * C + q * 8);
+#pragma unroll
+          for (int i = 0; i < (int)sizeof(e) / 16; ++i) to[i] = reinterpret_cast<const uint4*>(e)[i];
+        }
+        if constexpr (LAYER) {
+          hm = warp_sum(s) * inv;
+          s = 0.0f;
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            if ((lane + 32 * j) * 8 < C) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                x[j][i] -= hm;
+                s = fmaf(x[j][i], x[j][i], s);
+              }
+            }
+        }
+        const float hr = rsqrtf(fmaf(warp_sum(s), inv, a.eps));
+        if (a.stats && lane == 0) a.stats[row] = make_float4(hm, hr, dm, dr);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int q = lane + 32 * j;
+          if (q * 8 >= C) continue;
+          float unused[8], m[8], add[8];
+          if (table >= 0) {
+            tables.load(table + 1, q, m);
+            tables.load(table + 2, q, add);
+          } else {
+            fold(a, b, q * 8, unused, m, add);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) m[i] = fmaf(x[j][i] * hr, m[i], add[i]);
+          store_row<T, 8>(static_cast<T*>(a.y) + row * C + q * 8, m);
+        }
+      });
+  if (!ok && lane == 0) report(a.status, SV_DEVICE_WAIT_TIMEOUT);
+}
+
+// The backward pass of a piece, whose rows have one batch element. A row's tensors are read from the stage
+// twice: cheaper than holding 32 J values beside the sums.
+template <typename T, int J, bool LAYER, bool BRANCH>
+__global__ void __launch_bounds__(32 * ROW_WARPS, 1)
+    block_norm_rows_backward_kernel(const __grid_constant__ BackArgs a) {
+  using L = RowsLayout<T, J, 4, 2>;
+  using Ring = typename L::Ring;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int s_abort;
+  const BlockArgs& f = a.f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int C = f.channels;
+  const Folded<J> table{reinterpret_cast<float*>(smem + L::TABLE)};
+  Piece p{0, 0, 0};
+  if (a.offsets) {
+    p = find_piece<true>(a.offsets, (int)f.batch, (int)f.n, a.piece, blockIdx.x);
+  } else {
+    p.first = (int)min((int64_t)blockIdx.x * a.piece, f.n);
+    p.last = (int)min((int64_t)p.first + a.piece, f.n);
+    if (p.first >= p.last) p.group = -1;
+  }
+  if (p.group < 0) return;  // the whole block
+  if (threadIdx.x == 0) s_abort = 0;
+  const int64_t b = p.group < f.batch ? p.group : -1;
+  for (int q = threadIdx.x; q * 8 < C; q += 32 * ROW_WARPS) {
+    float g[8], m[8], s[8];
+    fold(f, b, q * 8, g, m, s);
+    table.store(0, q, g);
+    table.store(1, q, m);
+  }
+  __syncthreads();
+  const uint64_t seed = f.drop.cut ? seed_of(f.drop) : 0;
+  const bool with_d = BRANCH || a.want_e;
+  float sum_a[J][8], sum_b[J][8], sum_e[J][8];
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum_a[j][i] = sum_b[j][i] = sum_e[j][i] = 0.0f;
+  const float inv = 1.0f / (float)C;
+  // tensors that are there, in order: h, dy, dh, branch
+  const int at_dy = 1, at_dh = at_dy + (a.dy != nullptr), at_d = at_dh + (a.dh != nullptr);
+  const int tensors = at_d + with_d;
+  // The indices of the warp's rows 32 i .. 32 i + 31 and of the 32 behind them, a lane each, and the
+  // former's statistics: each row by itself waited for L2 three times.
+  auto index_of = [&](int64_t k) {
+    const int64_t at = min(p.first + warp + k * ROW_WARPS, (int64_t)p.last - 1);
+    return a.perm ? __ldg(a.perm + at) : (int)at;
+  };
+  int rows_now = 0, rows_next = index_of(lane), mine = 0;
+  float4 st_lane = make_float4(0.0f, 0.0f, 0.0f, 1.0f);
+  const bool ok = run_rows<T, J * (int)sizeof(T) / 2, 4, L::STAGES>(
+      smem, p.first + warp, ROW_WARPS, p.last, C * (int)sizeof(T), tensors, &s_abort,
+      [&](int64_t, int64_t k) -> int64_t {  // STAGES rows ahead of the row that is worked on
+        if ((k & 31) == 0) {
+          rows_now = rows_next;
+          rows_next = index_of(k + 32 + lane);
+        }
+        return __shfl_sync(0xffffffffu, rows_now, (int)(k & 31));
+      },
+      [&](int t, int64_t r) -> const void* {
+        if (t == 0) return static_cast<const T*>(f.h) + r * C;
+        if (t == at_d) return static_cast<const T*>(f.branch) + r * f.branch_stride;
+        return static_cast<const T*>(t == at_dh ? a.dh : a.dy) + r * C;
+      },
+      [&](int64_t, int64_t k, const uint8_t* stage, auto&& release) {
+        if ((k & 31) == 0) {
+          mine = index_of(k + lane);
+          st_lane = __ldg(f.stats + mine);
+        }
+        const int from = (int)(k & 31);
+        const int64_t row = __shfl_sync(0xffffffffu, mine, from);
+        float4 st;
+        st.x = __shfl_sync(0xffffffffu, st_lane.x, from);
+        st.y = __shfl_sync(0xffffffffu, st_lane.y, from);
+        st.z = __shfl_sync(0xffffffffu, st_lane.z, from);
+        st.w = __shfl_sync(0xffffffffu, st_lane.w, from);
+        // N(v) = v rstd - mean rstd: the product's rounding is below that of the mean
+        const float h_off = -st.x * st.y, d_off = -st.z * st.w;
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int q = lane + 32 * j;
+          if (q * 8 >= C || a.dy == nullptr) continue;
+          float n[8], dy[8], m[8];
+          load_eight<T>(stage, q, n);
+          load_eight<T>(stage + at_dy * Ring::ROW, q, dy);
+          table.load(1, q, m);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            n[i] = LAYER ? fmaf(n[i], st.y, h_off) : n[i] * st.y;
+            sum_a[j][i] = fmaf(dy[i], n[i], sum_a[j][i]);
+            sum_b[j][i] += dy[i];
+            const float g = dy[i] * m[i];
+            if constexpr (LAYER) s1 += g;
+            s2 = fmaf(g, n[i], s2);
+          }
+        }
+        const float m1 = LAYER ? warp_sum(s1) * inv : 0.0f, m2 = warp_sum(s2) * inv;
+        float D[J][8], u[BRANCH ? J : 1][8];
+        uint32_t kept[J];
+        s1 = s2 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int q = lane + 32 * j;
+          kept[j] = 0u;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) D[j][i] = 0.0f;
+          if (q * 8 >= C) continue;
+          if (a.dh) load_eight<T>(stage + at_dh * Ring::ROW, q, D[j]);
+          if (a.dy) {
+            float n[8], dy[8], m[8];
+            load_eight<T>(stage, q, n);
+            load_eight<T>(stage + at_dy * Ring::ROW, q, dy);
+            table.load(1, q, m);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              n[i] = LAYER ? fmaf(n[i], st.y, h_off) : n[i] * st.y;
+              const float g = fmaf(dy[i], m[i], LAYER ? fmaf(-n[i], m2, -m1) : -n[i] * m2);
+              D[j][i] = fmaf(st.y, g, D[j][i]);
+            }
+          }
+          if (a.dx) store_row<T, 8>(static_cast<T*>(a.dx) + row * C + q * 8, D[j]);
+          if (f.drop.cut)
+            kept[j] = kept_eight(philox(((uint64_t)row * C >> 3) + q, f.drop.subsequence, seed), f.drop);
+          if (with_d) {
+            float d[8];
+            load_eight<T>(stage + at_d * Ring::ROW, q, d);
+            if (f.drop.cut) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) d[i] = kept[j] >> i & 1u ? d[i] * f.drop.scale : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if constexpr (BRANCH) d[i] = LAYER ? fmaf(d[i], st.w, d_off) : d[i] * st.w;
+              sum_e[j][i] = fmaf(D[j][i], d[i], sum_e[j][i]);
+              if constexpr (BRANCH) u[j][i] = d[i];
+            }
+          }
+          float g[8];
+          table.load(0, q, g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            D[j][i] *= g[i];
+            if constexpr (BRANCH) {
+              if constexpr (LAYER) s1 += D[j][i];
+              s2 = fmaf(D[j][i], u[j][i], s2);
+            }
+          }
+        }
+        release();
+        if (a.dbranch == nullptr) return;
+        const float e1 = BRANCH && LAYER ? warp_sum(s1) * inv : 0.0f;
+        const float e2 = BRANCH ? warp_sum(s2) * inv : 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int q = lane + 32 * j;
+          if (q * 8 >= C) continue;
+          if constexpr (BRANCH) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) D[j][i] = st.w * (D[j][i] - e1 - u[j][i] * e2);
+          }
+          if (f.drop.cut) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) D[j][i] = kept[j] >> i & 1u ? D[j][i] * f.drop.scale : 0.0f;
+          }
+          store_row<T, 8>(static_cast<T*>(a.dbranch) + row * C + q * 8, D[j]);
+        }
+      });
+  if (!ok && lane == 0) report(f.status, SV_DEVICE_WAIT_TIMEOUT);
+  if (a.partial == nullptr) return;
+  __syncthreads();  // the rings are done with
+  float* held = reinterpret_cast<float*>(smem);  // [warps][3 planes]
+  static_assert(ROW_WARPS * 3 * Folded<J>::PLANE * 4 <= L::TABLE, "the sums take the rings' place");
+  const Folded<J> mine_at{held + warp * 3 * Folded<J>::PLANE};
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    mine_at.store(0, lane + 32 * j, sum_a[j]);
+    mine_at.store(1, lane + 32 * j, sum_b[j]);
+    mine_at.store(2, lane + 32 * j, sum_e[j]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 3 * C; i += 32 * ROW_WARPS) {
+    const int k = i / C, c = i - k * C;
+    const float* from = held + (k * 2 + (c >> 2 & 1)) * 4 * Folded<J>::Q + (c >> 3) * 4 + (c & 3);
+    float v = from[0];
+#pragma unroll
+    for (int w = 1; w < ROW_WARPS; ++w) v += from[w * 3 * Folded<J>::PLANE];
+    a.partial[(int64_t)blockIdx.x * 3 * C + i] = v;
+  }
+}
+
 // ---- the coefficients' gradients from the pieces' sums -------------------------------------------
 
 struct Grad {
@@ -682,8 +1084,43 @@ int launch_backward(const BackArgs& a, unsigned blocks, cudaStream_t s) {
   if ((C) <= 2048) return call(1, 8, 256);                                         \
   return call(1, 32, 256)
 
+template <typename T, int J, int TENSORS, int PLANES, typename K, typename A>
+int launch_rows(K kernel, const A& a, unsigned blocks, cudaStream_t s) {
+  constexpr int bytes = RowsLayout<T, J, TENSORS, PLANES>::SMEM;
+  SV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  kernel<<<blocks, 32 * ROW_WARPS, bytes, s>>>(a);
+  SV_LAUNCH_CHECK();
+  return SV_OK;
+}
+
+template <typename T, int J>
+int rows_forward(const BlockArgs& a, cudaStream_t s) {
+  auto kernel = a.layer ? (a.branch_norm ? block_norm_rows_kernel<T, J, true, true>
+                                         : block_norm_rows_kernel<T, J, true, false>)
+                        : (a.branch_norm ? block_norm_rows_kernel<T, J, false, true>
+                                         : block_norm_rows_kernel<T, J, false, false>);
+  return launch_rows<T, J, 2, 6>(kernel, a, (unsigned)(num_sms() * (sizeof(T) == 2 ? 2 : 1)), s);
+}
+
+template <typename T, int J>
+int rows_backward(const BackArgs& a, unsigned blocks, cudaStream_t s) {
+  auto kernel = a.f.layer ? (a.f.branch_norm ? block_norm_rows_backward_kernel<T, J, true, true>
+                                             : block_norm_rows_backward_kernel<T, J, true, false>)
+                          : (a.f.branch_norm ? block_norm_rows_backward_kernel<T, J, false, true>
+                                             : block_norm_rows_backward_kernel<T, J, false, false>);
+  return launch_rows<T, J, 4, 2>(kernel, a, blocks, s);
+}
+
+// Whether rows go through the warps' pipelines: rows that two to four eights a lane hold, and enough of
+// them that every warp gets four.
+bool pipelined(int64_t n, int channels, bool wide) {
+  return wide && channels > 256 && channels <= 1024 && n >= (int64_t)4 * ROW_WARPS * 2 * num_sms();
+}
+
 template <typename T>
 int forward_typed(const BlockArgs& a, cudaStream_t s) {
+  if (pipelined(a.n, a.channels, wide_rows(a)))
+    return a.channels <= 512 ? rows_forward<T, 2>(a, s) : rows_forward<T, 4>(a, s);
 #define SV_CALL(V, J, TPR) launch_forward<T, V, J, TPR>(a, s)
   SV_BLOCK_NORM_PICK(SV_CALL, a.channels, wide_rows(a));
 #undef SV_CALL
@@ -691,18 +1128,26 @@ int forward_typed(const BlockArgs& a, cudaStream_t s) {
 
 template <typename T>
 int backward_typed(const BackArgs& a, bool wide, unsigned blocks, cudaStream_t s) {
+  if (pipelined(a.f.n, a.f.channels, wide)) {
+    if (a.f.channels <= 512) return rows_backward<T, 2>(a, blocks, s);
+    // two stages of four such rows of fp32 for eight warps are more than the shared memory
+    if constexpr (sizeof(T) == 2) return rows_backward<T, 4>(a, blocks, s);
+  }
 #define SV_CALL(V, J, TPR) launch_backward<T, V, J, TPR>(a, blocks, s)
   SV_BLOCK_NORM_PICK(SV_CALL, a.f.channels, wide);
 #undef SV_CALL
 }
 
-// Rows of a piece, and how many pieces there can be (each batch element's last one is ragged).
+// Rows of a piece, and how many pieces there can be (each batch element's last one is ragged): four blocks
+// an SM of the direct kernel; one of the pipelined kernel, whose warps then have rows enough to fill
+// their pipelines (20,331 x 1024 bf16 in 592 pieces: 188 us).
 struct Pieces {
   int rows;
   int64_t most;
 };
-Pieces pieces_of(int64_t n, int64_t groups) {
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>((n + 15) / 16, (int64_t)num_sms() * BN_PIECES_PER_SM));
+Pieces pieces_of(int64_t n, int channels, int64_t groups) {
+  const int64_t per_sm = pipelined(n, channels, true) ? 1 : 4;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>((n + 15) / 16, num_sms() * per_sm));
   Pieces p;
   p.rows = (int)std::max<int64_t>(1, (n + want - 1) / want);
   p.most = (n + p.rows - 1) / p.rows + groups;
@@ -715,7 +1160,7 @@ struct BackPlan {
 };
 BackPlan back_plan(int64_t n, int channels, int64_t groups) {  // groups 0: rows are not sorted
   BackPlan p;
-  p.pieces = pieces_of(n, groups ? groups + 1 : 0);
+  p.pieces = pieces_of(n, channels, groups ? groups + 1 : 0);
   p.joined = align_up((size_t)p.pieces.most * 3 * channels * sizeof(float), 256);
   p.perm = p.joined + align_up((size_t)(groups + 1) * 3 * channels * sizeof(float), 256);
   p.offsets = p.perm + (groups ? align_up((size_t)n * sizeof(int32_t), 256) : 0);
@@ -821,7 +1266,8 @@ extern "C" size_t sv_block_norm_backward_workspace_bytes(int64_t n, int channels
 
 extern "C" int sv_block_norm_backward(const sv_block_norm_args* args, const void* dy, const void* dh,
                                       void* dx, void* dbranch, const sv_block_norm_grads* grads,
-                                      void* workspace, size_t workspace_bytes, sv_stream_t stream) {
+                                      void* workspace, size_t workspace_bytes, int32_t* status,
+                                      sv_stream_t stream) {
   BlockArgs f;
   const int rc = fill(args, "sv_block_norm_backward", &f);
   if (rc != SV_OK) return rc;
@@ -853,6 +1299,7 @@ extern "C" int sv_block_norm_backward(const sv_block_norm_args* args, const void
     SV_FAIL(SV_ERR_WORKSPACE, "sv_block_norm_backward: workspace too small or unaligned");
   cudaStream_t s = to_stream(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  f.status = status;
   BackArgs a{};
   a.f = f;
   a.dy = dy;

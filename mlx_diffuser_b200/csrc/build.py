@@ -21,7 +21,7 @@ PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libsparsevox.so")
 SOURCES = ["api.cu", "kmap.cu", "pool.cu", "topology.cu", "norm.cu", "rmsnorm.cu", "dropout.cu", "group.cu", "route.cu", "expert.cu", "expert_tc.cu", "blocknorm.cu", "linear.cu", "linear_tc.cu", "attention.cu", "attention_f32.cu", "attention_tc.cu", "backward.cu", "wgrad_tc.cu", "halo.cu", "conv_simt.cu", "conv_tc.cu", "conv_dd.cu", "conv_tf32.cu"]
-HEADERS = ["common.cuh", "dropout.cuh", "group.h", "conv.h", "linear.h", "gemm_f32.cuh", "gemm_tc.cuh", "raise.cuh", "expert.h", "attention.h"]
+HEADERS = ["common.cuh", "dropout.cuh", "rows.cuh", "group.h", "conv.h", "linear.h", "gemm_f32.cuh", "gemm_tc.cuh", "raise.cuh", "expert.h", "attention.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

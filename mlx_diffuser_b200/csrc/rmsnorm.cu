@@ -20,7 +20,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "common.cuh"
+#include "rows.cuh"
 
 namespace sv {
 namespace {
@@ -346,71 +346,6 @@ __global__ void __launch_bounds__(kBlock<TPR>)
 // row's load and its store. 40,662 x 1024 bf16 + residual to e4m3: 75 -> 50 us (5.9 TB/s); the backward
 // pass of 20,331 rows: 72 -> 35 us (4.8 TB/s).
 
-constexpr int ROW_WARPS = 8;
-
-template <typename T, int J>
-struct RowRing {
-  static constexpr int V = 16 / sizeof(T);
-  static constexpr int ROW = 32 * J * 16;  // bytes of the widest row
-  static constexpr int SMEM(int tensors, int stages) {
-    return ROW_WARPS * (tensors * stages * ROW + stages * 8) + 16;
-  }
-};
-
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4& raw, float (&v)[16 / sizeof(T)]) {
-  const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-  for (int k = 0; k < 16 / (int)sizeof(T); ++k) v[k] = to_f32(e[k]);
-}
-
-// Calls row(r, stage) for the warp's rows with their TENSORS rows in shared memory (base + tensor *
-// ROW), STAGES rows ahead; row() has read them when it returns.
-template <typename T, int J, int TENSORS, int STAGES, typename Src, typename Row>
-__device__ __forceinline__ bool run_rows(uint8_t* smem, int64_t n, uint32_t bytes, int tensors,
-                                         volatile int* abort_flag, Src&& src, Row&& row) {
-  using Ring = RowRing<T, J>;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* ring = smem + warp * TENSORS * STAGES * Ring::ROW;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ROW_WARPS * TENSORS * STAGES * Ring::ROW) +
-                   warp * STAGES;
-  if (lane == 0) {
-    for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
-  const int64_t first = (int64_t)blockIdx.x * ROW_WARPS + warp;
-  const int64_t step = (int64_t)gridDim.x * ROW_WARPS;
-  auto load = [&](int64_t r, int s) {
-    if (lane == 0 && r < n) {
-      mbar_arrive_expect_tx(&full[s], bytes * tensors);
-      for (int t = 0; t < tensors; ++t)
-        bulk_load(smem_u32(ring + (s * TENSORS + t) * Ring::ROW), src(t, r), bytes, &full[s]);
-    }
-  };
-#pragma unroll
-  for (int s = 0; s < STAGES; ++s) load(first + s * step, s);
-  int s = 0, phase = 0;
-  for (int64_t r = first; r < n; r += step) {
-    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], phase, abort_flag))) {
-      // the warp's copies in flight write its ring: let them land
-      const uint64_t t0 = global_timer_ns();
-      while (global_timer_ns() - t0 < 10000000ull) {
-      }
-      return false;
-    }
-    row(r, ring + s * TENSORS * Ring::ROW, [&] {
-      __syncwarp();  // every lane has read the stage
-      load(r + STAGES * step, s);
-    });
-    if (++s == STAGES) {
-      s = 0;
-      phase ^= 1;
-    }
-  }
-  return true;
-}
-
 template <typename T, int J, bool Q8>
 __global__ void __launch_bounds__(32 * ROW_WARPS, 2)
     rms_rows_kernel(const T* __restrict__ x, const T* __restrict__ res, RmsArgs a,
@@ -430,11 +365,13 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, 2)
     if (c < C) load_weight<V>(a.weight, c, w[j]);
   }
   const bool ok = run_rows<T, J, 2, STAGES>(
-      smem, a.n, C * (int)sizeof(T), res != nullptr ? 2 : 1, &s_abort,
-      [&](int t, int64_t r) -> const void* {
+      smem, (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5), (int64_t)gridDim.x * ROW_WARPS,
+      a.n,
+      C * (int)sizeof(T), res != nullptr ? 2 : 1, &s_abort,
+      [](int64_t r, int64_t) { return r; }, [&](int t, int64_t r) -> const void* {
         return t == 0 ? x + r * a.x_stride : res + r * a.res_stride;
       },
-      [&](int64_t row, const uint8_t* stage, auto&& release) {
+      [&](int64_t row, int64_t, const uint8_t* stage, auto&& release) {
         float v[J][V];
         float sq = 0.f;
 #pragma unroll
@@ -514,11 +451,13 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, 2)
   }
   const float inv_c = 1.0f / (float)C;
   const bool ok = run_rows<T, J, 3, STAGES>(
-      smem, a.n, C * (int)sizeof(T), dh != nullptr ? 3 : 2, &s_abort,
-      [&](int t, int64_t r) -> const void* {
+      smem, (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5), (int64_t)gridDim.x * ROW_WARPS,
+      a.n,
+      C * (int)sizeof(T), dh != nullptr ? 3 : 2, &s_abort,
+      [](int64_t r, int64_t) { return r; }, [&](int t, int64_t r) -> const void* {
         return t == 0 ? h + r * a.x_stride : (t == 1 ? dy : dh) + r * C;
       },
-      [&](int64_t row, const uint8_t* stage, auto&& release) {
+      [&](int64_t row, int64_t, const uint8_t* stage, auto&& release) {
         const float rstd = __ldg(a.rstd + row);
         float dot = 0.f;
 #pragma unroll

@@ -10,7 +10,8 @@
 // warp of the logit's bits in an order that integers have, then a minimum over the indices that have it:
 // two warp reductions. NaN counts as the largest and gives NaN weights, as a softmax does.
 // 40,662 rows of 64 fp32 logits are 10 MB: HBM's 2 us are below the launches, and the selection's
-// instructions and the sort's steps bound the call.
+// instructions and the sort's steps bound the call. The blocks that choose also count, which is the
+// sort's first step; for few rows one block does all of it.
 #include <algorithm>
 
 #include "group.h"
@@ -61,56 +62,94 @@ __device__ __forceinline__ float total_of(const uint32_t (&key)[L], float top) {
   return warp_sum(s);
 }
 
+// A row by a warp: lane j has choice j's expert (-1: none) and weight.
 template <typename T, int L>
-__global__ void __launch_bounds__(ROUTE_WARPS * 32)
-    route_kernel(const T* logits, int64_t stride, int64_t n, int experts, int k, bool normalize,
-                 int32_t* chosen, float* weights) {
+__device__ __forceinline__ void route_row(const T* row, int experts, int k, bool normalize, int& pick,
+                                          float& w) {
   const int lane = threadIdx.x & 31;
-  const int64_t step = (int64_t)gridDim.x * ROUTE_WARPS;
-  for (int64_t row = (int64_t)blockIdx.x * ROUTE_WARPS + (threadIdx.x >> 5); row < n; row += step) {
-    uint32_t key[L];
-    load_logits<T, L>(logits + row * stride, experts, key);
-    uint32_t mine = TAKEN;  // the lane's largest
+  uint32_t key[L];
+  load_logits<T, L>(row, experts, key);
+  uint32_t mine = TAKEN;  // the lane's largest
 #pragma unroll
-    for (int i = 0; i < L; ++i) mine = max(mine, key[i]);
-    const uint32_t first = __reduce_max_sync(0xffffffffu, mine);
-    const bool some = first > MINUS_INF;
-    const float top = some ? value_of(first) : 0.0f;
-    float total = 0.0f;
-    if (!normalize) total = total_of<L>(key, top);
-    int pick = -1;  // of choice `lane`
-    float value = 0.0f;
-    uint32_t best = first;
-    for (int j = 0; j < k && best > MINUS_INF; ++j) {
-      int at = INT32_MAX;
-      if (mine == best) {
+  for (int i = 0; i < L; ++i) mine = max(mine, key[i]);
+  uint32_t best = __reduce_max_sync(0xffffffffu, mine);
+  const float top = best > MINUS_INF ? value_of(best) : 0.0f;
+  float total = 0.0f;
+  if (!normalize) total = total_of<L>(key, top);
+  pick = -1;
+  float value = 0.0f;
+  for (int j = 0; j < k && best > MINUS_INF; ++j) {
+    int at = INT32_MAX;
+    if (mine == best) {
 #pragma unroll
-        for (int i = L - 1; i >= 0; --i)
-          if (key[i] == best) at = i * 32 + lane;
-      }
-      const int e = __reduce_min_sync(0xffffffffu, at);
-      if (lane == j) {
-        pick = e;
-        value = value_of(best);
-      }
-      if (at == e) {
-        mine = TAKEN;
-#pragma unroll
-        for (int i = 0; i < L; ++i) {
-          if (i * 32 + lane == e) key[i] = TAKEN;
-          mine = max(mine, key[i]);
-        }
-      }
-      best = __reduce_max_sync(0xffffffffu, mine);
+      for (int i = L - 1; i >= 0; --i)
+        if (key[i] == best) at = i * 32 + lane;
     }
-    float w = pick >= 0 ? expf(value - top) : 0.0f;
-    if (normalize) total = warp_sum(w);
-    if (pick >= 0) w /= total;
+    const int e = __reduce_min_sync(0xffffffffu, at);
+    if (lane == j) {
+      pick = e;
+      value = value_of(best);
+    }
+    if (at == e) {
+      mine = TAKEN;
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        if (i * 32 + lane == e) key[i] = TAKEN;
+        mine = max(mine, key[i]);
+      }
+    }
+    best = __reduce_max_sync(0xffffffffu, mine);
+  }
+  w = pick >= 0 ? expf(value - top) : 0.0f;
+  if (normalize) total = warp_sum(w);
+  if (pick >= 0) w /= total;
+}
+
+// Blocks take `per` rows each and count their slots by expert for the sort's second step.
+template <typename T, int L>
+__global__ void __launch_bounds__(1024)
+    route_kernel(const T* logits, int64_t stride, int64_t n, int64_t per, int experts, int k,
+                 bool normalize, int32_t* chosen, float* weights, int32_t* counts) {
+  __shared__ int32_t mine[ROUTE_MAX_EXPERTS + 1];
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i <= experts; i += 1024) mine[i] = 0;
+  __syncthreads();
+  const int64_t first = min(blockIdx.x * per, n), last = min(first + per, n);
+  for (int64_t row = first + (threadIdx.x >> 5); row < last; row += 32) {
+    int pick;
+    float w;
+    route_row<T, L>(logits + row * stride, experts, k, normalize, pick, w);
+    if (lane < k) {
+      chosen[row * k + lane] = pick;
+      weights[row * k + lane] = w;
+      atomicAdd(mine + (pick >= 0 ? pick : experts), 1);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i <= experts; i += 1024)
+    counts[(int64_t)i * gridDim.x + blockIdx.x] = mine[i];
+}
+
+// Few rows: choices and sort in one block.
+template <typename T, int L>
+__global__ void __launch_bounds__(1024)
+    route_small_kernel(const T* logits, int64_t stride, int n, int experts, int k, bool normalize,
+                       int32_t* chosen, float* weights, int32_t* order, int32_t* offsets,
+                       int32_t* place) {
+  extern __shared__ int32_t counts[];
+  __shared__ int32_t part[32];
+  const int lane = threadIdx.x & 31;
+  for (int row = threadIdx.x >> 5; row < n; row += 32) {
+    int pick;
+    float w;
+    route_row<T, L>(logits + row * stride, experts, k, normalize, pick, w);
     if (lane < k) {
       chosen[row * k + lane] = pick;
       weights[row * k + lane] = w;
     }
   }
+  __syncthreads();  // the block's choices are in memory
+  group_block(chosen, 1, n * k, experts, order, offsets, place, counts, part);
 }
 
 template <typename T, int L>
@@ -172,22 +211,48 @@ struct RouteArgs {
   float* weights;
   const float* dweights;  // the backward pass
   void* dlogits;
+  int32_t *order, *offsets, *place, *counts;  // the forward pass
 };
+
+// Rows that one block chooses for: eight a warp, about what a second launch costs.
+constexpr int ROUTE_SMALL = 256;
+// The rows' slots are cut between the blocks at rows.
+GroupPlan route_plan(int64_t n, int experts, int k) {
+  GroupPlan p = group_plan(n * k, experts);
+  p.small = p.small && n <= ROUTE_SMALL;
+  if (p.small) return p;
+  p.warps = std::max(1, std::min(16, GROUP_COUNTS / (experts + 1) - 2));
+  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((n + 31) / 32, num_sms()));
+  const int64_t rows = (n + blocks - 1) / blocks;
+  p.blocks = (int)blocks;
+  p.per = rows * k;
+  return p;
+}
 
 template <typename T, int L>
 int launch_route(const RouteArgs& a, cudaStream_t s) {
-  const unsigned blocks = (unsigned)std::min<int64_t>((a.n + ROUTE_WARPS - 1) / ROUTE_WARPS,
-                                                      (int64_t)num_sms() * 8);
   const T* x = static_cast<const T*>(a.logits);
-  if (a.dlogits)
+  if (a.dlogits) {
+    const unsigned blocks = (unsigned)std::min<int64_t>((a.n + ROUTE_WARPS - 1) / ROUTE_WARPS,
+                                                        (int64_t)num_sms() * 8);
     route_backward_kernel<T, L><<<blocks, ROUTE_WARPS * 32, 0, s>>>(
         x, a.stride, a.n, a.experts, a.k, a.normalize, a.chosen, a.weights, a.dweights,
         static_cast<T*>(a.dlogits));
-  else
-    route_kernel<T, L><<<blocks, ROUTE_WARPS * 32, 0, s>>>(x, a.stride, a.n, a.experts, a.k,
-                                                           a.normalize, a.chosen, a.weights);
+    SV_LAUNCH_CHECK();
+    return SV_OK;
+  }
+  const GroupPlan p = route_plan(a.n, a.experts, a.k);
+  if (p.small) {
+    const size_t bytes = (size_t)(a.experts + 1) * 64 * sizeof(int32_t);
+    route_small_kernel<T, L><<<1, 1024, bytes, s>>>(x, a.stride, (int)a.n, a.experts, a.k, a.normalize,
+                                                    a.chosen, a.weights, a.order, a.offsets, a.place);
+    SV_LAUNCH_CHECK();
+    return SV_OK;
+  }
+  route_kernel<T, L><<<p.blocks, 1024, 0, s>>>(x, a.stride, a.n, p.per / a.k, a.experts, a.k,
+                                               a.normalize, a.chosen, a.weights, a.counts);
   SV_LAUNCH_CHECK();
-  return SV_OK;
+  return group_place(p, a.chosen, 1, a.n * a.k, a.experts, a.counts, a.order, a.offsets, a.place, s);
 }
 
 template <typename T>
@@ -228,7 +293,8 @@ using namespace sv;
 
 extern "C" size_t sv_route_workspace_bytes(int64_t n, int experts, int k) {
   if (check_route(n, experts, k, SV_FLOAT32, "sv_route") != SV_OK) return 0;
-  return group_rows_bytes(n * k, experts);
+  const GroupPlan p = route_plan(n, experts, k);
+  return p.small ? 0 : align_up((size_t)(experts + 1) * p.blocks * sizeof(int32_t), 256);
 }
 
 extern "C" int sv_route(const void* logits, int64_t stride, int64_t n, int experts, int k, int dtype,
@@ -240,16 +306,12 @@ extern "C" int sv_route(const void* logits, int64_t stride, int64_t n, int exper
   if (!offsets || (n > 0 && (!logits || !chosen || !weights || !order || !place)))
     SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_route: null pointer");
   if (stride < experts) SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_route: row stride below the row length");
-  const size_t need = group_rows_bytes(n * k, experts);
+  const size_t need = sv_route_workspace_bytes(n, experts, k);
   if (need && (!workspace || workspace_bytes < need))
     SV_FAIL(SV_ERR_WORKSPACE, "sv_route: workspace too small");
-  cudaStream_t s = to_stream(stream);
-  if (n > 0) {
-    const RouteArgs a{logits, stride, n, experts, k, normalize != 0, chosen, weights, nullptr, nullptr};
-    const int bad = route_any(a, dtype, s);
-    if (bad != SV_OK) return bad;
-  }
-  return group_rows(chosen, 1, n * k, experts, order, offsets, place, workspace, s);
+  const RouteArgs a{logits, stride, n, experts, k, normalize != 0, chosen, weights, nullptr, nullptr,
+                    order, offsets, place, static_cast<int32_t*>(workspace)};
+  return route_any(a, dtype, to_stream(stream));
 }
 
 extern "C" int sv_route_backward(const void* logits, int64_t stride, int64_t n, int experts, int k,
@@ -264,6 +326,6 @@ extern "C" int sv_route_backward(const void* logits, int64_t stride, int64_t n, 
   if (stride < experts)
     SV_FAIL(SV_ERR_INVALID_ARGUMENT, "sv_route_backward: row stride below the row length");
   const RouteArgs a{logits, stride, n, experts, k, normalize != 0, const_cast<int32_t*>(chosen),
-                    const_cast<float*>(weights), dweights, dlogits};
+                    const_cast<float*>(weights), dweights, dlogits, nullptr, nullptr, nullptr, nullptr};
   return route_any(a, dtype, to_stream(stream));
 }

@@ -83,7 +83,7 @@ class _BlockNorm(torch.autograd.Function):
             ws = N.workspace(nbytes, dev)
         rc = N.call(dev, lib.sv_block_norm_backward, o.pack(0, 0, branch, h, stats, coords, seed_at),
                     N.ptr(dy), N.ptr(dh), N.ptr(dx), N.ptr(dbranch), N.BLOCK_NORM_GRADS.pack(*rows),
-                    N.ptr(ws), nbytes, N.stream(dev))
+                    N.ptr(ws), nbytes, N.status_word(dev).data_ptr(), N.stream(dev))
         if rc:
             N.check(rc, "block_norm (backward)")
         return dx, dbranch, None, None, None, *grads

@@ -50,19 +50,19 @@ def _route(logits, k, normalize):
     dev = logits.device
     lib = N.load()
     weights = torch.empty((n, k), dtype=torch.float32, device=dev)
-    # one allocation for what is integer: a call of few rows is bound by its host steps
-    slots = n * k
-    words = torch.empty((3 * slots + e + 1,), dtype=torch.int32, device=dev)
-    experts, place, order, offsets = words.split((slots, slots, slots, e + 1))
+    experts = torch.empty((n, k), dtype=torch.int32, device=dev)
+    place = torch.empty_like(experts)
+    order = experts.new_empty((n * k,))
+    offsets = experts.new_empty((e + 1,))
     nbytes = lib.sv_route_workspace_bytes(n, e, k)
     ws = N.workspace(nbytes, dev) if nbytes else None
-    at = words.data_ptr()
     rc = N.call(dev, lib.sv_route, logits.data_ptr(), max(logits.stride(0), e), n, e, k,
-                N.DTYPE_CODE[logits.dtype], normalize, at, weights.data_ptr(), at + 8 * slots,
-                at + 12 * slots, at + 4 * slots, N.ptr(ws), nbytes, N.stream(dev))
+                N.DTYPE_CODE[logits.dtype], normalize, experts.data_ptr(), weights.data_ptr(),
+                order.data_ptr(), offsets.data_ptr(), place.data_ptr(), N.ptr(ws), nbytes,
+                N.stream(dev))
     if rc:
         N.check(rc, "route")
-    return weights, experts.view(n, k), order, offsets, place.view(n, k)
+    return weights, experts, order, offsets, place
 
 
 class _Route(torch.autograd.Function):
