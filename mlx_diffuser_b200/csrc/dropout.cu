@@ -8,51 +8,76 @@ namespace sv {
 namespace {
 
 template <typename T>
-__device__ __forceinline__ void load_eight(const T* p, float (&v)[8]) {
+struct Eight {
   alignas(16) T e[8];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(e) / 16; ++i)
-    reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < (int)sizeof(e) / 16; ++i)
+      reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
-}
+    for (int i = 0; i < (int)sizeof(e) / 16; ++i)
+      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
+  }
+};
 
-// A thread takes counters (eight elements) a grid apart. WIDE: every pointer 16-byte aligned, so that
-// only the last counter is read and written element by element.
+// A thread takes AHEAD counters (eight elements each) a grid apart at a time, their loads together. WIDE:
+// every pointer 16-byte aligned, and all but the last counter's elements in 16-byte accesses. A pass over
+// 40,662 x 1024 bf16 is 167 MB, 25 us of HBM, and 160 instructions a counter took 38 us: a counter's ten
+// rounds are 40 with the keys in registers, and the eight selections 28.
 template <typename T, bool WIDE, bool RES>
 __global__ void __launch_bounds__(256)
-    dropout_kernel(const T* x, const T* residual, T* out,
-                   int64_t cells, Dropout d) {
-  const uint64_t seed = seed_of(d);
-  const int64_t groups = (cells + 7) / 8, step = (int64_t)gridDim.x * 256;
-#pragma unroll 2
-  for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < groups; g += step) {
-    const int64_t at = g * 8;
-    const int left = (int)min((int64_t)8, cells - at);
-    float v[8], r[8];
-    if (WIDE && left == 8) {
-      load_eight(x + at, v);
-      if constexpr (RES) load_eight(residual + at, r);
-    } else {
+    dropout_kernel(const T* x, const T* residual, T* out, int64_t cells, Dropout d) {
+  constexpr int AHEAD = 2;
+  PhiloxKeys keys(seed_of(d));
+  keys.held();
+  const int64_t step = (int64_t)gridDim.x * 256, whole = WIDE ? cells / 8 : 0;
+  int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  auto work = [&](int64_t at, const Eight<T>& from, const Eight<T>& add, Eight<T>& to) {
+    float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = i < left ? to_f32(x[at + i]) : 0.0f;
-        if constexpr (RES) r[i] = i < left ? to_f32(residual[at + i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(from.e[i]);
+    if (d.cut) drop_eight(v, philox((uint64_t)at, d.subsequence, keys), d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) to.e[i] = from_f32<T>(RES ? v[i] + to_f32(add.e[i]) : v[i]);
+  };
+  if constexpr (WIDE) {
+    for (; g + (AHEAD - 1) * step < whole; g += AHEAD * step) {
+      Eight<T> from[AHEAD], add[AHEAD];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        from[a].load(x + (g + a * step) * 8);
+        if constexpr (RES) add[a].load(residual + (g + a * step) * 8);
+      }
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        Eight<T> to;
+        work(g + a * step, from[a], add[a], to);
+        to.store(out + (g + a * step) * 8);
       }
     }
-    if (d.cut) drop_eight(v, philox((uint64_t)g, d.subsequence, seed), d);
-    alignas(16) T e[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(RES ? v[i] + r[i] : v[i]);
-    if (WIDE && left == 8) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(e) / 16; ++i)
-        reinterpret_cast<uint4*>(out + at)[i] = reinterpret_cast<const uint4*>(e)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < left) out[at + i] = e[i];
+    for (; g < whole; g += step) {
+      Eight<T> from, add, to;
+      from.load(x + g * 8);
+      if constexpr (RES) add.load(residual + g * 8);
+      work(g, from, add, to);
+      to.store(out + g * 8);
     }
+  }
+  for (; g * 8 < cells; g += step) {  // element by element
+    Eight<T> from, add, to;
+    const int64_t at = g * 8;
+    const int left = (int)min((int64_t)8, cells - at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      from.e[i] = i < left ? x[at + i] : from_f32<T>(0.0f);
+      if constexpr (RES) add.e[i] = i < left ? residual[at + i] : from_f32<T>(0.0f);
+    }
+    work(g, from, add, to);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) out[at + i] = to.e[i];
   }
 }
 

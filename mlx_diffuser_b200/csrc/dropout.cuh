@@ -36,21 +36,38 @@ __device__ __forceinline__ uint64_t seed_of(const Dropout& d) {
   return d.seed_at ? __ldg(reinterpret_cast<const unsigned long long*>(d.seed_at)) : d.seed;
 }
 
-__device__ __forceinline__ uint4 philox(uint64_t group, uint64_t subsequence, uint64_t seed) {
+// The keys of the ten rounds. held(): in registers, where a loop has 20 to spare; left to itself the
+// compiler adds them up again for every counter, a sixth of its instructions.
+struct PhiloxKeys {
+  uint32_t low[10], high[10];
+  __device__ __forceinline__ explicit PhiloxKeys(uint64_t seed) {
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+      low[r] = (uint32_t)seed + (uint32_t)r * 0x9E3779B9u;
+      high[r] = (uint32_t)(seed >> 32) + (uint32_t)r * 0xBB67AE85u;
+    }
+  }
+  __device__ __forceinline__ void held() {
+#pragma unroll
+    for (int r = 0; r < 10; ++r) asm volatile("" : "+r"(low[r]), "+r"(high[r]));
+  }
+};
+
+__device__ __forceinline__ uint4 philox(uint64_t group, uint64_t subsequence, const PhiloxKeys& key) {
   uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32);
   uint32_t c2 = (uint32_t)subsequence, c3 = (uint32_t)(subsequence >> 32);
-  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ key.low[r];
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ key.high[r];
     c3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
+}
+__device__ __forceinline__ uint4 philox(uint64_t group, uint64_t subsequence, uint64_t seed) {
+  return philox(group, subsequence, PhiloxKeys(seed));
 }
 
 // Bit i: element i of the counter's eight is kept. A half is compared where it stands, in a word's upper
@@ -69,12 +86,17 @@ __device__ __forceinline__ uint32_t kept_eight(const uint4& r, const Dropout& d)
 
 // v[0..7], the elements of one counter: scaled, or zero whatever they were.
 __device__ __forceinline__ void drop_eight(float (&v)[8], const uint4& r, const Dropout& d) {
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w}, cut = d.cut << 16;
-  const bool none = d.cut >= 65536u;
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  if (d.cut >= 65536u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    return;
+  }
+  const uint32_t cut = d.cut << 16;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[2 * i] = (w[i] << 16) >= cut && !none ? v[2 * i] * d.scale : 0.0f;
-    v[2 * i + 1] = w[i] >= cut && !none ? v[2 * i + 1] * d.scale : 0.0f;
+    v[2 * i] = (w[i] << 16) >= cut ? v[2 * i] * d.scale : 0.0f;
+    v[2 * i + 1] = w[i] >= cut ? v[2 * i + 1] * d.scale : 0.0f;
   }
 }
 
