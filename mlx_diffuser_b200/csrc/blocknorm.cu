@@ -66,6 +66,7 @@ struct BackArgs {
   const int32_t* offsets;  // [batch + 1], or null: one group
   int piece;               // rows of a piece
   float* partial;          // [pieces][3][C], or null: no sums are wanted
+  int* done;               // set to zero
   bool want_e;
 };
 
@@ -222,14 +223,14 @@ __device__ __forceinline__ int column(int j, int t) {
 // Which of a thread's elements are kept, bit i of word j: the V elements of access j.
 template <int V, int J, int TPR>
 __device__ __forceinline__ void kept_row(uint32_t (&kept)[J], int64_t row, int channels, int t,
-                                         uint64_t seed, const Dropout& d) {
+                                         const PhiloxKeys& keys, const Dropout& d) {
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int c = (j * TPR + t) * V;
     kept[j] = 0u;
     if (c >= channels) continue;
     const uint64_t at = (uint64_t)row * channels + c;
-    kept[j] = V == 8 ? kept_eight(philox(at >> 3, d.subsequence, seed), d) : kept_one(at, seed, d);
+    kept[j] = V == 8 ? kept_eight(philox(at >> 3, d.subsequence, keys), d) : kept_one(at, keys, d);
   }
 }
 template <int V, int J>
@@ -281,7 +282,8 @@ __global__ void __launch_bounds__(kThreads<TPR>)
   RowSum<TPR> sum{part, 0};
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int C = a.channels;
-  const uint64_t seed = a.drop.cut ? seed_of(a.drop) : 0;
+  PhiloxKeys keys(a.drop.cut ? seed_of(a.drop) : 0);
+  keys.held();
   float gg[J][V], mul[J][V], add[J][V];
   int64_t held = -2, b_next = -2;
   Raw<T, V> raw_x[J], raw_d[J];
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(kThreads<TPR>)
     }
     if (a.drop.cut) {
       uint32_t kept[J];
-      kept_row<V, J, TPR>(kept, row, C, t, seed, a.drop);
+      kept_row<V, J, TPR>(kept, row, C, t, keys, a.drop);
       drop_row<V, J>(d, kept, a.drop.scale);
     }
     float2 sd = make_float2(0.0f, 1.0f);
@@ -374,6 +376,7 @@ __global__ void __launch_bounds__(kThreads<TPR>)
   __shared__ float joined[ROWS > 1 ? THREADS * V * J : 1];
   RowSum<TPR> sum{part, 0};
   const BlockArgs& f = a.f;
+  if (a.done && blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int C = f.channels;
   Piece p{0, 0, 0};
@@ -386,7 +389,8 @@ __global__ void __launch_bounds__(kThreads<TPR>)
   }
   if (p.group < 0) return;  // the whole block
   const int64_t b = p.group < f.batch ? p.group : -1;
-  const uint64_t seed = f.drop.cut ? seed_of(f.drop) : 0;
+  PhiloxKeys keys(f.drop.cut ? seed_of(f.drop) : 0);
+  keys.held();
   float gg[J][V], mul[J][V];
   auto coefs = [&](int j, float (&g)[V], float (&m)[V]) {
     const int c = column<V, TPR>(j, t);
@@ -454,7 +458,7 @@ __global__ void __launch_bounds__(kThreads<TPR>)
     }
     uint32_t kept[J];  // for the branch and for its gradient
     if (f.drop.cut) {
-      kept_row<V, J, TPR>(kept, row, C, t, seed, f.drop);
+      kept_row<V, J, TPR>(kept, row, C, t, keys, f.drop);
       drop_row<V, J>(d, kept, f.drop.scale);
     }
     float s1 = 0.0f, s2 = 0.0f;
@@ -644,7 +648,8 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, sizeof(T) == 2 ? 2 : 1)
   }
   __syncthreads();
   int b_lane = 0;  // the batch elements of the warp's next 32 rows, a lane each
-  const uint64_t seed = a.drop.cut ? seed_of(a.drop) : 0;
+  PhiloxKeys keys(a.drop.cut ? seed_of(a.drop) : 0);
+  keys.held();
   const float inv = 1.0f / (float)C;
   const bool ok = run_rows<T, J * (int)sizeof(T) / 2, 2, L::STAGES>(
       smem, first + warp, ROW_WARPS, last, C * (int)sizeof(T), 2, &s_abort,
@@ -669,7 +674,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, sizeof(T) == 2 ? 2 : 1)
             load_eight<T>(stage, q, x[j]);
             load_eight<T>(stage + Ring::ROW, q, d[j]);
             if (a.drop.cut)
-              drop_eight(d[j], philox(((uint64_t)row * C >> 3) + q, a.drop.subsequence, seed), a.drop);
+              drop_eight(d[j], philox(((uint64_t)row * C >> 3) + q, a.drop.subsequence, keys), a.drop);
           } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[j][i] = d[j][i] = 0.0f;
@@ -766,6 +771,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = f.channels;
   const Folded<J> table{reinterpret_cast<float*>(smem + L::TABLE)};
+  if (a.done && blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
   Piece p{0, 0, 0};
   if (a.offsets) {
     p = find_piece<true>(a.offsets, (int)f.batch, (int)f.n, a.piece, blockIdx.x);
@@ -784,7 +790,8 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, 1)
     table.store(1, q, m);
   }
   __syncthreads();
-  const uint64_t seed = f.drop.cut ? seed_of(f.drop) : 0;
+  PhiloxKeys keys(f.drop.cut ? seed_of(f.drop) : 0);
+  keys.held();
   const bool with_d = BRANCH || a.want_e;
   float sum_a[J][8], sum_b[J][8], sum_e[J][8];
 #pragma unroll
@@ -876,7 +883,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, 1)
           }
           if (a.dx) store_row<T, 8>(static_cast<T*>(a.dx) + row * C + q * 8, D[j]);
           if (f.drop.cut)
-            kept[j] = kept_eight(philox(((uint64_t)row * C >> 3) + q, f.drop.subsequence, seed), f.drop);
+            kept[j] = kept_eight(philox(((uint64_t)row * C >> 3) + q, f.drop.subsequence, keys), f.drop);
           if (with_d) {
             float d[8];
             load_eight<T>(stage + at_d * Ring::ROW, q, d);
@@ -953,8 +960,12 @@ struct Grad {
 };
 struct SumArgs {
   BlockArgs f;
-  int groups;         // batch elements, and one for the rows without
-  const float* sums;  // [groups][3][C]
+  const int32_t* offsets;
+  int piece;
+  const float* partial;
+  int groups;   // batch elements, and one for the rows without
+  float* sums;  // [groups][3][C]
+  int* done;    // zeroed by the kernel before
   Grad weight, bias, branch_weight, gate, scale, shift;
 };
 
@@ -965,53 +976,16 @@ __device__ __forceinline__ void store_grad(const Grad& g, int64_t b, int c, floa
   else static_cast<__nv_bfloat16*>(g.p)[at] = __float2bfloat16_rn(v);
 }
 
-// The sums of a batch element's pieces (blockIdx.y), 32 of the 3 C columns a block: its 32 warps share the
-// pieces and are joined in order.
-__global__ void __launch_bounds__(1024)
-    block_norm_join_kernel(const float* partial, const int32_t* offsets, int64_t n, int batch,
-                           int piece, int64_t cols, float* out) {
-  __shared__ float s[32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-  int64_t first = 0, pieces = (n + piece - 1) / piece;
-  if (offsets) {
-    for (int g0 = 0; g0 <= (int)blockIdx.y; g0 += 32) {
-      const int g = g0 + lane;
-      int mine = 0;
-      if (g <= (int)blockIdx.y) {
-        const int rows = (g < batch ? __ldg(offsets + g + 1) : (int)n) - __ldg(offsets + g);
-        mine = (rows + piece - 1) / piece;
-      }
-      const int all = __reduce_add_sync(0xffffffffu, g < (int)blockIdx.y ? mine : 0);
-      first += all;
-      pieces = __reduce_add_sync(0xffffffffu, g == (int)blockIdx.y ? mine : 0);
-    }
-  }
-  float v = 0.0f;
-  if (c < cols) {
-    const float* from = partial + (first + warp) * cols + c;
-#pragma unroll 8
-    for (int64_t p = warp; p < pieces; p += 32, from += 32 * cols) v += __ldg(from);
-  }
-  s[warp][lane] = v;
-  __syncthreads();
-  if (warp != 0 || c >= cols) return;
-#pragma unroll
-  for (int i = 1; i < 32; ++i) v += s[i][lane];
-  out[blockIdx.y * cols + c] = v;
-}
-
-// A channel a thread, the batch elements in order.
-__global__ void __launch_bounds__(64) block_norm_sums_kernel(const __grid_constant__ SumArgs a) {
+// What the sums of every batch element give one channel.
+__device__ __forceinline__ void finish_channel(const SumArgs& a, int c) {
   const BlockArgs& f = a.f;
-  const int c = blockIdx.x * 64 + threadIdx.x, C = f.channels;
-  if (c >= C) return;
+  const int C = f.channels;
   float dw = 0.0f, dbeta = 0.0f, dwb = 0.0f, dgate = 0.0f, dscale = 0.0f, dshift = 0.0f;
   const float w = coef_at(f.weight, 0, c, 1.0f), beta = coef_at(f.bias, 0, c, 0.0f);
   const float wb = coef_at(f.branch_weight, 0, c, 1.0f);
   for (int g = 0; g < a.groups; ++g) {
-    const float* from = a.sums + (int64_t)g * 3 * C + c;
-    const float A = __ldg(from), B = __ldg(from + C), E = __ldg(from + 2 * C);
+    const float* from = a.sums + (int64_t)g * 3 * C + c;  // written by this launch: not through L1
+    const float A = __ldcg(from), B = __ldcg(from + C), E = __ldcg(from + 2 * C);
     const bool mod = !f.per_batch || g < f.batch;  // rows without a batch element are not modulated
     const float one = 1.0f + (mod ? coef_at(f.scale, g, c, 0.0f) : 0.0f);
     const float gate = mod ? coef_at(f.gate, g, c, 1.0f) : 1.0f;
@@ -1033,6 +1007,49 @@ __global__ void __launch_bounds__(64) block_norm_sums_kernel(const __grid_consta
   if (a.gate.p && !a.gate.stride) store_grad(a.gate, 0, c, dgate);
   if (a.scale.p && !a.scale.stride) store_grad(a.scale, 0, c, dscale);
   if (a.shift.p && !a.shift.stride) store_grad(a.shift, 0, c, dshift);
+}
+
+// The sums of a batch element's pieces (blockIdx.y), 32 of the 3 C columns a block: its 32 warps share the
+// pieces and are joined in order. The block that ends last then forms the gradients: which one that is
+// changes no sum.
+__global__ void __launch_bounds__(1024) block_norm_join_kernel(const __grid_constant__ SumArgs a) {
+  __shared__ float s[32][33];
+  __shared__ bool is_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t cols = 3 * (int64_t)a.f.channels, c = (int64_t)blockIdx.x * 32 + lane;
+  int64_t first = 0, pieces = (a.f.n + a.piece - 1) / a.piece;
+  if (a.offsets) {
+    for (int g0 = 0; g0 <= (int)blockIdx.y; g0 += 32) {
+      const int g = g0 + lane;
+      int mine = 0;
+      if (g <= (int)blockIdx.y) {
+        const int rows = (g < a.f.batch ? __ldg(a.offsets + g + 1) : (int)a.f.n) - __ldg(a.offsets + g);
+        mine = (rows + a.piece - 1) / a.piece;
+      }
+      first += __reduce_add_sync(0xffffffffu, g < (int)blockIdx.y ? mine : 0);
+      pieces = __reduce_add_sync(0xffffffffu, g == (int)blockIdx.y ? mine : 0);
+    }
+  }
+  float v = 0.0f;
+  if (c < cols) {
+    const float* from = a.partial + (first + warp) * cols + c;
+#pragma unroll 8
+    for (int64_t p = warp; p < pieces; p += 32, from += 32 * cols) v += __ldg(from);
+  }
+  s[warp][lane] = v;
+  __syncthreads();
+  if (warp == 0 && c < cols) {
+#pragma unroll
+    for (int i = 1; i < 32; ++i) v += s[i][lane];
+    a.sums[blockIdx.y * cols + c] = v;
+    __threadfence();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) is_last = atomicAdd(a.done, 1) == (int)(gridDim.x * gridDim.y) - 1;
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  for (int i = threadIdx.x; i < a.f.channels; i += 1024) finish_channel(a, i);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -1156,13 +1173,14 @@ Pieces pieces_of(int64_t n, int channels, int64_t groups) {
 
 struct BackPlan {
   Pieces pieces;
-  size_t joined, perm, offsets, scratch, total;  // `partial` is at the start
+  size_t joined, done, perm, offsets, scratch, total;  // `partial` is at the start
 };
 BackPlan back_plan(int64_t n, int channels, int64_t groups) {  // groups 0: rows are not sorted
   BackPlan p;
   p.pieces = pieces_of(n, channels, groups ? groups + 1 : 0);
   p.joined = align_up((size_t)p.pieces.most * 3 * channels * sizeof(float), 256);
-  p.perm = p.joined + align_up((size_t)(groups + 1) * 3 * channels * sizeof(float), 256);
+  p.done = p.joined + align_up((size_t)(groups + 1) * 3 * channels * sizeof(float), 256);
+  p.perm = p.done + 256;
   p.offsets = p.perm + (groups ? align_up((size_t)n * sizeof(int32_t), 256) : 0);
   p.scratch = p.offsets + (groups ? align_up((size_t)(groups + 1) * sizeof(int32_t), 256) : 0);
   p.total = p.scratch + (groups ? group_rows_bytes(n, (int)groups) : 0);
@@ -1308,6 +1326,7 @@ extern "C" int sv_block_norm_backward(const sv_block_norm_args* args, const void
   a.dbranch = dbranch;
   a.piece = plan.pieces.rows;
   a.partial = sums ? reinterpret_cast<float*>(ws) : nullptr;
+  a.done = sums ? reinterpret_cast<int*>(ws + plan.done) : nullptr;
   a.want_e = grads->gate.data || grads->branch_weight.data;
   if (groups) {
     int32_t* perm = reinterpret_cast<int32_t*>(ws + plan.perm);
@@ -1331,15 +1350,15 @@ extern "C" int sv_block_norm_backward(const sv_block_norm_args* args, const void
     if (bad != SV_OK) return bad;
   }
   if (!sums) return SV_OK;
-  const int64_t cols = 3 * (int64_t)f.channels;
+  if (f.n == 0) SV_CUDA_TRY(cudaMemsetAsync(a.done, 0, sizeof(int), s));
   SumArgs g{};
   g.f = f;
+  g.offsets = a.offsets;
+  g.piece = a.piece;
+  g.partial = a.partial;
   g.groups = f.per_batch ? (int)f.batch + 1 : 1;
-  float* joined = reinterpret_cast<float*>(ws + plan.joined);
-  g.sums = joined;
-  block_norm_join_kernel<<<dim3((unsigned)((cols + 31) / 32), (unsigned)g.groups), 1024, 0, s>>>(
-      a.partial, a.offsets, f.n, (int)f.batch, a.piece, cols, joined);
-  SV_LAUNCH_CHECK();
+  g.sums = reinterpret_cast<float*>(ws + plan.joined);
+  g.done = a.done;
   g.weight = to_grad(grads->weight);
   g.bias = to_grad(grads->bias);
   g.branch_weight = to_grad(grads->branch_weight);
@@ -1347,7 +1366,8 @@ extern "C" int sv_block_norm_backward(const sv_block_norm_args* args, const void
   g.scale = to_grad(grads->scale);
   g.shift = to_grad(grads->shift);
   g.weight.stride = g.bias.stride = g.branch_weight.stride = 0;
-  block_norm_sums_kernel<<<(unsigned)((f.channels + 63) / 64), 64, 0, s>>>(g);
+  const dim3 grid((unsigned)((3 * f.channels + 31) / 32), (unsigned)g.groups);
+  block_norm_join_kernel<<<grid, 1024, 0, s>>>(g);
   SV_LAUNCH_CHECK();
   return SV_OK;
 }

@@ -66,10 +66,6 @@ __device__ __forceinline__ uint4 philox(uint64_t group, uint64_t subsequence, co
   }
   return make_uint4(c0, c1, c2, c3);
 }
-__device__ __forceinline__ uint4 philox(uint64_t group, uint64_t subsequence, uint64_t seed) {
-  return philox(group, subsequence, PhiloxKeys(seed));
-}
-
 // Bit i: element i of the counter's eight is kept. A half is compared where it stands, in a word's upper
 // half: the lower bits of the word cannot change the comparison with cut 2^16.
 __device__ __forceinline__ uint32_t kept_eight(const uint4& r, const Dropout& d) {
@@ -101,8 +97,8 @@ __device__ __forceinline__ void drop_eight(float (&v)[8], const uint4& r, const 
 }
 
 // Whether element `at` by itself is kept.
-__device__ __forceinline__ uint32_t kept_one(uint64_t at, uint64_t seed, const Dropout& d) {
-  return kept_eight(philox(at >> 3, d.subsequence, seed), d) >> ((uint32_t)at & 7u) & 1u;
+__device__ __forceinline__ uint32_t kept_one(uint64_t at, const PhiloxKeys& keys, const Dropout& d) {
+  return kept_eight(philox(at >> 3, d.subsequence, keys), d) >> ((uint32_t)at & 7u) & 1u;
 }
 #endif
 

@@ -2,9 +2,9 @@
 //
 // Every warp takes a contiguous run of rows, ranks 32 of them at a time among those with the same key,
 // and knows how many rows of each key are before its own. Nothing depends on the order of execution. Up
-// to 32,768 rows one block counts, scans and places (20,331 rows in 2 groups: 8 us); more take two launches:
-// blocks count their rows, then each placing block sums the counts of the blocks before it.
-// 162,648 rows in 65 bins: 3 + 6 us; a launch's host step costs as much, and that is what bounds both.
+// to 8192 rows one block counts, scans and places; more take two launches: blocks count their rows, then
+// each placing block sums the counts of the blocks before it. 20,331 rows in 2 groups: 18 us in one
+// block, 8 us in two launches.
 #include <algorithm>
 
 #include "group.h"
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(512)
 GroupPlan group_plan(int64_t n, int groups) {
   const int bins = groups + 1;
   GroupPlan p{};
-  p.small = n <= 32768 && bins * 64 + 32 <= GROUP_COUNTS;
+  p.small = n <= 8192 && bins * 64 + 32 <= GROUP_COUNTS;
   if (p.small) return p;
   // a placing block holds a counter a warp and bin, and two more a bin
   p.warps = std::max(1, std::min(16, GROUP_COUNTS / bins - 2));
