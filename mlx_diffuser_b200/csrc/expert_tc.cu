@@ -56,6 +56,7 @@ struct ExArgs {
   int32_t steps;           // kRows
   uint32_t idesc;
   bool b_mn, wide_io, zero_tail;
+  bool direct;             // rows of the result are whole sectors
   const CUtensorMap* maps;  // kWeights: [experts][2]
 };
 
@@ -152,6 +153,60 @@ __device__ __forceinline__ void ex_finish(const Epilogue& ep, float (&v)[R][W], 
     else if (ep.act == SV_ACT_GELU) activate_all<SV_ACT_GELU>(v);
     else if (ep.act == SV_ACT_GELU_TANH) activate_all<SV_ACT_GELU_TANH>(v);
     store(static_cast<float*>(ep.out));
+  }
+}
+
+// 32 bytes to global memory in one access: a whole sector by one lane.
+__device__ __forceinline__ void store_sector(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// A lane's 32 consecutive columns of one row, straight from TMEM to whole sectors of global memory: no
+// turn through shared memory, half of the instructions an element. `bias`, `scale`: in shared memory,
+// the same address in all lanes.
+template <typename O, bool WIDE>
+__device__ __forceinline__ void ex_direct(const Epilogue& ep, float (&v)[1][32], const float* bias,
+                                          const float* scale, int64_t at) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    if (ep.col_scale) {
+      const float4 f = *reinterpret_cast<const float4*>(scale + j);
+      v[0][j] *= f.x; v[0][j + 1] *= f.y; v[0][j + 2] *= f.z; v[0][j + 3] *= f.w;
+    }
+    if (ep.bias) {
+      const float4 f = *reinterpret_cast<const float4*>(bias + j);
+      v[0][j] += f.x; v[0][j + 1] += f.y; v[0][j + 2] += f.z; v[0][j + 3] += f.w;
+    }
+  }
+  auto store32 = [&](float* to) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[0][j + i]);
+      store_sector(to + j, w);
+    }
+  };
+  if (ep.preact) store32(ep.preact + at);
+  if (ep.act == SV_ACT_SILU) activate_all<SV_ACT_SILU>(v);
+  else if (ep.act == SV_ACT_GELU) activate_all<SV_ACT_GELU>(v);
+  else if (ep.act == SV_ACT_GELU_TANH) activate_all<SV_ACT_GELU_TANH>(v);
+  if constexpr (WIDE) {
+    store32(static_cast<float*>(ep.out) + at);
+  } else {
+    O* to = static_cast<O*>(ep.out) + at;
+#pragma unroll
+    for (int j = 0; j < 32; j += 16) {
+      alignas(16) O e[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) e[i] = from_f32<O>(v[0][j + i]);
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const uint32_t*>(e)[i];
+      store_sector(to + j, w);
+    }
   }
 }
 
@@ -375,6 +430,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) raw[j] = 0u;
         }
+        if (a.direct && col + 32 <= a.n) {
+          if (lane < rows) {
+            float v[1][32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[0][j] = __uint_as_float(raw[j]);
+            ex_direct<O, WIDE>(out, v, s_bias + c, s_scale + c, (row0 + lane) * a.n + col);
+          }
+          continue;
+        }
         __syncwarp();  // the previous chunk has been read
 #pragma unroll
         for (int j = 0; j < 32; j += 4)
@@ -556,6 +620,9 @@ int launch_expert(const ExpertGemm& g, CUtensorMap* maps, int32_t* status, cudaS
   if (pieces * a.tiles_n > INT32_MAX / 2) SV_FAIL(SV_ERR_UNSUPPORTED, "expert_linear: too many tiles");
   const Epilogue& ep = g.ep;
   a.wide_io = g.n % 8 == 0 && aligned16(ep.out) && (!ep.preact || aligned16(ep.preact));
+  auto sectors = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; };
+  a.direct = g.n * (WIDE ? 4 : ES) % 32 == 0 && sectors(ep.out) && g.n % 8 == 0 && sectors(ep.preact) &&
+             (WIDE || g.m * g.n % 16 == 0);
   units = (int)std::min<int64_t>(pieces * a.tiles_n, units);
   config.gridDim = dim3((unsigned)(units * (PAIR ? 2 : 1)));
   SV_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, map_a, map_b, a, ep, status));
