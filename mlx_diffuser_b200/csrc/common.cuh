@@ -133,12 +133,16 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
                                                   volatile int* abort_flag,
                                                   uint64_t timeout_ns = 2000000000ull) {
   if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_timer_ns();
+  // The timer is read once in 256 tries: read before the second one, it was most of a short wait (a product's
+  // k steps waited 2,000 cycles a tile longer).
+  uint64_t t0 = 0;
   uint32_t spins = 0;
   while (!mbar_try_wait(bar, parity)) {
     if ((++spins & 255u) == 0) {
       if (*abort_flag) return false;
-      if (global_timer_ns() - t0 > timeout_ns) {
+      const uint64_t now = global_timer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > timeout_ns) {
         *abort_flag = 1;
         return false;
       }

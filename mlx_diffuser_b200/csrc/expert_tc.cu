@@ -2,7 +2,7 @@
 //
 // The tiles, stages and warp roles are those of linear_tc.cu: persistent CTAs, or pairs of them
 // (cta_group::2) on tiles of 256 rows, operands by TMA into 128-byte swizzled stages, one issuing
-// thread, two accumulators in TMEM, and eight epilogue warps that work on one tile while the next is
+// thread, two accumulators in TMEM, and epilogue warps that work on one tile while the next is
 // formed. What differs is where the tiles are:
 //
 //   kRows      Every expert's positions are cut into tiles of their own, so that a tile has one weight.
@@ -19,6 +19,7 @@
 //
 // Every wait on an mbarrier is bounded, and unwinds as in linear_tc.cu.
 #include <algorithm>
+#include <type_traits>
 
 #include "expert.h"
 #include "gemm_tc.cuh"
@@ -27,18 +28,28 @@ namespace sv {
 namespace {
 
 constexpr int EX_MAX = 1024;  // experts
+// Sixteen epilogue warps, four to a quadrant of TMEM lanes: with eight, the activation's special functions
+// and the rest of the epilogue did not overlap well enough to hide behind the next tile's products
+// (81,324 x 1024 x 4096 GELU: 583 us with eight; the products and loads alone: 459).
+constexpr int EX_EPI_WARPS = 16;
+constexpr int EX_EPI_THREADS = 32 * EX_EPI_WARPS;
+constexpr int EX_THREADS = 64 + EX_EPI_THREADS;
+
+__device__ __forceinline__ void ex_epi_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(EX_EPI_THREADS) : "memory");
+}
 
 template <int BN, bool PAIR>
 struct ExLayout {
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // of one CTA
   static constexpr int A_STAGE = TM * 128;
   static constexpr int B_STAGE = B_ROWS * 128;
-  static constexpr int FIT = (176 * 1024) / (A_STAGE + B_STAGE);
+  static constexpr int FIT = (140 * 1024) / (A_STAGE + B_STAGE);
   static constexpr int STAGES = FIT > 7 ? 7 : FIT;
   static constexpr int A_OFF = 0;
   static constexpr int B_OFF = STAGES * A_STAGE;
-  static constexpr int CHUNK_OFF = B_OFF + STAGES * B_STAGE;  // float [8 warps][32][CHUNK_LD]
-  static constexpr int COL_OFF = CHUNK_OFF + EPI_WARPS * 32 * CHUNK_LD * 4;  // [2][bias, scale][BN]
+  static constexpr int CHUNK_OFF = B_OFF + STAGES * B_STAGE;  // float [warps][32][CHUNK_LD]
+  static constexpr int COL_OFF = CHUNK_OFF + EX_EPI_WARPS * 32 * CHUNK_LD * 4;  // [2][bias, scale][BN]
   static constexpr int FIRST_OFF = COL_OFF + 2 * 2 * BN * 4;  // int [experts + 1]
   static constexpr int MISC_OFF = FIRST_OFF + (EX_MAX + 4) * 4;
   static constexpr int BAR_OFF = MISC_OFF + 16;
@@ -119,41 +130,43 @@ __device__ __forceinline__ ExTile ex_tile(const ExArgs& a, const int32_t* first,
   return o;
 }
 
-// finish() of gemm_tc.cuh for what the experts' epilogue has: scale, bias, argument kept, activation, and
-// results in O or, WIDE, in fp32.
+// The epilogue of R rows of W consecutive columns that came through shared memory: scale, bias, argument
+// kept, activation, and results in O or, WIDE, in fp32.
 template <typename O, bool WIDE, int R, int W>
 __device__ __forceinline__ void ex_finish(const Epilogue& ep, float (&v)[R][W], const float* bias,
                                           const float* scale, int64_t row, int step, int rows,
                                           int64_t n, int64_t col) {
-  if constexpr (!WIDE) {
-    finish<O, R, W>(ep, v, bias, scale, ep.col_scale != nullptr, row, step, rows, n, col);
-  } else {
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        if (ep.col_scale) v[i][j] *= scale[j];
-        if (ep.bias) v[i][j] += bias[j];
+    for (int j = 0; j < W; ++j) {
+      if (ep.col_scale) v[i][j] *= scale[j];
+      if (ep.bias) v[i][j] += bias[j];
+    }
+  auto store = [&](auto* to) {
+    using S = std::remove_pointer_t<decltype(to)>;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (i * step >= rows) continue;
+      S* dst = to + (row + i * step) * n + col;
+      alignas(16) S e[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) e[j] = from_f32<S>(v[i][j]);
+      if constexpr (W == 8) {
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(e) / 16; ++j)
+          reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(e)[j];
+      } else {
+        *dst = e[0];
       }
-    auto store = [&](float* to) {
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        if (i * step >= rows) continue;
-        float* dst = to + (row + i * step) * n + col;
-        if constexpr (W == 8) {
-          *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(v[i]);
-          *reinterpret_cast<float4*>(dst + 4) = *reinterpret_cast<const float4*>(v[i] + 4);
-        } else {
-          *dst = v[i][0];
-        }
-      }
-    };
-    if (ep.preact) store(ep.preact);
-    if (ep.act == SV_ACT_SILU) activate_all<SV_ACT_SILU>(v);
-    else if (ep.act == SV_ACT_GELU) activate_all<SV_ACT_GELU>(v);
-    else if (ep.act == SV_ACT_GELU_TANH) activate_all<SV_ACT_GELU_TANH>(v);
-    store(static_cast<float*>(ep.out));
-  }
+    }
+  };
+  if (ep.preact) store(ep.preact);
+  if (ep.act == SV_ACT_SILU) activate_all<SV_ACT_SILU>(v);
+  else if (ep.act == SV_ACT_GELU) activate_all<SV_ACT_GELU>(v);
+  else if (ep.act == SV_ACT_GELU_TANH) activate_all<SV_ACT_GELU_TANH>(v);
+  if constexpr (WIDE) store(static_cast<float*>(ep.out));
+  else store(static_cast<O*>(ep.out));
 }
 
 // 32 bytes to global memory in one access: a whole sector by one lane.
@@ -163,14 +176,14 @@ __device__ __forceinline__ void store_sector(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-// A lane's 32 consecutive columns of one row, straight from TMEM to whole sectors of global memory: no
+// A lane's 16 consecutive columns of one row, straight from TMEM to whole sectors of global memory: no
 // turn through shared memory, half of the instructions an element. `bias`, `scale`: in shared memory,
 // the same address in all lanes.
 template <typename O, bool WIDE>
-__device__ __forceinline__ void ex_direct(const Epilogue& ep, float (&v)[1][32], const float* bias,
+__device__ __forceinline__ void ex_direct(const Epilogue& ep, float (&v)[1][16], const float* bias,
                                           const float* scale, int64_t at) {
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
+  for (int j = 0; j < 16; j += 4) {
     if (ep.col_scale) {
       const float4 f = *reinterpret_cast<const float4*>(scale + j);
       v[0][j] *= f.x; v[0][j + 1] *= f.y; v[0][j + 2] *= f.z; v[0][j + 3] *= f.w;
@@ -182,7 +195,7 @@ __device__ __forceinline__ void ex_direct(const Epilogue& ep, float (&v)[1][32],
   }
   auto store32 = [&](float* to) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
+    for (int j = 0; j < 16; j += 8) {
       uint32_t w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[0][j + i]);
@@ -196,22 +209,18 @@ __device__ __forceinline__ void ex_direct(const Epilogue& ep, float (&v)[1][32],
   if constexpr (WIDE) {
     store32(static_cast<float*>(ep.out) + at);
   } else {
-    O* to = static_cast<O*>(ep.out) + at;
+    alignas(16) O e[16];
 #pragma unroll
-    for (int j = 0; j < 32; j += 16) {
-      alignas(16) O e[16];
+    for (int i = 0; i < 16; ++i) e[i] = from_f32<O>(v[0][i]);
+    uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) e[i] = from_f32<O>(v[0][j + i]);
-      uint32_t w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const uint32_t*>(e)[i];
-      store_sector(to + j, w);
-    }
+    for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const uint32_t*>(e)[i];
+    store_sector(static_cast<O*>(ep.out) + at, w);
   }
 }
 
 template <int BN, bool PAIR, typename O, bool WEIGHTS, bool WIDE>
-__global__ void __launch_bounds__(TC_THREADS, 1)
+__global__ void __launch_bounds__(EX_THREADS, 1)
     expert_tc_kernel(const __grid_constant__ CUtensorMap map_a,
                      const __grid_constant__ CUtensorMap map_b, ExArgs a, Epilogue ep,
                      int32_t* status) {
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], (PAIR ? 2 : 1) * EPI_WARPS);
+      mbar_init(&acc_empty[b], (PAIR ? 2 : 1) * EX_EPI_WARPS);
     }
     mbar_init(drained, 1);
     *s_abort = 0;
@@ -255,7 +264,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   }
   if (warp == 1) alloc_tmem<PAIR>(s_tmem, 2 * BN);
   if constexpr (!WEIGHTS) {
-    for (int e = threadIdx.x; e < a.experts; e += TC_THREADS) {
+    for (int e = threadIdx.x; e < a.experts; e += EX_THREADS) {
       const int2 s = segment(a, e);
       s_first[e + 1] = (s.y - s.x + ROWS - 1) / ROWS;
     }
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0, seen = -1;
+      int slot = 0, phase = 1, seen = -1;
       for (int32_t t = unit; t < total && ok; t += units) {
         const ExTile w = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, t);
         const CUtensorMap* ma = &map_a;
@@ -301,9 +310,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           }
         }
         const int32_t m0 = w.row + (int32_t)rank * TM, n0 = w.n0 + (int32_t)rank * L::B_ROWS;
-        for (int k = 0; k < w.k1; ++k, ++it) {
-          const int slot = it % S;
-          if (!mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, s_abort)) {
+        for (int k = 0; k < w.k1; ++k) {
+          if (!mbar_wait_bounded(&empty[slot], phase, s_abort)) {
             ok = false;
             break;
           }
@@ -337,6 +345,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
               load3(sb, mb, kk, n0);
             }
           }
+          if (++slot == S) {
+            slot = 0;
+            phase ^= 1;
+          }
         }
       }
       if (!ok) {
@@ -349,9 +361,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      int it = 0, local = 0;
+      // What this thread does a k step has to fit into the step's 512 cycles beside the epilogue warps on its
+      // scheduler: descriptors are a 32-bit addition each, and the next step's barrier is tried before
+      // this step's products are issued.
+      const uint64_t a0 = WEIGHTS ? smem_desc_mn_sw128(smem_u32(smem + L::A_OFF), MN_STRIDE, ATOM)
+                                  : smem_desc_sw128(smem_u32(smem + L::A_OFF));
+      const bool b_mn = WEIGHTS || a.b_mn;
+      const uint64_t b0 = b_mn ? smem_desc_mn_sw128(smem_u32(smem + L::B_OFF), MN_STRIDE, ATOM)
+                               : smem_desc_sw128(smem_u32(smem + L::B_OFF));
+      constexpr uint32_t A_STEP = WEIGHTS ? 2 * ATOM / 16 : 2;  // 16 of k, in the descriptor's units
+      const uint32_t b_step = b_mn ? 2 * ATOM / 16 : 2;
+      const uint32_t a_high = (uint32_t)(a0 >> 32), b_high = (uint32_t)(b0 >> 32);
+      int slot = 0, phase = 0, local = 0;
+      bool there = false;
       for (int32_t t = unit; t < total && ok; t += units, ++local) {
-        const ExTile w = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, t);
+        const int32_t k1 = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, t).k1;
         const int ab = local & 1;
         if (!mbar_wait_bounded(&acc_empty[ab], ((local >> 1) & 1) ^ 1, s_abort)) {
           ok = false;
@@ -359,25 +383,28 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(ab * BN);
-        for (int k = 0; k < w.k1; ++k, ++it) {
-          const int slot = it % S;
-          if (!mbar_wait_bounded(&full[slot], (it / S) & 1, s_abort)) {
+        for (int k = 0; k < k1; ++k) {
+          if (!there && !mbar_wait_bounded(&full[slot], phase, s_abort)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + L::A_OFF + slot * L::A_STAGE);
-          const uint32_t sb = smem_u32(smem + L::B_OFF + slot * L::B_STAGE);
+          uint32_t a_low = (uint32_t)a0 + slot * (L::A_STAGE / 16);
+          uint32_t b_low = (uint32_t)b0 + slot * (L::B_STAGE / 16);
+          uint64_t* const free_slot = &empty[slot];
+          if (++slot == S) {
+            slot = 0;
+            phase ^= 1;
+          }
+          there = mbar_try_wait(&full[slot], phase);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {  // 16 of k: one instruction
-            const uint64_t da = WEIGHTS ? smem_desc_mn_sw128(sa + j * 2 * ATOM, MN_STRIDE, ATOM)
-                                        : smem_desc_sw128(sa + j * 32);
-            const uint64_t db = WEIGHTS || a.b_mn
-                                    ? smem_desc_mn_sw128(sb + j * 2 * ATOM, MN_STRIDE, ATOM)
-                                    : smem_desc_sw128(sb + j * 32);
-            issue_mma<PAIR, false>(d, da, db, a.idesc, (k > 0 || j > 0) ? 1u : 0u);
+            issue_mma<PAIR, false>(d, (uint64_t)a_high << 32 | a_low, (uint64_t)b_high << 32 | b_low,
+                                   a.idesc, (k > 0 || j > 0) ? 1u : 0u);
+            a_low += A_STEP;
+            b_low += b_step;
           }
-          commit<PAIR>(&empty[slot]);
+          commit<PAIR>(free_slot);
         }
         if (ok) commit<PAIR>(&acc_full[ab]);
       }
@@ -390,7 +417,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
   } else {
     const int q = warp & 3;            // TMEM lanes 32 q .. 32 q + 31
-    const int half = (warp - 2) >> 2;  // columns half * BN / 2 ..
+    constexpr int PARTS = BN >= 128 ? 4 : 2, COLS = BN / PARTS;  // a warp's columns
+    const int part = (warp - 2) >> 2;
     const int e = threadIdx.x - 64;
     float* chunk = reinterpret_cast<float*>(smem + L::CHUNK_OFF) + (warp - 2) * 32 * CHUNK_LD;
     const bool scaled = ep.col_scale != nullptr;
@@ -403,13 +431,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       Epilogue out = ep;
       if constexpr (WEIGHTS) out.out = static_cast<O*>(ep.out) + (int64_t)w.e * a.m * a.n;
       // this buffer's last readers were two tiles ago, before the previous epi_sync
-      for (int c = e; c < BN; c += EPI_THREADS) {
+      for (int c = e; c < BN; c += EX_EPI_THREADS) {
         const bool in = w.n0 + c < a.n;
         if (ep.bias)
           s_bias[c] = in ? to_f32(static_cast<const O*>(ep.bias)[w.e * a.n + w.n0 + c]) : 0.f;
         if (scaled) s_scale[c] = in ? __ldg(ep.col_scale + w.n0 + c) : 1.f;
       }
-      epi_sync();
+      ex_epi_sync();
       if (!ok) continue;
       const int64_t row0 = (int64_t)w.row + rank * TM + q * 32;  // the warp's first row
       const int rows = (int)max((int64_t)0, min((int64_t)32, w.last - row0));
@@ -420,30 +448,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       tc_fence_after();
       const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * BN);
 #pragma unroll 1
-      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-        uint32_t raw[32];
-        tmem_ld_32x32b_x32(t_row + c, raw);
-        tc_wait_ld();
+      for (int c = part * COLS; c < min((part + 1) * COLS, BN); c += 32) {
         const int64_t col = (int64_t)w.n0 + c;
         if (rows == 0 || col >= a.n) continue;  // the same in all lanes
-        if (w.k1 == 0) {  // an expert without positions: nothing was formed
-#pragma unroll
-          for (int j = 0; j < 32; ++j) raw[j] = 0u;
-        }
         if (a.direct && col + 32 <= a.n) {
-          if (lane < rows) {
-            float v[1][32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[0][j] = __uint_as_float(raw[j]);
-            ex_direct<O, WIDE>(out, v, s_bias + c, s_scale + c, (row0 + lane) * a.n + col);
+          for (int h = 0; h < 32; h += 16) {
+            uint32_t raw[16];
+            tmem_ld_32x32b_x16(t_row + c + h, raw);
+            tc_wait_ld();
+            if (lane < rows) {
+              float v[1][16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j)  // an expert without positions: nothing was formed
+                v[0][j] = w.k1 == 0 ? 0.f : __uint_as_float(raw[j]);
+              ex_direct<O, WIDE>(out, v, s_bias + c + h, s_scale + c + h, (row0 + lane) * a.n + col + h);
+            }
+            __syncwarp();
           }
           continue;
         }
         __syncwarp();  // the previous chunk has been read
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          *reinterpret_cast<uint4*>(chunk + lane * CHUNK_LD + j) =
-              make_uint4(raw[j], raw[j + 1], raw[j + 2], raw[j + 3]);
+        for (int h = 0; h < 32; h += 16) {
+          uint32_t raw[16];
+          tmem_ld_32x32b_x16(t_row + c + h, raw);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; j += 4)
+            *reinterpret_cast<uint4*>(chunk + lane * CHUNK_LD + h + j) =
+                w.k1 == 0 ? make_uint4(0u, 0u, 0u, 0u)
+                          : make_uint4(raw[j], raw[j + 1], raw[j + 2], raw[j + 3]);
+        }
         __syncwarp();
         const int cols = (int)min((int64_t)32, a.n - col);
         if (a.wide_io && cols == 32) {
@@ -458,24 +494,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
               *reinterpret_cast<float4*>(scale + x) =
                   *reinterpret_cast<const float4*>(s_scale + c + j + x);
           }
-          float v[4][8];
+#pragma unroll 1
+          for (int i = 0; i < 32; i += 16) {  // two groups of eight rows
+            float v[2][8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float* src = chunk + (i * 8 + (lane >> 2)) * CHUNK_LD + j;
-            *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(src);
-            *reinterpret_cast<float4*>(v[i] + 4) = *reinterpret_cast<const float4*>(src + 4);
+            for (int x = 0; x < 2; ++x) {
+              const float* src = chunk + (i + x * 8 + (lane >> 2)) * CHUNK_LD + j;
+              *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(src);
+              *reinterpret_cast<float4*>(v[x] + 4) = *reinterpret_cast<const float4*>(src + 4);
+            }
+            ex_finish<O, WIDE, 2, 8>(out, v, bias, scale, row0 + i + (lane >> 2), 8,
+                                     rows - i - (lane >> 2), a.n, col + j);
           }
-          ex_finish<O, WIDE, 4, 8>(out, v, bias, scale, row0 + (lane >> 2), 8, rows - (lane >> 2), a.n,
-                                   col + j);
         } else if (lane < cols) {
           const float bias[1] = {ep.bias ? s_bias[c + lane] : 0.f};
           const float scale[1] = {scaled ? s_scale[c + lane] : 1.f};
 #pragma unroll 1
-          for (int r = 0; r < rows; r += 16) {
-            float v[16][1];
+          for (int r = 0; r < rows; r += 8) {
+            float v[8][1];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i][0] = chunk[(r + i) * CHUNK_LD + lane];
-            ex_finish<O, WIDE, 16, 1>(out, v, bias, scale, row0 + r, 1, rows - r, a.n, col + lane);
+            for (int i = 0; i < 8; ++i) v[i][0] = chunk[(r + i) * CHUNK_LD + lane];
+            ex_finish<O, WIDE, 8, 1>(out, v, bias, scale, row0 + r, 1, rows - r, a.n, col + lane);
           }
         }
       }
@@ -489,8 +528,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
     if (!WEIGHTS && a.zero_tail) {
       const int64_t end = a.slots * a.n;
-      for (int64_t i = (int64_t)segment(a, a.experts - 1).y * a.n + (int64_t)blockIdx.x * EPI_THREADS + e;
-           i < end; i += (int64_t)gridDim.x * EPI_THREADS)
+      for (int64_t i = (int64_t)segment(a, a.experts - 1).y * a.n + (int64_t)blockIdx.x * EX_EPI_THREADS + e;
+           i < end; i += (int64_t)gridDim.x * EX_EPI_THREADS)
         static_cast<O*>(ep.out)[i] = from_f32<O>(0.f);
     }
   }
@@ -558,7 +597,7 @@ int launch_expert(const ExpertGemm& g, CUtensorMap* maps, int32_t* status, cudaS
   int dev = 0;
   SV_CUDA_TRY(cudaGetDevice(&dev));
   cudaLaunchConfig_t config{};
-  config.blockDim = dim3(TC_THREADS);
+  config.blockDim = dim3(EX_THREADS);
   config.dynamicSmemBytes = L::SMEM;
   config.stream = s;
   cudaLaunchAttribute attr{};
