@@ -28,10 +28,9 @@ namespace sv {
 namespace {
 
 constexpr int EX_MAX = 1024;  // experts
-// Sixteen epilogue warps, four to a quadrant of TMEM lanes: with eight, the activation's special functions
-// and the rest of the epilogue did not overlap well enough to hide behind the next tile's products
-// (81,324 x 1024 x 4096 GELU: 583 us with eight; the products and loads alone: 459).
-constexpr int EX_EPI_WARPS = 16;
+// Eight epilogue warps: sixteen have 96 registers each, and took 868,000 cycles where eight take 714,000
+// (81,324 x 1024 x 4096 without an activation).
+constexpr int EX_EPI_WARPS = 8;
 constexpr int EX_EPI_THREADS = 32 * EX_EPI_WARPS;
 constexpr int EX_THREADS = 64 + EX_EPI_THREADS;
 
@@ -44,20 +43,30 @@ struct ExLayout {
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // of one CTA
   static constexpr int A_STAGE = TM * 128;
   static constexpr int B_STAGE = B_ROWS * 128;
-  static constexpr int FIT = (140 * 1024) / (A_STAGE + B_STAGE);
+  static constexpr int FIT = (160 * 1024) / (A_STAGE + B_STAGE);
   static constexpr int STAGES = FIT > 7 ? 7 : FIT;
   static constexpr int A_OFF = 0;
   static constexpr int B_OFF = STAGES * A_STAGE;
   static constexpr int CHUNK_OFF = B_OFF + STAGES * B_STAGE;  // float [warps][32][CHUNK_LD]
   static constexpr int COL_OFF = CHUNK_OFF + EX_EPI_WARPS * 32 * CHUNK_LD * 4;  // [2][bias, scale][BN]
   static constexpr int FIRST_OFF = COL_OFF + 2 * 2 * BN * 4;  // int [experts + 1]
-  static constexpr int MISC_OFF = FIRST_OFF + (EX_MAX + 4) * 4;
+  static constexpr int SEG_OFF = FIRST_OFF + (EX_MAX + 4) * 4;  // int2 [experts]
+  static constexpr int MISC_OFF = SEG_OFF + EX_MAX * 8;
   static constexpr int BAR_OFF = MISC_OFF + 16;
   static constexpr int NUM_BARS = 2 * STAGES + 5;
   static constexpr int SMEM = BAR_OFF + NUM_BARS * 8 + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
   static_assert(STAGES >= 4, "pipeline depth");
 };
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
 
 struct ExArgs {
   const int32_t* offsets;
@@ -101,7 +110,8 @@ struct ExTile {
 };
 
 template <int BN, bool PAIR, bool WEIGHTS>
-__device__ __forceinline__ ExTile ex_tile(const ExArgs& a, const int32_t* first, int32_t t) {
+__device__ __forceinline__ ExTile ex_tile(const ExArgs& a, const int32_t* first, const int2* seg,
+                                          int32_t t) {
   constexpr int ROWS = PAIR ? 2 * TM : TM;
   ExTile o;
   const int32_t piece = t / a.tiles_n;
@@ -110,7 +120,7 @@ __device__ __forceinline__ ExTile ex_tile(const ExArgs& a, const int32_t* first,
     o.e = piece / a.tiles_m;
     o.row = (piece - o.e * a.tiles_m) * ROWS;
     o.last = (int32_t)a.m;
-    const int2 s = segment(a, o.e);
+    const int2 s = seg[o.e];
     o.base = s.x;
     o.k1 = (s.y - s.x + 63) / 64;
   } else {
@@ -120,7 +130,7 @@ __device__ __forceinline__ ExTile ex_tile(const ExArgs& a, const int32_t* first,
       if (first[mid] <= piece) lo = mid;
       else hi = mid;
     }
-    const int2 s = segment(a, lo);
+    const int2 s = seg[lo];
     o.e = lo;
     o.row = s.x + (piece - first[lo]) * ROWS;
     o.last = s.y;
@@ -232,6 +242,7 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
                                              ~static_cast<uintptr_t>(1023));
   float* s_cols = reinterpret_cast<float*>(smem + L::COL_OFF);
   int32_t* s_first = reinterpret_cast<int32_t*>(smem + L::FIRST_OFF);
+  int2* s_seg = reinterpret_cast<int2*>(smem + L::SEG_OFF);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
@@ -263,11 +274,10 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
     }
   }
   if (warp == 1) alloc_tmem<PAIR>(s_tmem, 2 * BN);
-  if constexpr (!WEIGHTS) {
-    for (int e = threadIdx.x; e < a.experts; e += EX_THREADS) {
-      const int2 s = segment(a, e);
-      s_first[e + 1] = (s.y - s.x + ROWS - 1) / ROWS;
-    }
+  for (int e = threadIdx.x; e < a.experts; e += EX_THREADS) {
+    const int2 s = segment(a, e);
+    s_seg[e] = s;
+    s_first[e + 1] = (s.y - s.x + ROWS - 1) / ROWS;
   }
   __syncthreads();
   if (!WEIGHTS && warp == 2) {  // tiles of the experts before each
@@ -297,7 +307,7 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
     if (lane == 0) {
       int slot = 0, phase = 1, seen = -1;
       for (int32_t t = unit; t < total && ok; t += units) {
-        const ExTile w = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, t);
+        const ExTile w = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, s_seg, t);
         const CUtensorMap* ma = &map_a;
         const CUtensorMap* mb = &map_b;
         if constexpr (WEIGHTS) {
@@ -360,10 +370,11 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      // What this thread does a k step has to fit into the step's 512 cycles beside the epilogue warps on its
-      // scheduler: descriptors are a 32-bit addition each, and the next step's barrier is tried before
-      // this step's products are issued.
+    if (rank == 0) {
+      // What this warp does a k step has to fit into the step's 512 cycles beside the epilogue warps on its
+      // scheduler. All of it walks the loop, so that descriptors and addresses are uniform registers, one
+      // lane issues; the next step's barrier is tried before this step's products are issued.
+      const bool lead = elect_one();
       const uint64_t a0 = WEIGHTS ? smem_desc_mn_sw128(smem_u32(smem + L::A_OFF), MN_STRIDE, ATOM)
                                   : smem_desc_sw128(smem_u32(smem + L::A_OFF));
       const bool b_mn = WEIGHTS || a.b_mn;
@@ -375,72 +386,89 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
       int slot = 0, phase = 0, local = 0;
       bool there = false;
       for (int32_t t = unit; t < total && ok; t += units, ++local) {
-        const int32_t k1 = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, t).k1;
+        const int32_t k1 = (int32_t)__reduce_max_sync(
+            0xffffffffu, (uint32_t)ex_tile<BN, PAIR, WEIGHTS>(a, s_first, s_seg, t).k1);
         const int ab = local & 1;
-        if (!mbar_wait_bounded(&acc_empty[ab], ((local >> 1) & 1) ^ 1, s_abort)) {
-          ok = false;
-          break;
-        }
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait_bounded(&acc_empty[ab], ((local >> 1) & 1) ^ 1, s_abort));
+        if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(ab * BN);
         for (int k = 0; k < k1; ++k) {
-          if (!there && !mbar_wait_bounded(&full[slot], phase, s_abort)) {
-            ok = false;
-            break;
+          if (!there) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[slot], phase, s_abort));
+            if (!ok) break;
           }
           tc_fence_after();
-          uint32_t a_low = (uint32_t)a0 + slot * (L::A_STAGE / 16);
-          uint32_t b_low = (uint32_t)b0 + slot * (L::B_STAGE / 16);
+          const uint32_t a_low = (uint32_t)a0 + slot * (L::A_STAGE / 16);
+          const uint32_t b_low = (uint32_t)b0 + slot * (L::B_STAGE / 16);
           uint64_t* const free_slot = &empty[slot];
           if (++slot == S) {
             slot = 0;
             phase ^= 1;
           }
-          there = mbar_try_wait(&full[slot], phase);
+          there = __all_sync(0xffffffffu, mbar_try_wait(&full[slot], phase));
+          if (lead) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {  // 16 of k: one instruction
-            issue_mma<PAIR, false>(d, (uint64_t)a_high << 32 | a_low, (uint64_t)b_high << 32 | b_low,
-                                   a.idesc, (k > 0 || j > 0) ? 1u : 0u);
-            a_low += A_STEP;
-            b_low += b_step;
+            for (int j = 0; j < 4; ++j)  // 16 of k: one instruction
+              issue_mma<PAIR, false>(d, (uint64_t)a_high << 32 | (a_low + j * A_STEP),
+                                     (uint64_t)b_high << 32 | (b_low + j * b_step), a.idesc,
+                                     (k > 0 || j > 0) ? 1u : 0u);
+            commit<PAIR>(free_slot);
           }
-          commit<PAIR>(free_slot);
+          __syncwarp();
         }
-        if (ok) commit<PAIR>(&acc_full[ab]);
+        if (ok && lead) commit<PAIR>(&acc_full[ab]);
+        __syncwarp();
       }
-      if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
-      // the products in flight read both CTAs' shared memory: let them finish
-      commit<PAIR>(drained);
-      const uint64_t t0 = global_timer_ns();
-      while (!mbar_try_wait(drained, 0) && global_timer_ns() - t0 < 1000000000ull) {
+      if (lead) {
+        if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
+        // the products in flight read both CTAs' shared memory: let them finish
+        commit<PAIR>(drained);
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(drained, 0) && global_timer_ns() - t0 < 1000000000ull) {
+        }
       }
+      __syncwarp();
     }
   } else {
     const int q = warp & 3;            // TMEM lanes 32 q .. 32 q + 31
-    constexpr int PARTS = BN >= 128 ? 4 : 2, COLS = BN / PARTS;  // a warp's columns
+    constexpr int PARTS = BN >= 128 ? EX_EPI_WARPS / 4 : 2, COLS = BN / PARTS;  // a warp's columns
     const int part = (warp - 2) >> 2;
     const int e = threadIdx.x - 64;
     float* chunk = reinterpret_cast<float*>(smem + L::CHUNK_OFF) + (warp - 2) * 32 * CHUNK_LD;
     const bool scaled = ep.col_scale != nullptr;
+    static_assert(BN <= EX_EPI_THREADS, "a thread holds a column's bias");
+    ExTile w{};
+    float bias_held = 0.f, scale_held = 1.f;
+    // the tile and its columns' bias, found while the tile before is worked on: 1,500 cycles a tile
+    auto look_up = [&](int32_t t) {
+      if (t >= total) return;
+      w = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, s_seg, t);
+      const bool in = e < BN && w.n0 + e < a.n;
+      if (ep.bias) bias_held = in ? to_f32(static_cast<const O*>(ep.bias)[w.e * a.n + w.n0 + e]) : 0.f;
+      if (scaled) scale_held = in ? __ldg(ep.col_scale + w.n0 + e) : 1.f;
+    };
+    look_up(unit);
     int local = 0;
     for (int32_t t = unit; t < total; t += units, ++local) {  // left by all warps alike
-      const ExTile w = ex_tile<BN, PAIR, WEIGHTS>(a, s_first, t);
       const int ab = local & 1;
       float* s_bias = s_cols + ab * 2 * BN;
       float* s_scale = s_bias + BN;
       Epilogue out = ep;
       if constexpr (WEIGHTS) out.out = static_cast<O*>(ep.out) + (int64_t)w.e * a.m * a.n;
-      // this buffer's last readers were two tiles ago, before the previous epi_sync
-      for (int c = e; c < BN; c += EX_EPI_THREADS) {
-        const bool in = w.n0 + c < a.n;
-        if (ep.bias)
-          s_bias[c] = in ? to_f32(static_cast<const O*>(ep.bias)[w.e * a.n + w.n0 + c]) : 0.f;
-        if (scaled) s_scale[c] = in ? __ldg(ep.col_scale + w.n0 + c) : 1.f;
+      // this buffer's last readers were two tiles ago, before the previous barrier
+      if (e < BN) {
+        if (ep.bias) s_bias[e] = bias_held;
+        if (scaled) s_scale[e] = scale_held;
       }
       ex_epi_sync();
-      if (!ok) continue;
       const int64_t row0 = (int64_t)w.row + rank * TM + q * 32;  // the warp's first row
       const int rows = (int)max((int64_t)0, min((int64_t)32, w.last - row0));
+      const int n0 = w.n0;
+      const bool formed = w.k1 > 0;  // an expert without positions: nothing was
+      look_up(t + units);
+      if (!ok) continue;
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[ab], (local >> 1) & 1, s_abort))) {
         ok = false;
         continue;
@@ -449,23 +477,22 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
       const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * BN);
 #pragma unroll 1
       for (int c = part * COLS; c < min((part + 1) * COLS, BN); c += 32) {
-        const int64_t col = (int64_t)w.n0 + c;
+        const int64_t col = (int64_t)n0 + c;
         if (rows == 0 || col >= a.n) continue;  // the same in all lanes
         if (a.direct && col + 32 <= a.n) {
+          uint32_t raw[32];
+          tmem_ld_32x32b_x32(t_row + c, raw);
+          tc_wait_ld();
+          if (lane < rows) {
 #pragma unroll
-          for (int h = 0; h < 32; h += 16) {
-            uint32_t raw[16];
-            tmem_ld_32x32b_x16(t_row + c + h, raw);
-            tc_wait_ld();
-            if (lane < rows) {
+            for (int h = 0; h < 32; h += 16) {
               float v[1][16];
 #pragma unroll
-              for (int j = 0; j < 16; ++j)  // an expert without positions: nothing was formed
-                v[0][j] = w.k1 == 0 ? 0.f : __uint_as_float(raw[j]);
+              for (int j = 0; j < 16; ++j) v[0][j] = formed ? __uint_as_float(raw[h + j]) : 0.f;
               ex_direct<O, WIDE>(out, v, s_bias + c + h, s_scale + c + h, (row0 + lane) * a.n + col + h);
             }
-            __syncwarp();
           }
+          __syncwarp();
           continue;
         }
         __syncwarp();  // the previous chunk has been read
@@ -477,8 +504,8 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 16; j += 4)
             *reinterpret_cast<uint4*>(chunk + lane * CHUNK_LD + h + j) =
-                w.k1 == 0 ? make_uint4(0u, 0u, 0u, 0u)
-                          : make_uint4(raw[j], raw[j + 1], raw[j + 2], raw[j + 3]);
+                formed ? make_uint4(raw[j], raw[j + 1], raw[j + 2], raw[j + 3])
+                       : make_uint4(0u, 0u, 0u, 0u);
         }
         __syncwarp();
         const int cols = (int)min((int64_t)32, a.n - col);
