@@ -2,7 +2,8 @@
 ``SparseTensor`` / ``build_neighbor_map`` / ``SparseConv3D`` / ``sparse_conv3d`` /
 ``sparse_downsample`` / ``sparse_upsample``, backed by ``libsparsevox.so``, and the operators of a
 transformer block over the same rows: ``rms_norm``, ``linear`` and ``sparse_self_attention`` with a
-learned relative position bias."""
+learned relative position bias, ``block_norm`` at the borders between blocks, ``dropout``, and a mixture of
+experts (``route``, ``expert_linear``)."""
 
 from ._native import check_device_status
 from .kernels.block_norm import block_norm

@@ -266,6 +266,13 @@ def call(device: torch.device, fn, *args) -> int:
         return fn(*args)
 
 
+def savable(t: torch.Tensor | None) -> torch.Tensor | None:
+    """``t`` as autograd can save it: a tensor made under inference mode (coordinates or routes of a forward
+    pass there) is copied."""
+
+    return t.clone() if t is not None and t.is_inference() else t
+
+
 def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
     """Raise where a tensor carries a forward-mode tangent: kernels write through pointers, and the
     result would come back without one."""

@@ -155,7 +155,8 @@ def block_norm(
             coefs.append(None)
             continue
         size = t.shape
-        if not 1 <= len(size) <= rank or size[-1] != c or t.dtype not in N.DTYPE_CODE:
+        if not 1 <= len(size) <= rank or size[-1] != c or t.dtype not in N.DTYPE_CODE or \
+                (len(size) == 2 and size[0] < 1):
             raise ValueError(f"block_norm: {name} must be a float tensor of shape "
                              + (f"(B, {c})" if rank == 2 else f"({c},)"))
         if t.device != dev:
@@ -208,6 +209,7 @@ def block_norm(
     o.layer, o.branch_norm = int(norm == "layer"), int(bool(branch_norm))
     o.residual_scale, o.eps = float(residual_scale), float(eps)
     if some:
+        coords, seed_at = N.savable(coords), N.savable(seed_at)
         y, h = _BlockNorm.apply(x, branch, coords, seed_at, o, *coefs)
     else:
         y, h, _ = _forward(x, branch, coords, seed_at, o, False)

@@ -99,7 +99,7 @@ def dropout(
     residual = None if residual is None else residual.contiguous()
     if torch.is_grad_enabled() and (
             x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _Dropout.apply(x, residual, seed_at, p, seed, subsequence)
+        return _Dropout.apply(x, residual, N.savable(seed_at), p, seed, subsequence)
     return _forward(x, residual, p, seed, seed_at, subsequence)
 
 

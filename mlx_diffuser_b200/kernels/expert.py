@@ -129,7 +129,8 @@ def _pack(x, weight, bias, p, order, offsets, place, preact, rows, o) -> bytes:
     n, k = p.shape
     return N.EXPERT_ARGS.pack(
         n, x.data_ptr(), _ld(x), weight.data_ptr(), max(weight.stride(1), inputs),
-        weight.stride(0), 0 if bias is None else bias.data_ptr(), order.data_ptr(),
+        weight.stride(0) if experts > 1 else outputs * max(weight.stride(1), inputs),
+        0 if bias is None else bias.data_ptr(), order.data_ptr(),
         offsets.data_ptr(), place.data_ptr(), p.data_ptr(), 0 if preact is None else preact.data_ptr(),
         0 if rows is None else rows.data_ptr(), inputs, outputs, k, experts, N.DTYPE_CODE[x.dtype],
         *o)
@@ -267,7 +268,8 @@ def expert_linear(
     if torch.is_grad_enabled() and (
             x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
             or (combine and p.requires_grad)):
-        return _ExpertLinear.apply(x, weight, bias, p, order, offsets, place, o)
+        return _ExpertLinear.apply(x, weight, bias, N.savable(p), N.savable(order),
+                                   N.savable(offsets), N.savable(place), o)
     return _forward(x, weight, bias, p, order, offsets, place, o, False)[0]
 
 

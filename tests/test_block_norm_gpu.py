@@ -240,6 +240,58 @@ def test_many_rows():
     _compare(a, dy, dh, dropout=0.1, seed=SEED)
 
 
+# Rows of 33 to 128 eights, and 64 rows an SM: a pipeline of bulk copies per warp.
+@pytest.mark.parametrize("c", [264, 512, 520, 1000, 1024])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pipelined_rows(c, dtype):
+    n = 64 * torch.cuda.get_device_properties(DEV).multi_processor_count + 37
+    for i, norm in enumerate(("layer", "rms")):
+        a, dy, dh = _case(n, c, dtype, c + i, batch=3)
+        _compare(a, dy, dh, norm=norm, residual_scale=0.5)
+        del a["branch_weight"]
+        a["branch_norm"] = False
+        _compare(a, dy, dh, norm=norm, dropout=0.25, seed=SEED, subsequence=9)
+
+
+def test_pipelined_rows_of_many_batch_elements():
+    """Blocks whose rows have more batch elements than tables; rows in any order; some without one; one of
+    the results without a gradient; nothing per batch element."""
+    n = 64 * torch.cuda.get_device_properties(DEV).multi_processor_count + 5
+    a, dy, dh = _case(n, 264, torch.bfloat16, 15, batch=700)
+    _compare(a, dy, None)
+    _compare(a, None, dh)
+    g = torch.Generator(device=DEV).manual_seed(16)
+    a["coords"][:, 0] = torch.randint(0, 700, (n,), device=DEV, generator=g)
+    _compare(a, dy, dh, norm="rms")
+    a["coords"][::7, 0] = 700
+    a["coords"][3::7, 0] = -1
+    with pytest.raises(RuntimeError, match="out of range"):
+        _compare(a, dy, dh)
+    for names in ((), ("weight",), ("gate",)):
+        a, dy, dh = _case(n, 264, torch.bfloat16, 17, per_batch=False, names=names)
+        _compare(a, dy, dh)
+    # rows apart, and the same results every time
+    a, dy, dh = _case(n, 264, torch.bfloat16, 18, batch=2)
+    wide = torch.zeros((n, 600), dtype=torch.bfloat16, device=DEV)
+    wide[:, 8:272], wide[:, 280:544] = a["x"], a["branch"]
+    b = {**a, "x": wide[:, 8:272], "branch": wide[:, 280:544]}
+    first, again = _step(a, dy, dh), _step(b, dy, dh)
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    assert all(torch.equal(first[2][k], again[2][k]) for k in first[2])
+
+
+def test_coordinates_made_under_inference_mode():
+    a, dy, dh = _case(100, 64, torch.float32, 19)
+    want = _step(a, dy, dh)
+    with torch.inference_mode():
+        held = a["coords"].clone()
+        assert held.is_inference()
+        y, h = block_norm(**{**a, "x": a["x"].clone()})
+    assert torch.equal(y, want[0]) and torch.equal(h, want[1])
+    got = _step({**a, "coords": held}, dy, dh)
+    assert all(torch.equal(got[2][k], want[2][k]) for k in want[2])
+
+
 def test_unsorted_and_bad_batch_elements():
     """Rows of batch elements in any order, some without one: not modulated, reported, and their
     gradients reach x, branch and the weights only."""

@@ -400,6 +400,22 @@ def test_routes_of_other_makings():
     torch.cuda.synchronize()
 
 
+def test_routes_made_under_inference_mode():
+    n, e, k, i, o = 90, 4, 2, 64, 72
+    x, w, b = _inputs(n, e, k, i, o, torch.bfloat16, True)
+    logits, dy = _rand((n, e), torch.float32, 3), _rand((n, o), torch.bfloat16, 4)
+    want = _step(x, w, b, route(logits, k), dy, "silu", True, True)
+    with torch.inference_mode():
+        held = route(logits.clone(), k)
+        assert held.order.is_inference()
+        y = expert_linear(x, w, held, b, activation="silu", gather=True, combine=True)
+    assert torch.equal(y, want[0])
+    xg = x.detach().requires_grad_(True)
+    y = expert_linear(xg, w, held, b, activation="silu", gather=True, combine=True)
+    (dx,) = torch.autograd.grad(y, (xg,), dy)
+    assert torch.equal(dx, want[1]["x"])
+
+
 def test_gradients_against_differences():
     n, e, k, i, o = 12, 3, 2, 20, 24
     x, w, b = _inputs(n, e, k, i, o, torch.float32, True)
