@@ -157,12 +157,10 @@ __device__ __forceinline__ void unpack_row(const Raw<T, V> (&raw)[J], float (&v)
 template <typename T, int V>
 __device__ __forceinline__ void store_row(T* p, const float (&v)[V]) {
   if constexpr (V == 8) {
-    alignas(16) T e[8];
+    uint4 w[sizeof(T) / 2];
+    pack_eight<T>(v, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(e) / 16; ++i)
-      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
   } else {
     *p = from_f32<T>(v[0]);
   }
@@ -711,18 +709,20 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, sizeof(T) == 2 ? 2 : 1)
           float g[8], unused[8], other[8];
           if (table >= 0) tables.load(table, q, g);
           else fold(a, b, q * 8, g, unused, other);
-          alignas(16) T e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            x[j][i] = fmaf(g[i], BRANCH ? d[j][i] * dr : d[j][i], x[j][i]);
+          alignas(16) uint4 e[sizeof(T) / 2];
+          pack_eight<T>(x[j], e);
+          uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.h) + row * C + q * 8);
+#pragma unroll
+          for (int i = 0; i < (int)sizeof(T) / 2; ++i) to[i] = e[i];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float u = BRANCH ? d[j][i] * dr : d[j][i];
-            e[i] = from_f32<T>(fmaf(g[i], u, x[j][i]));
-            x[j][i] = to_f32(e[i]);
+            x[j][i] = to_f32(reinterpret_cast<const T*>(e)[i]);
             if constexpr (LAYER) s += x[j][i];
             else s = fmaf(x[j][i], x[j][i], s);
           }
-          uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.h) + row * C + q * 8);
-#pragma unroll
-          for (int i = 0; i < (int)sizeof(e) / 16; ++i) to[i] = reinterpret_cast<const uint4*>(e)[i];
         }
         if constexpr (LAYER) {
           hm = warp_sum(s) * inv;

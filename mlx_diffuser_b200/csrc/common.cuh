@@ -84,6 +84,34 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
+// Two values, rounded and packed by one instruction of the arithmetic pipe.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_two(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_two<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_two<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Eight values as they are stored.
+template <typename T>
+__device__ __forceinline__ void pack_eight(const float (&v)[8], uint4 (&w)[sizeof(T) / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    w[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                      __float_as_uint(v[3]));
+    w[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]),
+                      __float_as_uint(v[7]));
+  } else {
+    w[0] = make_uint4(pack_two<T>(v[0], v[1]), pack_two<T>(v[2], v[3]), pack_two<T>(v[4], v[5]),
+                      pack_two<T>(v[6], v[7]));
+  }
+}
+
 __device__ __forceinline__ void report(int32_t* status, int bit) {
   if (status) atomicOr(status, bit);
 }

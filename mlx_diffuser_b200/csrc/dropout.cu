@@ -39,8 +39,11 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_f32(from.e[i]);
     if (d.cut) drop_eight(v, philox((uint64_t)at, d.subsequence, keys), d);
+    if constexpr (RES) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) to.e[i] = from_f32<T>(RES ? v[i] + to_f32(add.e[i]) : v[i]);
+      for (int i = 0; i < 8; ++i) v[i] += to_f32(add.e[i]);
+    }
+    pack_eight<T>(v, *reinterpret_cast<uint4(*)[sizeof(T) / 2]>(to.e));
   };
   if constexpr (WIDE) {
     for (; g + (AHEAD - 1) * step < whole; g += AHEAD * step) {

@@ -305,13 +305,13 @@ __device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
 
 template <typename T, int V>
 __device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
-  if constexpr (V * sizeof(T) % 16 == 0) {
-    alignas(16) T e[V];
+  if constexpr (V == 8) {
+    uint4 w[sizeof(T) / 2];
+    pack_eight<T>(v, w);
 #pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = from_f32<T>(v[i]);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(e) / 16; ++i)
-      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+  } else if constexpr (V * sizeof(T) == 16) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) p[i] = from_f32<T>(v[i]);

@@ -76,7 +76,7 @@ struct ExArgs {
   int32_t steps;           // kRows
   uint32_t idesc;
   bool b_mn, wide_io, zero_tail;
-  bool direct;             // rows of the result are whole sectors
+  bool direct;             // the result's rows are multiples of 16 columns on 32-byte boundaries
   const CUtensorMap* maps;  // kWeights: [experts][2]
 };
 
@@ -186,46 +186,55 @@ __device__ __forceinline__ void store_sector(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-// A lane's 16 consecutive columns of one row, straight from TMEM to whole sectors of global memory: no
-// turn through shared memory, half of the instructions an element. `bias`, `scale`: in shared memory,
-// the same address in all lanes.
-template <typename O, bool WIDE>
-__device__ __forceinline__ void ex_direct(const Epilogue& ep, float (&v)[1][16], const float* bias,
-                                          const float* scale, int64_t at) {
+// A warp's columns [c0, c1) of a tile, a row a lane, straight from TMEM to whole sectors of global memory: no
+// turn through shared memory, half of the instructions an element. `bias`, `scale`: in shared memory, the
+// same address in all lanes, 0 and 1 where there are none: a multiply-add an element and no branch, which
+// between 4 elements each cost more than the elements (12 cycles an element of the tile's 256 a scheduler).
+// `to`, `kept`: the lane's row at column 0 of the tile; formed: the sums are there, else they are zeros.
+template <typename O, bool WIDE, int ACT>
+__device__ __forceinline__ void ex_direct(uint32_t t_row, int c0, int c1, const float* bias,
+                                          const float* scale, bool formed, bool in, void* to,
+                                          float* kept) {
+#pragma unroll 1
+  for (int c = c0; c < c1; c += 16) {
+    uint32_t raw[16];
+    tmem_ld_32x32b_x16(t_row + c, raw);
+    float v[1][16];
+    float4 m[4], s[4];
 #pragma unroll
-  for (int j = 0; j < 16; j += 4) {
-    if (ep.col_scale) {
-      const float4 f = *reinterpret_cast<const float4*>(scale + j);
-      v[0][j] *= f.x; v[0][j + 1] *= f.y; v[0][j + 2] *= f.z; v[0][j + 3] *= f.w;
+    for (int j = 0; j < 4; ++j) {
+      m[j] = *reinterpret_cast<const float4*>(scale + c + 4 * j);
+      s[j] = *reinterpret_cast<const float4*>(bias + c + 4 * j);
     }
-    if (ep.bias) {
-      const float4 f = *reinterpret_cast<const float4*>(bias + j);
-      v[0][j] += f.x; v[0][j + 1] += f.y; v[0][j + 2] += f.z; v[0][j + 3] += f.w;
-    }
-  }
-  auto store32 = [&](float* to) {
+    tc_wait_ld();
 #pragma unroll
-    for (int j = 0; j < 16; j += 8) {
+    for (int j = 0; j < 16; ++j) v[0][j] = formed ? __uint_as_float(raw[j]) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[0][4 * j] = fmaf(v[0][4 * j], m[j].x, s[j].x);
+      v[0][4 * j + 1] = fmaf(v[0][4 * j + 1], m[j].y, s[j].y);
+      v[0][4 * j + 2] = fmaf(v[0][4 * j + 2], m[j].z, s[j].z);
+      v[0][4 * j + 3] = fmaf(v[0][4 * j + 3], m[j].w, s[j].w);
+    }
+    auto store32 = [&](float* at) {
+#pragma unroll
+      for (int j = 0; j < 16; j += 8) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[0][j + i]);
+        if (in) store_sector(at + j, w);
+      }
+    };
+    if (kept) store32(kept + c);
+    activate_all<ACT>(v);
+    if constexpr (WIDE) {
+      store32(static_cast<float*>(to) + c);
+    } else {
       uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[0][j + i]);
-      store_sector(to + j, w);
+      for (int i = 0; i < 8; ++i) w[i] = pack_two<O>(v[0][2 * i], v[0][2 * i + 1]);
+      if (in) store_sector(static_cast<O*>(to) + c, w);
     }
-  };
-  if (ep.preact) store32(ep.preact + at);
-  if (ep.act == SV_ACT_SILU) activate_all<SV_ACT_SILU>(v);
-  else if (ep.act == SV_ACT_GELU) activate_all<SV_ACT_GELU>(v);
-  else if (ep.act == SV_ACT_GELU_TANH) activate_all<SV_ACT_GELU_TANH>(v);
-  if constexpr (WIDE) {
-    store32(static_cast<float*>(ep.out) + at);
-  } else {
-    alignas(16) O e[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) e[i] = from_f32<O>(v[0][i]);
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const uint32_t*>(e)[i];
-    store_sector(static_cast<O*>(ep.out) + at, w);
   }
 }
 
@@ -459,8 +468,8 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
       if constexpr (WEIGHTS) out.out = static_cast<O*>(ep.out) + (int64_t)w.e * a.m * a.n;
       // this buffer's last readers were two tiles ago, before the previous barrier
       if (e < BN) {
-        if (ep.bias) s_bias[e] = bias_held;
-        if (scaled) s_scale[e] = scale_held;
+        s_bias[e] = bias_held;
+        s_scale[e] = scale_held;
       }
       ex_epi_sync();
       const int64_t row0 = (int64_t)w.row + rank * TM + q * 32;  // the warp's first row
@@ -475,26 +484,26 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
       }
       tc_fence_after();
       const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * BN);
+      if (a.direct && rows > 0) {
+        using R = std::conditional_t<WIDE, float, O>;
+        const int c1 = (int)min(a.n - n0, (int64_t)min((part + 1) * COLS, BN));
+        const int64_t at = (row0 + min(lane, rows - 1)) * a.n + n0;
+        R* to = static_cast<R*>(out.out) + at;
+        float* kept = out.preact ? out.preact + at : nullptr;
+        auto columns = [&](auto act) {
+          ex_direct<O, WIDE, decltype(act)::value>(t_row, part * COLS, c1, s_bias, s_scale, formed,
+                                                   lane < rows, to, kept);
+        };
+        if (WEIGHTS || ep.act == SV_ACT_NONE) columns(std::integral_constant<int, SV_ACT_NONE>());
+        else if (ep.act == SV_ACT_SILU) columns(std::integral_constant<int, SV_ACT_SILU>());
+        else if (ep.act == SV_ACT_GELU) columns(std::integral_constant<int, SV_ACT_GELU>());
+        else columns(std::integral_constant<int, SV_ACT_GELU_TANH>());
+        __syncwarp();
+      }
 #pragma unroll 1
       for (int c = part * COLS; c < min((part + 1) * COLS, BN); c += 32) {
         const int64_t col = (int64_t)n0 + c;
-        if (rows == 0 || col >= a.n) continue;  // the same in all lanes
-        if (a.direct && col + 32 <= a.n) {
-          uint32_t raw[32];
-          tmem_ld_32x32b_x32(t_row + c, raw);
-          tc_wait_ld();
-          if (lane < rows) {
-#pragma unroll
-            for (int h = 0; h < 32; h += 16) {
-              float v[1][16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[0][j] = formed ? __uint_as_float(raw[h + j]) : 0.f;
-              ex_direct<O, WIDE>(out, v, s_bias + c + h, s_scale + c + h, (row0 + lane) * a.n + col + h);
-            }
-          }
-          __syncwarp();
-          continue;
-        }
+        if (a.direct || rows == 0 || col >= a.n) continue;  // the same in all lanes
         __syncwarp();  // the previous chunk has been read
 #pragma unroll
         for (int h = 0; h < 32; h += 16) {
@@ -687,8 +696,7 @@ int launch_expert(const ExpertGemm& g, CUtensorMap* maps, int32_t* status, cudaS
   const Epilogue& ep = g.ep;
   a.wide_io = g.n % 8 == 0 && aligned16(ep.out) && (!ep.preact || aligned16(ep.preact));
   auto sectors = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; };
-  a.direct = g.n * (WIDE ? 4 : ES) % 32 == 0 && sectors(ep.out) && g.n % 8 == 0 && sectors(ep.preact) &&
-             (WIDE || g.m * g.n % 16 == 0);
+  a.direct = g.n % 16 == 0 && sectors(ep.out) && sectors(ep.preact);
   units = (int)std::min<int64_t>(pieces * a.tiles_n, units);
   config.gridDim = dim3((unsigned)(units * (PAIR ? 2 : 1)));
   SV_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, map_a, map_b, a, ep, status));
