@@ -605,20 +605,21 @@ __device__ __forceinline__ void load_eight(const uint8_t* stage, int q, float (&
   for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
 }
 
-// Stages that fit two blocks an SM of 16-bit rows, or one of fp32 rows.
-template <typename T, int J, int TENSORS, int PLANES>
+// x and branch, two rows ahead, and the tables of two batch elements: two blocks an SM of 16-bit rows, or
+// one of fp32 rows.
+template <typename T, int J>
 struct RowsLayout {
   using Ring = RowRing<T, J * (int)sizeof(T) / 2>;  // 32 J eights: as many 16-byte accesses, twice for fp32
   static constexpr int STAGES = 2;
-  static constexpr int TABLE = Ring::SMEM(TENSORS, STAGES);
-  static constexpr int SMEM = TABLE + PLANES * Folded<J>::PLANE * 4;
+  static constexpr int TABLE = Ring::SMEM(2, STAGES);
+  static constexpr int SMEM = TABLE + 6 * Folded<J>::PLANE * 4;
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
 
 template <typename T, int J, bool LAYER, bool BRANCH>
 __global__ void __launch_bounds__(32 * ROW_WARPS, sizeof(T) == 2 ? 2 : 1)
     block_norm_rows_kernel(const __grid_constant__ BlockArgs a) {
-  using L = RowsLayout<T, J, 2, 6>;
+  using L = RowsLayout<T, J>;
   using Ring = typename L::Ring;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int s_abort;
@@ -756,199 +757,6 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, sizeof(T) == 2 ? 2 : 1)
         }
       });
   if (!ok && lane == 0) report(a.status, SV_DEVICE_WAIT_TIMEOUT);
-}
-
-// The backward pass of a piece, whose rows have one batch element. A row's tensors are read from the stage
-// twice: cheaper than holding 32 J values beside the sums.
-template <typename T, int J, bool LAYER, bool BRANCH>
-__global__ void __launch_bounds__(32 * ROW_WARPS, 1)
-    block_norm_rows_backward_kernel(const __grid_constant__ BackArgs a) {
-  using L = RowsLayout<T, J, 4, 2>;
-  using Ring = typename L::Ring;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int s_abort;
-  const BlockArgs& f = a.f;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int C = f.channels;
-  const Folded<J> table{reinterpret_cast<float*>(smem + L::TABLE)};
-  if (a.done && blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
-  Piece p{0, 0, 0};
-  if (a.offsets) {
-    p = find_piece<true>(a.offsets, (int)f.batch, (int)f.n, a.piece, blockIdx.x);
-  } else {
-    p.first = (int)min((int64_t)blockIdx.x * a.piece, f.n);
-    p.last = (int)min((int64_t)p.first + a.piece, f.n);
-    if (p.first >= p.last) p.group = -1;
-  }
-  if (p.group < 0) return;  // the whole block
-  if (threadIdx.x == 0) s_abort = 0;
-  const int64_t b = p.group < f.batch ? p.group : -1;
-  for (int q = threadIdx.x; q * 8 < C; q += 32 * ROW_WARPS) {
-    float g[8], m[8], s[8];
-    fold(f, b, q * 8, g, m, s);
-    table.store(0, q, g);
-    table.store(1, q, m);
-  }
-  __syncthreads();
-  PhiloxKeys keys(f.drop.cut ? seed_of(f.drop) : 0);
-  keys.held();
-  const bool with_d = BRANCH || a.want_e;
-  float sum_a[J][8], sum_b[J][8], sum_e[J][8];
-#pragma unroll
-  for (int j = 0; j < J; ++j)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum_a[j][i] = sum_b[j][i] = sum_e[j][i] = 0.0f;
-  const float inv = 1.0f / (float)C;
-  // tensors that are there, in order: h, dy, dh, branch
-  const int at_dy = 1, at_dh = at_dy + (a.dy != nullptr), at_d = at_dh + (a.dh != nullptr);
-  const int tensors = at_d + with_d;
-  // The indices of the warp's rows 32 i .. 32 i + 31 and of the 32 behind them, a lane each, and the
-  // former's statistics: each row by itself waited for L2 three times.
-  auto index_of = [&](int64_t k) {
-    const int64_t at = min(p.first + warp + k * ROW_WARPS, (int64_t)p.last - 1);
-    return a.perm ? __ldg(a.perm + at) : (int)at;
-  };
-  int rows_now = 0, rows_next = index_of(lane), mine = 0;
-  float4 st_lane = make_float4(0.0f, 0.0f, 0.0f, 1.0f);
-  const bool ok = run_rows<T, J * (int)sizeof(T) / 2, 4, L::STAGES>(
-      smem, p.first + warp, ROW_WARPS, p.last, C * (int)sizeof(T), tensors, &s_abort,
-      [&](int64_t, int64_t k) -> int64_t {  // STAGES rows ahead of the row that is worked on
-        if ((k & 31) == 0) {
-          rows_now = rows_next;
-          rows_next = index_of(k + 32 + lane);
-        }
-        return __shfl_sync(0xffffffffu, rows_now, (int)(k & 31));
-      },
-      [&](int t, int64_t r) -> const void* {
-        if (t == 0) return static_cast<const T*>(f.h) + r * C;
-        if (t == at_d) return static_cast<const T*>(f.branch) + r * f.branch_stride;
-        return static_cast<const T*>(t == at_dh ? a.dh : a.dy) + r * C;
-      },
-      [&](int64_t, int64_t k, const uint8_t* stage, auto&& release) {
-        if ((k & 31) == 0) {
-          mine = index_of(k + lane);
-          st_lane = __ldg(f.stats + mine);
-        }
-        const int from = (int)(k & 31);
-        const int64_t row = __shfl_sync(0xffffffffu, mine, from);
-        float4 st;
-        st.x = __shfl_sync(0xffffffffu, st_lane.x, from);
-        st.y = __shfl_sync(0xffffffffu, st_lane.y, from);
-        st.z = __shfl_sync(0xffffffffu, st_lane.z, from);
-        st.w = __shfl_sync(0xffffffffu, st_lane.w, from);
-        // N(v) = v rstd - mean rstd: the product's rounding is below that of the mean
-        const float h_off = -st.x * st.y, d_off = -st.z * st.w;
-        float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int q = lane + 32 * j;
-          if (q * 8 >= C || a.dy == nullptr) continue;
-          float n[8], dy[8], m[8];
-          load_eight<T>(stage, q, n);
-          load_eight<T>(stage + at_dy * Ring::ROW, q, dy);
-          table.load(1, q, m);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            n[i] = LAYER ? fmaf(n[i], st.y, h_off) : n[i] * st.y;
-            sum_a[j][i] = fmaf(dy[i], n[i], sum_a[j][i]);
-            sum_b[j][i] += dy[i];
-            const float g = dy[i] * m[i];
-            if constexpr (LAYER) s1 += g;
-            s2 = fmaf(g, n[i], s2);
-          }
-        }
-        const float m1 = LAYER ? warp_sum(s1) * inv : 0.0f, m2 = warp_sum(s2) * inv;
-        float D[J][8], u[BRANCH ? J : 1][8];
-        uint32_t kept[J];
-        s1 = s2 = 0.0f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int q = lane + 32 * j;
-          kept[j] = 0u;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) D[j][i] = 0.0f;
-          if (q * 8 >= C) continue;
-          if (a.dh) load_eight<T>(stage + at_dh * Ring::ROW, q, D[j]);
-          if (a.dy) {
-            float n[8], dy[8], m[8];
-            load_eight<T>(stage, q, n);
-            load_eight<T>(stage + at_dy * Ring::ROW, q, dy);
-            table.load(1, q, m);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              n[i] = LAYER ? fmaf(n[i], st.y, h_off) : n[i] * st.y;
-              const float g = fmaf(dy[i], m[i], LAYER ? fmaf(-n[i], m2, -m1) : -n[i] * m2);
-              D[j][i] = fmaf(st.y, g, D[j][i]);
-            }
-          }
-          if (a.dx) store_row<T, 8>(static_cast<T*>(a.dx) + row * C + q * 8, D[j]);
-          if (f.drop.cut)
-            kept[j] = kept_eight(philox(((uint64_t)row * C >> 3) + q, f.drop.subsequence, keys), f.drop);
-          if (with_d) {
-            float d[8];
-            load_eight<T>(stage + at_d * Ring::ROW, q, d);
-            if (f.drop.cut) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) d[i] = kept[j] >> i & 1u ? d[i] * f.drop.scale : 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if constexpr (BRANCH) d[i] = LAYER ? fmaf(d[i], st.w, d_off) : d[i] * st.w;
-              sum_e[j][i] = fmaf(D[j][i], d[i], sum_e[j][i]);
-              if constexpr (BRANCH) u[j][i] = d[i];
-            }
-          }
-          float g[8];
-          table.load(0, q, g);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            D[j][i] *= g[i];
-            if constexpr (BRANCH) {
-              if constexpr (LAYER) s1 += D[j][i];
-              s2 = fmaf(D[j][i], u[j][i], s2);
-            }
-          }
-        }
-        release();
-        if (a.dbranch == nullptr) return;
-        const float e1 = BRANCH && LAYER ? warp_sum(s1) * inv : 0.0f;
-        const float e2 = BRANCH ? warp_sum(s2) * inv : 0.0f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int q = lane + 32 * j;
-          if (q * 8 >= C) continue;
-          if constexpr (BRANCH) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) D[j][i] = st.w * (D[j][i] - e1 - u[j][i] * e2);
-          }
-          if (f.drop.cut) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) D[j][i] = kept[j] >> i & 1u ? D[j][i] * f.drop.scale : 0.0f;
-          }
-          store_row<T, 8>(static_cast<T*>(a.dbranch) + row * C + q * 8, D[j]);
-        }
-      });
-  if (!ok && lane == 0) report(f.status, SV_DEVICE_WAIT_TIMEOUT);
-  if (a.partial == nullptr) return;
-  __syncthreads();  // the rings are done with
-  float* held = reinterpret_cast<float*>(smem);  // [warps][3 planes]
-  static_assert(ROW_WARPS * 3 * Folded<J>::PLANE * 4 <= L::TABLE, "the sums take the rings' place");
-  const Folded<J> mine_at{held + warp * 3 * Folded<J>::PLANE};
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    mine_at.store(0, lane + 32 * j, sum_a[j]);
-    mine_at.store(1, lane + 32 * j, sum_b[j]);
-    mine_at.store(2, lane + 32 * j, sum_e[j]);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 3 * C; i += 32 * ROW_WARPS) {
-    const int k = i / C, c = i - k * C;
-    const float* from = held + (k * 2 + (c >> 2 & 1)) * 4 * Folded<J>::Q + (c >> 3) * 4 + (c & 3);
-    float v = from[0];
-#pragma unroll
-    for (int w = 1; w < ROW_WARPS; ++w) v += from[w * 3 * Folded<J>::PLANE];
-    a.partial[(int64_t)blockIdx.x * 3 * C + i] = v;
-  }
 }
 
 // ---- the coefficients' gradients from the pieces' sums -------------------------------------------
@@ -1101,39 +909,26 @@ int launch_backward(const BackArgs& a, unsigned blocks, cudaStream_t s) {
   if ((C) <= 2048) return call(1, 8, 256);                                         \
   return call(1, 32, 256)
 
-template <typename T, int J, int TENSORS, int PLANES, typename K, typename A>
-int launch_rows(K kernel, const A& a, unsigned blocks, cudaStream_t s) {
-  constexpr int bytes = RowsLayout<T, J, TENSORS, PLANES>::SMEM;
-  SV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  kernel<<<blocks, 32 * ROW_WARPS, bytes, s>>>(a);
-  SV_LAUNCH_CHECK();
-  return SV_OK;
-}
-
 template <typename T, int J>
 int rows_forward(const BlockArgs& a, cudaStream_t s) {
   auto kernel = a.layer ? (a.branch_norm ? block_norm_rows_kernel<T, J, true, true>
                                          : block_norm_rows_kernel<T, J, true, false>)
                         : (a.branch_norm ? block_norm_rows_kernel<T, J, false, true>
                                          : block_norm_rows_kernel<T, J, false, false>);
-  return launch_rows<T, J, 2, 6>(kernel, a, (unsigned)(num_sms() * (sizeof(T) == 2 ? 2 : 1)), s);
-}
-
-template <typename T, int J>
-int rows_backward(const BackArgs& a, unsigned blocks, cudaStream_t s) {
-  auto kernel = a.f.layer ? (a.f.branch_norm ? block_norm_rows_backward_kernel<T, J, true, true>
-                                             : block_norm_rows_backward_kernel<T, J, true, false>)
-                          : (a.f.branch_norm ? block_norm_rows_backward_kernel<T, J, false, true>
-                                             : block_norm_rows_backward_kernel<T, J, false, false>);
-  return launch_rows<T, J, 4, 2>(kernel, a, blocks, s);
+  constexpr int bytes = RowsLayout<T, J>::SMEM;
+  SV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  kernel<<<num_sms() * (sizeof(T) == 2 ? 2 : 1), 32 * ROW_WARPS, bytes, s>>>(a);
+  SV_LAUNCH_CHECK();
+  return SV_OK;
 }
 
 // Whether rows go through the warps' pipelines: rows that two to four eights a lane hold, and enough of
-// them that every warp gets four.
+// them that every warp gets four. 9,472 rows, launch included, pipelined against the direct kernel: 1024
+// channels of bf16 14.3 / 22.1 us, 512 9.1 / 15.0, 320 9.0 / 15.3; 1024 of fp32 28.5 / 33.5. The backward pass has no such form: its three sums leave
+// one block an SM (1024 channels of bf16, 40,000 rows: 101 us so, 95 us by the direct kernel; 320: 66 / 48).
 bool pipelined(int64_t n, int channels, bool wide) {
   return wide && channels > 256 && channels <= 1024 && n >= (int64_t)4 * ROW_WARPS * 2 * num_sms();
 }
-
 template <typename T>
 int forward_typed(const BlockArgs& a, cudaStream_t s) {
   if (pipelined(a.n, a.channels, wide_rows(a)))
@@ -1145,26 +940,19 @@ int forward_typed(const BlockArgs& a, cudaStream_t s) {
 
 template <typename T>
 int backward_typed(const BackArgs& a, bool wide, unsigned blocks, cudaStream_t s) {
-  if (pipelined(a.f.n, a.f.channels, wide)) {
-    if (a.f.channels <= 512) return rows_backward<T, 2>(a, blocks, s);
-    // two stages of four such rows of fp32 for eight warps are more than the shared memory
-    if constexpr (sizeof(T) == 2) return rows_backward<T, 4>(a, blocks, s);
-  }
 #define SV_CALL(V, J, TPR) launch_backward<T, V, J, TPR>(a, blocks, s)
   SV_BLOCK_NORM_PICK(SV_CALL, a.f.channels, wide);
 #undef SV_CALL
 }
 
 // Rows of a piece, and how many pieces there can be (each batch element's last one is ragged): four blocks
-// an SM of the direct kernel; one of the pipelined kernel, whose warps then have rows enough to fill
-// their pipelines (20,331 x 1024 bf16 in 592 pieces: 188 us).
+// an SM run at the same time.
 struct Pieces {
   int rows;
   int64_t most;
 };
-Pieces pieces_of(int64_t n, int channels, int64_t groups) {
-  const int64_t per_sm = pipelined(n, channels, true) ? 1 : 4;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>((n + 15) / 16, num_sms() * per_sm));
+Pieces pieces_of(int64_t n, int64_t groups) {
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>((n + 15) / 16, (int64_t)num_sms() * 4));
   Pieces p;
   p.rows = (int)std::max<int64_t>(1, (n + want - 1) / want);
   p.most = (n + p.rows - 1) / p.rows + groups;
@@ -1177,7 +965,7 @@ struct BackPlan {
 };
 BackPlan back_plan(int64_t n, int channels, int64_t groups) {  // groups 0: rows are not sorted
   BackPlan p;
-  p.pieces = pieces_of(n, channels, groups ? groups + 1 : 0);
+  p.pieces = pieces_of(n, groups ? groups + 1 : 0);
   p.joined = align_up((size_t)p.pieces.most * 3 * channels * sizeof(float), 256);
   p.done = p.joined + align_up((size_t)(groups + 1) * 3 * channels * sizeof(float), 256);
   p.perm = p.done + 256;

@@ -8,7 +8,7 @@
 //     dx_p = dz_p W_e, and dx_n = sum_j dx[place_nj] where x was gathered
 //
 // The products' sizes differ by expert and are known on the device only. Three kernels form them:
-//   expert_few_kernel   up to FEW_SLOTS positions: the chosen experts' weights read once;
+//   expert_few_kernel   up to FEW_SLOTS positions: the chosen experts' weights read once, on the CUDA cores;
 //   expert_f32_kernel   fp32: the register tiles of gemm_f32.cuh;
 //   expert_tc.cu        fp16 / bf16: tcgen05 tiles fed by TMA.
 // What is summed over a row's choices is held in fp32: rounded to 16 bits before, it costs the sum a second
@@ -27,7 +27,11 @@ namespace {
 
 constexpr int EXPERT_MAX = 1024;
 constexpr int FEW_ROWS = 8;     // positions of a piece
-constexpr int FEW_SLOTS = 32;
+// Positions that the kernel for few takes. bf16, against the tensor cores' tiles: 16 experts of 1024 -> 4096
+// 8 positions 27 us (44), 16 55 (44); 8 of 1024 -> 1024 8 8.4 (17), 16 13.7 (17); 2 of 1024 -> 4096 8
+// 18.5 (17), 16 32 (17). It takes fp32 as long, whose tiles took 285, 56 and 56 us for 32 positions
+// where bf16 took 95, 22 and 59 by this kernel.
+constexpr int FEW_SLOTS = 8, FEW_SLOTS_F32 = 32;
 constexpr int DZ_ROWS = 64;     // positions of a piece of the backward pass's element-wise step
 constexpr int ALIGN = 256;
 
@@ -69,19 +73,14 @@ __device__ __forceinline__ void store_result(const Epilogue& ep, int64_t i, int6
   static_cast<float*>(ep.out)[i * n + j] = activate(acc, ep.act);
 }
 
-// A block takes a piece of an expert's positions (blockIdx.y) and eight columns, a warp each, or one
-// column with all its warps. As few_rows_kernel in linear.cu, with the rows found through the routing.
+// One column's sums for up to ROWS rows of a piece: W warps a column (8: the block's), lanes along k in
+// accesses of V elements, the rows' accesses in flight together (rows past the last read it again).
 template <typename T, int ROWS, int V, int W>
-__global__ void __launch_bounds__(256)
-    expert_few_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
-                      int64_t w_expert, Routing r, bool gather, bool zero_tail, int64_t n,
-                      int64_t k, Epilogue ep, int32_t* status) {
-  __shared__ float part[W > 1 ? 8 : 1][ROWS];
+__device__ __forceinline__ void few_rows(const T* x, int64_t ldx, const T* w, const Routing& r,
+                                         bool gather, const Piece& p, int64_t j, int64_t n, int64_t k,
+                                         const Epilogue& ep, float (&part)[8][FEW_ROWS],
+                                         int32_t* status) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (zero_tail && blockIdx.y == 0) clear_tail(r, n, static_cast<T*>(ep.out), blockIdx.x, gridDim.x);
-  const Piece p = find_piece<false>(r.offsets, r.experts, (int)r.slots, ROWS, blockIdx.y);
-  if (p.group < 0) return;
-  const int64_t j = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
   const int slot = W > 1 ? (int)threadIdx.x : lane;
   const T* from[ROWS];
   bool bad[ROWS];
@@ -97,14 +96,13 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) acc[i] = 0.f;
   if (j < n) {
-    const T* wr = w + p.group * w_expert + j * ldw;
-#pragma unroll 2
+#pragma unroll(ROWS <= 2 ? 4 : 2)
     for (int64_t c = (int64_t)slot * V; c < k; c += 32 * W * V) {
       alignas(16) T we[V];
       if constexpr (V * sizeof(T) == 16)
-        *reinterpret_cast<uint4*>(we) = __ldg(reinterpret_cast<const uint4*>(wr + c));
+        *reinterpret_cast<uint4*>(we) = __ldg(reinterpret_cast<const uint4*>(w + c));
       else
-        we[0] = wr[c];
+        we[0] = w[c];
       alignas(16) T xe[ROWS][V];
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
@@ -125,7 +123,6 @@ __global__ void __launch_bounds__(256)
     for (int o = 16; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
     if (bad[i]) acc[i] = 0.f;
   }
-  if (ep.bias) ep.bias = static_cast<const T*>(ep.bias) + p.group * n;
   const int rows = p.last - p.first;
   if constexpr (W > 1) {
     if (lane == 0) {
@@ -144,6 +141,30 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < ROWS; ++i)
       if (lane == i && i < rows) store_result<T>(ep, p.first + i, j, n, acc[i]);
   }
+}
+
+// A block takes a piece of an expert's positions (blockIdx.y) and eight columns, a warp each, or one
+// column with all its warps, by the code for as many rows as the piece has: experts mostly have one
+// or two, and the code for eight reads x eight times (8 positions of 16 experts, 1024 x 4096: 40 us by the
+// code for four, 27 so). LONE: one position, whose code alone has more warps an SM (7.1 against 9.2 us).
+template <typename T, bool LONE, int V, int W>
+__global__ void __launch_bounds__(256)
+    expert_few_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
+                      int64_t w_expert, Routing r, bool gather, bool zero_tail, int64_t n,
+                      int64_t k, Epilogue ep, int32_t* status) {
+  __shared__ float part[8][FEW_ROWS];
+  if (zero_tail && blockIdx.y == 0) clear_tail(r, n, static_cast<T*>(ep.out), blockIdx.x, gridDim.x);
+  const Piece p = find_piece<false>(r.offsets, r.experts, (int)r.slots, FEW_ROWS, blockIdx.y);
+  if (p.group < 0) return;
+  const int64_t j = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const T* we = w + p.group * w_expert + min(j, n - 1) * ldw;
+  if (ep.bias) ep.bias = static_cast<const T*>(ep.bias) + p.group * n;
+  const int rows = p.last - p.first;
+  if constexpr (LONE) few_rows<T, 1, V, W>(x, ldx, we, r, gather, p, j, n, k, ep, part, status);
+  else if (rows == 1) few_rows<T, 1, V, W>(x, ldx, we, r, gather, p, j, n, k, ep, part, status);
+  else if (rows == 2) few_rows<T, 2, V, W>(x, ldx, we, r, gather, p, j, n, k, ep, part, status);
+  else if (rows <= 4) few_rows<T, 4, V, W>(x, ldx, we, r, gather, p, j, n, k, ep, part, status);
+  else few_rows<T, FEW_ROWS, V, W>(x, ldx, we, r, gather, p, j, n, k, ep, part, status);
 }
 
 template <typename T>
@@ -579,35 +600,31 @@ int combine(const float* rows, const Routing& r, bool weighted, int64_t cols, in
   }
 }
 
-template <typename T, int ROWS>
-int launch_few(const sv_expert_args& g, const Routing& r, const Epilogue& ep, int32_t* status,
-               cudaStream_t s) {
+template <typename T>
+int few_typed(const sv_expert_args& g, const Routing& r, const Epilogue& ep, int32_t* status,
+              cudaStream_t s) {
   constexpr int VE = 16 / sizeof(T);
   const T* x = static_cast<const T*>(g.x);
   const T* w = static_cast<const T*>(g.weight);
   const bool vec = aligned16(x) && aligned16(w) && g.inputs % VE == 0 && g.ldx % VE == 0 &&
                    g.ldw % VE == 0 && g.w_expert % VE == 0;
   // pieces: every slot its own expert at most, or whole pieces and a ragged one an expert
-  const int64_t pieces = std::min<int64_t>(r.slots, r.slots / ROWS + std::min<int64_t>(g.experts, r.slots));
-  const bool wide = g.outputs * pieces >= 8 * num_sms();
+  const int64_t pieces =
+      std::min<int64_t>(r.slots, r.slots / FEW_ROWS + std::min<int64_t>(g.experts, r.slots));
   if (pieces > 65535) SV_FAIL(SV_ERR_UNSUPPORTED, "expert_linear: too many rows without inputs");
+  const bool wide = g.outputs * pieces >= 8 * num_sms();
   const dim3 grid((unsigned)(wide ? (g.outputs + 7) / 8 : g.outputs), (unsigned)pieces);
-  auto kernel = vec ? (wide ? expert_few_kernel<T, ROWS, VE, 1> : expert_few_kernel<T, ROWS, VE, 8>)
-                    : (wide ? expert_few_kernel<T, ROWS, 1, 1> : expert_few_kernel<T, ROWS, 1, 8>);
+  auto pick = [&](auto lone) {
+    constexpr bool L = decltype(lone)::value;
+    return vec ? (wide ? expert_few_kernel<T, L, VE, 1> : expert_few_kernel<T, L, VE, 8>)
+               : (wide ? expert_few_kernel<T, L, 1, 1> : expert_few_kernel<T, L, 1, 8>);
+  };
+  // an expert has a row once: one row makes pieces of one position
+  auto kernel = g.n == 1 ? pick(std::true_type()) : pick(std::false_type());
   kernel<<<grid, 256, 0, s>>>(x, g.ldx, w, g.ldw, g.w_expert, r, g.gather != 0, !g.combine, g.outputs,
                               g.inputs, ep, status);
   SV_LAUNCH_CHECK();
   return SV_OK;
-}
-
-template <typename T>
-int few_typed(const sv_expert_args& g, const Routing& r, const Epilogue& ep, int32_t* status,
-              cudaStream_t s) {
-  // an expert has a row once, so n rows are the most that a piece can have
-  if (g.n <= 1) return launch_few<T, 1>(g, r, ep, status, s);
-  if (g.n <= 2) return launch_few<T, 2>(g, r, ep, status, s);
-  if (g.n <= 4) return launch_few<T, 4>(g, r, ep, status, s);
-  return launch_few<T, FEW_ROWS>(g, r, ep, status, s);
 }
 
 // The tile with the least estimated time: linear.cu's estimate for an expert's mean share of positions.
@@ -654,7 +671,9 @@ struct Layout {
   int64_t pieces;
 };
 
-bool few(const sv_expert_args& g) { return g.n * g.k <= FEW_SLOTS || g.inputs == 0; }
+bool few(const sv_expert_args& g) {
+  return g.n * g.k <= (g.dtype == SV_FLOAT32 ? FEW_SLOTS_F32 : FEW_SLOTS) || g.inputs == 0;
+}
 bool pad_x(const sv_expert_args& g) {
   return g.gather || (g.dtype != SV_FLOAT32 && !ready(g.x, g.ldx, g.dtype));
 }

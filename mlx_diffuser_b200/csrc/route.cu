@@ -214,8 +214,9 @@ struct RouteArgs {
   int32_t *order, *offsets, *place, *counts;  // the forward pass
 };
 
-// Rows that one block chooses for: eight a warp, about what a second launch costs.
-constexpr int ROUTE_SMALL = 256;
+// Rows that one block chooses for: four a warp. 64 experts, k 4: 12.6 us for 128 rows, 10.0 us in two
+// launches, whose second one costs the host 6 us more; 256 rows 20.6 us.
+constexpr int ROUTE_SMALL = 128;
 // The rows' slots are cut between the blocks at rows.
 GroupPlan route_plan(int64_t n, int experts, int k) {
   GroupPlan p = group_plan(n * k, experts);
