@@ -24,8 +24,8 @@ struct Eight {
 
 // A thread takes AHEAD counters (eight elements each) a grid apart at a time, their loads together. WIDE:
 // every pointer 16-byte aligned, and all but the last counter's elements in 16-byte accesses. A pass over
-// 40,662 x 1024 bf16 is 167 MB, 25 us of HBM, and 160 instructions a counter took 38 us: a counter's ten
-// rounds are 40 with the keys in registers, and the eight selections 28.
+// 40,662 x 1024 bf16 is 167 MB, 25 us of HBM, and takes 31 us (38 with the keys added up for every
+// counter): its instructions bound it, a counter's ten rounds 40 and the eight selections 28.
 template <typename T, bool WIDE, bool RES>
 __global__ void __launch_bounds__(256)
     dropout_kernel(const T* x, const T* residual, T* out, int64_t cells, Dropout d) {

@@ -410,3 +410,28 @@ def test_captured_step_beside_an_eager_one():
         for out in (got, again):
             assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
             assert all(torch.equal(out[2][k], want[2][k]) for k in want[2])
+
+
+def test_rows_past_32_bits():
+    """Offsets beyond 2^31 elements, forward and backward: the last rows are what they are by themselves."""
+    n, c = 2**21 + 5, 1032
+    for width in (c, 1024):  # the direct and the pipelined kernel
+        a, dy, dh = _case(64, width, torch.bfloat16, 20, batch=2)
+        last = n - 64
+        big = {k: torch.zeros((n, width), dtype=torch.bfloat16, device=DEV) for k in ("x", "branch")}
+        for k, t in big.items():
+            t[last:] = a[k]
+        coords = torch.zeros((n, 4), dtype=torch.int32, device=DEV)
+        coords[last:] = a["coords"]
+        g = torch.zeros((n, width), dtype=torch.bfloat16, device=DEV)
+        g[last:] = dy
+        b = {**a, **{k: t.requires_grad_(True) for k, t in big.items()}, "coords": coords}
+        y, h = block_norm(**b)
+        dx, db = torch.autograd.grad((y, h), (big["x"], big["branch"]), (g, g))
+        ref = _Reference(a, h[last:].detach())
+        _close(h[last:], ref.h, ref.h_bound, "h")
+        _close(y[last:], ref.y, ref.y_bound, "y")
+        want = ref.gradients(dy, dy)
+        _close(dx[last:], *want["x"], "dx")
+        _close(db[last:], *want["branch"], "dbranch")
+        del b, big, y, h, dx, db, g

@@ -516,3 +516,35 @@ def test_captured_step_and_two_at_once():
             assert torch.equal(y, want[0])
             assert all(torch.equal(grads[name], want[1][name]) for name in want[1])
     N.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_most_experts(dtype):
+    for n in (50, 3000):
+        x, w, b = _inputs(n, 1024, 2, 40, 48, dtype, True)
+        routes = _routes(n, 1024, 2)
+        dy = _rand((n, 48), dtype, 8)
+        y, grads = _step(x, w, b, routes, dy, "gelu", True, True)
+        ref = _Reference(x, w, b, routes, "gelu", True, True)
+        _close(y, ref.out, ref.bound, "y")
+        for name, (g, bound) in ref.gradients(dy).items():
+            _close(grads[name], g, bound, name)
+
+
+def test_results_past_32_bits():
+    """Offsets beyond 2^31 elements of the results: the last rows are what their formula gives."""
+    n, e, i, o = 2**19 + 3, 4, 64, 4112
+    x, w, b = _inputs(n, e, 1, i, o, torch.bfloat16, True)
+    logits = torch.zeros((n, e), device=DEV)
+    logits[torch.arange(n, device=DEV), torch.arange(n, device=DEV) * e // n] = 1  # in the experts' order
+    routes = route(logits, 1)
+    y = expert_linear(x, w, routes, b, activation="silu", gather=True)
+    rows = x[-64:].to(F64)
+    z = rows @ w[e - 1].to(F64).T + b[e - 1].to(F64)
+    bound = (2 * i + 64) * U * (rows.abs() @ w[e - 1].to(F64).abs().T + b[e - 1].to(F64).abs())
+    want = _act(z, "silu")[0]
+    _close(y[-64:], want, 1.2 * bound + 1.01 * _half(torch.bfloat16) * want.abs() + _tiny(torch.bfloat16), "y")
+    del y
+    y = expert_linear(x, w[:, :2056], routes, b[:, :2056], gather=True, combine=True)
+    want = z[:, :2056]
+    _close(y[-64:], want, bound[:, :2056] + 1.01 * _half(torch.bfloat16) * want.abs() + _tiny(torch.bfloat16), "y")
