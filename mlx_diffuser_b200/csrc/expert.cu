@@ -55,7 +55,7 @@ __device__ __forceinline__ int64_t row_of(const Routing& r, int64_t p) {
 // Zeros in the rows behind the last expert's position, by 256 threads of each of `blocks` blocks.
 template <typename T>
 __device__ __forceinline__ void clear_tail(const Routing& r, int64_t n, T* out, int block, int blocks) {
-  const int64_t first = min(max(__ldg(r.offsets + r.experts), 0), (int32_t)r.slots);
+  const int64_t first = segment_at(r.offsets, r.experts - 1, (int)r.slots).last;
   for (int64_t i = first * n + (int64_t)block * 256 + threadIdx.x; i < r.slots * n;
        i += (int64_t)blocks * 256)
     out[i] = from_f32<T>(0.f);
@@ -190,8 +190,9 @@ __global__ void __launch_bounds__(256, 2) expert_f32_kernel(ExpertGemm g) {
     i0 = (int64_t)(blockIdx.x / across) * T;
     j0 = (int64_t)(blockIdx.x % across) * T;
     m = g.m;
-    k0 = min(max(__ldg(g.offsets + e), 0), (int32_t)g.slots);
-    k1 = max((int64_t)min(__ldg(g.offsets + e + 1), (int32_t)g.slots), k0);
+    const Segment seg = segment_at(g.offsets, e, (int)g.slots);
+    k0 = seg.first;
+    k1 = seg.last;
     ep.out = static_cast<float*>(ep.out) + e * g.m * g.n;
   } else {
     const Piece p = find_piece<false>(g.offsets, g.experts, (int)g.slots, T, blockIdx.x / across);
@@ -399,31 +400,32 @@ __global__ void __launch_bounds__(256, 4) expert_dz_kernel(const __grid_constant
   }
   const Piece p = find_piece<false>(a.r.offsets, a.r.experts, (int)a.r.slots, DZ_ROWS, blockIdx.x);
   if (p.group < 0) return;
+  // the piece's rows and weights once: found row by row, two dependent loads stood before each row's own
+  __shared__ int s_row[DZ_ROWS];
+  __shared__ float s_weight[DZ_ROWS];
+  if (a.combine) {
+    if ((int)threadIdx.x < p.last - p.first) {
+      const int32_t slot = __ldg(a.r.order + p.first + threadIdx.x);
+      const bool in = slot >= 0 && slot < a.r.slots;
+      s_row[threadIdx.x] = in ? slot / a.r.k : -1;
+      s_weight[threadIdx.x] = in ? __ldg(a.r.weights + slot) : 0.0f;
+    }
+    __syncthreads();
+  }
   const int64_t c = ((int64_t)blockIdx.y * 32 + lane) * V;
   float sum[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sum[i] = 0.f;
   if (c < a.cols) {
-#pragma unroll 2
+#pragma unroll(ACT == SV_ACT_NONE ? 4 : 2)
     for (int at = p.first + warp; at < p.last; at += 8) {
-      int64_t row = at;
-      float w = 1.0f;
-      if (a.combine) {
-        const int32_t slot = __ldg(a.r.order + at);
-        const bool in = slot >= 0 && slot < a.r.slots;
-        row = in ? slot / a.r.k : -1;
-        w = in ? __ldg(a.r.weights + slot) : 0.0f;
-      }
+      const int64_t row = a.combine ? s_row[at - p.first] : at;
       float d[V];
-      if (row >= 0) {
-        load_v<T, V>(static_cast<const T*>(a.dy) + row * a.cols + c, d);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) d[i] = 0.f;
-      }
+      load_v<T, V>(static_cast<const T*>(a.dy) + max(row, (int64_t)0) * a.cols + c, d);
       if (a.combine) {
+        const float w = s_weight[at - p.first];
 #pragma unroll
-        for (int i = 0; i < V; ++i) d[i] *= w;
+        for (int i = 0; i < V; ++i) d[i] = row < 0 ? 0.f : d[i] * w;
       }
       if constexpr (ACT != SV_ACT_NONE) {
         float z[V];
@@ -467,29 +469,11 @@ __global__ void __launch_bounds__(256, 4) expert_dz_kernel(const __grid_constant
 // db_e = the sums of e's pieces in order. blockIdx.y: the expert; 32 columns a block.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    expert_dbias_kernel(const float* __restrict__ partial, int held, Routing r, int64_t cols, T* out) {
+    expert_dbias_kernel(const float* __restrict__ partial, Routing r, int64_t cols, T* out) {
   __shared__ float s[8][33];
-  __shared__ int before[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.y;
-  int count = 0, mine = 0;  // pieces of the experts before, and of this one
-  for (int g = threadIdx.x; g <= e; g += 256) {
-    const int a = min(max(__ldg(r.offsets + g), 0), (int32_t)r.slots);
-    const int b = max(min(__ldg(r.offsets + g + 1), (int32_t)r.slots), a);
-    const int pieces = (b - a + DZ_ROWS - 1) / DZ_ROWS;
-    if (g < e) count += pieces;
-  }
-  {
-    const int a = min(max(__ldg(r.offsets + e), 0), (int32_t)r.slots);
-    const int b = max(min(__ldg(r.offsets + e + 1), (int32_t)r.slots), a);
-    mine = (b - a + DZ_ROWS - 1) / DZ_ROWS;
-  }
-  count = __reduce_add_sync(0xffffffffu, count);
-  if (lane == 0) before[warp] = count;
-  __syncthreads();
-  int first = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) first += before[i];
-  mine = min(mine, held - first);  // offsets that fall make more pieces than there are
+  const int2 pieces = pieces_at(r.offsets, e, (int)r.slots, DZ_ROWS);
+  const int first = pieces.x, mine = pieces.y;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float v = 0.f;
   if (c < cols)
@@ -786,7 +770,7 @@ int elementwise_back(const sv_expert_args& g, const DzArgs& a, int64_t pieces, c
   const int rc = wide ? launch_dz<T, V>(a, act, grid, s) : launch_dz<T, 1>(a, act, grid, s);
   if (rc != SV_OK || !dbias) return rc;
   const dim3 columns((unsigned)((g.outputs + 31) / 32), (unsigned)g.experts);
-  expert_dbias_kernel<T><<<columns, 256, 0, s>>>(a.partial, (int)pieces, a.r, g.outputs, static_cast<T*>(dbias));
+  expert_dbias_kernel<T><<<columns, 256, 0, s>>>(a.partial, a.r, g.outputs, static_cast<T*>(dbias));
   SV_LAUNCH_CHECK();
   return SV_OK;
 }

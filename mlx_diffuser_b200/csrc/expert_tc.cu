@@ -29,6 +29,7 @@
 
 #include "expert.h"
 #include "gemm_tc.cuh"
+#include "group.h"
 
 namespace sv {
 namespace {
@@ -102,12 +103,6 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap,
       " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
       "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z)
       : "memory");
-}
-
-// The segment of an expert, whatever the offsets are.
-__device__ __forceinline__ int2 segment(const ExArgs& a, int e) {
-  const int first = min(max(__ldg(a.offsets + e), 0), a.slots);
-  return make_int2(first, max(min(__ldg(a.offsets + e + 1), a.slots), first));
 }
 
 struct ExTile {
@@ -290,22 +285,28 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
   }
   if (warp == 1) alloc_tmem<PAIR>(s_tmem, 2 * BN);
   for (int e = threadIdx.x; e < a.experts; e += EX_THREADS) {
-    const int2 s = segment(a, e);
-    s_seg[e] = s;
-    s_first[e + 1] = (s.y - s.x + ROWS - 1) / ROWS;
+    s_seg[e] = make_int2(inside(a.offsets, e, a.slots), inside(a.offsets, e + 1, a.slots));
   }
   __syncthreads();
-  if (!WEIGHTS && warp == 2) {  // tiles of the experts before each
-    int before = 0;
+  if (warp == 2) {  // segments that do not overlap (group.h), and the tiles of the experts before each
+    int before = 0, top = 0;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
-      int v = e0 + lane < a.experts ? s_first[e0 + lane + 1] : 0;
+      const bool in = e0 + lane < a.experts;
+      int2 seg = in ? s_seg[e0 + lane] : make_int2(0, 0);
+      seg.x = rising(seg.x, top);
+      seg.y = in ? max(seg.x, seg.y) : seg.x;
+      top = __shfl_sync(0xffffffffu, seg.x, 31);
+      int v = (seg.y - seg.x + ROWS - 1) / ROWS;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
       }
       v += before;
-      if (e0 + lane < a.experts) s_first[e0 + lane + 1] = v;
+      if (in) {
+        s_seg[e0 + lane] = seg;
+        s_first[e0 + lane + 1] = v;
+      }
       before = __shfl_sync(0xffffffffu, v, 31);
     }
     if (lane == 0) s_first[0] = 0;
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
     if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
     if (!WEIGHTS && a.zero_tail) {
       const int64_t end = a.slots * a.n;
-      for (int64_t i = (int64_t)segment(a, a.experts - 1).y * a.n + (int64_t)blockIdx.x * EX_EPI_THREADS + e;
+      for (int64_t i = (int64_t)s_seg[a.experts - 1].y * a.n + (int64_t)blockIdx.x * EX_EPI_THREADS + e;
            i < end; i += (int64_t)gridDim.x * EX_EPI_THREADS)
         static_cast<O*>(ep.out)[i] = from_f32<O>(0.f);
     }
@@ -594,10 +595,10 @@ __global__ void __launch_bounds__(32)
   const int e = blockIdx.x, lane = threadIdx.x;
   held[0][lane] = reinterpret_cast<const uint32_t*>(&map_a)[lane];
   held[1][lane] = reinterpret_cast<const uint32_t*>(&map_b)[lane];
+  // an expert without positions is not loaded; an extent is at least one
+  const uint32_t rows = (uint32_t)max(1, segment_at(offsets, e, slots).last);
   __syncwarp();
   if (lane < 2) {
-    // an expert without positions is not loaded; an extent is at least one
-    const uint32_t rows = (uint32_t)max(1, min(__ldg(offsets + e + 1), slots));
     asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;" ::"r"(
                      smem_u32(held[lane])),
                  "r"(rows)

@@ -151,10 +151,36 @@ __device__ __forceinline__ void group_block(const int32_t* keys, int64_t stride,
   place_part(keys, stride, a, b, groups, by_warp + warp * bins, perm, place);
 }
 
-// The lanes of a warp cut the segments of `offsets` [groups + 1] into pieces of `unit` rows, in order;
-// TAIL: the rows behind the last segment, up to `limit`, are segment `groups`. Piece `index` is rows
-// [first, last) of segment `group`; group < 0: there are fewer pieces. Offsets are taken into
-// [0, limit] and made to rise, whatever they are.
+// Segments of `offsets` [groups + 1], found by a warp: offsets are taken into [0, limit] and made to rise,
+// whatever they are, so that segments never overlap (an offset below one before it is that one). What
+// is done for all of them is then bounded by `limit`.
+struct Segment {
+  int first, last;
+};
+__device__ __forceinline__ int inside(const int32_t* offsets, int g, int limit) {
+  return min(max(__ldg(offsets + g), 0), limit);
+}
+__device__ __forceinline__ Segment segment_at(const int32_t* offsets, int g, int limit) {
+  int first = 0;
+  for (int j0 = 0; j0 <= g; j0 += 32) {
+    const int j = j0 + (int)(threadIdx.x & 31);
+    first = max(first, __reduce_max_sync(0xffffffffu, j <= g ? inside(offsets, j, limit) : 0));
+  }
+  return {first, max(first, inside(offsets, g + 1, limit))};
+}
+// A lane's inclusive maximum over the lanes up to it, and `before`.
+__device__ __forceinline__ int rising(int v, int before) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v = max(v, u);
+  }
+  return max(v, before);
+}
+
+// The segments cut into pieces of `unit` rows, in order; TAIL: the rows behind the last segment, up to
+// `limit`, are segment `groups`. Piece `index` is rows [first, last) of segment `group`; group < 0:
+// there are fewer pieces.
 struct Piece {
   int group, first, last;
 };
@@ -163,13 +189,13 @@ __device__ __forceinline__ Piece find_piece(const int32_t* offsets, int groups, 
                                             int64_t index) {
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
+  int top = 0;
   for (int g0 = 0; g0 < groups + TAIL; g0 += 32) {
     const int g = g0 + lane;
-    int a = 0, b = 0;
-    if (g < groups + TAIL) {
-      a = min(max(__ldg(offsets + g), 0), limit);
-      b = g < groups ? max(min(__ldg(offsets + g + 1), limit), a) : limit;
-    }
+    const bool in = g < groups + TAIL;
+    const int a = rising(in ? inside(offsets, g, limit) : 0, top);
+    const int b = !in ? a : g < groups ? max(a, inside(offsets, g + 1, limit)) : limit;
+    top = __shfl_sync(0xffffffffu, a, 31);
     const int64_t count = ((int64_t)b - a + unit - 1) / unit;
     int64_t upto = count;
 #pragma unroll
@@ -192,6 +218,21 @@ __device__ __forceinline__ Piece find_piece(const int32_t* offsets, int groups, 
     before = __shfl_sync(0xffffffffu, upto, 31);
   }
   return {-1, 0, 0};
+}
+
+// How many pieces there are before segment g, and of it.
+__device__ __forceinline__ int2 pieces_at(const int32_t* offsets, int g, int limit, int unit) {
+  const int lane = threadIdx.x & 31;
+  int before = 0, top = 0;
+  for (int j0 = 0; j0 < g; j0 += 32) {
+    const int j = j0 + lane;
+    const int a = rising(j < g ? inside(offsets, j, limit) : 0, top);
+    const int b = j < g ? max(a, inside(offsets, j + 1, limit)) : a;
+    top = __shfl_sync(0xffffffffu, a, 31);
+    before += __reduce_add_sync(0xffffffffu, (b - a + unit - 1) / unit);
+  }
+  const Segment s = segment_at(offsets, g, limit);
+  return make_int2(before, (s.last - s.first + unit - 1) / unit);
 }
 #endif
 

@@ -393,9 +393,15 @@ def test_routes_of_other_makings():
     assert (expert_linear(x, w, bad, gather=True, combine=True) == 0).all()
     bad = dataclasses.replace(r, offsets=torch.tensor([-7, 50, 20, 10**9, 3], dtype=torch.int32, device=DEV))
     y = expert_linear(x, w, bad, gather=True)
-    # experts 0 and 2 share positions 20 to 49, which have one's result or the other's
+    # an offset below one before it is that one: experts 0 and 2 have positions 0 to 49 and the others
     rows = [linear(x, w[j]).repeat_interleave(2, 0) for j in (0, 2)]
-    assert torch.equal(y[:20], rows[0][:20]) and torch.equal(y[50:], rows[1][50:])
+    assert torch.equal(y[:50], rows[0][:50]) and torch.equal(y[50:], rows[1][50:])
+    for dtype in DTYPES:
+        x2, w2, b2 = _inputs(n, e, k, i, o, dtype, False)
+        good = dataclasses.replace(r, offsets=torch.tensor([0, 50, 50, n * k, n * k], dtype=torch.int32, device=DEV))
+        dy = _rand((n * k, o), dtype, 2)
+        a, c = (_step(x2, w2, b2, q, dy, "silu", False, False) for q in (bad, good))
+        assert torch.equal(a[0], c[0]) and all(torch.equal(a[1][name], c[1][name]) for name in c[1])
     _step(x, w, _rand((e, o), torch.bfloat16, 1), bad, _rand((n, o), torch.bfloat16, 2), "silu", True, True)
     torch.cuda.synchronize()
 
