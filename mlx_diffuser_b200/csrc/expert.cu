@@ -146,7 +146,8 @@ __device__ __forceinline__ void few_rows(const T* x, int64_t ldx, const T* w, co
 // A block takes a piece of an expert's positions (blockIdx.y) and eight columns, a warp each, or one
 // column with all its warps, by the code for as many rows as the piece has: experts mostly have one
 // or two, and the code for eight reads x eight times (8 positions of 16 experts, 1024 x 4096: 40 us by the
-// code for four, 27 so). LONE: one position, whose code alone has more warps an SM (7.1 against 9.2 us).
+// code for four, 27 so). LONE: pieces of one position, whose code alone has more warps an SM (7.1 against
+// 9.2 us).
 template <typename T, bool LONE, int V, int W>
 __global__ void __launch_bounds__(256)
     expert_few_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(256)
                       int64_t k, Epilogue ep, int32_t* status) {
   __shared__ float part[8][FEW_ROWS];
   if (zero_tail && blockIdx.y == 0) clear_tail(r, n, static_cast<T*>(ep.out), blockIdx.x, gridDim.x);
-  const Piece p = find_piece<false>(r.offsets, r.experts, (int)r.slots, FEW_ROWS, blockIdx.y);
+  const Piece p = find_piece<false>(r.offsets, r.experts, (int)r.slots, LONE ? 1 : FEW_ROWS, blockIdx.y);
   if (p.group < 0) return;
   const int64_t j = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const T* we = w + p.group * w_expert + min(j, n - 1) * ldw;
@@ -592,9 +593,12 @@ int few_typed(const sv_expert_args& g, const Routing& r, const Epilogue& ep, int
   const T* w = static_cast<const T*>(g.weight);
   const bool vec = aligned16(x) && aligned16(w) && g.inputs % VE == 0 && g.ldx % VE == 0 &&
                    g.ldw % VE == 0 && g.w_expert % VE == 0;
+  // One row's choices are mostly different experts: a piece each, and one that is named twice has two.
+  const bool lone = g.n == 1 && r.slots <= FEW_SLOTS_F32;
   // pieces: every slot its own expert at most, or whole pieces and a ragged one an expert
   const int64_t pieces =
-      std::min<int64_t>(r.slots, r.slots / FEW_ROWS + std::min<int64_t>(g.experts, r.slots));
+      lone ? r.slots
+           : std::min<int64_t>(r.slots, r.slots / FEW_ROWS + std::min<int64_t>(g.experts, r.slots));
   if (pieces > 65535) SV_FAIL(SV_ERR_UNSUPPORTED, "expert_linear: too many rows without inputs");
   const bool wide = g.outputs * pieces >= 8 * num_sms();
   const dim3 grid((unsigned)(wide ? (g.outputs + 7) / 8 : g.outputs), (unsigned)pieces);
@@ -603,8 +607,7 @@ int few_typed(const sv_expert_args& g, const Routing& r, const Epilogue& ep, int
     return vec ? (wide ? expert_few_kernel<T, L, VE, 1> : expert_few_kernel<T, L, VE, 8>)
                : (wide ? expert_few_kernel<T, L, 1, 1> : expert_few_kernel<T, L, 1, 8>);
   };
-  // an expert has a row once: one row makes pieces of one position
-  auto kernel = g.n == 1 ? pick(std::true_type()) : pick(std::false_type());
+  auto kernel = lone ? pick(std::true_type()) : pick(std::false_type());
   kernel<<<grid, 256, 0, s>>>(x, g.ldx, w, g.ldw, g.w_expert, r, g.gather != 0, !g.combine, g.outputs,
                               g.inputs, ep, status);
   SV_LAUNCH_CHECK();

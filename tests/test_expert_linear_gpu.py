@@ -554,3 +554,56 @@ def test_results_past_32_bits():
     y = expert_linear(x, w[:, :2056], routes, b[:, :2056], gather=True, combine=True)
     want = z[:, :2056]
     _close(y[-64:], want, bound[:, :2056] + 1.01 * _half(torch.bfloat16) * want.abs() + _tiny(torch.bfloat16), "y")
+
+
+def _made(chosen, e, offsets=None):
+    """Routes of the given experts (-1: none), made by hand: a row may name one expert more than once."""
+    n, k = len(chosen), len(chosen[0])
+    keys = torch.tensor(chosen).flatten()
+    keys = torch.where(keys < 0, e, keys)
+    order = torch.sort(keys, stable=True).indices
+    place = torch.empty_like(order)
+    place[order] = torch.arange(n * k)
+    place = torch.where(keys < e, place, -1).view(n, k)
+    if offsets is None:
+        offsets = [0, *torch.bincount(keys, minlength=e + 1)[:e].cumsum(0).tolist()]
+    weights = torch.rand((n, k), generator=torch.Generator().manual_seed(n + k)) + 0.1
+    return ExpertRoutes(*(t.to(DEV, kind) for t, kind in (
+        (torch.tensor(chosen), torch.int32), (weights, torch.float32), (order, torch.int32),
+        (torch.tensor(offsets), torch.int32), (place, torch.int32))))
+
+
+def _poison(*shapes):
+    """Memory that the next tensors of these shapes are likely to get is filled with NaN."""
+    held = [torch.full(shape, float("nan"), dtype=t, device=DEV)
+            for shape in shapes for t in DTYPES for _ in range(4)]
+    del held
+
+
+def _check_all(x, w, b, routes, act, gather, combine, seed=60):
+    n, k = routes.experts.shape
+    o = w.shape[1]
+    dy = _rand((n if combine else n * k, o), x.dtype, seed)
+    _poison((n, o), (n * k, o), (n * k, x.shape[1]), x.shape, w.shape)
+    y, grads = _step(x, w, b, routes, dy, act, gather, combine)
+    ref = _Reference(x, w, b, routes, act, gather, combine)
+    _close(y, ref.out, ref.bound, "y")
+    for name, (g, bound) in ref.gradients(dy).items():
+        if name in grads:
+            _close(grads[name], g, bound, (name, act, gather, combine))
+    _poison((n, o), (n * k, o))
+    with torch.no_grad():
+        again = expert_linear(x, w, routes, b, activation=act, gather=gather, combine=combine)
+    assert torch.equal(y, again)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("chosen", [[2, 2], [1, 3, 1], [0] * 8, [3, 2, 3, -1, 2], [1] * 9, [2] * 32,
+                                    [0, 1, 2, 3] * 8, [1] * 40], ids=lambda c: f"{len(c)}:{c[:4]}")
+def test_one_row_that_names_an_expert_more_than_once(dtype, chosen):
+    e = 4
+    for i, o in ((64, 200), (33, 65), (64, 1)):
+        for f, (gather, combine) in enumerate(FORMS):
+            x, w, b = _inputs(1, e, len(chosen), i, o, dtype, gather, f)
+            _check_all(x, w, b if f else None, _made([chosen], e), ACTS[f], gather, combine)
+    N.check_device_status(DEV)
