@@ -23,26 +23,38 @@ def _row(t: torch.Tensor) -> tuple[int, int, int]:
     return t.data_ptr(), t.stride(0) if per_batch else 0, N.DTYPE_CODE[t.dtype]
 
 
+def _laid_out(t: torch.Tensor, c: int) -> torch.Tensor:
+    """Coefficients as ``_row`` takes them: contiguous rows that do not overlap."""
+
+    if t.is_contiguous() or (
+            (t.stride(-1) == 1 or c <= 1) and (t.ndim == 1 or t.stride(0) >= c)):
+        return t
+    return t.contiguous()
+
+
 class _Call:
-    """What both passes hand to the library beside the tensors of their own."""
+    """What both passes hand to the library beside their tensors. No address and no stride: the tensors that
+    autograd hands to the backward pass may be others than those it was given (recomputed by a checkpoint,
+    or brought back from the host)."""
 
-    __slots__ = ("n", "c", "code", "batch", "per_batch", "branch_stride", "rows", "p", "seed",
-                 "subsequence", "layer", "branch_norm", "residual_scale", "eps")
+    __slots__ = ("n", "c", "code", "batch", "per_batch", "p", "seed", "subsequence", "layer",
+                 "branch_norm", "residual_scale", "eps")
 
-    def pack(self, x, x_stride, branch, h, stats, coords, seed_at) -> bytes:
+    def pack(self, x, x_stride, branch, h, stats, coords, rows, seed_at) -> bytes:
         return N.BLOCK_NORM_ARGS.pack(
-            self.n, self.batch, x, x_stride, branch.data_ptr(), self.branch_stride, h.data_ptr(),
+            self.n, self.batch, x, x_stride, branch.data_ptr(), max(branch.stride(0), self.c),
+            h.data_ptr(),
             0 if stats is None else stats.data_ptr(), 0 if coords is None else coords.data_ptr(),
-            *self.rows, self.p, self.seed, 0 if seed_at is None else seed_at.data_ptr(),
+            *rows, self.p, self.seed, 0 if seed_at is None else seed_at.data_ptr(),
             self.subsequence, self.c, self.code, self.layer, self.branch_norm,
             self.residual_scale, self.eps)
 
 
-def _forward(x, branch, coords, seed_at, o, keep):
+def _forward(x, branch, coords, seed_at, o, rows, keep):
     n, c, dev = o.n, o.c, x.device
     h, y = x.new_empty((n, c)), x.new_empty((n, c))
     stats = torch.empty((n, 4), dtype=torch.float32, device=dev) if keep else None
-    args = o.pack(x.data_ptr(), max(x.stride(0), c), branch, h, stats, coords, seed_at)
+    args = o.pack(x.data_ptr(), max(x.stride(0), c), branch, h, stats, coords, rows, seed_at)
     rc = N.call(dev, N.load().sv_block_norm, args, y.data_ptr(), N.status_word(dev).data_ptr(),
                 N.stream(dev))
     if rc:
@@ -52,8 +64,8 @@ def _forward(x, branch, coords, seed_at, o, keep):
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, branch, coords, seed_at, o, *coefs):
-        y, h, stats = _forward(x, branch, coords, seed_at, o, True)
+    def forward(ctx, x, branch, coords, seed_at, o, rows, *coefs):
+        y, h, stats = _forward(x, branch, coords, seed_at, o, rows, True)
         ctx.save_for_backward(branch, h, stats, coords, seed_at, *coefs)
         ctx.options = o
         ctx.set_materialize_grads(False)
@@ -63,30 +75,38 @@ class _BlockNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dh):
         branch, h, stats, coords, seed_at, *coefs = ctx.saved_tensors
-        need_x, need_branch, _, _, _, *need = ctx.needs_input_grad
+        need_x, need_branch, _, _, _, _, *need = ctx.needs_input_grad
         if dy is None and dh is None:
-            return (None,) * (5 + len(need))
+            return (None,) * (6 + len(need))
         o, dev = ctx.options, h.device
+        h, stats = h.contiguous(), stats.contiguous()
+        coords = None if coords is None else coords.contiguous()
+        if o.c:
+            branch = _rows(branch, o.c)
+        rows = []
+        coefs = [None if t is None else _laid_out(t, o.c) for t in coefs]
+        for t in coefs:
+            rows += _NONE if t is None else _row(t)
         dy = None if dy is None else dy.contiguous()
         dh = None if dh is None else dh.contiguous()
         dx = torch.empty_like(h) if need_x else None
         dbranch = torch.empty_like(h) if need_branch else None
         grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if want else None
                  for t, want in zip(coefs, need)]
-        rows = []
+        wanted = []
         for t in grads:
-            rows += _NONE if t is None else _row(t)
+            wanted += _NONE if t is None else _row(t)
         lib = N.load()
         nbytes, ws = 0, None
         if o.per_batch or any(need):
             nbytes = lib.sv_block_norm_backward_workspace_bytes(o.n, o.c, o.batch if o.per_batch else 0)
             ws = N.workspace(nbytes, dev)
-        rc = N.call(dev, lib.sv_block_norm_backward, o.pack(0, 0, branch, h, stats, coords, seed_at),
-                    N.ptr(dy), N.ptr(dh), N.ptr(dx), N.ptr(dbranch), N.BLOCK_NORM_GRADS.pack(*rows),
+        rc = N.call(dev, lib.sv_block_norm_backward, o.pack(0, 0, branch, h, stats, coords, rows, seed_at),
+                    N.ptr(dy), N.ptr(dh), N.ptr(dx), N.ptr(dbranch), N.BLOCK_NORM_GRADS.pack(*wanted),
                     N.ptr(ws), nbytes, N.status_word(dev).data_ptr(), N.stream(dev))
         if rc:
             N.check(rc, "block_norm (backward)")
-        return dx, dbranch, None, None, None, *grads
+        return dx, dbranch, None, None, None, None, *grads
 
 
 def block_norm(
@@ -165,9 +185,7 @@ def block_norm(
             if largest not in (1, size[0]):
                 raise ValueError(f"block_norm: {name} has {size[0]} rows, others {largest}")
             largest = size[0]
-        if not t.is_contiguous() and not (
-                (t.stride(-1) == 1 or c <= 1) and (len(size) == 1 or t.stride(0) >= c)):
-            t = t.contiguous()
+        t = _laid_out(t, c)
         some = some or (grads and t.requires_grad)
         coefs.append(t)
         packed += _row(t)
@@ -203,16 +221,15 @@ def block_norm(
         x = _rows(x, c) if c else x.reshape(rows, 0)
     if not (flat and branch.is_contiguous()):
         branch = _rows(branch, c) if c else branch.reshape(rows, 0)
-    o.n, o.c, o.code, o.batch, o.per_batch, o.rows = rows, c, N.DTYPE_CODE[dtype], batch, largest != 1, packed
-    o.branch_stride = max(branch.stride(0), c)
+    o.n, o.c, o.code, o.batch, o.per_batch = rows, c, N.DTYPE_CODE[dtype], batch, largest != 1
     o.p, o.seed, o.subsequence = p, seed_value, subsequence
     o.layer, o.branch_norm = int(norm == "layer"), int(bool(branch_norm))
     o.residual_scale, o.eps = float(residual_scale), float(eps)
     if some:
         coords, seed_at = N.savable(coords), N.savable(seed_at)
-        y, h = _BlockNorm.apply(x, branch, coords, seed_at, o, *coefs)
+        y, h = _BlockNorm.apply(x, branch, coords, seed_at, o, packed, *coefs)
     else:
-        y, h, _ = _forward(x, branch, coords, seed_at, o, False)
+        y, h, _ = _forward(x, branch, coords, seed_at, o, packed, False)
     return (y, h) if flat else (y.reshape(shape), h.reshape(shape))
 
 

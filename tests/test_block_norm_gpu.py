@@ -435,3 +435,40 @@ def test_rows_past_32_bits():
         _close(dx[last:], *want["x"], "dx")
         _close(db[last:], *want["branch"], "dbranch")
         del b, big, y, h, dx, db, g
+
+
+def _hooked(how, run, *leaves):
+    if how == "checkpoint":
+        from torch.utils.checkpoint import checkpoint
+
+        return checkpoint(run, *leaves, use_reentrant=False)
+    with torch.autograd.graph.save_on_cpu(pin_memory=how == "pinned"):
+        return run(*leaves)
+
+
+@pytest.mark.parametrize("how", ["checkpoint", "host", "pinned"])
+def test_saved_tensors_that_come_back_as_others(how):
+    """Coefficients formed inside the region and rows apart: the backward pass gets tensors at other addresses
+    with other strides, and the first ones' memory is gone."""
+    n, c = 300, 72
+    g = torch.Generator(device=DEV).manual_seed(23)
+    leaves = [torch.randn(s, device=DEV, generator=g).requires_grad_(True)
+              for s in ((n, 3 * c), (2, 16), (16, 3 * c), (c,))]
+    coords = torch.zeros((n, 4), dtype=torch.int32, device=DEV)
+    coords[n // 3:, 0] = 1
+
+    def run(rows, cond, weight, norm):
+        gate, scale, shift = (cond @ weight).chunk(3, 1)
+        return block_norm(rows[:, :c], rows[:, 2 * c:], gate=gate, scale=scale, shift=shift,
+                          weight=2 * norm, branch_norm=True, branch_weight=norm + 1, coords=coords,
+                          dropout=0.25, seed=torch.tensor(7, device=DEV))
+
+    outs = []
+    for i in range(2):
+        y, h = _hooked(how, run, *leaves) if i else run(*leaves)
+        spill = [torch.full((n, 3 * c), float("nan"), device=DEV) for _ in range(8)]  # over what was freed
+        outs.append((y, h, *torch.autograd.grad((y, h), leaves, (y.detach(), h.detach()))))
+        del spill
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    N.check_device_status(DEV)

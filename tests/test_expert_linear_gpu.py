@@ -607,3 +607,31 @@ def test_one_row_that_names_an_expert_more_than_once(dtype, chosen):
             x, w, b = _inputs(1, e, len(chosen), i, o, dtype, gather, f)
             _check_all(x, w, b if f else None, _made([chosen], e), ACTS[f], gather, combine)
     N.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("how", ["checkpoint", "host"])
+def test_saved_tensors_that_come_back_as_others(how):
+    from mlx_diffuser_b200 import dropout
+    from tests.test_block_norm_gpu import _hooked
+
+    n, e, k, i, o = 200, 4, 2, 64, 72
+    x, w, b = (t.requires_grad_(True) for t in _inputs(n, e, k, i, o, torch.bfloat16, True))
+    logits = _rand((n, e), torch.float32, 5).requires_grad_(True)
+    wide = _rand((e, o, 2 * i), torch.bfloat16, 6).requires_grad_(True)
+
+    def run(x, w, b, logits, wide):
+        r = route(2 * logits, k)
+        z = expert_linear(x * 2, wide[:, :, i:], r, b, activation="silu", gather=True)
+        z = expert_linear(z, w.transpose(1, 2), r, combine=True)
+        return dropout(z, 0.25, torch.tensor(3, device=DEV), residual=x)
+
+    leaves, outs = [x, w, b, logits, wide], []
+    dy = _rand((n, i), torch.bfloat16, 7)
+    for j in range(2):
+        y = _hooked(how, run, *leaves) if j else run(*leaves)
+        spill = [torch.full((n * k, 2 * i), float("nan"), device=DEV) for _ in range(16)]
+        outs.append((y, *torch.autograd.grad(y, leaves, dy)))
+        del spill
+    for a, c in zip(*outs):
+        assert torch.equal(a, c)
+    N.check_device_status(DEV)

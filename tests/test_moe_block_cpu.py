@@ -327,3 +327,63 @@ def test_experts_epilogue_warps_meet_their_barrier_equally_often():
     assert "continue" not in head
     assert tail.index("if (!ok) continue;") < tail.index("mbar_wait_bounded")
     assert "mbar_try_wait" not in loop
+
+
+class _Recorder:
+    """Stands for the library: keeps the packed arguments and launches nothing."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        if name.endswith("_bytes"):
+            return lambda *args: 256
+
+        def entry(*args):
+            self.calls.append((name, args))
+            return N.SV_OK
+
+        return entry
+
+
+def test_block_norm_backward_reads_the_tensors_that_autograd_hands_it(monkeypatch):
+    """Saved tensors that come back as others (a checkpoint's recomputation, copies on the host) lie at other
+    addresses with other strides than those of the forward call, whose memory may be gone."""
+    lib = _Recorder()
+    monkeypatch.setattr(N, "load", lambda: lib)
+    monkeypatch.setattr(N, "require_cuda", lambda t, name: None)
+    monkeypatch.setattr(N, "call", lambda device, fn, *args: fn(*args))
+    monkeypatch.setattr(N, "stream", lambda device: 0)
+    monkeypatch.setattr(N, "status_word", lambda device: torch.zeros(1, dtype=torch.int32))
+    back = []
+
+    def unpack(t):  # another tensor, dense
+        back.append(t.clone(memory_format=torch.contiguous_format))
+        return back[-1]
+
+    n, c = 6, 8
+    wide = torch.randn((n, 24))
+    six = torch.randn((3, 6 * c))
+    leaves = {"x": torch.randn((n, c)), "branch": wide[:, 8:16], "weight": torch.randn(c),
+              "bias": torch.randn(2 * c)[::2], "branch_weight": torch.randn(c), "gate": six[:, :c],
+              "scale": six[:, c:2 * c], "shift": torch.randn((1, c))}
+    leaves = {k: t.requires_grad_(True) for k, t in leaves.items()}
+    coords = torch.zeros((n, 4), dtype=torch.int32)
+    seed = torch.ones(1, dtype=torch.int64)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y, h = block_norm(**leaves, branch_norm=True, coords=coords, batch_size=3, dropout=0.5, seed=seed)
+    torch.autograd.grad((y, h), list(leaves.values()), (torch.ones_like(y), torch.ones_like(h)))
+    (first, forward), (second, backward) = lib.calls
+    assert (first, second) == ("sv_block_norm", "sv_block_norm_backward")
+    a = _BlockNormArgs.from_buffer_copy(forward[0])
+    assert (a.branch, a.branch_stride) == (leaves["branch"].data_ptr(), 24)
+    assert (a.gate.data, a.gate.stride) == (leaves["gate"].data_ptr(), 6 * c)
+    b = _BlockNormArgs.from_buffer_copy(backward[0])
+    held = {t.data_ptr(): t for t in back}
+    for name in ("branch", "h", "stats", "coords", "seed_at"):
+        assert getattr(b, name) in held, name
+    assert b.branch_stride == c
+    for name in ("weight", "bias", "branch_weight", "gate", "scale", "shift"):
+        row = getattr(b, name)
+        assert row.data in held and held[row.data].shape == leaves[name].shape, name
+        assert row.stride == (c if name in ("gate", "scale") else 0), name
