@@ -52,13 +52,13 @@ __device__ __forceinline__ int64_t row_of(const Routing& r, int64_t p) {
   return slot >= 0 && slot < r.slots ? slot / r.k : -1;
 }
 
-// Zeros in the rows behind the last expert's position, by 256 threads of each of `blocks` blocks.
+// Zeros in the rows that no expert has, by 256 threads of each of `blocks` blocks.
 template <typename T>
-__device__ __forceinline__ void clear_tail(const Routing& r, int64_t n, T* out, int block, int blocks) {
-  const int64_t first = segment_at(r.offsets, r.experts - 1, (int)r.slots).last;
-  for (int64_t i = first * n + (int64_t)block * 256 + threadIdx.x; i < r.slots * n;
-       i += (int64_t)blocks * 256)
-    out[i] = from_f32<T>(0.f);
+__device__ __forceinline__ void clear_rest(const Routing& r, int64_t n, T* out, int block, int blocks) {
+  const Segment has = covered(r.offsets, r.experts, (int)r.slots);
+  const int64_t head = has.first * n, skip = (has.last - has.first) * n;
+  for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < r.slots * n - skip; i += (int64_t)blocks * 256)
+    out[i < head ? i : i + skip] = from_f32<T>(0.f);
 }
 
 // ---- few positions -------------------------------------------------------------------------------
@@ -151,10 +151,10 @@ __device__ __forceinline__ void few_rows(const T* x, int64_t ldx, const T* w, co
 template <typename T, bool LONE, int V, int W>
 __global__ void __launch_bounds__(256)
     expert_few_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
-                      int64_t w_expert, Routing r, bool gather, bool zero_tail, int64_t n,
+                      int64_t w_expert, Routing r, bool gather, bool zero_rest, int64_t n,
                       int64_t k, Epilogue ep, int32_t* status) {
   __shared__ float part[8][FEW_ROWS];
-  if (zero_tail && blockIdx.y == 0) clear_tail(r, n, static_cast<T*>(ep.out), blockIdx.x, gridDim.x);
+  if (zero_rest && blockIdx.y == 0) clear_rest(r, n, static_cast<T*>(ep.out), blockIdx.x, gridDim.x);
   const Piece p = find_piece<false>(r.offsets, r.experts, (int)r.slots, LONE ? 1 : FEW_ROWS, blockIdx.y);
   if (p.group < 0) return;
   const int64_t j = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -169,8 +169,8 @@ __global__ void __launch_bounds__(256)
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) expert_tail_kernel(Routing r, int64_t n, T* out) {
-  clear_tail(r, n, out, blockIdx.x, gridDim.x);
+__global__ void __launch_bounds__(256) expert_rest_kernel(Routing r, int64_t n, T* out) {
+  clear_rest(r, n, out, blockIdx.x, gridDim.x);
 }
 
 // ---- fp32 ----------------------------------------------------------------------------------------
@@ -341,12 +341,14 @@ __device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
   }
 }
 
-// out[n] = sum_j w_nj rows[place_nj], in the order of the choices (not weighted: ones). V elements a thread.
+// out[n] = sum_j w_nj rows[place_nj], in the order of the choices (not weighted: ones), over the places that
+// an expert has: the others' rows were not formed. V elements a thread.
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
     expert_combine_kernel(const float* __restrict__ rows, Routing r, bool weighted, int64_t cols,
                           T* __restrict__ out) {
   const int64_t across = cols / V, total = r.n * across;
+  const Segment has = covered(r.offsets, r.experts, (int)r.slots);
   for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total;
        at += (int64_t)gridDim.x * 256) {
     const int64_t n = total <= UINT32_MAX ? (uint32_t)at / (uint32_t)across : at / across;
@@ -357,7 +359,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll 2
     for (int j = 0; j < r.k; ++j) {
       const int32_t p = __ldg(r.place + n * r.k + j);
-      if (p < 0 || p >= r.slots) continue;
+      if (p < has.first || p >= has.last) continue;
       const float w = weighted ? __ldg(r.weights + n * r.k + j) : 1.f;
       float v[V];
       load_v<float, V>(rows + (int64_t)p * cols + c, v);
@@ -495,10 +497,11 @@ __global__ void __launch_bounds__(256)
                            int64_t cols, float* __restrict__ out) {
   const int lane = threadIdx.x & 31;
   const int64_t step = (int64_t)gridDim.x * 8;
+  const Segment has = covered(r.offsets, r.experts, (int)r.slots);
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < r.slots; i += step) {
     const int32_t p = __ldg(r.place + i);
     float sum = 0.f;
-    if (p >= 0 && p < r.slots) {
+    if (p >= has.first && p < has.last) {
       const T* g = dy + i / r.k * cols;
       const float* v = rows + (int64_t)p * cols;
 #pragma unroll 2
@@ -639,9 +642,9 @@ ExpertTile pick_tile(int64_t experts, int64_t m, int64_t n, int64_t k) {
 int product(const ExpertGemm& g, void* maps, int32_t* status, cudaStream_t s) {
   if (g.dtype == SV_FLOAT32) {
     const int rc = expert_gemm_f32(g, s);
-    if (rc != SV_OK || !g.zero_tail) return rc;
+    if (rc != SV_OK || !g.zero_rest) return rc;
     const Routing r{nullptr, g.offsets, nullptr, nullptr, 0, 1, g.experts, g.slots};
-    expert_tail_kernel<float><<<num_sms(), 256, 0, s>>>(r, g.n, static_cast<float*>(g.ep.out));
+    expert_rest_kernel<float><<<num_sms(), 256, 0, s>>>(r, g.n, static_cast<float*>(g.ep.out));
     SV_LAUNCH_CHECK();
     return SV_OK;
   }
@@ -827,7 +830,7 @@ extern "C" int sv_expert_linear(const sv_expert_args* args, void* out, void* wor
     e.n = g.outputs;
     e.k = g.inputs;
     e.dtype = g.dtype;
-    e.zero_tail = !g.combine;
+    e.zero_rest = !g.combine;
     e.ep = ep;
     if (g.inputs > 0 && pad_x(g)) {
       bad = gather_rows(g.x, g.ldx, r, g.gather != 0, g.inputs, g.dtype, ws + l.x, l.ldx, status, s);
@@ -937,7 +940,7 @@ extern "C" int sv_expert_linear_backward(const sv_expert_args* args, const void*
   }
   e.n = g.inputs;
   e.k = g.outputs;
-  e.zero_tail = !g.gather;
+  e.zero_rest = !g.gather;
   e.ep = {nullptr, nullptr, 0, nullptr, a.raise.down, rows, nullptr, nullptr,
           g.gather ? (int)SV_FLOAT32 : g.dtype, SV_ACT_NONE};
   bad = product(e, nullptr, status, s);

@@ -22,9 +22,9 @@ struct ExpertGemm {
   int64_t slots;
   int64_t m, n, k;          // kRows: columns n, sum over k; kWeights: an expert's [m][n]
   int dtype;
-  bool zero_tail;           // kRows: positions behind the last expert's are set to zero
+  bool zero_rest;           // kRows: positions that no expert has are set to zero
   Epilogue ep;              // bias: [experts][n]; out: [slots][n] or [experts][m][n], in out_dtype: dtype,
-                            // or fp32 for kRows without zero_tail
+                            // or fp32 for kRows without zero_rest
 };
 
 // expert_tc.cu (fp16 / bf16): operands and strides of multiples of 16 bytes. kWeights needs

@@ -82,7 +82,7 @@ struct ExArgs {
   int32_t tiles_m, tiles_n;  // tiles_m: kWeights
   int32_t steps;           // kRows
   uint32_t idesc;
-  bool b_mn, wide_io, zero_tail;
+  bool b_mn, wide_io, zero_rest;
   bool direct;             // the result's rows are multiples of 16 columns on 32-byte boundaries
   const CUtensorMap* maps;  // kWeights: [experts][2]
 };
@@ -569,11 +569,11 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
       }
     }
     if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
-    if (!WEIGHTS && a.zero_tail) {
-      const int64_t end = a.slots * a.n;
-      for (int64_t i = (int64_t)s_seg[a.experts - 1].y * a.n + (int64_t)blockIdx.x * EX_EPI_THREADS + e;
-           i < end; i += (int64_t)gridDim.x * EX_EPI_THREADS)
-        static_cast<O*>(ep.out)[i] = from_f32<O>(0.f);
+    if (!WEIGHTS && a.zero_rest) {
+      const int64_t head = s_seg[0].x * a.n, skip = s_seg[a.experts - 1].y * a.n - head;
+      for (int64_t i = (int64_t)blockIdx.x * EX_EPI_THREADS + e; i < a.slots * a.n - skip;
+           i += (int64_t)gridDim.x * EX_EPI_THREADS)
+        static_cast<O*>(ep.out)[i < head ? i : i + skip] = from_f32<O>(0.f);
     }
   }
 
@@ -695,7 +695,7 @@ int launch_expert(const ExpertGemm& g, CUtensorMap* maps, int32_t* status, cudaS
   a.tiles_m = (int32_t)((g.m + ROWS - 1) / ROWS);
   a.steps = (int32_t)((g.k + 63) / 64);
   a.b_mn = g.b.mn;
-  a.zero_tail = g.zero_tail;
+  a.zero_rest = g.zero_rest;
   a.maps = maps;
   a.idesc = idesc_f16_major(g.dtype == SV_BFLOAT16, ROWS, BN, WEIGHTS, WEIGHTS || g.b.mn);
   const int64_t pieces = WEIGHTS ? (int64_t)g.experts * a.tiles_m : g.slots / ROWS + g.experts;

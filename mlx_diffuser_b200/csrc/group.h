@@ -168,6 +168,13 @@ __device__ __forceinline__ Segment segment_at(const int32_t* offsets, int g, int
   }
   return {first, max(first, inside(offsets, g + 1, limit))};
 }
+// The positions that segments have, all of them together: those before the first segment and behind the last
+// one have none.
+__device__ __forceinline__ Segment covered(const int32_t* offsets, int groups, int limit) {
+  int last = 0;
+  for (int j = threadIdx.x & 31; j <= groups; j += 32) last = max(last, inside(offsets, j, limit));
+  return {inside(offsets, 0, limit), __reduce_max_sync(0xffffffffu, last)};
+}
 // A lane's inclusive maximum over the lanes up to it, and `before`.
 __device__ __forceinline__ int rising(int v, int before) {
 #pragma unroll

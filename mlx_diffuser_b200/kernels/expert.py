@@ -208,9 +208,9 @@ def expert_linear(
     ``weight`` is (experts, N, K), ``bias`` (experts, N); ``activation`` as in
     :func:`~mlx_diffuser_b200.linear`. With ``gather``, ``x`` is (rows, K) and each position takes its
     row; without it, ``x`` is (rows * k, K) in the order of the experts, such as the result of a call
-    without ``combine``: (rows * k, N), zeros behind the last expert's position. With ``combine`` the result
-    is (rows, N): ``sum_j routes.weights[:, j] * r[routes.place[:, j]]`` over the choices that have an
-    expert, where r, held in float32, are the positions' results. A feed-forward block of experts is
+    without ``combine``: (rows * k, N), zeros where no expert has the position. With ``combine`` the result
+    is (rows, N): ``sum_j routes.weights[:, j] * r[routes.place[:, j]]`` over the places that an expert
+    has, where r, held in float32, are the positions' results. A feed-forward block of experts is
 
         h = expert_linear(x, up, routes, activation="gelu_tanh", gather=True)
         y = expert_linear(h, down, routes, combine=True)

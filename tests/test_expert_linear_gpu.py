@@ -576,7 +576,7 @@ def _made(chosen, e, offsets=None):
 def _poison(*shapes):
     """Memory that the next tensors of these shapes are likely to get is filled with NaN."""
     held = [torch.full(shape, float("nan"), dtype=t, device=DEV)
-            for shape in shapes for t in DTYPES for _ in range(4)]
+            for shape in (*shapes, (2**15,), (2**21,)) for t in DTYPES for _ in range(4)]
     del held
 
 
@@ -634,4 +634,22 @@ def test_saved_tensors_that_come_back_as_others(how):
         del spill
     for a, c in zip(*outs):
         assert torch.equal(a, c)
+    N.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, offsets", [(100, [10, 50, 50, 120, 120]), (100, [200, 200, 200, 200, 200]),
+                                        (700, [1, 300, 300, 1300, 1399]), (700, [1400, 1400, 1400, 1400, 1400]),
+                                        (3, [1, 2, 2, 4, 5]), (1, [1, 1, 2, 2, 2]), (2, [4, 4, 4, 4, 4])],
+                         ids=str)
+def test_positions_that_no_expert_has(dtype, n, offsets):
+    """Before the first offset and behind the last one: zeros, in the results and in x's gradient, and a place
+    there counts as none. Nothing is read that was not written."""
+    e = 4
+    g = torch.Generator().manual_seed(n)
+    routes = _made(torch.randint(0, e, (n, 2), generator=g).tolist(), e, offsets)
+    for i, o in ((64, 72), (33, 65)):
+        for f, (gather, combine) in enumerate(FORMS):
+            x, w, b = _inputs(n, e, 2, i, o, dtype, gather, f)
+            _check_all(x, w, b, routes, ACTS[f], gather, combine)
     N.check_device_status(DEV)
