@@ -382,7 +382,6 @@ struct DzArgs {
   int64_t ld_dz;
   float* partial;        // [pieces][cols], or null
   Raise raise;           // fp16
-  float headroom;        // what raise_of is multiplied by
 };
 
 // dz_p = w dy act'(z), rounded to the feature type as the products' operand (raise.cuh), and the column
@@ -396,7 +395,8 @@ __global__ void __launch_bounds__(256, 4) expert_dz_kernel(const __grid_constant
   if constexpr (std::is_same<T, __half>::value) {
     if (a.raise.top != nullptr) {
       // the largest finite |dy|: one expert's infinity leaves the others' gradients their range
-      up = raise_of(__ldg(a.raise.top)) * a.headroom;
+      up = raise_of(__ldg(a.raise.top));
+      if (a.combine) up *= room_of(__ldg(a.raise.top + 1));
       if (blockIdx.x == 0 && blockIdx.y == 0)
         for (int64_t i = threadIdx.x; i < a.raise.k; i += 256) a.raise.down[i] = 1.0f / up;
     }
@@ -892,11 +892,11 @@ extern "C" int sv_expert_linear_backward(const sv_expert_args* args, const void*
   a.dz = hold && (dx || dweight) ? ws + l.dz : nullptr;
   a.ld_dz = l.ld_dz;
   a.partial = dbias ? reinterpret_cast<float*>(ws + l.partial) : nullptr;
-  a.headroom = g.combine ? 0.0625f : 1.0f;  // weights of up to 16 keep dz in fp16's range
   if (a.dz && (act || g.combine) && g.dtype == SV_FLOAT16) {
     a.raise = {reinterpret_cast<unsigned*>(ws + l.raise),
                reinterpret_cast<float*>(ws + l.raise + ALIGN), g.inputs};
-    const int bad = find_top<true>(dout, (g.combine ? g.n : r.slots) * g.outputs, a.raise.top, s);
+    const int bad = g.combine ? find_top<true>(dout, g.n * g.outputs, g.weights, r.slots, a.raise.top, s)
+                              : find_top<true>(dout, r.slots * g.outputs, nullptr, 0, a.raise.top, s);
     if (bad != SV_OK) return bad;
   }
   int bad = g.dtype == SV_FLOAT32

@@ -445,7 +445,7 @@ template <typename T>
 int dz_typed(const void* dy, const float* z, int64_t m, int64_t n, int act, void* dz, int64_t ld,
              void* db, float* partial, const Raise& raise, cudaStream_t s) {
   if (raise.top) {
-    const int rc = find_top<false>(dy, m * n, raise.top, s);
+    const int rc = find_top<false>(dy, m * n, nullptr, 0, raise.top, s);
     if (rc != SV_OK) return rc;
   }
   const bool vec = n % 4 == 0 && aligned16(dy) && aligned16(z) && aligned16(dz);

@@ -9,11 +9,13 @@ namespace sv {
 
 // dz is rounded to the feature type, since the tensor cores take it as an operand of both products: half
 // a step more beside the result's own (0.0023 against 0.0017 over the gradients of 12,001 x 1024 x 1024
-// bf16). fp16's is raised by a power of two first, and the products' column scales take that back: below 2^-14 a half has no 11 bits, and the gradients of a mean loss lie there. The power puts the
-// largest |dy| below 2^15 (the activations' slopes are below 1.13), so values down to 2^-28 of it keep
-// all their bits. It costs a pass over dy: 12,001 x 1024 in 7 us.
+// bf16). fp16's is raised by a power of two first, and the products' column scales take that back: below
+// 2^-14 a half has no 11 bits, and the gradients of a mean loss lie there. The power puts the largest |dy|
+// times the largest |weight| that it is multiplied by below 2^15 (the activations' slopes are below 1.13),
+// so values down to 2^-28 of it keep all their bits. It costs a pass over dy: 12,001 x 1024 in 7 us.
 struct Raise {
-  unsigned* top;  // bits of the largest |dy|, as a half; null: dz is not raised
+  unsigned* top;  // [2]: bits of the largest |dy|, as a half, and of the largest finite |weight|; null: dz
+                  // is not raised
   float* down;    // [k]: what the products are multiplied by
   int64_t k;
 };
@@ -21,6 +23,11 @@ __device__ __forceinline__ float raise_of(unsigned top) {
   if (top == 0u || top >= 0x7c00u) return 1.0f;  // nothing, or not a number
   const float x = __half2float(__ushort_as_half((unsigned short)top));
   return __uint_as_float((268u - (__float_as_uint(x) >> 23)) << 23);  // 2^14 <= x * this < 2^15
+}
+// The power of two that puts the weight with these bits into [1/2, 1), between 2^-100 and 2^64: with
+// raise_of's (2^-1 to 2^38) it and its reciprocal stay normal numbers.
+__device__ __forceinline__ float room_of(unsigned weight) {
+  return __uint_as_float(min(max(253 - (int)(weight >> 23), 27), 191) << 23);
 }
 
 namespace {
@@ -34,7 +41,8 @@ __device__ __forceinline__ unsigned larger(unsigned most, unsigned x) {
 
 template <int V, bool FINITE>
 __global__ void __launch_bounds__(256)
-    top_kernel(const unsigned short* __restrict__ x, int64_t cells, unsigned* __restrict__ top) {
+    top_kernel(const unsigned short* __restrict__ x, int64_t cells, const float* __restrict__ weights,
+               int64_t count, unsigned* __restrict__ top) {
   unsigned most = 0u;  // of both halves of a word
   const int64_t step = (int64_t)gridDim.x * 256 * V;
 #pragma unroll 4
@@ -47,26 +55,38 @@ __global__ void __launch_bounds__(256)
       most = larger<FINITE>(most, x[i]);
     }
   }
-  __shared__ unsigned s_top[8];
+  __shared__ unsigned s_top[2][8];
+  unsigned heavy = 0u;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    const unsigned w = __float_as_uint(__ldg(weights + i)) & 0x7fffffffu;
+    if (w < 0x7f800000u) heavy = max(heavy, w);
+  }
   const unsigned one = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
-  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = one;
+  heavy = __reduce_max_sync(0xffffffffu, heavy);
+  if ((threadIdx.x & 31) == 0) {
+    s_top[0][threadIdx.x >> 5] = one;
+    s_top[1][threadIdx.x >> 5] = heavy;
+  }
   __syncthreads();
   if (threadIdx.x < 32) {  // one atomic a block: one a warp took 11 us
-    const unsigned all = __reduce_max_sync(0xffffffffu, threadIdx.x < 8 ? s_top[threadIdx.x] : 0u);
+    const unsigned all = __reduce_max_sync(0xffffffffu, threadIdx.x < 8 ? s_top[0][threadIdx.x] : 0u);
+    heavy = __reduce_max_sync(0xffffffffu, threadIdx.x < 8 ? s_top[1][threadIdx.x] : 0u);
     if (threadIdx.x == 0 && all) atomicMax(top, all);
+    if (threadIdx.x == 0 && heavy) atomicMax(top + 1, heavy);
   }
 }
 
-// *top = the largest magnitude of `cells` halves, as the bits of a half.
+// top[0] = the largest magnitude of `cells` halves, as the bits of a half, top[1] = that of `count` weights.
 template <bool FINITE>
-inline int find_top(const void* dy, int64_t cells, unsigned* top, cudaStream_t s) {
-  SV_CUDA_TRY(cudaMemsetAsync(top, 0, sizeof(unsigned), s));
+inline int find_top(const void* dy, int64_t cells, const float* weights, int64_t count, unsigned* top,
+                    cudaStream_t s) {
+  SV_CUDA_TRY(cudaMemsetAsync(top, 0, 2 * sizeof(unsigned), s));
   const unsigned short* x = static_cast<const unsigned short*>(dy);
   const bool wide = cells % 8 == 0 && aligned16(dy);
   const unsigned blocks = (unsigned)std::min<int64_t>((cells / (wide ? 8 : 1) + 255) / 256,
                                                       (int64_t)num_sms() * 8);
-  if (wide) top_kernel<8, FINITE><<<blocks, 256, 0, s>>>(x, cells, top);
-  else top_kernel<1, FINITE><<<blocks, 256, 0, s>>>(x, cells, top);
+  if (wide) top_kernel<8, FINITE><<<blocks, 256, 0, s>>>(x, cells, weights, count, top);
+  else top_kernel<1, FINITE><<<blocks, 256, 0, s>>>(x, cells, weights, count, top);
   SV_LAUNCH_CHECK();
   return SV_OK;
 }

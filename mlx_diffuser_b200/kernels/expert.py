@@ -216,9 +216,8 @@ def expert_linear(
         y = expert_linear(h, down, routes, combine=True)
 
     float32 (exact fp32 products), float16 and bfloat16 (tensor cores), every tensor of one type but the
-    routes' float32 weights, with gradients for all of them. In float16 the weights may be up to 16 in
-    magnitude: larger ones can take the products of the backward pass out of the type's range. No size
-    is read back to the host, whatever the experts' shares are.
+    routes' float32 weights, with gradients for all of them. No size is read back to the host, whatever the
+    experts' shares are.
     """
 
     x, weight = N.as_tensor(x), N.as_tensor(weight)

@@ -653,3 +653,37 @@ def test_positions_that_no_expert_has(dtype, n, offsets):
             x, w, b = _inputs(n, e, 2, i, o, dtype, gather, f)
             _check_all(x, w, b, routes, ACTS[f], gather, combine)
     N.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("scale", [2.0**-14, 1.0, 17.0, 500.0, 2.0**20])
+def test_large_and_small_weights_in_half_precision(scale):
+    """dz holds the products of dy and the weights: their range is taken into account, not dy's alone."""
+    n, e, k, i, o = 300, 4, 2, 72, 136
+    x, w, b = _inputs(n, e, k, i, o, torch.float16, True)
+    routes = _routes(n, e, k)
+    routes = dataclasses.replace(routes, weights=routes.weights * scale)
+    for act in (None, "gelu"):
+        # the result itself has to stay in the type's range
+        x1, w1 = (x, w * min(1.0, 2.0**-9 * 500 / scale)) if act is None else (x * 2.0**-10, w)
+        dy = _rand((n, o), torch.float16, 9, 2.0**-4 / max(1.0, scale / 100))
+        _, grads = _step(x1, w1, None, routes, dy, act, True, True)
+        ref = _Reference(x1, w1, None, routes, act, True, True)
+        for name, (g, bound) in ref.gradients(dy).items():
+            if name in grads:
+                assert torch.isfinite(grads[name]).all(), (name, act)
+                _close(grads[name], g, bound, (name, act))
+
+
+def test_a_weight_that_is_no_number_stays_with_its_row():
+    n, e, k, i, o = 300, 4, 2, 72, 136
+    x, w, b = _inputs(n, e, k, i, o, torch.float16, True)
+    routes = _routes(n, e, k, 0, "even")
+    dy = _rand((n, o), torch.float16, 9)
+    want = _Reference(x, w, b, routes, "silu", True, True).gradients(dy)["x"]
+    for bad in (float("inf"), float("nan")):
+        weights = routes.weights.clone()
+        weights[7] = bad
+        y, grads = _step(x, w, b, dataclasses.replace(routes, weights=weights), dy, "silu", True, True)
+        others = torch.arange(n, device=DEV) != 7
+        assert torch.isfinite(y[others]).all() and not torch.isfinite(grads["x"][7]).any()
+        _close(grads["x"][others], *(v[others] for v in want), bad)
