@@ -177,9 +177,7 @@ class _ExpertLinear(torch.autograd.Function):
         dx = x.new_empty(x.shape) if need_x else None
         dw = x.new_empty(weight.shape) if need_w else None
         db = x.new_empty(ctx.bias_shape) if need_b else None
-        dp = None
-        if need_p:  # without the weighted sum nothing reaches the weights
-            dp = torch.empty_like(p) if o[2] else torch.zeros_like(p)
+        dp = torch.empty_like(p) if need_p else None
         a = _pack(x, weight, None, p, order, offsets, place, preact, rows, o)
         lib = N.load()
         at = dout.data_ptr()
@@ -216,8 +214,8 @@ def expert_linear(
         y = expert_linear(h, down, routes, combine=True)
 
     float32 (exact fp32 products), float16 and bfloat16 (tensor cores), every tensor of one type but the
-    routes' float32 weights, with gradients for all of them. No size is read back to the host, whatever the
-    experts' shares are.
+    routes' float32 weights, with gradients for all of them (for the weights with ``combine``, which alone
+    reads them). No size is read back to the host, whatever the experts' shares are.
     """
 
     x, weight = N.as_tensor(x), N.as_tensor(weight)
@@ -263,11 +261,12 @@ def expert_linear(
         weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     order, offsets, place = routes.order.contiguous(), routes.offsets.contiguous(), routes.place.contiguous()
-    p = p.contiguous()
+    # without the weighted sum the weights are not read, and nothing goes back to the router
+    p = p.contiguous() if combine else p.detach() if p.requires_grad else p
     o = N.ACTIVATION_CODE[activation], int(bool(gather)), int(bool(combine))
     if torch.is_grad_enabled() and (
             x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-            or (combine and p.requires_grad)):
+            or p.requires_grad):
         return _ExpertLinear.apply(x, weight, bias, N.savable(p), N.savable(order),
                                    N.savable(offsets), N.savable(place), o)
     return _forward(x, weight, bias, p, order, offsets, place, o, False)[0]

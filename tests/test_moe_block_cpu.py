@@ -387,3 +387,26 @@ def test_block_norm_backward_reads_the_tensors_that_autograd_hands_it(monkeypatc
         row = getattr(b, name)
         assert row.data in held and held[row.data].shape == leaves[name].shape, name
         assert row.stride == (c if name in ("gate", "scale") else 0), name
+
+
+def test_routing_weights_that_are_not_read_get_no_gradient(monkeypatch):
+    """Without the weighted sum the result does not depend on them: no zeros go back through the router."""
+    lib = _Recorder()
+    monkeypatch.setattr(N, "load", lambda: lib)
+    monkeypatch.setattr(N, "require_cuda", lambda t, name: None)
+    monkeypatch.setattr(N, "call", lambda device, fn, *args: fn(*args))
+    monkeypatch.setattr(N, "stream", lambda device: 0)
+    monkeypatch.setattr(N, "status_word", lambda device: torch.zeros(1, dtype=torch.int32))
+    r, x = _routes(), torch.randn((6, 8), requires_grad=True)
+    p = torch.rand((6, 2), requires_grad=True)
+    w = torch.randn((4, 10, 8), requires_grad=True)
+    for combine in (False, True):
+        y = expert_linear(x, w, dataclasses.replace(r, weights=p * 1), gather=True, combine=combine)
+        lib.calls.clear()
+        dx, dw, dp = torch.autograd.grad(y, (x, w, p), torch.ones_like(y), allow_unused=True)
+        assert dx.shape == x.shape and dw.shape == w.shape
+        assert (dp is not None) == combine
+        ((name, args),) = lib.calls
+        assert name == "sv_expert_linear_backward" and (args[5] is not None) == combine
+    y = expert_linear(x.detach(), w.detach(), dataclasses.replace(r, weights=p), gather=True)
+    assert not y.requires_grad
