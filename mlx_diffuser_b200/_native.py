@@ -313,7 +313,8 @@ def status_word(device: torch.device) -> torch.Tensor:
     index = device.index if device.index is not None else torch.cuda.current_device()
     word = _status.get(index)
     if word is None:
-        word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        with torch.inference_mode(False):  # it is cleared in place wherever it is read
+            word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
         _status[index] = word
     return word
 

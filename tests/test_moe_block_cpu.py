@@ -410,3 +410,17 @@ def test_routing_weights_that_are_not_read_get_no_gradient(monkeypatch):
         assert name == "sv_expert_linear_backward" and (args[5] is not None) == combine
     y = expert_linear(x.detach(), w.detach(), dataclasses.replace(r, weights=p), gather=True)
     assert not y.requires_grad
+
+
+def test_status_word_made_under_inference_mode(monkeypatch):
+    """A process whose first call is under inference mode reads and clears the word outside of it."""
+    zeros, cuda = torch.zeros, torch.device("cuda", 0)
+    monkeypatch.setattr(torch, "zeros", lambda *args, device=None, **kw: zeros(*args, **kw))
+    monkeypatch.setattr(N, "_status", {})
+    with torch.inference_mode():
+        word = N.status_word(cuda)
+    assert not word.is_inference()
+    word.fill_(N.SV_DEVICE_BAD_INDEX)
+    with pytest.raises(RuntimeError, match="out of range"):
+        N.check_device_status(cuda)
+    N.check_device_status(cuda)
