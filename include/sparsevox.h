@@ -523,8 +523,9 @@ SV_API int sv_route_backward(const void* logits, int64_t stride, int64_t n, int 
  * inputs]), else x[p] (x [n k, inputs]); rows `ldx` apart. weight: rows `ldw` apart, experts `w_expert`
  * elements apart; bias [experts, outputs] or null. The result is r [n k, outputs], zeros where
  * no expert has the position, or with `combine` sum_j weights[n, j] r[place[n, j]], [n, outputs]; then
- * `rows` [n k, outputs] holds r in fp32. preact: receives the activation's argument in fp32, or null. dtype fp32 / fp16 / bf16,
- * fp32 sums; 16-bit types run on the tensor cores. An entry of order that is no slot counts as a row of
+ * `rows` [n k, outputs] holds r in fp32, with `combine` 2 as near as fp32 sums are (the tensor cores' are less
+ * near), for the weights' gradients. preact: receives the activation's argument in fp32, or null. dtype
+ * fp32 / fp16 / bf16, fp32 sums; 16-bit types run on the tensor cores. An entry of order that is no slot counts as a row of
  * zeros (SV_DEVICE_BAD_INDEX), one of place that no expert has as none; offsets are taken into [0, n k] and made
  * to rise. */
 typedef struct sv_expert_args {

@@ -831,6 +831,7 @@ extern "C" int sv_expert_linear(const sv_expert_args* args, void* out, void* wor
     e.k = g.inputs;
     e.dtype = g.dtype;
     e.zero_rest = !g.combine;
+    e.runs = g.combine > 1;
     e.ep = ep;
     if (g.inputs > 0 && pad_x(g)) {
       bad = gather_rows(g.x, g.ldx, r, g.gather != 0, g.inputs, g.dtype, ws + l.x, l.ldx, status, s);

@@ -23,6 +23,7 @@ struct ExpertGemm {
   int64_t m, n, k;          // kRows: columns n, sum over k; kWeights: an expert's [m][n]
   int dtype;
   bool zero_rest;           // kRows: positions that no expert has are set to zero
+  bool runs;                // kRows in fp32: sums over k as near as fp32's own (expert_tc.cu)
   Epilogue ep;              // bias: [experts][n]; out: [slots][n] or [experts][m][n], in out_dtype: dtype,
                             // or fp32 for kRows without zero_rest
 };

@@ -75,12 +75,22 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 
+// The tensor cores cut off what lies below a sum's last place at every addition, so that a sum's error grows with
+// k and has one sign: 2.1e-6 of the result at k 2048, where an fp32 sum is 3.9e-7 off. 16 bits do not
+// show it, but what is formed from results held in fp32 does (the gradients of the routing's weights: 1.9e-6
+// off, and 4.4e-7 so). For them the tensor cores add up runs of a few steps of 64, and the epilogue warps add
+// the runs up in fp32: of 4 steps up to k 512 (2.3e-7, where an fp32 sum is 1.6e-7 off), else of up to 8
+// (4.7e-7; the fp32 sum 2.5e-7 at k 1024). An epilogue warp takes 1,200 cycles for a run beside its stores:
+// 24,002 x 2048 -> 1024 takes 95 us in one sum, 113 in runs of 8 and took 16 more in runs of 4.
+inline int run_steps(int64_t steps) { return steps <= 8 ? 4 : 8; }
+
 struct ExArgs {
   const int32_t* offsets;
   int32_t experts, slots;
   int64_t m, n;            // m: kWeights
   int32_t tiles_m, tiles_n;  // tiles_m: kWeights
   int32_t steps;           // kRows
+  int32_t run, runs;       // not kOne: steps of a run, and runs of a tile
   uint32_t idesc;
   bool b_mn, wide_io, zero_rest;
   bool direct;             // the result's rows are multiples of 16 columns on 32-byte boundaries
@@ -187,6 +197,55 @@ __device__ __forceinline__ void store_sector(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
+// Adds COLS columns from TMEM to a lane's sums.
+template <int COLS>
+__device__ __forceinline__ void ex_add(float (&sum)[COLS], uint32_t t_row) {
+#pragma unroll
+  for (int i = 0; i < COLS; i += 16) {
+    uint32_t raw[16];
+    tmem_ld_32x32b_x16(t_row + i, raw);
+    tc_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum[i + j] += __uint_as_float(raw[j]);
+  }
+}
+
+// Sums that were added up in registers, without an activation: scaled, and to whole sectors of the lane's
+// row `to`, the columns from c0 on that are below c1. Arguments as ex_direct's.
+template <int COLS>
+__device__ __forceinline__ void ex_sums(const float (&sum)[COLS], int c0, int c1, const float* bias,
+                                        const float* scale, bool in, float* to) {
+#pragma unroll
+  for (int i = 0; i < COLS; i += 8) {
+    const int c = c0 + i;
+    if (c >= c1) continue;
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+      const float4 m = *reinterpret_cast<const float4*>(scale + c + j);
+      const float4 s = *reinterpret_cast<const float4*>(bias + c + j);
+      w[j] = __float_as_uint(fmaf(sum[i + j], m.x, s.x));
+      w[j + 1] = __float_as_uint(fmaf(sum[i + j + 1], m.y, s.y));
+      w[j + 2] = __float_as_uint(fmaf(sum[i + j + 2], m.z, s.z));
+      w[j + 3] = __float_as_uint(fmaf(sum[i + j + 3], m.w, s.w));
+    }
+    if (in) store_sector(to + c, w);
+  }
+}
+
+// Columns [at, at + 32) of a lane's sums into its row of the warp's staging.
+template <int COLS>
+__device__ __forceinline__ void ex_stage(const float (&sum)[COLS], int at, float* row) {
+#pragma unroll
+  for (int i = 0; i < COLS; i += 32) {
+    if (i != at) continue;  // registers have no index
+#pragma unroll
+    for (int j = 0; j < 32; j += 4)
+      *reinterpret_cast<float4*>(row + j) =
+          make_float4(sum[i + j], sum[i + j + 1], sum[i + j + 2], sum[i + j + 3]);
+  }
+}
+
 // A warp's columns [c0, c1) of a tile, a row a lane, straight from TMEM to whole sectors of global memory: no
 // turn through shared memory, half of the instructions an element. `bias`, `scale`: in shared memory, the
 // same address in all lanes, 0 and 1 where there are none: a multiply-add an element and no branch, which
@@ -239,7 +298,34 @@ __device__ __forceinline__ void ex_direct(uint32_t t_row, int c0, int c1, const 
   }
 }
 
-template <int BN, bool PAIR, typename O, bool WEIGHTS, bool WIDE>
+// Adds the sums of a tile's runs but the last one up, a row a lane and COLS columns from t_row on, and gives
+// their accumulators back. False: a wait has run out.
+template <int COLS, int BN, typename Give>
+__device__ __forceinline__ bool ex_collect(float (&sum)[COLS], uint32_t t_row, int runs, int& local,
+                                           uint64_t* acc_full, volatile int* abort_flag, Give&& give) {
+#pragma unroll
+  for (int i = 0; i < COLS; ++i) sum[i] = 0.f;
+  for (int r = 1; r < runs; ++r, ++local) {
+    const int ab = local & 1;
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[ab], (local >> 1) & 1, abort_flag)))
+      return false;
+    tc_fence_after();
+    ex_add<COLS>(sum, t_row + (uint32_t)(ab * BN));
+    give(ab);
+  }
+  return true;
+}
+
+// What a sum over k is made of, and where its result goes from.
+enum class Sums {
+  kOne,     // one sum in TMEM
+  kRuns,    // kRows in fp32: runs, added up in registers and stored from there in whole sectors, without an
+            // activation
+  kStaged,  // kRows in fp32: runs, with an activation or other columns: through shared memory (its registers
+            // spill: 580 bytes a thread, where kRuns spills 78)
+};
+
+template <int BN, bool PAIR, typename O, bool WEIGHTS, bool WIDE, Sums SUMS>
 __global__ void __launch_bounds__(EX_THREADS, 1)
     expert_tc_kernel(const __grid_constant__ CUtensorMap map_a,
                      const __grid_constant__ CUtensorMap map_b, ExArgs a, Epilogue ep,
@@ -247,6 +333,8 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
   using L = ExLayout<BN, PAIR>;
   constexpr int S = L::STAGES;
   constexpr int ROWS = PAIR ? 2 * TM : TM;
+  constexpr bool RUNS = SUMS != Sums::kOne;
+  static_assert(!RUNS || (WIDE && !WEIGHTS), "results in fp32");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -409,8 +497,22 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
                         mbar_wait_bounded(&acc_empty[ab], ((local >> 1) & 1) ^ 1, s_abort));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(ab * BN);
+        uint32_t d = tmem + (uint32_t)(ab * BN);
+        int first = 0;  // the sum's first step
         for (int k = 0; k < k1; ++k) {
+          if constexpr (RUNS) {
+            if (k - first == a.run) {  // the next sum, in the other accumulator
+              if (lead) commit<PAIR>(&acc_full[local & 1]);
+              __syncwarp();
+              ++local;
+              ok = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_empty[local & 1],
+                                                             ((local >> 1) & 1) ^ 1, s_abort));
+              if (!ok) break;
+              tc_fence_after();
+              d = tmem + (uint32_t)((local & 1) * BN);
+              first = k;
+            }
+          }
           if (!there) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[slot], phase, s_abort));
             if (!ok) break;
@@ -429,12 +531,12 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
             for (int j = 0; j < 4; ++j)  // 16 of k: one instruction
               issue_mma<PAIR, false>(d, (uint64_t)a_high << 32 | (a_low + j * A_STEP),
                                      (uint64_t)b_high << 32 | (b_low + j * b_step), a.idesc,
-                                     (k > 0 || j > 0) ? 1u : 0u);
+                                     (k > first || j > 0) ? 1u : 0u);
             commit<PAIR>(free_slot);
           }
           __syncwarp();
         }
-        if (ok && lead) commit<PAIR>(&acc_full[ab]);
+        if (ok && lead) commit<PAIR>(&acc_full[local & 1]);
         __syncwarp();
       }
       if (lead) {
@@ -465,11 +567,20 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
       if (ep.bias) bias_held = in ? to_f32(static_cast<const O*>(ep.bias)[w.e * a.n + w.n0 + e]) : 0.f;
       if (scaled) scale_held = in ? __ldg(ep.col_scale + w.n0 + e) : 1.f;
     };
+    auto give = [&](int ab) {  // the accumulator has been read
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) arrive_at(in_first(smem_u32(&acc_empty[ab])));
+        else arrive_at(smem_u32(&acc_empty[ab]));
+      }
+    };
+    const uint32_t t_warp = tmem + ((uint32_t)(q * 32) << 16);
     look_up(unit);
-    int local = 0;
-    for (int32_t t = unit; t < total; t += units, ++local) {  // left by all warps alike
-      const int ab = local & 1;
-      float* s_bias = s_cols + ab * 2 * BN;
+    int local = 0, turn = 0;
+    for (int32_t t = unit; t < total; t += units, ++local, turn ^= 1) {  // left by all warps alike
+      if constexpr (RUNS) look_up(t);  // registers are short there, and time is not
+      float* s_bias = s_cols + turn * 2 * BN;
       float* s_scale = s_bias + BN;
       Epilogue out = ep;
       if constexpr (WEIGHTS) out.out = static_cast<O*>(ep.out) + (int64_t)w.e * a.m * a.n;
@@ -483,15 +594,30 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
       const int rows = (int)max((int64_t)0, min((int64_t)32, w.last - row0));
       const int n0 = w.n0;
       const bool formed = w.k1 > 0;  // an expert without positions: nothing was
-      look_up(t + units);
+      if constexpr (!RUNS) look_up(t + units);
       if (!ok) continue;
+      float sum[RUNS ? COLS : 1];
+      if constexpr (RUNS) {
+        ok = ex_collect<COLS, BN>(sum, t_warp + part * COLS, a.runs, local, acc_full, s_abort, give);
+        if (!ok) continue;
+      }
+      const int ab = local & 1;
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[ab], (local >> 1) & 1, s_abort))) {
         ok = false;
         continue;
       }
       tc_fence_after();
-      const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ab * BN);
-      if (a.direct && rows > 0) {
+      const uint32_t t_row = t_warp + (uint32_t)(ab * BN);
+      if constexpr (RUNS) {
+        ex_add<COLS>(sum, t_row + part * COLS);
+        give(ab);  // the next tile's sums need not wait for the stores
+        if constexpr (SUMS == Sums::kRuns) {
+          ex_sums<COLS>(sum, part * COLS, (int)min(a.n - n0, (int64_t)BN), s_bias, s_scale, lane < rows,
+                        static_cast<float*>(out.out) + (row0 + lane) * a.n + n0);
+          continue;
+        }
+      }
+      if (!RUNS && a.direct && rows > 0) {
         using R = std::conditional_t<WIDE, float, O>;
         const int c1 = (int)min(a.n - n0, (int64_t)min((part + 1) * COLS, BN));
         const int64_t at = (row0 + min(lane, rows - 1)) * a.n + n0;
@@ -510,18 +636,22 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
 #pragma unroll 1
       for (int c = part * COLS; c < min((part + 1) * COLS, BN); c += 32) {
         const int64_t col = (int64_t)n0 + c;
-        if (a.direct || rows == 0 || col >= a.n) continue;  // the same in all lanes
+        if ((!RUNS && a.direct) || rows == 0 || col >= a.n) continue;  // the same in all lanes
         __syncwarp();  // the previous chunk has been read
+        if constexpr (RUNS) {
+          ex_stage<COLS>(sum, c - part * COLS, chunk + lane * CHUNK_LD);
+        } else {
 #pragma unroll
-        for (int h = 0; h < 32; h += 16) {
-          uint32_t raw[16];
-          tmem_ld_32x32b_x16(t_row + c + h, raw);
-          tc_wait_ld();
+          for (int h = 0; h < 32; h += 16) {
+            uint32_t raw[16];
+            tmem_ld_32x32b_x16(t_row + c + h, raw);
+            tc_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 16; j += 4)
-            *reinterpret_cast<uint4*>(chunk + lane * CHUNK_LD + h + j) =
-                formed ? make_uint4(raw[j], raw[j + 1], raw[j + 2], raw[j + 3])
-                       : make_uint4(0u, 0u, 0u, 0u);
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<uint4*>(chunk + lane * CHUNK_LD + h + j) =
+                  formed ? make_uint4(raw[j], raw[j + 1], raw[j + 2], raw[j + 3])
+                         : make_uint4(0u, 0u, 0u, 0u);
+          }
         }
         __syncwarp();
         const int cols = (int)min((int64_t)32, a.n - col);
@@ -561,12 +691,7 @@ __global__ void __launch_bounds__(EX_THREADS, 1)
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (PAIR) arrive_at(in_first(smem_u32(&acc_empty[ab])));
-        else arrive_at(smem_u32(&acc_empty[ab]));
-      }
+      if constexpr (!RUNS) give(ab);
     }
     if (!ok) report(status, SV_DEVICE_WAIT_TIMEOUT);
     if (!WEIGHTS && a.zero_rest) {
@@ -632,10 +757,15 @@ int expert_map(const void* p, int rank, const cuuint64_t* dims, const cuuint64_t
   return SV_OK;
 }
 
-template <int BN, bool PAIR, typename O, bool WEIGHTS, bool WIDE>
+bool direct_of(const ExpertGemm& g) {
+  auto sectors = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; };
+  return g.n % 16 == 0 && sectors(g.ep.out) && sectors(g.ep.preact);
+}
+
+template <int BN, bool PAIR, typename O, bool WEIGHTS, bool WIDE, Sums SUMS>
 int launch_expert(const ExpertGemm& g, CUtensorMap* maps, int32_t* status, cudaStream_t s) {
   using L = ExLayout<BN, PAIR>;
-  auto kernel = expert_tc_kernel<BN, PAIR, O, WEIGHTS, WIDE>;
+  auto kernel = expert_tc_kernel<BN, PAIR, O, WEIGHTS, WIDE, SUMS>;
   constexpr int ROWS = PAIR ? 2 * TM : TM;
   int dev = 0;
   SV_CUDA_TRY(cudaGetDevice(&dev));
@@ -694,6 +824,11 @@ int launch_expert(const ExpertGemm& g, CUtensorMap* maps, int32_t* status, cudaS
   a.tiles_n = (int32_t)((g.n + BN - 1) / BN);
   a.tiles_m = (int32_t)((g.m + ROWS - 1) / ROWS);
   a.steps = (int32_t)((g.k + 63) / 64);
+  if constexpr (SUMS != Sums::kOne) {  // of one length, but for the last
+    const int32_t most = run_steps(a.steps), sums = (a.steps + most - 1) / most;
+    a.run = (a.steps + sums - 1) / sums;
+    a.runs = (a.steps + a.run - 1) / a.run;
+  }
   a.b_mn = g.b.mn;
   a.zero_rest = g.zero_rest;
   a.maps = maps;
@@ -702,23 +837,36 @@ int launch_expert(const ExpertGemm& g, CUtensorMap* maps, int32_t* status, cudaS
   if (pieces * a.tiles_n > INT32_MAX / 2) SV_FAIL(SV_ERR_UNSUPPORTED, "expert_linear: too many tiles");
   const Epilogue& ep = g.ep;
   a.wide_io = g.n % 8 == 0 && aligned16(ep.out) && (!ep.preact || aligned16(ep.preact));
-  auto sectors = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; };
-  a.direct = g.n % 16 == 0 && sectors(ep.out) && sectors(ep.preact);
+  a.direct = direct_of(g);
   units = (int)std::min<int64_t>(pieces * a.tiles_n, units);
   config.gridDim = dim3((unsigned)(units * (PAIR ? 2 : 1)));
   SV_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, map_a, map_b, a, ep, status));
   return SV_OK;
 }
 
-template <typename O, bool WEIGHTS, bool WIDE>
+template <typename O, bool WEIGHTS, bool WIDE, Sums SUMS>
 int launch_form(const ExpertGemm& g, ExpertTile tile, CUtensorMap* maps, int32_t* status,
                 cudaStream_t s) {
   switch (tile) {
-    case ExpertTile::kPair256: return launch_expert<256, true, O, WEIGHTS, WIDE>(g, maps, status, s);
-    case ExpertTile::kPair128: return launch_expert<128, true, O, WEIGHTS, WIDE>(g, maps, status, s);
-    case ExpertTile::kOne128: return launch_expert<128, false, O, WEIGHTS, WIDE>(g, maps, status, s);
-    default: return launch_expert<64, false, O, WEIGHTS, WIDE>(g, maps, status, s);
+    case ExpertTile::kPair256: return launch_expert<256, true, O, WEIGHTS, WIDE, SUMS>(g, maps, status, s);
+    case ExpertTile::kPair128: return launch_expert<128, true, O, WEIGHTS, WIDE, SUMS>(g, maps, status, s);
+    case ExpertTile::kOne128: return launch_expert<128, false, O, WEIGHTS, WIDE, SUMS>(g, maps, status, s);
+    default: return launch_expert<64, false, O, WEIGHTS, WIDE, SUMS>(g, maps, status, s);
   }
+}
+
+template <typename O>
+int launch_typed(const ExpertGemm& g, ExpertTile tile, CUtensorMap* maps, int32_t* status,
+                 cudaStream_t s) {
+  if (g.form == ExpertForm::kWeights)
+    return launch_form<O, true, false, Sums::kOne>(g, tile, maps, status, s);
+  if (g.ep.out_dtype != SV_FLOAT32)
+    return launch_form<O, false, false, Sums::kOne>(g, tile, maps, status, s);
+  if (!g.runs || g.k <= 64 * run_steps((g.k + 63) / 64))
+    return launch_form<O, false, true, Sums::kOne>(g, tile, maps, status, s);
+  return direct_of(g) && g.ep.act == SV_ACT_NONE
+             ? launch_form<O, false, true, Sums::kRuns>(g, tile, maps, status, s)
+             : launch_form<O, false, true, Sums::kStaged>(g, tile, maps, status, s);
 }
 
 }  // namespace
@@ -728,15 +876,8 @@ size_t expert_maps_bytes(int experts) { return (size_t)experts * 2 * sizeof(CUte
 int expert_gemm_tc(const ExpertGemm& g, ExpertTile tile, void* maps, int32_t* status,
                    cudaStream_t s) {
   CUtensorMap* at = static_cast<CUtensorMap*>(maps);
-  const bool half = g.dtype == SV_FLOAT16;
-  if (g.form == ExpertForm::kWeights)
-    return half ? launch_form<__half, true, false>(g, tile, at, status, s)
-                : launch_form<__nv_bfloat16, true, false>(g, tile, at, status, s);
-  if (g.ep.out_dtype == SV_FLOAT32)
-    return half ? launch_form<__half, false, true>(g, tile, at, status, s)
-                : launch_form<__nv_bfloat16, false, true>(g, tile, at, status, s);
-  return half ? launch_form<__half, false, false>(g, tile, at, status, s)
-              : launch_form<__nv_bfloat16, false, false>(g, tile, at, status, s);
+  return g.dtype == SV_FLOAT16 ? launch_typed<__half>(g, tile, at, status, s)
+                               : launch_typed<__nv_bfloat16>(g, tile, at, status, s);
 }
 
 }  // namespace sv

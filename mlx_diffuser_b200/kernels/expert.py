@@ -161,7 +161,11 @@ def _forward(x, weight, bias, p, order, offsets, place, o, keep):
 class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, p, order, offsets, place, o):
-        out, preact, rows = _forward(x, weight, bias, p, order, offsets, place, o, True)
+        act, gather, combine = o
+        if combine and ctx.needs_input_grad[3]:
+            combine = 2  # the weights' gradients are formed from the positions' results
+        out, preact, rows = _forward(x, weight, bias, p, order, offsets, place, (act, gather, combine),
+                                     True)
         ctx.save_for_backward(x, weight, p, order, offsets, place, preact, rows)
         ctx.options = o
         ctx.bias_shape = None if bias is None else bias.shape

@@ -687,3 +687,48 @@ def test_a_weight_that_is_no_number_stays_with_its_row():
         others = torch.arange(n, device=DEV) != 7
         assert torch.isfinite(y[others]).all() and not torch.isfinite(grads["x"][7]).any()
         _close(grads["x"][others], *(v[others] for v in want), bad)
+
+
+@pytest.mark.parametrize("outputs", [64, 65])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_sums_behind_the_weights_gradients(dtype, outputs):
+    """One sum on the tensor cores loses its last place at each of its k / 16 additions, always downwards.
+    x in [1, 2) with 7 bits behind the point and weights there with 5: products have 12 and a run of
+    512 of them is below 2^11, 23 bits, exact. What is left is the runs' addition, k / 512 roundings of U
+    each (fp32 products: k / 16 of them, and one more at the end of a thread's own terms). In one sum the
+    result needs 28 bits: 1,024 cuts of half a place of 2 U on average, at half of the sum's size each, are
+    500 U."""
+    n, e, k = 40, 2, 16384
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = (1 + torch.randint(0, 128, (n, k), device=DEV, generator=g) / 128).to(dtype)
+    w = (1 + torch.randint(0, 32, (e, outputs, k), device=DEV, generator=g) / 32).to(dtype)
+    routes = _routes(n, e, 1, 0, "even")
+    expert = routes.experts[:, 0].long()
+    for column in (0, 37, outputs - 1):
+        dy = torch.zeros((n, outputs), dtype=dtype, device=DEV)
+        dy[:, column] = 1  # the gradient is the column of the results
+        p = routes.weights.detach().requires_grad_(True)
+        y = expert_linear(x, w, dataclasses.replace(routes, weights=p), gather=True, combine=True)
+        (got,) = torch.autograd.grad(y, (p,), dy)
+        want = (x.to(F64) * w.to(F64)[expert, column]).sum(1)
+        bound = (k / 512 + 1 if dtype != torch.float32 else k / 16 + 1) * U * want
+        _close(got[:, 0], want, bound, column)
+
+
+@pytest.mark.parametrize("shape", [(3000, 4, 2, 1100, 512), (700, 3, 1, 2048, 264), (200, 8, 2, 520, 200),
+                                   (900, 2, 1, 331, 1000), (60, 5, 2, 4160, 136)], ids=str)
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+def test_gradients_with_long_sums(shape, dtype):
+    n, e, k, i, o = shape
+    for f, (gather, combine) in enumerate(FORMS):
+        x, w, b = _inputs(n, e, k, i, o, dtype, gather, f)
+        routes = _routes(n, e, k, f)
+        dy = _rand((n if combine else n * k, o), dtype, 50)
+        for act in (None, ACTS[1 + f % 3]):
+            y, grads = _step(x, w, b, routes, dy, act, gather, combine)
+            ref = _Reference(x, w, b, routes, act, gather, combine)
+            _close(y, ref.out, ref.bound, "y")
+            for name, (g, bound) in ref.gradients(dy).items():
+                if name in grads:
+                    _close(grads[name], g, bound, (name, act, gather, combine))
+    N.check_device_status(DEV)
