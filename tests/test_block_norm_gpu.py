@@ -472,3 +472,26 @@ def test_saved_tensors_that_come_back_as_others(how):
     for a, b in zip(*outs):
         assert torch.equal(a, b)
     N.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("batch", [7, 8, 31, 32, 33, 1000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_over_many_batch_elements(batch, dtype):
+    """Rows of coefficients per batch element beside rows that all share, elements without rows, rows without
+    an element, and no rows at all; the sums are the same every time."""
+    for n, c in ((2000, 72), (333, 63), (40, 1024)):
+        a, dy, dh = _case(n, c, dtype, batch + c, batch)
+        a["coords"][n // 2:, 0] = batch - 1
+        _compare(a, dy, dh, dropout=0.25, seed=SEED)
+        for shared in ("gate", "scale", "shift"):
+            _compare({**a, shared: a[shared][0].contiguous()}, dy, dh, norm="rms", residual_scale=0.5)
+        first, again = _step(a, dy, dh), _step(a, dy, dh)
+        assert all(torch.equal(first[2][k], again[2][k]) for k in first[2])
+        a["coords"][::3, 0] = batch
+        with pytest.raises(RuntimeError, match="out of range"):
+            _compare(a, dy, dh)
+        empty = {**a, "x": a["x"][:0], "branch": a["branch"][:0], "coords": a["coords"][:0]}
+        _, _, grads = _step(empty, dy[:0], dh[:0])
+        assert all((grads[k] == 0).all() for k in COEFS)
+        a, dy, dh = _case(n, c, dtype, batch, batch, names=("gate", "scale", "shift"))
+        _compare(a, dy, dh)  # nothing that is summed over the batch elements
