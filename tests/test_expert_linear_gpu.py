@@ -732,3 +732,33 @@ def test_gradients_with_long_sums(shape, dtype):
                 if name in grads:
                     _close(grads[name], g, bound, (name, act, gather, combine))
     N.check_device_status(DEV)
+
+
+def test_captured_step_with_long_sums_and_two_at_once():
+    n, e, k, i, o = 700, 6, 2, 1100, 192
+    x, w, b = _inputs(n, e, k, i, o, torch.bfloat16, True)
+    routes = _routes(n, e, k)
+    dy = _rand((n, o), torch.bfloat16, 41)
+    for act in (None, "silu"):
+        want = _step(x, w, b, routes, dy, act, True, True)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        graphs, outs = [], []
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                _step(x, w, b, routes, dy, act, True, True)
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=s):
+                    outs.append(_step(x, w, b, routes, dy, act, True, True))
+                graphs.append(g)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+            eager = _step(x, w, b, routes, dy, act, True, True)
+            torch.cuda.synchronize()
+            for y, grads in (*outs, eager):
+                assert torch.equal(y, want[0])
+                assert all(torch.equal(grads[name], want[1][name]) for name in want[1])
+    N.check_device_status(DEV)
