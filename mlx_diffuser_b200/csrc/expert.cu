@@ -29,8 +29,9 @@ constexpr int EXPERT_MAX = 1024;
 constexpr int FEW_ROWS = 8;     // positions of a piece
 // Positions that the kernel for few takes. bf16, against the tensor cores' tiles: 16 experts of 1024 -> 4096
 // 8 positions 27 us (44), 16 55 (44); 8 of 1024 -> 1024 8 8.4 (17), 16 13.7 (17); 2 of 1024 -> 4096 8
-// 18.5 (17), 16 32 (17). It takes fp32 as long, whose tiles took 285, 56 and 56 us for 32 positions
-// where bf16 took 95, 22 and 59 by this kernel.
+// 18.5 (17), 16 32 (17). What decides is the positions an expert, which the host does not know: where few
+// experts share eight, the tiles would be as quick. fp32 takes up to 32, whose tiles took 285, 56 and 56 us for 32
+// positions where bf16 took 95, 22 and 59 by this kernel.
 constexpr int FEW_SLOTS = 8, FEW_SLOTS_F32 = 32;
 constexpr int DZ_ROWS = 64;     // positions of a piece of the backward pass's element-wise step
 constexpr int ALIGN = 256;

@@ -20,8 +20,9 @@
 // 81,324 positions of 8 experts, 1024 -> 4096 bf16 with bias and GELU: 525 us (1,300 TFLOP/s), 482 without
 // an activation (the library's product of that size without groups: 478). What bounds it is the epilogue:
 // a tile's products are 8,200 cycles of a pair, GELU's special functions alone 4,100 of a CTA. 24,002
-// positions of 16 experts, 2048 -> 1024: 93 us forward, 86 dx, 98 dW (1,080, 1,170 and 1,030 TFLOP/s; 5.5
-// rounds of tiles, of which an expert's last is half empty).
+// positions of 16 experts, 2048 -> 1024: 93 us forward (113 where the sum over k is made of runs, see
+// run_steps), 86 dx, 98 dW (1,080, 890, 1,170 and 1,030 TFLOP/s; 5.5 rounds of tiles, of which an expert's last
+// is half empty).
 //
 // Every wait on an mbarrier is bounded, and unwinds as in linear_tc.cu.
 #include <algorithm>
